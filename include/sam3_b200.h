@@ -32,7 +32,8 @@ enum {
     S3B_ERR_CUDA = -4,
     S3B_ERR_STATE = -5,
     S3B_ERR_UNSUPPORTED = -6,
-    S3B_ERR_DEVICE = -7, /* a kernel's bounded wait expired; see s3b_last_error */
+    S3B_ERR_DEVICE = -7, /* a kernel reported an error (a bounded wait expired, an index in device memory was
+                            out of range); see s3b_last_error */
     S3B_ERR_OOM = -8
 };
 
@@ -526,6 +527,82 @@ int s3b_op_gemm_q(s3b_ctx* ctx, const void* A, int64_t lda, const void* blocks, 
 /* Dequantises nrows rows of ne0 values of q4_0 / q4_1 / q8_0 blocks to f32,
  * bit-exactly as ggml's type-traits to_float (sam3.cpp:1076-1077). */
 int s3b_op_dequantize(s3b_ctx* ctx, const void* src, int type, int64_t ne0, int64_t nrows, float* dst);
+
+/* ---------------------------------------------------------------- quantised key / value cache */
+
+/* A cache of key and value rows in caller-owned device memory, held in the
+ * block formats of the .ggml files. It has n_pages * page_size token slots
+ * (slot = page * page_size + position in the page); each slot holds, for each
+ * of `heads` key / value heads, one key and one value row of d values in
+ * blocks of 32:
+ *   S3B_Q4_0  codes 0..15,       value = (code - 8) * scale
+ *   S3B_Q4_1  codes 0..15,       value = code * scale + minimum
+ *   S3B_Q8_0  codes -127..127,   value = code * scale
+ * with f16 scale and minimum: 2 * d * {0.5625, 0.625, 1.0625} bytes per slot
+ * and head, the same as those formats' rows, in an order of the library's own
+ * (groups of 16 tokens laid out for the attention kernels; all slots of one
+ * page and head are contiguous, so a page can be copied or swapped out as
+ * s3b_kv_cache_bytes(type, heads, d, page_size, 1) bytes at data + page * that).
+ * d is 64, 128 or 256; page_size a multiple of 16; data 16-byte aligned.
+ * ggml keeps such caches as tensors of these types that ggml_cpy writes and
+ * ggml_flash_attn_ext (sam3.cpp:9267, 9312) reads. */
+typedef struct s3b_kv_cache {
+    int32_t type;
+    int32_t heads;
+    int32_t d;
+    int32_t page_size;
+    int64_t n_pages;
+    void* data;
+} s3b_kv_cache;
+
+/* Bytes of the memory of such a cache, or S3B_ERR_ARG. */
+int64_t s3b_kv_cache_bytes(int type, int heads, int d, int page_size, int64_t n_pages);
+
+/* Quantises n tokens into the cache. k, v: device rows of `dtype` (S3B_F16 or
+ * S3B_F32), token i and head h at k + i * k_n + h * k_h (elements, each row of
+ * d contiguous; pointers and strides multiples of 16 bytes); slots[i] (device)
+ * is the token's slot, < 0 skips the token. Two tokens of one call must not
+ * share a slot. The codes are those of s3b_quantize_rows bit for bit. Values
+ * beyond +-65024 (infinities too) are held to it and a NaN counts as 0, so that
+ * no row of the cache can hold one: a token that a mask hides cannot reach
+ * another row's result. A slot past the end is skipped, and the next s3b_sync
+ * returns S3B_ERR_DEVICE. */
+int s3b_op_cache_write(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* k, int64_t k_n, int64_t k_h, const void* v,
+                       int64_t v_n, int64_t v_h, int dtype, const int64_t* slots, int64_t n);
+
+/* Reads n tokens back: the rows that slots[i] stands for as f16 or f32 (one
+ * rounding from the exact value for f16), at k_out + i * k_n + h * k_h and
+ * likewise v_out (either may be NULL). slots[i] < 0 gives zero rows; a slot
+ * past the end too, and the next s3b_sync returns S3B_ERR_DEVICE. */
+int s3b_op_cache_read(s3b_ctx* ctx, const s3b_kv_cache* cache, const int64_t* slots, int64_t n, void* k_out,
+                      int64_t k_n, int64_t k_h, void* v_out, int64_t v_n, int64_t v_h, int dtype);
+
+/* Attention over the cache: out = softmax(scale q K^T) V, with K and V read in
+ * block form. batch sequences of nq query tokens each; query head h reads
+ * key / value head h / (heads / cache->heads).
+ *   q    f16, sequence b, query i, head h at q + b * q_b + i * q_n + h * q_h
+ *   out  f16 or f32 (out_f32), at out + b * o_b + i * o_n + h * o_h
+ *        (pointers and strides multiples of 16 bytes)
+ *   lse  f32 [batch][nq][heads] or NULL: ln of the sum of exp(scale q.k),
+ *        -inf for a row that sees no token (to join with attention over
+ *        tokens outside the cache)
+ *   pages [batch][pages_stride] (device): sequence b's tokens lie in order in
+ *        its first ceil(lengths[b] / page_size) pages, of at most max_pages
+ *   lengths [batch] (device), 0 allowed
+ *   causal  query i is the token at position lengths[b] - nq + i and sees no
+ *        later one; window > 0 (with causal): only the last `window` positions
+ *        up to its own.
+ * A row that sees no token is zero. scale must be positive and finite.
+ * A length outside 0 .. max_pages * page_size is clamped, a page outside the
+ * cache is read as page 0, and the next s3b_sync returns S3B_ERR_DEVICE.
+ * Results do not depend on the order in which blocks run. The call only
+ * enqueues work on the context stream; its workspace is the context's.
+ * The reference attends over f16 keys and values of one sequence
+ * (ggml_flash_attn_ext, sam3.cpp:9267, 9312). */
+int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* q, int64_t q_b, int64_t q_n,
+                           int64_t q_h, void* out, int out_f32, int64_t o_b, int64_t o_n, int64_t o_h, float* lse,
+                           const int32_t* pages, int64_t pages_stride, int max_pages, const int32_t* lengths, int batch,
+                           int nq, int heads, float scale, int causal, int window);
 
 /* ---------------------------------------------------------------- host format helpers */
 

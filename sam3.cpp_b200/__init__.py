@@ -38,6 +38,12 @@ class TensorDesc(ctypes.Structure):
                 ("ne", ctypes.c_int64 * 4), ("data", ctypes.c_void_p)]
 
 
+class KVCacheDesc(ctypes.Structure):
+    """s3b_kv_cache: a quantised key / value cache in caller-owned device memory."""
+    _fields_ = [("type", ctypes.c_int32), ("heads", ctypes.c_int32), ("d", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("n_pages", ctypes.c_int64), ("data", ctypes.c_void_p)]
+
+
 # Every symbol declared in include/sam3_b200.h: (name, restype, argtypes)
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -101,6 +107,11 @@ SYMBOLS = [
     ("s3b_conv3x3_noalloc", _I, [_P, _I, _I, _I, _I, _P, _P, _P, _I, _P]),
     ("s3b_conv3x3_noalloc_status", _I, [ctypes.POINTER(_I)]),
     ("s3b_op_dequantize", _I, [_P, _P, _I, _I64, _I64, _P]),
+    ("s3b_kv_cache_bytes", _I64, [_I, _I, _I, _I, _I64]),
+    ("s3b_op_cache_write", _I, [_P, ctypes.POINTER(KVCacheDesc), _P, _I64, _I64, _P, _I64, _I64, _I, _P, _I64]),
+    ("s3b_op_cache_read", _I, [_P, ctypes.POINTER(KVCacheDesc), _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I]),
+    ("s3b_op_cache_attention", _I, [_P, ctypes.POINTER(KVCacheDesc), _P, _I64, _I64, _I64, _P, _I, _I64, _I64, _I64, _P,
+                                    _P, _I64, _I, _P, _I, _I, _I, _F, _I, _I]),
     ("s3b_row_size", _I64, [_I, _I64]),
     ("s3b_quantize_rows", _I, [_I, _P, _I64, _I64, _P]),
     ("s3b_dequantize_rows", _I, [_I, _P, _I64, _I64, _P]),
@@ -178,6 +189,34 @@ def dequantize_rows(qtype: int, raw: np.ndarray, ne0: int) -> np.ndarray:
     if rc != 0:
         raise S3BError(f"s3b_dequantize_rows: {ERRORS.get(rc, rc)}")
     return out
+
+
+def kv_cache_bytes(qtype: int, heads: int, d: int, page_size: int, n_pages: int) -> int:
+    """Bytes of a quantised key / value cache (s3b_kv_cache_bytes)."""
+    n = int(lib().s3b_kv_cache_bytes(qtype, heads, d, page_size, n_pages))
+    if n < 0:
+        raise S3BError(f"s3b_kv_cache_bytes: {ERRORS.get(n, n)}")
+    return n
+
+
+class KVCache:
+    """A quantised key / value cache of n_pages pages of page_size token slots (s3b_kv_cache), in `data`: a uint8 CUDA
+    tensor of kv_cache_bytes() bytes, made here unless given."""
+
+    def __init__(self, qtype: int, n_pages: int, page_size: int, heads: int, d: int, data=None, device="cuda"):
+        nbytes = kv_cache_bytes(qtype, heads, d, page_size, n_pages)
+        if data is None:
+            import torch
+            data = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        elif data.numel() * data.element_size() < nbytes or not data.is_contiguous():
+            raise S3BError(f"KVCache: data must be {nbytes} contiguous bytes")
+        self.data = data
+        self.qtype, self.n_pages, self.page_size, self.heads, self.d = qtype, n_pages, page_size, heads, d
+        self.desc = KVCacheDesc(qtype, heads, d, page_size, n_pages, data.data_ptr())
+
+    @property
+    def n_slots(self) -> int:
+        return self.n_pages * self.page_size
 
 
 def sam_best_mask(iou, multimask: bool) -> int:
@@ -633,3 +672,70 @@ class Engine:
     def dequantize(self, raw, qtype: int, ne0: int, nrows: int, out):
         rc = self._L.s3b_op_dequantize(self.h, raw.data_ptr(), qtype, ne0, nrows, out.data_ptr())
         self._check(rc, "s3b_op_dequantize")
+
+    # -- quantised key / value cache
+    def _cache_rows(self, what: str, cache: KVCache, n: int, **rows):
+        """dtype code of the row tensors [n, heads, d] after the checks that raw pointers cannot carry."""
+        dtypes = {str(t.dtype) for t in rows.values()}
+        if len(dtypes) != 1 or not dtypes <= {"torch.float16", "torch.float32"}:
+            raise S3BError(f"{what}: rows must be all f16 or all f32, got {sorted(dtypes)}")
+        for name, t in rows.items():
+            if tuple(t.shape) != (n, cache.heads, cache.d) or (t.numel() and t.stride(2) != 1):
+                raise S3BError(f"{what}: {name} must be [{n}, {cache.heads}, {cache.d}] with contiguous rows")
+        return S3B_F16 if dtypes == {"torch.float16"} else S3B_F32
+
+    @staticmethod
+    def _strides(t, n: int):
+        """The first n strides of t, 0 for a dimension of one (whose stride means nothing)."""
+        return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(n)]
+
+    @staticmethod
+    def _index(what: str, name: str, t, dtype: str, shape=None):
+        if str(t.dtype) != dtype or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
+            raise S3BError(f"{what}: {name} must be contiguous {dtype}" + (f" {list(shape)}" if shape else ""))
+
+    def cache_write(self, cache: KVCache, k, v, slots):
+        """Quantises the tokens k, v [n, heads, d] (f16 or f32 CUDA tensors, rows contiguous) into the slots int64 [n]
+        (< 0: skipped)."""
+        n = int(slots.shape[0])
+        self._index("cache_write", "slots", slots, "torch.int64", (n,))
+        dtype = self._cache_rows("cache_write", cache, n, k=k, v=v)
+        rc = self._L.s3b_op_cache_write(self.h, ctypes.byref(cache.desc), k.data_ptr(), *self._strides(k, 2),
+                                        v.data_ptr(), *self._strides(v, 2), dtype, slots.data_ptr(), n)
+        self._check(rc, "s3b_op_cache_write")
+
+    def cache_read(self, cache: KVCache, slots, k_out, v_out):
+        """Reads the tokens of the slots int64 [n] (< 0: zeros) into k_out, v_out [n, heads, d] (f16 or f32; one of them
+        may be None)."""
+        n = int(slots.shape[0])
+        self._index("cache_read", "slots", slots, "torch.int64", (n,))
+        rows = {m: t for m, t in (("k_out", k_out), ("v_out", v_out)) if t is not None}
+        dtype = self._cache_rows("cache_read", cache, n, **rows) if rows else S3B_F16
+        ks, vs = (self._strides(t, 2) if t is not None else (0, 0) for t in (k_out, v_out))
+        rc = self._L.s3b_op_cache_read(self.h, ctypes.byref(cache.desc), slots.data_ptr(), n, _ptr(k_out), *ks,
+                                       _ptr(v_out), *vs, dtype)
+        self._check(rc, "s3b_op_cache_read")
+
+    def cache_attention(self, cache: KVCache, q, out, pages, lengths, scale: float, causal: bool = False,
+                        window: int = 0, lse=None):
+        """out = softmax(scale q K^T) V over the cache (s3b_op_cache_attention): q f16 [batch, nq, heads, d], out the same
+        shape in f16 or f32, pages int32 [batch, max_pages], lengths int32 [batch], lse f32 [batch, nq, heads] or None."""
+        b, nq, heads, d = q.shape
+        what = "cache_attention"
+        if str(q.dtype) != "torch.float16" or d != cache.d or (q.numel() and q.stride(3) != 1):
+            raise S3BError(f"{what}: q must be f16 [batch, nq, heads, {cache.d}] with contiguous rows")
+        if out.shape != q.shape or str(out.dtype) not in ("torch.float16", "torch.float32") or \
+                (out.numel() and out.stride(3) != 1):
+            raise S3BError(f"{what}: out must have q's shape, in f16 or f32, with contiguous rows")
+        if pages.dim() != 2 or int(pages.shape[0]) != b or str(pages.dtype) != "torch.int32" or \
+                (pages.numel() and pages.stride(1) != 1):
+            raise S3BError(f"{what}: pages must be int32 [{b}, max_pages] with contiguous rows")
+        self._index(what, "lengths", lengths, "torch.int32", (b,))
+        if lse is not None:
+            self._index(what, "lse", lse, "torch.float32", (b, nq, heads))
+        rc = self._L.s3b_op_cache_attention(self.h, ctypes.byref(cache.desc), q.data_ptr(), *self._strides(q, 3),
+                                            out.data_ptr(), 1 if out.dtype.itemsize == 4 else 0,
+                                            *self._strides(out, 3), _ptr(lse), pages.data_ptr(),
+                                            pages.stride(0), int(pages.shape[1]), lengths.data_ptr(), b, nq, heads,
+                                            float(scale), 1 if causal else 0, int(window))
+        self._check(rc, "s3b_op_cache_attention")

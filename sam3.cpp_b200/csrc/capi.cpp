@@ -43,6 +43,8 @@ int read_dev_err(s3b_ctx* ctx) {
     // cleared in the context stream's order, so no later kernel's code can be wiped by it
     cudaMemsetAsync(ctx->d_err, 0, sizeof(int), ctx->stream);
     cudaStreamSynchronize(ctx->stream);
+    if (h == kDevErrIndex)
+      return set_error(ctx, kErrDevice, "a slot, page or length in device memory is out of range (code %d)", h);
     return set_error(ctx, kErrDevice, "device-side wait timed out (code %d)", h);
   }
   return kOk;
@@ -1352,6 +1354,140 @@ int s3b_op_gemm_q(s3b_ctx* ctx, const void* A, int64_t lda, const void* blocks, 
   w.scales = qs->as<__half>();
   rc = gemm_q(reinterpret_cast<const __half*>(A), lda, w, M, N, K, ep, ctx->d_err, ctx->stream);
   if (rc) return set_error(ctx, launcher_status_code(rc), "gemm_q launch failed (%d)", rc);
+  return kOk;
+}
+
+int64_t s3b_kv_cache_bytes(int type, int heads, int d, int page_size, int64_t n_pages) {
+  KvCache c;
+  c.type = type;
+  c.heads = heads;
+  c.d = d;
+  c.page_size = page_size;
+  c.n_pages = n_pages;
+  const long long n = kv_cache_bytes(c);
+  return n < 0 ? kErrArg : n;
+}
+
+static int kv_cache_arg(s3b_ctx* ctx, const s3b_kv_cache* cache, KvCache* c) {
+  if (!cache || !cache->data) return set_error(ctx, kErrArg, "null cache");
+  c->type = cache->type;
+  c->heads = cache->heads;
+  c->d = cache->d;
+  c->page_size = cache->page_size;
+  c->n_pages = cache->n_pages;
+  c->data = reinterpret_cast<uint8_t*>(cache->data);
+  if (kv_cache_bytes(*c) < 0)
+    return set_error(ctx, kErrArg, "bad cache: type %d, %d heads, d %d, %lld pages of %d", c->type, c->heads, c->d,
+                     c->n_pages, c->page_size);
+  if (reinterpret_cast<uintptr_t>(c->data) & 15) return set_error(ctx, kErrArg, "cache memory is not 16-byte aligned");
+  return kOk;
+}
+
+// pointer and strides (elements of esize bytes) multiples of 16 bytes
+static bool rows_aligned(const void* p, int esize, int64_t a, int64_t b, int64_t c = 0) {
+  return !(reinterpret_cast<uintptr_t>(p) & 15) && !((a * esize) & 15) && !((b * esize) & 15) && !((c * esize) & 15);
+}
+
+int s3b_op_cache_write(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* k, int64_t k_n, int64_t k_h, const void* v,
+                       int64_t v_n, int64_t v_h, int dtype, const int64_t* slots, int64_t n) {
+  int rc = ctx_enter(ctx);
+  if (rc) return rc;
+  KvCache c;
+  if ((rc = kv_cache_arg(ctx, cache, &c))) return rc;
+  if (n < 0) return set_error(ctx, kErrArg, "cache_write: %lld tokens", (long long)n);
+  if (dtype != S3B_F16 && dtype != S3B_F32) return set_error(ctx, kErrUnsupported, "cache_write takes f16 or f32 rows");
+  if (n == 0) return kOk;
+  if (!k || !v || !slots) return set_error(ctx, kErrArg, "cache_write: null pointer");
+  const int es = dtype == S3B_F16 ? 2 : 4;
+  if (!rows_aligned(k, es, k_n, k_h) || !rows_aligned(v, es, v_n, v_h))
+    return set_error(ctx, kErrArg, "cache_write: rows must start on 16-byte boundaries");
+  KvRows r;
+  r.k = const_cast<void*>(k);
+  r.v = const_cast<void*>(v);
+  r.k_n = k_n;
+  r.k_h = k_h;
+  r.v_n = v_n;
+  r.v_h = v_h;
+  r.f32 = dtype == S3B_F32;
+  rc = kv_cache_write(c, r, reinterpret_cast<const long long*>(slots), n, ctx->d_err, ctx->stream);
+  if (rc) return set_error(ctx, launcher_status_code(rc), "cache_write launch failed (%d)", rc);
+  count_launch(ctx);
+  return kOk;
+}
+
+int s3b_op_cache_read(s3b_ctx* ctx, const s3b_kv_cache* cache, const int64_t* slots, int64_t n, void* k_out,
+                      int64_t k_n, int64_t k_h, void* v_out, int64_t v_n, int64_t v_h, int dtype) {
+  int rc = ctx_enter(ctx);
+  if (rc) return rc;
+  KvCache c;
+  if ((rc = kv_cache_arg(ctx, cache, &c))) return rc;
+  if (n < 0) return set_error(ctx, kErrArg, "cache_read: %lld tokens", (long long)n);
+  if (dtype != S3B_F16 && dtype != S3B_F32) return set_error(ctx, kErrUnsupported, "cache_read gives f16 or f32 rows");
+  if (n == 0 || (!k_out && !v_out)) return kOk;
+  if (!slots) return set_error(ctx, kErrArg, "cache_read: null pointer");
+  const int es = dtype == S3B_F16 ? 2 : 4;
+  if ((k_out && !rows_aligned(k_out, es, k_n, k_h)) || (v_out && !rows_aligned(v_out, es, v_n, v_h)))
+    return set_error(ctx, kErrArg, "cache_read: rows must start on 16-byte boundaries");
+  KvRows r;
+  r.k = k_out;
+  r.v = v_out;
+  r.k_n = k_n;
+  r.k_h = k_h;
+  r.v_n = v_n;
+  r.v_h = v_h;
+  r.f32 = dtype == S3B_F32;
+  rc = kv_cache_read(c, r, reinterpret_cast<const long long*>(slots), n, ctx->d_err, ctx->stream);
+  if (rc) return set_error(ctx, launcher_status_code(rc), "cache_read launch failed (%d)", rc);
+  count_launch(ctx);
+  return kOk;
+}
+
+int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* q, int64_t q_b, int64_t q_n,
+                           int64_t q_h, void* out, int out_f32, int64_t o_b, int64_t o_n, int64_t o_h, float* lse,
+                           const int32_t* pages, int64_t pages_stride, int max_pages, const int32_t* lengths, int batch,
+                           int nq, int heads, float scale, int causal, int window) {
+  int rc = ctx_enter(ctx);
+  if (rc) return rc;
+  KvAttnParams p;
+  if ((rc = kv_cache_arg(ctx, cache, &p.c))) return rc;
+  if (batch < 0 || nq < 0 || max_pages < 0) return set_error(ctx, kErrArg, "cache_attention: negative size");
+  if (heads <= 0 || heads % p.c.heads)
+    return set_error(ctx, kErrArg, "cache_attention: %d query heads over %d key / value heads", heads, p.c.heads);
+  if (!(scale > 0.f) || scale > 3.4e38f) return set_error(ctx, kErrArg, "cache_attention: scale must be positive");
+  if (window < 0 || (window > 0 && !causal))
+    return set_error(ctx, kErrArg, "cache_attention: a window must be positive and causal");
+  if (batch == 0 || nq == 0) return kOk;
+  if (!q || !out || !lengths || (!pages && max_pages > 0)) return set_error(ctx, kErrArg, "cache_attention: null pointer");
+  if (max_pages > 0 && batch > 1 && pages_stride < max_pages)
+    return set_error(ctx, kErrArg, "cache_attention: page table rows of %lld hold no %d pages", (long long)pages_stride,
+                     max_pages);
+  if ((long long)max_pages * p.c.page_size > 0x7fffffffLL || (long long)nq * heads > 0x3fffffffLL)
+    return set_error(ctx, kErrUnsupported, "cache_attention: a sequence may hold 2^31 - 1 tokens at most");
+  if (!rows_aligned(q, 2, q_b, q_n, q_h) || !rows_aligned(out, out_f32 ? 4 : 2, o_b, o_n, o_h))
+    return set_error(ctx, kErrArg, "cache_attention: rows must start on 16-byte boundaries");
+  p.q = reinterpret_cast<const __half*>(q);
+  p.q_b = q_b;
+  p.q_n = q_n;
+  p.q_h = q_h;
+  p.out = out;
+  p.out_f32 = out_f32 ? 1 : 0;
+  p.o_b = o_b;
+  p.o_n = o_n;
+  p.o_h = o_h;
+  p.lse = lse;
+  p.pages = pages;
+  p.pages_stride = pages_stride;
+  p.max_pages = max_pages;
+  p.lengths = lengths;
+  p.batch = batch;
+  p.nq = nq;
+  p.heads = heads;
+  p.scale = scale;
+  p.causal = causal ? 1 : 0;
+  p.window = window;
+  rc = kv_attention(p, ctx->d_err, ctx->stream);
+  if (rc) return set_error(ctx, launcher_status_code(rc), "cache_attention launch failed (%d)", rc);
+  count_launch(ctx);
   return kOk;
 }
 

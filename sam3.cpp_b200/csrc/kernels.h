@@ -352,4 +352,45 @@ inline int kernel_setup(K* kernel, size_t smem) {
 // failed launch, or an earlier asynchronous fault reported at this point).
 int launch_status(const char* what);
 
+// ---------------------------------------------------------------- quantised key / value cache
+// Device error code of an index in device memory (slot, page, length) that is out of range.
+constexpr int kDevErrIndex = 7;
+
+// s3b_kv_cache with its memory; kv_cache_bytes returns its size, or -1 when the fields are not a cache.
+struct KvCache {
+  int type = 0, heads = 0, d = 0, page_size = 0;
+  long long n_pages = 0;
+  uint8_t* data = nullptr;
+};
+long long kv_cache_bytes(const KvCache& c);
+
+// Rows to write or read: token i, head h at k + i * k_n + h * k_h (elements of f16, or f32 with `f32`).
+struct KvRows {
+  void* k = nullptr;
+  void* v = nullptr;
+  long long k_n = 0, k_h = 0, v_n = 0, v_h = 0;
+  int f32 = 0;
+};
+int kv_cache_write(const KvCache& c, const KvRows& r, const long long* slots, long long n, int* err, cudaStream_t st);
+int kv_cache_read(const KvCache& c, const KvRows& r, const long long* slots, long long n, int* err, cudaStream_t st);
+
+// The arguments of s3b_op_cache_attention.
+struct KvAttnParams {
+  KvCache c;
+  const __half* q = nullptr;
+  long long q_b = 0, q_n = 0, q_h = 0;
+  void* out = nullptr;
+  int out_f32 = 0;
+  long long o_b = 0, o_n = 0, o_h = 0;
+  float* lse = nullptr;
+  const int* pages = nullptr;
+  long long pages_stride = 0;
+  int max_pages = 0;
+  const int* lengths = nullptr;
+  int batch = 0, nq = 0, heads = 0;
+  float scale = 1.f;
+  int causal = 0, window = 0;
+};
+int kv_attention(const KvAttnParams& p, int* err, cudaStream_t st);
+
 }  // namespace s3b

@@ -1,0 +1,57 @@
+// Layout of the quantised key / value cache, shared by the kernels that write, read and attend over it.
+//
+// The cache is a sequence of (page, head) regions, each a sequence of groups of 16 tokens. A group of KvL<QT, D>::kGroup
+// bytes holds, in this order, the key values, the value values, the key scales (q4_1: then the key minima) and the value
+// scales (then minima) of its 16 tokens. The order of the values inside a group is that of the m16n8k16 fragments of the
+// few-query attention kernel, so that lane (g, t) = (lane / 4, lane % 4) of a warp finds its share of the group as whole
+// 8- or 16-byte words, contiguous over the lanes:
+//   keys    A operand of S^T = K Q^T, rows = tokens: lane (g, t) takes tokens g and g + 8, and of every block of 32 the
+//           8 consecutive values 8 t .. 8 t + 7 (the contraction may run in any order that Q shares).
+//   values  A operand of O^T = V^T P^T, columns = tokens: lane (g, t) takes tokens 2t, 2t + 1, 2t + 8, 2t + 9, and of
+//           every block of 32 the 4 values 4 g .. 4 g + 3 (the rows of O^T may stand in any order).
+// Values come in super-blocks of 128 (4 bits) or 64 (8 bits, or D = 64), the widest that one 16-byte load per lane takes.
+#pragma once
+#include "common.cuh"
+#include "kernels.h"
+
+namespace s3b {
+
+template <int QT, int D>
+struct KvL {
+  static constexpr int kBits = QT == QT_Q8_0 ? 8 : 4;
+  static constexpr int kNB = D / 32;                                         // blocks of a row
+  static constexpr int kSB = (kBits == 4 && D >= 128) ? 128 : 64;            // values of a super-block
+  static constexpr int kNBS = kSB / 32;                                      // blocks of a super-block
+  static constexpr int kSuper = 16 * kSB * kBits / 8;                        // bytes of a super-block of 16 tokens
+  static constexpr int kVal = 16 * D * kBits / 8;                            // bytes of the keys (or values) of a group
+  static constexpr int kPlanes = QT == QT_Q4_1 ? 2 : 1;                      // scale, minimum
+  static constexpr int kSc = 16 * kNB * 2;                                   // bytes of one plane
+  static constexpr int kGroup = 2 * kVal + 2 * kPlanes * kSc;
+
+  // byte offsets in a group
+  // keys: values 8 t .. 8 t + 7 of block b of token tok (4 or 8 bytes)
+  static __host__ __device__ constexpr int k_val(int tok, int b, int t) {
+    return (b / kNBS) * kSuper + tok * (kSB * kBits / 8) + (t * kNBS + b % kNBS) * kBits;
+  }
+  // values: values 4 g .. 4 g + 3 of block b of token tok (2 or 4 bytes)
+  static __host__ __device__ constexpr int v_val(int tok, int b, int g) {
+    return kVal + (b / kNBS) * kSuper +
+           ((((tok >> 3) * 32 + g * 4 + ((tok & 7) >> 1)) * 2 + (tok & 1)) * kNBS + b % kNBS) * (kBits / 2);
+  }
+  static __host__ __device__ constexpr int k_scale(int tok, int b) { return 2 * kVal + (tok * kNB + b) * 2; }
+  // the four tokens of lane t (2t, 2t + 1, 2t + 8, 2t + 9) side by side
+  static __host__ __device__ constexpr int v_scale(int tok, int b) {
+    return 2 * kVal + kPlanes * kSc + ((((tok & 7) >> 1) * kNB + b) * 4 + (tok & 1) + 2 * (tok >> 3)) * 2;
+  }
+};
+
+// Byte offset of the group of 16 tokens `group` of (page, head).
+template <int QT, int D>
+__device__ __forceinline__ long long kv_group_offset(const KvCache& c, long long page, int head, int group) {
+  return ((page * c.heads + head) * (c.page_size >> 4) + group) * (long long)KvL<QT, D>::kGroup;
+}
+
+// The 8 nibbles of a key word: value 2p in nibble p, value 2p + 1 in nibble p + 4. The 4 nibbles of a value half-word
+// stand in order. 8-bit codes are stored with 128 added, in order.
+
+}  // namespace s3b
