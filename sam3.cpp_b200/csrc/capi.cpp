@@ -1485,7 +1485,22 @@ int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* 
   p.scale = scale;
   p.causal = causal ? 1 : 0;
   p.window = window;
-  rc = kv_attention(p, ctx->d_err, ctx->stream);
+  KvAttnWork w;
+  w.sms = num_sms();
+  size_t part_bytes, count_bytes;
+  kv_attention_work(p, w.sms, &part_bytes, &count_bytes);
+  if (part_bytes) {
+    w.part = ctx->buf("kv_attn_part", part_bytes, &rc)->as<float>();
+    if (rc) return rc;
+    DevBuf* count = ctx->buf("kv_attn_count", 0, &rc);
+    if (count->bytes < count_bytes) {
+      if (count->reserve(std::max<size_t>(count_bytes, 4096)) ||
+          cudaMemsetAsync(count->p, 0, count->bytes, ctx->stream) != cudaSuccess)
+        return set_error(ctx, kErrOOM, "cache_attention: %zu bytes of counts", count_bytes);
+    }
+    w.count = count->as<int>();
+  }
+  rc = kv_attention(p, w, ctx->d_err, ctx->stream);
   if (rc) return set_error(ctx, launcher_status_code(rc), "cache_attention launch failed (%d)", rc);
   count_launch(ctx);
   return kOk;

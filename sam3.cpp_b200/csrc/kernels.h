@@ -391,6 +391,14 @@ struct KvAttnParams {
   float scale = 1.f;
   int causal = 0, window = 0;
 };
-int kv_attention(const KvAttnParams& p, int* err, cudaStream_t st);
+// Workspace of the attention: parts of units that several CTAs share, and their arrival counts, which are zero before
+// and after every launch.
+struct KvAttnWork {
+  float* part = nullptr;
+  int* count = nullptr;
+  int sms = 0;
+};
+void kv_attention_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes);
+int kv_attention(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st);
 
 }  // namespace s3b

@@ -1,6 +1,14 @@
 // Attention over the quantised key / value cache (layout: kv_cache.cuh).
 //   s_j = scale * q . k_j,  p_j = exp(s_j - max s),  out = sum_j p_j v_j / sum_j p_j
 // over the tokens j that the query sees.
+//
+// Few query rows (rows of one key / value head = queries x heads of its group): rows_kernel. The cache is read once, so
+// HBM bounds it; the products run on m16n8k16 fragments whose A operand is the cache (16 tokens, or 16 values of a row)
+// and whose 8 columns are the query rows, so that a single row wastes no more than the padding of its column. Codes
+// enter the products as exact small integers; a block's scale multiplies the 32-value partial score in f32 (keys), or
+// the weight before it is rounded to f16 (values), so no dequantised value is ever formed or rounded.
+#include <algorithm>
+
 #include "kv_cache.cuh"
 
 namespace s3b {
@@ -8,6 +16,8 @@ namespace s3b {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNoScore = -1e30f;  // reference maximum before the first visible token: finite, so that no inf - inf arises
 
 // Tokens of sequence b, held to what its page table can name.
 __device__ __forceinline__ int sequence_length(const KvAttnParams& p, int b, int* err) {
@@ -20,7 +30,636 @@ __device__ __forceinline__ int sequence_length(const KvAttnParams& p, int b, int
   return n;
 }
 
-// Values 32 b + lane of a key (KV = 0) or value row.
+// Tokens [lo, hi) that query i of a sequence of len tokens sees.
+__device__ __forceinline__ void row_span(const KvAttnParams& p, int len, int i, int* lo, int* hi) {
+  *lo = 0;
+  *hi = len;
+  if (p.causal) {
+    *hi = max(0, len - p.nq + i + 1);
+    if (p.window) *lo = max(0, *hi - p.window);
+  }
+}
+
+// Groups of 16 tokens [g0, g1) that queries [i0, i1] of a sequence of len tokens see between them.
+__device__ __forceinline__ void group_span(const KvAttnParams& p, int len, int i0, int i1, int* g0, int* g1) {
+  int lo, hi, none;
+  row_span(p, len, i0, &lo, &none);
+  row_span(p, len, i1, &none, &hi);
+  *g0 = lo >> 4;
+  *g1 = max(*g0, (hi + 15) >> 4);
+}
+
+__device__ __forceinline__ void store_out(const KvAttnParams& p, long long at, float4 v) {
+  if (p.out_f32) {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = v;
+  } else {
+    __half2 h[2] = {__floats2half2_rn(v.x, v.y), __floats2half2_rn(v.z, v.w)};
+    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + at) = *reinterpret_cast<uint2*>(h);
+  }
+}
+
+// ---------------------------------------------------------------- fragments
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// transpose of the 8 x 8 matrix of 16-bit values that a warp holds as one m8n8 fragment
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ uint32_t h2_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 u32_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+// Exact f16 pairs of the codes (less 8 for q4_0) whose nibbles lie at bits 0, 4, 8, 12 of each half of w: a nibble under
+// the exponent of 1024 reads 1024 + c at bit 0 and 1024 + 16 c at bit 4; one subtraction (or multiply-add by 1/16)
+// leaves the integer.
+template <int QT>
+__device__ __forceinline__ void nibble_pairs(uint32_t w, uint32_t (&out)[4]) {
+  const __half2 off0 = __float2half2_rn(QT == QT_Q4_0 ? -1032.f : -1024.f);
+  const __half2 off1 = __float2half2_rn(QT == QT_Q4_0 ? -72.f : -64.f);
+  const __half2 sixteenth = __float2half2_rn(0.0625f);
+  const uint32_t x = w >> 8;
+  out[0] = h2_u32(__hadd2(u32_h2((w & 0x000F000Fu) | 0x64006400u), off0));
+  out[1] = h2_u32(__hfma2(u32_h2((w & 0x00F000F0u) | 0x64006400u), sixteenth, off1));
+  out[2] = h2_u32(__hadd2(u32_h2((x & 0x000F000Fu) | 0x64006400u), off0));
+  out[3] = h2_u32(__hfma2(u32_h2((x & 0x00F000F0u) | 0x64006400u), sixteenth, off1));
+}
+// The same for the bytes 0, 1 and 2, 3 of w (8-bit codes with 128 added).
+__device__ __forceinline__ void byte_pairs(uint32_t w, uint32_t& a, uint32_t& b) {
+  const __half2 off = __float2half2_rn(-1152.f);
+  a = h2_u32(__hadd2(u32_h2(__byte_perm(w, 0x64646464u, 0x4140)), off));
+  b = h2_u32(__hadd2(u32_h2(__byte_perm(w, 0x64646464u, 0x4342)), off));
+}
+
+template <int BYTES>
+__device__ __forceinline__ void lds(const uint8_t* at, uint32_t (&r)[BYTES / 4]) {
+  if (BYTES == 16) {
+    const uint4 v = *reinterpret_cast<const uint4*>(at);
+    r[0] = v.x;
+    r[1] = v.y;
+    r[BYTES / 4 - 2] = v.z;
+    r[BYTES / 4 - 1] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
+    r[0] = v.x;
+    r[1] = v.y;
+  }
+}
+
+// ---------------------------------------------------------------- few query rows
+// The work is one line of chunks of W groups of 16 tokens, unit after unit (a unit is one sequence and key / value
+// head), cut into equal shares for the CTAs, so sequences of uneven length leave no SM idle and one long sequence
+// spreads over all of them. In a share each warp takes every W-th group: its own ring of bulk copies, its own running
+// maximum, sum and output (no barrier in the loop); the W states are joined in shared memory at the end of a unit's
+// part. A unit that several CTAs share leaves its parts in the workspace and the last CTA to arrive joins them in the
+// order of the shares, so the result does not depend on who that is.
+template <int QT, int D, int NT, int W>
+struct Rows {
+  typedef KvL<QT, D> L;
+  static constexpr int kRows = 8 * NT;
+  static constexpr bool kQSmem = NT * D > 128;  // the query fragments of more would not fit beside the output's registers
+  static constexpr int kWarps = QT == QT_Q8_0 && D == 256 ? 8 : 16;  // of an SM, each with its ring
+  static constexpr int kCtas = kWarps / W;
+  static constexpr int kQBytes = kQSmem ? NT * L::kNB * 512 : 0;
+  static constexpr int kOStride = D + 4;        // floats; the padding spreads the rows of a store over the banks
+  static constexpr int kJoin = W * kRows * kOStride * 4;
+  static constexpr int kFixed = kQBytes + 3 * W * kRows * 4 + 1024;
+  static constexpr int kBudget = (225 * 1024) / kCtas - kFixed - 1024;
+  static constexpr int kFit = kBudget / (W * L::kGroup);
+  static constexpr int kStages = kFit > 6 ? 6 : kFit;
+  static constexpr int kRing = W * kStages * L::kGroup;
+  static constexpr int kMain = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kSmem = kMain + kFixed;
+  static_assert(kStages >= 2 && kMain + kFixed + 1024 <= (227 * 1024) / kCtas, "shared memory of rows_kernel");
+};
+
+struct RowsArgs {
+  KvAttnParams p;
+  float* part;  // [2 * grid] x (kRows * D outputs, kRows maxima, kRows sums)
+  int* count;   // [units], zero between launches
+};
+
+template <int QT, int D, int NT, int W>
+__global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel(const __grid_constant__ RowsArgs a, int* err) {
+  typedef KvL<QT, D> L;
+  typedef Rows<QT, D, NT, W> C;
+  constexpr int NB = L::kNB, NS = C::kStages;
+  constexpr float kBias = QT == QT_Q8_0 ? 4.f : 0.f;  // weights are 2^kBias at the reference: their products with the
+                                                       // block scales then use f16's range as the values would
+  constexpr float kLazy = 2.9f;                        // and stay below f16's largest: 2^(kBias + 2.9) * scale < 65504
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* s_q = smem + C::kMain;
+  float* s_m = reinterpret_cast<float*>(s_q + C::kQBytes);  // [W][rows]
+  float* s_l = s_m + W * C::kRows;
+  float* s_f = s_l + W * C::kRows;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_f + W * C::kRows);
+  __shared__ long long s_total, s_base;
+  __shared__ int s_b, s_abort_word, s_last;
+  volatile int* s_abort = &s_abort_word;
+  static_assert(W * NS * 8 <= 1024, "barriers of rows_kernel");
+  (void)NB;
+
+  const KvAttnParams& p = a.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int group_heads = p.heads / p.c.heads;
+  const int n_rows = p.nq * group_heads;
+  const int per_page = p.c.page_size >> 4;
+
+  auto chunks_of = [&](int b, int* g0, int* g1) -> int {
+    group_span(p, sequence_length(p, b, err), 0, p.nq - 1, g0, g1);
+    return (*g1 - *g0 + W - 1) / W;
+  };
+
+  if (threadIdx.x < W * NS) mbar_init(&bars[threadIdx.x], 1);
+  if (threadIdx.x == 0) {
+    s_abort_word = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  // total chunks, then the sequence in which this CTA's share begins
+  if (warp == 0) {
+    long long total = 0;
+    int g0, g1;
+    for (int b = lane; b < p.batch; b += 32) total += chunks_of(b, &g0, &g1);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(~0u, total, x);
+    total *= p.c.heads;
+    const long long ctas = min((long long)gridDim.x, total);
+    const long long first = ctas ? total * blockIdx.x / ctas : 0;
+    long long base = 0;
+    int found = -1;
+    if ((int)blockIdx.x < ctas) {
+      for (int b0 = 0; b0 < p.batch && found < 0; b0 += 32) {
+        const long long n = b0 + lane < p.batch ? (long long)chunks_of(b0 + lane, &g0, &g1) * p.c.heads : 0;
+        long long end = n;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+          const long long up = __shfl_up_sync(~0u, end, x);
+          if (lane >= x) end += up;
+        }
+        const uint32_t past = __ballot_sync(~0u, base + end > first);
+        if (past) {
+          const int who = __ffs(past) - 1;
+          found = b0 + who;
+          base += __shfl_sync(~0u, end - n, who);
+        } else {
+          base += __shfl_sync(~0u, end, 31);
+        }
+      }
+    }
+    if (lane == 0) {
+      s_total = total;
+      s_base = base;
+      s_b = found;
+    }
+  }
+  __syncthreads();
+  const long long total = s_total;
+  const long long ctas = min((long long)gridDim.x, total);
+
+  // sequences of which no query sees a token
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    int g0, g1;
+    if (chunks_of(b, &g0, &g1)) continue;
+    for (int e = threadIdx.x; e < p.nq * p.heads * (D / 4); e += 32 * W) {
+      const int h = e / (D / 4) % p.heads, i = e / (D / 4) / p.heads;
+      store_out(p, b * p.o_b + i * p.o_n + h * p.o_h + e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+      if (p.lse && e % (D / 4) == 0) p.lse[((long long)b * p.nq + i) * p.heads + h] = -INFINITY;
+    }
+  }
+  if ((int)blockIdx.x >= ctas) return;
+
+  const long long p0 = total * blockIdx.x / ctas, p1 = total * (blockIdx.x + 1) / ctas;
+  const float sl2 = p.scale * kLog2e;
+  uint8_t* ring = smem + warp * NS * L::kGroup;
+  uint64_t* full = bars + warp * NS;
+  int stage = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+
+  long long pos = p0, base = s_base;
+  for (int b = s_b; pos < p1; ++b) {
+    int g0, g1;
+    const int n_chunks = chunks_of(b, &g0, &g1);
+    const int len = sequence_length(p, b, err);
+    int min_lo, max_lo, min_hi, max_hi;  // of the spans of the unit's rows
+    row_span(p, len, 0, &min_lo, &min_hi);
+    row_span(p, len, p.nq - 1, &max_lo, &max_hi);
+    const int* table = p.pages + b * p.pages_stride;
+    for (; pos < p1 && pos < base + (long long)n_chunks * p.c.heads;) {
+      const int head = (int)((pos - base) / n_chunks);
+      const long long unit_start = base + (long long)head * n_chunks;
+      const int ca = (int)(pos - unit_start);
+      const int cb = (int)min((long long)n_chunks, p1 - unit_start);
+      pos += cb - ca;
+
+      // ---- this warp's groups: g0 + chunk * W + warp
+      const int first = g0 + ca * W + warp;
+      const int n_it = first < g1 ? min(cb - ca, (g1 - first + W - 1) / W) : 0;
+      long long src = 0;  // lane i: address of iteration (batch of 32) + i
+      auto locate = [&](int it0) {
+        const int gi = first + (it0 + lane) * W;
+        if (it0 + lane < n_it) {
+          long long page = table[gi / per_page];
+          if (page < 0 || page >= p.c.n_pages) {
+            atomicCAS(err, 0, kDevErrIndex);
+            page = 0;
+          }
+          src = kv_group_offset<QT, D>(p.c, page, head, gi % per_page);
+        }
+      };
+      int st_issue = stage;
+      auto issue = [&](int it) {
+        const long long from = __shfl_sync(~0u, src, it & 31);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&full[st_issue], L::kGroup);
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                           smem_u32(ring + st_issue * L::kGroup)),
+                       "l"(p.c.data + from), "r"(L::kGroup), "r"(smem_u32(&full[st_issue]))
+                       : "memory");
+        }
+        st_issue = st_issue + 1 == NS ? 0 : st_issue + 1;
+      };
+      locate(0);
+      int issued = 0;
+      for (; issued < min(NS, n_it); ++issued) issue(issued);
+
+      // ---- query fragments: column g of tile nt is row 8 nt + g; block n's values 8 t .. 8 t + 7
+      uint32_t qf[C::kQSmem ? 1 : NT * NB][4];
+      uint32_t qmin[NT][2];  // q4_1: sums of the query over blocks 2t, 2t + 1, as f16 and f16 remainder
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = 8 * nt + g;
+        const int i = r / group_heads, h = head * group_heads + r % group_heads;
+        const __half* q = p.q + b * p.q_b + i * p.q_n + h * p.q_h + 8 * t;
+        float lo = 0.f, hi = 0.f;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (r < n_rows) v = *reinterpret_cast<const uint4*>(q + 32 * n);
+          if (C::kQSmem) {
+            if (warp == 0) *reinterpret_cast<uint4*>(s_q + ((nt * NB + n) * 32 + lane) * 16) = v;
+          } else {
+            qf[C::kQSmem ? 0 : nt * NB + n][0] = v.x;
+            qf[C::kQSmem ? 0 : nt * NB + n][1] = v.y;
+            qf[C::kQSmem ? 0 : nt * NB + n][2] = v.z;
+            qf[C::kQSmem ? 0 : nt * NB + n][3] = v.w;
+          }
+          if (QT == QT_Q4_1) {
+            const float2 x0 = __half22float2(u32_h2(v.x)), x1 = __half22float2(u32_h2(v.y));
+            const float2 x2 = __half22float2(u32_h2(v.z)), x3 = __half22float2(u32_h2(v.w));
+            float sum = ((x0.x + x0.y) + (x1.x + x1.y)) + ((x2.x + x2.y) + (x3.x + x3.y));
+            sum += __shfl_xor_sync(~0u, sum, 1);
+            sum += __shfl_xor_sync(~0u, sum, 2);
+            if (n == 2 * t) lo = sum;
+            if (n == 2 * t + 1) hi = sum;
+          }
+        }
+        if (QT == QT_Q4_1) {
+          const __half2 s = __floats2half2_rn(lo, hi);
+          const float2 f = __half22float2(s);
+          qmin[nt][0] = h2_u32(s);
+          qmin[nt][1] = h2_u32(__floats2half2_rn(lo - f.x, hi - f.y));
+        }
+      }
+      if (C::kQSmem) __syncthreads();
+
+      // ---- state: columns 2t, 2t + 1 of each tile
+      float o[NT][D / 16][4], omin[NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][x][e] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) omin[nt][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          m[nt][c] = kNoScore;
+          l[nt][c] = 0.f;
+        }
+      }
+
+      for (int it = 0; it < n_it; ++it) {
+        if (!mbar_wait(&full[stage], phase, s_abort, err, kErrWaitFull)) ok = false;
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        const uint8_t* gp = ring + stage * L::kGroup;
+        const int tok0 = (first + it * W) * 16;
+        const bool whole = tok0 >= max_lo && tok0 + 16 <= min_hi;
+
+        // -- scores
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+        if (QT == QT_Q4_1) {  // sum over blocks of minimum * (sum of the query over the block)
+          uint32_t am[4] = {0, 0, 0, 0};
+          if (2 * t < NB) {
+            am[0] = am[2] = *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g, 2 * t));
+            am[1] = am[3] = *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g + 8, 2 * t));
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816(s[nt], am, qmin[nt][0], qmin[nt][1]);
+        }
+#pragma unroll
+        for (int sb = 0; sb < D / L::kSB; ++sb) {
+          constexpr int PB = L::kNBS * L::kBits;  // bytes of a lane's piece of one token
+          uint32_t k0[PB / 4], k1[PB / 4];
+          lds<PB>(gp + L::k_val(g, sb * L::kNBS, t), k0);
+          lds<PB>(gp + L::k_val(g + 8, sb * L::kNBS, t), k1);
+#pragma unroll
+          for (int nn = 0; nn < L::kNBS; ++nn) {
+            const int n = sb * L::kNBS + nn;
+            uint32_t x0[4], x1[4];
+            if (QT == QT_Q8_0) {
+              byte_pairs(k0[2 * nn], x0[0], x0[1]);
+              byte_pairs(k0[2 * nn + 1], x0[2], x0[3]);
+              byte_pairs(k1[2 * nn], x1[0], x1[1]);
+              byte_pairs(k1[2 * nn + 1], x1[2], x1[3]);
+            } else {
+              nibble_pairs<QT>(k0[nn], x0);
+              nibble_pairs<QT>(k1[nn], x1);
+            }
+            const uint32_t a0[4] = {x0[0], x1[0], x0[1], x1[1]}, a1[4] = {x0[2], x1[2], x0[3], x1[3]};
+            const float f0 = __half2float(*reinterpret_cast<const __half*>(gp + L::k_scale(g, n)));
+            const float f1 = __half2float(*reinterpret_cast<const __half*>(gp + L::k_scale(g + 8, n)));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              uint4 qv;
+              if (C::kQSmem)
+                qv = *reinterpret_cast<const uint4*>(s_q + ((nt * NB + n) * 32 + lane) * 16);
+              else
+                qv = make_uint4(qf[C::kQSmem ? 0 : nt * NB + n][0], qf[C::kQSmem ? 0 : nt * NB + n][1], qf[C::kQSmem ? 0 : nt * NB + n][2],
+                                qf[C::kQSmem ? 0 : nt * NB + n][3]);
+              float c[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816(c, a0, qv.x, qv.y);
+              mma16816(c, a1, qv.z, qv.w);
+              s[nt][0] = fmaf(f0, c[0], s[nt][0]);
+              s[nt][1] = fmaf(f0, c[1], s[nt][1]);
+              s[nt][2] = fmaf(f1, c[2], s[nt][2]);
+              s[nt][3] = fmaf(f1, c[3], s[nt][3]);
+            }
+          }
+        }
+
+        // -- weights: the reference maximum of a column moves only when a score passes it by kLazy
+        bool move = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] *= sl2;
+          if (!whole) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              int lo, hi;
+              row_span(p, len, min((8 * nt + 2 * t + c) / group_heads, p.nq - 1), &lo, &hi);
+              if (tok0 + g < lo || tok0 + g >= hi) s[nt][c] = -INFINITY;
+              if (tok0 + g + 8 < lo || tok0 + g + 8 >= hi) s[nt][c + 2] = -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) move |= fmaxf(s[nt][c], s[nt][c + 2]) > m[nt][c] + kBias + kLazy;
+        }
+        if (__any_sync(~0u, move)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float f[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float top = fmaxf(s[nt][c], s[nt][c + 2]);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+              const float m2 = fmaxf(m[nt][c], top - kBias);
+              f[c] = ex2_approx(m[nt][c] - m2);
+              m[nt][c] = m2;
+              l[nt][c] *= f[c];
+            }
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nt][x][e] *= f[e & 1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) omin[nt][e] *= f[e & 1];
+          }
+        }
+        uint32_t w0[NT], w1[NT];  // weights of column g for tokens 2t, 2t + 1 and 2t + 8, 2t + 9
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float e4[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) e4[e] = ex2_approx(s[nt][e] - m[nt][e & 1]);
+          l[nt][0] += e4[0] + e4[2];
+          l[nt][1] += e4[1] + e4[3];
+          w0[nt] = movmatrix(h2_u32(__floats2half2_rn(e4[0], e4[1])));
+          w1[nt] = movmatrix(h2_u32(__floats2half2_rn(e4[2], e4[3])));
+        }
+
+        // -- outputs; tokens outside the sequence's span may hold anything, so their scales count as zero
+        uint32_t keep0 = ~0u, keep1 = ~0u;
+        if (!whole) {
+          auto in = [&](int tok) -> bool { return tok0 + tok >= min_lo && tok0 + tok < max_hi; };
+          keep0 = (in(2 * t) ? 0xFFFFu : 0u) | (in(2 * t + 1) ? 0xFFFF0000u : 0u);
+          keep1 = (in(2 * t + 8) ? 0xFFFFu : 0u) | (in(2 * t + 9) ? 0xFFFF0000u : 0u);
+        }
+        if (QT == QT_Q4_1) {  // sum over tokens of weight * minimum, a row for each block
+          uint32_t am[4] = {0, 0, 0, 0};
+          if (g < NB) {
+            const uint2 v = *reinterpret_cast<const uint2*>(gp + L::kSc + L::v_scale(2 * t, g));
+            am[0] = v.x & keep0;
+            am[2] = v.y & keep1;
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816(omin[nt], am, w0[nt], w1[nt]);
+        }
+#pragma unroll
+        for (int sb = 0; sb < D / L::kSB; ++sb) {
+          constexpr int PB = L::kNBS * L::kBits;  // bytes of a lane's piece of two tokens
+          constexpr int PW = PB / 8;              // words of a token's
+          uint32_t va[PB / 4], vb[PB / 4];
+          lds<PB>(gp + L::v_val(2 * t, sb * L::kNBS, g), va);
+          lds<PB>(gp + L::v_val(2 * t + 8, sb * L::kNBS, g), vb);
+#pragma unroll
+          for (int nn = 0; nn < L::kNBS; ++nn) {
+            const int n = sb * L::kNBS + nn;
+            uint32_t x0[4], x1[4];  // values 4g .. 4g + 3 of tokens (2t, 2t + 1) and (2t + 8, 2t + 9)
+            if (QT == QT_Q8_0) {
+              byte_pairs(__byte_perm(va[nn], va[PW + nn], 0x5140), x0[0], x0[1]);
+              byte_pairs(__byte_perm(va[nn], va[PW + nn], 0x7362), x0[2], x0[3]);
+              byte_pairs(__byte_perm(vb[nn], vb[PW + nn], 0x5140), x1[0], x1[1]);
+              byte_pairs(__byte_perm(vb[nn], vb[PW + nn], 0x7362), x1[2], x1[3]);
+            } else {
+              nibble_pairs<QT>(__byte_perm(va[nn / 2], va[PW + nn / 2], nn & 1 ? 0x7632 : 0x5410), x0);
+              nibble_pairs<QT>(__byte_perm(vb[nn / 2], vb[PW + nn / 2], nn & 1 ? 0x7632 : 0x5410), x1);
+            }
+            const uint32_t a0[4] = {x0[0], x0[1], x1[0], x1[1]}, a1[4] = {x0[2], x0[3], x1[2], x1[3]};
+            const uint2 sc = *reinterpret_cast<const uint2*>(gp + L::v_scale(2 * t, n));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint32_t b0 = h2_u32(__hmul2(u32_h2(w0[nt]), u32_h2(sc.x & keep0)));
+              const uint32_t b1 = h2_u32(__hmul2(u32_h2(w1[nt]), u32_h2(sc.y & keep1)));
+              mma16816(o[nt][2 * n], a0, b0, b1);
+              mma16816(o[nt][2 * n + 1], a1, b0, b1);
+            }
+          }
+        }
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        if (stage == 0) phase ^= 1;
+        __syncwarp();
+        if (issued < n_it) {
+          if ((issued & 31) == 0) locate(issued);
+          issue(issued);
+          ++issued;
+        }
+      }
+
+      // ---- join the warps: maxima and sums, then the scaled outputs
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) l[nt][c] += __shfl_xor_sync(~0u, l[nt][c], x);
+          if (g == 0) {
+            s_m[warp * C::kRows + 8 * nt + 2 * t + c] = m[nt][c];
+            s_l[warp * C::kRows + 8 * nt + 2 * t + c] = l[nt][c];
+          }
+        }
+      if (!ok) *s_abort = 1;
+      __syncthreads();
+      if (*s_abort) {  // a wait ran out: no copy may still be landing when the CTA exits
+        ok = false;
+        break;
+      }
+      float* s_o = reinterpret_cast<float*>(smem);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float f[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float top = kNoScore;
+#pragma unroll
+          for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w * C::kRows + 8 * nt + 2 * t + c]);
+          f[c] = ex2_approx(m[nt][c] - top);
+          if (g == 0) s_f[warp * C::kRows + 8 * nt + 2 * t + c] = f[c];
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          float mn[2] = {0.f, 0.f};
+          if (QT == QT_Q4_1) {
+            mn[0] = __shfl_sync(~0u, omin[nt][0], 4 * n + t);
+            mn[1] = __shfl_sync(~0u, omin[nt][1], 4 * n + t);
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            *reinterpret_cast<float4*>(s_o + (warp * C::kRows + 8 * nt + 2 * t + c) * C::kOStride + 32 * n + 4 * g) =
+                make_float4((o[nt][2 * n][c] + mn[c]) * f[c], (o[nt][2 * n][c + 2] + mn[c]) * f[c],
+                            (o[nt][2 * n + 1][c] + mn[c]) * f[c], (o[nt][2 * n + 1][c + 2] + mn[c]) * f[c]);
+        }
+      }
+      __syncthreads();
+      const bool split = ca > 0 || cb < n_chunks;
+      const long long unit = (long long)b * p.c.heads + head;
+      constexpr int kPart = C::kRows * (D + 2);
+      float* part = a.part + (2 * (long long)blockIdx.x + (unit_start > p0 ? 1 : 0)) * kPart;
+      auto finish = [&](int r, int d4, float4 v, float top, float sum) {
+        const int i = r / group_heads, h = head * group_heads + r % group_heads;
+        const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+        store_out(p, b * p.o_b + i * p.o_n + h * p.o_h + d4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        if (p.lse && d4 == 0)
+          p.lse[((long long)b * p.nq + i) * p.heads + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+      };
+      for (int e = threadIdx.x; e < n_rows * (D / 4); e += 32 * W) {
+        const int r = e / (D / 4), d4 = e % (D / 4) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f, top = kNoScore;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(s_o + (w * C::kRows + r) * C::kOStride + d4);
+          v.x += x.x;
+          v.y += x.y;
+          v.z += x.z;
+          v.w += x.w;
+          sum = fmaf(s_l[w * C::kRows + r], s_f[w * C::kRows + r], sum);
+          top = fmaxf(top, s_m[w * C::kRows + r]);
+        }
+        if (split) {
+          __stcg(reinterpret_cast<float4*>(part + r * D + d4), v);
+          if (d4 == 0) {
+            __stcg(part + C::kRows * D + r, top);
+            __stcg(part + C::kRows * (D + 1) + r, sum);
+          }
+        } else {
+          finish(r, d4, v, top, sum);
+        }
+      }
+      if (split) {
+        // CTAs whose shares touch the unit: those of its first and last chunk, and all between
+        const long long c0 = ((unit_start + 1) * ctas - 1) / total, c1 = ((unit_start + n_chunks) * ctas - 1) / total;
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) s_last = atomicAdd(a.count + unit, 1) == (int)(c1 - c0);
+        __syncthreads();
+        if (s_last) {
+          __threadfence();
+          auto part_of = [&](long long c) { return a.part + (2 * c + (unit_start > total * c / ctas ? 1 : 0)) * kPart; };
+          for (int e = threadIdx.x; e < n_rows * (D / 4); e += 32 * W) {
+            const int r = e / (D / 4), d4 = e % (D / 4) * 4;
+            float top = kNoScore, sum = 0.f;
+            for (long long c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(part_of(c) + C::kRows * D + r));
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (long long c = c0; c <= c1; ++c) {
+              const float* from = part_of(c);
+              const float f = ex2_approx(__ldcg(from + C::kRows * D + r) - top);
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(from + r * D + d4));
+              sum = fmaf(__ldcg(from + C::kRows * (D + 1) + r), f, sum);
+              v.x = fmaf(x.x, f, v.x);
+              v.y = fmaf(x.y, f, v.y);
+              v.z = fmaf(x.z, f, v.z);
+              v.w = fmaf(x.w, f, v.w);
+            }
+            finish(r, d4, v, top, sum);
+          }
+          if (threadIdx.x == 0) a.count[unit] = 0;
+        }
+      }
+      fence_proxy_async_smem();  // the ring is written by copies again
+      __syncthreads();
+    }
+    if (!ok) break;
+    base += (long long)n_chunks * p.c.heads;
+  }
+  if (!ok) {
+    // bounded: copies of this warp that were issued and not waited for
+    for (int s = 0; s < NS; ++s) {
+      const unsigned long long t0 = globaltimer_ns();
+      while (!mbar_try_wait(&full[s], s >= stage ? phase : phase ^ 1) && globaltimer_ns() - t0 < 10000000ull) {
+      }
+    }
+  }
+}
+
+template <int QT, int D, int NT, int W>
+int launch_rows(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
+  typedef Rows<QT, D, NT, W> C;
+  auto* k = rows_kernel<QT, D, NT, W>;
+  if (kernel_setup(k, C::kSmem) <= 0) return -13;
+  RowsArgs a;
+  a.p = p;
+  a.part = w.part;
+  a.count = w.count;
+  k<<<C::kCtas * w.sms, 32 * W, C::kSmem, st>>>(a, err);
+  return cudaGetLastError() == cudaSuccess ? 0 : -12;
+}
+
+// ---------------------------------------------------------------- any number of rows, one warp per query row
 template <int QT, int D, int KV>
 __device__ __forceinline__ float cached(const uint8_t* gp, int tok, int b, int lane) {
   typedef KvL<QT, D> L;
@@ -38,7 +677,6 @@ __device__ __forceinline__ float cached(const uint8_t* gp, int tok, int b, int l
   return (float)code * __half2float(sp[0]) + (QT == QT_Q4_1 ? __half2float(sp[L::kSc / 2]) : 0.f);
 }
 
-// One warp per query row, one token after the other.
 template <int QT, int D>
 __global__ void __launch_bounds__(128) row_kernel(KvAttnParams p, int* err) {
   typedef KvL<QT, D> L;
@@ -48,11 +686,8 @@ __global__ void __launch_bounds__(128) row_kernel(KvAttnParams p, int* err) {
   const int h = (int)(row % p.heads), i = (int)(row / p.heads % p.nq), b = (int)(row / p.heads / p.nq);
   const int kvh = h / (p.heads / p.c.heads);
   const int len = sequence_length(p, b, err);
-  int lo = 0, hi = len;
-  if (p.causal) {
-    hi = len - p.nq + i + 1;
-    if (p.window) lo = max(0, hi - p.window);
-  }
+  int lo, hi;
+  row_span(p, len, i, &lo, &hi);
   const __half* q = p.q + b * p.q_b + i * p.q_n + h * p.q_h;
   float qv[L::kNB], o[L::kNB];
 #pragma unroll
@@ -93,22 +728,53 @@ __global__ void __launch_bounds__(128) row_kernel(KvAttnParams p, int* err) {
   if (p.lse && lane == 0) p.lse[row] = hi > lo ? (m + log2f(l)) / kLog2e : -INFINITY;
 }
 
-typedef void (*AttnKernel)(KvAttnParams, int*);
+template <int QT, int D>
+int launch_row(const KvAttnParams& p, int* err, cudaStream_t st) {
+  const long long rows = (long long)p.batch * p.nq * p.heads;
+  if ((rows + 3) / 4 > 0x7fffffffLL) return -2;
+  row_kernel<QT, D><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(p, err);
+  return cudaGetLastError() == cudaSuccess ? 0 : -12;
+}
+
+// Rows of one key / value head that rows_kernel takes: the output registers of 8 rows are D / 4, so 8 * (256 / D).
+int most_rows(int d) { return 2048 / d; }
+
+template <int QT, int D, int W>
+int launch_rows_nt(const KvAttnParams& p, const KvAttnWork& w, int rows, int* err, cudaStream_t st) {
+  if (rows <= 8) return launch_rows<QT, D, 1, W>(p, w, err, st);
+  if (D <= 128 && rows <= 16) return launch_rows<QT, D, D <= 128 ? 2 : 1, W>(p, w, err, st);
+  return launch_rows<QT, D, D <= 64 ? 4 : 1, W>(p, w, err, st);
+}
+
+template <int QT, int D>
+int attend(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
+  const int rows = p.nq * (p.heads / p.c.heads);
+  if (rows > most_rows(D)) return launch_row<QT, D>(p, err, st);
+  constexpr int kMost = Rows<QT, D, 1, 4>::kWarps;
+  if ((long long)p.batch * p.c.heads >= 2 * w.sms) return launch_rows_nt<QT, D, 4>(p, w, rows, err, st);
+  return launch_rows_nt<QT, D, kMost>(p, w, rows, err, st);
+}
 
 template <int QT>
-AttnKernel attn_kernel(int d) {
-  return d == 64 ? row_kernel<QT, 64> : d == 128 ? row_kernel<QT, 128> : row_kernel<QT, 256>;
+int attend_d(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
+  return p.c.d == 64 ? attend<QT, 64>(p, w, err, st)
+                     : p.c.d == 128 ? attend<QT, 128>(p, w, err, st) : attend<QT, 256>(p, w, err, st);
 }
 
 }  // namespace
 
-int kv_attention(const KvAttnParams& p, int* err, cudaStream_t st) {
-  const long long rows = (long long)p.batch * p.nq * p.heads;
-  if ((rows + 3) / 4 > 0x7fffffffLL) return -2;
-  const AttnKernel k = p.c.type == QT_Q4_0 ? attn_kernel<QT_Q4_0>(p.c.d)
-                       : p.c.type == QT_Q4_1 ? attn_kernel<QT_Q4_1>(p.c.d) : attn_kernel<QT_Q8_0>(p.c.d);
-  k<<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(p, err);
-  return cudaGetLastError() == cudaSuccess ? 0 : -12;
+void kv_attention_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes) {
+  const int rows = p.nq * (p.heads / p.c.heads);
+  *part_bytes = *count_bytes = 0;
+  if (rows > most_rows(p.c.d)) return;
+  const int padded = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  *part_bytes = (size_t)2 * 8 * sms * padded * (p.c.d + 2) * 4;
+  *count_bytes = (size_t)p.batch * p.c.heads * 4;
+}
+
+int kv_attention(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
+  return p.c.type == QT_Q4_0 ? attend_d<QT_Q4_0>(p, w, err, st)
+                             : p.c.type == QT_Q4_1 ? attend_d<QT_Q4_1>(p, w, err, st) : attend_d<QT_Q8_0>(p, w, err, st);
 }
 
 }  // namespace s3b
