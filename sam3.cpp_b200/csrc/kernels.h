@@ -400,5 +400,8 @@ struct KvAttnWork {
 };
 void kv_attention_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes);
 int kv_attention(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st);
+// The tensor-core kernel for tiles of 128 query rows (kv_attention picks it for more rows than its own kernel takes).
+void kv_attention_tc_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes);
+int kv_attention_tc(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st);
 
 }  // namespace s3b

@@ -9,54 +9,11 @@
 // the weight before it is rounded to f16 (values), so no dequantised value is ever formed or rounded.
 #include <algorithm>
 
-#include "kv_cache.cuh"
+#include "kv_attention.cuh"
 
 namespace s3b {
 
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kNoScore = -1e30f;  // reference maximum before the first visible token: finite, so that no inf - inf arises
-
-// Tokens of sequence b, held to what its page table can name.
-__device__ __forceinline__ int sequence_length(const KvAttnParams& p, int b, int* err) {
-  const int n = p.lengths[b];
-  const int most = p.max_pages * p.c.page_size;
-  if (n < 0 || n > most) {
-    atomicCAS(err, 0, kDevErrIndex);
-    return n < 0 ? 0 : most;
-  }
-  return n;
-}
-
-// Tokens [lo, hi) that query i of a sequence of len tokens sees.
-__device__ __forceinline__ void row_span(const KvAttnParams& p, int len, int i, int* lo, int* hi) {
-  *lo = 0;
-  *hi = len;
-  if (p.causal) {
-    *hi = max(0, len - p.nq + i + 1);
-    if (p.window) *lo = max(0, *hi - p.window);
-  }
-}
-
-// Groups of 16 tokens [g0, g1) that queries [i0, i1] of a sequence of len tokens see between them.
-__device__ __forceinline__ void group_span(const KvAttnParams& p, int len, int i0, int i1, int* g0, int* g1) {
-  int lo, hi, none;
-  row_span(p, len, i0, &lo, &none);
-  row_span(p, len, i1, &none, &hi);
-  *g0 = lo >> 4;
-  *g1 = max(*g0, (hi + 15) >> 4);
-}
-
-__device__ __forceinline__ void store_out(const KvAttnParams& p, long long at, float4 v) {
-  if (p.out_f32) {
-    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = v;
-  } else {
-    __half2 h[2] = {__floats2half2_rn(v.x, v.y), __floats2half2_rn(v.z, v.w)};
-    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + at) = *reinterpret_cast<uint2*>(h);
-  }
-}
 
 // ---------------------------------------------------------------- fragments
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -71,30 +28,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-__device__ __forceinline__ uint32_t h2_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 u32_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-
-// Exact f16 pairs of the codes (less 8 for q4_0) whose nibbles lie at bits 0, 4, 8, 12 of each half of w: a nibble under
-// the exponent of 1024 reads 1024 + c at bit 0 and 1024 + 16 c at bit 4; one subtraction (or multiply-add by 1/16)
-// leaves the integer.
-template <int QT>
-__device__ __forceinline__ void nibble_pairs(uint32_t w, uint32_t (&out)[4]) {
-  const __half2 off0 = __float2half2_rn(QT == QT_Q4_0 ? -1032.f : -1024.f);
-  const __half2 off1 = __float2half2_rn(QT == QT_Q4_0 ? -72.f : -64.f);
-  const __half2 sixteenth = __float2half2_rn(0.0625f);
-  const uint32_t x = w >> 8;
-  out[0] = h2_u32(__hadd2(u32_h2((w & 0x000F000Fu) | 0x64006400u), off0));
-  out[1] = h2_u32(__hfma2(u32_h2((w & 0x00F000F0u) | 0x64006400u), sixteenth, off1));
-  out[2] = h2_u32(__hadd2(u32_h2((x & 0x000F000Fu) | 0x64006400u), off0));
-  out[3] = h2_u32(__hfma2(u32_h2((x & 0x00F000F0u) | 0x64006400u), sixteenth, off1));
-}
-// The same for the bytes 0, 1 and 2, 3 of w (8-bit codes with 128 added).
-__device__ __forceinline__ void byte_pairs(uint32_t w, uint32_t& a, uint32_t& b) {
-  const __half2 off = __float2half2_rn(-1152.f);
-  a = h2_u32(__hadd2(u32_h2(__byte_perm(w, 0x64646464u, 0x4140)), off));
-  b = h2_u32(__hadd2(u32_h2(__byte_perm(w, 0x64646464u, 0x4342)), off));
-}
-
 template <int BYTES>
 __device__ __forceinline__ void lds(const uint8_t* at, uint32_t (&r)[BYTES / 4]) {
   if (BYTES == 16) {
@@ -659,83 +592,7 @@ int launch_rows(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream
   return cudaGetLastError() == cudaSuccess ? 0 : -12;
 }
 
-// ---------------------------------------------------------------- any number of rows, one warp per query row
-template <int QT, int D, int KV>
-__device__ __forceinline__ float cached(const uint8_t* gp, int tok, int b, int lane) {
-  typedef KvL<QT, D> L;
-  const __half* sp = reinterpret_cast<const __half*>(gp + (KV ? L::v_scale(tok, b) : L::k_scale(tok, b)));
-  int code;
-  if (L::kBits == 8) {
-    code = (int)gp[KV ? L::v_val(tok, b, lane / 4) + lane % 4 : L::k_val(tok, b, lane / 8) + lane % 8] - 128;
-  } else if (KV) {
-    code = *reinterpret_cast<const uint16_t*>(gp + L::v_val(tok, b, lane / 4)) >> (4 * (lane % 4)) & 15;
-  } else {
-    code = *reinterpret_cast<const uint32_t*>(gp + L::k_val(tok, b, lane / 8)) >>
-               (4 * (lane % 8 / 2) + 16 * (lane % 2)) & 15;
-  }
-  if (QT == QT_Q4_0) code -= 8;
-  return (float)code * __half2float(sp[0]) + (QT == QT_Q4_1 ? __half2float(sp[L::kSc / 2]) : 0.f);
-}
-
-template <int QT, int D>
-__global__ void __launch_bounds__(128) row_kernel(KvAttnParams p, int* err) {
-  typedef KvL<QT, D> L;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= (long long)p.batch * p.nq * p.heads) return;
-  const int h = (int)(row % p.heads), i = (int)(row / p.heads % p.nq), b = (int)(row / p.heads / p.nq);
-  const int kvh = h / (p.heads / p.c.heads);
-  const int len = sequence_length(p, b, err);
-  int lo, hi;
-  row_span(p, len, i, &lo, &hi);
-  const __half* q = p.q + b * p.q_b + i * p.q_n + h * p.q_h;
-  float qv[L::kNB], o[L::kNB];
-#pragma unroll
-  for (int n = 0; n < L::kNB; ++n) {
-    qv[n] = __half2float(q[32 * n + lane]) * p.scale * kLog2e;
-    o[n] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int j = lo; j < hi; ++j) {
-    long long page = p.pages[b * p.pages_stride + j / p.c.page_size];
-    if (page < 0 || page >= p.c.n_pages) {
-      atomicCAS(err, 0, kDevErrIndex);
-      page = 0;
-    }
-    const int pos = j % p.c.page_size;
-    const uint8_t* gp = p.c.data + kv_group_offset<QT, D>(p.c, page, kvh, pos >> 4);
-    float s = 0.f;
-#pragma unroll
-    for (int n = 0; n < L::kNB; ++n) s += qv[n] * cached<QT, D, 0>(gp, pos & 15, n, lane);
-#pragma unroll
-    for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
-    const float m2 = fmaxf(m, s);
-    const float a = exp2f(m - m2), w = exp2f(s - m2);
-    m = m2;
-    l = l * a + w;
-#pragma unroll
-    for (int n = 0; n < L::kNB; ++n) o[n] = o[n] * a + w * cached<QT, D, 1>(gp, pos & 15, n, lane);
-  }
-  const float inv = hi > lo ? 1.f / l : 0.f;
-#pragma unroll
-  for (int n = 0; n < L::kNB; ++n) {
-    const long long at = b * p.o_b + i * p.o_n + h * p.o_h + 32 * n + lane;
-    if (p.out_f32)
-      reinterpret_cast<float*>(p.out)[at] = o[n] * inv;
-    else
-      reinterpret_cast<__half*>(p.out)[at] = __float2half_rn(o[n] * inv);
-  }
-  if (p.lse && lane == 0) p.lse[row] = hi > lo ? (m + log2f(l)) / kLog2e : -INFINITY;
-}
-
-template <int QT, int D>
-int launch_row(const KvAttnParams& p, int* err, cudaStream_t st) {
-  const long long rows = (long long)p.batch * p.nq * p.heads;
-  if ((rows + 3) / 4 > 0x7fffffffLL) return -2;
-  row_kernel<QT, D><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(p, err);
-  return cudaGetLastError() == cudaSuccess ? 0 : -12;
-}
-
+// ---------------------------------------------------------------- dispatch
 // Rows of one key / value head that rows_kernel takes: the output registers of 8 rows are D / 4, so 8 * (256 / D).
 int most_rows(int d) { return 2048 / d; }
 
@@ -749,7 +606,6 @@ int launch_rows_nt(const KvAttnParams& p, const KvAttnWork& w, int rows, int* er
 template <int QT, int D>
 int attend(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
   const int rows = p.nq * (p.heads / p.c.heads);
-  if (rows > most_rows(D)) return launch_row<QT, D>(p, err, st);
   constexpr int kMost = Rows<QT, D, 1, 4>::kWarps;
   if ((long long)p.batch * p.c.heads >= 2 * w.sms) return launch_rows_nt<QT, D, 4>(p, w, rows, err, st);
   return launch_rows_nt<QT, D, kMost>(p, w, rows, err, st);
@@ -764,15 +620,16 @@ int attend_d(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t 
 }  // namespace
 
 void kv_attention_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes) {
-  const int rows = p.nq * (p.heads / p.c.heads);
+  const long long rows = p.nq * (long long)(p.heads / p.c.heads);
   *part_bytes = *count_bytes = 0;
-  if (rows > most_rows(p.c.d)) return;
+  if (rows > most_rows(p.c.d)) return kv_attention_tc_work(p, sms, part_bytes, count_bytes);
   const int padded = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
   *part_bytes = (size_t)2 * 8 * sms * padded * (p.c.d + 2) * 4;
   *count_bytes = (size_t)p.batch * p.c.heads * 4;
 }
 
 int kv_attention(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
+  if (p.nq * (long long)(p.heads / p.c.heads) > most_rows(p.c.d)) return kv_attention_tc(p, w, err, st);
   return p.c.type == QT_Q4_0 ? attend_d<QT_Q4_0>(p, w, err, st)
                              : p.c.type == QT_Q4_1 ? attend_d<QT_Q4_1>(p, w, err, st) : attend_d<QT_Q8_0>(p, w, err, st);
 }

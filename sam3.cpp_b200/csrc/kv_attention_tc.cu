@@ -1,0 +1,944 @@
+// Attention over the quantised key / value cache for many query rows: tcgen05 tiles of 128 query rows by 128 tokens.
+//
+// A unit is one key / value head, one sequence and one block of TQ x 128 query rows (queries x heads of the group side by
+// side, so all of them share one pass over the cache). The line of 128-token tiles of all units is cut into equal shares,
+// one for each CTA (one per SM): uneven lengths, causal diagonals and few long units all fill the GPU. A unit that
+// several CTAs share leaves unnormalised parts in the workspace, and the last warp to arrive for its 32 rows joins them
+// in the order of the shares.
+//
+// Roles (16 warps):
+//   warps 0, 1     one thread each issues the MMAs of query tile 0 / 1: S = Q K^T (128 x 128 x D) into TMEM, then
+//                  O += P V (128 x D x 128) with P read from TMEM
+//   softmax        one warpgroup per query tile, a thread per query row with its 128 scores in registers: running
+//                  reference maximum (moved only when a row's maximum passes it by 2^8), p = 2^(s - m) written as f16
+//                  over the scores, sum in f32; at a unit's end O / sum to the output
+//   dequantising   the remaining warps read the cache in block form, one item (K or V of 128 tokens) ahead in registers,
+//                  and write f16 operands into a ring of 16 KB slots in the 128-byte swizzle; they also load Q
+// D = 64, 128: TQ = 2 tiles ping-pong (one softmax runs beside the other tile's MMAs), one S region each, so S_{j+1} of a
+// tile follows its P V_j. D = 256: one tile, two S regions (O takes half of TMEM), S_{j+1} beside the softmax of tile j.
+//
+// The f16 operand is code * scale (+ minimum) rounded once. The 16 tokens of a group stand in the order
+// 0 1 8 9 2 3 10 11 4 5 12 13 6 7 14 15 (both in K's rows and V's columns; a softmax does not mind), which is the order
+// in which a lane holds them, so V goes to shared memory transposed, [D values][64 tokens], in 8-byte pieces and is a
+// K-major operand like K.
+#include "kv_attention.cuh"
+
+namespace s3b {
+
+namespace {
+
+#define KV_TMEM_LD32(taddr, R)                                                                               \
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "                                                     \
+               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"                                     \
+               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"                    \
+               : "=r"((R)[0]), "=r"((R)[1]), "=r"((R)[2]), "=r"((R)[3]), "=r"((R)[4]), "=r"((R)[5]),         \
+                 "=r"((R)[6]), "=r"((R)[7]), "=r"((R)[8]), "=r"((R)[9]), "=r"((R)[10]), "=r"((R)[11]),       \
+                 "=r"((R)[12]), "=r"((R)[13]), "=r"((R)[14]), "=r"((R)[15]), "=r"((R)[16]), "=r"((R)[17]),   \
+                 "=r"((R)[18]), "=r"((R)[19]), "=r"((R)[20]), "=r"((R)[21]), "=r"((R)[22]), "=r"((R)[23]),   \
+                 "=r"((R)[24]), "=r"((R)[25]), "=r"((R)[26]), "=r"((R)[27]), "=r"((R)[28]), "=r"((R)[29]),   \
+                 "=r"((R)[30]), "=r"((R)[31])                                                                \
+               : "r"(taddr))
+#define KV_TMEM_ST32(taddr, R)                                                                               \
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "                                               \
+               "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"                                    \
+               "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),             \
+               "r"((R)[0]), "r"((R)[1]), "r"((R)[2]), "r"((R)[3]), "r"((R)[4]), "r"((R)[5]), "r"((R)[6]),    \
+               "r"((R)[7]), "r"((R)[8]), "r"((R)[9]), "r"((R)[10]), "r"((R)[11]), "r"((R)[12]),              \
+               "r"((R)[13]), "r"((R)[14]), "r"((R)[15]), "r"((R)[16]), "r"((R)[17]), "r"((R)[18]),           \
+               "r"((R)[19]), "r"((R)[20]), "r"((R)[21]), "r"((R)[22]), "r"((R)[23]), "r"((R)[24]),           \
+               "r"((R)[25]), "r"((R)[26]), "r"((R)[27]), "r"((R)[28]), "r"((R)[29]), "r"((R)[30]),           \
+               "r"((R)[31])                                                                                  \
+               : "memory")
+#define KV_TMEM_ST8(taddr, R)                                                                                \
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),        \
+               "r"((R)[0]), "r"((R)[1]), "r"((R)[2]), "r"((R)[3]), "r"((R)[4]), "r"((R)[5]), "r"((R)[6]),    \
+               "r"((R)[7])                                                                                   \
+               : "memory")
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// 2^x, x <= 8, on the FMA pipe (the range reduction and the degree-3 fit of attention_tc.cu's softmax).
+__device__ __forceinline__ float exp2_fma(float x) {
+  x = fmaxf(x, -126.f);
+  const float j = x + 12582912.f;
+  const float f = x - (j - 12582912.f);
+  const float p = fmaf(fmaf(fmaf(0.0551716685f, f, 0.2426111251f), f, 0.6932609677f), f, 0.9999280572f);
+  return __int_as_float(__float_as_int(p) + (__float_as_int(j) << 23));
+}
+
+constexpr int kTile = 128;          // query rows of a tile and tokens of a tile
+constexpr int kSlotBytes = 16384;   // 128 x 64 f16
+constexpr int kSlots = 8;
+constexpr float kLazy = 8.f;        // log2 of the largest weight before the reference maximum moves
+constexpr int kThreads = 512;
+constexpr int kPoly = 2;            // of every 8 exponentials, how many run on the FMA pipe
+
+template <int QT, int D>
+struct Tc {
+  typedef KvL<QT, D> L;
+  static constexpr int kTQ = D == 256 ? 1 : 2;
+  static constexpr int kSBuf = D == 256 ? 2 : 1;
+  static constexpr int kDeqWarp0 = D == 256 ? 8 : 12;
+  static constexpr int kDeqWarps = 16 - kDeqWarp0;
+  static constexpr int kParts = D / 64;                     // slots of an item (K: 64-value chunks; V: D x 64 tokens)
+  static constexpr int kNSB = D / L::kSB;                   // super-blocks of a row
+  static constexpr int kTasks = 8 * kNSB / kDeqWarps;       // (16-token group, super-block) tasks of a warp per item
+  static constexpr int kQBytes = kTQ * kTile * D * 2;
+  static constexpr int kSmem = 1024 + kQBytes + kSlots * kSlotBytes + 512;
+  static constexpr int kOCol = 256;                         // TMEM: S regions at 0 and 128, O after them
+  // register shares of the four warpgroups add up to the launch's 4 x 128
+  static constexpr int kRegsIssue = 56;
+  static constexpr int kRegsSoft = D == 256 ? 216 : 184;
+  static constexpr int kRegsDeq = D == 256 ? 120 : 88;
+  static constexpr int kPart = kTQ * kTile * (D + 2);       // floats of a unit's part
+};
+
+struct TcArgs {
+  KvAttnParams p;
+  float* part;  // [2 * grid][TQ][128 * D outputs, as [D / 4][128] float4; 128 maxima; 128 sums]
+  int* count;   // [kv heads][sequences x row blocks][TQ][4], zero between launches
+  int blocks;   // row blocks of a sequence
+};
+
+// Rows of a unit: packed row r = query * group + head of the group.
+struct Unit {
+  int b, head, row0;  // sequence, key / value head, first packed row
+  int len, t0, tiles; // tokens, first 128-token tile, tiles
+  int lo, hi;         // tokens that any row sees
+};
+
+template <int ROWS>
+__device__ __forceinline__ int unit_tiles(const KvAttnParams& p, int group, int len, int block, int* lo, int* hi) {
+  int none;
+  row_span(p, len, block * ROWS / group, lo, &none);
+  row_span(p, len, min(p.nq - 1, (block * ROWS + ROWS - 1) / group), &none, hi);
+  return *hi > *lo ? (*hi + kTile - 1) / kTile - *lo / kTile : 0;
+}
+
+// The segments (unit, tiles [ca, cb) of it) of the share [pos, end) of the line, in order.
+template <int ROWS>
+struct Walk {
+  const KvAttnParams& p;
+  int* err;
+  int group, blocks;
+  long long pos, end, start;  // start: position of the unit's first tile
+  int head, pair;
+  Unit u;
+  int ca, cb;
+  __device__ Walk(const KvAttnParams& p_, int* err_, int blocks_) : p(p_), err(err_), blocks(blocks_) {
+    group = p.heads / p.c.heads;
+  }
+  __device__ void load() {
+    u.b = pair / blocks;
+    u.head = head;
+    const int block = pair - u.b * blocks;
+    u.row0 = block * ROWS;
+    u.len = sequence_length(p, u.b, err);
+    u.tiles = unit_tiles<ROWS>(p, group, u.len, block, &u.lo, &u.hi);
+    u.t0 = u.lo / kTile;
+  }
+  __device__ bool next() {
+    while (pos < end) {
+      load();
+      if (pos < start + u.tiles) {
+        ca = (int)(pos - start);
+        cb = (int)min((long long)u.tiles, end - start);
+        pos += cb - ca;
+        return true;
+      }
+      start += u.tiles;
+      if (++pair == p.batch * blocks) {
+        pair = 0;
+        ++head;
+      }
+    }
+    return false;
+  }
+};
+
+// One task's raw bytes in registers: 16 tokens x one super-block of K or V.
+template <int QT, int D>
+struct Raw {
+  typedef KvL<QT, D> L;
+  static constexpr int kPW = L::kNBS * L::kBits / 2;          // words of both pieces
+  uint32_t w[kPW];
+  uint32_t s[L::kPlanes * 2 * L::kNBS];                       // V: 4 tokens x blocks; K: 2 tokens x blocks (half of it)
+};
+
+template <int WORDS>
+__device__ __forceinline__ void ldg(const uint8_t* at, uint32_t* r) {
+  if (WORDS == 4) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
+    r[0] = v.x;
+    r[1] = v.y;
+    r[2] = v.z;
+    r[3] = v.w;
+  } else if (WORDS == 2) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
+    r[0] = v.x;
+    r[1] = v.y;
+  } else {
+    r[0] = __ldg(reinterpret_cast<const uint32_t*>(at));
+  }
+}
+
+// token of a group that stands at position p
+__host__ __device__ constexpr int token_at(int p) { return 2 * (p >> 2) + (p & 1) + 8 * ((p >> 1) & 1); }
+
+// K task: lane l holds positions l % 8 and 8 + l % 8, quarter l / 8 of each block. gp null: tokens outside the sequence.
+template <int QT, int D>
+__device__ __forceinline__ void load_k(const uint8_t* gp, int sb, int lane, Raw<QT, D>& r) {
+  typedef KvL<QT, D> L;
+  constexpr int PW = Raw<QT, D>::kPW / 2;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int tok = token_at(8 * x + (lane & 7));
+    if (gp) {
+      ldg<PW>(gp + L::k_val(tok, sb * L::kNBS, lane >> 3), r.w + x * PW);
+#pragma unroll
+      for (int pl = 0; pl < L::kPlanes; ++pl)
+        ldg<L::kNBS / 2>(gp + pl * L::kSc + L::k_scale(tok, sb * L::kNBS), r.s + (pl * 2 + x) * (L::kNBS / 2));
+    }
+  }
+}
+// V task: lane (g, t) holds tokens 2t, 2t + 1 (+ 8), values 4g .. 4g + 3 of each block.
+template <int QT, int D>
+__device__ __forceinline__ void load_v(const uint8_t* gp, int sb, int lane, Raw<QT, D>& r) {
+  typedef KvL<QT, D> L;
+  constexpr int PW = Raw<QT, D>::kPW / 2;
+  const int g = lane >> 2, t = lane & 3;
+  if (!gp) return;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) ldg<PW>(gp + L::v_val(2 * t + 8 * x, sb * L::kNBS, g), r.w + x * PW);
+#pragma unroll
+  for (int pl = 0; pl < L::kPlanes; ++pl)
+#pragma unroll
+    for (int n = 0; n < L::kNBS; n += 2)
+      ldg<4>(gp + pl * L::kSc + L::v_scale(2 * t, sb * L::kNBS + n), r.s + (pl * L::kNBS + n) * 2);
+}
+
+template <int QT>
+__device__ __forceinline__ uint32_t scaled(uint32_t code, uint32_t s, uint32_t m) {
+  return QT == QT_Q4_1 ? h2_u32(__hfma2(u32_h2(code), u32_h2(s), u32_h2(m))) : h2_u32(__hmul2(u32_h2(code), u32_h2(s)));
+}
+
+// half n of the words s, twice
+__device__ __forceinline__ uint32_t both(const uint32_t* s, int n) {
+  return __byte_perm(s[n >> 1], 0, n & 1 ? 0x3232 : 0x1010);
+}
+
+// K task into the item at `item`: chunk (sb * kSB + 32 n) / 64, row = position in the tile, 16-byte column in the swizzle.
+template <int QT, int D>
+__device__ __forceinline__ void emit_k(const Raw<QT, D>& r, bool live, uint8_t* item, int grp, int sb, int lane) {
+  typedef KvL<QT, D> L;
+  constexpr int PW = Raw<QT, D>::kPW / 2;
+  const int l8 = lane & 7, t = lane >> 3;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    uint8_t* row = item + (grp * 16 + 8 * x + l8) * 128;
+    const uint32_t* s = r.s + x * (L::kNBS / 2);
+    const uint32_t* m = r.s + (2 + x) * (L::kNBS / 2);
+#pragma unroll
+    for (int n = 0; n < L::kNBS; ++n) {
+      uint32_t v[4];
+      if (QT == QT_Q8_0) {
+        byte_pairs(r.w[x * PW + 2 * n], v[0], v[1]);
+        byte_pairs(r.w[x * PW + 2 * n + 1], v[2], v[3]);
+      } else {
+        nibble_pairs<QT>(r.w[x * PW + n], v);
+      }
+      const uint32_t sc = both(s, n), mn = QT == QT_Q4_1 ? both(m, n) : 0u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = live ? scaled<QT>(v[e], sc, mn) : 0u;
+      *reinterpret_cast<uint4*>(row + (sb * L::kSB + 32 * n) / 64 * kSlotBytes + (((n & 1) * 4 + t) ^ l8) * 16) =
+          make_uint4(v[0], v[1], v[2], v[3]);
+    }
+  }
+}
+
+// V task into the item: half grp / 4 at D * 128 bytes, row = value, 64 tokens. Lanes whose rows would meet another lane's
+// banks (bit 1 of g) take the values of a block in the order 2, 3, 0, 1.
+template <int QT, int D>
+__device__ __forceinline__ void emit_v(const Raw<QT, D>& r, uint32_t keep0, uint32_t keep1, uint8_t* item, int grp, int sb,
+                                       int lane) {
+  typedef KvL<QT, D> L;
+  constexpr int PW = Raw<QT, D>::kPW / 2;
+  const int g = lane >> 2, t = lane & 3, f = (g >> 1) & 1;
+  uint8_t* base = item + (grp >> 2) * (D * 128) + (sb * L::kSB + 4 * g) * 128 + (t & 1) * 8;
+  const int at0 = (f << 8) | ((((t >> 1) ^ ((g & 1) * 4) ^ (2 * f)) * 16) ^ ((grp & 3) * 32));
+#pragma unroll
+  for (int n = 0; n < L::kNBS; ++n) {
+    uint32_t v0[4], v1[4];
+    if (QT == QT_Q8_0) {
+      const int lo = f ? 0x7362 : 0x5140, hi = f ? 0x5140 : 0x7362;
+      byte_pairs(__byte_perm(r.w[n], r.w[PW / 2 + n], lo), v0[0], v0[1]);
+      byte_pairs(__byte_perm(r.w[n], r.w[PW / 2 + n], hi), v0[2], v0[3]);
+      byte_pairs(__byte_perm(r.w[PW + n], r.w[PW + PW / 2 + n], lo), v1[0], v1[1]);
+      byte_pairs(__byte_perm(r.w[PW + n], r.w[PW + PW / 2 + n], hi), v1[2], v1[3]);
+    } else {
+      const int sel = n & 1 ? (f ? 0x6723 : 0x7632) : (f ? 0x4501 : 0x5410);
+      nibble_pairs<QT>(__byte_perm(r.w[n / 2], r.w[PW / 2 + n / 2], sel), v0);
+      nibble_pairs<QT>(__byte_perm(r.w[PW + n / 2], r.w[PW + PW / 2 + n / 2], sel), v1);
+    }
+    const uint32_t s0 = r.s[2 * n], s1 = r.s[2 * n + 1];
+    const uint32_t m0 = QT == QT_Q4_1 ? r.s[2 * (L::kNBS + n)] : 0u, m1 = QT == QT_Q4_1 ? r.s[2 * (L::kNBS + n) + 1] : 0u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      *reinterpret_cast<uint2*>(base + n * (32 * 128) + (at0 ^ (e * 144))) =
+          make_uint2(scaled<QT>(v0[e], s0, m0) & keep0, scaled<QT>(v1[e], s1, m1) & keep1);
+  }
+}
+
+// One token tile of one query row: the row's 128 scores from TMEM at `at`, the lazy reference maximum, the weights as f16
+// pairs over the first 64 columns, the sum into l. MASKED: only tokens [lo, hi) of the tile count. Returns true when the
+// maximum moved and the row of O has to be scaled by alpha.
+template <bool MASKED>
+__device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float sl2, float& m_ref, float& l, float& alpha) {
+  uint32_t r[kTile];
+  KV_TMEM_LD32(at, r);
+  KV_TMEM_LD32(at + 32, r + 32);
+  KV_TMEM_LD32(at + 64, r + 64);
+  KV_TMEM_LD32(at + 96, r + 96);
+  tc_wait_ld();
+  if (MASKED) {
+#pragma unroll
+    for (int c = 0; c < kTile; ++c) {
+      const int tok = (c & ~15) + token_at(c & 15);
+      if (tok < lo || tok >= hi) r[c] = __float_as_uint(-INFINITY);
+    }
+  }
+  float mx[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    mx[k] = max3(__uint_as_float(r[3 * k]), __uint_as_float(r[3 * k + 1]), __uint_as_float(r[3 * k + 2]));
+#pragma unroll
+  for (int c = 12; c < 124; c += 8)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1]));
+#pragma unroll
+  for (int k = 0; k < 2; ++k) mx[k] = max3(mx[k], __uint_as_float(r[124 + 2 * k]), __uint_as_float(r[125 + 2 * k]));
+  const float top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * sl2;
+  alpha = 1.f;
+  bool moved = false;
+  if (top > m_ref + kLazy) {
+    alpha = ex2_approx(m_ref - top);
+    m_ref = top;
+    l *= alpha;
+    moved = true;
+  }
+  const unsigned long long sl2x2 = f2_pack(sl2, sl2), negm2 = f2_pack(-m_ref, -m_ref);
+  unsigned long long acc0 = f2_pack(0.f, 0.f), acc1 = acc0;
+#pragma unroll
+  for (int c = 0; c < kTile / 16; ++c) {
+    uint32_t pk[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float pv[8];
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const int i = 16 * c + 8 * u + e;
+        float x0, x1;
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), sl2x2, negm2), x0, x1);
+        // a hidden token's -inf gives 0 exactly, so a row that sees nothing keeps the sum 0
+        pv[e] = !MASKED && e < kPoly ? exp2_fma(x0) : ex2_approx(x0);
+        pv[e + 1] = !MASKED && e + 1 < kPoly ? exp2_fma(x1) : ex2_approx(x1);
+      }
+      acc0 = f2_add(acc0, f2_add(f2_pack(pv[0], pv[1]), f2_pack(pv[4], pv[5])));
+      acc1 = f2_add(acc1, f2_add(f2_pack(pv[2], pv[3]), f2_pack(pv[6], pv[7])));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pk[4 * u + e] = h2_u32(__floats2half2_rn(pv[2 * e], pv[2 * e + 1]));
+    }
+    KV_TMEM_ST8(at + 8 * c, pk);
+  }
+  float a0, a1, b0, b1;
+  f2_unpack(acc0, a0, a1);
+  f2_unpack(acc1, b0, b1);
+  l += (a0 + a1) + (b0 + b1);
+  return moved;
+}
+
+template <int QT, int D>
+__global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constant__ TcArgs a, int* err) {
+  typedef KvL<QT, D> L;
+  typedef Tc<QT, D> C;
+  constexpr int TQ = C::kTQ, ROWS = TQ * kTile;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* s_q = smem;                       // [TQ][D / 64 chunks][128 rows][64]
+  uint8_t* s_ring = s_q + C::kQBytes;        // [kSlots] x 16 KB
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_ring + kSlots * kSlotBytes);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* full = bars + 2;                 // [kSlots]
+  uint64_t* empty = full + kSlots;           // [kSlots]
+  uint64_t* s_full = empty + kSlots;         // [2 regions]
+  uint64_t* p_full = s_full + 2;             // [2 tiles]
+  uint64_t* pv_done = p_full + 2;            // [2 tiles]
+  uint64_t* mma_done = pv_done + 2;          // [2 tiles]
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort_word, s_pair;
+  __shared__ long long s_sum[16], s_start;
+  volatile int* s_abort = &s_abort_word;
+
+  const KvAttnParams& p = a.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = p.heads / p.c.heads;
+  const int n_rows = p.nq * group;
+  const int pairs = p.batch * a.blocks;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, C::kDeqWarps);
+    mbar_init(q_empty, TQ);
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&full[s], C::kDeqWarps);
+      mbar_init(&empty[s], TQ);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x], 4);
+      mbar_init(&pv_done[x], 1);
+      mbar_init(&mma_done[x], 1);
+    }
+    s_abort_word = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 3) {
+    tmem_alloc(&s_tmem, 512);
+    tmem_relinquish();
+  }
+
+  // ---- tiles of one head, by sixteenths of the (sequence, row block) pairs; then the pair in which the share begins
+  const int per_warp = (pairs + 15) / 16;
+  auto pair_tiles = [&](int k) -> int {
+    if (k >= pairs) return 0;
+    const int b = k / a.blocks;
+    int lo, hi;
+    return unit_tiles<ROWS>(p, group, sequence_length(p, b, err), k - b * a.blocks, &lo, &hi);
+  };
+  {
+    long long sum = 0;
+    for (int k = warp * per_warp + lane; k < min(pairs, (warp + 1) * per_warp); k += 32) sum += pair_tiles(k);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
+    if (lane == 0) s_sum[warp] = sum;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  long long per_head = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) per_head += s_sum[w];
+  const long long total = per_head * p.c.heads;
+  const long long ctas = min((long long)gridDim.x, total);
+  const bool works = (int)blockIdx.x < ctas;
+  const long long p0 = works ? total * blockIdx.x / ctas : 0, p1 = works ? total * (blockIdx.x + 1) / ctas : 0;
+  if (works) {
+    const int head = (int)(p0 / per_head);
+    const long long rem = p0 - head * per_head;
+    long long before = 0;
+    int w = 0;
+    while (w < 15 && before + s_sum[w] <= rem) before += s_sum[w++];
+    if (warp == w) {
+      for (int k0 = w * per_warp;; k0 += 32) {
+        const long long n = k0 + lane < min(pairs, (w + 1) * per_warp) ? pair_tiles(k0 + lane) : 0;
+        long long end = n;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+          const long long up = __shfl_up_sync(~0u, end, x);
+          if (lane >= x) end += up;
+        }
+        const uint32_t past = __ballot_sync(~0u, before + end > rem);
+        if (past || k0 + 32 >= (w + 1) * per_warp) {
+          const int who = past ? __ffs(past) - 1 : 0;
+          const long long skipped = __shfl_sync(~0u, end - n, who);
+          if (lane == 0) {
+            s_pair = k0 + who;
+            s_start = head * per_head + before + skipped;
+          }
+          break;
+        }
+        before += __shfl_sync(~0u, end, 31);
+      }
+    }
+  }
+  __syncthreads();
+  auto walk = [&]() {
+    Walk<ROWS> w(p, err, a.blocks);
+    w.pos = p0;
+    w.end = p1;
+    w.start = s_start;
+    w.head = works ? (int)(p0 / per_head) : 0;
+    w.pair = s_pair;
+    return w;
+  };
+  const float sl2 = p.scale * kLog2e;
+
+  if (warp < 4) {
+    regs_dec<C::kRegsIssue>();
+    if (warp >= TQ) {
+      // row blocks that see no token
+      if (warp == 2)
+        for (int k = blockIdx.x; k < pairs; k += gridDim.x) {
+          if (pair_tiles(k)) continue;
+          const int b = k / a.blocks, row0 = (k - b * a.blocks) * ROWS;
+          for (int h = 0; h < p.c.heads; ++h)
+            for (int e = lane; e < min(ROWS, n_rows - row0) * (D / 4); e += 32) {
+              const int r = row0 + e / (D / 4), i = r / group, hq = h * group + r % group;
+              store_out(p, b * p.o_b + i * p.o_n + hq * p.o_h + e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+              if (p.lse && e % (D / 4) == 0) p.lse[((long long)b * p.nq + i) * p.heads + hq] = -INFINITY;
+            }
+        }
+    } else if (lane == 0) {
+      // ---- MMA issue for query tile `warp`
+      const int t = warp;
+      constexpr uint32_t idesc_s = idesc_f16(kTile, kTile, 0), idesc_o = idesc_f16(kTile, D, 0);
+      const uint32_t q_base = smem_u32(s_q) + t * (kTile * D * 2), ring = smem_u32(s_ring);
+      const uint32_t o_tmem = tmem + C::kOCol + t * D;
+      uint32_t slot = 0, q_n = 0, ns = 0, npv = 0;  // slots, Q loads, S and P V products so far
+      bool ok = true, issued = false;
+      auto wait_slot = [&](uint32_t s) -> bool {
+        if (!mbar_wait(&full[s % kSlots], (s / kSlots) & 1, s_abort, err, kErrWaitFull)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto s_region = [&](uint32_t n) -> uint32_t { return C::kSBuf == 2 ? (n & 1) : (uint32_t)t; };
+      auto issue_s = [&](bool last) -> bool {
+        const uint32_t reg = s_region(ns);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c, ++slot) {
+          if (!wait_slot(slot)) return false;
+          const uint64_t dq = sdesc_k_sw128(q_base + c * kSlotBytes);
+          const uint64_t dk = sdesc_k_sw128(ring + slot % kSlots * kSlotBytes);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            tc_mma_f16(tmem + 128 * reg, dq + kk * 2, dk + kk * 2, idesc_s, c != 0 || kk != 0);
+          tc_commit(&empty[slot % kSlots]);
+        }
+        tc_commit(&s_full[reg]);
+        if (last) tc_commit(q_empty);
+        ++ns;
+        issued = true;
+        return true;
+      };
+      auto issue_pv = [&](bool first) -> bool {
+        if (!mbar_wait(&p_full[t], npv & 1, s_abort, err, kErrWaitMisc)) return false;
+        tc_fence_after();
+        const uint32_t pa = tmem + 128 * s_region(npv);
+        const uint32_t item = ring + slot % kSlots * kSlotBytes;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (D > 64 || half == 0) {
+            if (!wait_slot(slot)) return false;
+          }
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            tc_mma_f16_ts(o_tmem, pa + half * 32 + kk * 8, sdesc_k_sw128(item + half * (D * 128)) + kk * 2, idesc_o,
+                          !first || half != 0 || kk != 0);
+          if (D == 64) {
+            if (half == 1) tc_commit(&empty[slot++ % kSlots]);
+          } else {
+#pragma unroll
+            for (int x = 0; x < D / 128; ++x) tc_commit(&empty[slot++ % kSlots]);
+          }
+        }
+        tc_commit(&pv_done[t]);
+        ++npv;
+        issued = true;
+        return true;
+      };
+      Walk<ROWS> w = walk();
+      while (ok && w.next()) {
+        const int n = w.cb - w.ca;
+        if (!mbar_wait(q_full, q_n & 1, s_abort, err, kErrWaitFull)) { ok = false; break; }
+        ++q_n;
+        tc_fence_after();
+        if (w.u.row0 + t * kTile >= n_rows) {
+          // no second tile: release the slots as they fill, so that the counts of both issuers stay in step
+          mbar_arrive(q_empty);
+          for (int x = 0; x < n * 2 * C::kParts && ok; ++x, ++slot) {
+            if (!wait_slot(slot)) { ok = false; break; }
+            mbar_arrive(&empty[slot % kSlots]);
+          }
+          continue;
+        }
+        if (!issue_s(n == 1)) { ok = false; break; }
+        for (int j = 0; j < n && ok; ++j) {
+          if (C::kSBuf == 2 && j + 1 < n && !issue_s(j + 2 == n)) { ok = false; break; }
+          if (!issue_pv(j == 0)) { ok = false; break; }
+          if (C::kSBuf == 1 && j + 1 < n && !issue_s(j + 2 == n)) { ok = false; break; }
+        }
+      }
+      if (issued) {
+        tc_commit(&mma_done[t]);
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_try_wait(&mma_done[t], 0)) {
+          if (globaltimer_ns() - t0 > kWaitNs) {
+            atomicCAS(err, 0, kErrWaitDrain);
+            break;
+          }
+        }
+      }
+    }
+  } else if (warp < 4 + 4 * TQ) {
+    // ---- softmax and output of query tile t, one row per thread
+    regs_inc<C::kRegsSoft>();
+    const int t = (warp - 4) >> 2, w4 = warp & 3, row = w4 * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(w4 * 32) << 16;
+    const uint32_t o_at = tmem + lane_off + C::kOCol + t * D;
+    uint32_t n = 0;  // token tiles of this query tile so far
+    bool ok = true;
+    Walk<ROWS> w = walk();
+    while (ok && w.next()) {
+      const int r0 = w.u.row0 + t * kTile;
+      if (r0 >= n_rows) continue;
+      const int r = r0 + row;
+      const int i = min(r, n_rows - 1) / group, h = w.u.head * group + r % group;
+      int lo, hi, all_lo, all_hi, none;
+      row_span(p, w.u.len, i, &lo, &hi);
+      row_span(p, w.u.len, r0 / group, &none, &all_hi);
+      row_span(p, w.u.len, min(n_rows - 1, r0 + kTile - 1) / group, &all_lo, &none);
+      float m_ref = kNoScore, l = 0.f;
+      for (int j = w.ca; j < w.cb; ++j, ++n) {
+        const uint32_t reg = C::kSBuf == 2 ? (n & 1) : (uint32_t)t;
+        if (!mbar_wait(&s_full[reg], (C::kSBuf == 2 ? n >> 1 : n) & 1, s_abort, err, kErrWaitTmemFull)) ok = false;
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t s_at = tmem + lane_off + 128 * reg;
+        const int tok0 = (w.u.t0 + j) * kTile;
+        float alpha;
+        const bool moved = tok0 >= all_lo && tok0 + kTile <= all_hi
+                               ? softmax_tile<false>(s_at, 0, 0, sl2, m_ref, l, alpha)
+                               : softmax_tile<true>(s_at, lo - tok0, hi - tok0, sl2, m_ref, l, alpha);
+        if (j > w.ca) {
+          // O is current once the previous P V product of this tile has completed
+          if (!mbar_wait(&pv_done[t], (n - 1) & 1, s_abort, err, kErrWaitMisc)) ok = false;
+          ok = __all_sync(~0u, ok);
+          if (!ok) break;
+          tc_fence_after();
+          if (__any_sync(~0u, moved)) {
+            const float f = moved ? alpha : 1.f;
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              KV_TMEM_LD32(o_at + c, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              KV_TMEM_ST32(o_at + c, o);
+            }
+          }
+        }
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      if (!ok) break;
+      if (!mbar_wait(&pv_done[t], (n - 1) & 1, s_abort, err, kErrWaitMisc)) ok = false;
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const bool real = r < n_rows;
+      const long long o_row = w.u.b * p.o_b + i * p.o_n + h * p.o_h;
+      auto finish = [&](int c, const float* v, float inv) {  // 32 values of the row from column c
+        if (!real) return;
+        if (p.out_f32) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + o_row + c + e) =
+                make_float4(v[e] * inv, v[e + 1] * inv, v[e + 2] * inv, v[e + 3] * inv);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint4 x;
+            x.x = h2_u32(__floats2half2_rn(v[e] * inv, v[e + 1] * inv));
+            x.y = h2_u32(__floats2half2_rn(v[e + 2] * inv, v[e + 3] * inv));
+            x.z = h2_u32(__floats2half2_rn(v[e + 4] * inv, v[e + 5] * inv));
+            x.w = h2_u32(__floats2half2_rn(v[e + 6] * inv, v[e + 7] * inv));
+            *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(p.out) + o_row + c + e) = x;
+          }
+        }
+      };
+      auto finish_lse = [&](float top, float sum) {
+        if (real && p.lse)
+          p.lse[((long long)w.u.b * p.nq + i) * p.heads + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+      };
+      if (w.ca == 0 && w.cb == w.u.tiles) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          KV_TMEM_LD32(o_at + c, o);
+          tc_wait_ld();
+          finish(c, reinterpret_cast<float*>(o), inv);
+        }
+        finish_lse(m_ref, l);
+        continue;
+      }
+      // part of a unit: outputs as [D / 4][128 rows] float4, maxima, sums
+      auto part_of = [&](long long c) -> float* {
+        return a.part + (2 * c + (w.start > total * c / ctas ? 1 : 0)) * C::kPart + t * (kTile * (D + 2));
+      };
+      float* mine = part_of(blockIdx.x);
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        KV_TMEM_LD32(o_at + c, o);
+        tc_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+          __stcg(reinterpret_cast<float4*>(mine) + (c + e) / 4 * kTile + row,
+                 make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                             __uint_as_float(o[e + 3])));
+      }
+      __stcg(mine + kTile * D + row, m_ref);
+      __stcg(mine + kTile * (D + 1) + row, l);
+      const long long c0 = ((w.start + 1) * ctas - 1) / total, c1 = ((w.start + w.u.tiles) * ctas - 1) / total;
+      int* count = a.count + ((((long long)w.head * pairs + w.pair) * TQ + t) << 2) + w4;
+      __threadfence();
+      __syncwarp();
+      int last = 0;
+      if (lane == 0) last = atomicAdd(count, 1) == (int)(c1 - c0);
+      if (!__shfl_sync(~0u, last, 0)) continue;
+      __threadfence();
+      float top = kNoScore, sum = 0.f;
+      for (long long c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(part_of(c) + kTile * D + row));
+      for (long long c = c0; c <= c1; ++c)
+        sum = fmaf(__ldcg(part_of(c) + kTile * (D + 1) + row), ex2_approx(__ldcg(part_of(c) + kTile * D + row) - top), sum);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = 0.f;
+        for (long long k = c0; k <= c1; ++k) {
+          const float* from = part_of(k);
+          const float f = ex2_approx(__ldcg(from + kTile * D + row) - top);
+          float4 x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = __ldcg(reinterpret_cast<const float4*>(from) + (c / 4 + e) * kTile + row);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[4 * e] = fmaf(x[e].x, f, v[4 * e]);
+            v[4 * e + 1] = fmaf(x[e].y, f, v[4 * e + 1]);
+            v[4 * e + 2] = fmaf(x[e].z, f, v[4 * e + 2]);
+            v[4 * e + 3] = fmaf(x[e].w, f, v[4 * e + 3]);
+          }
+        }
+        finish(c, v, inv);
+      }
+      finish_lse(top, sum);
+      if (lane == 0) *count = 0;
+    }
+  } else {
+    // ---- dequantising warps
+    if (C::kRegsDeq < 128) regs_dec<C::kRegsDeq>();
+    const int dw = warp - C::kDeqWarp0;
+    const int per_page = p.c.page_size >> 4;
+    uint32_t slot = 0, q_n = 0;
+    bool ok = true;
+    Raw<QT, D> raw[C::kTasks];
+    auto wait_empty = [&](uint32_t s) {
+      if (ok && !mbar_wait(&empty[s % kSlots], ((s / kSlots) & 1) ^ 1, s_abort, err, kErrWaitEmpty)) ok = false;
+      ok = __all_sync(~0u, ok);
+    };
+    auto publish = [&](uint64_t* bar) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    Walk<ROWS> w = walk();
+    while (ok && w.next()) {
+      const int* table = p.pages + w.u.b * p.pages_stride;
+      // lane k < 8: the address of group k of a tile, null outside the tokens that the unit sees
+      auto locate = [&](int j) -> const uint8_t* {
+        const int gi = (w.u.t0 + j) * 8 + (lane & 7);
+        if (j >= w.cb || gi * 16 >= w.u.hi || gi * 16 + 16 <= w.u.lo) return nullptr;
+        long long page = __ldg(table + gi / per_page);
+        if (page < 0 || page >= p.c.n_pages) {
+          atomicCAS(err, 0, kDevErrIndex);
+          page = 0;
+        }
+        return p.c.data + kv_group_offset<QT, D>(p.c, page, w.u.head, gi % per_page);
+      };
+      auto group_at = [&](const uint8_t* addr, int grp) -> const uint8_t* {
+        return reinterpret_cast<const uint8_t*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(addr), grp));
+      };
+      // task k of this warp in a K item (super-block after super-block) and in a V item (groups in order)
+      auto k_task = [&](int k, int* grp, int* sb) {
+        const int id = k * C::kDeqWarps + dw;
+        *grp = id & 7;
+        *sb = C::kNSB == 1 ? 0 : id >> 3;
+      };
+      auto v_task = [&](int k, int* grp, int* sb) {
+        const int id = k * C::kDeqWarps + dw;
+        *sb = id % C::kNSB;
+        *grp = id / C::kNSB;
+      };
+      auto load_k_task = [&](const uint8_t* addr, int k) {
+        int grp, sb;
+        k_task(k, &grp, &sb);
+        load_k<QT, D>(group_at(addr, grp), sb, lane, raw[k]);
+      };
+      auto load_v_task = [&](const uint8_t* addr, int k) {
+        int grp, sb;
+        v_task(k, &grp, &sb);
+        load_v<QT, D>(group_at(addr, grp), sb, lane, raw[k]);
+      };
+      // An item from the registers; each task's registers then take the same task of the next item (at null: none).
+      auto load_task = [&](bool next_k, const uint8_t* addr, int k) {
+        if (next_k)
+          load_k_task(addr, k);
+        else
+          load_v_task(addr, k);
+      };
+      auto k_item = [&](const uint8_t* addr, bool next_k, const uint8_t* next) {
+        constexpr int kPerSb = 8 / C::kDeqWarps;  // tasks of this warp per super-block
+        constexpr int kSlotsPerSb = L::kSB / 64;
+#pragma unroll
+        for (int k = 0; k < C::kTasks; ++k) {
+          int grp, sb;
+          k_task(k, &grp, &sb);
+          const uint32_t s0 = slot + k / kPerSb * kSlotsPerSb;
+          if (k % kPerSb == 0)
+#pragma unroll
+            for (int x = 0; x < kSlotsPerSb; ++x) wait_empty(s0 + x);
+          if (!ok) return;
+          emit_k<QT, D>(raw[k], group_at(addr, grp) != nullptr, s_ring + slot % kSlots * kSlotBytes, grp, sb, lane);
+          load_task(next_k, next, k);
+          if (k % kPerSb == kPerSb - 1) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane < kSlotsPerSb) mbar_arrive(&full[(s0 + lane) % kSlots]);
+          }
+        }
+        slot += C::kParts;
+      };
+      auto v_item = [&](int j, bool next_k, const uint8_t* next) {
+        constexpr int kPerPart = D > 64 ? C::kTasks / 2 : C::kTasks;  // tasks of this warp per half (D = 64: both)
+        constexpr int kSlotsPerPart = D > 64 ? D / 128 : 1;
+        const int tok0 = (w.u.t0 + j) * kTile;
+        const bool whole = tok0 >= w.u.lo && tok0 + kTile <= w.u.hi;
+#pragma unroll
+        for (int k = 0; k < C::kTasks; ++k) {
+          int grp, sb;
+          v_task(k, &grp, &sb);
+          const uint32_t s0 = slot + k / kPerPart * kSlotsPerPart;
+          if (k % kPerPart == 0)
+#pragma unroll
+            for (int x = 0; x < kSlotsPerPart; ++x) wait_empty(s0 + x);
+          if (!ok) return;
+          uint32_t keep0 = ~0u, keep1 = ~0u;
+          if (!whole) {
+            const int first = tok0 + grp * 16 + 2 * (lane & 3);
+            auto in = [&](int tok) -> bool { return tok >= w.u.lo && tok < w.u.hi; };
+            keep0 = (in(first) ? 0xFFFFu : 0u) | (in(first + 1) ? 0xFFFF0000u : 0u);
+            keep1 = (in(first + 8) ? 0xFFFFu : 0u) | (in(first + 9) ? 0xFFFF0000u : 0u);
+          }
+          emit_v<QT, D>(raw[k], keep0, keep1, s_ring + slot % kSlots * kSlotBytes, grp, sb, lane);
+          load_task(next_k, next, k);
+          if (k % kPerPart == kPerPart - 1) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane < kSlotsPerPart) mbar_arrive(&full[(s0 + lane) % kSlots]);
+          }
+        }
+        slot += C::kParts;
+      };
+
+      const uint8_t *at0 = locate(w.ca), *at1 = locate(w.ca + 1), *at2 = locate(w.ca + 2);  // of tiles j, j + 1, j + 2
+#pragma unroll
+      for (int k = 0; k < C::kTasks; ++k) load_k_task(at0, k);
+      // Q rows into the swizzled chunks
+      if (ok && !mbar_wait(q_empty, (q_n & 1) ^ 1, s_abort, err, kErrWaitEmpty)) ok = false;
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      ++q_n;
+      for (int e = dw * 32 + lane; e < ROWS * (D / 8); e += 32 * C::kDeqWarps) {
+        const int rr = e / (D / 8), c16 = e % (D / 8), r = w.u.row0 + rr;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < n_rows) {
+          const int i = r / group, h = w.u.head * group + r % group;
+          v = __ldg(reinterpret_cast<const uint4*>(p.q + w.u.b * p.q_b + i * p.q_n + h * p.q_h + c16 * 8));
+        }
+        *reinterpret_cast<uint4*>(s_q + rr / kTile * (kTile * D * 2) + c16 / 8 * kSlotBytes + rr % kTile * 128 +
+                                  ((c16 & 7) ^ (rr & 7)) * 16) = v;
+      }
+      publish(q_full);
+
+      // one S region: K_0 V_0 K_1 V_1 ...; two: K_0 K_1 V_0 K_2 V_1 ... V_last, the order in which the MMAs take them
+      if (C::kSBuf == 2) k_item(at0, w.ca + 1 < w.cb, w.ca + 1 < w.cb ? at1 : at0);
+      for (int j = w.ca; j < w.cb && ok; ++j) {
+        const uint8_t* at3 = locate(j + 3);
+        if (C::kSBuf == 1) {
+          k_item(at0, false, at0);
+          if (ok) v_item(j, true, at1);
+        } else {
+          if (j + 1 < w.cb) k_item(at1, false, at0);
+          if (ok) v_item(j, j + 2 < w.cb, j + 2 < w.cb ? at2 : at1);
+        }
+        at0 = at1;
+        at1 = at2;
+        at2 = at3;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 3) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int QT, int D>
+int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
+  typedef Tc<QT, D> C;
+  auto* k = tiles_kernel<QT, D>;
+  if (kernel_setup(k, C::kSmem) <= 0) return -13;
+  TcArgs a;
+  a.p = p;
+  a.part = w.part;
+  a.count = w.count;
+  a.blocks = (p.nq * (p.heads / p.c.heads) + C::kTQ * kTile - 1) / (C::kTQ * kTile);
+  k<<<w.sms, kThreads, C::kSmem, st>>>(a, err);
+  return cudaGetLastError() == cudaSuccess ? 0 : -12;
+}
+
+template <int QT>
+int launch_tiles_d(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
+  return p.c.d == 64 ? launch_tiles<QT, 64>(p, w, err, st)
+                     : p.c.d == 128 ? launch_tiles<QT, 128>(p, w, err, st) : launch_tiles<QT, 256>(p, w, err, st);
+}
+
+}  // namespace
+
+void kv_attention_tc_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes) {
+  const int tq = p.c.d == 256 ? 1 : 2;
+  const long long blocks = (p.nq * (long long)(p.heads / p.c.heads) + tq * kTile - 1) / (tq * kTile);
+  *part_bytes = (size_t)2 * sms * tq * kTile * (p.c.d + 2) * 4;
+  *count_bytes = (size_t)p.batch * p.c.heads * blocks * tq * 16;
+}
+
+int kv_attention_tc(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
+  return p.c.type == QT_Q4_0 ? launch_tiles_d<QT_Q4_0>(p, w, err, st)
+                             : p.c.type == QT_Q4_1 ? launch_tiles_d<QT_Q4_1>(p, w, err, st)
+                                                   : launch_tiles_d<QT_Q8_0>(p, w, err, st);
+}
+
+}  // namespace s3b
