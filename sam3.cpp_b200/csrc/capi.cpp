@@ -1502,7 +1502,7 @@ int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* 
   }
   rc = kv_attention(p, w, ctx->d_err, ctx->stream);
   if (rc) return set_error(ctx, launcher_status_code(rc), "cache_attention launch failed (%d)", rc);
-  count_launch(ctx);
+  count_launch(ctx, count_bytes ? 1 : 2);
   return kOk;
 }
 

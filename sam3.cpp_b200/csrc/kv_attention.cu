@@ -62,9 +62,9 @@ struct Rows {
   static constexpr int kJoin = W * kRows * kOStride * 4;
   static constexpr int kFixed = kQBytes + 3 * W * kRows * 4 + 1024;
   static constexpr int kBudget = (225 * 1024) / kCtas - kFixed - 1024;
-  static constexpr int kFit = kBudget / (W * L::kGroup);
+  static constexpr int kFit = kBudget / (W * (2 * L::kHalf));
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
-  static constexpr int kRing = W * kStages * L::kGroup;
+  static constexpr int kRing = W * kStages * (2 * L::kHalf);
   static constexpr int kMain = kRing > kJoin ? kRing : kJoin;
   static constexpr int kSmem = kMain + kFixed;
   static_assert(kStages >= 2 && kMain + kFixed + 1024 <= (227 * 1024) / kCtas, "shared memory of rows_kernel");
@@ -168,7 +168,8 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
 
   const long long p0 = total * blockIdx.x / ctas, p1 = total * (blockIdx.x + 1) / ctas;
   const float sl2 = p.scale * kLog2e;
-  uint8_t* ring = smem + warp * NS * L::kGroup;
+  const long long v_offset = (long long)per_page * L::kHalf;  // of a page's values from its keys
+  uint8_t* ring = smem + warp * NS * (2 * L::kHalf);
   uint64_t* full = bars + warp * NS;
   int stage = 0;
   uint32_t phase = 0;
@@ -202,18 +203,17 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
             atomicCAS(err, 0, kDevErrIndex);
             page = 0;
           }
-          src = kv_group_offset<QT, D>(p.c, page, head, gi % per_page);
+          src = kv_group_offset<QT, D>(p.c, page, head, 0, gi % per_page);
         }
       };
       int st_issue = stage;
       auto issue = [&](int it) {
         const long long from = __shfl_sync(~0u, src, it & 31);
         if (lane == 0) {
-          mbar_arrive_expect_tx(&full[st_issue], L::kGroup);
-          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                           smem_u32(ring + st_issue * L::kGroup)),
-                       "l"(p.c.data + from), "r"(L::kGroup), "r"(smem_u32(&full[st_issue]))
-                       : "memory");
+          mbar_arrive_expect_tx(&full[st_issue], (2 * L::kHalf));
+          uint8_t* to = ring + st_issue * (2 * L::kHalf);
+          bulk_load(to, p.c.data + from, L::kHalf, &full[st_issue]);
+          bulk_load(to + L::kHalf, p.c.data + from + v_offset, L::kHalf, &full[st_issue]);
         }
         st_issue = st_issue + 1 == NS ? 0 : st_issue + 1;
       };
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
         if (!mbar_wait(&full[stage], phase, s_abort, err, kErrWaitFull)) ok = false;
         ok = __all_sync(~0u, ok);
         if (!ok) break;
-        const uint8_t* gp = ring + stage * L::kGroup;
+        const uint8_t *gp = ring + stage * (2 * L::kHalf), *vp = gp + L::kHalf;
         const int tok0 = (first + it * W) * 16;
         const bool whole = tok0 >= max_lo && tok0 + 16 <= min_hi;
 
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
         if (QT == QT_Q4_1) {  // sum over tokens of weight * minimum, a row for each block
           uint32_t am[4] = {0, 0, 0, 0};
           if (g < NB) {
-            const uint2 v = *reinterpret_cast<const uint2*>(gp + L::kSc + L::v_scale(2 * t, g));
+            const uint2 v = *reinterpret_cast<const uint2*>(vp + L::kSc + L::v_scale(2 * t, g));
             am[0] = v.x & keep0;
             am[2] = v.y & keep1;
           }
@@ -416,8 +416,8 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
           constexpr int PB = L::kNBS * L::kBits;  // bytes of a lane's piece of two tokens
           constexpr int PW = PB / 8;              // words of a token's
           uint32_t va[PB / 4], vb[PB / 4];
-          lds<PB>(gp + L::v_val(2 * t, sb * L::kNBS, g), va);
-          lds<PB>(gp + L::v_val(2 * t + 8, sb * L::kNBS, g), vb);
+          lds<PB>(vp + L::v_val(2 * t, sb * L::kNBS, g), va);
+          lds<PB>(vp + L::v_val(2 * t + 8, sb * L::kNBS, g), vb);
 #pragma unroll
           for (int nn = 0; nn < L::kNBS; ++nn) {
             const int n = sb * L::kNBS + nn;
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
               nibble_pairs<QT>(__byte_perm(vb[nn / 2], vb[PW + nn / 2], nn & 1 ? 0x7632 : 0x5410), x1);
             }
             const uint32_t a0[4] = {x0[0], x0[1], x1[0], x1[1]}, a1[4] = {x0[2], x0[3], x1[2], x1[3]};
-            const uint2 sc = *reinterpret_cast<const uint2*>(gp + L::v_scale(2 * t, n));
+            const uint2 sc = *reinterpret_cast<const uint2*>(vp + L::v_scale(2 * t, n));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               const uint32_t b0 = h2_u32(__hmul2(u32_h2(w0[nt]), u32_h2(sc.x & keep0)));

@@ -47,6 +47,14 @@ __device__ __forceinline__ void store_out(const KvAttnParams& p, long long at, f
   }
 }
 
+// Asynchronous copy of `bytes` (a multiple of 16) from 16-byte aligned global memory, counted on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 // ---------------------------------------------------------------- codes
 __device__ __forceinline__ uint32_t h2_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 u32_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
@@ -56,9 +64,9 @@ __device__ __forceinline__ __half2 u32_h2(uint32_t u) { return *reinterpret_cast
 // leaves the integer.
 template <int QT>
 __device__ __forceinline__ void nibble_pairs(uint32_t w, uint32_t (&out)[4]) {
-  const __half2 off0 = __float2half2_rn(QT == QT_Q4_0 ? -1032.f : -1024.f);
-  const __half2 off1 = __float2half2_rn(QT == QT_Q4_0 ? -72.f : -64.f);
-  const __half2 sixteenth = __float2half2_rn(0.0625f);
+  const __half2 off0 = u32_h2(QT == QT_Q4_0 ? 0xE408E408u : 0xE400E400u);  // -1032, -1024
+  const __half2 off1 = u32_h2(QT == QT_Q4_0 ? 0xD480D480u : 0xD400D400u);  // -72, -64
+  const __half2 sixteenth = u32_h2(0x2C002C00u);
   const uint32_t x = w >> 8;
   out[0] = h2_u32(__hadd2(u32_h2((w & 0x000F000Fu) | 0x64006400u), off0));
   out[1] = h2_u32(__hfma2(u32_h2((w & 0x00F000F0u) | 0x64006400u), sixteenth, off1));
@@ -67,7 +75,7 @@ __device__ __forceinline__ void nibble_pairs(uint32_t w, uint32_t (&out)[4]) {
 }
 // The same for the bytes 0, 1 and 2, 3 of w (8-bit codes with 128 added).
 __device__ __forceinline__ void byte_pairs(uint32_t w, uint32_t& a, uint32_t& b) {
-  const __half2 off = __float2half2_rn(-1152.f);
+  const __half2 off = u32_h2(0xE480E480u);  // -1152
   a = h2_u32(__hadd2(u32_h2(__byte_perm(w, 0x64646464u, 0x4140)), off));
   b = h2_u32(__hadd2(u32_h2(__byte_perm(w, 0x64646464u, 0x4342)), off));
 }

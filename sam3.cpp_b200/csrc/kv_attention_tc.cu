@@ -3,8 +3,7 @@
 // A unit is one key / value head, one sequence and one block of TQ x 128 query rows (queries x heads of the group side by
 // side, so all of them share one pass over the cache). The line of 128-token tiles of all units is cut into equal shares,
 // one for each CTA (one per SM): uneven lengths, causal diagonals and few long units all fill the GPU. A unit that
-// several CTAs share leaves unnormalised parts in the workspace, and the last warp to arrive for its 32 rows joins them
-// in the order of the shares.
+// several CTAs share leaves unnormalised parts in the workspace, which join_kernel adds up in the order of the shares.
 //
 // Roles (16 warps):
 //   warps 0, 1     one thread each issues the MMAs of query tile 0 / 1: S = Q K^T (128 x 128 x D) into TMEM, then
@@ -12,8 +11,9 @@
 //   softmax        one warpgroup per query tile, a thread per query row with its 128 scores in registers: running
 //                  reference maximum (moved only when a row's maximum passes it by 2^8), p = 2^(s - m) written as f16
 //                  over the scores, sum in f32; at a unit's end O / sum to the output
-//   dequantising   the remaining warps read the cache in block form, one item (K or V of 128 tokens) ahead in registers,
-//                  and write f16 operands into a ring of 16 KB slots in the 128-byte swizzle; they also load Q
+//   warp 2         copies the cache in block form (bulk copies of the keys or values of 16 tokens) into a ring
+//   dequantising   the remaining warps turn that ring's contents into f16 operands in a ring of 16 KB slots in the
+//                  128-byte swizzle, item by item (K or V of 128 tokens); they also load Q
 // D = 64, 128: TQ = 2 tiles ping-pong (one softmax runs beside the other tile's MMAs), one S region each, so S_{j+1} of a
 // tile follows its P V_j. D = 256: one tile, two S regions (O takes half of TMEM), S_{j+1} beside the softmax of tile j.
 //
@@ -80,7 +80,7 @@ __device__ __forceinline__ float exp2_fma(float x) {
 
 constexpr int kTile = 128;          // query rows of a tile and tokens of a tile
 constexpr int kSlotBytes = 16384;   // 128 x 64 f16
-constexpr int kSlots = 8;
+constexpr int kUnit = 64;           // tokens of an entry of the block-form ring
 constexpr float kLazy = 8.f;        // log2 of the largest weight before the reference maximum moves
 constexpr int kThreads = 512;
 constexpr int kPoly = 2;            // of every 8 exponentials, how many run on the FMA pipe
@@ -96,20 +96,31 @@ struct Tc {
   static constexpr int kNSB = D / L::kSB;                   // super-blocks of a row
   static constexpr int kTasks = 8 * kNSB / kDeqWarps;       // (16-token group, super-block) tasks of a warp per item
   static constexpr int kQBytes = kTQ * kTile * D * 2;
-  static constexpr int kSmem = 1024 + kQBytes + kSlots * kSlotBytes + 512;
+  static constexpr int kSlots = D == 256 ? 6 : 8;
+  static constexpr int kUnitBytes = kUnit / 16 * L::kHalf;
+  static constexpr int kRawFit = (224 * 1024 - 1024 - kQBytes - kSlots * kSlotBytes - 512) / kUnitBytes;
+  static constexpr int kRaw = kRawFit > 8 ? 8 : kRawFit;  // entries of the block-form ring
+  static constexpr int kSmem = 1024 + kQBytes + kSlots * kSlotBytes + kRaw * kUnitBytes + 512;
+  static_assert(kRaw >= 3, "K of a tile takes two entries of tiles_kernel's ring, and one has to be on its way");
   static constexpr int kOCol = 256;                         // TMEM: S regions at 0 and 128, O after them
   // register shares of the four warpgroups add up to the launch's 4 x 128
-  static constexpr int kRegsIssue = 56;
-  static constexpr int kRegsSoft = D == 256 ? 216 : 184;
-  static constexpr int kRegsDeq = D == 256 ? 120 : 88;
+  static constexpr int kRegsIssue = 80;
+  static constexpr int kRegsSoft = D == 256 ? 192 : 176;
+  static constexpr int kRegsDeq = D == 256 ? 120 : 80;
   static constexpr int kPart = kTQ * kTile * (D + 2);       // floats of a unit's part
+};
+
+// A unit that several CTAs share, written by the CTA in whose share it begins (its entry's index).
+struct Shared {
+  int valid, b, head, row0;
+  int c1, second;  // last of its CTAs; whether its first CTA's part is that CTA's second
 };
 
 struct TcArgs {
   KvAttnParams p;
-  float* part;  // [2 * grid][TQ][128 * D outputs, as [D / 4][128] float4; 128 maxima; 128 sums]
-  int* count;   // [kv heads][sequences x row blocks][TQ][4], zero between launches
-  int blocks;   // row blocks of a sequence
+  float* part;     // [2 * grid][TQ][128 * D outputs, as [D / 4][128] float4; 128 maxima; 128 sums]
+  Shared* shared;  // [grid]
+  int blocks;      // row blocks of a sequence
 };
 
 // Rows of a unit: packed row r = query * group + head of the group.
@@ -127,106 +138,72 @@ __device__ __forceinline__ int unit_tiles(const KvAttnParams& p, int group, int 
   return *hi > *lo ? (*hi + kTile - 1) / kTile - *lo / kTile : 0;
 }
 
-// The segments (unit, tiles [ca, cb) of it) of the share [pos, end) of the line, in order.
-template <int ROWS>
+// The segments (unit, tiles [ca, cb) of it) of the share [pos, end) of the line, in order. Kept in shared memory, one for
+// each warp, so that the roles' loops hold only what they use.
 struct Walk {
-  const KvAttnParams& p;
-  int* err;
-  int group, blocks;
   long long pos, end, start;  // start: position of the unit's first tile
   int head, pair;
   Unit u;
-  int ca, cb;
-  __device__ Walk(const KvAttnParams& p_, int* err_, int blocks_) : p(p_), err(err_), blocks(blocks_) {
-    group = p.heads / p.c.heads;
-  }
-  __device__ void load() {
-    u.b = pair / blocks;
-    u.head = head;
-    const int block = pair - u.b * blocks;
+  int ca, cb, more;
+};
+
+// The next segment; false at the share's end. One thread.
+template <int ROWS>
+__device__ __forceinline__ bool walk_next(const KvAttnParams& p, int blocks, int* err, Walk* w) {
+  const int group = p.heads / p.c.heads;
+  w->more = 0;
+  while (w->pos < w->end) {
+    Unit u;
+    u.b = w->pair / blocks;
+    u.head = w->head;
+    const int block = w->pair - u.b * blocks;
     u.row0 = block * ROWS;
     u.len = sequence_length(p, u.b, err);
     u.tiles = unit_tiles<ROWS>(p, group, u.len, block, &u.lo, &u.hi);
     u.t0 = u.lo / kTile;
-  }
-  __device__ bool next() {
-    while (pos < end) {
-      load();
-      if (pos < start + u.tiles) {
-        ca = (int)(pos - start);
-        cb = (int)min((long long)u.tiles, end - start);
-        pos += cb - ca;
-        return true;
-      }
-      start += u.tiles;
-      if (++pair == p.batch * blocks) {
-        pair = 0;
-        ++head;
-      }
+    if (w->pos < w->start + u.tiles) {
+      w->u = u;
+      w->ca = (int)(w->pos - w->start);
+      w->cb = (int)min((long long)u.tiles, w->end - w->start);
+      w->pos += w->cb - w->ca;
+      w->more = 1;
+      break;
     }
-    return false;
+    w->start += u.tiles;
+    if (++w->pair == p.batch * blocks) {
+      w->pair = 0;
+      ++w->head;
+    }
   }
-};
-
-// One task's raw bytes in registers: 16 tokens x one super-block of K or V.
-template <int QT, int D>
-struct Raw {
-  typedef KvL<QT, D> L;
-  static constexpr int kPW = L::kNBS * L::kBits / 2;          // words of both pieces
-  uint32_t w[kPW];
-  uint32_t s[L::kPlanes * 2 * L::kNBS];                       // V: 4 tokens x blocks; K: 2 tokens x blocks (half of it)
-};
-
-template <int WORDS>
-__device__ __forceinline__ void ldg(const uint8_t* at, uint32_t* r) {
-  if (WORDS == 4) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
-    r[0] = v.x;
-    r[1] = v.y;
-    r[2] = v.z;
-    r[3] = v.w;
-  } else if (WORDS == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
-    r[0] = v.x;
-    r[1] = v.y;
-  } else {
-    r[0] = __ldg(reinterpret_cast<const uint32_t*>(at));
-  }
+  return w->more;
+}
+// The same for a whole warp.
+template <int ROWS>
+__device__ __forceinline__ bool walk_next_warp(const KvAttnParams& p, int blocks, int* err, Walk* w, int lane) {
+  __syncwarp();
+  if (lane == 0) walk_next<ROWS>(p, blocks, err, w);
+  __syncwarp();
+  return *const_cast<volatile int*>(&w->more) != 0;
 }
 
 // token of a group that stands at position p
 __host__ __device__ constexpr int token_at(int p) { return 2 * (p >> 2) + (p & 1) + 8 * ((p >> 1) & 1); }
 
-// K task: lane l holds positions l % 8 and 8 + l % 8, quarter l / 8 of each block. gp null: tokens outside the sequence.
-template <int QT, int D>
-__device__ __forceinline__ void load_k(const uint8_t* gp, int sb, int lane, Raw<QT, D>& r) {
-  typedef KvL<QT, D> L;
-  constexpr int PW = Raw<QT, D>::kPW / 2;
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int tok = token_at(8 * x + (lane & 7));
-    if (gp) {
-      ldg<PW>(gp + L::k_val(tok, sb * L::kNBS, lane >> 3), r.w + x * PW);
-#pragma unroll
-      for (int pl = 0; pl < L::kPlanes; ++pl)
-        ldg<L::kNBS / 2>(gp + pl * L::kSc + L::k_scale(tok, sb * L::kNBS), r.s + (pl * 2 + x) * (L::kNBS / 2));
-    }
+template <int WORDS>
+__device__ __forceinline__ void lds(const uint8_t* at, uint32_t* r) {
+  if (WORDS == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(at);
+    r[0] = v.x;
+    r[1] = v.y;
+    r[2] = v.z;
+    r[3] = v.w;
+  } else if (WORDS == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
+    r[0] = v.x;
+    r[1] = v.y;
+  } else {
+    r[0] = *reinterpret_cast<const uint32_t*>(at);
   }
-}
-// V task: lane (g, t) holds tokens 2t, 2t + 1 (+ 8), values 4g .. 4g + 3 of each block.
-template <int QT, int D>
-__device__ __forceinline__ void load_v(const uint8_t* gp, int sb, int lane, Raw<QT, D>& r) {
-  typedef KvL<QT, D> L;
-  constexpr int PW = Raw<QT, D>::kPW / 2;
-  const int g = lane >> 2, t = lane & 3;
-  if (!gp) return;
-#pragma unroll
-  for (int x = 0; x < 2; ++x) ldg<PW>(gp + L::v_val(2 * t + 8 * x, sb * L::kNBS, g), r.w + x * PW);
-#pragma unroll
-  for (int pl = 0; pl < L::kPlanes; ++pl)
-#pragma unroll
-    for (int n = 0; n < L::kNBS; n += 2)
-      ldg<4>(gp + pl * L::kSc + L::v_scale(2 * t, sb * L::kNBS + n), r.s + (pl * L::kNBS + n) * 2);
 }
 
 template <int QT>
@@ -234,70 +211,89 @@ __device__ __forceinline__ uint32_t scaled(uint32_t code, uint32_t s, uint32_t m
   return QT == QT_Q4_1 ? h2_u32(__hfma2(u32_h2(code), u32_h2(s), u32_h2(m))) : h2_u32(__hmul2(u32_h2(code), u32_h2(s)));
 }
 
-// half n of the words s, twice
-__device__ __forceinline__ uint32_t both(const uint32_t* s, int n) {
-  return __byte_perm(s[n >> 1], 0, n & 1 ? 0x3232 : 0x1010);
-}
-
-// K task into the item at `item`: chunk (sb * kSB + 32 n) / 64, row = position in the tile, 16-byte column in the swizzle.
+// Keys of 16 tokens (at `half`, block form), super-block sb, into its slots at `item`: chunk n / 2, row =
+// position in the tile, 16-byte column in the swizzle. Lane (g, t) takes tokens g and g + 8, quarter t of each block:
+// reads and writes then meet no bank twice once the lanes of odd rows take the blocks of a pair in the other order. Rows
+// of tokens outside the sequence may hold anything: their scores are masked.
 template <int QT, int D>
-__device__ __forceinline__ void emit_k(const Raw<QT, D>& r, bool live, uint8_t* item, int grp, int sb, int lane) {
+__device__ __forceinline__ void emit_k(const uint8_t* half, uint8_t* item, int grp, int sb, int lane) {
   typedef KvL<QT, D> L;
-  constexpr int PW = Raw<QT, D>::kPW / 2;
-  const int l8 = lane & 7, t = lane >> 3;
+  constexpr int PW = L::kNBS * L::kBits / 4, PB = PW / L::kNBS;  // words of a piece, of a block in it
+  const int g = lane >> 2, t = lane & 3, odd = g & 1;
+  const uint32_t sel[2] = {odd ? 0x3232u : 0x1010u, odd ? 0x1010u : 0x3232u};
+  uint32_t w[2][PW], s[2][L::kNBS / 2], m[2][L::kNBS / 2];
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    uint8_t* row = item + (grp * 16 + 8 * x + l8) * 128;
-    const uint32_t* s = r.s + x * (L::kNBS / 2);
-    const uint32_t* m = r.s + (2 + x) * (L::kNBS / 2);
+    lds<PW>(half + L::k_val(g + 8 * x, sb * L::kNBS, t), w[x]);
+    lds<L::kNBS / 2>(half + L::k_scale(g + 8 * x, sb * L::kNBS), s[x]);
+    if (QT == QT_Q4_1) lds<L::kNBS / 2>(half + L::kSc + L::k_scale(g + 8 * x, sb * L::kNBS), m[x]);
+  }
+  // position of token g: 4 (g / 2) + g % 2, of token g + 8: two further
+  uint8_t* row = item + (grp * 16 + 4 * (g >> 1) + odd) * 128;
+  const int col = (odd * 4 + t) ^ (4 * ((g >> 1) & 1) + odd);  // of the first block taken, for token g
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
 #pragma unroll
     for (int n = 0; n < L::kNBS; ++n) {
-      uint32_t v[4];
-      if (QT == QT_Q8_0) {
-        byte_pairs(r.w[x * PW + 2 * n], v[0], v[1]);
-        byte_pairs(r.w[x * PW + 2 * n + 1], v[2], v[3]);
-      } else {
-        nibble_pairs<QT>(r.w[x * PW + n], v);
-      }
-      const uint32_t sc = both(s, n), mn = QT == QT_Q4_1 ? both(m, n) : 0u;
+      uint32_t v[4], u[PB];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = live ? scaled<QT>(v[e], sc, mn) : 0u;
-      *reinterpret_cast<uint4*>(row + (sb * L::kSB + 32 * n) / 64 * kSlotBytes + (((n & 1) * 4 + t) ^ l8) * 16) =
+      for (int e = 0; e < PB; ++e) u[e] = odd ? w[x][(n ^ 1) * PB + e] : w[x][n * PB + e];
+      if (QT == QT_Q8_0) {
+        byte_pairs(u[0], v[0], v[1]);
+        byte_pairs(u[PB - 1], v[2], v[3]);
+      } else {
+        nibble_pairs<QT>(u[0], v);
+      }
+      const uint32_t sc = __byte_perm(s[x][n >> 1], 0, sel[n & 1]);
+      const uint32_t mn = QT == QT_Q4_1 ? __byte_perm(m[x][n >> 1], 0, sel[n & 1]) : 0u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = scaled<QT>(v[e], sc, mn);
+      *reinterpret_cast<uint4*>(row + x * 256 + n / 2 * kSlotBytes + ((col ^ (4 * (n & 1)) ^ (2 * x)) * 16)) =
           make_uint4(v[0], v[1], v[2], v[3]);
     }
   }
 }
 
-// V task into the item: half grp / 4 at D * 128 bytes, row = value, 64 tokens. Lanes whose rows would meet another lane's
-// banks (bit 1 of g) take the values of a block in the order 2, 3, 0, 1.
+// Values of 16 tokens (at `half`), super-block sb, into the slots of their 64 tokens at `item`, row = value.
+// Lane (g, t) holds tokens 2t, 2t + 1, 2t + 8, 2t + 9 (positions 4t .. 4t + 3), values 4g .. 4g + 3 of each block; lanes
+// whose rows would meet another lane's banks (bit 1 of g) take the values in the order 2, 3, 0, 1. keep: masks of the
+// token pairs that the sequence holds; the scales of others count as zero.
 template <int QT, int D>
-__device__ __forceinline__ void emit_v(const Raw<QT, D>& r, uint32_t keep0, uint32_t keep1, uint8_t* item, int grp, int sb,
+__device__ __forceinline__ void emit_v(const uint8_t* half, uint32_t keep0, uint32_t keep1, uint8_t* item, int grp, int sb,
                                        int lane) {
   typedef KvL<QT, D> L;
-  constexpr int PW = Raw<QT, D>::kPW / 2;
+  constexpr int PW = L::kNBS * L::kBits / 4, TW = PW / 2;  // words of a piece (two tokens), of a token
   const int g = lane >> 2, t = lane & 3, f = (g >> 1) & 1;
-  uint8_t* base = item + (grp >> 2) * (D * 128) + (sb * L::kSB + 4 * g) * 128 + (t & 1) * 8;
+  uint32_t w0[PW], w1[PW], s[2 * L::kNBS], m[2 * L::kNBS];
+  lds<PW>(half + L::v_val(2 * t, sb * L::kNBS, g), w0);
+  lds<PW>(half + L::v_val(2 * t + 8, sb * L::kNBS, g), w1);
+#pragma unroll
+  for (int n = 0; n < L::kNBS; n += 2) {
+    lds<4>(half + L::v_scale(2 * t, sb * L::kNBS + n), s + 2 * n);
+    if (QT == QT_Q4_1) lds<4>(half + L::kSc + L::v_scale(2 * t, sb * L::kNBS + n), m + 2 * n);
+  }
+  uint8_t* base = item + (sb * L::kSB + 4 * g) * 128 + (t & 1) * 8;
   const int at0 = (f << 8) | ((((t >> 1) ^ ((g & 1) * 4) ^ (2 * f)) * 16) ^ ((grp & 3) * 32));
 #pragma unroll
   for (int n = 0; n < L::kNBS; ++n) {
     uint32_t v0[4], v1[4];
     if (QT == QT_Q8_0) {
       const int lo = f ? 0x7362 : 0x5140, hi = f ? 0x5140 : 0x7362;
-      byte_pairs(__byte_perm(r.w[n], r.w[PW / 2 + n], lo), v0[0], v0[1]);
-      byte_pairs(__byte_perm(r.w[n], r.w[PW / 2 + n], hi), v0[2], v0[3]);
-      byte_pairs(__byte_perm(r.w[PW + n], r.w[PW + PW / 2 + n], lo), v1[0], v1[1]);
-      byte_pairs(__byte_perm(r.w[PW + n], r.w[PW + PW / 2 + n], hi), v1[2], v1[3]);
+      byte_pairs(__byte_perm(w0[n], w0[TW + n], lo), v0[0], v0[1]);
+      byte_pairs(__byte_perm(w0[n], w0[TW + n], hi), v0[2], v0[3]);
+      byte_pairs(__byte_perm(w1[n], w1[TW + n], lo), v1[0], v1[1]);
+      byte_pairs(__byte_perm(w1[n], w1[TW + n], hi), v1[2], v1[3]);
     } else {
       const int sel = n & 1 ? (f ? 0x6723 : 0x7632) : (f ? 0x4501 : 0x5410);
-      nibble_pairs<QT>(__byte_perm(r.w[n / 2], r.w[PW / 2 + n / 2], sel), v0);
-      nibble_pairs<QT>(__byte_perm(r.w[PW + n / 2], r.w[PW + PW / 2 + n / 2], sel), v1);
+      nibble_pairs<QT>(__byte_perm(w0[n / 2], w0[TW + n / 2], sel), v0);
+      nibble_pairs<QT>(__byte_perm(w1[n / 2], w1[TW + n / 2], sel), v1);
     }
-    const uint32_t s0 = r.s[2 * n], s1 = r.s[2 * n + 1];
-    const uint32_t m0 = QT == QT_Q4_1 ? r.s[2 * (L::kNBS + n)] : 0u, m1 = QT == QT_Q4_1 ? r.s[2 * (L::kNBS + n) + 1] : 0u;
+    const uint32_t s0 = s[2 * n] & keep0, s1 = s[2 * n + 1] & keep1;
+    const uint32_t m0 = QT == QT_Q4_1 ? m[2 * n] & keep0 : 0u, m1 = QT == QT_Q4_1 ? m[2 * n + 1] & keep1 : 0u;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       *reinterpret_cast<uint2*>(base + n * (32 * 128) + (at0 ^ (e * 144))) =
-          make_uint2(scaled<QT>(v0[e], s0, m0) & keep0, scaled<QT>(v1[e], s1, m1) & keep1);
+          make_uint2(scaled<QT>(v0[e], s0, m0), scaled<QT>(v1[e], s1, m1));
   }
 }
 
@@ -373,12 +369,13 @@ template <int QT, int D>
 __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constant__ TcArgs a, int* err) {
   typedef KvL<QT, D> L;
   typedef Tc<QT, D> C;
-  constexpr int TQ = C::kTQ, ROWS = TQ * kTile;
+  constexpr int TQ = C::kTQ, ROWS = TQ * kTile, kSlots = C::kSlots;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* s_q = smem;                       // [TQ][D / 64 chunks][128 rows][64]
   uint8_t* s_ring = s_q + C::kQBytes;        // [kSlots] x 16 KB
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_ring + kSlots * kSlotBytes);
+  uint8_t* s_raw = s_ring + kSlots * kSlotBytes;  // [kRaw] keys or values of 64 tokens in block form
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_raw + C::kRaw * C::kUnitBytes);
   uint64_t* q_full = bars;
   uint64_t* q_empty = bars + 1;
   uint64_t* full = bars + 2;                 // [kSlots]
@@ -387,9 +384,13 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   uint64_t* p_full = s_full + 2;             // [2 tiles]
   uint64_t* pv_done = p_full + 2;            // [2 tiles]
   uint64_t* mma_done = pv_done + 2;          // [2 tiles]
+  uint64_t* raw_full = mma_done + 2;         // [kRaw]
+  uint64_t* raw_empty = raw_full + C::kRaw;  // [kRaw]
+  static_assert((2 + 2 * kSlots + 8 + 2 * C::kRaw) * 8 <= 512, "barriers of tiles_kernel");
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort_word, s_pair;
   __shared__ long long s_sum[16], s_start;
+  __shared__ Walk s_walk[16];
   volatile int* s_abort = &s_abort_word;
 
   const KvAttnParams& p = a.p;
@@ -410,6 +411,10 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       mbar_init(&p_full[x], 4);
       mbar_init(&pv_done[x], 1);
       mbar_init(&mma_done[x], 1);
+    }
+    for (int x = 0; x < C::kRaw; ++x) {
+      mbar_init(&raw_full[x], 1);
+      mbar_init(&raw_empty[x], C::kDeqWarps);
     }
     s_abort_word = 0;
     fence_mbar_init();
@@ -476,33 +481,123 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     }
   }
   __syncthreads();
-  auto walk = [&]() {
-    Walk<ROWS> w(p, err, a.blocks);
+  Walk& w = s_walk[warp];
+  if (lane == 0) {
     w.pos = p0;
     w.end = p1;
     w.start = s_start;
     w.head = works ? (int)(p0 / per_head) : 0;
     w.pair = s_pair;
-    return w;
-  };
+  }
+  __syncwarp();
   const float sl2 = p.scale * kLog2e;
+  // Item x of a segment of n tiles: K or V of tile *j. One S region: K_0 V_0 K_1 V_1 ...; two: K_0 K_1 V_0 K_2 V_1 ...
+  // V_last; the order in which the MMAs take them.
+  auto order = [](int x, int n, int* j) -> bool {
+    if (C::kSBuf == 1 || x == 0) {
+      *j = x >> 1;
+      return !(x & 1);
+    }
+    const bool k = (x & 1) && x != 2 * n - 1;
+    *j = x == 2 * n - 1 ? n - 1 : k ? (x + 1) >> 1 : (x >> 1) - 1;
+    return k;
+  };
 
   if (warp < 4) {
     regs_dec<C::kRegsIssue>();
-    if (warp >= TQ) {
+    if (warp == 3) {
       // row blocks that see no token
-      if (warp == 2)
-        for (int k = blockIdx.x; k < pairs; k += gridDim.x) {
-          if (pair_tiles(k)) continue;
-          const int b = k / a.blocks, row0 = (k - b * a.blocks) * ROWS;
-          for (int h = 0; h < p.c.heads; ++h)
-            for (int e = lane; e < min(ROWS, n_rows - row0) * (D / 4); e += 32) {
-              const int r = row0 + e / (D / 4), i = r / group, hq = h * group + r % group;
-              store_out(p, b * p.o_b + i * p.o_n + hq * p.o_h + e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-              if (p.lse && e % (D / 4) == 0) p.lse[((long long)b * p.nq + i) * p.heads + hq] = -INFINITY;
+      for (int k = blockIdx.x; k < pairs; k += gridDim.x) {
+        if (pair_tiles(k)) continue;
+        const int b = k / a.blocks, row0 = (k - b * a.blocks) * ROWS;
+        for (int h = 0; h < p.c.heads; ++h)
+          for (int e = lane; e < min(ROWS, n_rows - row0) * (D / 4); e += 32) {
+            const int r = row0 + e / (D / 4), i = r / group, hq = h * group + r % group;
+            store_out(p, b * p.o_b + i * p.o_n + hq * p.o_h + e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+            if (p.lse && e % (D / 4) == 0) p.lse[((long long)b * p.nq + i) * p.heads + hq] = -INFINITY;
+          }
+      }
+    } else if (warp == 2) {
+      // ---- copies of the cache in block form: two ring entries per item, as few copies as the pages allow
+      const int per_page = p.c.page_size >> 4;
+      int entry = 0;
+      uint32_t phase = 0, armed = 0, armed_phase = 0;
+      bool ok = true;
+      while (ok && walk_next_warp<ROWS>(p, a.blocks, err, &w, lane)) {
+        const int* table = p.pages + w.u.b * p.pages_stride;
+        const int t0 = w.u.t0, ca = w.ca, cb = w.cb, head = w.u.head, g_lo = w.u.lo >> 4, g_hi = (w.u.hi + 15) >> 4;
+        // lane k < 8: where the keys of group k of tile j are, -1 outside the groups that the unit sees. A copy begins at a
+        // group that does not follow its predecessor in memory, and takes those that follow it.
+        auto locate = [&](int j) -> long long {
+          const int gi = (t0 + j) * 8 + (lane & 7);
+          if (j >= cb || gi < g_lo || gi >= g_hi) return -1;
+          long long page = __ldg(table + gi / per_page);
+          if (page < 0 || page >= p.c.n_pages) {
+            atomicCAS(err, 0, kDevErrIndex);
+            page = 0;
+          }
+          return kv_group_offset<QT, D>(p.c, page, head, 0, gi % per_page);
+        };
+        const long long v_offset = (long long)per_page * L::kHalf;
+        long long at0 = locate(ca), at1 = locate(ca + 1);  // of tiles j, j + 1
+        const int n = cb - ca;
+        int first = 0;
+        for (int x = 0; x < 2 * n && ok; ++x) {
+          int j;
+          const bool is_k = order(x, n, &j);
+          const long long mine = j == first ? at0 : at1;
+          const long long before = __shfl_up_sync(~0u, mine, 1);
+          const int grp = lane & 7;
+          // runs end at an entry's end too
+          const bool starts = lane < 8 && mine >= 0 && ((grp & 3) == 0 || before != mine - L::kHalf);
+          const uint32_t heads = __ballot_sync(~0u, starts), live = __ballot_sync(~0u, lane < 8 && mine >= 0);
+          for (int half = 0; half < 2; ++half) {
+            if (lane == 0) {
+              ok = mbar_wait(&raw_empty[entry], phase ^ 1, s_abort, err, kErrWaitEmpty);
+              const int groups = __popc(live >> (4 * half) & 15);
+              if (ok && groups) {
+                mbar_arrive_expect_tx(&raw_full[entry], groups * L::kHalf);
+                armed |= 1u << entry;
+                armed_phase = (armed_phase & ~(1u << entry)) | (phase << entry);
+              } else if (ok) {
+                mbar_arrive(&raw_full[entry]);
+                armed &= ~(1u << entry);
+              }
             }
+            ok = __shfl_sync(~0u, (int)ok, 0);
+            if (!ok) break;
+            if (starts && grp >> 2 == half) {
+              // groups up to the next start, the next hole or the entry's end
+              const uint32_t stop = (heads | ~live | 0xFFFFFFF0u << (4 * half)) >> (grp + 1);
+              bulk_load(s_raw + entry * C::kUnitBytes + (grp & 3) * L::kHalf, p.c.data + mine + (is_k ? 0 : v_offset),
+                        __ffs(stop) * L::kHalf, &raw_full[entry]);
+            }
+            __syncwarp();
+            if (++entry == C::kRaw) {
+              entry = 0;
+              phase ^= 1;
+            }
+          }
+          if (!is_k) {  // the last use of tile j's addresses
+            ++first;
+            at0 = at1;
+            at1 = locate(ca + first + 1);
+          }
         }
-    } else if (lane == 0) {
+      }
+      // no copy may still be landing when the CTA exits
+      if (lane == 0)
+        for (int x = 0; x < C::kRaw; ++x)
+          if (armed >> x & 1) {
+            const unsigned long long t0 = globaltimer_ns();
+            while (!mbar_try_wait(&raw_full[x], armed_phase >> x & 1)) {
+              if (globaltimer_ns() - t0 > kWaitNs) {
+                atomicCAS(err, 0, kErrWaitDrain);
+                break;
+              }
+            }
+          }
+    } else if (warp < TQ && lane == 0) {
       // ---- MMA issue for query tile `warp`
       const int t = warp;
       constexpr uint32_t idesc_s = idesc_f16(kTile, kTile, 0), idesc_o = idesc_f16(kTile, D, 0);
@@ -538,7 +633,6 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         if (!mbar_wait(&p_full[t], npv & 1, s_abort, err, kErrWaitMisc)) return false;
         tc_fence_after();
         const uint32_t pa = tmem + 128 * s_region(npv);
-        const uint32_t item = ring + slot % kSlots * kSlotBytes;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           if (D > 64 || half == 0) {
@@ -546,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
           }
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            tc_mma_f16_ts(o_tmem, pa + half * 32 + kk * 8, sdesc_k_sw128(item + half * (D * 128)) + kk * 2, idesc_o,
+            tc_mma_f16_ts(o_tmem, pa + half * 32 + kk * 8, sdesc_k_sw128(ring + slot % kSlots * kSlotBytes + (D == 64 ? half * (D * 128) : 0)) + kk * 2, idesc_o,
                           !first || half != 0 || kk != 0);
           if (D == 64) {
             if (half == 1) tc_commit(&empty[slot++ % kSlots]);
@@ -560,8 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         issued = true;
         return true;
       };
-      Walk<ROWS> w = walk();
-      while (ok && w.next()) {
+      while (ok && walk_next<ROWS>(p, a.blocks, err, &w)) {
         const int n = w.cb - w.ca;
         if (!mbar_wait(q_full, q_n & 1, s_abort, err, kErrWaitFull)) { ok = false; break; }
         ++q_n;
@@ -601,30 +694,28 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     const uint32_t o_at = tmem + lane_off + C::kOCol + t * D;
     uint32_t n = 0;  // token tiles of this query tile so far
     bool ok = true;
-    Walk<ROWS> w = walk();
-    while (ok && w.next()) {
+    if (t == 0 && row == 0) a.shared[blockIdx.x].valid = 0;
+    while (ok && walk_next_warp<ROWS>(p, a.blocks, err, &w, lane)) {
       const int r0 = w.u.row0 + t * kTile;
       if (r0 >= n_rows) continue;
-      const int r = r0 + row;
-      const int i = min(r, n_rows - 1) / group, h = w.u.head * group + r % group;
       int lo, hi, all_lo, all_hi, none;
-      row_span(p, w.u.len, i, &lo, &hi);
+      row_span(p, w.u.len, min(r0 + row, n_rows - 1) / group, &lo, &hi);
       row_span(p, w.u.len, r0 / group, &none, &all_hi);
       row_span(p, w.u.len, min(n_rows - 1, r0 + kTile - 1) / group, &all_lo, &none);
+      const int tok_first = (w.u.t0 + w.ca) * kTile, tok_end = (w.u.t0 + w.cb) * kTile;
       float m_ref = kNoScore, l = 0.f;
-      for (int j = w.ca; j < w.cb; ++j, ++n) {
+      for (int tok0 = tok_first; tok0 < tok_end; tok0 += kTile, ++n) {
         const uint32_t reg = C::kSBuf == 2 ? (n & 1) : (uint32_t)t;
         if (!mbar_wait(&s_full[reg], (C::kSBuf == 2 ? n >> 1 : n) & 1, s_abort, err, kErrWaitTmemFull)) ok = false;
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         tc_fence_after();
         const uint32_t s_at = tmem + lane_off + 128 * reg;
-        const int tok0 = (w.u.t0 + j) * kTile;
         float alpha;
         const bool moved = tok0 >= all_lo && tok0 + kTile <= all_hi
                                ? softmax_tile<false>(s_at, 0, 0, sl2, m_ref, l, alpha)
                                : softmax_tile<true>(s_at, lo - tok0, hi - tok0, sl2, m_ref, l, alpha);
-        if (j > w.ca) {
+        if (tok0 > tok_first) {
           // O is current once the previous P V product of this tile has completed
           if (!mbar_wait(&pv_done[t], (n - 1) & 1, s_abort, err, kErrWaitMisc)) ok = false;
           ok = __all_sync(~0u, ok);
@@ -653,18 +744,19 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       ok = __all_sync(~0u, ok);
       if (!ok) break;
       tc_fence_after();
+      const int r = r0 + row, i = min(r, n_rows - 1) / group, h = w.u.head * group + r % group;
       const bool real = r < n_rows;
       const long long o_row = w.u.b * p.o_b + i * p.o_n + h * p.o_h;
-      auto finish = [&](int c, const float* v, float inv) {  // 32 values of the row from column c
+      auto finish = [&](int c, const float* v, float inv) {  // 16 values of the row from column c
         if (!real) return;
         if (p.out_f32) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
+          for (int e = 0; e < 16; e += 4)
             *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + o_row + c + e) =
                 make_float4(v[e] * inv, v[e + 1] * inv, v[e + 2] * inv, v[e + 3] * inv);
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
+          for (int e = 0; e < 16; e += 8) {
             uint4 x;
             x.x = h2_u32(__floats2half2_rn(v[e] * inv, v[e + 1] * inv));
             x.y = h2_u32(__floats2half2_rn(v[e + 2] * inv, v[e + 3] * inv));
@@ -686,15 +778,13 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
           KV_TMEM_LD32(o_at + c, o);
           tc_wait_ld();
           finish(c, reinterpret_cast<float*>(o), inv);
+          finish(c + 16, reinterpret_cast<float*>(o) + 16, inv);
         }
         finish_lse(m_ref, l);
         continue;
       }
-      // part of a unit: outputs as [D / 4][128 rows] float4, maxima, sums
-      auto part_of = [&](long long c) -> float* {
-        return a.part + (2 * c + (w.start > total * c / ctas ? 1 : 0)) * C::kPart + t * (kTile * (D + 2));
-      };
-      float* mine = part_of(blockIdx.x);
+      // part of a unit that CTAs c0 .. c1 share: outputs as [D / 4][128 rows] float4, maxima, sums
+      float* mine = a.part + (2 * (long long)blockIdx.x + (w.start > p0 ? 1 : 0)) * C::kPart + t * (kTile * (D + 2));
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
@@ -708,165 +798,31 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       }
       __stcg(mine + kTile * D + row, m_ref);
       __stcg(mine + kTile * (D + 1) + row, l);
-      const long long c0 = ((w.start + 1) * ctas - 1) / total, c1 = ((w.start + w.u.tiles) * ctas - 1) / total;
-      int* count = a.count + ((((long long)w.head * pairs + w.pair) * TQ + t) << 2) + w4;
-      __threadfence();
-      __syncwarp();
-      int last = 0;
-      if (lane == 0) last = atomicAdd(count, 1) == (int)(c1 - c0);
-      if (!__shfl_sync(~0u, last, 0)) continue;
-      __threadfence();
-      float top = kNoScore, sum = 0.f;
-      for (long long c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(part_of(c) + kTile * D + row));
-      for (long long c = c0; c <= c1; ++c)
-        sum = fmaf(__ldcg(part_of(c) + kTile * (D + 1) + row), ex2_approx(__ldcg(part_of(c) + kTile * D + row) - top), sum);
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        float v[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = 0.f;
-        for (long long k = c0; k <= c1; ++k) {
-          const float* from = part_of(k);
-          const float f = ex2_approx(__ldcg(from + kTile * D + row) - top);
-          float4 x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = __ldcg(reinterpret_cast<const float4*>(from) + (c / 4 + e) * kTile + row);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            v[4 * e] = fmaf(x[e].x, f, v[4 * e]);
-            v[4 * e + 1] = fmaf(x[e].y, f, v[4 * e + 1]);
-            v[4 * e + 2] = fmaf(x[e].z, f, v[4 * e + 2]);
-            v[4 * e + 3] = fmaf(x[e].w, f, v[4 * e + 3]);
-          }
-        }
-        finish(c, v, inv);
+      if (w.ca == 0 && t == 0 && row == 0) {
+        Shared* e = a.shared + blockIdx.x;
+        e->valid = 1;
+        e->b = w.u.b;
+        e->head = w.u.head;
+        e->row0 = w.u.row0;
+        e->c1 = (int)(((w.start + w.u.tiles) * ctas - 1) / total);
+        e->second = w.start > p0;
       }
-      finish_lse(top, sum);
-      if (lane == 0) *count = 0;
     }
   } else {
     // ---- dequantising warps
     if (C::kRegsDeq < 128) regs_dec<C::kRegsDeq>();
     const int dw = warp - C::kDeqWarp0;
-    const int per_page = p.c.page_size >> 4;
     uint32_t slot = 0, q_n = 0;
+    int raw0 = 0;            // ring entry of the current item's first group
+    uint32_t raw_phase = 0;  // and its phase
     bool ok = true;
-    Raw<QT, D> raw[C::kTasks];
-    auto wait_empty = [&](uint32_t s) {
-      if (ok && !mbar_wait(&empty[s % kSlots], ((s / kSlots) & 1) ^ 1, s_abort, err, kErrWaitEmpty)) ok = false;
+    auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
+      if (ok && !mbar_wait(bar, parity, s_abort, err, code)) ok = false;
       ok = __all_sync(~0u, ok);
     };
-    auto publish = [&](uint64_t* bar) {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
-    };
-    Walk<ROWS> w = walk();
-    while (ok && w.next()) {
-      const int* table = p.pages + w.u.b * p.pages_stride;
-      // lane k < 8: the address of group k of a tile, null outside the tokens that the unit sees
-      auto locate = [&](int j) -> const uint8_t* {
-        const int gi = (w.u.t0 + j) * 8 + (lane & 7);
-        if (j >= w.cb || gi * 16 >= w.u.hi || gi * 16 + 16 <= w.u.lo) return nullptr;
-        long long page = __ldg(table + gi / per_page);
-        if (page < 0 || page >= p.c.n_pages) {
-          atomicCAS(err, 0, kDevErrIndex);
-          page = 0;
-        }
-        return p.c.data + kv_group_offset<QT, D>(p.c, page, w.u.head, gi % per_page);
-      };
-      auto group_at = [&](const uint8_t* addr, int grp) -> const uint8_t* {
-        return reinterpret_cast<const uint8_t*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(addr), grp));
-      };
-      // task k of this warp in a K item (super-block after super-block) and in a V item (groups in order)
-      auto k_task = [&](int k, int* grp, int* sb) {
-        const int id = k * C::kDeqWarps + dw;
-        *grp = id & 7;
-        *sb = C::kNSB == 1 ? 0 : id >> 3;
-      };
-      auto v_task = [&](int k, int* grp, int* sb) {
-        const int id = k * C::kDeqWarps + dw;
-        *sb = id % C::kNSB;
-        *grp = id / C::kNSB;
-      };
-      auto load_k_task = [&](const uint8_t* addr, int k) {
-        int grp, sb;
-        k_task(k, &grp, &sb);
-        load_k<QT, D>(group_at(addr, grp), sb, lane, raw[k]);
-      };
-      auto load_v_task = [&](const uint8_t* addr, int k) {
-        int grp, sb;
-        v_task(k, &grp, &sb);
-        load_v<QT, D>(group_at(addr, grp), sb, lane, raw[k]);
-      };
-      // An item from the registers; each task's registers then take the same task of the next item (at null: none).
-      auto load_task = [&](bool next_k, const uint8_t* addr, int k) {
-        if (next_k)
-          load_k_task(addr, k);
-        else
-          load_v_task(addr, k);
-      };
-      auto k_item = [&](const uint8_t* addr, bool next_k, const uint8_t* next) {
-        constexpr int kPerSb = 8 / C::kDeqWarps;  // tasks of this warp per super-block
-        constexpr int kSlotsPerSb = L::kSB / 64;
-#pragma unroll
-        for (int k = 0; k < C::kTasks; ++k) {
-          int grp, sb;
-          k_task(k, &grp, &sb);
-          const uint32_t s0 = slot + k / kPerSb * kSlotsPerSb;
-          if (k % kPerSb == 0)
-#pragma unroll
-            for (int x = 0; x < kSlotsPerSb; ++x) wait_empty(s0 + x);
-          if (!ok) return;
-          emit_k<QT, D>(raw[k], group_at(addr, grp) != nullptr, s_ring + slot % kSlots * kSlotBytes, grp, sb, lane);
-          load_task(next_k, next, k);
-          if (k % kPerSb == kPerSb - 1) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane < kSlotsPerSb) mbar_arrive(&full[(s0 + lane) % kSlots]);
-          }
-        }
-        slot += C::kParts;
-      };
-      auto v_item = [&](int j, bool next_k, const uint8_t* next) {
-        constexpr int kPerPart = D > 64 ? C::kTasks / 2 : C::kTasks;  // tasks of this warp per half (D = 64: both)
-        constexpr int kSlotsPerPart = D > 64 ? D / 128 : 1;
-        const int tok0 = (w.u.t0 + j) * kTile;
-        const bool whole = tok0 >= w.u.lo && tok0 + kTile <= w.u.hi;
-#pragma unroll
-        for (int k = 0; k < C::kTasks; ++k) {
-          int grp, sb;
-          v_task(k, &grp, &sb);
-          const uint32_t s0 = slot + k / kPerPart * kSlotsPerPart;
-          if (k % kPerPart == 0)
-#pragma unroll
-            for (int x = 0; x < kSlotsPerPart; ++x) wait_empty(s0 + x);
-          if (!ok) return;
-          uint32_t keep0 = ~0u, keep1 = ~0u;
-          if (!whole) {
-            const int first = tok0 + grp * 16 + 2 * (lane & 3);
-            auto in = [&](int tok) -> bool { return tok >= w.u.lo && tok < w.u.hi; };
-            keep0 = (in(first) ? 0xFFFFu : 0u) | (in(first + 1) ? 0xFFFF0000u : 0u);
-            keep1 = (in(first + 8) ? 0xFFFFu : 0u) | (in(first + 9) ? 0xFFFF0000u : 0u);
-          }
-          emit_v<QT, D>(raw[k], keep0, keep1, s_ring + slot % kSlots * kSlotBytes, grp, sb, lane);
-          load_task(next_k, next, k);
-          if (k % kPerPart == kPerPart - 1) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane < kSlotsPerPart) mbar_arrive(&full[(s0 + lane) % kSlots]);
-          }
-        }
-        slot += C::kParts;
-      };
-
-      const uint8_t *at0 = locate(w.ca), *at1 = locate(w.ca + 1), *at2 = locate(w.ca + 2);  // of tiles j, j + 1, j + 2
-#pragma unroll
-      for (int k = 0; k < C::kTasks; ++k) load_k_task(at0, k);
+    while (ok && walk_next_warp<ROWS>(p, a.blocks, err, &w, lane)) {
       // Q rows into the swizzled chunks
-      if (ok && !mbar_wait(q_empty, (q_n & 1) ^ 1, s_abort, err, kErrWaitEmpty)) ok = false;
-      ok = __all_sync(~0u, ok);
+      wait_all(q_empty, (q_n & 1) ^ 1, kErrWaitEmpty);
       if (!ok) break;
       ++q_n;
       for (int e = dw * 32 + lane; e < ROWS * (D / 8); e += 32 * C::kDeqWarps) {
@@ -879,22 +835,63 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         *reinterpret_cast<uint4*>(s_q + rr / kTile * (kTile * D * 2) + c16 / 8 * kSlotBytes + rr % kTile * 128 +
                                   ((c16 & 7) ^ (rr & 7)) * 16) = v;
       }
-      publish(q_full);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
 
-      // one S region: K_0 V_0 K_1 V_1 ...; two: K_0 K_1 V_0 K_2 V_1 ... V_last, the order in which the MMAs take them
-      if (C::kSBuf == 2) k_item(at0, w.ca + 1 < w.cb, w.ca + 1 < w.cb ? at1 : at0);
-      for (int j = w.ca; j < w.cb && ok; ++j) {
-        const uint8_t* at3 = locate(j + 3);
-        if (C::kSBuf == 1) {
-          k_item(at0, false, at0);
-          if (ok) v_item(j, true, at1);
-        } else {
-          if (j + 1 < w.cb) k_item(at1, false, at0);
-          if (ok) v_item(j, j + 2 < w.cb, j + 2 < w.cb ? at2 : at1);
+      const int n = w.cb - w.ca, tok_first = (w.u.t0 + w.ca) * kTile, lo = w.u.lo, hi = w.u.hi;
+      for (int x = 0; x < 2 * n && ok; ++x) {
+        int j;
+        const bool is_k = order(x, n, &j);
+        const int tok0 = tok_first + j * kTile;
+        const bool whole = tok0 >= lo && tok0 + kTile <= hi;
+        // tasks (16-token group, super-block) of this warp, in parts that are published on their own: a super-block of
+        // keys, 64 tokens of values (D = 64: the one slot)
+        constexpr int kPerK = 8 / C::kDeqWarps, kPerV = D > 64 ? C::kTasks / 2 : C::kTasks;
+        constexpr int kSlotsK = L::kSB / 64, kSlotsV = D > 64 ? D / 128 : 1;
+        const int per = is_k ? kPerK : kPerV, slots = is_k ? kSlotsK : kSlotsV;
+        // the ring entries of tokens 0 .. 63 and 64 .. 127
+        const int e1 = raw0 + 1 == C::kRaw ? 0 : raw0 + 1;
+        const uint32_t ph1 = e1 ? raw_phase : raw_phase ^ 1;
+#pragma unroll 1
+        for (int k0 = 0; k0 < C::kTasks; k0 += per) {
+          for (int y = 0; y < slots; ++y)
+            wait_all(&empty[(slot + y) % kSlots], (((slot + y) / kSlots) & 1) ^ 1, kErrWaitEmpty);
+          if (k0 == 0) wait_all(&raw_full[raw0], raw_phase, kErrWaitFull);
+          if (k0 == 0 ? is_k || D == 64 : !is_k) wait_all(&raw_full[e1], ph1, kErrWaitFull);
+          if (!ok) break;
+          uint8_t* dst = s_ring + slot % kSlots * kSlotBytes;
+#pragma unroll 1
+          for (int k = k0; k < k0 + per; ++k) {
+            const int id = k * C::kDeqWarps + dw;
+            const int grp = is_k ? id & 7 : id / C::kNSB;
+            const int sb = C::kNSB == 1 ? 0 : is_k ? id >> 3 : id % C::kNSB;
+            const uint8_t* half = s_raw + (grp < 4 ? raw0 : e1) * C::kUnitBytes + (grp & 3) * L::kHalf;
+            if (is_k) {
+              emit_k<QT, D>(half, dst, grp, sb, lane);
+            } else {
+              uint32_t keep0 = ~0u, keep1 = ~0u;
+              if (!whole) {
+                const int first = tok0 + grp * 16 + 2 * (lane & 3);
+                auto in = [&](int tok) -> bool { return tok >= lo && tok < hi; };
+                keep0 = (in(first) ? 0xFFFFu : 0u) | (in(first + 1) ? 0xFFFF0000u : 0u);
+                keep1 = (in(first + 8) ? 0xFFFFu : 0u) | (in(first + 9) ? 0xFFFF0000u : 0u);
+              }
+              emit_v<QT, D>(half, keep0, keep1, D == 64 ? dst + (grp >> 2) * (D * 128) : dst, grp, sb, lane);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane < slots) mbar_arrive(&full[(slot + lane) % kSlots]);
+          slot += slots;
         }
-        at0 = at1;
-        at1 = at2;
-        at2 = at3;
+        if (!ok) break;
+        if (lane < 2) mbar_arrive(&raw_empty[lane ? e1 : raw0]);
+        raw0 += 2;
+        if (raw0 >= C::kRaw) {
+          raw0 -= C::kRaw;
+          raw_phase ^= 1;
+        }
       }
     }
   }
@@ -906,6 +903,80 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   }
 }
 
+// Joins the parts of the units that several CTAs of tiles_kernel share: block (c, y) the rows 32 y .. 32 y + 31 of the unit
+// that begins in CTA c's share, if one does. HBM / L2 traffic only: each part is read once.
+template <int D, int TQ>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArgs a) {
+  constexpr int kPart = TQ * kTile * (D + 2), kMost = 160;
+  __shared__ float s_f[kMost][32], s_top[8][32], s_sum[8][32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c0 = blockIdx.x;
+  const Shared u = a.shared[c0];
+  if (!u.valid) return;
+  const KvAttnParams& p = a.p;
+  const int group = p.heads / p.c.heads, n_rows = p.nq * group;
+  const int tile = blockIdx.y >> 2, row0 = (blockIdx.y & 3) * 32;
+  if (u.row0 + tile * kTile + row0 >= n_rows) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = u.c1 - c0 + 1;
+  auto part_of = [&](int k) -> const float* {
+    return a.part + (2 * (long long)(c0 + k) + (k == 0 ? u.second : 0)) * kPart + tile * (kTile * (D + 2));
+  };
+  // factors of the parts, lane = row
+  float top = kNoScore;
+  for (int k = warp; k < n; k += 8) top = fmaxf(top, s_f[k][lane] = __ldcg(part_of(k) + kTile * D + row0 + lane));
+  s_top[warp][lane] = top;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = fmaxf(top, s_top[k][lane]);
+  float sum = 0.f;
+  for (int k = warp; k < n; k += 8) {
+    const float f = ex2_approx(s_f[k][lane] - top);
+    s_f[k][lane] = f;
+    sum = fmaf(__ldcg(part_of(k) + kTile * (D + 1) + row0 + lane), f, sum);
+  }
+  s_sum[warp][lane] = sum;
+  __syncthreads();
+  if (warp == 0 && p.lse) {
+    sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += s_sum[k][lane];
+    const int r = u.row0 + tile * kTile + row0 + lane;
+    if (r < n_rows)
+      p.lse[((long long)u.b * p.nq + r / group) * p.heads + u.head * group + r % group] =
+          sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  }
+  // warp w: rows 4 w .. 4 w + 3; lane: one row, every eighth float4 of it
+  const int rr = 4 * warp + (lane >> 3), r = u.row0 + tile * kTile + row0 + rr;
+  float total = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) total += s_sum[k][rr];
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  float4 v[D / 32];
+#pragma unroll
+  for (int x = 0; x < D / 32; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+  for (int k = 0; k < n; ++k) {
+    const float4* from = reinterpret_cast<const float4*>(part_of(k)) + (lane & 7) * kTile + row0 + rr;
+    const float f = s_f[k][rr];
+    float4 x[D / 32];
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) x[e] = __ldcg(from + 8 * e * kTile);
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      v[e].x = fmaf(x[e].x, f, v[e].x);
+      v[e].y = fmaf(x[e].y, f, v[e].y);
+      v[e].z = fmaf(x[e].z, f, v[e].z);
+      v[e].w = fmaf(x[e].w, f, v[e].w);
+    }
+  }
+  if (r >= n_rows) return;
+  const long long at = u.b * p.o_b + r / group * p.o_n + (u.head * group + r % group) * p.o_h + (lane & 7) * 4;
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e)
+    store_out(p, at + 32 * e, make_float4(v[e].x * inv, v[e].y * inv, v[e].z * inv, v[e].w * inv));
+}
+
 template <int QT, int D>
 int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
   typedef Tc<QT, D> C;
@@ -914,10 +985,22 @@ int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStrea
   TcArgs a;
   a.p = p;
   a.part = w.part;
-  a.count = w.count;
+  a.shared = reinterpret_cast<Shared*>(w.part + (size_t)2 * w.sms * C::kPart);
   a.blocks = (p.nq * (p.heads / p.c.heads) + C::kTQ * kTile - 1) / (C::kTQ * kTile);
+  if (w.sms > 160) return -2;  // join_kernel's table of factors
   k<<<w.sms, kThreads, C::kSmem, st>>>(a, err);
-  return cudaGetLastError() == cudaSuccess ? 0 : -12;
+  if (cudaGetLastError() != cudaSuccess) return -12;
+  // launched while tiles_kernel still runs; it waits for its end before it reads
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(w.sms, C::kTQ * 4);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_kernel<D, C::kTQ>, a) == cudaSuccess ? 0 : -12;
 }
 
 template <int QT>
@@ -930,9 +1013,8 @@ int launch_tiles_d(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStr
 
 void kv_attention_tc_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes) {
   const int tq = p.c.d == 256 ? 1 : 2;
-  const long long blocks = (p.nq * (long long)(p.heads / p.c.heads) + tq * kTile - 1) / (tq * kTile);
-  *part_bytes = (size_t)2 * sms * tq * kTile * (p.c.d + 2) * 4;
-  *count_bytes = (size_t)p.batch * p.c.heads * blocks * tq * 16;
+  *part_bytes = (size_t)2 * sms * tq * kTile * (p.c.d + 2) * 4 + sms * sizeof(Shared);
+  *count_bytes = 0;
 }
 
 int kv_attention_tc(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {

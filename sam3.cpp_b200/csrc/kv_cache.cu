@@ -55,7 +55,7 @@ struct Job {
 
 // Group address and token of a slot; false for a slot that is skipped.
 template <int QT, int D>
-__device__ __forceinline__ bool slot_group(const Job& j, long long slot, int head, uint8_t** group, int* tok) {
+__device__ __forceinline__ bool slot_group(const Job& j, long long slot, int head, int kv, uint8_t** group, int* tok) {
   if (slot < 0) return false;
   const long long page = slot / j.c.page_size;
   if (page >= j.c.n_pages) {
@@ -63,7 +63,7 @@ __device__ __forceinline__ bool slot_group(const Job& j, long long slot, int hea
     return false;
   }
   const int pos = (int)(slot - page * j.c.page_size);
-  *group = j.c.data + kv_group_offset<QT, D>(j.c, page, head, pos >> 4);
+  *group = j.c.data + kv_group_offset<QT, D>(j.c, page, head, kv, pos >> 4);
   *tok = pos & 15;
   return true;
 }
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(128) write_kernel(Job j) {
   if (i >= j.n) return;
   uint8_t* gp;
   int tok;
-  if (!slot_group<QT, D>(j, j.slots[i], head, &gp, &tok)) return;
+  if (!slot_group<QT, D>(j, j.slots[i], head, kv, &gp, &tok)) return;
   const T* src = reinterpret_cast<const T*>(kv ? j.r.v : j.r.k) + i * (kv ? j.r.v_n : j.r.k_n) +
                  head * (kv ? j.r.v_h : j.r.k_h) + b * 32;
   float x[32];
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(128) read_kernel(Job j) {
            b * 32;
   uint8_t* gp;
   int tok;
-  if (!slot_group<QT, D>(j, j.slots[i], head, &gp, &tok)) {
+  if (!slot_group<QT, D>(j, j.slots[i], head, kv, &gp, &tok)) {
     for (int e = 0; e < 32; ++e) dst[e] = (T)0.f;
     return;
   }

@@ -1,10 +1,10 @@
 // Layout of the quantised key / value cache, shared by the kernels that write, read and attend over it.
 //
-// The cache is a sequence of (page, head) regions, each a sequence of groups of 16 tokens. A group of KvL<QT, D>::kGroup
-// bytes holds, in this order, the key values, the value values, the key scales (q4_1: then the key minima) and the value
-// scales (then minima) of its 16 tokens. The order of the values inside a group is that of the m16n8k16 fragments of the
-// few-query attention kernel, so that lane (g, t) = (lane / 4, lane % 4) of a warp finds its share of the group as whole
-// 8- or 16-byte words, contiguous over the lanes:
+// The cache is a sequence of (page, head) regions; a region holds the keys of its tokens and then their values, both as a
+// sequence of groups of 16 tokens, so that the keys (or values) of neighbouring tokens of a page are one piece of memory.
+// A group of KvL<QT, D>::kHalf bytes holds its quantised values, then their scales, then for q4_1 their minima. The order
+// of the values inside a group is that of the m16n8k16 fragments of the few-query attention kernel, so that lane (g, t) =
+// (lane / 4, lane % 4) of a warp finds its share of the group as whole 8- or 16-byte words, contiguous over the lanes:
 //   keys    A operand of S^T = K Q^T, rows = tokens: lane (g, t) takes tokens g and g + 8, and of every block of 32 the
 //           8 consecutive values 8 t .. 8 t + 7 (the contraction may run in any order that Q shares).
 //   values  A operand of O^T = V^T P^T, columns = tokens: lane (g, t) takes tokens 2t, 2t + 1, 2t + 8, 2t + 9, and of
@@ -26,29 +26,29 @@ struct KvL {
   static constexpr int kVal = 16 * D * kBits / 8;                            // bytes of the keys (or values) of a group
   static constexpr int kPlanes = QT == QT_Q4_1 ? 2 : 1;                      // scale, minimum
   static constexpr int kSc = 16 * kNB * 2;                                   // bytes of one plane
-  static constexpr int kGroup = 2 * kVal + 2 * kPlanes * kSc;
+  static constexpr int kHalf = kVal + kPlanes * kSc;                         // bytes of a group
 
-  // byte offsets in a group
+  // byte offsets in a group of keys (k_) or of values (v_)
   // keys: values 8 t .. 8 t + 7 of block b of token tok (4 or 8 bytes)
   static __host__ __device__ constexpr int k_val(int tok, int b, int t) {
     return (b / kNBS) * kSuper + tok * (kSB * kBits / 8) + (t * kNBS + b % kNBS) * kBits;
   }
   // values: values 4 g .. 4 g + 3 of block b of token tok (2 or 4 bytes)
   static __host__ __device__ constexpr int v_val(int tok, int b, int g) {
-    return kVal + (b / kNBS) * kSuper +
+    return (b / kNBS) * kSuper +
            ((((tok >> 3) * 32 + g * 4 + ((tok & 7) >> 1)) * 2 + (tok & 1)) * kNBS + b % kNBS) * (kBits / 2);
   }
-  static __host__ __device__ constexpr int k_scale(int tok, int b) { return 2 * kVal + (tok * kNB + b) * 2; }
+  static __host__ __device__ constexpr int k_scale(int tok, int b) { return kVal + (tok * kNB + b) * 2; }
   // the four tokens of lane t (2t, 2t + 1, 2t + 8, 2t + 9) side by side
   static __host__ __device__ constexpr int v_scale(int tok, int b) {
-    return 2 * kVal + kPlanes * kSc + ((((tok & 7) >> 1) * kNB + b) * 4 + (tok & 1) + 2 * (tok >> 3)) * 2;
+    return kVal + ((((tok & 7) >> 1) * kNB + b) * 4 + (tok & 1) + 2 * (tok >> 3)) * 2;
   }
 };
 
-// Byte offset of the group of 16 tokens `group` of (page, head).
+// Byte offset of the keys (kv = 0) or values (1) of the group of 16 tokens `group` of (page, head).
 template <int QT, int D>
-__device__ __forceinline__ long long kv_group_offset(const KvCache& c, long long page, int head, int group) {
-  return ((page * c.heads + head) * (c.page_size >> 4) + group) * (long long)KvL<QT, D>::kGroup;
+__device__ __forceinline__ long long kv_group_offset(const KvCache& c, long long page, int head, int kv, int group) {
+  return (((page * c.heads + head) * 2 + kv) * (c.page_size >> 4) + group) * (long long)KvL<QT, D>::kHalf;
 }
 
 // The 8 nibbles of a key word: value 2p in nibble p, value 2p + 1 in nibble p + 4. The 4 nibbles of a value half-word
