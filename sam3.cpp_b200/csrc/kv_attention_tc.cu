@@ -5,7 +5,7 @@
 // one for each CTA (one per SM): uneven lengths, causal diagonals and few long units all fill the GPU. A unit that
 // several CTAs share leaves unnormalised parts in the workspace, which join_kernel adds up in the order of the shares.
 //
-// Roles (16 warps):
+// Roles (20 warps, 24 for D = 256):
 //   warps 0, 1     one thread each issues the MMAs of query tile 0 / 1: S = Q K^T (128 x 128 x D) into TMEM, then
 //                  O += P V (128 x D x 128) with P read from TMEM
 //   softmax        one warpgroup per query tile, a thread per query row with its 128 scores in registers: running
@@ -82,7 +82,6 @@ constexpr int kTile = 128;          // query rows of a tile and tokens of a tile
 constexpr int kSlotBytes = 16384;   // 128 x 64 f16
 constexpr int kUnit = 64;           // tokens of an entry of the block-form ring
 constexpr float kLazy = 8.f;        // log2 of the largest weight before the reference maximum moves
-constexpr int kThreads = 512;
 constexpr int kPoly = 2;            // of every 8 exponentials, how many run on the FMA pipe
 
 template <int QT, int D>
@@ -90,11 +89,16 @@ struct Tc {
   typedef KvL<QT, D> L;
   static constexpr int kTQ = D == 256 ? 1 : 2;
   static constexpr int kSBuf = D == 256 ? 2 : 1;
-  static constexpr int kDeqWarp0 = D == 256 ? 8 : 12;
-  static constexpr int kDeqWarps = 16 - kDeqWarp0;
+  // dequantising warps: teams of 8; with two teams, team p makes part p of every item (K: 128 of the 256 values of a row,
+  // V: 64 of the 128 tokens), so a part is published on its own
+  static constexpr int kTeams = D == 256 ? 2 : 1;
+  static constexpr int kDeqWarp0 = 4 + 4 * kTQ;
+  static constexpr int kDeqWarps = 8 * kTeams;
+  static constexpr int kThreads = 32 * (kDeqWarp0 + kDeqWarps);
   static constexpr int kParts = D / 64;                     // slots of an item (K: 64-value chunks; V: D x 64 tokens)
+  static constexpr int kTeamSlots = kParts / kTeams;        // slots that a warp's item publishes
   static constexpr int kNSB = D / L::kSB;                   // super-blocks of a row
-  static constexpr int kTasks = 8 * kNSB / kDeqWarps;       // (16-token group, super-block) tasks of a warp per item
+  static constexpr int kTasks = kNSB / kTeams;              // super-blocks of 16 tokens that a warp makes of an item
   static constexpr int kQBytes = kTQ * kTile * D * 2;
   static constexpr int kSlots = D == 256 ? 6 : 8;
   static constexpr int kUnitBytes = kUnit / 16 * L::kHalf;
@@ -103,10 +107,13 @@ struct Tc {
   static constexpr int kSmem = 1024 + kQBytes + kSlots * kSlotBytes + kRaw * kUnitBytes + 512;
   static_assert(kRaw >= 3, "K of a tile takes two entries of tiles_kernel's ring, and one has to be on its way");
   static constexpr int kOCol = 256;                         // TMEM: S regions at 0 and 128, O after them
-  // register shares of the four warpgroups add up to the launch's 4 x 128
-  static constexpr int kRegsIssue = 80;
-  static constexpr int kRegsSoft = D == 256 ? 192 : 176;
-  static constexpr int kRegsDeq = D == 256 ? 120 : 80;
+  // Registers a thread at launch (65536 / threads, whole eights) and after the warpgroups trade: the issuing one, softmax
+  // (kTQ warpgroups), dequantising (2 kTeams). The sum over warpgroups stays within the launch's.
+  static constexpr int kRegsLaunch = 65536 / kThreads / 8 * 8;
+  static constexpr int kRegsIssue = 72;
+  static constexpr int kRegsSoft = 120;
+  static constexpr int kRegsDeq = D == 256 ? 72 : 80;
+  static_assert(kRegsIssue + kTQ * kRegsSoft + 2 * kTeams * kRegsDeq <= kThreads / 128 * kRegsLaunch, "register shares");
   static constexpr int kPart = kTQ * kTile * (D + 2);       // floats of a unit's part
 };
 
@@ -299,32 +306,30 @@ __device__ __forceinline__ void emit_v(const uint8_t* half, uint32_t keep0, uint
 
 // One token tile of one query row: the row's 128 scores from TMEM at `at`, the lazy reference maximum, the weights as f16
 // pairs over the first 64 columns, the sum into l. MASKED: only tokens [lo, hi) of the tile count. Returns true when the
-// maximum moved and the row of O has to be scaled by alpha.
+// maximum moved and the row of O has to be scaled by alpha. The scores are read twice, 32 or 64 at a time, in loops that
+// stay rolled: the softmax and the dequantising code of a sub-partition then fit its instruction cache together (with
+// all 128 scores unrolled most issue slots went to waiting for instructions).
 template <bool MASKED>
 __device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float sl2, float& m_ref, float& l, float& alpha) {
-  uint32_t r[kTile];
-  KV_TMEM_LD32(at, r);
-  KV_TMEM_LD32(at + 32, r + 32);
-  KV_TMEM_LD32(at + 64, r + 64);
-  KV_TMEM_LD32(at + 96, r + 96);
-  tc_wait_ld();
-  if (MASKED) {
+  uint32_t r[64];
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+  for (int c0 = 0; c0 < kTile; c0 += 64) {
+    KV_TMEM_LD32(at + c0, r);
+    KV_TMEM_LD32(at + c0 + 32, r + 32);
+    tc_wait_ld();
+    if (MASKED) {
 #pragma unroll
-    for (int c = 0; c < kTile; ++c) {
-      const int tok = (c & ~15) + token_at(c & 15);
-      if (tok < lo || tok >= hi) r[c] = __float_as_uint(-INFINITY);
+      for (int c = 0; c < 64; ++c) {
+        const int tok = c0 + (c & ~15) + token_at(c & 15);
+        if (tok < lo || tok >= hi) r[c] = __float_as_uint(-INFINITY);
+      }
     }
+#pragma unroll
+    for (int c = 0; c < 64; c += 8)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1]));
   }
-  float mx[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    mx[k] = max3(__uint_as_float(r[3 * k]), __uint_as_float(r[3 * k + 1]), __uint_as_float(r[3 * k + 2]));
-#pragma unroll
-  for (int c = 12; c < 124; c += 8)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1]));
-#pragma unroll
-  for (int k = 0; k < 2; ++k) mx[k] = max3(mx[k], __uint_as_float(r[124 + 2 * k]), __uint_as_float(r[125 + 2 * k]));
   const float top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * sl2;
   alpha = 1.f;
   bool moved = false;
@@ -336,17 +341,24 @@ __device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float 
   }
   const unsigned long long sl2x2 = f2_pack(sl2, sl2), negm2 = f2_pack(-m_ref, -m_ref);
   unsigned long long acc0 = f2_pack(0.f, 0.f), acc1 = acc0;
+#pragma unroll 1
+  for (int c0 = 0; c0 < kTile; c0 += 32) {
+    KV_TMEM_LD32(at + c0, r);
+    tc_wait_ld();
+    uint32_t pk[16];
 #pragma unroll
-  for (int c = 0; c < kTile / 16; ++c) {
-    uint32_t pk[8];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < 4; ++u) {
       float pv[8];
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        const int i = 16 * c + 8 * u + e;
+        const int c = 8 * u + e;
+        if (MASKED) {
+          const int tok0 = c0 + (c & ~15) + token_at(c & 15), tok1 = c0 + (c & ~15) + token_at((c + 1) & 15);
+          if (tok0 < lo || tok0 >= hi) r[c] = __float_as_uint(-INFINITY);
+          if (tok1 < lo || tok1 >= hi) r[c + 1] = __float_as_uint(-INFINITY);
+        }
         float x0, x1;
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), sl2x2, negm2), x0, x1);
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl2x2, negm2), x0, x1);
         // a hidden token's -inf gives 0 exactly, so a row that sees nothing keeps the sum 0
         pv[e] = !MASKED && e < kPoly ? exp2_fma(x0) : ex2_approx(x0);
         pv[e + 1] = !MASKED && e + 1 < kPoly ? exp2_fma(x1) : ex2_approx(x1);
@@ -356,7 +368,9 @@ __device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float 
 #pragma unroll
       for (int e = 0; e < 4; ++e) pk[4 * u + e] = h2_u32(__floats2half2_rn(pv[2 * e], pv[2 * e + 1]));
     }
-    KV_TMEM_ST8(at + 8 * c, pk);
+    // columns c0 / 2 .. c0 / 2 + 15 held scores that have been read
+    KV_TMEM_ST8(at + c0 / 2, pk);
+    KV_TMEM_ST8(at + c0 / 2 + 8, pk + 8);
   }
   float a0, a1, b0, b1;
   f2_unpack(acc0, a0, a1);
@@ -366,7 +380,7 @@ __device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float 
 }
 
 template <int QT, int D>
-__global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constant__ TcArgs a, int* err) {
+__global__ void __launch_bounds__(Tc<QT, D>::kThreads, 1) tiles_kernel(const __grid_constant__ TcArgs a, int* err) {
   typedef KvL<QT, D> L;
   typedef Tc<QT, D> C;
   constexpr int TQ = C::kTQ, ROWS = TQ * kTile, kSlots = C::kSlots;
@@ -389,8 +403,8 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   static_assert((2 + 2 * kSlots + 8 + 2 * C::kRaw) * 8 <= 512, "barriers of tiles_kernel");
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort_word, s_pair;
-  __shared__ long long s_sum[16], s_start;
-  __shared__ Walk s_walk[16];
+  __shared__ long long s_sum[24], s_start;
+  __shared__ Walk s_walk[24];
   volatile int* s_abort = &s_abort_word;
 
   const KvAttnParams& p = a.p;
@@ -403,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     mbar_init(q_full, C::kDeqWarps);
     mbar_init(q_empty, TQ);
     for (int s = 0; s < kSlots; ++s) {
-      mbar_init(&full[s], C::kDeqWarps);
+      mbar_init(&full[s], 8);  // the warps of a team
       mbar_init(&empty[s], TQ);
     }
     for (int x = 0; x < 2; ++x) {
@@ -414,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     }
     for (int x = 0; x < C::kRaw; ++x) {
       mbar_init(&raw_full[x], 1);
-      mbar_init(&raw_empty[x], C::kDeqWarps);
+      mbar_init(&raw_empty[x], C::kDeqWarps / 2);  // each warp reads one of an item's two entries
     }
     s_abort_word = 0;
     fence_mbar_init();
@@ -425,8 +439,9 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     tmem_relinquish();
   }
 
-  // ---- tiles of one head, by sixteenths of the (sequence, row block) pairs; then the pair in which the share begins
-  const int per_warp = (pairs + 15) / 16;
+  // ---- tiles of one head, by the warps' shares of the (sequence, row block) pairs; then the pair in which the share begins
+  constexpr int kWarps = C::kThreads / 32;
+  const int per_warp = (pairs + kWarps - 1) / kWarps;
   auto pair_tiles = [&](int k) -> int {
     if (k >= pairs) return 0;
     const int b = k / a.blocks;
@@ -446,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
   const uint32_t tmem = s_tmem;
   long long per_head = 0;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) per_head += s_sum[w];
+  for (int w = 0; w < kWarps; ++w) per_head += s_sum[w];
   const long long total = per_head * p.c.heads;
   const long long ctas = min((long long)gridDim.x, total);
   const bool works = (int)blockIdx.x < ctas;
@@ -456,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     const long long rem = p0 - head * per_head;
     long long before = 0;
     int w = 0;
-    while (w < 15 && before + s_sum[w] <= rem) before += s_sum[w++];
+    while (w < kWarps - 1 && before + s_sum[w] <= rem) before += s_sum[w++];
     if (warp == w) {
       for (int k0 = w * per_warp;; k0 += 32) {
         const long long n = k0 + lane < min(pairs, (w + 1) * per_warp) ? pair_tiles(k0 + lane) : 0;
@@ -810,19 +825,15 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     }
   } else {
     // ---- dequantising warps
-    if (C::kRegsDeq < 128) regs_dec<C::kRegsDeq>();
-    const int dw = warp - C::kDeqWarp0;
-    uint32_t slot = 0, q_n = 0;
-    int raw0 = 0;            // ring entry of the current item's first group
-    uint32_t raw_phase = 0;  // and its phase
+    regs_dec<C::kRegsDeq>();
+    const int dw = warp - C::kDeqWarp0, team = dw >> 3, tw = dw & 7;
+    uint32_t slot = team * C::kTeamSlots, q_n = 0;
+    int raw0 = 0;            // block-form ring entry of the item's tokens 0 .. 63; 64 .. 127 follow
+    uint32_t raw_phase = 0;  // its phase
     bool ok = true;
-    auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
-      if (ok && !mbar_wait(bar, parity, s_abort, err, code)) ok = false;
-      ok = __all_sync(~0u, ok);
-    };
     while (ok && walk_next_warp<ROWS>(p, a.blocks, err, &w, lane)) {
       // Q rows into the swizzled chunks
-      wait_all(q_empty, (q_n & 1) ^ 1, kErrWaitEmpty);
+      ok = __all_sync(~0u, mbar_wait(q_empty, (q_n & 1) ^ 1, s_abort, err, kErrWaitEmpty));
       if (!ok) break;
       ++q_n;
       for (int e = dw * 32 + lane; e < ROWS * (D / 8); e += 32 * C::kDeqWarps) {
@@ -840,53 +851,50 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
       if (lane == 0) mbar_arrive(q_full);
 
       const int n = w.cb - w.ca, tok_first = (w.u.t0 + w.ca) * kTile, lo = w.u.lo, hi = w.u.hi;
-      for (int x = 0; x < 2 * n && ok; ++x) {
+#pragma unroll 1
+      for (int x = 0; x < 2 * n; ++x) {
         int j;
         const bool is_k = order(x, n, &j);
-        const int tok0 = tok_first + j * kTile;
-        const bool whole = tok0 >= lo && tok0 + kTile <= hi;
-        // tasks (16-token group, super-block) of this warp, in parts that are published on their own: a super-block of
-        // keys, 64 tokens of values (D = 64: the one slot)
-        constexpr int kPerK = 8 / C::kDeqWarps, kPerV = D > 64 ? C::kTasks / 2 : C::kTasks;
-        constexpr int kSlotsK = L::kSB / 64, kSlotsV = D > 64 ? D / 128 : 1;
-        const int per = is_k ? kPerK : kPerV, slots = is_k ? kSlotsK : kSlotsV;
-        // the ring entries of tokens 0 .. 63 and 64 .. 127
-        const int e1 = raw0 + 1 == C::kRaw ? 0 : raw0 + 1;
-        const uint32_t ph1 = e1 ? raw_phase : raw_phase ^ 1;
-#pragma unroll 1
-        for (int k0 = 0; k0 < C::kTasks; k0 += per) {
-          for (int y = 0; y < slots; ++y)
-            wait_all(&empty[(slot + y) % kSlots], (((slot + y) / kSlots) & 1) ^ 1, kErrWaitEmpty);
-          if (k0 == 0) wait_all(&raw_full[raw0], raw_phase, kErrWaitFull);
-          if (k0 == 0 ? is_k || D == 64 : !is_k) wait_all(&raw_full[e1], ph1, kErrWaitFull);
-          if (!ok) break;
-          uint8_t* dst = s_ring + slot % kSlots * kSlotBytes;
-#pragma unroll 1
-          for (int k = k0; k < k0 + per; ++k) {
-            const int id = k * C::kDeqWarps + dw;
-            const int grp = is_k ? id & 7 : id / C::kNSB;
-            const int sb = C::kNSB == 1 ? 0 : is_k ? id >> 3 : id % C::kNSB;
-            const uint8_t* half = s_raw + (grp < 4 ? raw0 : e1) * C::kUnitBytes + (grp & 3) * L::kHalf;
-            if (is_k) {
-              emit_k<QT, D>(half, dst, grp, sb, lane);
-            } else {
-              uint32_t keep0 = ~0u, keep1 = ~0u;
-              if (!whole) {
-                const int first = tok0 + grp * 16 + 2 * (lane & 3);
-                auto in = [&](int tok) -> bool { return tok >= lo && tok < hi; };
-                keep0 = (in(first) ? 0xFFFFu : 0u) | (in(first + 1) ? 0xFFFF0000u : 0u);
-                keep1 = (in(first + 8) ? 0xFFFFu : 0u) | (in(first + 9) ? 0xFFFF0000u : 0u);
-              }
-              emit_v<QT, D>(half, keep0, keep1, D == 64 ? dst + (grp >> 2) * (D * 128) : dst, grp, sb, lane);
-            }
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane < slots) mbar_arrive(&full[(slot + lane) % kSlots]);
-          slot += slots;
+        // this warp's 16 tokens of the tile and its super-blocks of them
+        const int grp = C::kTeams == 1 || is_k ? tw : 4 * team + (tw & 3);
+        const int sb0 = C::kTeams == 1 ? 0 : (is_k ? team : tw >> 2) * C::kTasks;
+        int e = raw0 + (grp >> 2);
+        uint32_t ph = raw_phase;
+        if (e >= C::kRaw) {
+          e -= C::kRaw;
+          ph ^= 1;
         }
+        const uint32_t slot_i = slot % kSlots, slot_ph = ((slot / kSlots) & 1) ^ 1;
+        bool got = mbar_wait(&raw_full[e], ph, s_abort, err, kErrWaitFull);
+#pragma unroll
+        for (int y = 0; y < C::kTeamSlots; ++y)  // side by side: the slots of an item never wrap
+          got = got && mbar_wait(&empty[slot_i + y], slot_ph, s_abort, err, kErrWaitEmpty);
+        ok = __all_sync(~0u, got);
         if (!ok) break;
-        if (lane < 2) mbar_arrive(&raw_empty[lane ? e1 : raw0]);
+        uint8_t* dst = s_ring + slot_i * kSlotBytes;
+        const uint8_t* from = s_raw + e * C::kUnitBytes + (grp & 3) * L::kHalf;
+        if (is_k) {
+#pragma unroll 1
+          for (int k = 0; k < C::kTasks; ++k)
+            emit_k<QT, D>(from, dst + k * (L::kSB / 64) * kSlotBytes, grp, sb0 + k, lane);
+        } else {
+          const int tok0 = tok_first + j * kTile;
+          uint32_t keep0 = ~0u, keep1 = ~0u;
+          if (tok0 < lo || tok0 + kTile > hi) {
+            const int first = tok0 + grp * 16 + 2 * (lane & 3);
+            auto in = [&](int tok) -> bool { return tok >= lo && tok < hi; };
+            keep0 = (in(first) ? 0xFFFFu : 0u) | (in(first + 1) ? 0xFFFF0000u : 0u);
+            keep1 = (in(first + 8) ? 0xFFFFu : 0u) | (in(first + 9) ? 0xFFFF0000u : 0u);
+          }
+          if (C::kTeams == 1) dst += (grp >> 2) * (D * 128);
+#pragma unroll 1
+          for (int k = 0; k < C::kTasks; ++k) emit_v<QT, D>(from, keep0, keep1, dst, grp, sb0 + k, lane);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane < C::kTeamSlots) mbar_arrive(&full[slot_i + lane]);
+        if (lane == C::kTeamSlots) mbar_arrive(&raw_empty[e]);
+        slot += C::kParts;
         raw0 += 2;
         if (raw0 >= C::kRaw) {
           raw0 -= C::kRaw;
@@ -988,7 +996,7 @@ int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStrea
   a.shared = reinterpret_cast<Shared*>(w.part + (size_t)2 * w.sms * C::kPart);
   a.blocks = (p.nq * (p.heads / p.c.heads) + C::kTQ * kTile - 1) / (C::kTQ * kTile);
   if (w.sms > 160) return -2;  // join_kernel's table of factors
-  k<<<w.sms, kThreads, C::kSmem, st>>>(a, err);
+  k<<<w.sms, C::kThreads, C::kSmem, st>>>(a, err);
   if (cudaGetLastError() != cudaSuccess) return -12;
   // launched while tiles_kernel still runs; it waits for its end before it reads
   cudaLaunchConfig_t cfg = {};
