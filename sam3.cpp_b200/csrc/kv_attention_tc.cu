@@ -82,7 +82,6 @@ constexpr int kTile = 128;          // query rows of a tile and tokens of a tile
 constexpr int kSlotBytes = 16384;   // 128 x 64 f16
 constexpr int kUnit = 64;           // tokens of an entry of the block-form ring
 constexpr float kLazy = 8.f;        // log2 of the largest weight before the reference maximum moves
-constexpr int kPoly = 2;            // of every 8 exponentials, how many run on the FMA pipe
 
 template <int QT, int D>
 struct Tc {
@@ -115,6 +114,8 @@ struct Tc {
   static constexpr int kRegsDeq = D == 256 ? 72 : 80;
   static_assert(kRegsIssue + kTQ * kRegsSoft + 2 * kTeams * kRegsDeq <= kThreads / 128 * kRegsLaunch, "register shares");
   static constexpr int kPart = kTQ * kTile * (D + 2);       // floats of a unit's part
+  // of every 8 exponentials, how many run on the FMA pipe: 2 where two softmax warpgroups share the MUFU units
+  static constexpr int kPoly = kTQ == 2 ? 2 : 0;
 };
 
 // A unit that several CTAs share, written by the CTA in whose share it begins (its entry's index).
@@ -304,31 +305,68 @@ __device__ __forceinline__ void emit_v(const uint8_t* half, uint32_t keep0, uint
   }
 }
 
+template <bool MASKED>
+__device__ __forceinline__ void mask_scores(uint32_t (&r)[32], int c0, int lo, int hi) {
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    const int tok = c0 + (c & 16) + token_at(c & 15);
+    if (MASKED && (tok < lo || tok >= hi)) r[c] = __float_as_uint(-INFINITY);
+  }
+}
+__device__ __forceinline__ void max_scores(const uint32_t (&r)[32], float (&mx)[4]) {
+#pragma unroll
+  for (int c = 0; c < 32; c += 8)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1]));
+}
+// weights of 32 scores to the 16 columns at `at`; acc: the sums of even and odd pairs
+template <bool MASKED, int POLY>
+__device__ __forceinline__ void weigh_scores(const uint32_t (&r)[32], uint32_t at, unsigned long long sl2x2,
+                                             unsigned long long negm2, unsigned long long& acc0, unsigned long long& acc1) {
+  uint32_t pk[16];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    float pv[8];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const int c = 8 * u + e;
+      float x0, x1;
+      f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl2x2, negm2), x0, x1);
+      // a hidden token's -inf gives 0 exactly, so a row that sees nothing keeps the sum 0
+      pv[e] = !MASKED && e < POLY ? exp2_fma(x0) : ex2_approx(x0);
+      pv[e + 1] = !MASKED && e + 1 < POLY ? exp2_fma(x1) : ex2_approx(x1);
+    }
+    acc0 = f2_add(acc0, f2_add(f2_pack(pv[0], pv[1]), f2_pack(pv[4], pv[5])));
+    acc1 = f2_add(acc1, f2_add(f2_pack(pv[2], pv[3]), f2_pack(pv[6], pv[7])));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pk[4 * u + e] = h2_u32(__floats2half2_rn(pv[2 * e], pv[2 * e + 1]));
+  }
+  KV_TMEM_ST8(at, pk);
+  KV_TMEM_ST8(at + 8, pk + 8);
+}
+
 // One token tile of one query row: the row's 128 scores from TMEM at `at`, the lazy reference maximum, the weights as f16
 // pairs over the first 64 columns, the sum into l. MASKED: only tokens [lo, hi) of the tile count. Returns true when the
-// maximum moved and the row of O has to be scaled by alpha. The scores are read twice, 32 or 64 at a time, in loops that
-// stay rolled: the softmax and the dequantising code of a sub-partition then fit its instruction cache together (with
+// maximum moved and the row of O has to be scaled by alpha. The scores are read twice, 32 at a time, in loops that stay
+// rolled: the softmax and the dequantising code of a sub-partition then fit its instruction cache together (with
 // all 128 scores unrolled most issue slots went to waiting for instructions).
-template <bool MASKED>
+template <bool MASKED, int POLY>
 __device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float sl2, float& m_ref, float& l, float& alpha) {
-  uint32_t r[64];
+  // 32 scores are in flight while the 32 before them are worked on
+  uint32_t ra[32], rb[32];
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  KV_TMEM_LD32(at, ra);
+  tc_wait_ld();
 #pragma unroll 1
   for (int c0 = 0; c0 < kTile; c0 += 64) {
-    KV_TMEM_LD32(at + c0, r);
-    KV_TMEM_LD32(at + c0 + 32, r + 32);
+    KV_TMEM_LD32(at + c0 + 32, rb);
+    mask_scores<MASKED>(ra, c0, lo, hi);
+    max_scores(ra, mx);
     tc_wait_ld();
-    if (MASKED) {
-#pragma unroll
-      for (int c = 0; c < 64; ++c) {
-        const int tok = c0 + (c & ~15) + token_at(c & 15);
-        if (tok < lo || tok >= hi) r[c] = __float_as_uint(-INFINITY);
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < 64; c += 8)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1]));
+    KV_TMEM_LD32(at + ((c0 + 64) & 127), ra);  // at the end the first ones again
+    mask_scores<MASKED>(rb, c0 + 32, lo, hi);
+    max_scores(rb, mx);
+    tc_wait_ld();
   }
   const float top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * sl2;
   alpha = 1.f;
@@ -342,35 +380,16 @@ __device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float 
   const unsigned long long sl2x2 = f2_pack(sl2, sl2), negm2 = f2_pack(-m_ref, -m_ref);
   unsigned long long acc0 = f2_pack(0.f, 0.f), acc1 = acc0;
 #pragma unroll 1
-  for (int c0 = 0; c0 < kTile; c0 += 32) {
-    KV_TMEM_LD32(at + c0, r);
+  for (int c0 = 0; c0 < kTile; c0 += 64) {
+    // the weights of 32 scores go over columns whose scores have been read
+    KV_TMEM_LD32(at + c0 + 32, rb);
+    mask_scores<MASKED>(ra, c0, lo, hi);
+    weigh_scores<MASKED, POLY>(ra, at + c0 / 2, sl2x2, negm2, acc0, acc1);
     tc_wait_ld();
-    uint32_t pk[16];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      float pv[8];
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const int c = 8 * u + e;
-        if (MASKED) {
-          const int tok0 = c0 + (c & ~15) + token_at(c & 15), tok1 = c0 + (c & ~15) + token_at((c + 1) & 15);
-          if (tok0 < lo || tok0 >= hi) r[c] = __float_as_uint(-INFINITY);
-          if (tok1 < lo || tok1 >= hi) r[c + 1] = __float_as_uint(-INFINITY);
-        }
-        float x0, x1;
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl2x2, negm2), x0, x1);
-        // a hidden token's -inf gives 0 exactly, so a row that sees nothing keeps the sum 0
-        pv[e] = !MASKED && e < kPoly ? exp2_fma(x0) : ex2_approx(x0);
-        pv[e + 1] = !MASKED && e + 1 < kPoly ? exp2_fma(x1) : ex2_approx(x1);
-      }
-      acc0 = f2_add(acc0, f2_add(f2_pack(pv[0], pv[1]), f2_pack(pv[4], pv[5])));
-      acc1 = f2_add(acc1, f2_add(f2_pack(pv[2], pv[3]), f2_pack(pv[6], pv[7])));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pk[4 * u + e] = h2_u32(__floats2half2_rn(pv[2 * e], pv[2 * e + 1]));
-    }
-    // columns c0 / 2 .. c0 / 2 + 15 held scores that have been read
-    KV_TMEM_ST8(at + c0 / 2, pk);
-    KV_TMEM_ST8(at + c0 / 2 + 8, pk + 8);
+    KV_TMEM_LD32(at + ((c0 + 64) & 127), ra);  // unused at the end
+    mask_scores<MASKED>(rb, c0 + 32, lo, hi);
+    weigh_scores<MASKED, POLY>(rb, at + c0 / 2 + 16, sl2x2, negm2, acc0, acc1);
+    tc_wait_ld();
   }
   float a0, a1, b0, b1;
   f2_unpack(acc0, a0, a1);
@@ -728,8 +747,8 @@ __global__ void __launch_bounds__(Tc<QT, D>::kThreads, 1) tiles_kernel(const __g
         const uint32_t s_at = tmem + lane_off + 128 * reg;
         float alpha;
         const bool moved = tok0 >= all_lo && tok0 + kTile <= all_hi
-                               ? softmax_tile<false>(s_at, 0, 0, sl2, m_ref, l, alpha)
-                               : softmax_tile<true>(s_at, lo - tok0, hi - tok0, sl2, m_ref, l, alpha);
+                               ? softmax_tile<false, C::kPoly>(s_at, 0, 0, sl2, m_ref, l, alpha)
+                               : softmax_tile<true, 0>(s_at, lo - tok0, hi - tok0, sl2, m_ref, l, alpha);
         if (tok0 > tok_first) {
           // O is current once the previous P V product of this tile has completed
           if (!mbar_wait(&pv_done[t], (n - 1) & 1, s_abort, err, kErrWaitMisc)) ok = false;
