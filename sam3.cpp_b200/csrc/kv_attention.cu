@@ -22,6 +22,13 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// the same onto zeros
+__device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 // transpose of the 8 x 8 matrix of 16-bit values that a warp holds as one m8n8 fragment
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   uint32_t d;
@@ -30,16 +37,18 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
 }
 template <int BYTES>
 __device__ __forceinline__ void lds(const uint8_t* at, uint32_t (&r)[BYTES / 4]) {
-  if (BYTES == 16) {
+  if (BYTES == 4) {
+    r[0] = *reinterpret_cast<const uint32_t*>(at);
+  } else if (BYTES == 16) {
     const uint4 v = *reinterpret_cast<const uint4*>(at);
     r[0] = v.x;
-    r[1] = v.y;
-    r[BYTES / 4 - 2] = v.z;
+    r[BYTES >= 8 ? 1 : 0] = v.y;
+    r[BYTES >= 8 ? BYTES / 4 - 2 : 0] = v.z;
     r[BYTES / 4 - 1] = v.w;
   } else {
     const uint2 v = *reinterpret_cast<const uint2*>(at);
     r[0] = v.x;
-    r[1] = v.y;
+    r[BYTES >= 8 ? 1 : 0] = v.y;
   }
 }
 
@@ -287,6 +296,9 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
         const bool whole = tok0 >= max_lo && tok0 + 16 <= min_hi;
 
         // -- scores
+        uint32_t sc0[NB / 2], sc1[NB / 2];  // scales of tokens g and g + 8
+        lds<NB * 2>(gp + L::k_scale(g, 0), sc0);
+        lds<NB * 2>(gp + L::k_scale(g + 8, 0), sc1);
         float s[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -321,8 +333,8 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
               nibble_pairs<QT>(k1[nn], x1);
             }
             const uint32_t a0[4] = {x0[0], x1[0], x0[1], x1[1]}, a1[4] = {x0[2], x1[2], x0[3], x1[3]};
-            const float f0 = __half2float(*reinterpret_cast<const __half*>(gp + L::k_scale(g, n)));
-            const float f1 = __half2float(*reinterpret_cast<const __half*>(gp + L::k_scale(g + 8, n)));
+            const __half2 h0 = u32_h2(sc0[n / 2]), h1 = u32_h2(sc1[n / 2]);
+            const float f0 = n & 1 ? __high2float(h0) : __low2float(h0), f1 = n & 1 ? __high2float(h1) : __low2float(h1);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               uint4 qv;
@@ -331,8 +343,8 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
               else
                 qv = make_uint4(qf[C::kQSmem ? 0 : nt * NB + n][0], qf[C::kQSmem ? 0 : nt * NB + n][1], qf[C::kQSmem ? 0 : nt * NB + n][2],
                                 qf[C::kQSmem ? 0 : nt * NB + n][3]);
-              float c[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816(c, a0, qv.x, qv.y);
+              float c[4];
+              mma16816_first(c, a0, qv.x, qv.y);
               mma16816(c, a1, qv.z, qv.w);
               s[nt][0] = fmaf(f0, c[0], s[nt][0]);
               s[nt][1] = fmaf(f0, c[1], s[nt][1]);
@@ -394,19 +406,22 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
           w1[nt] = movmatrix(h2_u32(__floats2half2_rn(e4[2], e4[3])));
         }
 
-        // -- outputs; tokens outside the sequence's span may hold anything, so their scales count as zero
-        uint32_t keep0 = ~0u, keep1 = ~0u;
+        // -- outputs; tokens outside the sequence's span may hold anything, so their scales become zero
         if (!whole) {
-          auto in = [&](int tok) -> bool { return tok0 + tok >= min_lo && tok0 + tok < max_hi; };
-          keep0 = (in(2 * t) ? 0xFFFFu : 0u) | (in(2 * t + 1) ? 0xFFFF0000u : 0u);
-          keep1 = (in(2 * t + 8) ? 0xFFFFu : 0u) | (in(2 * t + 9) ? 0xFFFF0000u : 0u);
+          __half* scales = reinterpret_cast<__half*>(ring + stage * (2 * L::kHalf) + L::kHalf + L::kVal);
+          for (int e = lane; e < 16 * NB * L::kPlanes; e += 32) {
+            const int lane_t = e % (16 * NB) / (4 * NB), tok = tok0 + 2 * lane_t + (e & 1) + 4 * (e & 2);
+            if (tok < min_lo || tok >= max_hi) scales[e] = __ushort_as_half(0);
+          }
+          fence_proxy_async_smem();  // the next copy into this stage comes after these writes
+          __syncwarp();
         }
         if (QT == QT_Q4_1) {  // sum over tokens of weight * minimum, a row for each block
           uint32_t am[4] = {0, 0, 0, 0};
           if (g < NB) {
             const uint2 v = *reinterpret_cast<const uint2*>(vp + L::kSc + L::v_scale(2 * t, g));
-            am[0] = v.x & keep0;
-            am[2] = v.y & keep1;
+            am[0] = v.x;
+            am[2] = v.y;
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma16816(omin[nt], am, w0[nt], w1[nt]);
@@ -435,8 +450,8 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
             const uint2 sc = *reinterpret_cast<const uint2*>(vp + L::v_scale(2 * t, n));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const uint32_t b0 = h2_u32(__hmul2(u32_h2(w0[nt]), u32_h2(sc.x & keep0)));
-              const uint32_t b1 = h2_u32(__hmul2(u32_h2(w1[nt]), u32_h2(sc.y & keep1)));
+              const uint32_t b0 = h2_u32(__hmul2(u32_h2(w0[nt]), u32_h2(sc.x)));
+              const uint32_t b1 = h2_u32(__hmul2(u32_h2(w1[nt]), u32_h2(sc.y)));
               mma16816(o[nt][2 * n], a0, b0, b1);
               mma16816(o[nt][2 * n + 1], a1, b0, b1);
             }
@@ -541,24 +556,58 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
         __syncthreads();
         if (s_last) {
           __threadfence();
-          auto part_of = [&](long long c) { return a.part + (2 * c + (unit_start > total * c / ctas ? 1 : 0)) * kPart; };
+          // the unit begins inside the first CTA's share or with it, and inside no other's
+          const int n = (int)(c1 - c0) + 1, second = unit_start > total * c0 / ctas;
+          auto part_of = [&](int k) { return a.part + (2 * (c0 + k) + (k == 0 ? second : 0)) * kPart; };
+          // maxima of the rows over the parts: a warp a row
+          for (int r = warp; r < n_rows; r += W) {
+            float top = kNoScore;
+            for (int k = lane; k < n; k += 32) top = fmaxf(top, __ldcg(part_of(k) + C::kRows * D + r));
+#pragma unroll
+            for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+            if (lane == 0) s_m[r] = top;
+          }
+          __syncthreads();
+          // the threads share the parts between them where there are fewer outputs than threads
+          constexpr int kItems = C::kRows * (D / 4), kShare = 32 * W > kItems ? 32 * W / kItems : 1;
+          float4* s_v = reinterpret_cast<float4*>(smem);  // [kShare][kItems], and behind it the sums
+          float* s_sum = reinterpret_cast<float*>(s_v + kShare * kItems);
+          for (int e0 = threadIdx.x; e0 < kShare * kItems; e0 += 32 * W) {
+            const int e = e0 % kItems, r = e / (D / 4), d4 = e % (D / 4) * 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            float sum = 0.f;
+            if (r < n_rows) {
+              const float top = s_m[r];
+#pragma unroll 8
+              for (int k = e0 / kItems; k < n; k += kShare) {
+                const float* from = part_of(k);
+                const float f = ex2_approx(__ldcg(from + C::kRows * D + r) - top);
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(from + r * D + d4));
+                sum = fmaf(__ldcg(from + C::kRows * (D + 1) + r), f, sum);
+                v.x = fmaf(x.x, f, v.x);
+                v.y = fmaf(x.y, f, v.y);
+                v.z = fmaf(x.z, f, v.z);
+                v.w = fmaf(x.w, f, v.w);
+              }
+            }
+            s_v[e0] = v;
+            if (d4 == 0) s_sum[e0 / kItems * C::kRows + r] = sum;
+          }
+          __syncthreads();
           for (int e = threadIdx.x; e < n_rows * (D / 4); e += 32 * W) {
             const int r = e / (D / 4), d4 = e % (D / 4) * 4;
-            float top = kNoScore, sum = 0.f;
-            for (long long c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(part_of(c) + C::kRows * D + r));
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (long long c = c0; c <= c1; ++c) {
-              const float* from = part_of(c);
-              const float f = ex2_approx(__ldcg(from + C::kRows * D + r) - top);
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(from + r * D + d4));
-              sum = fmaf(__ldcg(from + C::kRows * (D + 1) + r), f, sum);
-              v.x = fmaf(x.x, f, v.x);
-              v.y = fmaf(x.y, f, v.y);
-              v.z = fmaf(x.z, f, v.z);
-              v.w = fmaf(x.w, f, v.w);
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < kShare; ++k) {
+              const float4 x = s_v[k * kItems + e];
+              v.x += x.x;
+              v.y += x.y;
+              v.z += x.z;
+              v.w += x.w;
+              sum += s_sum[k * C::kRows + r];
             }
-            finish(r, d4, v, top, sum);
+            finish(r, d4, v, s_m[r], sum);
           }
           if (threadIdx.x == 0) a.count[unit] = 0;
         }
@@ -607,7 +656,7 @@ template <int QT, int D>
 int attend(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
   const int rows = p.nq * (p.heads / p.c.heads);
   constexpr int kMost = Rows<QT, D, 1, 4>::kWarps;
-  if ((long long)p.batch * p.c.heads >= 2 * w.sms) return launch_rows_nt<QT, D, 4>(p, w, rows, err, st);
+  if ((long long)p.batch * p.c.heads >= w.sms) return launch_rows_nt<QT, D, 4>(p, w, rows, err, st);
   return launch_rows_nt<QT, D, kMost>(p, w, rows, err, st);
 }
 
