@@ -83,7 +83,8 @@ constexpr int kSlotBytes = 16384;   // 128 x 64 f16
 constexpr int kUnit = 64;           // tokens of an entry of the block-form ring
 constexpr float kLazy = 8.f;        // log2 of the largest weight before the reference maximum moves
 
-template <int QT, int D>
+// STAGED: the operands come as f16 slot images (stage_kernel) instead of being dequantised by warps of the kernel.
+template <int QT, int D, bool STAGED>
 struct Tc {
   typedef KvL<QT, D> L;
   static constexpr int kTQ = D == 256 ? 1 : 2;
@@ -92,19 +93,19 @@ struct Tc {
   // V: 64 of the 128 tokens), so a part is published on its own
   static constexpr int kTeams = D == 256 ? 2 : 1;
   static constexpr int kDeqWarp0 = 4 + 4 * kTQ;
-  static constexpr int kDeqWarps = 8 * kTeams;
+  static constexpr int kDeqWarps = STAGED ? 0 : 8 * kTeams;
   static constexpr int kThreads = 32 * (kDeqWarp0 + kDeqWarps);
   static constexpr int kParts = D / 64;                     // slots of an item (K: 64-value chunks; V: D x 64 tokens)
   static constexpr int kTeamSlots = kParts / kTeams;        // slots that a warp's item publishes
   static constexpr int kNSB = D / L::kSB;                   // super-blocks of a row
   static constexpr int kTasks = kNSB / kTeams;              // super-blocks of 16 tokens that a warp makes of an item
   static constexpr int kQBytes = kTQ * kTile * D * 2;
-  static constexpr int kSlots = D == 256 ? 6 : 8;
+  static constexpr int kSlots = STAGED ? (D == 64 ? 11 : D == 128 ? 9 : 8) : D == 256 ? 6 : 8;
   static constexpr int kUnitBytes = kUnit / 16 * L::kHalf;
   static constexpr int kRawFit = (224 * 1024 - 1024 - kQBytes - kSlots * kSlotBytes - 512) / kUnitBytes;
-  static constexpr int kRaw = kRawFit > 8 ? 8 : kRawFit;  // entries of the block-form ring
+  static constexpr int kRaw = STAGED ? 0 : kRawFit > 8 ? 8 : kRawFit;  // entries of the block-form ring
   static constexpr int kSmem = 1024 + kQBytes + kSlots * kSlotBytes + kRaw * kUnitBytes + 512;
-  static_assert(kRaw >= 3, "K of a tile takes two entries of tiles_kernel's ring, and one has to be on its way");
+  static_assert(STAGED || kRaw >= 3, "K of a tile takes two entries of tiles_kernel's ring, and one has to be on its way");
   static constexpr int kOCol = 256;                         // TMEM: S regions at 0 and 128, O after them
   // Registers a thread at launch (65536 / threads, whole eights) and after the warpgroups trade: the issuing one, softmax
   // (kTQ warpgroups), dequantising (2 kTeams). The sum over warpgroups stays within the launch's.
@@ -112,7 +113,7 @@ struct Tc {
   static constexpr int kRegsIssue = 72;
   static constexpr int kRegsSoft = 120;
   static constexpr int kRegsDeq = D == 256 ? 72 : 80;
-  static_assert(kRegsIssue + kTQ * kRegsSoft + 2 * kTeams * kRegsDeq <= kThreads / 128 * kRegsLaunch, "register shares");
+  static_assert(STAGED || kRegsIssue + kTQ * kRegsSoft + 2 * kTeams * kRegsDeq <= kThreads / 128 * kRegsLaunch, "register shares");
   static constexpr int kPart = kTQ * kTile * (D + 2);       // floats of a unit's part
   // of every 8 exponentials, how many run on the FMA pipe: 2 where two softmax warpgroups share the MUFU units
   static constexpr int kPoly = kTQ == 2 ? 2 : 0;
@@ -129,6 +130,10 @@ struct TcArgs {
   float* part;     // [2 * grid][TQ][128 * D outputs, as [D / 4][128] float4; 128 maxima; 128 sums]
   Shared* shared;  // [grid]
   int blocks;      // row blocks of a sequence
+  // staged operands: [sequence][head][tiles] of a K and a V item (D * 256 bytes each), and [sequence][head][blocks] of Q
+  uint8_t* image;
+  uint8_t* q_image;
+  int tiles;       // token tiles that a page table can name
 };
 
 // Rows of a unit: packed row r = query * group + head of the group.
@@ -398,10 +403,10 @@ __device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float 
   return moved;
 }
 
-template <int QT, int D>
-__global__ void __launch_bounds__(Tc<QT, D>::kThreads, 1) tiles_kernel(const __grid_constant__ TcArgs a, int* err) {
+template <int QT, int D, bool STAGED>
+__global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(const __grid_constant__ TcArgs a, int* err) {
   typedef KvL<QT, D> L;
-  typedef Tc<QT, D> C;
+  typedef Tc<QT, D, STAGED> C;
   constexpr int TQ = C::kTQ, ROWS = TQ * kTile, kSlots = C::kSlots;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -433,10 +438,10 @@ __global__ void __launch_bounds__(Tc<QT, D>::kThreads, 1) tiles_kernel(const __g
   const int pairs = p.batch * a.blocks;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, C::kDeqWarps);
+    mbar_init(q_full, STAGED ? 1 : C::kDeqWarps);
     mbar_init(q_empty, TQ);
     for (int s = 0; s < kSlots; ++s) {
-      mbar_init(&full[s], 8);  // the warps of a team
+      mbar_init(&full[s], STAGED ? 1 : 8);  // the copy, or the warps of a team
       mbar_init(&empty[s], TQ);
     }
     for (int x = 0; x < 2; ++x) {
@@ -538,7 +543,7 @@ __global__ void __launch_bounds__(Tc<QT, D>::kThreads, 1) tiles_kernel(const __g
   };
 
   if (warp < 4) {
-    regs_dec<C::kRegsIssue>();
+    if (!STAGED) regs_dec<C::kRegsIssue>();
     if (warp == 3) {
       // row blocks that see no token
       for (int k = blockIdx.x; k < pairs; k += gridDim.x) {
@@ -551,9 +556,50 @@ __global__ void __launch_bounds__(Tc<QT, D>::kThreads, 1) tiles_kernel(const __g
             if (p.lse && e % (D / 4) == 0) p.lse[((long long)b * p.nq + i) * p.heads + hq] = -INFINITY;
           }
       }
+    } else if (warp == 2 && STAGED) {
+      // ---- copies of the staged operands, slot by slot
+      if (lane == 0) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // stage_kernel has written them
+        uint32_t slot = 0, q_n = 0;
+        bool ok = true;
+        while (ok && walk_next<ROWS>(p, a.blocks, err, &w)) {
+          const long long unit = (long long)w.u.b * p.c.heads + w.u.head;
+          const int q_tiles = w.u.row0 + kTile < n_rows ? TQ : 1;
+          if (!mbar_wait(q_empty, (q_n & 1) ^ 1, s_abort, err, kErrWaitEmpty)) break;
+          mbar_arrive_expect_tx(q_full, q_tiles * kTile * D * 2);
+          bulk_load(s_q, a.q_image + (unit * a.blocks + w.u.row0 / ROWS) * (ROWS * D * 2), q_tiles * kTile * D * 2, q_full);
+          ++q_n;
+          const uint8_t* tiles = a.image + (unit * a.tiles + w.u.t0 + w.ca) * (D * 512);
+          const int n = w.cb - w.ca;
+          for (int x = 0; x < 2 * n && ok; ++x) {
+            int j;
+            const bool is_k = order(x, n, &j);
+            const uint8_t* from = tiles + (long long)j * (D * 512) + (is_k ? 0 : D * 256);
+            for (int c = 0; c < C::kParts; ++c, ++slot) {
+              const uint32_t s = slot % kSlots;
+              if (!mbar_wait(&empty[s], ((slot / kSlots) & 1) ^ 1, s_abort, err, kErrWaitEmpty)) { ok = false; break; }
+              mbar_arrive_expect_tx(&full[s], kSlotBytes);
+              bulk_load(s_ring + s * kSlotBytes, from + c * kSlotBytes, kSlotBytes, &full[s]);
+            }
+          }
+        }
+        // no copy may still be landing when the CTA exits
+        auto drain = [&](uint64_t* bar, uint32_t parity) {
+          const unsigned long long t0 = globaltimer_ns();
+          while (!mbar_try_wait(bar, parity)) {
+            if (globaltimer_ns() - t0 > kWaitNs) {
+              atomicCAS(err, 0, kErrWaitDrain);
+              break;
+            }
+          }
+        };
+        if (q_n) drain(q_full, (q_n - 1) & 1);
+        for (uint32_t x = slot > kSlots ? slot - kSlots : 0; x < slot; ++x) drain(&full[x % kSlots], (x / kSlots) & 1);
+      }
     } else if (warp == 2) {
       // ---- copies of the cache in block form: two ring entries per item, as few copies as the pages allow
       const int per_page = p.c.page_size >> 4;
+      constexpr int kRaw = C::kRaw > 0 ? C::kRaw : 1;
       int entry = 0;
       uint32_t phase = 0, armed = 0, armed_phase = 0;
       bool ok = true;
@@ -607,7 +653,7 @@ __global__ void __launch_bounds__(Tc<QT, D>::kThreads, 1) tiles_kernel(const __g
                         __ffs(stop) * L::kHalf, &raw_full[entry]);
             }
             __syncwarp();
-            if (++entry == C::kRaw) {
+            if (++entry == kRaw) {
               entry = 0;
               phase ^= 1;
             }
@@ -722,7 +768,7 @@ __global__ void __launch_bounds__(Tc<QT, D>::kThreads, 1) tiles_kernel(const __g
     }
   } else if (warp < 4 + 4 * TQ) {
     // ---- softmax and output of query tile t, one row per thread
-    regs_inc<C::kRegsSoft>();
+    if (!STAGED) regs_inc<C::kRegsSoft>();
     const int t = (warp - 4) >> 2, w4 = warp & 3, row = w4 * 32 + lane;
     const uint32_t lane_off = (uint32_t)(w4 * 32) << 16;
     const uint32_t o_at = tmem + lane_off + C::kOCol + t * D;
@@ -842,7 +888,7 @@ __global__ void __launch_bounds__(Tc<QT, D>::kThreads, 1) tiles_kernel(const __g
         e->second = w.start > p0;
       }
     }
-  } else {
+  } else if (!STAGED) {
     // ---- dequantising warps
     regs_dec<C::kRegsDeq>();
     const int dw = warp - C::kDeqWarp0, team = dw >> 3, tw = dw & 7;
@@ -855,7 +901,7 @@ __global__ void __launch_bounds__(Tc<QT, D>::kThreads, 1) tiles_kernel(const __g
       ok = __all_sync(~0u, mbar_wait(q_empty, (q_n & 1) ^ 1, s_abort, err, kErrWaitEmpty));
       if (!ok) break;
       ++q_n;
-      for (int e = dw * 32 + lane; e < ROWS * (D / 8); e += 32 * C::kDeqWarps) {
+      for (int e = dw * 32 + lane; e < ROWS * (D / 8); e += 32 * (C::kDeqWarps + STAGED)) {
         const int rr = e / (D / 8), c16 = e % (D / 8), r = w.u.row0 + rr;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (r < n_rows) {
@@ -1004,30 +1050,133 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArg
     store_out(p, at + 32 * e, make_float4(v[e].x * inv, v[e].y * inv, v[e].z * inv, v[e].w * inv));
 }
 
+// The f16 operands of tiles_kernel, once for all its CTAs: block (x < kv_blocks) the K and V items of one token tile of one
+// sequence and head, a warp for each 16 tokens; the blocks after them the Q rows of one tile. Bound by HBM and L2: the
+// cache read once, 4 bytes written per value pair of K and V.
 template <int QT, int D>
-int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
-  typedef Tc<QT, D> C;
-  auto* k = tiles_kernel<QT, D>;
-  if (kernel_setup(k, C::kSmem) <= 0) return -13;
-  TcArgs a;
-  a.p = p;
-  a.part = w.part;
-  a.shared = reinterpret_cast<Shared*>(w.part + (size_t)2 * w.sms * C::kPart);
-  a.blocks = (p.nq * (p.heads / p.c.heads) + C::kTQ * kTile - 1) / (C::kTQ * kTile);
-  if (w.sms > 160) return -2;  // join_kernel's table of factors
-  k<<<w.sms, C::kThreads, C::kSmem, st>>>(a, err);
-  if (cudaGetLastError() != cudaSuccess) return -12;
-  // launched while tiles_kernel still runs; it waits for its end before it reads
+__global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ TcArgs a, int kv_blocks, int* err) {
+  typedef KvL<QT, D> L;
+  constexpr int TQ = D == 256 ? 1 : 2;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const KvAttnParams& p = a.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = p.heads / p.c.heads;
+  if ((int)blockIdx.x >= kv_blocks) {
+    const int x = blockIdx.x - kv_blocks, tile = x % (a.blocks * TQ), unit = x / (a.blocks * TQ);
+    const int head = unit % p.c.heads, b = unit / p.c.heads;
+    uint8_t* to = a.q_image + (long long)x * (kTile * D * 2);
+    for (int e = threadIdx.x; e < kTile * (D / 8); e += 256) {
+      const int rr = e / (D / 8), c16 = e % (D / 8), r = tile * kTile + rr;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < p.nq * group)
+        v = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_b + r / group * p.q_n +
+                                                 (head * group + r % group) * p.q_h + c16 * 8));
+      *reinterpret_cast<uint4*>(to + c16 / 8 * kSlotBytes + rr * 128 + ((c16 & 7) ^ (rr & 7)) * 16) = v;
+    }
+    return;
+  }
+  const int j = blockIdx.x % a.tiles, unit = blockIdx.x / a.tiles;
+  const int head = unit % p.c.heads, b = unit / p.c.heads;
+  const int len = sequence_length(p, b, err);
+  int lo, hi, none;
+  row_span(p, len, 0, &lo, &none);
+  row_span(p, len, p.nq - 1, &none, &hi);
+  const int tok0 = j * kTile, first = tok0 + warp * 16;
+  if (tok0 >= hi || tok0 + kTile <= lo) return;
+  const int per_page = p.c.page_size >> 4;
+  // tokens outside the span: their keys may hold anything, their values become zero
+  const bool live = first < hi && first + 16 > lo;
+  const int gi = live ? first >> 4 : max(lo, tok0) >> 4;
+  long long page = __ldg(p.pages + b * p.pages_stride + gi / per_page);
+  if (page < 0 || page >= p.c.n_pages) {
+    atomicCAS(err, 0, kDevErrIndex);
+    page = 0;
+  }
+  const uint8_t* k = p.c.data + kv_group_offset<QT, D>(p.c, page, head, 0, gi % per_page);
+  const uint8_t* v = k + (long long)per_page * L::kHalf;
+  uint8_t* item = a.image + (long long)blockIdx.x * (D * 512);
+  const int mine = first + 2 * (lane & 3);
+  auto in = [&](int tok) -> bool { return tok >= lo && tok < hi; };
+  const uint32_t keep0 = (in(mine) ? 0xFFFFu : 0u) | (in(mine + 1) ? 0xFFFF0000u : 0u);
+  const uint32_t keep1 = (in(mine + 8) ? 0xFFFFu : 0u) | (in(mine + 9) ? 0xFFFF0000u : 0u);
+#pragma unroll
+  for (int sb = 0; sb < D / L::kSB; ++sb) {
+    emit_k<QT, D>(k, item + sb * (L::kSB / 64) * kSlotBytes, warp, sb, lane);
+    emit_v<QT, D>(v, keep0, keep1, item + D * 256 + (warp >> 2) * (D * 128), warp, sb, lane);
+  }
+}
+
+// Whether the operands are staged as f16 first: where several row blocks of a unit would each dequantise the whole cache
+// again, and the images fit a bounded workspace. With one block (at most 256 rows, 128 at D = 256) the kernel that
+// dequantises for itself moves an eighth of the bytes.
+constexpr long long kStageMost = 1LL << 30;
+struct TcPlan {
+  int tq;
+  long long blocks, tiles, kv_bytes, q_bytes;
+  bool staged;
+};
+TcPlan tc_plan(const KvAttnParams& p) {
+  TcPlan t;
+  t.tq = p.c.d == 256 ? 1 : 2;
+  t.blocks = (p.nq * (long long)(p.heads / p.c.heads) + t.tq * kTile - 1) / (t.tq * kTile);
+  t.tiles = ((long long)p.max_pages * p.c.page_size + kTile - 1) / kTile;
+  const long long units = (long long)p.batch * p.c.heads;
+  t.kv_bytes = units * t.tiles * p.c.d * 512;
+  t.q_bytes = units * t.blocks * t.tq * kTile * p.c.d * 2;
+  t.staged = t.blocks >= 2 && t.tiles > 0 && units < (1 << 24) && t.tiles < (1 << 24) &&
+             t.kv_bytes + t.q_bytes <= kStageMost;
+  return t;
+}
+size_t part_floats(int sms, int tq, int d) { return (size_t)2 * sms * tq * kTile * (d + 2); }
+
+template <typename K, typename... A>
+int launch_dependent(K* kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  // may begin while its predecessor still runs; it waits for the predecessor's end before it reads its results
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(w.sms, C::kTQ * 4);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel<D, C::kTQ>, a) == cudaSuccess ? 0 : -12;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? 0 : -12;
+}
+
+template <int QT, int D>
+int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
+  constexpr int TQ = D == 256 ? 1 : 2;
+  if (w.sms > 160) return -2;  // join_kernel's table of factors
+  const TcPlan t = tc_plan(p);
+  TcArgs a;
+  a.p = p;
+  a.part = w.part;
+  a.shared = reinterpret_cast<Shared*>(w.part + part_floats(w.sms, TQ, D));
+  a.blocks = (int)t.blocks;
+  a.tiles = (int)t.tiles;
+  a.image = reinterpret_cast<uint8_t*>(w.part) + (part_floats(w.sms, TQ, D) * 4 + w.sms * sizeof(Shared) + 127) / 128 * 128;
+  a.q_image = a.image + t.kv_bytes;
+  int rc;
+  if (t.staged) {
+    typedef Tc<QT_Q4_0, D, true> C;  // the staged kernel does not depend on the cache's type
+    auto* k = tiles_kernel<QT_Q4_0, D, true>;
+    if (kernel_setup(k, C::kSmem) <= 0) return -13;
+    const long long kv_blocks = (long long)p.batch * p.c.heads * t.tiles;
+    const long long q_blocks = (long long)p.batch * p.c.heads * t.blocks * TQ;
+    stage_kernel<QT, D><<<(unsigned)(kv_blocks + q_blocks), 256, 0, st>>>(a, (int)kv_blocks, err);
+    if (cudaGetLastError() != cudaSuccess) return -12;
+    rc = launch_dependent(k, dim3(w.sms), C::kThreads, C::kSmem, st, a, err);
+  } else {
+    typedef Tc<QT, D, false> C;
+    auto* k = tiles_kernel<QT, D, false>;
+    if (kernel_setup(k, C::kSmem) <= 0) return -13;
+    k<<<w.sms, C::kThreads, C::kSmem, st>>>(a, err);
+    rc = cudaGetLastError() == cudaSuccess ? 0 : -12;
+  }
+  if (rc) return rc;
+  return launch_dependent(join_kernel<D, TQ>, dim3(w.sms, TQ * 4), 256, 0, st, a);
 }
 
 template <int QT>
@@ -1039,8 +1188,9 @@ int launch_tiles_d(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStr
 }  // namespace
 
 void kv_attention_tc_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes) {
-  const int tq = p.c.d == 256 ? 1 : 2;
-  *part_bytes = (size_t)2 * sms * tq * kTile * (p.c.d + 2) * 4 + sms * sizeof(Shared);
+  const TcPlan t = tc_plan(p);
+  *part_bytes = part_floats(sms, t.tq, p.c.d) * 4 + sms * sizeof(Shared) + 128 +
+                (t.staged ? (size_t)(t.kv_bytes + t.q_bytes) : 0);
   *count_bytes = 0;
 }
 
