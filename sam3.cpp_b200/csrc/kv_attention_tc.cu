@@ -14,8 +14,8 @@
 //   warp 2         copies the cache in block form (bulk copies of the keys or values of 16 tokens) into a ring
 //   dequantising   the remaining warps turn that ring's contents into f16 operands in a ring of 16 KB slots in the
 //                  128-byte swizzle, item by item (K or V of 128 tokens); they also load Q
-// D = 64, 128: TQ = 2 tiles ping-pong (one softmax runs beside the other tile's MMAs), one S region each, so S_{j+1} of a
-// tile follows its P V_j. D = 256: one tile, two S regions (O takes half of TMEM), S_{j+1} beside the softmax of tile j.
+// Every query tile has two S regions, so S of the next tokens runs beside the softmax of these: 64 tokens a region for D =
+// 64 and 128 (two query tiles and their O fill TMEM), 128 for D = 256 (one tile: O takes half of TMEM).
 //
 // The f16 operand is code * scale (+ minimum) rounded once. The 16 tokens of a group stand in the order
 // 0 1 8 9 2 3 10 11 4 5 12 13 6 7 14 15 (both in K's rows and V's columns; a softmax does not mind), which is the order
@@ -88,7 +88,8 @@ template <int QT, int D, bool STAGED>
 struct Tc {
   typedef KvL<QT, D> L;
   static constexpr int kTQ = D == 256 ? 1 : 2;
-  static constexpr int kSBuf = D == 256 ? 2 : 1;
+  static constexpr int kSub = D == 256 ? 128 : 64;          // tokens of an S region
+  static constexpr int kSubs = kTile / kSub;
   // dequantising warps: teams of 8; with two teams, team p makes part p of every item (K: 128 of the 256 values of a row,
   // V: 64 of the 128 tokens), so a part is published on its own
   static constexpr int kTeams = D == 256 ? 2 : 1;
@@ -106,7 +107,7 @@ struct Tc {
   static constexpr int kRaw = STAGED ? 0 : kRawFit > 8 ? 8 : kRawFit;  // entries of the block-form ring
   static constexpr int kSmem = 1024 + kQBytes + kSlots * kSlotBytes + kRaw * kUnitBytes + 512;
   static_assert(STAGED || kRaw >= 3, "K of a tile takes two entries of tiles_kernel's ring, and one has to be on its way");
-  static constexpr int kOCol = 256;                         // TMEM: S regions at 0 and 128, O after them
+  static constexpr int kOCol = 256;                         // TMEM: two S regions of kSub columns a tile, then O
   // Registers a thread at launch (65536 / threads, whole eights) and after the warpgroups trade: the issuing one, softmax
   // (kTQ warpgroups), dequantising (2 kTeams). The sum over warpgroups stays within the launch's.
   static constexpr int kRegsLaunch = 65536 / kThreads / 8 * 8;
@@ -350,28 +351,35 @@ __device__ __forceinline__ void weigh_scores(const uint32_t (&r)[32], uint32_t a
   KV_TMEM_ST8(at + 8, pk + 8);
 }
 
-// One token tile of one query row: the row's 128 scores from TMEM at `at`, the lazy reference maximum, the weights as f16
-// pairs over the first 64 columns, the sum into l. MASKED: only tokens [lo, hi) of the tile count. Returns true when the
-// maximum moved and the row of O has to be scaled by alpha. The scores are read twice, 32 at a time, in loops that stay
-// rolled: the softmax and the dequantising code of a sub-partition then fit its instruction cache together (with
-// all 128 scores unrolled most issue slots went to waiting for instructions).
-template <bool MASKED, int POLY>
+// One S region (N tokens) of one query row: the row's scores from TMEM at `at`, the lazy reference maximum, the weights as
+// f16 pairs over the first half of the region, the sum into l. MASKED: only tokens [lo, hi) of the region count. Returns
+// true when the maximum moved and the row of O has to be scaled by alpha. 64 scores stay in registers; 128 are read twice,
+// 32 at a time with 32 more on their way, in loops that stay rolled (unrolled, the loop's code was fetched again and again).
+template <int N, bool MASKED, int POLY>
 __device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float sl2, float& m_ref, float& l, float& alpha) {
-  // 32 scores are in flight while the 32 before them are worked on
   uint32_t ra[32], rb[32];
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
   KV_TMEM_LD32(at, ra);
-  tc_wait_ld();
-#pragma unroll 1
-  for (int c0 = 0; c0 < kTile; c0 += 64) {
-    KV_TMEM_LD32(at + c0 + 32, rb);
-    mask_scores<MASKED>(ra, c0, lo, hi);
+  if (N == 64) {
+    KV_TMEM_LD32(at + 32, rb);
+    tc_wait_ld();
+    mask_scores<MASKED>(ra, 0, lo, hi);
+    mask_scores<MASKED>(rb, 32, lo, hi);
     max_scores(ra, mx);
-    tc_wait_ld();
-    KV_TMEM_LD32(at + ((c0 + 64) & 127), ra);  // at the end the first ones again
-    mask_scores<MASKED>(rb, c0 + 32, lo, hi);
     max_scores(rb, mx);
+  } else {
     tc_wait_ld();
+#pragma unroll 1
+    for (int c0 = 0; c0 < N; c0 += 64) {
+      KV_TMEM_LD32(at + c0 + 32, rb);
+      mask_scores<MASKED>(ra, c0, lo, hi);
+      max_scores(ra, mx);
+      tc_wait_ld();
+      KV_TMEM_LD32(at + ((c0 + 64) & (N - 1)), ra);  // at the end the first ones again
+      mask_scores<MASKED>(rb, c0 + 32, lo, hi);
+      max_scores(rb, mx);
+      tc_wait_ld();
+    }
   }
   const float top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * sl2;
   alpha = 1.f;
@@ -384,17 +392,22 @@ __device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float 
   }
   const unsigned long long sl2x2 = f2_pack(sl2, sl2), negm2 = f2_pack(-m_ref, -m_ref);
   unsigned long long acc0 = f2_pack(0.f, 0.f), acc1 = acc0;
+  if (N == 64) {
+    weigh_scores<MASKED, POLY>(ra, at, sl2x2, negm2, acc0, acc1);
+    weigh_scores<MASKED, POLY>(rb, at + 16, sl2x2, negm2, acc0, acc1);
+  } else {
 #pragma unroll 1
-  for (int c0 = 0; c0 < kTile; c0 += 64) {
-    // the weights of 32 scores go over columns whose scores have been read
-    KV_TMEM_LD32(at + c0 + 32, rb);
-    mask_scores<MASKED>(ra, c0, lo, hi);
-    weigh_scores<MASKED, POLY>(ra, at + c0 / 2, sl2x2, negm2, acc0, acc1);
-    tc_wait_ld();
-    KV_TMEM_LD32(at + ((c0 + 64) & 127), ra);  // unused at the end
-    mask_scores<MASKED>(rb, c0 + 32, lo, hi);
-    weigh_scores<MASKED, POLY>(rb, at + c0 / 2 + 16, sl2x2, negm2, acc0, acc1);
-    tc_wait_ld();
+    for (int c0 = 0; c0 < N; c0 += 64) {
+      // the weights of 32 scores go over columns whose scores have been read
+      KV_TMEM_LD32(at + c0 + 32, rb);
+      mask_scores<MASKED>(ra, c0, lo, hi);
+      weigh_scores<MASKED, POLY>(ra, at + c0 / 2, sl2x2, negm2, acc0, acc1);
+      tc_wait_ld();
+      KV_TMEM_LD32(at + ((c0 + 64) & (N - 1)), ra);  // unused at the end
+      mask_scores<MASKED>(rb, c0 + 32, lo, hi);
+      weigh_scores<MASKED, POLY>(rb, at + c0 / 2 + 16, sl2x2, negm2, acc0, acc1);
+      tc_wait_ld();
+    }
   }
   float a0, a1, b0, b1;
   f2_unpack(acc0, a0, a1);
@@ -418,13 +431,13 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
   uint64_t* q_empty = bars + 1;
   uint64_t* full = bars + 2;                 // [kSlots]
   uint64_t* empty = full + kSlots;           // [kSlots]
-  uint64_t* s_full = empty + kSlots;         // [2 regions]
-  uint64_t* p_full = s_full + 2;             // [2 tiles]
+  uint64_t* s_full = empty + kSlots;         // [2 tiles][2 regions]
+  uint64_t* p_full = s_full + 4;             // [2 tiles]
   uint64_t* pv_done = p_full + 2;            // [2 tiles]
   uint64_t* mma_done = pv_done + 2;          // [2 tiles]
   uint64_t* raw_full = mma_done + 2;         // [kRaw]
   uint64_t* raw_empty = raw_full + C::kRaw;  // [kRaw]
-  static_assert((2 + 2 * kSlots + 8 + 2 * C::kRaw) * 8 <= 512, "barriers of tiles_kernel");
+  static_assert((2 + 2 * kSlots + 10 + 2 * C::kRaw) * 8 <= 512, "barriers of tiles_kernel");
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort_word, s_pair;
   __shared__ long long s_sum[24], s_start;
@@ -445,7 +458,8 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
       mbar_init(&empty[s], TQ);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&s_full[x], 1);
+      mbar_init(&s_full[2 * x], 1);
+      mbar_init(&s_full[2 * x + 1], 1);
       mbar_init(&p_full[x], 4);
       mbar_init(&pv_done[x], 1);
       mbar_init(&mma_done[x], 1);
@@ -530,10 +544,10 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
   }
   __syncwarp();
   const float sl2 = p.scale * kLog2e;
-  // Item x of a segment of n tiles: K or V of tile *j. One S region: K_0 V_0 K_1 V_1 ...; two: K_0 K_1 V_0 K_2 V_1 ...
-  // V_last; the order in which the MMAs take them.
+  // Item x of a segment of n tiles: K or V of tile *j, in the order in which the MMAs first take them. Tiles of two S
+  // regions: K_0 V_0 K_1 V_1 ...; of one: K_0 K_1 V_0 K_2 V_1 ... V_last.
   auto order = [](int x, int n, int* j) -> bool {
-    if (C::kSBuf == 1 || x == 0) {
+    if (C::kSubs == 2 || x == 0) {
       *j = x >> 1;
       return !(x & 1);
     }
@@ -541,6 +555,9 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
     *j = x == 2 * n - 1 ? n - 1 : k ? (x + 1) >> 1 : (x >> 1) - 1;
     return k;
   };
+  // and the place of K_j and V_j in it
+  auto k_item = [](int j) -> int { return C::kSubs == 2 ? 2 * j : j ? 2 * j - 1 : 0; };
+  auto v_item = [](int j, int n) -> int { return C::kSubs == 2 ? 2 * j + 1 : j == n - 1 ? 2 * n - 1 : 2 * j + 2; };
 
   if (warp < 4) {
     if (!STAGED) regs_dec<C::kRegsIssue>();
@@ -680,53 +697,54 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
     } else if (warp < TQ && lane == 0) {
       // ---- MMA issue for query tile `warp`
       const int t = warp;
-      constexpr uint32_t idesc_s = idesc_f16(kTile, kTile, 0), idesc_o = idesc_f16(kTile, D, 0);
+      constexpr uint32_t idesc_s = idesc_f16(kTile, C::kSub, 0), idesc_o = idesc_f16(kTile, D, 0);
       const uint32_t q_base = smem_u32(s_q) + t * (kTile * D * 2), ring = smem_u32(s_ring);
       const uint32_t o_tmem = tmem + C::kOCol + t * D;
-      uint32_t slot = 0, q_n = 0, ns = 0, npv = 0;  // slots, Q loads, S and P V products so far
+      uint32_t slot0 = 0, q_n = 0, ns = 0, npv = 0;  // slots before the segment; Q loads, S and P V products so far
       bool ok = true, issued = false;
       auto wait_slot = [&](uint32_t s) -> bool {
         if (!mbar_wait(&full[s % kSlots], (s / kSlots) & 1, s_abort, err, kErrWaitFull)) return false;
         tc_fence_after();
         return true;
       };
-      auto s_region = [&](uint32_t n) -> uint32_t { return C::kSBuf == 2 ? (n & 1) : (uint32_t)t; };
-      auto issue_s = [&](bool last) -> bool {
-        const uint32_t reg = s_region(ns);
+      auto s_region = [&](uint32_t n) -> uint32_t { return tmem + (2 * t + (n & 1)) * C::kSub; };
+      // S of sub-tile u of the segment: kSub tokens of tile u / kSubs
+      auto issue_s = [&](int u, bool last) -> bool {
+        const int j = u / C::kSubs, sub = u % C::kSubs;
+        const uint32_t s0 = slot0 + k_item(j) * C::kParts;
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c, ++slot) {
-          if (!wait_slot(slot)) return false;
+        for (int c = 0; c < D / 64; ++c) {
+          if (sub == 0 && !wait_slot(s0 + c)) return false;
           const uint64_t dq = sdesc_k_sw128(q_base + c * kSlotBytes);
-          const uint64_t dk = sdesc_k_sw128(ring + slot % kSlots * kSlotBytes);
+          const uint64_t dk = sdesc_k_sw128(ring + (s0 + c) % kSlots * kSlotBytes + sub * (kSlotBytes / 2));
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma_f16(tmem + 128 * reg, dq + kk * 2, dk + kk * 2, idesc_s, c != 0 || kk != 0);
-          tc_commit(&empty[slot % kSlots]);
+          for (int kk = 0; kk < 4; ++kk) tc_mma_f16(s_region(ns), dq + kk * 2, dk + kk * 2, idesc_s, c != 0 || kk != 0);
+          if (sub == C::kSubs - 1) tc_commit(&empty[(s0 + c) % kSlots]);
         }
-        tc_commit(&s_full[reg]);
+        tc_commit(&s_full[2 * t + (ns & 1)]);
         if (last) tc_commit(q_empty);
         ++ns;
         issued = true;
         return true;
       };
-      auto issue_pv = [&](bool first) -> bool {
+      // O += P V of sub-tile u, by 64 tokens of V
+      auto issue_pv = [&](int u, int n) -> bool {
+        const int j = u / C::kSubs, sub = u % C::kSubs;
         if (!mbar_wait(&p_full[t], npv & 1, s_abort, err, kErrWaitMisc)) return false;
         tc_fence_after();
-        const uint32_t pa = tmem + 128 * s_region(npv);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (D > 64 || half == 0) {
-            if (!wait_slot(slot)) return false;
-          }
+        for (int x = 0; x < C::kSub / 64; ++x) {
+          const int half = C::kSubs == 2 ? sub : x;
+          const uint32_t s0 = slot0 + v_item(j, n) * C::kParts + (D == 64 ? 0 : half * (D / 128));
+          if ((D > 64 || half == 0) && !wait_slot(s0)) return false;
+          const uint32_t v = ring + s0 % kSlots * kSlotBytes + (D == 64 ? half * (D * 128) : 0);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            tc_mma_f16_ts(o_tmem, pa + half * 32 + kk * 8, sdesc_k_sw128(ring + slot % kSlots * kSlotBytes + (D == 64 ? half * (D * 128) : 0)) + kk * 2, idesc_o,
-                          !first || half != 0 || kk != 0);
-          if (D == 64) {
-            if (half == 1) tc_commit(&empty[slot++ % kSlots]);
-          } else {
+            tc_mma_f16_ts(o_tmem, s_region(npv) + x * 32 + kk * 8, sdesc_k_sw128(v) + kk * 2, idesc_o,
+                          u != 0 || x != 0 || kk != 0);
+          if (D > 64 || half == 1) {
 #pragma unroll
-            for (int x = 0; x < D / 128; ++x) tc_commit(&empty[slot++ % kSlots]);
+            for (int y = 0; y < (D > 64 ? D / 128 : 1); ++y) tc_commit(&empty[(s0 + y) % kSlots]);
           }
         }
         tc_commit(&pv_done[t]);
@@ -735,25 +753,26 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
         return true;
       };
       while (ok && walk_next<ROWS>(p, a.blocks, err, &w)) {
-        const int n = w.cb - w.ca;
+        const int n = w.cb - w.ca, subs = n * C::kSubs;
         if (!mbar_wait(q_full, q_n & 1, s_abort, err, kErrWaitFull)) { ok = false; break; }
         ++q_n;
         tc_fence_after();
         if (w.u.row0 + t * kTile >= n_rows) {
           // no second tile: release the slots as they fill, so that the counts of both issuers stay in step
           mbar_arrive(q_empty);
-          for (int x = 0; x < n * 2 * C::kParts && ok; ++x, ++slot) {
-            if (!wait_slot(slot)) { ok = false; break; }
-            mbar_arrive(&empty[slot % kSlots]);
+          for (int x = 0; x < n * 2 * C::kParts && ok; ++x) {
+            if (!wait_slot(slot0 + x)) { ok = false; break; }
+            mbar_arrive(&empty[(slot0 + x) % kSlots]);
           }
-          continue;
+        } else {
+          // S of the next sub-tile runs beside the softmax of this one
+          if (!issue_s(0, subs == 1)) { ok = false; break; }
+          for (int u = 0; u < subs && ok; ++u) {
+            if (u + 1 < subs && !issue_s(u + 1, u + 2 == subs)) { ok = false; break; }
+            if (!issue_pv(u, n)) { ok = false; break; }
+          }
         }
-        if (!issue_s(n == 1)) { ok = false; break; }
-        for (int j = 0; j < n && ok; ++j) {
-          if (C::kSBuf == 2 && j + 1 < n && !issue_s(j + 2 == n)) { ok = false; break; }
-          if (!issue_pv(j == 0)) { ok = false; break; }
-          if (C::kSBuf == 1 && j + 1 < n && !issue_s(j + 2 == n)) { ok = false; break; }
-        }
+        slot0 += n * 2 * C::kParts;
       }
       if (issued) {
         tc_commit(&mma_done[t]);
@@ -772,7 +791,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
     const int t = (warp - 4) >> 2, w4 = warp & 3, row = w4 * 32 + lane;
     const uint32_t lane_off = (uint32_t)(w4 * 32) << 16;
     const uint32_t o_at = tmem + lane_off + C::kOCol + t * D;
-    uint32_t n = 0;  // token tiles of this query tile so far
+    uint32_t n = 0;  // S regions of this query tile so far
     bool ok = true;
     if (t == 0 && row == 0) a.shared[blockIdx.x].valid = 0;
     while (ok && walk_next_warp<ROWS>(p, a.blocks, err, &w, lane)) {
@@ -784,17 +803,17 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
       row_span(p, w.u.len, min(n_rows - 1, r0 + kTile - 1) / group, &all_lo, &none);
       const int tok_first = (w.u.t0 + w.ca) * kTile, tok_end = (w.u.t0 + w.cb) * kTile;
       float m_ref = kNoScore, l = 0.f;
-      for (int tok0 = tok_first; tok0 < tok_end; tok0 += kTile, ++n) {
-        const uint32_t reg = C::kSBuf == 2 ? (n & 1) : (uint32_t)t;
-        if (!mbar_wait(&s_full[reg], (C::kSBuf == 2 ? n >> 1 : n) & 1, s_abort, err, kErrWaitTmemFull)) ok = false;
+      for (int tok0 = tok_first; tok0 < tok_end; tok0 += C::kSub, ++n) {
+        if (!mbar_wait(&s_full[2 * t + (n & 1)], (n >> 1) & 1, s_abort, err, kErrWaitTmemFull)) ok = false;
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t s_at = tmem + lane_off + 128 * reg;
+        const uint32_t s_at = tmem + lane_off + (2 * t + (n & 1)) * C::kSub;
         float alpha;
-        const bool moved = tok0 >= all_lo && tok0 + kTile <= all_hi
-                               ? softmax_tile<false, C::kPoly>(s_at, 0, 0, sl2, m_ref, l, alpha)
-                               : softmax_tile<true, 0>(s_at, lo - tok0, hi - tok0, sl2, m_ref, l, alpha);
+        const bool moved =
+            tok0 >= all_lo && tok0 + C::kSub <= all_hi
+                ? softmax_tile<C::kSub, false, C::kPoly>(s_at, 0, 0, sl2, m_ref, l, alpha)
+                : softmax_tile<C::kSub, true, 0>(s_at, lo - tok0, hi - tok0, sl2, m_ref, l, alpha);
         if (tok0 > tok_first) {
           // O is current once the previous P V product of this tile has completed
           if (!mbar_wait(&pv_done[t], (n - 1) & 1, s_abort, err, kErrWaitMisc)) ok = false;
