@@ -69,15 +69,6 @@ __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// 2^x, x <= 8, on the FMA pipe (the range reduction and the degree-3 fit of attention_tc.cu's softmax).
-__device__ __forceinline__ float exp2_fma(float x) {
-  x = fmaxf(x, -126.f);
-  const float j = x + 12582912.f;
-  const float f = x - (j - 12582912.f);
-  const float p = fmaf(fmaf(fmaf(0.0551716685f, f, 0.2426111251f), f, 0.6932609677f), f, 0.9999280572f);
-  return __int_as_float(__float_as_int(p) + (__float_as_int(j) << 23));
-}
-
 constexpr int kTile = 128;          // query rows of a tile and tokens of a tile
 constexpr int kSlotBytes = 16384;   // 128 x 64 f16
 constexpr int kUnit = 64;           // tokens of an entry of the block-form ring
@@ -116,8 +107,6 @@ struct Tc {
   static constexpr int kRegsDeq = D == 256 ? 72 : 80;
   static_assert(STAGED || kRegsIssue + kTQ * kRegsSoft + 2 * kTeams * kRegsDeq <= kThreads / 128 * kRegsLaunch, "register shares");
   static constexpr int kPart = kTQ * kTile * (D + 2);       // floats of a unit's part
-  // of every 8 exponentials, how many run on the FMA pipe: 2 where two softmax warpgroups share the MUFU units
-  static constexpr int kPoly = kTQ == 2 ? 2 : 0;
 };
 
 // A unit that several CTAs share, written by the CTA in whose share it begins (its entry's index).
@@ -326,7 +315,6 @@ __device__ __forceinline__ void max_scores(const uint32_t (&r)[32], float (&mx)[
     for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1]));
 }
 // weights of 32 scores to the 16 columns at `at`; acc: the sums of even and odd pairs
-template <bool MASKED, int POLY>
 __device__ __forceinline__ void weigh_scores(const uint32_t (&r)[32], uint32_t at, unsigned long long sl2x2,
                                              unsigned long long negm2, unsigned long long& acc0, unsigned long long& acc1) {
   uint32_t pk[16];
@@ -338,9 +326,10 @@ __device__ __forceinline__ void weigh_scores(const uint32_t (&r)[32], uint32_t a
       const int c = 8 * u + e;
       float x0, x1;
       f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl2x2, negm2), x0, x1);
-      // a hidden token's -inf gives 0 exactly, so a row that sees nothing keeps the sum 0
-      pv[e] = !MASKED && e < POLY ? exp2_fma(x0) : ex2_approx(x0);
-      pv[e + 1] = !MASKED && e + 1 < POLY ? exp2_fma(x1) : ex2_approx(x1);
+      // a hidden token's -inf gives 0 exactly, so a row that sees nothing keeps the sum 0; a share of the exponentials on
+      // the FMA pipe gained nothing (d = 64) or cost 5% (d = 128, 2 of 8)
+      pv[e] = ex2_approx(x0);
+      pv[e + 1] = ex2_approx(x1);
     }
     acc0 = f2_add(acc0, f2_add(f2_pack(pv[0], pv[1]), f2_pack(pv[4], pv[5])));
     acc1 = f2_add(acc1, f2_add(f2_pack(pv[2], pv[3]), f2_pack(pv[6], pv[7])));
@@ -355,7 +344,7 @@ __device__ __forceinline__ void weigh_scores(const uint32_t (&r)[32], uint32_t a
 // f16 pairs over the first half of the region, the sum into l. MASKED: only tokens [lo, hi) of the region count. Returns
 // true when the maximum moved and the row of O has to be scaled by alpha. 64 scores stay in registers; 128 are read twice,
 // 32 at a time with 32 more on their way, in loops that stay rolled (unrolled, the loop's code was fetched again and again).
-template <int N, bool MASKED, int POLY>
+template <int N, bool MASKED>
 __device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float sl2, float& m_ref, float& l, float& alpha) {
   uint32_t ra[32], rb[32];
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -393,19 +382,19 @@ __device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float 
   const unsigned long long sl2x2 = f2_pack(sl2, sl2), negm2 = f2_pack(-m_ref, -m_ref);
   unsigned long long acc0 = f2_pack(0.f, 0.f), acc1 = acc0;
   if (N == 64) {
-    weigh_scores<MASKED, POLY>(ra, at, sl2x2, negm2, acc0, acc1);
-    weigh_scores<MASKED, POLY>(rb, at + 16, sl2x2, negm2, acc0, acc1);
+    weigh_scores(ra, at, sl2x2, negm2, acc0, acc1);
+    weigh_scores(rb, at + 16, sl2x2, negm2, acc0, acc1);
   } else {
 #pragma unroll 1
     for (int c0 = 0; c0 < N; c0 += 64) {
       // the weights of 32 scores go over columns whose scores have been read
       KV_TMEM_LD32(at + c0 + 32, rb);
       mask_scores<MASKED>(ra, c0, lo, hi);
-      weigh_scores<MASKED, POLY>(ra, at + c0 / 2, sl2x2, negm2, acc0, acc1);
+      weigh_scores(ra, at + c0 / 2, sl2x2, negm2, acc0, acc1);
       tc_wait_ld();
       KV_TMEM_LD32(at + ((c0 + 64) & (N - 1)), ra);  // unused at the end
       mask_scores<MASKED>(rb, c0 + 32, lo, hi);
-      weigh_scores<MASKED, POLY>(rb, at + c0 / 2 + 16, sl2x2, negm2, acc0, acc1);
+      weigh_scores(rb, at + c0 / 2 + 16, sl2x2, negm2, acc0, acc1);
       tc_wait_ld();
     }
   }
@@ -434,10 +423,11 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
   uint64_t* s_full = empty + kSlots;         // [2 tiles][2 regions]
   uint64_t* p_full = s_full + 4;             // [2 tiles]
   uint64_t* pv_done = p_full + 2;            // [2 tiles]
-  uint64_t* mma_done = pv_done + 2;          // [2 tiles]
+  uint64_t* o_full = pv_done + 2;            // [2 tiles]
+  uint64_t* mma_done = o_full + 2;           // [2 tiles]
   uint64_t* raw_full = mma_done + 2;         // [kRaw]
   uint64_t* raw_empty = raw_full + C::kRaw;  // [kRaw]
-  static_assert((2 + 2 * kSlots + 10 + 2 * C::kRaw) * 8 <= 512, "barriers of tiles_kernel");
+  static_assert((2 + 2 * kSlots + 12 + 2 * C::kRaw) * 8 <= 512, "barriers of tiles_kernel");
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort_word, s_pair;
   __shared__ long long s_sum[24], s_start;
@@ -462,6 +452,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
       mbar_init(&s_full[2 * x + 1], 1);
       mbar_init(&p_full[x], 4);
       mbar_init(&pv_done[x], 1);
+      mbar_init(&o_full[x], 1);
       mbar_init(&mma_done[x], 1);
     }
     for (int x = 0; x < C::kRaw; ++x) {
@@ -771,6 +762,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
             if (u + 1 < subs && !issue_s(u + 1, u + 2 == subs)) { ok = false; break; }
             if (!issue_pv(u, n)) { ok = false; break; }
           }
+          if (ok) tc_commit(&o_full[t]);
         }
         slot0 += n * 2 * C::kParts;
       }
@@ -791,7 +783,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
     const int t = (warp - 4) >> 2, w4 = warp & 3, row = w4 * 32 + lane;
     const uint32_t lane_off = (uint32_t)(w4 * 32) << 16;
     const uint32_t o_at = tmem + lane_off + C::kOCol + t * D;
-    uint32_t n = 0;  // S regions of this query tile so far
+    uint32_t n = 0, segs = 0;  // S regions and segments of this query tile so far
     bool ok = true;
     if (t == 0 && row == 0) a.shared[blockIdx.x].valid = 0;
     while (ok && walk_next_warp<ROWS>(p, a.blocks, err, &w, lane)) {
@@ -812,25 +804,24 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
         float alpha;
         const bool moved =
             tok0 >= all_lo && tok0 + C::kSub <= all_hi
-                ? softmax_tile<C::kSub, false, C::kPoly>(s_at, 0, 0, sl2, m_ref, l, alpha)
-                : softmax_tile<C::kSub, true, 0>(s_at, lo - tok0, hi - tok0, sl2, m_ref, l, alpha);
-        if (tok0 > tok_first) {
-          // O is current once the previous P V product of this tile has completed
+                ? softmax_tile<C::kSub, false>(s_at, 0, 0, sl2, m_ref, l, alpha)
+                : softmax_tile<C::kSub, true>(s_at, lo - tok0, hi - tok0, sl2, m_ref, l, alpha);
+        if (tok0 > tok_first && __any_sync(~0u, moved)) {
+          // O is current once the previous P V product of this tile has completed. The one before it has: S of this
+          // region was issued after it, so the barrier cannot be a phase behind.
           if (!mbar_wait(&pv_done[t], (n - 1) & 1, s_abort, err, kErrWaitMisc)) ok = false;
           ok = __all_sync(~0u, ok);
           if (!ok) break;
           tc_fence_after();
-          if (__any_sync(~0u, moved)) {
-            const float f = moved ? alpha : 1.f;
+          const float f = moved ? alpha : 1.f;
 #pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              KV_TMEM_LD32(o_at + c, o);
-              tc_wait_ld();
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            KV_TMEM_LD32(o_at + c, o);
+            tc_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              KV_TMEM_ST32(o_at + c, o);
-            }
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            KV_TMEM_ST32(o_at + c, o);
           }
         }
         tc_wait_st();
@@ -839,9 +830,10 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
         if (lane == 0) mbar_arrive(&p_full[t]);
       }
       if (!ok) break;
-      if (!mbar_wait(&pv_done[t], (n - 1) & 1, s_abort, err, kErrWaitMisc)) ok = false;
+      if (!mbar_wait(&o_full[t], segs & 1, s_abort, err, kErrWaitMisc)) ok = false;
       ok = __all_sync(~0u, ok);
       if (!ok) break;
+      ++segs;
       tc_fence_after();
       const int r = r0 + row, i = min(r, n_rows - 1) / group, h = w.u.head * group + r % group;
       const bool real = r < n_rows;
