@@ -421,13 +421,14 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
   uint64_t* full = bars + 2;                 // [kSlots]
   uint64_t* empty = full + kSlots;           // [kSlots]
   uint64_t* s_full = empty + kSlots;         // [2 tiles][2 regions]
-  uint64_t* p_full = s_full + 4;             // [2 tiles]
-  uint64_t* pv_done = p_full + 2;            // [2 tiles]
+  uint64_t* p_full = s_full + 4;             // [2 tiles][2 regions]: the softmax of the next region may be done before the
+                                             // issuer looks at this one
+  uint64_t* pv_done = p_full + 4;            // [2 tiles]
   uint64_t* o_full = pv_done + 2;            // [2 tiles]
   uint64_t* mma_done = o_full + 2;           // [2 tiles]
   uint64_t* raw_full = mma_done + 2;         // [kRaw]
   uint64_t* raw_empty = raw_full + C::kRaw;  // [kRaw]
-  static_assert((2 + 2 * kSlots + 12 + 2 * C::kRaw) * 8 <= 512, "barriers of tiles_kernel");
+  static_assert((2 + 2 * kSlots + 14 + 2 * C::kRaw) * 8 <= 512, "barriers of tiles_kernel");
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort_word, s_pair;
   __shared__ long long s_sum[24], s_start;
@@ -450,7 +451,8 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
     for (int x = 0; x < 2; ++x) {
       mbar_init(&s_full[2 * x], 1);
       mbar_init(&s_full[2 * x + 1], 1);
-      mbar_init(&p_full[x], 4);
+      mbar_init(&p_full[2 * x], 4);
+      mbar_init(&p_full[2 * x + 1], 4);
       mbar_init(&pv_done[x], 1);
       mbar_init(&o_full[x], 1);
       mbar_init(&mma_done[x], 1);
@@ -721,7 +723,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
       // O += P V of sub-tile u, by 64 tokens of V
       auto issue_pv = [&](int u, int n) -> bool {
         const int j = u / C::kSubs, sub = u % C::kSubs;
-        if (!mbar_wait(&p_full[t], npv & 1, s_abort, err, kErrWaitMisc)) return false;
+        if (!mbar_wait(&p_full[2 * t + (npv & 1)], (npv >> 1) & 1, s_abort, err, kErrWaitMisc)) return false;
         tc_fence_after();
 #pragma unroll
         for (int x = 0; x < C::kSub / 64; ++x) {
@@ -827,7 +829,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        if (lane == 0) mbar_arrive(&p_full[2 * t + (n & 1)]);
       }
       if (!ok) break;
       if (!mbar_wait(&o_full[t], segs & 1, s_abort, err, kErrWaitMisc)) ok = false;
