@@ -60,6 +60,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// One lane of a converged warp, always the same. The compiler then knows that a single lane runs what follows and feeds the
+// MMAs from uniform registers: 78 clocks for a 128 x 128 x 16 product from TMEM, against 168 behind `lane == 0`.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 template <int N>
 __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
@@ -436,7 +443,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
   volatile int* s_abort = &s_abort_word;
 
   const KvAttnParams& p = a.p;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // uniform for the compiler
   const int group = p.heads / p.c.heads;
   const int n_rows = p.nq * group;
   const int pairs = p.batch * a.blocks;
@@ -687,19 +694,20 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
               }
             }
           }
-    } else if (warp < TQ && lane == 0) {
-      // ---- MMA issue for query tile `warp`
+    } else if (warp < TQ) {
+      // ---- MMA issue for query tile `warp`: the warp waits together, one lane issues
       const int t = warp;
       constexpr uint32_t idesc_s = idesc_f16(kTile, C::kSub, 0), idesc_o = idesc_f16(kTile, D, 0);
       const uint32_t q_base = smem_u32(s_q) + t * (kTile * D * 2), ring = smem_u32(s_ring);
       const uint32_t o_tmem = tmem + C::kOCol + t * D;
       uint32_t slot0 = 0, q_n = 0, ns = 0, npv = 0;  // slots before the segment; Q loads, S and P V products so far
       bool ok = true, issued = false;
-      auto wait_slot = [&](uint32_t s) -> bool {
-        if (!mbar_wait(&full[s % kSlots], (s / kSlots) & 1, s_abort, err, kErrWaitFull)) return false;
+      auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+        if (!__all_sync(~0u, mbar_wait(bar, parity, s_abort, err, code))) return false;
         tc_fence_after();
         return true;
       };
+      auto wait_slot = [&](uint32_t s) -> bool { return wait(&full[s % kSlots], (s / kSlots) & 1, kErrWaitFull); };
       auto s_region = [&](uint32_t n) -> uint32_t { return tmem + (2 * t + (n & 1)) * C::kSub; };
       // S of sub-tile u of the segment: kSub tokens of tile u / kSubs
       auto issue_s = [&](int u, bool last) -> bool {
@@ -710,12 +718,16 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
           if (sub == 0 && !wait_slot(s0 + c)) return false;
           const uint64_t dq = sdesc_k_sw128(q_base + c * kSlotBytes);
           const uint64_t dk = sdesc_k_sw128(ring + (s0 + c) % kSlots * kSlotBytes + sub * (kSlotBytes / 2));
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) tc_mma_f16(s_region(ns), dq + kk * 2, dk + kk * 2, idesc_s, c != 0 || kk != 0);
-          if (sub == C::kSubs - 1) tc_commit(&empty[(s0 + c) % kSlots]);
+            for (int kk = 0; kk < 4; ++kk) tc_mma_f16(s_region(ns), dq + kk * 2, dk + kk * 2, idesc_s, c != 0 || kk != 0);
+            if (sub == C::kSubs - 1) tc_commit(&empty[(s0 + c) % kSlots]);
+            if (c == D / 64 - 1) {
+              tc_commit(&s_full[2 * t + (ns & 1)]);
+              if (last) tc_commit(q_empty);
+            }
+          }
         }
-        tc_commit(&s_full[2 * t + (ns & 1)]);
-        if (last) tc_commit(q_empty);
         ++ns;
         issued = true;
         return true;
@@ -723,52 +735,52 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
       // O += P V of sub-tile u, by 64 tokens of V
       auto issue_pv = [&](int u, int n) -> bool {
         const int j = u / C::kSubs, sub = u % C::kSubs;
-        if (!mbar_wait(&p_full[2 * t + (npv & 1)], (npv >> 1) & 1, s_abort, err, kErrWaitMisc)) return false;
-        tc_fence_after();
+        if (!wait(&p_full[2 * t + (npv & 1)], (npv >> 1) & 1, kErrWaitMisc)) return false;
 #pragma unroll
         for (int x = 0; x < C::kSub / 64; ++x) {
           const int half = C::kSubs == 2 ? sub : x;
           const uint32_t s0 = slot0 + v_item(j, n) * C::kParts + (D == 64 ? 0 : half * (D / 128));
           if ((D > 64 || half == 0) && !wait_slot(s0)) return false;
-          const uint32_t v = ring + s0 % kSlots * kSlotBytes + (D == 64 ? half * (D * 128) : 0);
+          const uint64_t dv = sdesc_k_sw128(ring + s0 % kSlots * kSlotBytes + (D == 64 ? half * (D * 128) : 0));
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma_f16_ts(o_tmem, s_region(npv) + x * 32 + kk * 8, sdesc_k_sw128(v) + kk * 2, idesc_o,
-                          u != 0 || x != 0 || kk != 0);
-          if (D > 64 || half == 1) {
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma_f16_ts(o_tmem, s_region(npv) + x * 32 + kk * 8, dv + kk * 2, idesc_o, u != 0 || x != 0 || kk != 0);
+            if (D > 64 || half == 1) {
 #pragma unroll
-            for (int y = 0; y < (D > 64 ? D / 128 : 1); ++y) tc_commit(&empty[(s0 + y) % kSlots]);
+              for (int y = 0; y < (D > 64 ? D / 128 : 1); ++y) tc_commit(&empty[(s0 + y) % kSlots]);
+            }
+            if (x == C::kSub / 64 - 1) {
+              tc_commit(&pv_done[t]);
+              if (u == n * C::kSubs - 1) tc_commit(&o_full[t]);
+            }
           }
         }
-        tc_commit(&pv_done[t]);
         ++npv;
-        issued = true;
         return true;
       };
-      while (ok && walk_next<ROWS>(p, a.blocks, err, &w)) {
+      while (ok && walk_next_warp<ROWS>(p, a.blocks, err, &w, lane)) {
         const int n = w.cb - w.ca, subs = n * C::kSubs;
-        if (!mbar_wait(q_full, q_n & 1, s_abort, err, kErrWaitFull)) { ok = false; break; }
+        if (!wait(q_full, q_n & 1, kErrWaitFull)) break;
         ++q_n;
-        tc_fence_after();
         if (w.u.row0 + t * kTile >= n_rows) {
           // no second tile: release the slots as they fill, so that the counts of both issuers stay in step
-          mbar_arrive(q_empty);
+          if (lane == 0) mbar_arrive(q_empty);
           for (int x = 0; x < n * 2 * C::kParts && ok; ++x) {
-            if (!wait_slot(slot0 + x)) { ok = false; break; }
-            mbar_arrive(&empty[(slot0 + x) % kSlots]);
+            ok = wait_slot(slot0 + x);
+            if (ok && lane == 0) mbar_arrive(&empty[(slot0 + x) % kSlots]);
           }
         } else {
           // S of the next sub-tile runs beside the softmax of this one
-          if (!issue_s(0, subs == 1)) { ok = false; break; }
+          ok = issue_s(0, subs == 1);
           for (int u = 0; u < subs && ok; ++u) {
-            if (u + 1 < subs && !issue_s(u + 1, u + 2 == subs)) { ok = false; break; }
-            if (!issue_pv(u, n)) { ok = false; break; }
+            if (u + 1 < subs) ok = issue_s(u + 1, u + 2 == subs);
+            ok = ok && issue_pv(u, n);
           }
-          if (ok) tc_commit(&o_full[t]);
         }
         slot0 += n * 2 * C::kParts;
       }
-      if (issued) {
+      if (issued && elect_one()) {
         tc_commit(&mma_done[t]);
         const unsigned long long t0 = globaltimer_ns();
         while (!mbar_try_wait(&mma_done[t], 0)) {
