@@ -191,6 +191,29 @@ def dequantize_rows(qtype: int, raw: np.ndarray, ne0: int) -> np.ndarray:
     return out
 
 
+def _index(what: str, name: str, t, itemsize: int, dims: int) -> int:
+    """Length of an index tensor of `dims` dimensions (int32: itemsize 4, int64: 8) with contiguous rows."""
+    if t.dtype.itemsize != itemsize or t.dtype.is_floating_point or t.dtype.is_complex or t.dim() != dims or \
+            (t.stride(dims - 1) != 1 and t.numel()):
+        raise S3BError(f"{what}: {name} must be int{8 * itemsize} of {dims} dimension(s) with contiguous rows")
+    return t.shape[0]
+
+
+def _strides2(t):
+    """Strides of the first two dimensions, 0 where a dimension has one entry (its stride means nothing)."""
+    if t is None:
+        return 0, 0
+    a, b, _ = t.stride()
+    n, h, _ = t.shape
+    return a if n > 1 else 0, b if h > 1 else 0
+
+
+def _strides3(t):
+    a, b, c, _ = t.stride()
+    i, j, k, _ = t.shape
+    return a if i > 1 else 0, b if j > 1 else 0, c if k > 1 else 0
+
+
 def kv_cache_bytes(qtype: int, heads: int, d: int, page_size: int, n_pages: int) -> int:
     """Bytes of a quantised key / value cache (s3b_kv_cache_bytes)."""
     n = int(lib().s3b_kv_cache_bytes(qtype, heads, d, page_size, n_pages))
@@ -213,6 +236,7 @@ class KVCache:
         self.data = data
         self.qtype, self.n_pages, self.page_size, self.heads, self.d = qtype, n_pages, page_size, heads, d
         self.desc = KVCacheDesc(qtype, heads, d, page_size, n_pages, data.data_ptr())
+        self.ref = ctypes.byref(self.desc)
 
     @property
     def n_slots(self) -> int:
@@ -674,68 +698,63 @@ class Engine:
         self._check(rc, "s3b_op_dequantize")
 
     # -- quantised key / value cache
-    def _cache_rows(self, what: str, cache: KVCache, n: int, **rows):
-        """dtype code of the row tensors [n, heads, d] after the checks that raw pointers cannot carry."""
-        dtypes = {str(t.dtype) for t in rows.values()}
-        if len(dtypes) != 1 or not dtypes <= {"torch.float16", "torch.float32"}:
-            raise S3BError(f"{what}: rows must be all f16 or all f32, got {sorted(dtypes)}")
-        for name, t in rows.items():
-            if tuple(t.shape) != (n, cache.heads, cache.d) or (t.numel() and t.stride(2) != 1):
-                raise S3BError(f"{what}: {name} must be [{n}, {cache.heads}, {cache.d}] with contiguous rows")
-        return S3B_F16 if dtypes == {"torch.float16"} else S3B_F32
-
     @staticmethod
-    def _strides(t, n: int):
-        """The first n strides of t, 0 for a dimension of one (whose stride means nothing)."""
-        return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(n)]
-
-    @staticmethod
-    def _index(what: str, name: str, t, dtype: str, shape=None):
-        if str(t.dtype) != dtype or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
-            raise S3BError(f"{what}: {name} must be contiguous {dtype}" + (f" {list(shape)}" if shape else ""))
+    def _cache_rows(what: str, cache: KVCache, n: int, name: str, t, dtype: int | None) -> int:
+        """dtype code of the row tensor t [n, heads, d] (that of its partner, if given) after the checks that a raw pointer
+        cannot carry."""
+        size = t.dtype.itemsize
+        if not t.dtype.is_floating_point or size not in (2, 4) or "bfloat16" in str(t.dtype) or \
+                (dtype is not None and dtype != (S3B_F16 if size == 2 else S3B_F32)):
+            raise S3BError(f"{what}: rows must be all f16 or all f32, {name} is {t.dtype}")
+        if t.shape != (n, cache.heads, cache.d) or (t.stride(2) != 1 and n):
+            raise S3BError(f"{what}: {name} must be [{n}, {cache.heads}, {cache.d}] with contiguous rows")
+        return S3B_F16 if size == 2 else S3B_F32
 
     def cache_write(self, cache: KVCache, k, v, slots):
         """Quantises the tokens k, v [n, heads, d] (f16 or f32 CUDA tensors, rows contiguous) into the slots int64 [n]
         (< 0: skipped)."""
-        n = int(slots.shape[0])
-        self._index("cache_write", "slots", slots, "torch.int64", (n,))
-        dtype = self._cache_rows("cache_write", cache, n, k=k, v=v)
-        rc = self._L.s3b_op_cache_write(self.h, ctypes.byref(cache.desc), k.data_ptr(), *self._strides(k, 2),
-                                        v.data_ptr(), *self._strides(v, 2), dtype, slots.data_ptr(), n)
-        self._check(rc, "s3b_op_cache_write")
+        n = _index("cache_write", "slots", slots, 8, 1)
+        dtype = self._cache_rows("cache_write", cache, n, "k", k, None)
+        self._cache_rows("cache_write", cache, n, "v", v, dtype)
+        rc = self._L.s3b_op_cache_write(self.h, cache.ref, k.data_ptr(), *_strides2(k), v.data_ptr(), *_strides2(v),
+                                        dtype, slots.data_ptr(), n)
+        if rc:
+            self._check(rc, "s3b_op_cache_write")
 
     def cache_read(self, cache: KVCache, slots, k_out, v_out):
         """Reads the tokens of the slots int64 [n] (< 0: zeros) into k_out, v_out [n, heads, d] (f16 or f32; one of them
         may be None)."""
-        n = int(slots.shape[0])
-        self._index("cache_read", "slots", slots, "torch.int64", (n,))
-        rows = {m: t for m, t in (("k_out", k_out), ("v_out", v_out)) if t is not None}
-        dtype = self._cache_rows("cache_read", cache, n, **rows) if rows else S3B_F16
-        ks, vs = (self._strides(t, 2) if t is not None else (0, 0) for t in (k_out, v_out))
-        rc = self._L.s3b_op_cache_read(self.h, ctypes.byref(cache.desc), slots.data_ptr(), n, _ptr(k_out), *ks,
-                                       _ptr(v_out), *vs, dtype)
-        self._check(rc, "s3b_op_cache_read")
+        n = _index("cache_read", "slots", slots, 8, 1)
+        dtype = None
+        for name, t in (("k_out", k_out), ("v_out", v_out)):
+            if t is not None:
+                dtype = self._cache_rows("cache_read", cache, n, name, t, dtype)
+        rc = self._L.s3b_op_cache_read(self.h, cache.ref, slots.data_ptr(), n, _ptr(k_out), *_strides2(k_out),
+                                       _ptr(v_out), *_strides2(v_out), S3B_F16 if dtype is None else dtype)
+        if rc:
+            self._check(rc, "s3b_op_cache_read")
 
     def cache_attention(self, cache: KVCache, q, out, pages, lengths, scale: float, causal: bool = False,
                         window: int = 0, lse=None):
         """out = softmax(scale q K^T) V over the cache (s3b_op_cache_attention): q f16 [batch, nq, heads, d], out the same
         shape in f16 or f32, pages int32 [batch, max_pages], lengths int32 [batch], lse f32 [batch, nq, heads] or None."""
-        b, nq, heads, d = q.shape
         what = "cache_attention"
-        if str(q.dtype) != "torch.float16" or d != cache.d or (q.numel() and q.stride(3) != 1):
+        b, nq, heads, d = shape = q.shape
+        q_type, o_type = q.dtype, out.dtype
+        if not q_type.is_floating_point or q_type.itemsize != 2 or "bfloat16" in str(q_type) or d != cache.d or \
+                (q.stride(3) != 1 and q.numel()):
             raise S3BError(f"{what}: q must be f16 [batch, nq, heads, {cache.d}] with contiguous rows")
-        if out.shape != q.shape or str(out.dtype) not in ("torch.float16", "torch.float32") or \
-                (out.numel() and out.stride(3) != 1):
+        if out.shape != shape or (o_type is not q_type and (o_type.itemsize != 4 or not o_type.is_floating_point)) or \
+                (out.stride(3) != 1 and out.numel()):
             raise S3BError(f"{what}: out must have q's shape, in f16 or f32, with contiguous rows")
-        if pages.dim() != 2 or int(pages.shape[0]) != b or str(pages.dtype) != "torch.int32" or \
-                (pages.numel() and pages.stride(1) != 1):
-            raise S3BError(f"{what}: pages must be int32 [{b}, max_pages] with contiguous rows")
-        self._index(what, "lengths", lengths, "torch.int32", (b,))
-        if lse is not None:
-            self._index(what, "lse", lse, "torch.float32", (b, nq, heads))
-        rc = self._L.s3b_op_cache_attention(self.h, ctypes.byref(cache.desc), q.data_ptr(), *self._strides(q, 3),
-                                            out.data_ptr(), 1 if out.dtype.itemsize == 4 else 0,
-                                            *self._strides(out, 3), _ptr(lse), pages.data_ptr(),
-                                            pages.stride(0), int(pages.shape[1]), lengths.data_ptr(), b, nq, heads,
-                                            float(scale), 1 if causal else 0, int(window))
-        self._check(rc, "s3b_op_cache_attention")
+        if _index(what, "lengths", lengths, 4, 1) != b or _index(what, "pages", pages, 4, 2) != b:
+            raise S3BError(f"{what}: pages must be int32 [{b}, max_pages] with contiguous rows, lengths int32 [{b}]")
+        if lse is not None and (lse.shape != (b, nq, heads) or lse.dtype.itemsize != 4 or
+                                not lse.dtype.is_floating_point or not lse.is_contiguous()):
+            raise S3BError(f"{what}: lse must be contiguous f32 [{b}, {nq}, {heads}]")
+        rc = self._L.s3b_op_cache_attention(self.h, cache.ref, q.data_ptr(), *_strides3(q), out.data_ptr(),
+                                            0 if o_type is q_type else 1, *_strides3(out), _ptr(lse), pages.data_ptr(),
+                                            pages.stride(0), pages.shape[1], lengths.data_ptr(), b, nq, heads, scale,
+                                            1 if causal else 0, window)
+        if rc:
+            self._check(rc, "s3b_op_cache_attention")

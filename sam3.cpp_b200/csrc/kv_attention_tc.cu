@@ -1075,8 +1075,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArg
     store_out(p, at + 32 * e, make_float4(v[e].x * inv, v[e].y * inv, v[e].z * inv, v[e].w * inv));
 }
 
-// The f16 operands of tiles_kernel, once for all its CTAs: block (x < kv_blocks) the K and V items of one token tile of one
-// sequence and head, a warp for each 16 tokens; the blocks after them the Q rows of one tile. Bound by HBM and L2: the
+// The f16 operands of tiles_kernel, once for all its CTAs: block (x < kv_blocks) the K or the V item of one token tile of
+// one sequence and head, a warp for each 16 tokens; the blocks after them the Q rows of one tile. Bound by HBM and L2: the
 // cache read once, 4 bytes written per value pair of K and V.
 template <int QT, int D>
 __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ TcArgs a, int kv_blocks, int* err) {
@@ -1100,7 +1100,7 @@ __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ TcAr
     }
     return;
   }
-  const int j = blockIdx.x % a.tiles, unit = blockIdx.x / a.tiles;
+  const int kv = blockIdx.x & 1, x = blockIdx.x >> 1, j = x % a.tiles, unit = x / a.tiles;
   const int head = unit % p.c.heads, b = unit / p.c.heads;
   const int len = sequence_length(p, b, err);
   int lo, hi, none;
@@ -1117,17 +1117,20 @@ __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ TcAr
     atomicCAS(err, 0, kDevErrIndex);
     page = 0;
   }
-  const uint8_t* k = p.c.data + kv_group_offset<QT, D>(p.c, page, head, 0, gi % per_page);
-  const uint8_t* v = k + (long long)per_page * L::kHalf;
-  uint8_t* item = a.image + (long long)blockIdx.x * (D * 512);
-  const int mine = first + 2 * (lane & 3);
-  auto in = [&](int tok) -> bool { return tok >= lo && tok < hi; };
-  const uint32_t keep0 = (in(mine) ? 0xFFFFu : 0u) | (in(mine + 1) ? 0xFFFF0000u : 0u);
-  const uint32_t keep1 = (in(mine + 8) ? 0xFFFFu : 0u) | (in(mine + 9) ? 0xFFFF0000u : 0u);
+  const uint8_t* from = p.c.data + kv_group_offset<QT, D>(p.c, page, head, kv, gi % per_page);
+  uint8_t* item = a.image + (long long)blockIdx.x * (D * 256);
+  if (kv == 0) {
 #pragma unroll
-  for (int sb = 0; sb < D / L::kSB; ++sb) {
-    emit_k<QT, D>(k, item + sb * (L::kSB / 64) * kSlotBytes, warp, sb, lane);
-    emit_v<QT, D>(v, keep0, keep1, item + D * 256 + (warp >> 2) * (D * 128), warp, sb, lane);
+    for (int sb = 0; sb < D / L::kSB; ++sb)
+      emit_k<QT, D>(from, item + sb * (L::kSB / 64) * kSlotBytes, warp, sb, lane);
+  } else {
+    const int mine = first + 2 * (lane & 3);
+    auto in = [&](int tok) -> bool { return tok >= lo && tok < hi; };
+    const uint32_t keep0 = (in(mine) ? 0xFFFFu : 0u) | (in(mine + 1) ? 0xFFFF0000u : 0u);
+    const uint32_t keep1 = (in(mine + 8) ? 0xFFFFu : 0u) | (in(mine + 9) ? 0xFFFF0000u : 0u);
+#pragma unroll
+    for (int sb = 0; sb < D / L::kSB; ++sb)
+      emit_v<QT, D>(from, keep0, keep1, item + (warp >> 2) * (D * 128), warp, sb, lane);
   }
 }
 
@@ -1188,7 +1191,7 @@ int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStrea
     typedef Tc<QT_Q4_0, D, true> C;  // the staged kernel does not depend on the cache's type
     auto* k = tiles_kernel<QT_Q4_0, D, true>;
     if (kernel_setup(k, C::kSmem) <= 0) return -13;
-    const long long kv_blocks = (long long)p.batch * p.c.heads * t.tiles;
+    const long long kv_blocks = 2LL * p.batch * p.c.heads * t.tiles;
     const long long q_blocks = (long long)p.batch * p.c.heads * t.blocks * TQ;
     stage_kernel<QT, D><<<(unsigned)(kv_blocks + q_blocks), 256, 0, st>>>(a, (int)kv_blocks, err);
     if (cudaGetLastError() != cudaSuccess) return -12;
