@@ -13,26 +13,33 @@ struct Job {
   const long long* slots;
   long long n;
   int* err;
-  int vec;            // tokens that a block takes
+  int tokens;         // that a block takes
   unsigned div_mul;   // slot / page_size = (slot * div_mul) >> (32 + div_shift) for slots below 2^31; 0: 64-bit division
   int div_shift;
+  long long page_bytes, v_bytes;  // of a page; from a page's keys of a head to its values
 };
 
-// Page and position of a slot; false for a slot that is skipped.
-__device__ __forceinline__ bool slot_place(const Job& j, long long slot, long long* page, int* pos) {
+// Byte offset of the keys of a slot's group for head 0, and the token's place in the group; false for a slot that is
+// skipped.
+template <int HALF>
+__device__ __forceinline__ bool slot_place(const Job& j, long long slot, long long* at, int* tok) {
   if (slot < 0) return false;
   if (slot >= j.c.n_pages * j.c.page_size) {
     atomicCAS(j.err, 0, kDevErrIndex);
     return false;
   }
+  int pos;
   if (j.div_mul) {
     const unsigned s = (unsigned)slot, q = __umulhi(s, j.div_mul) >> j.div_shift;
-    *page = q;
-    *pos = (int)(s - q * j.c.page_size);
+    *at = q * j.page_bytes;
+    pos = (int)(s - q * j.c.page_size);
   } else {
-    *page = slot / j.c.page_size;
-    *pos = (int)(slot - *page * j.c.page_size);
+    const long long q = slot / j.c.page_size;
+    *at = q * j.page_bytes;
+    pos = (int)(slot - q * j.c.page_size);
   }
+  *at += (pos >> 4) * HALF;
+  *tok = pos & 15;
   return true;
 }
 
@@ -46,7 +53,7 @@ __device__ __forceinline__ void load8(const __half* at, float (&x)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+    const float2 f = __half22float2(u32_h2(w[e]));
     x[2 * e] = f.x, x[2 * e + 1] = f.y;
   }
 }
@@ -61,184 +68,223 @@ __device__ __forceinline__ void store8(__half* at, const float (&x)[8]) {
   *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(h);
 }
 
-// Quantises the block of 32 values that four neighbouring lanes hold, 8 each (t: which 8), in the steps of
-// quantize_row_host, each rounded to f32 as there. Truncation of a value >= 0 is an addition of 2^23 rounded to zero.
-template <int QT>
-__device__ __forceinline__ void quantise8(float (&x)[8], int t, uint32_t (&code)[8], __half& scale, __half& low) {
+__device__ __forceinline__ float max3n(float a, float b, float c) {  // a NaN among them stays
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float min3n(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// largest and smallest value of the block that four neighbouring lanes hold
+__device__ __forceinline__ void block_range(const float (&x)[8], float* hi, float* lo) {
+  *hi = max3n(max3n(x[0], x[1], x[2]), max3n(x[3], x[4], x[5]), max3n(x[6], x[7], x[7]));
+  *lo = min3n(min3n(x[0], x[1], x[2]), min3n(x[3], x[4], x[5]), min3n(x[6], x[7], x[7]));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = x[e] == x[e] ? fminf(fmaxf(x[e], -kLimit), kLimit) : 0.f;
-  low = __ushort_as_half(0);
-  auto whole = [](float f) -> uint32_t { return __float_as_uint(__fadd_rz(f, 8388608.f)) & 0x7FFFFFu; };
-  if (QT == QT_Q4_1) {
-    float lo = x[0], hi = x[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]);
-#pragma unroll
-    for (int s = 1; s < 4; s <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(~0u, lo, s));
-      hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, s));
-    }
-    const float d = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
-    const float id = d != 0.f ? __fdiv_rn(1.0f, d) : 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      code[e] = min(15u, whole(fmaxf(__fadd_rn(__fmul_rn(__fsub_rn(x[e], lo), id), 0.5f), 0.f)));
-    scale = __float2half_rn(d);
-    low = __float2half_rn(lo);
-  } else {
-    // the first value of largest magnitude
-    float amax = fabsf(x[0]), vmax = x[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e)
-      if (fabsf(x[e]) > amax) amax = fabsf(x[e]), vmax = x[e];
-#pragma unroll
-    for (int s = 1; s < 4; s <<= 1) {
-      const float v = __shfl_xor_sync(~0u, vmax, s);
-      if (fabsf(v) > amax || (fabsf(v) == amax && (t & s))) amax = fabsf(v), vmax = v;
-    }
-    const float d = QT == QT_Q4_0 ? vmax * -0.125f : __fdiv_rn(amax, 127.0f);
-    const float id = d != 0.f ? __fdiv_rn(1.0f, d) : 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float y = __fmul_rn(x[e], id);
-      if (QT == QT_Q4_0) {
-        code[e] = min(15u, whole(fmaxf(__fadd_rn(y, 8.5f), 0.f)));
-      } else {
-        const int q = (int)min(127u, whole(__fadd_rz(fabsf(y), 0.5f)));  // halves away from zero
-        code[e] = (uint32_t)((y < 0.f ? -q : q) + 128);
-      }
-    }
-    scale = __float2half_rn(d);
+  for (int s = 1; s < 4; s <<= 1) {
+    const float h = __shfl_xor_sync(~0u, *hi, s), l = __shfl_xor_sync(~0u, *lo, s);
+    *hi = max3n(*hi, h, h);
+    *lo = min3n(*lo, l, l);
   }
 }
 
+constexpr uint32_t kWhole = 0x4B000000u;  // 2^23 as f32
+
+// Quantises the block of 32 values that four neighbouring lanes hold, 8 each (t: which 8), in the steps of
+// quantize_row_host, each rounded to f32 as there. The codes come out as kWhole + code (q8_0: code + 128): truncation of
+// a value >= 0 is the addition of 2^23 rounded to zero.
+template <int QT>
+__device__ __forceinline__ void quantise8(float (&x)[8], int t, uint32_t (&code)[8], __half& scale, __half& low) {
+  float hi, lo;
+  block_range(x, &hi, &lo);
+  if (__any_sync(~0u, !(hi <= kLimit && lo >= -kLimit))) {  // what is not finite or beyond the limit, rare
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = x[e] == x[e] ? fminf(fmaxf(x[e], -kLimit), kLimit) : 0.f;
+    block_range(x, &hi, &lo);
+  }
+  low = __ushort_as_half(0);
+  float d;
+  if (QT == QT_Q4_1) {
+    d = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
+    low = __float2half_rn(lo);
+  } else if (QT == QT_Q8_0) {
+    d = __fdiv_rn(fmaxf(hi, -lo), 127.0f);
+  } else {
+    float v = hi > -lo ? hi : lo;
+    if (__any_sync(~0u, hi == -lo && hi != 0.f)) {  // the first of the two
+      int first = 32;
+#pragma unroll
+      for (int e = 7; e >= 0; --e)
+        if (fabsf(x[e]) == hi) first = 8 * t + e;
+      float mine = lo;
+#pragma unroll
+      for (int e = 7; e >= 0; --e)
+        if (fabsf(x[e]) == hi) mine = x[e];
+#pragma unroll
+      for (int s = 1; s < 4; s <<= 1) {
+        const int f = __shfl_xor_sync(~0u, first, s);
+        const float m = __shfl_xor_sync(~0u, mine, s);
+        if (f < first) first = f, mine = m;
+      }
+      if (hi == -lo) v = mine;
+    }
+    d = v * -0.125f;
+  }
+  const float id = d != 0.f ? __fdiv_rn(1.0f, d) : 0.f;
+  scale = __float2half_rn(d);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (QT == QT_Q8_0) {
+      const float y = __fmul_rn(x[e], id);
+      const uint32_t q = min(__float_as_uint(__fadd_rz(__fadd_rz(fabsf(y), 0.5f), 8388608.f)), kWhole + 127u);
+      code[e] = y < 0.f ? 2u * kWhole + 128u - q : q + 128u;  // halves away from zero
+    } else {
+      const float y = QT == QT_Q4_0 ? __fadd_rn(__fmul_rn(x[e], id), 8.5f)
+                                    : __fadd_rn(__fmul_rn(__fsub_rn(x[e], lo), id), 0.5f);
+      code[e] = min(__float_as_uint(__fadd_rz(y, 8388608.f)), kWhole + 15u);
+    }
+  }
+}
+
+// sum of code[i] << shift(i) of n codes less what their kWhole adds (all in 32 bits)
+template <int N, int S0, int S1>
+__device__ __forceinline__ uint32_t pack_codes(const uint32_t* code) {
+  uint32_t w = 0, off = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const int shift = (e >> 1) * S0 + (e & 1) * S1;
+    w += code[e] << shift;
+    off += kWhole << shift;
+  }
+  return w - off;
+}
+
 // Four lanes a block of 32 values, 8 each: rows are read in 16-byte pieces, and the 8 values of a lane are a whole word of
-// the keys' layout (4-bit codes; two words of 8-bit ones) and two pieces of the values'. Bound by HBM: a block of threads
-// reads its K and V rows of a few tokens before it quantises any of them, so that enough loads are in flight.
+// the keys' layout (4-bit codes; two words of 8-bit ones) and two pieces of the values'. K and V rows of two tokens are
+// read before any is quantised. Bound by instruction issue (about 14 a value) and HBM alike.
 template <int QT, int D, typename T>
 __global__ void __launch_bounds__(256) write_kernel(const __grid_constant__ Job j) {
   typedef KvL<QT, D> L;
   constexpr int kLanes = D / 8, kRows = 256 / kLanes;  // lanes of a row, rows of a pass
   const int head = blockIdx.x % j.c.heads;
-  const long long first = (long long)(blockIdx.x / j.c.heads) * j.vec;
+  const long long first = (long long)(blockIdx.x / j.c.heads) * j.tokens + threadIdx.x / kLanes;
   const int c8 = threadIdx.x % kLanes, t = c8 & 3, b = c8 >> 2;
-  for (int r0 = 0; r0 < j.vec; r0 += 2 * kRows) {
-    float x[2][2][8];
-    long long page[2];
-    int pos[2];
-    bool use[2];
+  uint8_t* base = j.c.data + head * 2 * j.v_bytes;
+  float x[2][2][8];
+  long long at[2];
+  int tok[2];
+  bool use[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const long long i = first + r0 + u * kRows + threadIdx.x / kLanes;
-      use[u] = r0 + u * kRows + threadIdx.x / kLanes < j.vec && i < j.n && slot_place(j, __ldg(j.slots + i), &page[u], &pos[u]);
-      if (use[u]) {
-        load8(reinterpret_cast<const T*>(j.r.k) + i * j.r.k_n + head * j.r.k_h + c8 * 8, x[u][0]);
-        load8(reinterpret_cast<const T*>(j.r.v) + i * j.r.v_n + head * j.r.v_h + c8 * 8, x[u][1]);
-      }
+  for (int u = 0; u < 2; ++u) {
+    const long long i = first + u * kRows;
+    use[u] = i < j.n && slot_place<L::kHalf>(j, __ldg(j.slots + i), &at[u], &tok[u]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[u][0][e] = x[u][1][e] = 0.f;
+    if (use[u]) {
+      load8(reinterpret_cast<const T*>(j.r.k) + i * j.r.k_n + head * j.r.k_h + c8 * 8, x[u][0]);
+      load8(reinterpret_cast<const T*>(j.r.v) + i * j.r.v_n + head * j.r.v_h + c8 * 8, x[u][1]);
     }
+  }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      uint32_t kc[8], vc[8];
-      __half ks, kl, vs, vl;
-      if (!use[u]) {
+  for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[u][0][e] = x[u][1][e] = 0.f;
-      }
-      quantise8<QT>(x[u][0], t, kc, ks, kl);
-      quantise8<QT>(x[u][1], t, vc, vs, vl);
+    for (int kv = 0; kv < 2; ++kv) {
+      uint32_t c[8];
+      __half scale, low;
+      quantise8<QT>(x[u][kv], t, c, scale, low);
       if (!use[u]) continue;
-      const int tok = pos[u] & 15;
-      uint8_t* kp = j.c.data + kv_group_offset<QT, D>(j.c, page[u], head, 0, pos[u] >> 4);
-      uint8_t* vp = j.c.data + kv_group_offset<QT, D>(j.c, page[u], head, 1, pos[u] >> 4);
+      uint8_t* gp = base + at[u] + kv * j.v_bytes;
       if (L::kBits == 8) {
-        *reinterpret_cast<uint2*>(kp + L::k_val(tok, b, t)) =
-            make_uint2(kc[0] | kc[1] << 8 | kc[2] << 16 | kc[3] << 24, kc[4] | kc[5] << 8 | kc[6] << 16 | kc[7] << 24);
-        *reinterpret_cast<uint32_t*>(vp + L::v_val(tok, b, 2 * t)) = vc[0] | vc[1] << 8 | vc[2] << 16 | vc[3] << 24;
-        *reinterpret_cast<uint32_t*>(vp + L::v_val(tok, b, 2 * t + 1)) = vc[4] | vc[5] << 8 | vc[6] << 16 | vc[7] << 24;
+        const uint32_t w0 = pack_codes<4, 16, 8>(c), w1 = pack_codes<4, 16, 8>(c + 4);
+        if (kv == 0) {
+          *reinterpret_cast<uint2*>(gp + L::k_val(tok[u], b, t)) = make_uint2(w0, w1);
+        } else {
+          *reinterpret_cast<uint32_t*>(gp + L::v_val(tok[u], b, 2 * t)) = w0;
+          *reinterpret_cast<uint32_t*>(gp + L::v_val(tok[u], b, 2 * t + 1)) = w1;
+        }
+      } else if (kv == 0) {
+        *reinterpret_cast<uint32_t*>(gp + L::k_val(tok[u], b, t)) = pack_codes<8, 4, 16>(c);
       } else {
-        *reinterpret_cast<uint32_t*>(kp + L::k_val(tok, b, t)) = kc[0] | kc[2] << 4 | kc[4] << 8 | kc[6] << 12 |
-                                                                 kc[1] << 16 | kc[3] << 20 | kc[5] << 24 | kc[7] << 28;
-        *reinterpret_cast<uint16_t*>(vp + L::v_val(tok, b, 2 * t)) =
-            (uint16_t)(vc[0] | vc[1] << 4 | vc[2] << 8 | vc[3] << 12);
-        *reinterpret_cast<uint16_t*>(vp + L::v_val(tok, b, 2 * t + 1)) =
-            (uint16_t)(vc[4] | vc[5] << 4 | vc[6] << 8 | vc[7] << 12);
+        const uint32_t w = pack_codes<8, 8, 4>(c);
+        *reinterpret_cast<uint16_t*>(gp + L::v_val(tok[u], b, 2 * t)) = (uint16_t)w;
+        *reinterpret_cast<uint16_t*>(gp + L::v_val(tok[u], b, 2 * t + 1)) = (uint16_t)(w >> 16);
       }
       if (t == 0) {
-        __half* sp = reinterpret_cast<__half*>(kp + L::k_scale(tok, b));
-        sp[0] = ks;
-        if (QT == QT_Q4_1) sp[L::kSc / 2] = kl;
-      } else if (t == 1) {
-        __half* sp = reinterpret_cast<__half*>(vp + L::v_scale(tok, b));
-        sp[0] = vs;
-        if (QT == QT_Q4_1) sp[L::kSc / 2] = vl;
+        __half* sp = reinterpret_cast<__half*>(gp + (kv ? L::v_scale(tok[u], b) : L::k_scale(tok[u], b)));
+        sp[0] = scale;
+        if (QT == QT_Q4_1) sp[L::kSc / 2] = low;
       }
     }
   }
 }
 
-// The reverse, in the same shape: 8 values of a row a lane.
+// The reverse, in the same shape: 8 values of a row a lane, K and V of two tokens read before any is unpacked.
 template <int QT, int D, typename T>
 __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Job j) {
   typedef KvL<QT, D> L;
   constexpr int kLanes = D / 8, kRows = 256 / kLanes;
   const int head = blockIdx.x % j.c.heads;
-  const long long first = (long long)(blockIdx.x / j.c.heads) * j.vec;
+  const long long first = (long long)(blockIdx.x / j.c.heads) * j.tokens + threadIdx.x / kLanes;
   const int c8 = threadIdx.x % kLanes, t = c8 & 3, b = c8 >> 2;
-  for (int r0 = 0; r0 < j.vec; r0 += 2 * kRows) {
-    uint32_t w[2][2][2];
-    __half sc[2][2], low[2][2];
-    long long i[2];
+  const uint8_t* base = j.c.data + head * 2 * j.v_bytes;
+  uint32_t w[2][2][2];
+  __half sc[2][2], low[2][2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      i[u] = first + r0 + u * kRows + threadIdx.x / kLanes;
-      if (r0 + u * kRows + threadIdx.x / kLanes >= j.vec) i[u] = j.n;
-      long long page;
-      int pos;
+  for (int u = 0; u < 2; ++u) {
+    const long long i = first + u * kRows;
+    long long at;
+    int tok;
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        w[u][kv][0] = w[u][kv][1] = L::kBits == 8 ? 0x80808080u : QT == QT_Q4_0 ? 0x88888888u : 0u;
-        sc[u][kv] = low[u][kv] = __ushort_as_half(0);
-      }
-      if (i[u] < j.n && slot_place(j, __ldg(j.slots + i[u]), &page, &pos)) {
-        const int tok = pos & 15;
-        const uint8_t* kp = j.c.data + kv_group_offset<QT, D>(j.c, page, head, 0, pos >> 4);
-        const uint8_t* vp = j.c.data + kv_group_offset<QT, D>(j.c, page, head, 1, pos >> 4);
-        if (L::kBits == 8) {
-          const uint2 k = __ldg(reinterpret_cast<const uint2*>(kp + L::k_val(tok, b, t)));
-          w[u][0][0] = k.x, w[u][0][1] = k.y;
-          w[u][1][0] = __ldg(reinterpret_cast<const uint32_t*>(vp + L::v_val(tok, b, 2 * t)));
-          w[u][1][1] = __ldg(reinterpret_cast<const uint32_t*>(vp + L::v_val(tok, b, 2 * t + 1)));
-        } else {
-          w[u][0][0] = __ldg(reinterpret_cast<const uint32_t*>(kp + L::k_val(tok, b, t)));
-          w[u][1][0] = (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(vp + L::v_val(tok, b, 2 * t))) |
-                       (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(vp + L::v_val(tok, b, 2 * t + 1))) << 16;
-        }
-        const __half* ks = reinterpret_cast<const __half*>(kp + L::k_scale(tok, b));
-        const __half* vs = reinterpret_cast<const __half*>(vp + L::v_scale(tok, b));
-        sc[u][0] = __ldg(ks), sc[u][1] = __ldg(vs);
-        if (QT == QT_Q4_1) low[u][0] = __ldg(ks + L::kSc / 2), low[u][1] = __ldg(vs + L::kSc / 2);
-      }
+    for (int kv = 0; kv < 2; ++kv) {  // of a skipped slot: zeros
+      w[u][kv][0] = w[u][kv][1] = L::kBits == 8 ? 0x80808080u : 0x88888888u;
+      sc[u][kv] = low[u][kv] = __ushort_as_half(0);
     }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (i[u] >= j.n) continue;
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        T* out = reinterpret_cast<T*>(kv ? j.r.v : j.r.k);
-        if (!out) continue;
-        const float s = __half2float(sc[u][kv]), m = __half2float(low[u][kv]);
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          int code;
-          if (L::kBits == 8)
-            code = (int)(w[u][kv][e >> 2] >> (8 * (e & 3)) & 255u) - 128;
-          else
-            code = (int)(w[u][kv][0] >> (kv ? 4 * e : 4 * (e >> 1) + 16 * (e & 1)) & 15u) - (QT == QT_Q4_0 ? 8 : 0);
-          x[e] = __fadd_rn(__fmul_rn((float)code, s), m);
-        }
-        store8(out + i[u] * (kv ? j.r.v_n : j.r.k_n) + head * (kv ? j.r.v_h : j.r.k_h) + c8 * 8, x);
+    if (i < j.n && slot_place<L::kHalf>(j, __ldg(j.slots + i), &at, &tok)) {
+      const uint8_t *kp = base + at, *vp = kp + j.v_bytes;
+      if (L::kBits == 8) {
+        const uint2 k = __ldg(reinterpret_cast<const uint2*>(kp + L::k_val(tok, b, t)));
+        w[u][0][0] = k.x, w[u][0][1] = k.y;
+        w[u][1][0] = __ldg(reinterpret_cast<const uint32_t*>(vp + L::v_val(tok, b, 2 * t)));
+        w[u][1][1] = __ldg(reinterpret_cast<const uint32_t*>(vp + L::v_val(tok, b, 2 * t + 1)));
+      } else {
+        w[u][0][0] = __ldg(reinterpret_cast<const uint32_t*>(kp + L::k_val(tok, b, t)));
+        w[u][1][0] = __byte_perm(__ldg(reinterpret_cast<const uint16_t*>(vp + L::v_val(tok, b, 2 * t))),
+                                 __ldg(reinterpret_cast<const uint16_t*>(vp + L::v_val(tok, b, 2 * t + 1))), 0x5410);
       }
+      const __half* ks = reinterpret_cast<const __half*>(kp + L::k_scale(tok, b));
+      const __half* vs = reinterpret_cast<const __half*>(vp + L::v_scale(tok, b));
+      sc[u][0] = __ldg(ks), sc[u][1] = __ldg(vs);
+      if (QT == QT_Q4_1) low[u][0] = __ldg(ks + L::kSc / 2), low[u][1] = __ldg(vs + L::kSc / 2);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const long long i = first + u * kRows;
+    if (i >= j.n) continue;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      T* out = reinterpret_cast<T*>(kv ? j.r.v : j.r.k);
+      if (!out) continue;
+      // codes as exact f16 pairs, then one f32 multiply-add: the product is exact, so one rounding (and one to f16)
+      uint32_t p[4];
+      if (L::kBits == 8) {
+        byte_pairs(w[u][kv][0], p[0], p[1]);
+        byte_pairs(w[u][kv][1], p[2], p[3]);
+      } else {
+        nibble_pairs<QT>(w[u][kv][0], p);
+      }
+      const float s = __half2float(sc[u][kv]), m = __half2float(low[u][kv]);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = __half22float2(u32_h2(p[e]));
+        const bool apart = L::kBits == 4 && kv;  // a value word pairs values e and e + 4
+        x[apart ? e : 2 * e] = fmaf(f.x, s, m);
+        x[apart ? e + 4 : 2 * e + 1] = fmaf(f.y, s, m);
+      }
+      store8(out + i * (kv ? j.r.v_n : j.r.k_n) + head * (kv ? j.r.v_h : j.r.k_h) + c8 * 8, x);
     }
   }
 }
@@ -258,13 +304,14 @@ JobKernel job_kernel_d(int d, bool write, bool f32) {
 
 int launch(bool write, const KvCache& c, const KvRows& r, const long long* slots, long long n, int* err,
            cudaStream_t st) {
-  Job j{c, r, slots, n, err, 2 * 256 / (c.d / 8), 0, 0};  // two passes of rows a block
+  const long long region = kv_cache_bytes(c) / c.n_pages / c.heads;  // of one page and head
+  Job j{c, r, slots, n, err, 2 * 256 / (c.d / 8), 0, 0, region * c.heads, region / 2};
   if (c.n_pages * c.page_size < (1LL << 31) && c.page_size > 1) {
     // shift = ceil(log2(page_size)) - 1, mul = ceil(2^(32 + shift) / page_size) < 2^32: exact for slots below 2^31
     while ((2LL << j.div_shift) < c.page_size) ++j.div_shift;
     j.div_mul = (unsigned)(((1ULL << (32 + j.div_shift)) + c.page_size - 1) / c.page_size);
   }
-  const long long blocks = (n + j.vec - 1) / j.vec * c.heads;
+  const long long blocks = (n + j.tokens - 1) / j.tokens * c.heads;
   if (blocks > 0x7fffffffLL) return -2;
   const JobKernel k = c.type == QT_Q4_0 ? job_kernel_d<QT_Q4_0>(c.d, write, r.f32)
                       : c.type == QT_Q4_1 ? job_kernel_d<QT_Q4_1>(c.d, write, r.f32)

@@ -54,4 +54,37 @@ __device__ __forceinline__ long long kv_group_offset(const KvCache& c, long long
 // The 8 nibbles of a key word: value 2p in nibble p, value 2p + 1 in nibble p + 4. The 4 nibbles of a value half-word
 // stand in order. 8-bit codes are stored with 128 added, in order.
 
+// ---------------------------------------------------------------- codes
+__device__ __forceinline__ uint32_t h2_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 u32_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+// (w & MASK) | 0x64006400 in one instruction
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t under_1024(uint32_t w) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "n"(MASK), "r"(0x64006400u));
+  return r;
+}
+
+// Exact f16 pairs of the codes (less 8 for q4_0) whose nibbles lie at bits 0, 4, 8, 12 of each half of w: a nibble under
+// the exponent of 1024 reads 1024 + c at bit 0 and 1024 + 16 c at bit 4; one subtraction (or multiply-add by 1/16)
+// leaves the integer.
+template <int QT>
+__device__ __forceinline__ void nibble_pairs(uint32_t w, uint32_t (&out)[4]) {
+  const __half2 off0 = u32_h2(QT == QT_Q4_0 ? 0xE408E408u : 0xE400E400u);  // -1032, -1024
+  const __half2 off1 = u32_h2(QT == QT_Q4_0 ? 0xD480D480u : 0xD400D400u);  // -72, -64
+  const __half2 sixteenth = u32_h2(0x2C002C00u);
+  const uint32_t x = w >> 8;
+  out[0] = h2_u32(__hadd2(u32_h2(under_1024<0x000F000Fu>(w)), off0));
+  out[1] = h2_u32(__hfma2(u32_h2(under_1024<0x00F000F0u>(w)), sixteenth, off1));
+  out[2] = h2_u32(__hadd2(u32_h2(under_1024<0x000F000Fu>(x)), off0));
+  out[3] = h2_u32(__hfma2(u32_h2(under_1024<0x00F000F0u>(x)), sixteenth, off1));
+}
+// The same for the bytes 0, 1 and 2, 3 of w (8-bit codes with 128 added).
+__device__ __forceinline__ void byte_pairs(uint32_t w, uint32_t& a, uint32_t& b) {
+  const __half2 off = u32_h2(0xE480E480u);  // -1152
+  a = h2_u32(__hadd2(u32_h2(__byte_perm(w, 0x64646464u, 0x4140)), off));
+  b = h2_u32(__hadd2(u32_h2(__byte_perm(w, 0x64646464u, 0x4342)), off));
+}
+
 }  // namespace s3b
