@@ -1,4 +1,6 @@
 // Writing and reading the quantised key / value cache (layout: kv_cache.cuh).
+#include <algorithm>
+
 #include "kv_cache.cuh"
 
 namespace s3b {
@@ -43,14 +45,23 @@ __device__ __forceinline__ bool slot_place(const Job& j, long long slot, long lo
   return true;
 }
 
-// 8 values of a row as f32.
-__device__ __forceinline__ void load8(const float* at, float (&x)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(at)), b = __ldg(reinterpret_cast<const float4*>(at) + 1);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+// 8 values of a row as they are in memory, and as f32.
+template <typename T>
+struct Eight {
+  uint4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ void load8(const T* at, Eight<T>& r) {
+#pragma unroll
+  for (int e = 0; e < (int)sizeof(T) / 2; ++e) r.w[e] = __ldg(reinterpret_cast<const uint4*>(at) + e);
 }
-__device__ __forceinline__ void load8(const __half* at, float (&x)[8]) {
-  const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ void floats8(const Eight<float>& r, float (&x)[8]) {
+  const uint32_t w[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w, r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e]);
+}
+__device__ __forceinline__ void floats8(const Eight<__half>& r, float (&x)[8]) {
+  const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float2 f = __half22float2(u32_h2(w[e]));
@@ -162,59 +173,81 @@ __device__ __forceinline__ uint32_t pack_codes(const uint32_t* code) {
 }
 
 // Four lanes a block of 32 values, 8 each: rows are read in 16-byte pieces, and the 8 values of a lane are a whole word of
-// the keys' layout (4-bit codes; two words of 8-bit ones) and two pieces of the values'. K and V rows of two tokens are
-// read before any is quantised. Bound by instruction issue (about 14 a value) and HBM alike.
+// the keys' layout (4-bit codes; two words of 8-bit ones) and two pieces of the values'. Bound by HBM: the blocks stay
+// and walk over the tokens of their head, and the K and V rows of the next two tokens are on their way while these are
+// quantised (loading, then quantising, then storing left the memory idle half of the time).
 template <int QT, int D, typename T>
 __global__ void __launch_bounds__(256) write_kernel(const __grid_constant__ Job j) {
   typedef KvL<QT, D> L;
   constexpr int kLanes = D / 8, kRows = 256 / kLanes;  // lanes of a row, rows of a pass
   const int head = blockIdx.x % j.c.heads;
-  const long long first = (long long)(blockIdx.x / j.c.heads) * j.tokens + threadIdx.x / kLanes;
+  const long long step = (long long)(gridDim.x / j.c.heads) * j.tokens;
   const int c8 = threadIdx.x % kLanes, t = c8 & 3, b = c8 >> 2;
   uint8_t* base = j.c.data + head * 2 * j.v_bytes;
-  float x[2][2][8];
-  long long at[2];
-  int tok[2];
-  bool use[2];
+  const T* k = reinterpret_cast<const T*>(j.r.k) + head * j.r.k_h + c8 * 8;
+  const T* v = reinterpret_cast<const T*>(j.r.v) + head * j.r.v_h + c8 * 8;
+  Eight<T> raw[2][2];
+  long long slot[2];
+  auto load = [&](long long i0) {
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const long long i = first + u * kRows;
-    use[u] = i < j.n && slot_place<L::kHalf>(j, __ldg(j.slots + i), &at[u], &tok[u]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[u][0][e] = x[u][1][e] = 0.f;
-    if (use[u]) {
-      load8(reinterpret_cast<const T*>(j.r.k) + i * j.r.k_n + head * j.r.k_h + c8 * 8, x[u][0]);
-      load8(reinterpret_cast<const T*>(j.r.v) + i * j.r.v_n + head * j.r.v_h + c8 * 8, x[u][1]);
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-#pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      uint32_t c[8];
-      __half scale, low;
-      quantise8<QT>(x[u][kv], t, c, scale, low);
-      if (!use[u]) continue;
-      uint8_t* gp = base + at[u] + kv * j.v_bytes;
-      if (L::kBits == 8) {
-        const uint32_t w0 = pack_codes<4, 16, 8>(c), w1 = pack_codes<4, 16, 8>(c + 4);
-        if (kv == 0) {
-          *reinterpret_cast<uint2*>(gp + L::k_val(tok[u], b, t)) = make_uint2(w0, w1);
-        } else {
-          *reinterpret_cast<uint32_t*>(gp + L::v_val(tok[u], b, 2 * t)) = w0;
-          *reinterpret_cast<uint32_t*>(gp + L::v_val(tok[u], b, 2 * t + 1)) = w1;
-        }
-      } else if (kv == 0) {
-        *reinterpret_cast<uint32_t*>(gp + L::k_val(tok[u], b, t)) = pack_codes<8, 4, 16>(c);
-      } else {
-        const uint32_t w = pack_codes<8, 8, 4>(c);
-        *reinterpret_cast<uint16_t*>(gp + L::v_val(tok[u], b, 2 * t)) = (uint16_t)w;
-        *reinterpret_cast<uint16_t*>(gp + L::v_val(tok[u], b, 2 * t + 1)) = (uint16_t)(w >> 16);
+    for (int u = 0; u < 2; ++u) {
+      const long long i = i0 + u * kRows;
+      slot[u] = -1;
+      if (i < j.n) {
+        slot[u] = __ldg(j.slots + i);
+        load8(k + i * j.r.k_n, raw[u][0]);
+        load8(v + i * j.r.v_n, raw[u][1]);
       }
-      if (t == 0) {
-        __half* sp = reinterpret_cast<__half*>(gp + (kv ? L::v_scale(tok[u], b) : L::k_scale(tok[u], b)));
-        sp[0] = scale;
-        if (QT == QT_Q4_1) sp[L::kSc / 2] = low;
+    }
+  };
+  long long i0 = (long long)(blockIdx.x / j.c.heads) * j.tokens;
+  load(i0 + threadIdx.x / kLanes);
+  for (; i0 < j.n; i0 += step) {
+    Eight<T> now[2][2];
+    long long at[2];
+    int tok[2];
+    bool use[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      now[u][0] = raw[u][0];
+      now[u][1] = raw[u][1];
+      use[u] = slot_place<L::kHalf>(j, slot[u], &at[u], &tok[u]);
+    }
+    load(i0 + step + threadIdx.x / kLanes);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        // the lanes of a skipped token go along, with zeros: the lanes of a block exchange values
+        float x[8];
+        uint32_t c[8];
+        __half scale, low;
+        floats8(now[u][kv], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = use[u] ? x[e] : 0.f;
+        quantise8<QT>(x, t, c, scale, low);
+        if (!use[u]) continue;
+        uint8_t* gp = base + at[u] + kv * j.v_bytes;
+        if (L::kBits == 8) {
+          const uint32_t w0 = pack_codes<4, 16, 8>(c), w1 = pack_codes<4, 16, 8>(c + 4);
+          if (kv == 0) {
+            *reinterpret_cast<uint2*>(gp + L::k_val(tok[u], b, t)) = make_uint2(w0, w1);
+          } else {
+            *reinterpret_cast<uint32_t*>(gp + L::v_val(tok[u], b, 2 * t)) = w0;
+            *reinterpret_cast<uint32_t*>(gp + L::v_val(tok[u], b, 2 * t + 1)) = w1;
+          }
+        } else if (kv == 0) {
+          *reinterpret_cast<uint32_t*>(gp + L::k_val(tok[u], b, t)) = pack_codes<8, 4, 16>(c);
+        } else {
+          const uint32_t w = pack_codes<8, 8, 4>(c);
+          *reinterpret_cast<uint16_t*>(gp + L::v_val(tok[u], b, 2 * t)) = (uint16_t)w;
+          *reinterpret_cast<uint16_t*>(gp + L::v_val(tok[u], b, 2 * t + 1)) = (uint16_t)(w >> 16);
+        }
+        if (t == 0) {
+          __half* sp = reinterpret_cast<__half*>(gp + (kv ? L::v_scale(tok[u], b) : L::k_scale(tok[u], b)));
+          sp[0] = scale;
+          if (QT == QT_Q4_1) sp[L::kSc / 2] = low;
+        }
       }
     }
   }
@@ -311,7 +344,11 @@ int launch(bool write, const KvCache& c, const KvRows& r, const long long* slots
     while ((2LL << j.div_shift) < c.page_size) ++j.div_shift;
     j.div_mul = (unsigned)(((1ULL << (32 + j.div_shift)) + c.page_size - 1) / c.page_size);
   }
-  const long long blocks = (n + j.tokens - 1) / j.tokens * c.heads;
+  long long blocks = (n + j.tokens - 1) / j.tokens * c.heads;
+  if (write) {  // blocks that stay: as many as are resident, a multiple of the heads
+    const long long resident = 6LL * num_sms() / c.heads * c.heads;
+    blocks = std::min(blocks, std::max(resident, (long long)c.heads));
+  }
   if (blocks > 0x7fffffffLL) return -2;
   const JobKernel k = c.type == QT_Q4_0 ? job_kernel_d<QT_Q4_0>(c.d, write, r.f32)
                       : c.type == QT_Q4_1 ? job_kernel_d<QT_Q4_1>(c.d, write, r.f32)
