@@ -71,9 +71,12 @@ struct Rows {
   static constexpr int kJoin = W * kRows * kOStride * 4;
   static constexpr int kFixed = kQBytes + 3 * W * kRows * 4 + 1024;
   static constexpr int kBudget = (225 * 1024) / kCtas - kFixed - 1024;
-  static constexpr int kFit = kBudget / (W * (2 * L::kHalf));
+  // groups of 16 tokens of a step: two share the waits, the votes and the copies where two stages of them fit
+  static constexpr int kG = NT == 1 && D <= (QT == QT_Q8_0 ? 64 : 128) ? 2 : 1;
+  static constexpr int kStageBytes = kG * 2 * L::kHalf;
+  static constexpr int kFit = kBudget / (W * kStageBytes);
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
-  static constexpr int kRing = W * kStages * (2 * L::kHalf);
+  static constexpr int kRing = W * kStages * kStageBytes;
   static constexpr int kMain = kRing > kJoin ? kRing : kJoin;
   static constexpr int kSmem = kMain + kFixed;
   static_assert(kStages >= 2 && kMain + kFixed + 1024 <= (227 * 1024) / kCtas, "shared memory of rows_kernel");
@@ -89,7 +92,7 @@ template <int QT, int D, int NT, int W>
 __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel(const __grid_constant__ RowsArgs a, int* err) {
   typedef KvL<QT, D> L;
   typedef Rows<QT, D, NT, W> C;
-  constexpr int NB = L::kNB, NS = C::kStages;
+  constexpr int NB = L::kNB, NS = C::kStages, G = C::kG;
   constexpr float kBias = QT == QT_Q8_0 ? 4.f : 0.f;  // weights are 2^kBias at the reference: their products with the
                                                        // block scales then use f16's range as the values would
   constexpr float kLazy = 2.9f;                        // and stay below f16's largest: 2^(kBias + 2.9) * scale < 65504
@@ -113,7 +116,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
 
   auto chunks_of = [&](int b, int* g0, int* g1) -> int {
     group_span(p, sequence_length(p, b, err), 0, p.nq - 1, g0, g1);
-    return (*g1 - *g0 + W - 1) / W;
+    return (*g1 - *g0 + W * G - 1) / (W * G);
   };
 
   if (threadIdx.x < W * NS) mbar_init(&bars[threadIdx.x], 1);
@@ -178,7 +181,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
   const long long p0 = total * blockIdx.x / ctas, p1 = total * (blockIdx.x + 1) / ctas;
   const float sl2 = p.scale * kLog2e;
   const long long v_offset = (long long)per_page * L::kHalf;  // of a page's values from its keys
-  uint8_t* ring = smem + warp * NS * (2 * L::kHalf);
+  uint8_t* ring = smem + warp * NS * C::kStageBytes;
   uint64_t* full = bars + warp * NS;
   int stage = 0;
   uint32_t phase = 0;
@@ -200,13 +203,13 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
       const int cb = (int)min((long long)n_chunks, p1 - unit_start);
       pos += cb - ca;
 
-      // ---- this warp's groups: g0 + chunk * W + warp
-      const int first = g0 + ca * W + warp;
-      const int n_it = first < g1 ? min(cb - ca, (g1 - first + W - 1) / W) : 0;
-      long long src = 0;  // lane i: address of iteration (batch of 32) + i
+      // ---- this warp's groups: G from g0 + (chunk * W + warp) * G
+      const int first = g0 + (ca * W + warp) * G;
+      const int n_it = first < g1 ? min(cb - ca, (g1 - first + W * G - 1) / (W * G)) : 0;
+      long long src = 0;  // lane i: address of group i % G of step (of a batch of 32 / G) + i / G
       auto locate = [&](int it0) {
-        const int gi = first + (it0 + lane) * W;
-        if (it0 + lane < n_it) {
+        const int gi = first + (it0 + lane / G) * (W * G) + lane % G;
+        if (it0 + lane / G < n_it && gi < g1) {
           long long page = table[gi / per_page];
           if (page < 0 || page >= p.c.n_pages) {
             atomicCAS(err, 0, kDevErrIndex);
@@ -217,12 +220,21 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
       };
       int st_issue = stage;
       auto issue = [&](int it) {
-        const long long from = __shfl_sync(~0u, src, it & 31);
+        const long long from = __shfl_sync(~0u, src, it * G & 31), from1 = G == 2 ? __shfl_sync(~0u, src, it * G + 1 & 31) : 0;
         if (lane == 0) {
-          mbar_arrive_expect_tx(&full[st_issue], (2 * L::kHalf));
-          uint8_t* to = ring + st_issue * (2 * L::kHalf);
-          bulk_load(to, p.c.data + from, L::kHalf, &full[st_issue]);
-          bulk_load(to + L::kHalf, p.c.data + from + v_offset, L::kHalf, &full[st_issue]);
+          const bool both = G == 2 && first + it * (W * G) + 1 < g1;
+          uint8_t* to = ring + st_issue * C::kStageBytes;
+          const uint8_t* k = p.c.data + from;
+          mbar_arrive_expect_tx(&full[st_issue], (both ? 4 : 2) * L::kHalf);
+          const bool joined = both && from1 == from + L::kHalf;  // neighbours in a page
+          const uint32_t bytes = joined ? 2 * L::kHalf : L::kHalf;
+          bulk_load(to, k, bytes, &full[st_issue]);
+          bulk_load(to + G * L::kHalf, k + v_offset, bytes, &full[st_issue]);
+          if (both && !joined) {
+            k = p.c.data + from1;
+            bulk_load(to + L::kHalf, k, L::kHalf, &full[st_issue]);
+            bulk_load(to + (G + 1) * L::kHalf, k + v_offset, L::kHalf, &full[st_issue]);
+          }
         }
         st_issue = st_issue + 1 == NS ? 0 : st_issue + 1;
       };
@@ -291,15 +303,18 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
         if (!mbar_wait(&full[stage], phase, s_abort, err, kErrWaitFull)) ok = false;
         ok = __all_sync(~0u, ok);
         if (!ok) break;
-        const uint8_t *gp = ring + stage * (2 * L::kHalf), *vp = gp + L::kHalf;
-        const int tok0 = (first + it * W) * 16;
-        const bool whole = tok0 >= max_lo && tok0 + 16 <= min_hi;
+        const int tok0 = (first + it * (W * G)) * 16;
+        const bool whole = tok0 >= max_lo && tok0 + 16 * G <= min_hi;
 
         // -- scores
+        float s_all[G][NT][4];
+#pragma unroll
+        for (int gg = 0; gg < G; ++gg) {
+        const uint8_t* gp = ring + stage * C::kStageBytes + gg * L::kHalf;
+        float (&s)[NT][4] = s_all[gg];
         uint32_t sc0[NB / 2], sc1[NB / 2];  // scales of tokens g and g + 8
         lds<NB * 2>(gp + L::k_scale(g, 0), sc0);
         lds<NB * 2>(gp + L::k_scale(g + 8, 0), sc1);
-        float s[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -354,23 +369,35 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
           }
         }
 
+        }
+
         // -- weights: the reference maximum of a column moves only when a score passes it by kLazy
         bool move = false;
+        float top[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][e] *= sl2;
-          if (!whole) {
+          for (int gg = 0; gg < G; ++gg) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              int lo, hi;
-              row_span(p, len, min((8 * nt + 2 * t + c) / group_heads, p.nq - 1), &lo, &hi);
-              if (tok0 + g < lo || tok0 + g >= hi) s[nt][c] = -INFINITY;
-              if (tok0 + g + 8 < lo || tok0 + g + 8 >= hi) s[nt][c + 2] = -INFINITY;
+            for (int e = 0; e < 4; ++e) s_all[gg][nt][e] *= sl2;
+            if (!whole) {
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                int lo, hi;
+                row_span(p, len, min((8 * nt + 2 * t + c) / group_heads, p.nq - 1), &lo, &hi);
+                const int tok = tok0 + 16 * gg + g;
+                if (tok < lo || tok >= hi) s_all[gg][nt][c] = -INFINITY;
+                if (tok + 8 < lo || tok + 8 >= hi) s_all[gg][nt][c + 2] = -INFINITY;
+              }
             }
           }
 #pragma unroll
-          for (int c = 0; c < 2; ++c) move |= fmaxf(s[nt][c], s[nt][c + 2]) > m[nt][c] + kBias + kLazy;
+          for (int c = 0; c < 2; ++c) {
+            top[nt][c] = fmaxf(s_all[0][nt][c], s_all[0][nt][c + 2]);
+#pragma unroll
+            for (int gg = 1; gg < G; ++gg) top[nt][c] = fmaxf(top[nt][c], fmaxf(s_all[gg][nt][c], s_all[gg][nt][c + 2]));
+            move |= top[nt][c] > m[nt][c] + kBias + kLazy;
+          }
         }
         if (__any_sync(~0u, move)) {
 #pragma unroll
@@ -378,10 +405,9 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
             float f[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float top = fmaxf(s[nt][c], s[nt][c + 2]);
 #pragma unroll
-              for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-              const float m2 = fmaxf(m[nt][c], top - kBias);
+              for (int x = 4; x < 32; x <<= 1) top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(~0u, top[nt][c], x));
+              const float m2 = fmaxf(m[nt][c], top[nt][c] - kBias);
               f[c] = ex2_approx(m[nt][c] - m2);
               m[nt][c] = m2;
               l[nt][c] *= f[c];
@@ -394,28 +420,37 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
             for (int e = 0; e < 4; ++e) omin[nt][e] *= f[e & 1];
           }
         }
-        uint32_t w0[NT], w1[NT];  // weights of column g for tokens 2t, 2t + 1 and 2t + 8, 2t + 9
+        // weights of column g for tokens 2t, 2t + 1 and 2t + 8, 2t + 9 of each group
+        uint32_t w0_all[G][NT], w1_all[G][NT];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float e4[4];
+        for (int gg = 0; gg < G; ++gg)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) e4[e] = ex2_approx(s[nt][e] - m[nt][e & 1]);
-          l[nt][0] += e4[0] + e4[2];
-          l[nt][1] += e4[1] + e4[3];
-          w0[nt] = movmatrix(h2_u32(__floats2half2_rn(e4[0], e4[1])));
-          w1[nt] = movmatrix(h2_u32(__floats2half2_rn(e4[2], e4[3])));
-        }
+          for (int nt = 0; nt < NT; ++nt) {
+            float e4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) e4[e] = ex2_approx(s_all[gg][nt][e] - m[nt][e & 1]);
+            l[nt][0] += e4[0] + e4[2];
+            l[nt][1] += e4[1] + e4[3];
+            w0_all[gg][nt] = movmatrix(h2_u32(__floats2half2_rn(e4[0], e4[1])));
+            w1_all[gg][nt] = movmatrix(h2_u32(__floats2half2_rn(e4[2], e4[3])));
+          }
 
         // -- outputs; tokens outside the sequence's span may hold anything, so their scales become zero
         if (!whole) {
-          __half* scales = reinterpret_cast<__half*>(ring + stage * (2 * L::kHalf) + L::kHalf + L::kVal);
-          for (int e = lane; e < 16 * NB * L::kPlanes; e += 32) {
-            const int lane_t = e % (16 * NB) / (4 * NB), tok = tok0 + 2 * lane_t + (e & 1) + 4 * (e & 2);
-            if (tok < min_lo || tok >= max_hi) scales[e] = __ushort_as_half(0);
+          for (int gg = 0; gg < G; ++gg) {
+            __half* scales = reinterpret_cast<__half*>(ring + stage * C::kStageBytes + (G + gg) * L::kHalf + L::kVal);
+            for (int e = lane; e < 16 * NB * L::kPlanes; e += 32) {
+              const int lane_t = e % (16 * NB) / (4 * NB), tok = tok0 + 16 * gg + 2 * lane_t + (e & 1) + 4 * (e & 2);
+              if (tok < min_lo || tok >= max_hi) scales[e] = __ushort_as_half(0);
+            }
           }
           fence_proxy_async_smem();  // the next copy into this stage comes after these writes
           __syncwarp();
         }
+#pragma unroll
+        for (int gg = 0; gg < G; ++gg) {
+        const uint8_t* vp = ring + stage * C::kStageBytes + (G + gg) * L::kHalf;
+        const uint32_t (&w0)[NT] = w0_all[gg], (&w1)[NT] = w1_all[gg];
         if (QT == QT_Q4_1) {  // sum over tokens of weight * minimum, a row for each block
           uint32_t am[4] = {0, 0, 0, 0};
           if (g < NB) {
@@ -457,11 +492,12 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
             }
           }
         }
+        }
         stage = stage + 1 == NS ? 0 : stage + 1;
         if (stage == 0) phase ^= 1;
         __syncwarp();
         if (issued < n_it) {
-          if ((issued & 31) == 0) locate(issued);
+          if (issued * G % 32 == 0) locate(issued);
           issue(issued);
           ++issued;
         }
