@@ -64,7 +64,9 @@ struct Rows {
   typedef KvL<QT, D> L;
   static constexpr int kRows = 8 * NT;
   static constexpr bool kQSmem = NT * D > 128;  // the query fragments of more would not fit beside the output's registers
-  static constexpr int kWarps = QT == QT_Q8_0 && D == 256 ? 8 : 16;  // of an SM, each with its ring
+  // Warps of an SM, each with its ring: the output takes NT * D / 4 registers, so 128, 168 or 255 registers a thread (12
+  // instead of 16 warps at 64 output registers: 16 rows of d = 128 133 -> 123 us, d = 256 61 -> 60 us; at 32 it cost 5%).
+  static constexpr int kWarps = NT * D >= 512 || (QT == QT_Q8_0 && D == 256) ? 8 : NT * D >= 256 ? 12 : 16;
   static constexpr int kCtas = kWarps / W;
   static constexpr int kQBytes = kQSmem ? NT * L::kNB * 512 : 0;
   static constexpr int kOStride = D + 4;        // floats; the padding spreads the rows of a store over the banks
@@ -678,22 +680,25 @@ int launch_rows(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream
 }
 
 // ---------------------------------------------------------------- dispatch
-// Rows of one key / value head that rows_kernel takes: the output registers of 8 rows are D / 4, so 8 * (256 / D).
-int most_rows(int d) { return 2048 / d; }
+// Rows of one key / value head that rows_kernel takes (its output registers end at 128 a thread).
+int most_rows(int d) { return d == 256 ? 16 : 32; }
 
-template <int QT, int D, int W>
-int launch_rows_nt(const KvAttnParams& p, const KvAttnWork& w, int rows, int* err, cudaStream_t st) {
-  if (rows <= 8) return launch_rows<QT, D, 1, W>(p, w, err, st);
-  if (D <= 128 && rows <= 16) return launch_rows<QT, D, D <= 128 ? 2 : 1, W>(p, w, err, st);
-  return launch_rows<QT, D, D <= 64 ? 4 : 1, W>(p, w, err, st);
+template <int QT, int D, int NT>
+int launch_rows_nt(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
+  // Blocks of four warps, several on an SM, where there is a unit for each SM: a unit's beginning and end then run beside
+  // other blocks' loops (32 sequences, 8 heads: 123 -> 96 us). One block an SM where few units are cut into many parts,
+  // which have to be joined (one sequence, 2 heads, 524288 tokens: 477 -> 119 us).
+  constexpr int kMost = Rows<QT, D, NT, 4>::kWarps;
+  if ((long long)p.batch * p.c.heads >= w.sms) return launch_rows<QT, D, NT, 4>(p, w, err, st);
+  return launch_rows<QT, D, NT, kMost>(p, w, err, st);
 }
 
 template <int QT, int D>
 int attend(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
   const int rows = p.nq * (p.heads / p.c.heads);
-  constexpr int kMost = Rows<QT, D, 1, 4>::kWarps;
-  if ((long long)p.batch * p.c.heads >= w.sms) return launch_rows_nt<QT, D, 4>(p, w, rows, err, st);
-  return launch_rows_nt<QT, D, kMost>(p, w, rows, err, st);
+  if (rows <= 8) return launch_rows_nt<QT, D, 1>(p, w, err, st);
+  if (D == 256 || rows <= 16) return launch_rows_nt<QT, D, 2>(p, w, err, st);
+  return launch_rows_nt<QT, D, D == 256 ? 2 : 4>(p, w, err, st);
 }
 
 template <int QT>
