@@ -386,6 +386,7 @@ __device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float 
     l *= alpha;
     moved = true;
   }
+  __syncwarp();  // the TMEM accesses below take the whole warp together
   const unsigned long long sl2x2 = f2_pack(sl2, sl2), negm2 = f2_pack(-m_ref, -m_ref);
   unsigned long long acc0 = f2_pack(0.f, 0.f), acc1 = acc0;
   if (N == 64) {
@@ -576,7 +577,6 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
     } else if (warp == 2 && STAGED) {
       // ---- copies of the staged operands, slot by slot
       if (lane == 0) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");  // stage_kernel has written them
         uint32_t slot = 0, q_n = 0;
         bool ok = true;
         while (ok && walk_next<ROWS>(p, a.blocks, err, &w)) {
@@ -740,7 +740,12 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
         for (int x = 0; x < C::kSub / 64; ++x) {
           const int half = C::kSubs == 2 ? sub : x;
           const uint32_t s0 = slot0 + v_item(j, n) * C::kParts + (D == 64 ? 0 : half * (D / 128));
-          if ((D > 64 || half == 0) && !wait_slot(s0)) return false;
+          // every slot of the product: staged ones land one by one
+          if (D > 64 || half == 0) {
+#pragma unroll
+            for (int y = 0; y < (D > 64 ? D / 128 : 1); ++y)
+              if (!wait_slot(s0 + y)) return false;
+          }
           const uint64_t dv = sdesc_k_sw128(ring + s0 % kSlots * kSlotBytes + (D == 64 ? half * (D * 128) : 0));
           if (elect_one()) {
 #pragma unroll
@@ -884,6 +889,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
           tc_wait_ld();
           finish(c, reinterpret_cast<float*>(o), inv);
           finish(c + 16, reinterpret_cast<float*>(o) + 16, inv);
+          __syncwarp();  // lanes of rows past the end come along
         }
         finish_lse(m_ref, l);
         continue;
@@ -1007,7 +1013,6 @@ template <int D, int TQ>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArgs a) {
   constexpr int kPart = TQ * kTile * (D + 2), kMost = 160;
   __shared__ float s_f[kMost][32], s_top[8][32], s_sum[8][32];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c0 = blockIdx.x;
   const Shared u = a.shared[c0];
   if (!u.valid) return;
@@ -1082,7 +1087,6 @@ template <int QT, int D>
 __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ TcArgs a, int kv_blocks, int* err) {
   typedef KvL<QT, D> L;
   constexpr int TQ = D == 256 ? 1 : 2;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const KvAttnParams& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = p.heads / p.c.heads;
@@ -1157,22 +1161,6 @@ TcPlan tc_plan(const KvAttnParams& p) {
 }
 size_t part_floats(int sms, int tq, int d) { return (size_t)2 * sms * tq * kTile * (d + 2); }
 
-template <typename K, typename... A>
-int launch_dependent(K* kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
-  // may begin while its predecessor still runs; it waits for the predecessor's end before it reads its results
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? 0 : -12;
-}
-
 template <int QT, int D>
 int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
   constexpr int TQ = D == 256 ? 1 : 2;
@@ -1195,7 +1183,8 @@ int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStrea
     const long long q_blocks = (long long)p.batch * p.c.heads * t.blocks * TQ;
     stage_kernel<QT, D><<<(unsigned)(kv_blocks + q_blocks), 256, 0, st>>>(a, (int)kv_blocks, err);
     if (cudaGetLastError() != cudaSuccess) return -12;
-    rc = launch_dependent(k, dim3(w.sms), C::kThreads, C::kSmem, st, a, err);
+    k<<<w.sms, C::kThreads, C::kSmem, st>>>(a, err);
+    rc = cudaGetLastError() == cudaSuccess ? 0 : -12;
   } else {
     typedef Tc<QT, D, false> C;
     auto* k = tiles_kernel<QT, D, false>;
@@ -1204,7 +1193,8 @@ int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStrea
     rc = cudaGetLastError() == cudaSuccess ? 0 : -12;
   }
   if (rc) return rc;
-  return launch_dependent(join_kernel<D, TQ>, dim3(w.sms, TQ * 4), 256, 0, st, a);
+  join_kernel<D, TQ><<<dim3(w.sms, TQ * 4), 256, 0, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -12;
 }
 
 template <int QT>
