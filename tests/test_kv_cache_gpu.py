@@ -247,6 +247,12 @@ def test_attention_query_counts(s3b, engine, d, nq):
     _check(s3b, engine, 2, d, 3, 1, nq, [260, nq + 1, 19], 32, True, out_dtype=torch.float32)
 
 
+@pytest.mark.parametrize("qtype,d,page", [(2, 256, 16), (8, 256, 64), (3, 128, 48), (2, 64, 16)])
+def test_attention_many_row_blocks(s3b, engine, qtype, d, page):
+    """Uneven sequences of several row blocks each: every share of the work begins and ends inside one."""
+    _check(s3b, engine, qtype, d, 4, 2, 600, [1200, 901, 33, 1100, 640, 1025], page, True)
+
+
 @pytest.mark.parametrize("nq", [1, 140])
 @pytest.mark.parametrize("qtype", [2, 8])
 def test_attention_peaked(s3b, engine, qtype, nq):
