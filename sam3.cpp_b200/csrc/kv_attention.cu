@@ -453,15 +453,25 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
         for (int gg = 0; gg < G; ++gg) {
         const uint8_t* vp = ring + stage * C::kStageBytes + (G + gg) * L::kHalf;
         const uint32_t (&w0)[NT] = w0_all[gg], (&w1)[NT] = w1_all[gg];
-        if (QT == QT_Q4_1) {  // sum over tokens of weight * minimum, a row for each block
-          uint32_t am[4] = {0, 0, 0, 0};
+        if (QT == QT_Q4_1) {
+          // v = scale * (code - 8) + (minimum + 8 scale): the second term summed over tokens with the weights, a row for each
+          // block. It is small where values surround 0; codes from 0 with the minimum would leave two large sums of opposite
+          // sign, and the output over 524288 tokens off by 1.6e-3 (accumulation in the tensor core) instead of 3.5e-4.
+          uint32_t am[4] = {0, 0, 0, 0}, as[4] = {0, 0, 0, 0};
           if (g < NB) {
             const uint2 v = *reinterpret_cast<const uint2*>(vp + L::kSc + L::v_scale(2 * t, g));
+            const uint2 s = *reinterpret_cast<const uint2*>(vp + L::v_scale(2 * t, g));
             am[0] = v.x;
             am[2] = v.y;
+            as[0] = s.x;
+            as[2] = s.y;
           }
+          const __half2 eight = u32_h2(0x48004800u);  // 8 times the weight, exact; 8 times the scale may pass f16's range
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816(omin[nt], am, w0[nt], w1[nt]);
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816(omin[nt], am, w0[nt], w1[nt]);
+            mma16816(omin[nt], as, h2_u32(__hmul2(u32_h2(w0[nt]), eight)), h2_u32(__hmul2(u32_h2(w1[nt]), eight)));
+          }
         }
 #pragma unroll
         for (int sb = 0; sb < D / L::kSB; ++sb) {
@@ -480,8 +490,8 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas) rows_kernel
               byte_pairs(__byte_perm(vb[nn], vb[PW + nn], 0x5140), x1[0], x1[1]);
               byte_pairs(__byte_perm(vb[nn], vb[PW + nn], 0x7362), x1[2], x1[3]);
             } else {
-              nibble_pairs<QT>(__byte_perm(va[nn / 2], va[PW + nn / 2], nn & 1 ? 0x7632 : 0x5410), x0);
-              nibble_pairs<QT>(__byte_perm(vb[nn / 2], vb[PW + nn / 2], nn & 1 ? 0x7632 : 0x5410), x1);
+              nibble_pairs<QT_Q4_0>(__byte_perm(va[nn / 2], va[PW + nn / 2], nn & 1 ? 0x7632 : 0x5410), x0);
+              nibble_pairs<QT_Q4_0>(__byte_perm(vb[nn / 2], vb[PW + nn / 2], nn & 1 ? 0x7632 : 0x5410), x1);
             }
             const uint32_t a0[4] = {x0[0], x0[1], x1[0], x1[1]}, a1[4] = {x0[2], x0[3], x1[2], x1[3]};
             const uint2 sc = *reinterpret_cast<const uint2*>(vp + L::v_scale(2 * t, n));
