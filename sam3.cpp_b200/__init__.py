@@ -191,27 +191,17 @@ def dequantize_rows(qtype: int, raw: np.ndarray, ne0: int) -> np.ndarray:
     return out
 
 
+# Row types of the cache operators and index types by size. Torch is imported where tensors are first needed: by KVCache.
+_ROW_TYPES: dict = {}
+_INDEX_TYPES: dict = {}
+
+
 def _index(what: str, name: str, t, itemsize: int, dims: int) -> int:
     """Length of an index tensor of `dims` dimensions (int32: itemsize 4, int64: 8) with contiguous rows."""
-    if t.dtype.itemsize != itemsize or t.dtype.is_floating_point or t.dtype.is_complex or t.dim() != dims or \
-            (t.stride(dims - 1) != 1 and t.numel()):
-        raise S3BError(f"{what}: {name} must be int{8 * itemsize} of {dims} dimension(s) with contiguous rows")
-    return t.shape[0]
-
-
-def _strides2(t):
-    """Strides of the first two dimensions, 0 where a dimension has one entry (its stride means nothing)."""
-    if t is None:
-        return 0, 0
-    a, b, _ = t.stride()
-    n, h, _ = t.shape
-    return a if n > 1 else 0, b if h > 1 else 0
-
-
-def _strides3(t):
-    a, b, c, _ = t.stride()
-    i, j, k, _ = t.shape
-    return a if i > 1 else 0, b if j > 1 else 0, c if k > 1 else 0
+    shape = t.shape
+    if t.dtype is not _INDEX_TYPES[itemsize] or len(shape) != dims or not t.is_cuda or (t.stride()[-1] != 1 and t.numel()):
+        raise S3BError(f"{what}: {name} must be CUDA int{8 * itemsize} of {dims} dimension(s) with contiguous rows")
+    return shape[0]
 
 
 def kv_cache_bytes(qtype: int, heads: int, d: int, page_size: int, n_pages: int) -> int:
@@ -228,11 +218,16 @@ class KVCache:
 
     def __init__(self, qtype: int, n_pages: int, page_size: int, heads: int, d: int, data=None, device="cuda"):
         nbytes = kv_cache_bytes(qtype, heads, d, page_size, n_pages)
+        import torch
+        if not _ROW_TYPES:
+            _INDEX_TYPES.update({4: torch.int32, 8: torch.int64})
+            _ROW_TYPES.update({torch.float16: S3B_F16, torch.float32: S3B_F32})
         if data is None:
-            import torch
             data = torch.zeros(nbytes, dtype=torch.uint8, device=device)
         elif data.numel() * data.element_size() < nbytes or not data.is_contiguous():
             raise S3BError(f"KVCache: data must be {nbytes} contiguous bytes")
+        if not data.is_cuda:
+            raise S3BError("KVCache: data must be a CUDA tensor")
         self.data = data
         self.qtype, self.n_pages, self.page_size, self.heads, self.d = qtype, n_pages, page_size, heads, d
         self.desc = KVCacheDesc(qtype, heads, d, page_size, n_pages, data.data_ptr())
@@ -699,25 +694,25 @@ class Engine:
 
     # -- quantised key / value cache
     @staticmethod
-    def _cache_rows(what: str, cache: KVCache, n: int, name: str, t, dtype: int | None) -> int:
-        """dtype code of the row tensor t [n, heads, d] (that of its partner, if given) after the checks that a raw pointer
-        cannot carry."""
-        size = t.dtype.itemsize
-        if not t.dtype.is_floating_point or size not in (2, 4) or "bfloat16" in str(t.dtype) or \
-                (dtype is not None and dtype != (S3B_F16 if size == 2 else S3B_F32)):
+    def _cache_rows(what: str, cache: KVCache, n: int, name: str, t, dtype: int | None):
+        """dtype code (that of its partner, if given), pointer and strides of the row tensor t [n, heads, d] after the checks
+        that a raw pointer cannot carry. The stride of a dimension of one entry means nothing and is given as 0."""
+        code = _ROW_TYPES.get(t.dtype)
+        if code is None or (dtype is not None and dtype != code):
             raise S3BError(f"{what}: rows must be all f16 or all f32, {name} is {t.dtype}")
-        if t.shape != (n, cache.heads, cache.d) or (t.stride(2) != 1 and n):
-            raise S3BError(f"{what}: {name} must be [{n}, {cache.heads}, {cache.d}] with contiguous rows")
-        return S3B_F16 if size == 2 else S3B_F32
+        heads = cache.heads
+        a, b, c = t.stride() if t.dim() == 3 else (0, 0, 0)
+        if t.shape != (n, heads, cache.d) or not t.is_cuda or (c != 1 and n):
+            raise S3BError(f"{what}: {name} must be a CUDA tensor [{n}, {heads}, {cache.d}] with contiguous rows")
+        return code, t.data_ptr(), a if n > 1 else 0, b if heads > 1 else 0
 
     def cache_write(self, cache: KVCache, k, v, slots):
         """Quantises the tokens k, v [n, heads, d] (f16 or f32 CUDA tensors, rows contiguous) into the slots int64 [n]
         (< 0: skipped)."""
         n = _index("cache_write", "slots", slots, 8, 1)
-        dtype = self._cache_rows("cache_write", cache, n, "k", k, None)
-        self._cache_rows("cache_write", cache, n, "v", v, dtype)
-        rc = self._L.s3b_op_cache_write(self.h, cache.ref, k.data_ptr(), *_strides2(k), v.data_ptr(), *_strides2(v),
-                                        dtype, slots.data_ptr(), n)
+        dtype, k_at, k_n, k_h = self._cache_rows("cache_write", cache, n, "k", k, None)
+        _, v_at, v_n, v_h = self._cache_rows("cache_write", cache, n, "v", v, dtype)
+        rc = self._L.s3b_op_cache_write(self.h, cache.ref, k_at, k_n, k_h, v_at, v_n, v_h, dtype, slots.data_ptr(), n)
         if rc:
             self._check(rc, "s3b_op_cache_write")
 
@@ -725,12 +720,13 @@ class Engine:
         """Reads the tokens of the slots int64 [n] (< 0: zeros) into k_out, v_out [n, heads, d] (f16 or f32; one of them
         may be None)."""
         n = _index("cache_read", "slots", slots, 8, 1)
-        dtype = None
-        for name, t in (("k_out", k_out), ("v_out", v_out)):
-            if t is not None:
-                dtype = self._cache_rows("cache_read", cache, n, name, t, dtype)
-        rc = self._L.s3b_op_cache_read(self.h, cache.ref, slots.data_ptr(), n, _ptr(k_out), *_strides2(k_out),
-                                       _ptr(v_out), *_strides2(v_out), S3B_F16 if dtype is None else dtype)
+        dtype, k_at, k_n, k_h, v_at, v_n, v_h = None, None, 0, 0, None, 0, 0
+        if k_out is not None:
+            dtype, k_at, k_n, k_h = self._cache_rows("cache_read", cache, n, "k_out", k_out, None)
+        if v_out is not None:
+            dtype, v_at, v_n, v_h = self._cache_rows("cache_read", cache, n, "v_out", v_out, dtype)
+        rc = self._L.s3b_op_cache_read(self.h, cache.ref, slots.data_ptr(), n, k_at, k_n, k_h, v_at, v_n, v_h,
+                                       S3B_F16 if dtype is None else dtype)
         if rc:
             self._check(rc, "s3b_op_cache_read")
 
@@ -739,21 +735,30 @@ class Engine:
         """out = softmax(scale q K^T) V over the cache (s3b_op_cache_attention): q f16 [batch, nq, heads, d], out the same
         shape in f16 or f32, pages int32 [batch, max_pages], lengths int32 [batch], lse f32 [batch, nq, heads] or None."""
         what = "cache_attention"
-        b, nq, heads, d = shape = q.shape
-        q_type, o_type = q.dtype, out.dtype
-        if not q_type.is_floating_point or q_type.itemsize != 2 or "bfloat16" in str(q_type) or d != cache.d or \
+        shape = q.shape
+        if _ROW_TYPES.get(q.dtype) != S3B_F16 or len(shape) != 4 or shape[3] != cache.d or not q.is_cuda or \
                 (q.stride(3) != 1 and q.numel()):
-            raise S3BError(f"{what}: q must be f16 [batch, nq, heads, {cache.d}] with contiguous rows")
-        if out.shape != shape or (o_type is not q_type and (o_type.itemsize != 4 or not o_type.is_floating_point)) or \
-                (out.stride(3) != 1 and out.numel()):
-            raise S3BError(f"{what}: out must have q's shape, in f16 or f32, with contiguous rows")
+            raise S3BError(f"{what}: q must be CUDA f16 [batch, nq, heads, {cache.d}] with contiguous rows")
+        b, nq, heads, _ = shape
+        o_type = _ROW_TYPES.get(out.dtype)
+        if o_type is None or out.shape != shape or not out.is_cuda or (out.stride(3) != 1 and out.numel()):
+            raise S3BError(f"{what}: out must be CUDA f16 or f32 of q's shape with contiguous rows")
         if _index(what, "lengths", lengths, 4, 1) != b or _index(what, "pages", pages, 4, 2) != b:
             raise S3BError(f"{what}: pages must be int32 [{b}, max_pages] with contiguous rows, lengths int32 [{b}]")
-        if lse is not None and (lse.shape != (b, nq, heads) or lse.dtype.itemsize != 4 or
-                                not lse.dtype.is_floating_point or not lse.is_contiguous()):
-            raise S3BError(f"{what}: lse must be contiguous f32 [{b}, {nq}, {heads}]")
-        rc = self._L.s3b_op_cache_attention(self.h, cache.ref, q.data_ptr(), *_strides3(q), out.data_ptr(),
-                                            0 if o_type is q_type else 1, *_strides3(out), _ptr(lse), pages.data_ptr(),
+        if lse is not None and (lse.shape != (b, nq, heads) or _ROW_TYPES.get(lse.dtype) != S3B_F32 or
+                                not lse.is_cuda or not lse.is_contiguous()):
+            raise S3BError(f"{what}: lse must be contiguous CUDA f32 [{b}, {nq}, {heads}]")
+        # the stride of a dimension of one entry means nothing and is given as 0
+        q_b, q_n, q_h, _ = q.stride()
+        o_b, o_n, o_h, _ = out.stride()
+        if b < 2:
+            q_b = o_b = 0
+        if nq < 2:
+            q_n = o_n = 0
+        if heads < 2:
+            q_h = o_h = 0
+        rc = self._L.s3b_op_cache_attention(self.h, cache.ref, q.data_ptr(), q_b, q_n, q_h, out.data_ptr(),
+                                            0 if o_type == S3B_F16 else 1, o_b, o_n, o_h, _ptr(lse), pages.data_ptr(),
                                             pages.stride(0), pages.shape[1], lengths.data_ptr(), b, nq, heads, scale,
                                             1 if causal else 0, window)
         if rc:

@@ -361,6 +361,16 @@ def test_refusals(s3b, engine):
     refuses(engine.cache_attention, cache, q, out[:, :, :2], pages, lens, 0.1)
     refuses(engine.cache_attention, cache, q, out, pages.long(), lens, 0.1)
     refuses(engine.cache_attention, cache, q, out, pages, lens.long(), 0.1)
+    # tensors that are not on the GPU
+    refuses(s3b.KVCache, 2, 4, 16, 2, 64, device="cpu")
+    refuses(engine.cache_write, cache, k.cpu(), k, slots)
+    refuses(engine.cache_write, cache, k, k, slots.cpu())
+    refuses(engine.cache_read, cache, slots, None, k.cpu())
+    refuses(engine.cache_attention, cache, q.cpu(), out, pages, lens, 0.1)
+    refuses(engine.cache_attention, cache, q, out.cpu(), pages, lens, 0.1)
+    refuses(engine.cache_attention, cache, q, out, pages.cpu(), lens, 0.1)
+    refuses(engine.cache_attention, cache, q, out, pages, lens.cpu(), 0.1)
+    refuses(engine.cache_attention, cache, q, out, pages, lens, 0.1, lse=torch.empty(1, 1, 4))
     for scale in (0.0, -1.0, math.inf, math.nan):
         refuses(engine.cache_attention, cache, q, out, pages, lens, scale)
     refuses(engine.cache_attention, cache, q, out, pages, lens, 0.1, window=4)
