@@ -68,17 +68,6 @@ __device__ __forceinline__ void floats8(const Eight<__half>& r, float (&x)[8]) {
     x[2 * e] = f.x, x[2 * e + 1] = f.y;
   }
 }
-__device__ __forceinline__ void store8(float* at, const float (&x)[8]) {
-  reinterpret_cast<float4*>(at)[0] = make_float4(x[0], x[1], x[2], x[3]);
-  reinterpret_cast<float4*>(at)[1] = make_float4(x[4], x[5], x[6], x[7]);
-}
-__device__ __forceinline__ void store8(__half* at, const float (&x)[8]) {
-  __half2 h[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
-  *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(h);
-}
-
 __device__ __forceinline__ float max3n(float a, float b, float c) {  // a NaN among them stays
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -103,9 +92,18 @@ __device__ __forceinline__ void block_range(const float (&x)[8], float* hi, floa
 
 constexpr uint32_t kWhole = 0x4B000000u;  // 2^23 as f32
 
+// x / N rounded to nearest: 1 / N as the sum of two floats, a product with each (Brisebarre, Muller and Raina, Accelerating
+// correctly rounded floating-point division when the divisor is known in advance). Holds for every significand with N = 15
+// and 127 (all 2^23 compared) where nothing is subnormal: far below, the scale is 0 in f16 and the codes mean nothing.
+template <int N>
+__device__ __forceinline__ float over(float x) {
+  constexpr float hi = 1.0f / N, lo = (float)(1.0 / N - (double)hi);
+  return __fmaf_rn(x, hi, __fmul_rn(x, lo));
+}
+
 // Quantises the block of 32 values that four neighbouring lanes hold, 8 each (t: which 8), in the steps of
 // quantize_row_host, each rounded to f32 as there. The codes come out as kWhole + code (q8_0: code + 128): truncation of
-// a value >= 0 is the addition of 2^23 rounded to zero.
+// a value >= 0 is the addition of 2^23 rounded to zero. A 4-bit code may still be 16 here: pack_nibbles takes it to 15.
 template <int QT>
 __device__ __forceinline__ void quantise8(float (&x)[8], int t, uint32_t (&code)[8], __half& scale, __half& low) {
   float hi, lo;
@@ -118,10 +116,10 @@ __device__ __forceinline__ void quantise8(float (&x)[8], int t, uint32_t (&code)
   low = __ushort_as_half(0);
   float d;
   if (QT == QT_Q4_1) {
-    d = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
+    d = over<15>(__fsub_rn(hi, lo));
     low = __float2half_rn(lo);
   } else if (QT == QT_Q8_0) {
-    d = __fdiv_rn(fmaxf(hi, -lo), 127.0f);
+    d = over<127>(fmaxf(hi, -lo));
   } else {
     float v = hi > -lo ? hi : lo;
     if (__any_sync(~0u, hi == -lo && hi != 0.f)) {  // the first of the two
@@ -143,7 +141,7 @@ __device__ __forceinline__ void quantise8(float (&x)[8], int t, uint32_t (&code)
     }
     d = v * -0.125f;
   }
-  const float id = d != 0.f ? __fdiv_rn(1.0f, d) : 0.f;
+  const float id = d != 0.f ? __frcp_rn(d) : 0.f;
   scale = __float2half_rn(d);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -154,22 +152,27 @@ __device__ __forceinline__ void quantise8(float (&x)[8], int t, uint32_t (&code)
     } else {
       const float y = QT == QT_Q4_0 ? __fadd_rn(__fmul_rn(x[e], id), 8.5f)
                                     : __fadd_rn(__fmul_rn(__fsub_rn(x[e], lo), id), 0.5f);
-      code[e] = min(__float_as_uint(__fadd_rz(y, 8388608.f)), kWhole + 15u);
+      code[e] = __float_as_uint(__fadd_rz(y, 8388608.f));
     }
   }
 }
 
-// sum of code[i] << shift(i) of n codes less what their kWhole adds (all in 32 bits)
-template <int N, int S0, int S1>
-__device__ __forceinline__ uint32_t pack_codes(const uint32_t* code) {
-  uint32_t w = 0, off = 0;
+// four 8-bit codes as bytes
+__device__ __forceinline__ uint32_t pack_bytes(const uint32_t* c) {
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+}
+// eight 4-bit codes, no more than 15 each: those of pair e at bits 4 e and 16 + 4 e. A pair is values 2 e, 2 e + 1 (keys) or
+// e, e + 4 (values).
+template <bool APART>
+__device__ __forceinline__ uint32_t pack_nibbles(const uint32_t (&c)[8]) {
+  uint32_t w = 0;
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const int shift = (e >> 1) * S0 + (e & 1) * S1;
-    w += code[e] << shift;
-    off += kWhole << shift;
+  for (int e = 0; e < 4; ++e) {
+    uint32_t pair = __byte_perm(APART ? c[e] : c[2 * e], APART ? c[e + 4] : c[2 * e + 1], 0x5410);
+    asm("min.u16x2 %0, %1, %2;" : "=r"(pair) : "r"(pair), "r"(0x000F000Fu));
+    w += pair << (4 * e);
   }
-  return w - off;
+  return w;
 }
 
 // Four lanes a block of 32 values, 8 each: rows are read in 16-byte pieces, and the 8 values of a lane are a whole word of
@@ -186,7 +189,7 @@ __global__ void __launch_bounds__(256) write_kernel(const __grid_constant__ Job 
   uint8_t* base = j.c.data + head * 2 * j.v_bytes;
   const T* k = reinterpret_cast<const T*>(j.r.k) + head * j.r.k_h + c8 * 8;
   const T* v = reinterpret_cast<const T*>(j.r.v) + head * j.r.v_h + c8 * 8;
-  Eight<T> raw[2][2];
+  Eight<T> raw[2][2] = {};
   long long slot[2];
   auto load = [&](long long i0) {
 #pragma unroll
@@ -218,18 +221,16 @@ __global__ void __launch_bounds__(256) write_kernel(const __grid_constant__ Job 
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        // the lanes of a skipped token go along, with zeros: the lanes of a block exchange values
+        // the lanes of a skipped token go along: the lanes of a block exchange values
         float x[8];
         uint32_t c[8];
         __half scale, low;
         floats8(now[u][kv], x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = use[u] ? x[e] : 0.f;
         quantise8<QT>(x, t, c, scale, low);
         if (!use[u]) continue;
         uint8_t* gp = base + at[u] + kv * j.v_bytes;
         if (L::kBits == 8) {
-          const uint32_t w0 = pack_codes<4, 16, 8>(c), w1 = pack_codes<4, 16, 8>(c + 4);
+          const uint32_t w0 = pack_bytes(c), w1 = pack_bytes(c + 4);
           if (kv == 0) {
             *reinterpret_cast<uint2*>(gp + L::k_val(tok[u], b, t)) = make_uint2(w0, w1);
           } else {
@@ -237,9 +238,9 @@ __global__ void __launch_bounds__(256) write_kernel(const __grid_constant__ Job 
             *reinterpret_cast<uint32_t*>(gp + L::v_val(tok[u], b, 2 * t + 1)) = w1;
           }
         } else if (kv == 0) {
-          *reinterpret_cast<uint32_t*>(gp + L::k_val(tok[u], b, t)) = pack_codes<8, 4, 16>(c);
+          *reinterpret_cast<uint32_t*>(gp + L::k_val(tok[u], b, t)) = pack_nibbles<false>(c);
         } else {
-          const uint32_t w = pack_codes<8, 8, 4>(c);
+          const uint32_t w = pack_nibbles<true>(c);
           *reinterpret_cast<uint16_t*>(gp + L::v_val(tok[u], b, 2 * t)) = (uint16_t)w;
           *reinterpret_cast<uint16_t*>(gp + L::v_val(tok[u], b, 2 * t + 1)) = (uint16_t)(w >> 16);
         }
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Job j
     for (int kv = 0; kv < 2; ++kv) {
       T* out = reinterpret_cast<T*>(kv ? j.r.v : j.r.k);
       if (!out) continue;
-      // codes as exact f16 pairs, then one f32 multiply-add: the product is exact, so one rounding (and one to f16)
+      // codes as exact f16 pairs, then one multiply-add in the output's type, rounded once: scales and minima are f16
       uint32_t p[4];
       if (L::kBits == 8) {
         byte_pairs(w[u][kv][0], p[0], p[1]);
@@ -308,16 +309,29 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Job j
       } else {
         nibble_pairs<QT>(w[u][kv][0], p);
       }
-      const float s = __half2float(sc[u][kv]), m = __half2float(low[u][kv]);
-      float x[8];
+      T* to = out + i * (kv ? j.r.v_n : j.r.k_n) + head * (kv ? j.r.v_h : j.r.k_h) + c8 * 8;
+      constexpr bool kWide = sizeof(T) == 4;
+      const bool apart = L::kBits == 4 && kv;  // a value word pairs values e and e + 4
+      if (kWide) {
+        const float s = __half2float(sc[u][kv]), m = __half2float(low[u][kv]);
+        float x[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = __half22float2(u32_h2(p[e]));
-        const bool apart = L::kBits == 4 && kv;  // a value word pairs values e and e + 4
-        x[apart ? e : 2 * e] = fmaf(f.x, s, m);
-        x[apart ? e + 4 : 2 * e + 1] = fmaf(f.y, s, m);
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = __half22float2(u32_h2(p[e]));
+          x[apart ? e : 2 * e] = fmaf(f.x, s, m);
+          x[apart ? e + 4 : 2 * e + 1] = fmaf(f.y, s, m);
+        }
+        reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(to)[1] = make_float4(x[4], x[5], x[6], x[7]);
+      } else {
+        const __half2 s = __half2half2(sc[u][kv]), m = __half2half2(low[u][kv]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = h2_u32(__hfma2(u32_h2(p[e]), s, m));
+        *reinterpret_cast<uint4*>(to) =
+            apart ? make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410),
+                               __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632))
+                  : make_uint4(p[0], p[1], p[2], p[3]);
       }
-      store8(out + i * (kv ? j.r.v_n : j.r.k_n) + head * (kv ? j.r.v_h : j.r.k_h) + c8 * 8, x);
     }
   }
 }
