@@ -5,17 +5,27 @@
 // one for each CTA (one per SM): uneven lengths, causal diagonals and few long units all fill the GPU. A unit that
 // several CTAs share leaves unnormalised parts in the workspace, which join_kernel adds up in the order of the shares.
 //
-// Roles (20 warps, 24 for D = 256):
-//   warps 0, 1     one thread each issues the MMAs of query tile 0 / 1: S = Q K^T (128 x 128 x D) into TMEM, then
-//                  O += P V (128 x D x 128) with P read from TMEM
-//   softmax        one warpgroup per query tile, a thread per query row with its 128 scores in registers: running
-//                  reference maximum (moved only when a row's maximum passes it by 2^8), p = 2^(s - m) written as f16
-//                  over the scores, sum in f32; at a unit's end O / sum to the output
-//   warp 2         copies the cache in block form (bulk copies of the keys or values of 16 tokens) into a ring
-//   dequantising   the remaining warps turn that ring's contents into f16 operands in a ring of 16 KB slots in the
-//                  128-byte swizzle, item by item (K or V of 128 tokens); they also load Q
+// Roles. The f16 operands come from the cache in one of two ways (tc_plan): staged by stage_kernel as images of the 16 KB
+// slots before this kernel runs, or made by warps of this kernel.
+//   warps 0, 1     issue the MMAs of query tile 0 / 1 (the warp waits together, one elected lane issues): S = Q K^T into
+//                  TMEM, then O += P V with P read from TMEM
+//   warp 2         staged: copies slot images and Q into the ring, slot by slot. Else: copies the cache in block form (64
+//                  tokens of keys or values an entry, as few copies as the pages allow) into a second ring
+//   warp 3         allocates TMEM
+//   softmax        one warpgroup per query tile, a thread per query row: running reference maximum (moved only when a row's
+//                  maximum passes it by 2^8), p = 2^(s - m) written as f16 over the scores, sum in f32; at a unit's end
+//                  O / sum to the output
+//   dequantising   not staged: 8 warps (16 at D = 256) turn the block form into slots in the 128-byte swizzle, item by item
+//                  (K or V of 128 tokens); they also load Q
 // Every query tile has two S regions, so S of the next tokens runs beside the softmax of these: 64 tokens a region for D =
 // 64 and 128 (two query tiles and their O fill TMEM), 128 for D = 256 (one tile: O takes half of TMEM).
+//
+// Rounded to f16: the operands of the two products (a value of the cache once, the weight once). Sums, maxima and O are f32.
+//
+// Measured, staged: 4096 rows over 28736 tokens, one head of 256: 137 us in all, of which this kernel 106 (tensor pipe 70% of
+// the cycles active; what is left is the chain S, softmax, P V of the only tile that fits). 4 x 2048 causal queries over 3 to
+// 8 thousand tokens, 16 heads on 4, d = 128: 346 us, 905 TFLOP/s (tensor pipe 53%, exponentials 54% of the MUFU's rate: the
+// two take turns on shared memory and TMEM ports). d = 64: 615 TFLOP/s, where the exponentials are twice as many a FLOP.
 //
 // The f16 operand is code * scale (+ minimum) rounded once. The 16 tokens of a group stand in the order
 // 0 1 8 9 2 3 10 11 4 5 12 13 6 7 14 15 (both in K's rows and V's columns; a softmax does not mind), which is the order
@@ -112,7 +122,8 @@ struct Tc {
   static constexpr int kRegsIssue = 72;
   static constexpr int kRegsSoft = 120;
   static constexpr int kRegsDeq = D == 256 ? 72 : 80;
-  static_assert(STAGED || kRegsIssue + kTQ * kRegsSoft + 2 * kTeams * kRegsDeq <= kThreads / 128 * kRegsLaunch, "register shares");
+  static_assert(STAGED || kRegsIssue + kTQ * kRegsSoft + 2 * kTeams * kRegsDeq <= kThreads / 128 * kRegsLaunch,
+                "register shares");
   static constexpr int kPart = kTQ * kTile * (D + 2);       // floats of a unit's part
 };
 
@@ -535,6 +546,17 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
     }
   }
   __syncthreads();
+  // row blocks that see no token
+  for (int k = blockIdx.x; k < pairs; k += gridDim.x) {
+    if (pair_tiles(k)) continue;
+    const int b = k / a.blocks, row0 = (k - b * a.blocks) * ROWS;
+    for (int h = 0; h < p.c.heads; ++h)
+      for (int e = threadIdx.x; e < min(ROWS, n_rows - row0) * (D / 4); e += C::kThreads) {
+        const int r = row0 + e / (D / 4), i = r / group, hq = h * group + r % group;
+        store_out(p, b * p.o_b + i * p.o_n + hq * p.o_h + e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+        if (p.lse && e % (D / 4) == 0) p.lse[((long long)b * p.nq + i) * p.heads + hq] = -INFINITY;
+      }
+  }
   Walk& w = s_walk[warp];
   if (lane == 0) {
     w.pos = p0;
@@ -562,19 +584,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
 
   if (warp < 4) {
     if (!STAGED) regs_dec<C::kRegsIssue>();
-    if (warp == 3) {
-      // row blocks that see no token
-      for (int k = blockIdx.x; k < pairs; k += gridDim.x) {
-        if (pair_tiles(k)) continue;
-        const int b = k / a.blocks, row0 = (k - b * a.blocks) * ROWS;
-        for (int h = 0; h < p.c.heads; ++h)
-          for (int e = lane; e < min(ROWS, n_rows - row0) * (D / 4); e += 32) {
-            const int r = row0 + e / (D / 4), i = r / group, hq = h * group + r % group;
-            store_out(p, b * p.o_b + i * p.o_n + hq * p.o_h + e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-            if (p.lse && e % (D / 4) == 0) p.lse[((long long)b * p.nq + i) * p.heads + hq] = -INFINITY;
-          }
-      }
-    } else if (warp == 2 && STAGED) {
+    if (warp == 2 && STAGED) {
       // ---- copies of the staged operands, slot by slot
       if (lane == 0) {
         // stage_kernel has written them. Every CTA waits, also one without work: no call may end before its stage_kernel.
@@ -1085,7 +1095,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArg
 
 // The f16 operands of tiles_kernel, once for all its CTAs: block (x < kv_blocks) the K or the V item of one token tile of
 // one sequence and head, a warp for each 16 tokens; the blocks after them the Q rows of one tile. Bound by HBM and L2: the
-// cache read once, 4 bytes written per value pair of K and V.
+// cache read once, 4 bytes written per value pair. Rows and tokens outside every span are left as they are.
 template <int QT, int D>
 __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ TcArgs a, int kv_blocks, int* err) {
   typedef KvL<QT, D> L;
@@ -1097,6 +1107,8 @@ __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ TcAr
   if ((int)blockIdx.x >= kv_blocks) {
     const int x = blockIdx.x - kv_blocks, tile = x % (a.blocks * TQ), unit = x / (a.blocks * TQ);
     const int head = unit % p.c.heads, b = unit / p.c.heads;
+    int lo, hi;
+    if (!unit_tiles<kTile>(p, group, sequence_length(p, b, err), tile, &lo, &hi)) return;  // rows that see no token
     uint8_t* to = a.q_image + (long long)x * (kTile * D * 2);
     for (int e = threadIdx.x; e < kTile * (D / 8); e += 256) {
       const int rr = e / (D / 8), c16 = e % (D / 8), r = tile * kTile + rr;
@@ -1142,9 +1154,13 @@ __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ TcAr
   }
 }
 
-// Whether the operands are staged as f16 first: where several row blocks of a unit would each dequantise the whole cache
-// again, and the images fit a bounded workspace. With one block (at most 256 rows, 128 at D = 256) the kernel that
-// dequantises for itself moves an eighth of the bytes.
+// Whether the operands are staged as f16 first. Each row block of a unit would dequantise the whole cache again; staged, it
+// is done once, at the cost of 4 bytes written and read for each value pair. Measured for 8 sequences, fused / staged:
+//   d = 64,  8192 tokens, 16 heads on 4, 1, 2, 3 blocks of 256 rows: 71 / 73, 99 / 93, 128 / 115 us
+//   d = 128, the same:                                               91 / 101, 122 / 126, 158 / 154 us
+//   d = 256, 16384 tokens, 1 head, 3, 4, 5 blocks of 128 rows:       111 / 119, 127 / 138, 142 / 144 us
+// and with many blocks 198 / 151 us (4096 rows over 28736 tokens, d = 256) and 417 / 362 (4 x 2048 causal queries, d = 128)
+// when staging came in. The images have to fit a bounded workspace.
 constexpr long long kStageMost = 1LL << 30;
 struct TcPlan {
   int tq;
@@ -1159,7 +1175,7 @@ TcPlan tc_plan(const KvAttnParams& p) {
   const long long units = (long long)p.batch * p.c.heads;
   t.kv_bytes = units * t.tiles * p.c.d * 512;
   t.q_bytes = units * t.blocks * t.tq * kTile * p.c.d * 2;
-  t.staged = t.blocks >= 2 && t.tiles > 0 && units < (1 << 24) && t.tiles < (1 << 24) &&
+  t.staged = t.blocks >= (p.c.d == 256 ? 6 : p.c.d == 128 ? 3 : 2) && t.tiles > 0 && units < (1 << 24) && t.tiles < (1 << 24) &&
              t.kv_bytes + t.q_bytes <= kStageMost;
   return t;
 }
@@ -1167,8 +1183,8 @@ size_t part_floats(int sms, int tq, int d) { return (size_t)2 * sms * tq * kTile
 
 template <typename K, typename... A>
 int launch_dependent(K* kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
-  // may begin while its predecessor still runs and waits for the predecessor's end before it reads its results: 142 -> 137 us
-  // (4096 rows over 28736 tokens, d = 256), 353 -> 346 (4 x 2048 causal queries, 16 heads on 4, d = 128), 232 -> 224 (d = 64)
+  // may begin while its predecessor still runs and waits for the predecessor's end before it reads its results: 142 -> 137
+  // us (4096 rows over 28736 tokens, d = 256), 353 -> 346 (4 x 2048 causal queries, 16 heads on 4, d = 128)
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
