@@ -562,7 +562,8 @@ int64_t s3b_kv_cache_bytes(int type, int heads, int d, int page_size, int64_t n_
  * S3B_F32), token i and head h at k + i * k_n + h * k_h (elements, each row of
  * d contiguous; pointers and strides multiples of 16 bytes); slots[i] (device)
  * is the token's slot, < 0 skips the token. Two tokens of one call must not
- * share a slot. The codes are those of s3b_quantize_rows bit for bit. Values
+ * share a slot. Scales and codes are those of s3b_quantize_rows bit for bit (but
+ * for the codes of a block whose scale is 0 in f16, which mean nothing). Values
  * beyond +-65024 (infinities too) are held to it and a NaN counts as 0, so that
  * no row of the cache can hold one: a token that a mask hides cannot reach
  * another row's result. A slot past the end is skipped, and the next s3b_sync

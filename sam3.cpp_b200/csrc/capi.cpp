@@ -42,6 +42,9 @@ int read_dev_err(s3b_ctx* ctx) {
   if (h != 0) {
     // cleared in the context stream's order, so no later kernel's code can be wiped by it
     cudaMemsetAsync(ctx->d_err, 0, sizeof(int), ctx->stream);
+    // blocks that gave up may have left the cache attention's counts unfinished
+    const auto count = ctx->ws.find("kv_attn_count");
+    if (count != ctx->ws.end() && count->second->bytes) cudaMemsetAsync(count->second->p, 0, count->second->bytes, ctx->stream);
     cudaStreamSynchronize(ctx->stream);
     if (h == kDevErrIndex)
       return set_error(ctx, kErrDevice, "a slot, page or length in device memory is out of range (code %d)", h);
@@ -1502,7 +1505,7 @@ int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* 
   }
   rc = kv_attention(p, w, ctx->d_err, ctx->stream);
   if (rc) return set_error(ctx, launcher_status_code(rc), "cache_attention launch failed (%d)", rc);
-  count_launch(ctx, count_bytes ? 1 : 2);
+  count_launch(ctx, kv_attention_launches(p));
   return kOk;
 }
 

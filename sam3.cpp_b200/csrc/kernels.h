@@ -400,8 +400,10 @@ struct KvAttnWork {
 };
 void kv_attention_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes);
 int kv_attention(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st);
+int kv_attention_launches(const KvAttnParams& p);  // kernels that the call launches
 // The tensor-core kernel for tiles of 128 query rows (kv_attention picks it for more rows than its own kernel takes).
 void kv_attention_tc_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes);
 int kv_attention_tc(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st);
+int kv_attention_tc_launches(const KvAttnParams& p);
 
 }  // namespace s3b

@@ -735,6 +735,10 @@ void kv_attention_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_
   *count_bytes = (size_t)p.batch * p.c.heads * 4;
 }
 
+int kv_attention_launches(const KvAttnParams& p) {
+  return p.nq * (long long)(p.heads / p.c.heads) > most_rows(p.c.d) ? kv_attention_tc_launches(p) : 1;
+}
+
 int kv_attention(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
   if (p.nq * (long long)(p.heads / p.c.heads) > most_rows(p.c.d)) return kv_attention_tc(p, w, err, st);
   return p.c.type == QT_Q4_0 ? attend_d<QT_Q4_0>(p, w, err, st)

@@ -1247,6 +1247,8 @@ void kv_attention_tc_work(const KvAttnParams& p, int sms, size_t* part_bytes, si
   *count_bytes = 0;
 }
 
+int kv_attention_tc_launches(const KvAttnParams& p) { return tc_plan(p).staged ? 3 : 2; }
+
 int kv_attention_tc(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
   return p.c.type == QT_Q4_0 ? launch_tiles_d<QT_Q4_0>(p, w, err, st)
                              : p.c.type == QT_Q4_1 ? launch_tiles_d<QT_Q4_1>(p, w, err, st)
