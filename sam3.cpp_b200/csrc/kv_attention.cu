@@ -135,6 +135,8 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
     fence_mbar_init();
     fence_proxy_async_smem();
   }
+  let_next();
+  wait_before();
   // total chunks, then the sequence in which this CTA's share begins
   if (warp == 0) {
     long long total = 0;
@@ -690,8 +692,7 @@ int launch_rows(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream
   a.p = p;
   a.part = w.part;
   a.count = w.count;
-  k<<<C::kCtas * w.sms, 32 * W, C::kSmem, st>>>(a, err);
-  return cudaGetLastError() == cudaSuccess ? 0 : -12;
+  return launch_dependent(k, dim3(C::kCtas * w.sms), 32 * W, C::kSmem, st, a, err);
 }
 
 // ---------------------------------------------------------------- dispatch

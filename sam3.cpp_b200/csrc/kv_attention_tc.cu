@@ -489,6 +489,9 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
     tmem_relinquish();
   }
 
+  // staged: the predecessor is stage_kernel, which lets this kernel in after its own wait; only the copies wait for its end
+  if (!STAGED) wait_before();
+
   // ---- tiles of one head, by the warps' shares of the (sequence, row block) pairs; then the pair in which the share begins
   constexpr int kWarps = C::kThreads / 32;
   const int per_warp = (pairs + kWarps - 1) / kWarps;
@@ -588,7 +591,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
       // ---- copies of the staged operands, slot by slot
       if (lane == 0) {
         // stage_kernel has written them. Every CTA waits, also one without work: no call may end before its stage_kernel.
-        asm volatile("griddepcontrol.wait;" ::: "memory");
+        wait_before();
         uint32_t slot = 0, q_n = 0;
         bool ok = true;
         while (ok && walk_next<ROWS>(p, a.blocks, err, &w)) {
@@ -1025,7 +1028,7 @@ template <int D, int TQ>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArgs a) {
   constexpr int kPart = TQ * kTile * (D + 2), kMost = 160;
   __shared__ float s_f[kMost][32], s_top[8][32], s_sum[8][32];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_before();
   const int c0 = blockIdx.x;
   const Shared u = a.shared[c0];
   if (!u.valid) return;
@@ -1100,7 +1103,8 @@ template <int QT, int D>
 __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ TcArgs a, int kv_blocks, int* err) {
   typedef KvL<QT, D> L;
   constexpr int TQ = D == 256 ? 1 : 2;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  wait_before();
+  let_next();
   const KvAttnParams& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = p.heads / p.c.heads;
@@ -1181,23 +1185,6 @@ TcPlan tc_plan(const KvAttnParams& p) {
 }
 size_t part_floats(int sms, int tq, int d) { return (size_t)2 * sms * tq * kTile * (d + 2); }
 
-template <typename K, typename... A>
-int launch_dependent(K* kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
-  // may begin while its predecessor still runs and waits for the predecessor's end before it reads its results: 142 -> 137
-  // us (4096 rows over 28736 tokens, d = 256), 353 -> 346 (4 x 2048 causal queries, 16 heads on 4, d = 128)
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? 0 : -12;
-}
-
 template <int QT, int D>
 int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
   constexpr int TQ = D == 256 ? 1 : 2;
@@ -1218,15 +1205,14 @@ int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStrea
     if (kernel_setup(k, C::kSmem) <= 0) return -13;
     const long long kv_blocks = 2LL * p.batch * p.c.heads * t.tiles;
     const long long q_blocks = (long long)p.batch * p.c.heads * t.blocks * TQ;
-    stage_kernel<QT, D><<<(unsigned)(kv_blocks + q_blocks), 256, 0, st>>>(a, (int)kv_blocks, err);
-    if (cudaGetLastError() != cudaSuccess) return -12;
+    rc = launch_dependent(stage_kernel<QT, D>, dim3((unsigned)(kv_blocks + q_blocks)), 256, 0, st, a, (int)kv_blocks, err);
+    if (rc) return rc;
     rc = launch_dependent(k, dim3(w.sms), C::kThreads, C::kSmem, st, a, err);
   } else {
     typedef Tc<QT, D, false> C;
     auto* k = tiles_kernel<QT, D, false>;
     if (kernel_setup(k, C::kSmem) <= 0) return -13;
-    k<<<w.sms, C::kThreads, C::kSmem, st>>>(a, err);
-    rc = cudaGetLastError() == cudaSuccess ? 0 : -12;
+    rc = launch_dependent(k, dim3(w.sms), C::kThreads, C::kSmem, st, a, err);
   }
   if (rc) return rc;
   return launch_dependent(join_kernel<D, TQ>, dim3(w.sms, TQ * 4), 256, 0, st, a);

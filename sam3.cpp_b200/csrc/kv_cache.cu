@@ -206,6 +206,8 @@ __global__ void __launch_bounds__(256) write_kernel(const __grid_constant__ Job 
       }
     }
   };
+  let_next();
+  wait_before();
   long long i0 = (long long)(blockIdx.x / j.c.heads) * j.tokens;
   load(i0 + threadIdx.x / kLanes);
   for (; i0 < j.n; i0 += step) {
@@ -270,6 +272,8 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Job j
   const uint8_t* base = j.c.data + head * 2 * j.v_bytes;
   uint32_t w[2][2][2];
   __half sc[2][2], low[2][2];
+  let_next();
+  wait_before();
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const long long i = first + u * kRows;
@@ -372,8 +376,7 @@ int launch(bool write, const KvCache& c, const KvRows& r, const long long* slots
   const JobKernel k = c.type == QT_Q4_0 ? job_kernel_d<QT_Q4_0>(c.d, write, r.f32)
                       : c.type == QT_Q4_1 ? job_kernel_d<QT_Q4_1>(c.d, write, r.f32)
                                           : job_kernel_d<QT_Q8_0>(c.d, write, r.f32);
-  k<<<(unsigned)blocks, 256, 0, st>>>(j);
-  return cudaGetLastError() == cudaSuccess ? 0 : -12;
+  return launch_dependent(k, dim3((unsigned)blocks), 256, 0, st, j);
 }
 
 }  // namespace
