@@ -1022,12 +1022,15 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
   }
 }
 
-// Joins the parts of the units that several CTAs of tiles_kernel share: block (c, y) the rows 32 y .. 32 y + 31 of the unit
-// that begins in CTA c's share, if one does. HBM / L2 traffic only: each part is read once.
+// Joins the parts of the units that several CTAs of tiles_kernel share: block (c, y, z) the columns 64 z .. 64 z + 63 of rows
+// 32 y .. 32 y + 31 of the unit that begins in CTA c's share, if one does. A lane is a row, as in the parts (512 bytes of
+// 32 rows side by side), a warp 8 columns; the outputs turn in shared memory. L2 and latency bound it: each part is read
+// once, by enough blocks to cover the waits.
 template <int D, int TQ>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArgs a) {
   constexpr int kPart = TQ * kTile * (D + 2), kMost = 160;
-  __shared__ float s_f[kMost][32], s_top[8][32], s_sum[8][32];
+  __shared__ float s_f[kMost][32], s_top[8][32], s_sum[8][32], s_inv[32];
+  __shared__ float4 s_v[32][17];
   wait_before();
   const int c0 = blockIdx.x;
   const Shared u = a.shared[c0];
@@ -1037,13 +1040,13 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArg
   const int tile = blockIdx.y >> 2, row0 = (blockIdx.y & 3) * 32;
   if (u.row0 + tile * kTile + row0 >= n_rows) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = u.c1 - c0 + 1;
+  const int n = u.c1 - c0 + 1, at = row0 + lane;
   auto part_of = [&](int k) -> const float* {
-    return a.part + (2 * (long long)(c0 + k) + (k == 0 ? u.second : 0)) * kPart + tile * (kTile * (D + 2));
+    return a.part + (2 * (long long)(c0 + k) + (k == 0 ? u.second : 0)) * kPart + tile * (kTile * (D + 2)) + at;
   };
-  // factors of the parts, lane = row
+  // factors of the parts
   float top = kNoScore;
-  for (int k = warp; k < n; k += 8) top = fmaxf(top, s_f[k][lane] = __ldcg(part_of(k) + kTile * D + row0 + lane));
+  for (int k = warp; k < n; k += 8) top = fmaxf(top, s_f[k][lane] = __ldcg(part_of(k) + kTile * D));
   s_top[warp][lane] = top;
   __syncthreads();
 #pragma unroll
@@ -1052,48 +1055,48 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArg
   for (int k = warp; k < n; k += 8) {
     const float f = ex2_approx(s_f[k][lane] - top);
     s_f[k][lane] = f;
-    sum = fmaf(__ldcg(part_of(k) + kTile * (D + 1) + row0 + lane), f, sum);
+    sum = fmaf(__ldcg(part_of(k) + kTile * (D + 1)), f, sum);
   }
   s_sum[warp][lane] = sum;
   __syncthreads();
-  if (warp == 0 && p.lse) {
+  const int first = u.row0 + tile * kTile + row0;  // row of lane 0
+  if (warp == 0) {
     sum = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum += s_sum[k][lane];
-    const int r = u.row0 + tile * kTile + row0 + lane;
-    if (r < n_rows)
+    s_inv[lane] = sum == 0.f ? 0.f : 1.f / sum;
+    const int r = first + lane;
+    if (p.lse && blockIdx.z == 0 && r < n_rows)
       p.lse[((long long)u.b * p.nq + r / group) * p.heads + u.head * group + r % group] =
           sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
   }
-  // warp w: rows 4 w .. 4 w + 3; lane: one row, every eighth float4 of it
-  const int rr = 4 * warp + (lane >> 3), r = u.row0 + tile * kTile + row0 + rr;
-  float total = 0.f;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) total += s_sum[k][rr];
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  float4 v[D / 32];
-#pragma unroll
-  for (int x = 0; x < D / 32; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
+  float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 4
   for (int k = 0; k < n; ++k) {
-    const float4* from = reinterpret_cast<const float4*>(part_of(k)) + (lane & 7) * kTile + row0 + rr;
-    const float f = s_f[k][rr];
-    float4 x[D / 32];
+    // float4 x of the parts' row: [D / 4][128 rows]
+    const float4* from = reinterpret_cast<const float4*>(part_of(k) - at) + (blockIdx.z * 16 + 2 * warp) * kTile + at;
+    const float f = s_f[k][lane];
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) x[e] = __ldcg(from + 8 * e * kTile);
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) {
-      v[e].x = fmaf(x[e].x, f, v[e].x);
-      v[e].y = fmaf(x[e].y, f, v[e].y);
-      v[e].z = fmaf(x[e].z, f, v[e].z);
-      v[e].w = fmaf(x[e].w, f, v[e].w);
+    for (int e = 0; e < 2; ++e) {
+      const float4 x = __ldcg(from + e * kTile);
+      v[e].x = fmaf(x.x, f, v[e].x);
+      v[e].y = fmaf(x.y, f, v[e].y);
+      v[e].z = fmaf(x.z, f, v[e].z);
+      v[e].w = fmaf(x.w, f, v[e].w);
     }
   }
-  if (r >= n_rows) return;
-  const long long at = u.b * p.o_b + r / group * p.o_n + (u.head * group + r % group) * p.o_h + (lane & 7) * 4;
+  s_v[lane][2 * warp] = v[0];
+  s_v[lane][2 * warp + 1] = v[1];
+  __syncthreads();
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e)
-    store_out(p, at + 32 * e, make_float4(v[e].x * inv, v[e].y * inv, v[e].z * inv, v[e].w * inv));
+  for (int e = threadIdx.x; e < 32 * 16; e += 256) {
+    const int rr = e >> 4, r = first + rr;
+    if (r >= n_rows) break;
+    const float4 x = s_v[rr][e & 15];
+    const float inv = s_inv[rr];
+    store_out(p, u.b * p.o_b + r / group * p.o_n + (u.head * group + r % group) * p.o_h + blockIdx.z * 64 + (e & 15) * 4,
+              make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+  }
 }
 
 // The f16 operands of tiles_kernel, once for all its CTAs: block (x < kv_blocks) the K or the V item of one token tile of
@@ -1215,7 +1218,7 @@ int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStrea
     rc = launch_dependent(k, dim3(w.sms), C::kThreads, C::kSmem, st, a, err);
   }
   if (rc) return rc;
-  return launch_dependent(join_kernel<D, TQ>, dim3(w.sms, TQ * 4), 256, 0, st, a);
+  return launch_dependent(join_kernel<D, TQ>, dim3(w.sms, TQ * 4, D / 64), 256, 0, st, a);
 }
 
 template <int QT>
