@@ -106,13 +106,17 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
   constexpr float kBias = QT == QT_Q8_0 ? 4.f : 0.f;  // weights are 2^kBias at the reference: their products with the
                                                        // block scales then use f16's range as the values would
   constexpr float kLazy = 2.9f;                        // and stay below f16's largest: 2^(kBias + 2.9) * scale < 65504
+  // Units of at most so many chunks stay whole where there is a block for each: two or three more chunks for a block cost less
+  // than joining parts (8 heads of 128, 2 chunks each: 10.3 us cut, 9.5 whole; 8 of 256, 3 chunks: 16.4, 14.3; 4 of 64, 3 chunks:
+  // 9.3, 8.7; but 8 of 128, 3 chunks: 10.7, 11.6, and 4 chunks 10.9, 13.7).
+  constexpr int kWhole = 3;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* s_q = smem + C::kMain;
   float* s_m = reinterpret_cast<float*>(s_q + C::kQBytes);  // [W][rows]
   float* s_l = s_m + W * C::kRows;
   float* s_f = s_l + W * C::kRows;
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_f + W * C::kRows);
-  __shared__ long long s_total, s_base;
+  __shared__ long long s_total, s_ctas, s_base, s_p0, s_p1;
   __shared__ int s_b, s_abort_word, s_last;
   volatile int* s_abort = &s_abort_word;
   static_assert(W * NS * 8 <= 1024, "barriers of rows_kernel");
@@ -137,19 +141,32 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
   }
   let_next();
   wait_before();
-  // total chunks, then the sequence in which this CTA's share begins
+  // total chunks, this CTA's share of them and the sequence in which it begins
   if (warp == 0) {
     long long total = 0;
-    int g0, g1;
-    for (int b = lane; b < p.batch; b += 32) total += chunks_of(b, &g0, &g1);
+    int most = 0, g0, g1;
+    for (int b = lane; b < p.batch; b += 32) {
+      const int n = chunks_of(b, &g0, &g1);
+      total += n;
+      most = max(most, n);
+    }
 #pragma unroll
     for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(~0u, total, x);
+    most = __reduce_max_sync(~0u, most);
     total *= p.c.heads;
-    const long long ctas = min((long long)gridDim.x, total);
-    const long long first = ctas ? total * blockIdx.x / ctas : 0;
-    long long base = 0;
+    long long ctas = min((long long)gridDim.x, total), base = 0, p0 = 0, p1 = 0;
     int found = -1;
-    if ((int)blockIdx.x < ctas) {
+    if (most <= kWhole && (long long)p.batch * p.c.heads <= gridDim.x) {
+      const int b = blockIdx.x / p.c.heads;
+      if (b < p.batch) {
+        const int n = chunks_of(b, &g0, &g1);
+        found = b;
+        p0 = (blockIdx.x - b * p.c.heads) * n;
+        p1 = p0 + n;
+      }
+    } else if ((int)blockIdx.x < ctas) {
+      p0 = total * blockIdx.x / ctas;
+      p1 = total * (blockIdx.x + 1) / ctas;
       for (int b0 = 0; b0 < p.batch && found < 0; b0 += 32) {
         const long long n = b0 + lane < p.batch ? (long long)chunks_of(b0 + lane, &g0, &g1) * p.c.heads : 0;
         long long end = n;
@@ -158,7 +175,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
           const long long up = __shfl_up_sync(~0u, end, x);
           if (lane >= x) end += up;
         }
-        const uint32_t past = __ballot_sync(~0u, base + end > first);
+        const uint32_t past = __ballot_sync(~0u, base + end > p0);
         if (past) {
           const int who = __ffs(past) - 1;
           found = b0 + who;
@@ -170,13 +187,14 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
     }
     if (lane == 0) {
       s_total = total;
+      s_ctas = ctas;
       s_base = base;
+      s_p0 = p0;
+      s_p1 = p1;
       s_b = found;
     }
   }
   __syncthreads();
-  const long long total = s_total;
-  const long long ctas = min((long long)gridDim.x, total);
 
   // sequences of which no query sees a token
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
@@ -188,9 +206,9 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
       if (p.lse && e % (D / 4) == 0) p.lse[((long long)b * p.nq + i) * p.heads + h] = -INFINITY;
     }
   }
-  if ((int)blockIdx.x >= ctas) return;
+  const long long p0 = s_p0, p1 = s_p1, total = s_total, ctas = s_ctas;
+  if (p0 >= p1) return;
 
-  const long long p0 = total * blockIdx.x / ctas, p1 = total * (blockIdx.x + 1) / ctas;
   const float sl2 = p.scale * kLog2e;
   const long long v_offset = (long long)per_page * L::kHalf;  // of a page's values from its keys
   uint8_t* ring = smem + warp * NS * C::kStageBytes;
