@@ -10,8 +10,8 @@
 // to f16 is the weight (as every f16 product of this kind does; sums of weights are f32 of the unrounded ones) and weight
 // times scale: the output is off by 3.5e-4 of its norm, where rounding it to f16 alone costs 2.1e-4.
 //
-// Measured: 32 sequences of 1384 to 16384 tokens, 32 heads on 8, d = 128, q4_0: 319 MB in 82 us, 3.9 TB/s of the 6.5 that a
-// copy reaches; one sequence of 524288 tokens, 16 heads on 2, q4_1: 168 MB in 53 us. Instruction issue bounds it (61% of
+// Measured: 32 sequences of 1384 to 16384 tokens, 32 heads on 8, d = 128, q4_0: 319 MB in 80 us, 4.0 TB/s of the 6.5 that a
+// copy reaches; one sequence of 524288 tokens, 16 heads on 2, q4_1: 168 MB in 51 us. Instruction issue bounds it (61% of
 // the cycles issue, the integer pipe is half busy): some 340 instructions for 16 tokens of a head, most of them unpacking
 // codes and scaling partial scores and weights.
 #include <algorithm>
@@ -65,7 +65,9 @@ __device__ __forceinline__ void lds(const uint8_t* at, uint32_t (&r)[BYTES / 4])
 // spreads over all of them. In a share each warp takes every W-th group: its own ring of bulk copies, its own running
 // maximum, sum and output (no barrier in the loop); the W states are joined in shared memory at the end of a unit's
 // part. A unit that several CTAs share leaves its parts in the workspace and the last CTA to arrive joins them in the
-// order of the shares, so the result does not depend on who that is.
+// order of the shares, so the result does not depend on who that is. (A kernel of its own for the joins took 16 us instead of
+// 24 for 8 sequences of 4096 tokens, 16 rows of 256, but 73 instead of 67 for 256 sequences of 100 to 1000 tokens, 32 heads on
+// 8, whose few parts are joined beside other blocks' work here.)
 template <int QT, int D, int NT, int W>
 struct Rows {
   typedef KvL<QT, D> L;

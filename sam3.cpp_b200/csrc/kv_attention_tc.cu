@@ -22,9 +22,9 @@
 //
 // Rounded to f16: the operands of the two products (a value of the cache once, the weight once). Sums, maxima and O are f32.
 //
-// Measured, staged: 4096 rows over 28736 tokens, one head of 256: 137 us in all, of which this kernel 106 (tensor pipe 70% of
+// Measured, staged: 4096 rows over 28736 tokens, one head of 256: 120 us in all, of which this kernel 100 (tensor pipe 70% of
 // the cycles active; what is left is the chain S, softmax, P V of the only tile that fits). 4 x 2048 causal queries over 3 to
-// 8 thousand tokens, 16 heads on 4, d = 128: 346 us, 905 TFLOP/s (tensor pipe 53%, exponentials 54% of the MUFU's rate: the
+// 8 thousand tokens, 16 heads on 4, d = 128: 342 us, 916 TFLOP/s (tensor pipe 53%, exponentials 54% of the MUFU's rate: the
 // two take turns on shared memory and TMEM ports). d = 64: 615 TFLOP/s, where the exponentials are twice as many a FLOP.
 //
 // The f16 operand is code * scale (+ minimum) rounded once. The 16 tokens of a group stand in the order
@@ -1025,7 +1025,8 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
 // Joins the parts of the units that several CTAs of tiles_kernel share: block (c, y, z) the columns 64 z .. 64 z + 63 of rows
 // 32 y .. 32 y + 31 of the unit that begins in CTA c's share, if one does. A lane is a row, as in the parts (512 bytes of
 // 32 rows side by side), a warp 8 columns; the outputs turn in shared memory. L2 and latency bound it: each part is read
-// once, by enough blocks to cover the waits.
+// once, by enough blocks to cover the waits (25 us with 64-byte pieces and a block for all columns, 10 now, both with the
+// parts out of L2: 148 shares, 20 MB).
 template <int D, int TQ>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArgs a) {
   constexpr int kPart = TQ * kTile * (D + 2), kMost = 160;
