@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
         auto locate = [&](int j) -> long long {
           const int gi = (t0 + j) * 8 + (lane & 7);
           if (j >= cb || gi < g_lo || gi >= g_hi) return -1;
-          long long page = __ldg(table + gi / per_page);
+          long long page = table[gi / per_page];
           if (page < 0 || page >= p.c.n_pages) {
             atomicCAS(err, 0, kDevErrIndex);
             page = 0;
@@ -952,7 +952,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
         uint4 v = make_uint4(0, 0, 0, 0);
         if (r < n_rows) {
           const int i = r / group, h = w.u.head * group + r % group;
-          v = __ldg(reinterpret_cast<const uint4*>(p.q + w.u.b * p.q_b + i * p.q_n + h * p.q_h + c16 * 8));
+          v = *reinterpret_cast<const uint4*>(p.q + w.u.b * p.q_b + i * p.q_n + h * p.q_h + c16 * 8);
         }
         *reinterpret_cast<uint4*>(s_q + rr / kTile * (kTile * D * 2) + c16 / 8 * kSlotBytes + rr % kTile * 128 +
                                   ((c16 & 7) ^ (rr & 7)) * 16) = v;
@@ -1122,8 +1122,7 @@ __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ TcAr
       const int rr = e / (D / 8), c16 = e % (D / 8), r = tile * kTile + rr;
       uint4 v = make_uint4(0, 0, 0, 0);
       if (r < p.nq * group)
-        v = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_b + r / group * p.q_n +
-                                                 (head * group + r % group) * p.q_h + c16 * 8));
+        v = *reinterpret_cast<const uint4*>(p.q + b * p.q_b + r / group * p.q_n + (head * group + r % group) * p.q_h + c16 * 8);
       *reinterpret_cast<uint4*>(to + c16 / 8 * kSlotBytes + rr * 128 + ((c16 & 7) ^ (rr & 7)) * 16) = v;
     }
     return;
@@ -1140,7 +1139,7 @@ __global__ void __launch_bounds__(256) stage_kernel(const __grid_constant__ TcAr
   // tokens outside the span: their keys may hold anything, their values become zero
   const bool live = first < hi && first + 16 > lo;
   const int gi = live ? first >> 4 : max(lo, tok0) >> 4;
-  long long page = __ldg(p.pages + b * p.pages_stride + gi / per_page);
+  long long page = p.pages[b * p.pages_stride + gi / per_page];
   if (page < 0 || page >= p.c.n_pages) {
     atomicCAS(err, 0, kDevErrIndex);
     page = 0;

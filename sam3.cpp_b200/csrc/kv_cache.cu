@@ -53,7 +53,7 @@ struct Eight {
 template <typename T>
 __device__ __forceinline__ void load8(const T* at, Eight<T>& r) {
 #pragma unroll
-  for (int e = 0; e < (int)sizeof(T) / 2; ++e) r.w[e] = __ldg(reinterpret_cast<const uint4*>(at) + e);
+  for (int e = 0; e < (int)sizeof(T) / 2; ++e) r.w[e] = reinterpret_cast<const uint4*>(at)[e];
 }
 __device__ __forceinline__ void floats8(const Eight<float>& r, float (&x)[8]) {
   const uint32_t w[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w, r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(256) write_kernel(const __grid_constant__ Job 
       const long long i = i0 + u * kRows;
       slot[u] = -1;
       if (i < j.n) {
-        slot[u] = __ldg(j.slots + i);
+        slot[u] = j.slots[i];
         load8(k + i * j.r.k_n, raw[u][0]);
         load8(v + i * j.r.v_n, raw[u][1]);
       }
@@ -274,32 +274,36 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Job j
   __half sc[2][2], low[2][2];
   let_next();
   wait_before();
+  long long slot[2], at[2];
+  int tok[2];
+  bool use[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) slot[u] = first + u * kRows < j.n ? j.slots[first + u * kRows] : -1;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) use[u] = slot_place<L::kHalf>(j, slot[u], &at[u], &tok[u]);
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const long long i = first + u * kRows;
-    long long at;
-    int tok;
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {  // of a skipped slot: zeros
       w[u][kv][0] = w[u][kv][1] = L::kBits == 8 ? 0x80808080u : 0x88888888u;
       sc[u][kv] = low[u][kv] = __ushort_as_half(0);
     }
-    if (i < j.n && slot_place<L::kHalf>(j, __ldg(j.slots + i), &at, &tok)) {
-      const uint8_t *kp = base + at, *vp = kp + j.v_bytes;
+    if (use[u]) {
+      const uint8_t *kp = base + at[u], *vp = kp + j.v_bytes;
       if (L::kBits == 8) {
-        const uint2 k = __ldg(reinterpret_cast<const uint2*>(kp + L::k_val(tok, b, t)));
+        const uint2 k = *reinterpret_cast<const uint2*>(kp + L::k_val(tok[u], b, t));
         w[u][0][0] = k.x, w[u][0][1] = k.y;
-        w[u][1][0] = __ldg(reinterpret_cast<const uint32_t*>(vp + L::v_val(tok, b, 2 * t)));
-        w[u][1][1] = __ldg(reinterpret_cast<const uint32_t*>(vp + L::v_val(tok, b, 2 * t + 1)));
+        w[u][1][0] = *reinterpret_cast<const uint32_t*>(vp + L::v_val(tok[u], b, 2 * t));
+        w[u][1][1] = *reinterpret_cast<const uint32_t*>(vp + L::v_val(tok[u], b, 2 * t + 1));
       } else {
-        w[u][0][0] = __ldg(reinterpret_cast<const uint32_t*>(kp + L::k_val(tok, b, t)));
-        w[u][1][0] = __byte_perm(__ldg(reinterpret_cast<const uint16_t*>(vp + L::v_val(tok, b, 2 * t))),
-                                 __ldg(reinterpret_cast<const uint16_t*>(vp + L::v_val(tok, b, 2 * t + 1))), 0x5410);
+        w[u][0][0] = *reinterpret_cast<const uint32_t*>(kp + L::k_val(tok[u], b, t));
+        w[u][1][0] = __byte_perm(*reinterpret_cast<const uint16_t*>(vp + L::v_val(tok[u], b, 2 * t)),
+                                 *reinterpret_cast<const uint16_t*>(vp + L::v_val(tok[u], b, 2 * t + 1)), 0x5410);
       }
-      const __half* ks = reinterpret_cast<const __half*>(kp + L::k_scale(tok, b));
-      const __half* vs = reinterpret_cast<const __half*>(vp + L::v_scale(tok, b));
-      sc[u][0] = __ldg(ks), sc[u][1] = __ldg(vs);
-      if (QT == QT_Q4_1) low[u][0] = __ldg(ks + L::kSc / 2), low[u][1] = __ldg(vs + L::kSc / 2);
+      const __half* ks = reinterpret_cast<const __half*>(kp + L::k_scale(tok[u], b));
+      const __half* vs = reinterpret_cast<const __half*>(vp + L::v_scale(tok[u], b));
+      sc[u][0] = *ks, sc[u][1] = *vs;
+      if (QT == QT_Q4_1) low[u][0] = ks[L::kSc / 2], low[u][1] = vs[L::kSc / 2];
     }
   }
 #pragma unroll

@@ -1,0 +1,85 @@
+"""The quantised key / value cache's kernels in a stream: each may take its place while its predecessor runs, so what one writes
+and the next reads is tested without a wait of the host between them."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("qtype,d,dtype", [(2, 128, torch.float16), (3, 256, torch.float16), (8, 64, torch.float32)])
+def test_calls_see_what_their_predecessors_wrote(s3b, engine, qtype, d, dtype):
+    """Read, overwrite the same slots, read, attend with few and with many rows, over and over, the calls back to back: every
+    result has to be, bit for bit, that of the same calls with a sync after each."""
+    g = torch.Generator(device="cuda").manual_seed(d)
+    n, heads, page, rounds = 3000, 2, 16, 12
+    cache = s3b.KVCache(qtype, 200, page, heads, d)
+    table = torch.randperm(200, device="cuda", generator=g).to(torch.int32)[None, :188].contiguous()
+    at = torch.arange(n, device="cuda")
+    slots = table[0].long()[at // page] * page + at % page
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    rows = [[torch.randn(n, heads, d, device="cuda", generator=g).to(dtype) for _ in "kv"] for _ in range(rounds)]
+    queries = [torch.randn(1, nq, 4, d, device="cuda", generator=g).half() for nq in (1, 300)]
+
+    def new(count, *shape):
+        return [torch.full(shape, 3.0, device="cuda", dtype=torch.float16) for _ in range(count)]
+
+    def go(wait):
+        cache.data.zero_()
+        outs = [new(4, n, heads, d) + [torch.empty_like(q) for q in queries] + [torch.empty_like(queries[0])] for _ in rows]
+        torch.cuda.synchronize()
+        for (k, v), (k0, v0, k1, v1, few, many, fed) in zip(rows, outs):
+            for call in (lambda: engine.cache_read(cache, slots, k0, v0),
+                         lambda: engine.cache_write(cache, k, v, slots),
+                         lambda: engine.cache_read(cache, slots, k1, v1),
+                         lambda: engine.cache_attention(cache, queries[0], few, table, lens, d ** -0.5),
+                         lambda: engine.cache_attention(cache, queries[1], many, table, lens, d ** -0.5),
+                         # a query that the call before has written
+                         lambda: engine.cache_attention(cache, few, fed, table, lens, d ** -0.5)):
+                call()
+                if wait:
+                    engine.sync()
+        engine.sync()
+        return outs
+
+    waited, queued = go(True), go(False)
+    for i, (a, b) in enumerate(zip(waited, queued)):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y), i
+    # each round reads first what the round before wrote, then its own
+    for before, after in zip(queued, queued[1:]):
+        assert torch.equal(before[2], after[0]) and torch.equal(before[3], after[1])
+        assert not torch.equal(after[0], after[2])
+
+
+def test_calls_see_indexes_made_on_the_device(s3b, engine):
+    """Slots, page table, lengths and rows of a call come from kernels just before it."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    d, page, pages = 64, 16, 40
+    cache = s3b.KVCache(8, pages, page, 1, d)
+    n = pages * page
+    got = []
+    for wait in (True, False):
+        cache.data.zero_()
+        g.manual_seed(7)
+        outs = []
+        for i in range(8):
+            table = torch.randperm(pages, device="cuda", generator=g).to(torch.int32)[None]
+            at = torch.arange(n, device="cuda")
+            slots = table[0].long()[at // page] * page + at % page
+            k, v = (torch.randn(n, 1, d, device="cuda", generator=g) for _ in "kv")
+            q = torch.randn(1, 1 + 140 * (i % 2), 1, d, device="cuda", generator=g).half()
+            lens = torch.full((1,), n - i, dtype=torch.int32, device="cuda")
+            out = torch.empty_like(q)
+            if wait:
+                engine.sync()
+            engine.cache_write(cache, k, v, slots)
+            if wait:
+                engine.sync()
+            engine.cache_attention(cache, q, out, table, lens, 0.125)
+            if wait:
+                engine.sync()
+            outs.append(out)
+        engine.sync()
+        got.append(outs)
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
