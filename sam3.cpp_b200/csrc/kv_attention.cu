@@ -278,6 +278,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
       // ---- query fragments: column g of tile nt is row 8 nt + g; block n's values 8 t .. 8 t + 7
       uint32_t qf[C::kQSmem ? 1 : NT * NB][4];
       uint32_t qmin[NT][2];  // q4_1: sums of the query over blocks 2t, 2t + 1, as f16 and f16 remainder
+      float q_sum[NT][2], q_most = 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int r = 8 * nt + g;
@@ -306,11 +307,20 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
             if (n == 2 * t + 1) hi = sum;
           }
         }
+        q_sum[nt][0] = lo;
+        q_sum[nt][1] = hi;
+        q_most = fmaxf(q_most, fmaxf(fabsf(lo), fabsf(hi)));
+      }
+      // 32 queries of one sign may sum to more than an f16 holds: a unit that has such a sum takes them all less 2^6
+      const bool q_large = QT == QT_Q4_1 && __any_sync(~0u, q_most >= 32768.f);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
         if (QT == QT_Q4_1) {
+          const float f = q_large ? 0.015625f : 1.f, lo = q_sum[nt][0] * f, hi = q_sum[nt][1] * f;
           const __half2 s = __floats2half2_rn(lo, hi);
-          const float2 f = __half22float2(s);
+          const float2 x = __half22float2(s);
           qmin[nt][0] = h2_u32(s);
-          qmin[nt][1] = h2_u32(__floats2half2_rn(lo - f.x, hi - f.y));
+          qmin[nt][1] = h2_u32(__floats2half2_rn(lo - x.x, hi - x.y));
         }
       }
       if (C::kQSmem) __syncthreads();
@@ -360,6 +370,12 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma16816(s[nt], am, qmin[nt][0], qmin[nt][1]);
+            if (q_large) {
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nt][e] *= 64.f;
+            }
           }
 #pragma unroll
           for (int sb = 0; sb < D / L::kSB; ++sb) {

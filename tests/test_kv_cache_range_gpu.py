@@ -1,0 +1,97 @@
+"""Attention over the quantised cache where magnitudes, counts and lengths go to their ends, against 64-bit arithmetic on the
+values that the cache holds.
+
+What is rounded to fewer than 32 bits, u = 2^-11 relative each at most: with few query rows the weight, its product with
+the block scale and an f16 output; with many the keys, the values, the weight and an f16 output. Each rounding is off by
+u / sqrt(3) at most in the mean square. So the error's norm over a whole output is below sqrt(3) u / sqrt(3) = u with few
+rows, and where the keys' roundings move the scores by no more than u / sqrt(3) (scores of deviation 1) below 1.16 u with many,
+which the bounds below take with a quarter added: NORM[few], NORM[many]. An element alone is off by (2 u) sum p |v| + u |out| at
+most with few rows."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -11
+NORM = {True: 1.25 * U, False: 1.45 * U}
+
+
+def most_few(d):
+    """Rows of a key / value head up to which the call counts as one of few rows."""
+    return 16 if d == 256 else 32
+
+
+def attend(s3b, engine, qtype, q, k, v, lengths, page=64, scale=None, causal=False, window=0, out_dtype=torch.float32):
+    """Attention of q f16 [batch, nq, heads, d] over the caches of k, v [batch, n, kv heads, d] in pages of a shuffled table:
+    the output, lse, and the keys and values held (f32)."""
+    batch, n, kv, d = k.shape
+    per = -(-n // page)
+    cache = s3b.KVCache(qtype, batch * per, page, kv, d)
+    cache.data.fill_(0xFF)
+    g = torch.Generator(device="cuda").manual_seed(n)
+    pages = torch.randperm(batch * per, device="cuda", generator=g).to(torch.int32).view(batch, per)
+    at = torch.arange(n, device="cuda")
+    held = []
+    for b in range(batch):
+        m = lengths[b]
+        slots = pages[b].long()[at[:m] // page] * page + at[:m] % page
+        engine.cache_write(cache, k[b, :m], v[b, :m], slots)
+        rows = [torch.empty(m, kv, d, device="cuda") for _ in "kv"]
+        engine.cache_read(cache, slots, *rows)
+        held.append(rows)
+    out = torch.empty(q.shape, device="cuda", dtype=out_dtype)
+    lse = torch.empty(q.shape[:3], device="cuda")
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    engine.cache_attention(cache, q, out, pages, lens, d ** -0.5 if scale is None else scale, causal=causal, window=window, lse=lse)
+    engine.sync()
+    return out, lse, held
+
+
+def exact(q, held, scale, causal=False, window=0):
+    """Attention of one sequence's q [nq, heads, d] over the values held in 64 bits: output, lse, sum p |v|."""
+    k, v = (t.double() for t in held)
+    nq, heads, d = q.shape
+    n, kv, _ = k.shape
+    group = heads // kv
+    hi = torch.arange(nq, device="cuda")[:, None] + (n - nq + 1) if causal else torch.full((nq, 1), n, device="cuda")
+    at = torch.arange(n, device="cuda")
+    hide = (at >= hi) | ((at < hi - window) if window else False)
+    out, lse, size = (torch.zeros(nq, heads, m, device="cuda", dtype=torch.float64) for m in (d, 1, d))
+    for h in range(heads):
+        s = (q[:, h].double() @ k[:, h // group].T * scale).masked_fill(hide, -math.inf)
+        lse[:, h, 0] = s.logsumexp(-1)
+        p = s.softmax(-1).nan_to_num(0.0)
+        out[:, h] = p @ v[:, h // group]
+        size[:, h] = p @ v[:, h // group].abs()
+    return out, lse[..., 0], size
+
+
+def off(x, y):
+    return ((x.double() - y).norm() / y.norm()).item()
+
+
+@pytest.mark.parametrize("qtype", [2, 3, 8])
+@pytest.mark.parametrize("d,nq,group", [(64, 1, 1), (128, 1, 4), (128, 5, 4), (64, 8, 4), (256, 1, 2), (256, 5, 3), (128, 70, 2)])
+def test_large_queries(s3b, engine, qtype, d, nq, group):
+    """Queries of 2047 to 60000 and of one sign: 32 of them sum past f16's largest. The scale brings the scores back to a
+    deviation of about 1, where f32 sums over d products keep them to 2^-20."""
+    g = torch.Generator(device="cuda").manual_seed(d + nq)
+    n, kv = 700, 2
+    k, v = (torch.randn(1, n, kv, d, device="cuda", generator=g) for _ in "kv")
+    q = 4096 + 2000 * torch.rand(1, nq, kv * group, d, device="cuda", generator=g)
+    q[:, :, ::2] *= -1
+    q[:, :, -1] *= 9.8
+    q = q.half()
+    scale = 1.0 / (5000 * math.sqrt(d))
+    q[:, :, 0] = torch.randn(nq, d, device="cuda", generator=g).half()  # a small row beside large ones
+    out, lse, held = attend(s3b, engine, qtype, q, k, v, [n], page=48, scale=scale)
+    ref, ref_lse, _ = exact(q[0], held[0], scale)
+    few = nq * group <= most_few(d)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    # the last head's scores deviate by about 10: with many rows the keys' roundings move them by as much more
+    heads = slice(None) if few else slice(0, -1)
+    assert off(out[0][:, heads], ref[:, heads]) < NORM[few]
+    if few:
+        assert (lse[0] - ref_lse).abs().max() < 1e-3
