@@ -113,6 +113,12 @@ struct Tc {
   static constexpr int kUnitBytes = kUnit / 16 * L::kHalf;
   static constexpr int kRawFit = (224 * 1024 - 1024 - kQBytes - kSlots * kSlotBytes - 512) / kUnitBytes;
   static constexpr int kRaw = STAGED ? 0 : kRawFit > 8 ? 8 : kRawFit;  // entries of the block-form ring
+  // An item takes two entries, tokens 0 .. 63 and 64 .. 127, and a warp reads one of them. In an odd ring it would meet a barrier
+  // in every other phase only, and its wait, which knows the phases' parity alone, could pass while the load before the one it
+  // waits for is still on its way. There each warp waits for both entries and gives both back. In an even ring the halves keep
+  // their entries: a warp that always reads the same half meets every phase, and with two teams (K by tokens, V by team) the
+  // slots of an item come free only when the item two before it has been read whole, which lies behind the entries' last use.
+  static constexpr bool kBoth = kRaw & 1;
   static constexpr int kSmem = 1024 + kQBytes + kSlots * kSlotBytes + kRaw * kUnitBytes + 512;
   static_assert(STAGED || kRaw >= 3, "K of a tile takes two entries of tiles_kernel's ring, and one has to be on its way");
   static constexpr int kOCol = 256;                         // TMEM: two S regions of kSub columns a tile, then O
@@ -478,7 +484,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
     }
     for (int x = 0; x < C::kRaw; ++x) {
       mbar_init(&raw_full[x], 1);
-      mbar_init(&raw_empty[x], C::kDeqWarps / 2);  // each warp reads one of an item's two entries
+      mbar_init(&raw_empty[x], C::kBoth ? C::kDeqWarps : C::kDeqWarps / 2);
     }
     s_abort_word = 0;
     fence_mbar_init();
@@ -969,14 +975,23 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
         // this warp's 16 tokens of the tile and its super-blocks of them
         const int grp = C::kTeams == 1 || is_k ? tw : 4 * team + (tw & 3);
         const int sb0 = C::kTeams == 1 ? 0 : (is_k ? team : tw >> 2) * C::kTasks;
-        int e = raw0 + (grp >> 2);
-        uint32_t ph = raw_phase;
+        int e = raw0 + (grp >> 2), other = raw0 + 1 - (grp >> 2);
+        uint32_t ph = raw_phase, other_ph = raw_phase;
         if (e >= C::kRaw) {
           e -= C::kRaw;
           ph ^= 1;
         }
+        if (other >= C::kRaw) {
+          other -= C::kRaw;
+          other_ph ^= 1;
+        }
         const uint32_t slot_i = slot % kSlots, slot_ph = ((slot / kSlots) & 1) ^ 1;
         bool got = mbar_wait(&raw_full[e], ph, s_abort, err, kErrWaitFull);
+        if (C::kBoth) {
+          got = got && mbar_wait(&raw_full[other], other_ph, s_abort, err, kErrWaitFull);
+          __syncwarp();
+          if (got && lane == 0) mbar_arrive(&raw_empty[other]);
+        }
 #pragma unroll
         for (int y = 0; y < C::kTeamSlots; ++y)  // side by side: the slots of an item never wrap
           got = got && mbar_wait(&empty[slot_i + y], slot_ph, s_abort, err, kErrWaitEmpty);

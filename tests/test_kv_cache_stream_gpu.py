@@ -83,3 +83,34 @@ def test_calls_see_indexes_made_on_the_device(s3b, engine):
         got.append(outs)
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("qtype,d,heads,kv,nq", [(8, 256, 1, 1, 30), (8, 256, 2, 1, 300), (8, 128, 8, 2, 40), (8, 128, 2, 2, 130),
+                                                 (3, 256, 2, 2, 60), (2, 128, 4, 1, 64)])
+def test_many_rows_while_the_cache_arrives_unevenly(s3b, engine, qtype, d, heads, kv, nq):
+    """Pages of 16 tokens spread over 2 GiB of memory that this call touches for the first time since another buffer was cleared,
+    so that the copies of a tile's halves land apart and out of order: every repetition has to give the same, and what the same
+    tokens give from a small cache in order."""
+    g = torch.Generator(device="cuda").manual_seed(d)
+    n, page = 20000, 16
+    at = torch.arange(n, device="cuda")
+    k, v = (torch.randn(n, kv, d, device="cuda", generator=g).half() for _ in "kv")
+    q = torch.randn(1, nq, heads, d, device="cuda", generator=g).half()
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    outs = []
+    for total in (n // page, (2 << 30) // s3b.kv_cache_bytes(qtype, kv, d, page, 1)):
+        cache = s3b.KVCache(qtype, total, page, kv, d, data=torch.full((s3b.kv_cache_bytes(qtype, kv, d, page, total),), 0xFF,
+                                                                       dtype=torch.uint8, device="cuda"))
+        table = torch.arange(total, device="cuda") if not outs else torch.randperm(total, device="cuda", generator=g)
+        table = table[:n // page].to(torch.int32)[None].contiguous()
+        engine.cache_write(cache, k, v, table[0].long()[at // page] * page + at % page)
+        for _ in range(1 if not outs else 12):
+            flush.zero_()
+            out = torch.empty_like(q)
+            engine.cache_attention(cache, q, out, table, lens, d ** -0.5)
+            outs.append(out)
+        engine.sync()
+    assert torch.isfinite(outs[0]).all()
+    for out in outs[1:]:
+        assert torch.equal(out, outs[0])
