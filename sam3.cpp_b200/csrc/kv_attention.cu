@@ -8,7 +8,8 @@
 // its column. Codes enter the products as exact small integers; a block's scale multiplies the 32-value partial score in
 // f32 (keys), or the weight before it is rounded to f16 (values), so no dequantised value is ever formed. What is rounded
 // to f16 is the weight (as every f16 product of this kind does; sums of weights are f32 of the unrounded ones) and weight
-// times scale: the output is off by 3.5e-4 of its norm, where rounding it to f16 alone costs 2.1e-4.
+// times scale: the output is off by 3.5e-4 of its norm, where rounding it to f16 alone costs 2.1e-4, for values of any size
+// (ScaleRange keeps both in f16's normal range).
 //
 // Measured: 32 sequences of 1384 to 16384 tokens, 32 heads on 8, d = 128, q4_0: 319 MB in 80 us, 4.0 TB/s of the 6.5 that a
 // copy reaches; one sequence of 524288 tokens, 16 heads on 2, q4_1: 168 MB in 51 us. Instruction issue bounds it (61% of
@@ -59,6 +60,54 @@ __device__ __forceinline__ void lds(const uint8_t* at, uint32_t (&r)[BYTES / 4])
   }
 }
 
+// ---------------------------------------------------------------- range of the values' scales
+// A weight w and its product w * scale are f16, and scales reach from 2^-24 to 2^13. So that neither of the two passes f16's
+// largest, and both keep their digits for tokens far below the maximum whatever the size of the values:
+//   weights are 2^kBias at the reference (and up to 2^(kBias + 2.9));
+//   for each of the D / 32 blocks of a row a warp holds a bound 2^A on the scales that it has met (A only grows). Where A
+//   lies outside kLow .. kHigh, the block's scales and minima are multiplied by 2^lift, lift = kHigh - A, in shared memory before
+//   their use, and its outputs by 2^-lift at the end.
+// A product then goes below f16's normal range (2^-14) for tokens whose weight is 2^-17 of the largest or less, and to zero
+// below 2^-28. The zone without a lift holds values (largest of a block) from 1/16 to 64 in q4_0, 1/8 to 120 in q8_0.
+// Lane i holds the state of block i % (2 NB) / 2, whose scales it reads.
+template <int QT, int NB>
+struct ScaleRange {
+  static constexpr int kBias = QT == QT_Q8_0 ? 13 : 10;
+  static constexpr int kHigh = 13 - kBias, kLow = kHigh - 8;
+  uint32_t limit = 0, limit_min = 0;  // 2^A as f16 twice, the same for the minima; 0: everything passes it
+  bool lifted = false;                // any block of the warp
+  __device__ __forceinline__ bool passed(uint32_t x, bool minima) const {
+    return !__hblt2(__habs2(u32_h2(x)), u32_h2(minima ? limit_min : limit));
+  }
+  __device__ __forceinline__ int lift() const {
+    const int a = (int)(limit >> 26) - 15;
+    return a < kLow || a > kHigh ? min(kHigh - a, 15) : 0;
+  }
+  __device__ __forceinline__ uint32_t factor() const { return (uint32_t)(15 + lift()) * 0x04000400u; }
+  __device__ __forceinline__ float lowered() const { return __int_as_float((127 - lift()) << 23); }
+  // Takes in the largest scale and minimum (f16 bits) that this lane has seen of a step; returns the factor on its block's
+  // outputs so far that comes of it. The whole warp.
+  __device__ __forceinline__ float raise(uint32_t most, uint32_t most_min) {
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      if (x > 1 && x < 2 * NB) continue;
+      most = max(most, __shfl_xor_sync(~0u, most, x));
+      if (QT == QT_Q4_1) most_min = max(most_min, __shfl_xor_sync(~0u, most_min, x));
+    }
+    const int before = lift();
+    if (most >= (limit & 0xFFFF) || (QT == QT_Q4_1 && most_min >= (limit_min & 0xFFFF))) {
+      // twice to four times the largest; where there is a lift, the minima have to be below 2^(A + 4)
+      int a = max(max((int)(limit >> 26) - 15, (int)(most >> 10) - 13), -14);
+      if (QT == QT_Q4_1 && a < kLow) a = max(a, min((int)(most_min >> 10) - 17, kLow));
+      a = min(a, 14);
+      limit = (uint32_t)(15 + a) * 0x04000400u;
+      limit_min = a < kLow ? (uint32_t)(19 + a) * 0x04000400u : 0x7C007C00u;
+    }
+    lifted = __any_sync(~0u, lift() != 0);
+    return __int_as_float((127 + lift() - before) << 23);
+  }
+};
+
 // ---------------------------------------------------------------- few query rows
 // The work is one line of chunks of W groups of 16 tokens, unit after unit (a unit is one sequence and key / value
 // head), cut into equal shares for the CTAs, so sequences of uneven length leave no SM idle and one long sequence
@@ -105,9 +154,9 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
   typedef KvL<QT, D> L;
   typedef Rows<QT, D, NT, W> C;
   constexpr int NB = L::kNB, NS = C::kStages, G = C::kG;
-  constexpr float kBias = QT == QT_Q8_0 ? 4.f : 0.f;  // weights are 2^kBias at the reference: their products with the
-                                                       // block scales then use f16's range as the values would
-  constexpr float kLazy = 2.9f;                        // and stay below f16's largest: 2^(kBias + 2.9) * scale < 65504
+  typedef ScaleRange<QT, NB> Range;
+  constexpr float kBias = Range::kBias;
+  constexpr float kLazy = 2.9f;  // log2 by which a score may pass the reference: 2^(kBias + 2.9) < 65504
   // Units of at most so many chunks stay whole where there is a block for each: two or three more chunks for a block cost less
   // than joining parts (8 heads of 128, 2 chunks each: 10.3 us cut, 9.5 whole; 8 of 256, 3 chunks: 16.4, 14.3; 4 of 64, 3 chunks:
   // 9.3, 8.7; but 8 of 128, 3 chunks: 10.7, 11.6, and 4 chunks 10.9, 13.7).
@@ -122,7 +171,6 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
   __shared__ int s_b, s_abort_word, s_last;
   volatile int* s_abort = &s_abort_word;
   static_assert(W * NS * 8 <= 1024, "barriers of rows_kernel");
-  (void)NB;
 
   const KvAttnParams& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -327,6 +375,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
 
       // ---- state: columns 2t, 2t + 1 of each tile
       float o[NT][D / 16][4], omin[NT][4], m[NT][2], l[NT][2];
+      Range range;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -348,6 +397,30 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
         if (!ok) break;
         const int tok0 = (first + it * (W * G)) * 16;
         const bool whole = tok0 >= max_lo && tok0 + 16 * G <= min_hi;
+
+        // -- scales (and minima) of the values, a word (two tokens) a lane; those of tokens outside the sequence's span, which
+        // may hold anything, become zero
+        uint8_t* v_scales = ring + stage * C::kStageBytes + G * L::kHalf + L::kVal;
+        auto each_scale = [&](auto&& f) {  // f(word, whether of the minima, tokens of the word after tok0)
+#pragma unroll
+          for (int gg = 0; gg < G; ++gg)
+#pragma unroll
+            for (int e0 = 0; e0 < 8 * NB * L::kPlanes; e0 += 32) {
+              const int e = e0 + lane, of = e % (8 * NB);
+              if (8 * NB * L::kPlanes % 32 == 0 || e < 8 * NB * L::kPlanes)
+                f(reinterpret_cast<uint32_t*>(v_scales + gg * L::kHalf) + e, e >= 8 * NB,
+                  16 * gg + of / (2 * NB) * 2 + 8 * (of & 1));
+            }
+        };
+        bool grow = false;
+        if (!whole) {
+          each_scale([&](uint32_t* at, bool, int after) {
+            const int tok = tok0 + after;
+            const uint32_t keep = (tok >= min_lo && tok < max_hi ? 0xFFFFu : 0u) | (tok + 1 >= min_lo && tok + 1 < max_hi ? 0xFFFF0000u : 0u);
+            *at &= keep;
+          });
+        }
+        each_scale([&](uint32_t* at, bool minima, int) { grow |= range.passed(*at, minima); });
 
         // -- scores
         float s_all[G][NT][4];
@@ -417,7 +490,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
         }
 
         // -- weights: the reference maximum of a column moves only when a score passes it by kLazy
-        bool move = false;
+        bool move = grow;
         float top[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -445,6 +518,32 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
           }
         }
         if (__any_sync(~0u, move)) {
+          if (__any_sync(~0u, grow)) {
+            uint32_t most[2] = {0, 0};
+            each_scale([&](uint32_t* at, bool minima, int) {
+              const uint32_t x = *at & 0x7FFF7FFFu;
+              most[minima] = max(most[minima], max(x & 0xFFFF, x >> 16));
+            });
+            const float by = range.raise(most[0], most[1]);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+              const float f = __shfl_sync(~0u, by, 2 * n);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  o[nt][2 * n][e] *= f;
+                  o[nt][2 * n + 1][e] *= f;
+                }
+            }
+            if (QT == QT_Q4_1) {
+              const float f = __shfl_sync(~0u, by, 2 * (g % NB));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) omin[nt][c] *= f;
+            }
+          }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float f[2];
@@ -480,15 +579,12 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
             w1_all[gg][nt] = movmatrix(h2_u32(__floats2half2_rn(e4[2], e4[3])));
           }
 
-        // -- outputs; tokens outside the sequence's span may hold anything, so their scales become zero
-        if (!whole) {
-          for (int gg = 0; gg < G; ++gg) {
-            __half* scales = reinterpret_cast<__half*>(ring + stage * C::kStageBytes + (G + gg) * L::kHalf + L::kVal);
-            for (int e = lane; e < 16 * NB * L::kPlanes; e += 32) {
-              const int lane_t = e % (16 * NB) / (4 * NB), tok = tok0 + 16 * gg + 2 * lane_t + (e & 1) + 4 * (e & 2);
-              if (tok < min_lo || tok >= max_hi) scales[e] = __ushort_as_half(0);
-            }
-          }
+        // -- outputs
+        if (range.lifted) {
+          const __half2 by = u32_h2(range.factor());
+          each_scale([&](uint32_t* at, bool, int) { *at = h2_u32(__hmul2(u32_h2(*at), by)); });
+        }
+        if (!whole || range.lifted) {
           fence_proxy_async_smem();  // the next copy into this stage comes after these writes
           __syncwarp();
         }
@@ -509,11 +605,13 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
               as[0] = s.x;
               as[2] = s.y;
             }
-            const __half2 eight = u32_h2(0x48004800u);  // the weight takes the 8: 8 scale may pass f16's range
+            const __half2 eight = u32_h2(0x48004800u);
+            as[0] = h2_u32(__hmul2(u32_h2(as[0]), eight));  // exact, and below f16's largest: ScaleRange
+            as[2] = h2_u32(__hmul2(u32_h2(as[2]), eight));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               mma16816(omin[nt], am, w0[nt], w1[nt]);
-              mma16816(omin[nt], as, h2_u32(__hmul2(u32_h2(w0[nt]), eight)), h2_u32(__hmul2(u32_h2(w1[nt]), eight)));
+              mma16816(omin[nt], as, w0[nt], w1[nt]);
             }
           }
 #pragma unroll
@@ -595,11 +693,12 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
             mn[0] = __shfl_sync(~0u, omin[nt][0], 4 * n + t);
             mn[1] = __shfl_sync(~0u, omin[nt][1], 4 * n + t);
           }
+          const float lowered = __shfl_sync(~0u, range.lowered(), 2 * n), fo[2] = {f[0] * lowered, f[1] * lowered};
 #pragma unroll
           for (int c = 0; c < 2; ++c)
             *reinterpret_cast<float4*>(s_o + (warp * C::kRows + 8 * nt + 2 * t + c) * C::kOStride + 32 * n + 4 * g) =
-                make_float4((o[nt][2 * n][c] + mn[c]) * f[c], (o[nt][2 * n][c + 2] + mn[c]) * f[c],
-                            (o[nt][2 * n + 1][c] + mn[c]) * f[c], (o[nt][2 * n + 1][c + 2] + mn[c]) * f[c]);
+                make_float4((o[nt][2 * n][c] + mn[c]) * fo[c], (o[nt][2 * n][c + 2] + mn[c]) * fo[c],
+                            (o[nt][2 * n + 1][c] + mn[c]) * fo[c], (o[nt][2 * n + 1][c + 2] + mn[c]) * fo[c]);
         }
       }
       __syncthreads();
