@@ -589,6 +589,7 @@ int s3b_op_cache_read(s3b_ctx* ctx, const s3b_kv_cache* cache, const int64_t* sl
  *        tokens outside the cache)
  *   pages [batch][pages_stride] (device): sequence b's tokens lie in order in
  *        its first ceil(lengths[b] / page_size) pages, of at most max_pages
+ *        (max_pages * page_size at most 2^31 - 8192)
  *   lengths [batch] (device), 0 allowed
  *   causal  query i is the token at position lengths[b] - nq + i and sees no
  *        later one; window > 0 (with causal): only the last `window` positions

@@ -1464,8 +1464,11 @@ int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* 
   if (max_pages > 0 && batch > 1 && pages_stride < max_pages)
     return set_error(ctx, kErrArg, "cache_attention: page table rows of %lld hold no %d pages", (long long)pages_stride,
                      max_pages);
-  if ((long long)max_pages * p.c.page_size > 0x7fffffffLL || (long long)nq * heads > 0x3fffffffLL)
-    return set_error(ctx, kErrUnsupported, "cache_attention: a sequence may hold 2^31 - 1 tokens at most");
+  // token numbers are 32-bit, and the kernels count up to the end of the step that holds the last one
+  if ((long long)max_pages * p.c.page_size > kMaxCacheTokens)
+    return set_error(ctx, kErrUnsupported, "cache_attention: a sequence may hold %lld tokens at most", kMaxCacheTokens);
+  if ((long long)nq * heads > 0x3fffffffLL)
+    return set_error(ctx, kErrUnsupported, "cache_attention: %d queries of %d heads", nq, heads);
   if (!rows_aligned(q, 2, q_b, q_n, q_h) || !rows_aligned(out, out_f32 ? 4 : 2, o_b, o_n, o_h))
     return set_error(ctx, kErrArg, "cache_attention: rows must start on 16-byte boundaries");
   p.q = reinterpret_cast<const __half*>(q);

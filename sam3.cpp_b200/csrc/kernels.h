@@ -356,6 +356,9 @@ int launch_status(const char* what);
 // Device error code of an index in device memory (slot, page, length) that is out of range.
 constexpr int kDevErrIndex = 7;
 
+// Tokens that a sequence's page table may name: 2^31 less some, so that a kernel's last step (512 tokens at most) ends below it.
+constexpr long long kMaxCacheTokens = (1LL << 31) - 8192;
+
 // s3b_kv_cache with its memory; kv_cache_bytes returns its size, or -1 when the fields are not a cache.
 struct KvCache {
   int type = 0, heads = 0, d = 0, page_size = 0;

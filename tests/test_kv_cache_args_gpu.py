@@ -1,0 +1,41 @@
+"""Arguments of the quantised cache's calls at their limits: what is refused before any kernel runs, and what has to be taken."""
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def call(s3b, engine):
+    """s3b_op_cache_attention over a cache of 4 pages of 16 tokens, 2 heads of 64, with one query of 4 heads; arguments by name.
+    Returns the status."""
+    cache = s3b.KVCache(2, 4, 16, 2, 64)
+    k = torch.ones(64, 2, 64, device="cuda")
+    engine.cache_write(cache, k, k, torch.arange(64, device="cuda"))
+    t = dict(q=torch.ones(2, 1, 4, 64, device="cuda", dtype=torch.float16), out=torch.zeros(2, 1, 4, 64, device="cuda"),
+             lse=torch.zeros(2, 1, 4, device="cuda"), pages=torch.arange(8, dtype=torch.int32, device="cuda") % 4,
+             lengths=torch.full((4,), 64, dtype=torch.int32, device="cuda"))
+
+    def go(batch=1, page_size=16, max_pages=4, stride=4, scale=0.125, offset=(), **kw):
+        at = {n: x.data_ptr() + dict(offset).get(n, 0) for n, x in t.items()}
+        desc = s3b.KVCacheDesc(2, 2, 64, page_size, 4 * 16 // page_size if page_size <= 64 else 1, cache.data.data_ptr())
+        return engine._L.s3b_op_cache_attention(engine.h, ctypes.byref(desc), at["q"], 256, 256, 64, at["out"], 1, 256, 256, 64, at["lse"],
+                                                at["pages"], stride, max_pages, at["lengths"], batch, 1, 4, scale, 0, 0)
+    go.tensors = t
+    yield go
+    engine.sync()
+
+
+@pytest.mark.parametrize("page_size,max_pages", [(16, (1 << 27) - 1), (16, (1 << 27) - 511), (64, (1 << 25) - 127), (2 ** 31 - 16, 1)])
+def test_refuses_page_tables_of_too_many_tokens(call, page_size, max_pages):
+    """Past 2^31 - 8192 tokens the kernels' 32-bit token numbers would wrap."""
+    assert call(page_size=page_size, max_pages=max_pages, stride=max_pages) == -6
+
+
+def test_takes_page_tables_of_nearly_2_to_31_tokens(call, engine):
+    """The width of the table alone costs nothing: the length says what is read."""
+    assert call(max_pages=(1 << 27) - 512, stride=1 << 27) == 0
+    engine.sync()
+    assert (call.tensors["out"][0] == 1).all()
