@@ -366,10 +366,13 @@ __device__ __forceinline__ void weigh_scores(const uint32_t (&r)[32], uint32_t a
 
 // One S region (N tokens) of one query row: the row's scores from TMEM at `at`, the lazy reference maximum, the weights as
 // f16 pairs over the first half of the region, the sum into l. MASKED: only tokens [lo, hi) of the region count. Returns
-// true when the maximum moved and the row of O has to be scaled by alpha. 64 scores stay in registers; 128 are read twice,
+// true when a maximum of the warp moved and the rows of O have to be scaled by alpha. any_large: whether the warp has a row
+// with a large reference. 64 scores stay in registers; 128 are read twice,
 // 32 at a time with 32 more on their way, in loops that stay rolled (unrolled, the loop's code was fetched again and again).
+__device__ __forceinline__ bool is_large(float m_ref) { return fabsf(m_ref) > 0x1p20f && m_ref > kNoScore; }
 template <int N, bool MASKED>
-__device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float sl2, float& m_ref, float& l, float& alpha) {
+__device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float sl2, float& m_ref, float& l, float& alpha,
+                                             bool& any_large) {
   uint32_t ra[32], rb[32];
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
   KV_TMEM_LD32(at, ra);
@@ -396,17 +399,32 @@ __device__ __forceinline__ bool softmax_tile(uint32_t at, int lo, int hi, float 
   }
   const float top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * sl2;
   alpha = 1.f;
-  bool moved = false;
-  if (top > m_ref + kLazy) {
-    alpha = ex2_approx(m_ref - top);
-    m_ref = top;
-    l *= alpha;
-    moved = true;
+  const bool moved = __any_sync(~0u, top > m_ref + kLazy);
+  if (moved) {
+    if (top > m_ref + kLazy) {
+      alpha = ex2_approx(m_ref - top);
+      m_ref = top;
+      l *= alpha;
+    }
+    any_large = __any_sync(~0u, is_large(m_ref));
   }
-  __syncwarp();  // the TMEM accesses below take the whole warp together
   const unsigned long long sl2x2 = f2_pack(sl2, sl2), negm2 = f2_pack(-m_ref, -m_ref);
   unsigned long long acc0 = f2_pack(0.f, 0.f), acc1 = acc0;
-  if (N == 64) {
+  // A weight's exponent is score * sl2 - m_ref in one rounding, m_ref the rounded product of another score. The difference that
+  // m_ref's rounding makes is common to a row and cancels, but for scores past 2^31 it leaves the exponent's range: rows of
+  // large scores take the rounded product of each score first.
+  if (any_large) {
+    const float first = is_large(m_ref) ? sl2 : 1.f, then = is_large(m_ref) ? 1.f : sl2;
+#pragma unroll 1
+    for (int c0 = 0; c0 < N; c0 += 32) {
+      KV_TMEM_LD32(at + c0, ra);
+      tc_wait_ld();
+      mask_scores<MASKED>(ra, c0, lo, hi);
+#pragma unroll
+      for (int c = 0; c < 32; ++c) ra[c] = __float_as_uint(__fmul_rn(__uint_as_float(ra[c]), first));
+      weigh_scores(ra, at + c0 / 2, f2_pack(then, then), negm2, acc0, acc1);
+    }
+  } else if (N == 64) {
     weigh_scores(ra, at, sl2x2, negm2, acc0, acc1);
     weigh_scores(rb, at + 16, sl2x2, negm2, acc0, acc1);
   } else {
@@ -835,6 +853,7 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
       row_span(p, w.u.len, min(n_rows - 1, r0 + kTile - 1) / group, &all_lo, &none);
       const int tok_first = (w.u.t0 + w.ca) * kTile, tok_end = (w.u.t0 + w.cb) * kTile;
       float m_ref = kNoScore, l = 0.f;
+      bool any_large = false;
       for (int tok0 = tok_first; tok0 < tok_end; tok0 += C::kSub, ++n) {
         if (!mbar_wait(&s_full[2 * t + (n & 1)], (n >> 1) & 1, s_abort, err, kErrWaitTmemFull)) ok = false;
         ok = __all_sync(~0u, ok);
@@ -844,23 +863,22 @@ __global__ void __launch_bounds__(Tc<QT, D, STAGED>::kThreads, 1) tiles_kernel(c
         float alpha;
         const bool moved =
             tok0 >= all_lo && tok0 + C::kSub <= all_hi
-                ? softmax_tile<C::kSub, false>(s_at, 0, 0, sl2, m_ref, l, alpha)
-                : softmax_tile<C::kSub, true>(s_at, lo - tok0, hi - tok0, sl2, m_ref, l, alpha);
-        if (tok0 > tok_first && __any_sync(~0u, moved)) {
+                ? softmax_tile<C::kSub, false>(s_at, 0, 0, sl2, m_ref, l, alpha, any_large)
+                : softmax_tile<C::kSub, true>(s_at, lo - tok0, hi - tok0, sl2, m_ref, l, alpha, any_large);
+        if (tok0 > tok_first && moved) {
           // O is current once the previous P V product of this tile has completed. The one before it has: S of this
           // region was issued after it, so the barrier cannot be a phase behind.
           if (!mbar_wait(&pv_done[t], (n - 1) & 1, s_abort, err, kErrWaitMisc)) ok = false;
           ok = __all_sync(~0u, ok);
           if (!ok) break;
           tc_fence_after();
-          const float f = moved ? alpha : 1.f;
 #pragma unroll
           for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
             KV_TMEM_LD32(o_at + c, o);
             tc_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
             KV_TMEM_ST32(o_at + c, o);
           }
         }

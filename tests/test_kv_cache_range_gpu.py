@@ -68,6 +68,11 @@ def exact(q, held, scale, causal=False, window=0, keys16=False):
     return out, lse[..., 0]
 
 
+def lse_off(d, score):
+    """How far f32 scores of this size may be off: d / 16 product steps, each kept to 2^-22, the scale and the logarithm."""
+    return (d / 16 + 2) * 2.0 ** -22 * score
+
+
 def off(x, y):
     return ((x.double() - y).norm() / y.norm()).item()
 
@@ -168,3 +173,23 @@ def test_sink_in_each_of_many_sequences(s3b, engine, qtype, d, nq):
         ref, ref_lse = exact(q[b], held[b], 0.125, keys16=not few)
         assert off(out[b], ref) < NORM[few], b
         assert (lse[b] - ref_lse).abs().max() < 1e-5
+
+
+@pytest.mark.parametrize("qtype", [2, 3, 8])
+@pytest.mark.parametrize("d,nq", [(64, 1), (64, 40), (128, 1), (128, 140), (256, 2), (256, 30), (256, 900)])
+def test_scores_of_ten_digits(s3b, engine, qtype, d, nq):
+    """Queries and keys near f16's largest, of either sign: scores past 2^31, whose f32 step is far more than 1. The row takes
+    the token with the largest; rows of small queries beside it are as ever."""
+    g = torch.Generator(device="cuda").manual_seed(nq)
+    n = 300
+    k = (30000 + 100 * torch.randperm(n, device="cuda", generator=g))[None, :, None, None].expand(1, n, 1, d).float()
+    v = torch.randn(1, n, 1, d, device="cuda", generator=g)
+    q = 1e-5 * torch.rand(1, nq, 1, d, device="cuda", generator=g)
+    q[:, ::3] = 6e4
+    q[:, 1::3] = -6e4
+    q = q.half()
+    out, lse, held = attend(s3b, engine, qtype, q, k, v, [n], page=16)
+    few = nq <= most_few(d)
+    ref, ref_lse = exact(q[0], held[0], d ** -0.5, keys16=not few)
+    assert off(out[0], ref) < NORM[few]
+    assert ((lse[0] - ref_lse).abs() <= lse_off(d, ref_lse.abs()) + 1e-5).all()
