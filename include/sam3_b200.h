@@ -594,7 +594,7 @@ int s3b_op_cache_read(s3b_ctx* ctx, const s3b_kv_cache* cache, const int64_t* sl
  *   causal  query i is the token at position lengths[b] - nq + i and sees no
  *        later one; window > 0 (with causal): only the last `window` positions
  *        up to its own.
- * A row that sees no token is zero. scale must be positive and finite.
+ * A row that sees no token is zero. scale must be positive and at most 2^56.
  * A length outside 0 .. max_pages * page_size is clamped, a page outside the
  * cache is read as page 0, and the next s3b_sync returns S3B_ERR_DEVICE.
  * Results do not depend on the order in which blocks run. The call only

@@ -1456,7 +1456,9 @@ int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* 
   if (batch < 0 || nq < 0 || max_pages < 0) return set_error(ctx, kErrArg, "cache_attention: negative size");
   if (heads <= 0 || heads % p.c.heads)
     return set_error(ctx, kErrArg, "cache_attention: %d query heads over %d key / value heads", heads, p.c.heads);
-  if (!(scale > 0.f) || scale > 3.4e38f) return set_error(ctx, kErrArg, "cache_attention: scale must be positive");
+  // f16 queries and keys give sums below 2^40: with scales up to 2^56 every score lies above the kernels' first reference, -1e30
+  if (!(scale > 0.f) || scale > 0x1p56f)
+    return set_error(ctx, kErrArg, "cache_attention: scale must be positive and at most 2^56");
   if (window < 0 || (window > 0 && !causal))
     return set_error(ctx, kErrArg, "cache_attention: a window must be positive and causal");
   if (batch == 0 || nq == 0) return kOk;

@@ -6,7 +6,8 @@ namespace s3b {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kNoScore = -1e30f;  // reference maximum before the first visible token: finite, so that no inf - inf arises
+constexpr float kNoScore = -1e30f;  // reference maximum before the first visible token: finite, so that no inf - inf arises, and
+                                    // below every score (f16 sums, a scale of 2^56 at most)
 
 // Tokens of sequence b, held to what its page table can name.
 __device__ __forceinline__ int sequence_length(const KvAttnParams& p, int b, int* err) {

@@ -39,3 +39,25 @@ def test_takes_page_tables_of_nearly_2_to_31_tokens(call, engine):
     assert call(max_pages=(1 << 27) - 512, stride=1 << 27) == 0
     engine.sync()
     assert (call.tensors["out"][0] == 1).all()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 57, 1e20, 3e38])
+def test_refuses_scales_past_the_scores_range(call, scale):
+    """Scores of -1e30 and less would count as none at all, and the row as one that sees nothing."""
+    assert call(scale=scale) == -1
+
+
+@pytest.mark.parametrize("nq", [1, 140])
+def test_largest_scale(s3b, engine, nq):
+    """Every score far below zero: the row still takes the largest."""
+    cache = s3b.KVCache(8, 2, 16, 1, 64)
+    k = -100.0 * torch.ones(32, 1, 64, device="cuda")
+    k[17] = -90.0
+    v = torch.arange(32, device="cuda", dtype=torch.float32)[:, None, None].expand(32, 1, 64).contiguous()
+    engine.cache_write(cache, k, v, torch.arange(32, device="cuda"))
+    q = torch.full((1, nq, 1, 64), 6e4, device="cuda", dtype=torch.float16)
+    out = torch.empty(q.shape, device="cuda")
+    engine.cache_attention(cache, q, out, torch.arange(2, dtype=torch.int32, device="cuda")[None],
+                           torch.tensor([32], dtype=torch.int32, device="cuda"), 2.0 ** 56)
+    engine.sync()
+    assert (out - 17).abs().max() < 17 * 2.0 ** -10
