@@ -1391,6 +1391,8 @@ static bool rows_aligned(const void* p, int esize, int64_t a, int64_t b, int64_t
   return !(reinterpret_cast<uintptr_t>(p) & 15) && !((a * esize) & 15) && !((b * esize) & 15) && !((c * esize) & 15);
 }
 
+static bool multiple_of(const void* p, unsigned bytes) { return !(reinterpret_cast<uintptr_t>(p) & (bytes - 1)); }
+
 int s3b_op_cache_write(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* k, int64_t k_n, int64_t k_h, const void* v,
                        int64_t v_n, int64_t v_h, int dtype, const int64_t* slots, int64_t n) {
   int rc = ctx_enter(ctx);
@@ -1404,6 +1406,7 @@ int s3b_op_cache_write(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* k, i
   const int es = dtype == S3B_F16 ? 2 : 4;
   if (!rows_aligned(k, es, k_n, k_h) || !rows_aligned(v, es, v_n, v_h))
     return set_error(ctx, kErrArg, "cache_write: rows must start on 16-byte boundaries");
+  if (!multiple_of(slots, 8)) return set_error(ctx, kErrArg, "cache_write: slots are not 8-byte aligned");
   KvRows r;
   r.k = const_cast<void*>(k);
   r.v = const_cast<void*>(v);
@@ -1431,6 +1434,7 @@ int s3b_op_cache_read(s3b_ctx* ctx, const s3b_kv_cache* cache, const int64_t* sl
   const int es = dtype == S3B_F16 ? 2 : 4;
   if ((k_out && !rows_aligned(k_out, es, k_n, k_h)) || (v_out && !rows_aligned(v_out, es, v_n, v_h)))
     return set_error(ctx, kErrArg, "cache_read: rows must start on 16-byte boundaries");
+  if (!multiple_of(slots, 8)) return set_error(ctx, kErrArg, "cache_read: slots are not 8-byte aligned");
   KvRows r;
   r.k = k_out;
   r.v = v_out;
@@ -1473,6 +1477,8 @@ int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* 
     return set_error(ctx, kErrUnsupported, "cache_attention: %d queries of %d heads", nq, heads);
   if (!rows_aligned(q, 2, q_b, q_n, q_h) || !rows_aligned(out, out_f32 ? 4 : 2, o_b, o_n, o_h))
     return set_error(ctx, kErrArg, "cache_attention: rows must start on 16-byte boundaries");
+  if (!multiple_of(pages, 4) || !multiple_of(lengths, 4) || !multiple_of(lse, 4))
+    return set_error(ctx, kErrArg, "cache_attention: pages, lengths and lse must be 4-byte aligned");
   p.q = reinterpret_cast<const __half*>(q);
   p.q_b = q_b;
   p.q_n = q_n;

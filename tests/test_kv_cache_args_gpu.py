@@ -61,3 +61,17 @@ def test_largest_scale(s3b, engine, nq):
                            torch.tensor([32], dtype=torch.int32, device="cuda"), 2.0 ** 56)
     engine.sync()
     assert (out - 17).abs().max() < 17 * 2.0 ** -10
+
+
+@pytest.mark.parametrize("name,offset", [("pages", 2), ("lengths", 1), ("lse", 2), ("q", 8), ("out", 4)])
+def test_refuses_pointers_off_their_size(call, name, offset):
+    assert call(offset=[(name, offset)], max_pages=3) == -1
+
+
+def test_refuses_slots_off_their_size(s3b, engine):
+    cache = s3b.KVCache(2, 1, 16, 1, 64)
+    rows, slots = torch.zeros(2, 1, 64, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    k, at = rows.data_ptr(), slots.data_ptr() + 4
+    assert engine._L.s3b_op_cache_write(engine.h, cache.ref, k, 64, 64, k, 64, 64, 0, at, 2) == -1
+    assert engine._L.s3b_op_cache_read(engine.h, cache.ref, at, 2, k, 64, 64, None, 0, 0, 0) == -1
+    engine.sync()
