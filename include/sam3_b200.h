@@ -587,7 +587,8 @@ int s3b_op_cache_read(s3b_ctx* ctx, const s3b_kv_cache* cache, const int64_t* sl
  *   lse  f32 [batch][nq][heads] or NULL: ln of the sum of exp(scale q.k),
  *        -inf for a row that sees no token (to join with attention over
  *        tokens outside the cache)
- *   pages [batch][pages_stride] (device): sequence b's tokens lie in order in
+ *   pages [batch][pages_stride] (device; a stride of 0: one row for all
+ *        sequences): sequence b's tokens lie in order in
  *        its first ceil(lengths[b] / page_size) pages, of at most max_pages
  *        (max_pages * page_size at most 2^31 - 8192)
  *   lengths [batch] (device), 0 allowed

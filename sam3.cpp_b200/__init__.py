@@ -197,9 +197,9 @@ _INDEX_TYPES: dict = {}
 
 
 def _index(what: str, name: str, t, itemsize: int, dims: int) -> int:
-    """Length of an index tensor of `dims` dimensions (int32: itemsize 4, int64: 8) with contiguous rows."""
+    """Length of an index tensor of `dims` dimensions (int32: itemsize 4, int64: 8) with contiguous rows (of one entry: any)."""
     shape = t.shape
-    if t.dtype is not _INDEX_TYPES[itemsize] or len(shape) != dims or not t.is_cuda or (t.stride()[-1] != 1 and t.numel()):
+    if t.dtype is not _INDEX_TYPES[itemsize] or len(shape) != dims or not t.is_cuda or (shape[-1] > 1 and t.stride()[-1] != 1):
         raise S3BError(f"{what}: {name} must be CUDA int{8 * itemsize} of {dims} dimension(s) with contiguous rows")
     return shape[0]
 
@@ -733,7 +733,7 @@ class Engine:
     def cache_attention(self, cache: KVCache, q, out, pages, lengths, scale: float, causal: bool = False,
                         window: int = 0, lse=None):
         """out = softmax(scale q K^T) V over the cache (s3b_op_cache_attention): q f16 [batch, nq, heads, d], out the same
-        shape in f16 or f32, pages int32 [batch, max_pages], lengths int32 [batch], lse f32 [batch, nq, heads] or None."""
+        shape in f16 or f32, pages int32 [batch, max_pages] (the rows may be one row expanded), lengths int32 [batch], lse f32 [batch, nq, heads] or None."""
         what = "cache_attention"
         shape = q.shape
         if _ROW_TYPES.get(q.dtype) != S3B_F16 or len(shape) != 4 or shape[3] != cache.d or not q.is_cuda or \

@@ -1467,7 +1467,7 @@ int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* 
     return set_error(ctx, kErrArg, "cache_attention: a window must be positive and causal");
   if (batch == 0 || nq == 0) return kOk;
   if (!q || !out || !lengths || (!pages && max_pages > 0)) return set_error(ctx, kErrArg, "cache_attention: null pointer");
-  if (max_pages > 0 && batch > 1 && pages_stride < max_pages)
+  if (max_pages > 0 && batch > 1 && pages_stride != 0 && pages_stride < max_pages)
     return set_error(ctx, kErrArg, "cache_attention: page table rows of %lld hold no %d pages", (long long)pages_stride,
                      max_pages);
   // token numbers are 32-bit, and the kernels count up to the end of the step that holds the last one

@@ -75,3 +75,43 @@ def test_refuses_slots_off_their_size(s3b, engine):
     assert engine._L.s3b_op_cache_write(engine.h, cache.ref, k, 64, 64, k, 64, 64, 0, at, 2) == -1
     assert engine._L.s3b_op_cache_read(engine.h, cache.ref, at, 2, k, 64, 64, None, 0, 0, 0) == -1
     engine.sync()
+
+
+@pytest.mark.parametrize("nq", [1, 300])
+def test_one_page_row_for_all_sequences(s3b, engine, nq):
+    """A row of the page table expanded over the batch, as sequences over one cache have it."""
+    g = torch.Generator(device="cuda").manual_seed(nq)
+    cache = s3b.KVCache(2, 9, 16, 2, 64)
+    k, v = (torch.randn(144, 2, 64, device="cuda", generator=g) for _ in "kv")
+    engine.cache_write(cache, k, v, torch.arange(144, device="cuda"))
+    row = torch.randperm(9, device="cuda", generator=g).to(torch.int32)[None]
+    q = torch.randn(5, nq, 4, 64, device="cuda", generator=g).half()
+    lens = torch.tensor([144, 0, 100, 17, 1], dtype=torch.int32, device="cuda")
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    engine.cache_attention(cache, q, a, row.expand(5, -1), lens, 0.125)
+    engine.cache_attention(cache, q, b, row.repeat(5, 1), lens, 0.125)
+    engine.sync()
+    assert torch.equal(a, b)
+
+
+def test_strides_of_one_entry_mean_nothing(s3b, engine):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    cache = s3b.KVCache(8, 4, 16, 1, 64)
+    k, v = (torch.randn(1, 1, 64, device="cuda", generator=g) for _ in "kv")
+    slots = torch.arange(40, 44, device="cuda")[::4]
+    assert slots.shape == (1,) and slots.stride() == (4,)
+    engine.cache_write(cache, k, v, slots)
+    q = torch.randn(1, 1, 1, 64, device="cuda", generator=g).half()
+    out = torch.empty(1, 1, 1, 64, device="cuda")
+    kept = torch.empty(1, 1, 64, device="cuda")
+    engine.cache_read(cache, slots, None, kept)
+    engine.cache_write(cache, k, v, torch.tensor([32], device="cuda"))
+    pages, lens = torch.tensor([[2, 7]], dtype=torch.int32, device="cuda")[:, ::2], torch.ones(3, dtype=torch.int32, device="cuda")[::3]
+    engine.cache_attention(cache, q, out, pages, lens, 0.125)
+    engine.sync()
+    assert (out[0, 0] - kept[0]).abs().max() <= 2.0 ** -10 * kept.abs().max()
+
+
+def test_refuses_page_rows_that_overlap(call):
+    assert call(batch=2, stride=3) == -1
+    assert call(batch=2, stride=-4) == -1
