@@ -196,11 +196,11 @@ _ROW_TYPES: dict = {}
 _INDEX_TYPES: dict = {}
 
 
-def _index(what: str, name: str, t, itemsize: int, dims: int) -> int:
+def _index(what: str, name: str, t, itemsize: int, dims: int, device: int) -> int:
     """Length of an index tensor of `dims` dimensions (int32: itemsize 4, int64: 8) with contiguous rows (of one entry: any)."""
     shape = t.shape
-    if t.dtype is not _INDEX_TYPES[itemsize] or len(shape) != dims or not t.is_cuda or (shape[-1] > 1 and t.stride()[-1] != 1):
-        raise S3BError(f"{what}: {name} must be CUDA int{8 * itemsize} of {dims} dimension(s) with contiguous rows")
+    if t.dtype is not _INDEX_TYPES[itemsize] or len(shape) != dims or t.get_device() != device or (shape[-1] > 1 and t.stride()[-1] != 1):
+        raise S3BError(f"{what}: {name} must be int{8 * itemsize} of {dims} dimension(s) with contiguous rows on cuda:{device}")
     return shape[0]
 
 
@@ -228,7 +228,7 @@ class KVCache:
             raise S3BError(f"KVCache: data must be {nbytes} contiguous bytes")
         if not data.is_cuda:
             raise S3BError("KVCache: data must be a CUDA tensor")
-        self.data = data
+        self.data, self.device = data, data.get_device()
         self.qtype, self.n_pages, self.page_size, self.heads, self.d = qtype, n_pages, page_size, heads, d
         self.desc = KVCacheDesc(qtype, heads, d, page_size, n_pages, data.data_ptr())
         self.ref = ctypes.byref(self.desc)
@@ -693,8 +693,7 @@ class Engine:
         self._check(rc, "s3b_op_dequantize")
 
     # -- quantised key / value cache
-    @staticmethod
-    def _cache_rows(what: str, cache: KVCache, n: int, name: str, t, dtype: int | None):
+    def _cache_rows(self, what: str, cache: KVCache, n: int, name: str, t, dtype: int | None):
         """dtype code (that of its partner, if given), pointer and strides of the row tensor t [n, heads, d] after the checks
         that a raw pointer cannot carry. The stride of a dimension of one entry means nothing and is given as 0."""
         code = _ROW_TYPES.get(t.dtype)
@@ -702,14 +701,14 @@ class Engine:
             raise S3BError(f"{what}: rows must be all f16 or all f32, {name} is {t.dtype}")
         heads = cache.heads
         a, b, c = t.stride() if t.dim() == 3 else (0, 0, 0)
-        if t.shape != (n, heads, cache.d) or not t.is_cuda or (c != 1 and n):
-            raise S3BError(f"{what}: {name} must be a CUDA tensor [{n}, {heads}, {cache.d}] with contiguous rows")
+        if t.shape != (n, heads, cache.d) or t.get_device() != self.device or cache.device != self.device or (c != 1 and n):
+            raise S3BError(f"{what}: {name} must be [{n}, {heads}, {cache.d}] with contiguous rows, on the engine's and the cache's GPU")
         return code, t.data_ptr(), a if n > 1 else 0, b if heads > 1 else 0
 
     def cache_write(self, cache: KVCache, k, v, slots):
         """Quantises the tokens k, v [n, heads, d] (f16 or f32 CUDA tensors, rows contiguous) into the slots int64 [n]
         (< 0: skipped)."""
-        n = _index("cache_write", "slots", slots, 8, 1)
+        n = _index("cache_write", "slots", slots, 8, 1, self.device)
         dtype, k_at, k_n, k_h = self._cache_rows("cache_write", cache, n, "k", k, None)
         _, v_at, v_n, v_h = self._cache_rows("cache_write", cache, n, "v", v, dtype)
         rc = self._L.s3b_op_cache_write(self.h, cache.ref, k_at, k_n, k_h, v_at, v_n, v_h, dtype, slots.data_ptr(), n)
@@ -719,7 +718,7 @@ class Engine:
     def cache_read(self, cache: KVCache, slots, k_out, v_out):
         """Reads the tokens of the slots int64 [n] (< 0: zeros) into k_out, v_out [n, heads, d] (f16 or f32; one of them
         may be None)."""
-        n = _index("cache_read", "slots", slots, 8, 1)
+        n = _index("cache_read", "slots", slots, 8, 1, self.device)
         dtype, k_at, k_n, k_h, v_at, v_n, v_h = None, None, 0, 0, None, 0, 0
         if k_out is not None:
             dtype, k_at, k_n, k_h = self._cache_rows("cache_read", cache, n, "k_out", k_out, None)
@@ -735,19 +734,19 @@ class Engine:
         """out = softmax(scale q K^T) V over the cache (s3b_op_cache_attention): q f16 [batch, nq, heads, d], out the same
         shape in f16 or f32, pages int32 [batch, max_pages] (the rows may be one row expanded), lengths int32 [batch], lse f32 [batch, nq, heads] or None."""
         what = "cache_attention"
-        shape = q.shape
-        if _ROW_TYPES.get(q.dtype) != S3B_F16 or len(shape) != 4 or shape[3] != cache.d or not q.is_cuda or \
+        shape, device = q.shape, self.device
+        if _ROW_TYPES.get(q.dtype) != S3B_F16 or len(shape) != 4 or shape[3] != cache.d or q.get_device() != device or cache.device != device or \
                 (q.stride(3) != 1 and q.numel()):
-            raise S3BError(f"{what}: q must be CUDA f16 [batch, nq, heads, {cache.d}] with contiguous rows")
+            raise S3BError(f"{what}: q must be f16 [batch, nq, heads, {cache.d}] with contiguous rows, on the engine's and the cache's GPU")
         b, nq, heads, _ = shape
         o_type = _ROW_TYPES.get(out.dtype)
-        if o_type is None or out.shape != shape or not out.is_cuda or (out.stride(3) != 1 and out.numel()):
-            raise S3BError(f"{what}: out must be CUDA f16 or f32 of q's shape with contiguous rows")
-        if _index(what, "lengths", lengths, 4, 1) != b or _index(what, "pages", pages, 4, 2) != b:
+        if o_type is None or out.shape != shape or out.get_device() != device or (out.stride(3) != 1 and out.numel()):
+            raise S3BError(f"{what}: out must be f16 or f32 of q's shape with contiguous rows on cuda:{device}")
+        if _index(what, "lengths", lengths, 4, 1, device) != b or _index(what, "pages", pages, 4, 2, device) != b:
             raise S3BError(f"{what}: pages must be int32 [{b}, max_pages] with contiguous rows, lengths int32 [{b}]")
         if lse is not None and (lse.shape != (b, nq, heads) or _ROW_TYPES.get(lse.dtype) != S3B_F32 or
-                                not lse.is_cuda or not lse.is_contiguous()):
-            raise S3BError(f"{what}: lse must be contiguous CUDA f32 [{b}, {nq}, {heads}]")
+                                lse.get_device() != device or not lse.is_contiguous()):
+            raise S3BError(f"{what}: lse must be contiguous f32 [{b}, {nq}, {heads}] on cuda:{device}")
         # the stride of a dimension of one entry means nothing and is given as 0
         q_b, q_n, q_h, _ = q.stride()
         o_b, o_n, o_h, _ = out.stride()
