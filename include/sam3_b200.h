@@ -599,7 +599,10 @@ int s3b_op_cache_read(s3b_ctx* ctx, const s3b_kv_cache* cache, const int64_t* sl
  * A length outside 0 .. max_pages * page_size is clamped, a page outside the
  * cache is read as page 0, and the next s3b_sync returns S3B_ERR_DEVICE.
  * Results do not depend on the order in which blocks run. The call only
- * enqueues work on the context stream; its workspace is the context's.
+ * enqueues work on the context stream; its workspace is the context's. It may
+ * be captured into a CUDA graph once a call of its shape has run (else
+ * S3B_ERR_STATE where the workspace would have to grow); later calls leave what
+ * the graph holds in place.
  * The reference attends over f16 keys and values of one sequence
  * (ggml_flash_attn_ext, sam3.cpp:9267, 9312). */
 int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* q, int64_t q_b, int64_t q_n,

@@ -45,6 +45,8 @@ int read_dev_err(s3b_ctx* ctx) {
     // blocks that gave up may have left the cache attention's counts unfinished
     const auto count = ctx->ws.find("kv_attn_count");
     if (count != ctx->ws.end() && count->second->bytes) cudaMemsetAsync(count->second->p, 0, count->second->bytes, ctx->stream);
+    for (const auto& b : ctx->graph_kept)
+      if (b.first == "kv_attn_count") cudaMemsetAsync(b.second->p, 0, b.second->bytes, ctx->stream);
     cudaStreamSynchronize(ctx->stream);
     if (h == kDevErrIndex)
       return set_error(ctx, kErrDevice, "a slot, page or length in device memory is out of range (code %d)", h);
@@ -1449,6 +1451,30 @@ int s3b_op_cache_read(s3b_ctx* ctx, const s3b_kv_cache* cache, const int64_t* sl
   return kOk;
 }
 
+// ctx->buf for a call that may be captured into a caller's CUDA graph: no allocation during a capture, and a buffer that a
+// capture has seen is kept, not freed, when a later call needs a larger one. *grown: the buffer is new.
+static DevBuf* graph_buf(s3b_ctx* ctx, const char* name, size_t bytes, bool capturing, bool* grown, int* rc) {
+  auto& b = ctx->ws[name];
+  auto& held = ctx->graph_held;
+  const bool kept = std::find(held.begin(), held.end(), name) != held.end();
+  *grown = !b || bytes > b->bytes;
+  if (*grown) {
+    if (capturing) {
+      *rc = set_error(ctx, kErrState, "workspace '%s' has to grow to %zu bytes during a stream capture: run the shape once before",
+                      name, bytes);
+      return nullptr;
+    }
+    if (kept) {
+      ctx->graph_kept.emplace_back(name, b);
+      held.erase(std::find(held.begin(), held.end(), name));
+      b.reset();
+    }
+    return ctx->buf(name, bytes, rc);
+  }
+  if (capturing && !kept) held.push_back(name);
+  return b.get();
+}
+
 int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* q, int64_t q_b, int64_t q_n,
                            int64_t q_h, void* out, int out_f32, int64_t o_b, int64_t o_n, int64_t o_h, float* lse,
                            const int32_t* pages, int64_t pages_stride, int max_pages, const int32_t* lengths, int batch,
@@ -1501,18 +1527,28 @@ int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* 
   p.window = window;
   KvAttnWork w;
   w.sms = num_sms();
-  size_t part_bytes, count_bytes;
-  kv_attention_work(p, w.sms, &part_bytes, &count_bytes);
-  if (part_bytes) {
-    w.part = ctx->buf("kv_attn_part", part_bytes, &rc)->as<float>();
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(ctx->stream, &capture) != cudaSuccess) cudaGetLastError();
+  const bool capturing = capture != cudaStreamCaptureStatusNone;
+  const KvAttnBytes need = kv_attention_work(p, w.sms);
+  bool grown;
+  DevBuf* part = graph_buf(ctx, "kv_attn_part", need.part, capturing, &grown, &rc);
+  if (rc) return rc;
+  w.part = part->as<float>();
+  // counts and images in powers of two: what graphs keep of them is less than what is in use
+  auto power = [](size_t n, size_t least) {
+    while (least < n) least *= 2;
+    return least;
+  };
+  DevBuf* count = graph_buf(ctx, "kv_attn_count", power(need.count, 1 << 16), capturing, &grown, &rc);
+  if (rc) return rc;
+  if (grown && cudaMemsetAsync(count->p, 0, count->bytes, ctx->stream) != cudaSuccess)
+    return set_error(ctx, kErrCuda, "cache_attention: clearing the counts");
+  w.count = count->as<int>();
+  if (need.image) {
+    DevBuf* image = graph_buf(ctx, "kv_attn_image", power(need.image, 1 << 20), capturing, &grown, &rc);
     if (rc) return rc;
-    DevBuf* count = ctx->buf("kv_attn_count", 0, &rc);
-    if (count->bytes < count_bytes) {
-      if (count->reserve(std::max<size_t>(count_bytes, 4096)) ||
-          cudaMemsetAsync(count->p, 0, count->bytes, ctx->stream) != cudaSuccess)
-        return set_error(ctx, kErrOOM, "cache_attention: %zu bytes of counts", count_bytes);
-    }
-    w.count = count->as<int>();
+    w.image = image->as<uint8_t>();
   }
   rc = kv_attention(p, w, ctx->d_err, ctx->stream);
   if (rc) return set_error(ctx, launcher_status_code(rc), "cache_attention launch failed (%d)", rc);

@@ -358,6 +358,10 @@ struct s3b_ctx {
   cudaEvent_t next_event();
 
   s3b::DevBuf* buf(const std::string& name, size_t bytes, int* rc);
+  // workspaces of calls that a caller's CUDA graph may hold (capi.cpp, graph_buf): names that a capture has seen, and buffers
+  // that grew since, kept for the graphs until the context goes
+  std::vector<std::string> graph_held;
+  std::vector<std::pair<std::string, std::shared_ptr<s3b::DevBuf>>> graph_kept;
 };
 
 namespace s3b {

@@ -394,18 +394,23 @@ struct KvAttnParams {
   float scale = 1.f;
   int causal = 0, window = 0;
 };
-// Workspace of the attention: parts of units that several CTAs share, and their arrival counts, which are zero before
-// and after every launch.
+// Workspace of the attention: parts of units that several CTAs share; their arrival counts, which are zero before and after
+// every launch; f16 images of the operands where they are staged.
 struct KvAttnWork {
   float* part = nullptr;
   int* count = nullptr;
+  uint8_t* image = nullptr;
   int sms = 0;
 };
-void kv_attention_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes);
+struct KvAttnBytes {
+  size_t part, count, image;  // part: the same for every call; image: 0 where nothing is staged
+};
+KvAttnBytes kv_attention_work(const KvAttnParams& p, int sms);
 int kv_attention(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st);
 int kv_attention_launches(const KvAttnParams& p);  // kernels that the call launches
 // The tensor-core kernel for tiles of 128 query rows (kv_attention picks it for more rows than its own kernel takes).
-void kv_attention_tc_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes);
+size_t kv_attention_tc_parts(int sms);                 // bytes of the parts, the most of any call
+size_t kv_attention_tc_image(const KvAttnParams& p);
 int kv_attention_tc(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st);
 int kv_attention_tc_launches(const KvAttnParams& p);
 

@@ -862,13 +862,18 @@ int attend_d(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t 
 
 }  // namespace
 
-void kv_attention_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes) {
-  const long long rows = p.nq * (long long)(p.heads / p.c.heads);
-  *part_bytes = *count_bytes = 0;
-  if (rows > most_rows(p.c.d)) return kv_attention_tc_work(p, sms, part_bytes, count_bytes);
-  const int padded = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
-  *part_bytes = (size_t)2 * 8 * sms * padded * (p.c.d + 2) * 4;
-  *count_bytes = (size_t)p.batch * p.c.heads * 4;
+KvAttnBytes kv_attention_work(const KvAttnParams& p, int sms) {
+  // two parts for each of rows_kernel's CTAs: at most 4 an SM with 8 rows, 3 with 16 and 2 with 32 of d = 128, or with 16 of 256
+  constexpr int kMost = 2 * Rows<QT_Q4_0, 128, 4, 4>::kCtas * 32 * (128 + 2);
+  static_assert(2 * Rows<QT_Q4_0, 128, 1, 4>::kCtas * 8 * 130 <= kMost && 2 * Rows<QT_Q4_0, 128, 2, 4>::kCtas * 16 * 130 <= kMost &&
+                    2 * Rows<QT_Q4_0, 64, 4, 4>::kCtas * 32 * 66 <= kMost && 2 * Rows<QT_Q4_0, 64, 2, 4>::kCtas * 16 * 66 <= kMost &&
+                    2 * Rows<QT_Q4_0, 256, 1, 4>::kCtas * 8 * 258 <= kMost && 2 * Rows<QT_Q4_0, 256, 2, 4>::kCtas * 16 * 258 <= kMost,
+                "parts of rows_kernel");
+  KvAttnBytes b;
+  b.part = std::max((size_t)sms * kMost * 4, kv_attention_tc_parts(sms));
+  b.count = (size_t)p.batch * p.c.heads * 4;
+  b.image = p.nq * (long long)(p.heads / p.c.heads) > most_rows(p.c.d) ? kv_attention_tc_image(p) : 0;
+  return b;
 }
 
 int kv_attention_launches(const KvAttnParams& p) {

@@ -31,6 +31,8 @@
 // 0 1 8 9 2 3 10 11 4 5 12 13 6 7 14 15 (both in K's rows and V's columns; a softmax does not mind), which is the order
 // in which a lane holds them, so V goes to shared memory transposed, [D values][64 tokens], in 8-byte pieces and is a
 // K-major operand like K.
+#include <algorithm>
+
 #include "kv_attention.cuh"
 
 namespace s3b {
@@ -1232,7 +1234,7 @@ int launch_tiles(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStrea
   a.shared = reinterpret_cast<Shared*>(w.part + part_floats(w.sms, TQ, D));
   a.blocks = (int)t.blocks;
   a.tiles = (int)t.tiles;
-  a.image = reinterpret_cast<uint8_t*>(w.part) + (part_floats(w.sms, TQ, D) * 4 + w.sms * sizeof(Shared) + 127) / 128 * 128;
+  a.image = w.image;
   a.q_image = a.image + t.kv_bytes;
   int rc;
   if (t.staged) {
@@ -1262,11 +1264,13 @@ int launch_tiles_d(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStr
 
 }  // namespace
 
-void kv_attention_tc_work(const KvAttnParams& p, int sms, size_t* part_bytes, size_t* count_bytes) {
+size_t kv_attention_tc_parts(int sms) {
+  return std::max(part_floats(sms, 2, 128), part_floats(sms, 1, 256)) * 4 + sms * sizeof(Shared);
+}
+
+size_t kv_attention_tc_image(const KvAttnParams& p) {
   const TcPlan t = tc_plan(p);
-  *part_bytes = part_floats(sms, t.tq, p.c.d) * 4 + sms * sizeof(Shared) + 128 +
-                (t.staged ? (size_t)(t.kv_bytes + t.q_bytes) : 0);
-  *count_bytes = 0;
+  return t.staged ? (size_t)(t.kv_bytes + t.q_bytes) : 0;
 }
 
 int kv_attention_tc_launches(const KvAttnParams& p) { return tc_plan(p).staged ? 3 : 2; }

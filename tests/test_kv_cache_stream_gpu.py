@@ -114,3 +114,113 @@ def test_many_rows_while_the_cache_arrives_unevenly(s3b, engine, qtype, d, heads
     assert torch.isfinite(outs[0]).all()
     for out in outs[1:]:
         assert torch.equal(out, outs[0])
+
+
+@pytest.fixture
+def captured(s3b):
+    """An engine of its own on a stream of its own, and a function that runs a call under capture and returns the graph."""
+    stream = torch.cuda.Stream()
+    own = s3b.Engine(0)
+    own.set_stream(stream.cuda_stream)
+
+    def capture(call):
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            call()
+        return graph
+    yield own, stream, capture
+    torch.cuda.synchronize()
+    own.close()
+
+
+def _filled(s3b, engine, qtype, n, heads, d, page=16):
+    g = torch.Generator(device="cuda").manual_seed(n)
+    cache = s3b.KVCache(qtype, -(-n // page), page, heads, d)
+    k, v = (torch.randn(n, heads, d, device="cuda", generator=g).half() for _ in "kv")
+    engine.cache_write(cache, k, v, torch.arange(n, device="cuda"))
+    engine.sync()
+    return cache, torch.arange(-(-n // page), dtype=torch.int32, device="cuda")[None], torch.tensor([n], dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("nq,qtype,d", [(1, 2, 128), (6, 3, 64), (70, 8, 128), (900, 2, 256)])
+def test_graph_survives_a_larger_call(s3b, engine, captured, nq, qtype, d):
+    """A captured call, replayed with new queries before and after calls that need a larger workspace, which has to be another
+    buffer than the graph's."""
+    own, stream, capture = captured
+    cache, pages, lens = _filled(s3b, engine, qtype, 3000, 2, d)
+    big = _filled(s3b, engine, 2, 30000, 2, d)
+    g = torch.Generator(device="cuda").manual_seed(nq)
+    q = torch.randn(1, nq, 8, d, device="cuda", generator=g).half()
+    out, ref = torch.empty_like(q), torch.empty_like(q)
+    torch.cuda.synchronize()
+    own.cache_attention(cache, q, out, pages, lens, d ** -0.5)  # the shape once
+    own.sync()
+    graph = capture(lambda: own.cache_attention(cache, q, out, pages, lens, d ** -0.5))
+
+    def check():
+        q.copy_(torch.randn(q.shape, device="cuda", generator=g))
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        engine.cache_attention(cache, q, ref, pages, lens, d ** -0.5)
+        engine.sync()
+        assert torch.equal(out, ref)
+    check()
+    many = torch.randn(1, 5000, 8, d, device="cuda", generator=g).half()
+    wide = torch.randn(20000, 1, 2, d, device="cuda", generator=g).half()
+    torch.cuda.synchronize()
+    for big_q, rows in ((many, 1), (wide, len(wide))):  # more rows, then more sequences
+        got, again = torch.empty_like(big_q), torch.empty_like(big_q)
+        torch.cuda.synchronize()
+        tables, lengths = (t.expand(rows, *t.shape[1:]).contiguous() for t in big[1:])
+        lengths = (lengths // (1 if rows == 1 else 100)).contiguous()
+        torch.cuda.synchronize()
+        own.cache_attention(big[0], big_q, got, tables, lengths, d ** -0.5)
+        own.sync()
+        engine.cache_attention(big[0], big_q, again, tables, lengths, d ** -0.5)
+        engine.sync()
+        assert torch.equal(got, again)
+        check()
+        check()
+
+
+def test_few_rows_captured_after_many(s3b, engine, captured):
+    """A call of few rows is captured when only one of many rows has run: nothing may have to be allocated then."""
+    own, stream, capture = captured
+    cache, pages, lens = _filled(s3b, engine, 2, 2000, 2, 128)
+    many, few = (torch.randn(1, nq, 8, 128, device="cuda").half() for nq in (400, 1))
+    outs = [torch.empty_like(x) for x in (many, few, few)]
+    torch.cuda.synchronize()
+    own.cache_attention(cache, many, outs[0], pages, lens, 0.1)
+    own.sync()
+    graph = capture(lambda: own.cache_attention(cache, few, outs[1], pages, lens, 0.1))
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    engine.cache_attention(cache, few, outs[2], pages, lens, 0.1)
+    engine.sync()
+    assert torch.equal(outs[1], outs[2])
+
+
+def test_growing_during_a_capture_is_refused(s3b, engine, captured):
+    """The first call of an engine inside a capture: an error, no allocation, and the capture and the engine go on."""
+    own, stream, capture = captured
+    cache, pages, lens = _filled(s3b, engine, 2, 2000, 2, 128)
+    q = torch.randn(1, 1, 8, 128, device="cuda").half()
+    out, ref = torch.empty_like(q), torch.empty_like(q)
+    rows = [torch.empty(4, 2, 128, device="cuda", dtype=torch.float16) for _ in "kv"]
+    slots = torch.arange(4, device="cuda")
+
+    def call():
+        with pytest.raises(s3b.S3BError, match="capture"):
+            own.cache_attention(cache, q, out, pages, lens, 0.1)
+        own.cache_read(cache, slots, *rows)
+    graph = capture(call)
+    graph.replay()
+    own.cache_attention(cache, q, out, pages, lens, 0.1)
+    own.sync()
+    engine.cache_attention(cache, q, ref, pages, lens, 0.1)
+    engine.sync()
+    assert torch.equal(out, ref) and rows[0].any()
