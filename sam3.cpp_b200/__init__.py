@@ -214,7 +214,7 @@ def kv_cache_bytes(qtype: int, heads: int, d: int, page_size: int, n_pages: int)
 
 class KVCache:
     """A quantised key / value cache of n_pages pages of page_size token slots (s3b_kv_cache), in `data`: a uint8 CUDA
-    tensor of kv_cache_bytes() bytes, made here unless given."""
+    tensor of kv_cache_bytes() bytes, made here unless given (zeros, there when the constructor returns)."""
 
     def __init__(self, qtype: int, n_pages: int, page_size: int, heads: int, d: int, data=None, device="cuda"):
         nbytes = kv_cache_bytes(qtype, heads, d, page_size, n_pages)
@@ -224,6 +224,8 @@ class KVCache:
             _ROW_TYPES.update({torch.float16: S3B_F16, torch.float32: S3B_F32})
         if data is None:
             data = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+            if data.is_cuda:  # the first write may come on the engine's own stream
+                torch.cuda.current_stream(data.device).synchronize()
         elif data.numel() * data.element_size() < nbytes or not data.is_contiguous():
             raise S3BError(f"KVCache: data must be {nbytes} contiguous bytes")
         if not data.is_cuda:

@@ -224,3 +224,25 @@ def test_growing_during_a_capture_is_refused(s3b, engine, captured):
     engine.cache_attention(cache, q, ref, pages, lens, 0.1)
     engine.sync()
     assert torch.equal(out, ref) and rows[0].any()
+
+
+@pytest.mark.parametrize("side", [False, True])
+def test_new_cache_is_cleared_before_its_first_write(s3b, side):
+    """A cache of 4 GiB made on torch's stream (or a side stream) and written at once on the engine's own."""
+    own = s3b.Engine(0)
+    page, d = 64, 128
+    pages = (4 << 30) // s3b.kv_cache_bytes(8, 1, d, page, 1)
+    k, v = (torch.randn(64, 1, d, device="cuda") for _ in "kv")
+    slots = (pages - 1) * page + torch.arange(64, device="cuda")
+    rows = [torch.empty(64, 1, d, device="cuda") for _ in "kv"]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream() if side else torch.cuda.current_stream()):
+        cache = s3b.KVCache(8, pages, page, 1, d)
+    own.cache_write(cache, k, v, slots)
+    own.sync()
+    torch.cuda.synchronize()
+    own.cache_read(cache, slots, *rows)
+    own.sync()
+    own.close()
+    for x, y in zip(rows, (k, v)):
+        assert (x - y).abs().max() <= y.abs().max() / 127
