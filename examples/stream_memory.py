@@ -1,9 +1,11 @@
-"""A tracker's memory as a quantised key / value cache.
+"""A memory of the last frames of a stream as a quantised key / value cache.
 
-Every frame of a stream leaves a feat x feat map of 64-channel memory features and a few object-pointer tokens. Their keys
-and values (one head of 256, as the memory attention's) are projected once, quantised into the pages of a ring of the last
-`slots` frames, and every new frame attends over what the ring holds: the page table lists the pages of the frames to
-look at, so a frame is dropped or reused by changing the table, and a page can be read back or copied out as it is.
+Every frame leaves a feat x feat map of 64-channel features and a few pointer tokens. Their keys and values (one head of 256)
+are projected once, with random weights here, quantised into the pages of a ring of the last `slots` frames, and every new
+frame attends over what the ring holds: the page table lists the pages of the frames to look at, so a frame is dropped or
+reused by changing the table, and a page can be read back or copied out as it is. This holds for keys that stay as they
+are once written. The engine's own tracking step adds an encoding of a frame's age to its keys, which would have to be
+written anew each frame, and keeps the 64 channels instead.
 
   python examples/stream_memory.py [--feat 64] [--frames 12] [--slots 7] [--type q4_0]
 """
@@ -20,7 +22,7 @@ TYPES = {"q4_0": 2, "q4_1": 3, "q8_0": 8}
 
 
 class StreamMemory:
-    """Memory of one object: `slots` frames of feat * feat map tokens and `pointers` pointer tokens each."""
+    """Memory of `slots` frames of feat * feat map tokens and `pointers` pointer tokens each."""
 
     D = 256
 

@@ -563,7 +563,8 @@ int64_t s3b_kv_cache_bytes(int type, int heads, int d, int page_size, int64_t n_
  * d contiguous; pointers and strides multiples of 16 bytes); slots[i] (device)
  * is the token's slot, < 0 skips the token. Two tokens of one call must not
  * share a slot. Scales and codes are those of s3b_quantize_rows bit for bit (but
- * for the codes of a block whose scale is 0 in f16, which mean nothing). Values
+ * for the codes of a block whose scale is 0 in f16 and the sign of a scale or
+ * minimum of 0, which mean nothing). Values
  * beyond +-65024 (infinities too) are held to it and a NaN counts as 0, so that
  * no row of the cache can hold one: a token that a mask hides cannot reach
  * another row's result. A slot past the end is skipped, and the next s3b_sync
@@ -598,6 +599,10 @@ int s3b_op_cache_read(s3b_ctx* ctx, const s3b_kv_cache* cache, const int64_t* sl
  * A row that sees no token is zero. scale must be positive and at most 2^56.
  * A length outside 0 .. max_pages * page_size is clamped, a page outside the
  * cache is read as page 0, and the next s3b_sync returns S3B_ERR_DEVICE.
+ * Sums and softmax statistics are f32. Weights enter the products as f16, and
+ * so do, with up to 32 rows (nq * heads / cache->heads; 16 at d = 256), their
+ * products with the block scales, with more rows the cache's values: f32 outputs
+ * are off by 2e-4 to 4e-4 of their norm.
  * Results do not depend on the order in which blocks run. The call only
  * enqueues work on the context stream; its workspace is the context's. It may
  * be captured into a CUDA graph once a call of its shape has run (else

@@ -11,10 +11,12 @@
 // times scale: the output is off by 3.5e-4 of its norm, where rounding it to f16 alone costs 2.1e-4, for values of any size
 // (ScaleRange keeps both in f16's normal range).
 //
-// Measured: 32 sequences of 1384 to 16384 tokens, 32 heads on 8, d = 128, q4_0: 319 MB in 80 us, 4.0 TB/s of the 6.5 that a
-// copy reaches; one sequence of 524288 tokens, 16 heads on 2, q4_1: 168 MB in 51 us. Instruction issue bounds it (61% of
-// the cycles issue, the integer pipe is half busy): some 340 instructions for 16 tokens of a head, most of them unpacking
-// codes and scaling partial scores and weights.
+// Measured: 32 sequences of 1384 to 16384 tokens, 32 heads on 8, d = 128, q4_0: 319 MB in 82 us, 3.9 TB/s of the 6.5 that a
+// copy reaches; one sequence of 524288 tokens, 16 heads on 2, q4_1: 168 MB in 53 us. Instruction issue bounds it (62% of
+// the cycles issue, the integer pipe is half busy): some 350 instructions for 16 tokens of a head, most of them unpacking
+// codes and scaling partial scores and weights. Looking at the scales of each step (ScaleRange) is 3% of the time. The output's
+// and the query's registers leave 33 of the 48 variants 4 to 84 bytes of spills a thread (one query tile of d = 128 in q4_0: 24
+// and 32, in q4_1 16 and 32).
 #include <algorithm>
 
 #include "kv_attention.cuh"
@@ -833,7 +835,7 @@ int launch_rows(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream
 // ---------------------------------------------------------------- dispatch
 // Rows of one key / value head that rows_kernel takes (its output registers end at 128 a thread). tiles_kernel fills 128 or
 // 256 rows whatever the count, so this one is ahead as far as it goes: 32 rows over 32 x 8192 tokens and 8 heads of 128
-// take 203 us against 256, 16 rows over 8 x 28736 tokens and one head of 256 take 53 against 84.
+// take 207 us against 256, 16 rows over 8 x 28736 tokens and one head of 256 take 55 against 84.
 int most_rows(int d) { return d == 256 ? 16 : 32; }
 
 template <int QT, int D, int NT>

@@ -22,10 +22,11 @@
 //
 // Rounded to f16: the operands of the two products (a value of the cache once, the weight once). Sums, maxima and O are f32.
 //
-// Measured, staged: 4096 rows over 28736 tokens, one head of 256: 120 us in all, of which this kernel 100 (tensor pipe 70% of
-// the cycles active; what is left is the chain S, softmax, P V of the only tile that fits). 4 x 2048 causal queries over 3 to
-// 8 thousand tokens, 16 heads on 4, d = 128: 342 us, 916 TFLOP/s (tensor pipe 53%, exponentials 54% of the MUFU's rate: the
-// two take turns on shared memory and TMEM ports). d = 64: 615 TFLOP/s, where the exponentials are twice as many a FLOP.
+// Measured, staged, one call at a time: 4096 rows over 28736 tokens, one head of 256: 120 us in all, of which this kernel 100
+// (tensor pipe 69% of the cycles active; what is left is the chain S, softmax, P V of the only tile that fits). 4 x 2048
+// causal queries over 3 to 8 thousand tokens, 16 heads on 4, d = 128: 344 us, 910 TFLOP/s (tensor pipe 53%, exponentials 53%
+// of the MUFU's rate: the two take turns on shared memory and TMEM ports). d = 64: 618 TFLOP/s, where the exponentials are
+// twice as many a FLOP. (Back to back, under the power cap, the first two take 125 and 379 us.)
 //
 // The f16 operand is code * scale (+ minimum) rounded once. The 16 tokens of a group stand in the order
 // 0 1 8 9 2 3 10 11 4 5 12 13 6 7 14 15 (both in K's rows and V's columns; a softmax does not mind), which is the order

@@ -176,12 +176,12 @@ __device__ __forceinline__ uint32_t pack_nibbles(const uint32_t (&c)[8]) {
 }
 
 // Four lanes a block of 32 values, 8 each: rows are read in 16-byte pieces, and the 8 values of a lane are a whole word of
-// the keys' layout (4-bit codes; two words of 8-bit ones) and two pieces of the values'. Bound by HBM: the blocks stay
-// and walk over the tokens of their head, and the K and V rows of the next two tokens are on their way while these are
-// quantised (loading, then quantising, then storing left the memory idle half of the time: 72 -> 59 us for the case below).
-// Measured: 65536 tokens, 4 heads of 128, q4_1 from f16: 177 MB in 53 us, 3.3 TB/s (a copy of as many bytes takes 40 us).
-// Instruction issue bounds it (8 of 10 cycles): a block's range, its two divisions and five steps a value, all in f32 to
-// give the codes of the host's quantiser.
+// the keys' layout (4-bit codes; two words of 8-bit ones) and two pieces of the values'. The blocks walk over the tokens of
+// their head, and the K and V rows of the next two tokens are on their way while these are quantised (loading, then quantising,
+// then storing left the memory idle half of the time: 72 -> 59 us for the case below).
+// Measured: 65536 tokens, 4 heads of 128, q4_1 from f16: 176 MB in 53 us cold, 3.3 TB/s (a copy of as many bytes takes 35 us).
+// Instruction issue bounds it (77% of the cycles): a block's range, its two divisions and five steps a value, all in f32 to
+// give the codes of the host's quantiser, one value an instruction.
 template <int QT, int D, typename T>
 __global__ void __launch_bounds__(256) write_kernel(const __grid_constant__ Job j) {
   typedef KvL<QT, D> L;
@@ -260,8 +260,8 @@ __global__ void __launch_bounds__(256) write_kernel(const __grid_constant__ Job 
 }
 
 // The reverse, in the same shape: 8 values of a row a lane, K and V of two tokens read before any is unpacked. Bound by
-// memory: 65536 tokens, 4 heads of 128, q4_1 to f16: 177 MB in 45 us, 3.9 TB/s, where a copy of as many bytes takes 40 us.
-// Blocks that stay and read ahead (47 us) and streaming stores (47 us) were no faster.
+// memory: 65536 tokens, 4 heads of 128, q4_1 to f16: 176 MB in 43 us cold, 4.1 TB/s, where a copy of as many bytes takes 35 us.
+// Blocks that stay and read ahead and streaming stores were no faster (47 us each, against 45 of that time).
 template <int QT, int D, typename T>
 __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Job j) {
   typedef KvL<QT, D> L;
@@ -372,9 +372,9 @@ int launch(bool write, const KvCache& c, const KvRows& r, const long long* slots
     j.div_mul = (unsigned)(((1ULL << (32 + j.div_shift)) + c.page_size - 1) / c.page_size);
   }
   long long blocks = (n + j.tokens - 1) / j.tokens * c.heads;
-  if (write) {  // blocks that stay: as many as are resident, a multiple of the heads
-    const long long resident = 6LL * num_sms() / c.heads * c.heads;
-    blocks = std::min(blocks, std::max(resident, (long long)c.heads));
+  if (write) {  // blocks that walk: 6 an SM (71 to 95 registers: 2 or 3 of them at a time), a multiple of the heads
+    const long long walking = 6LL * num_sms() / c.heads * c.heads;
+    blocks = std::min(blocks, std::max(walking, (long long)c.heads));
   }
   if (blocks > 0x7fffffffLL) return -2;
   const JobKernel k = c.type == QT_Q4_0 ? job_kernel_d<QT_Q4_0>(c.d, write, r.f32)
