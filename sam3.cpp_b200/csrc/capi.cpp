@@ -1556,6 +1556,294 @@ int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* 
   return kOk;
 }
 
+// The arguments that the calls on long caches share, into p: the sequences, then the queries over them.
+static int kv_sequences(s3b_ctx* ctx, const char* what, KvAttnParams* p, const int32_t* pages, int64_t pages_stride,
+                        int max_pages, const int32_t* lengths, int batch) {
+  if (batch < 0 || max_pages < 0) return set_error(ctx, kErrArg, "%s: negative size", what);
+  if (batch > 0 && (!lengths || (!pages && max_pages > 0))) return set_error(ctx, kErrArg, "%s: null pointer", what);
+  if (max_pages > 0 && batch > 1 && pages_stride != 0 && pages_stride < max_pages)
+    return set_error(ctx, kErrArg, "%s: page table rows of %lld hold no %d pages", what, (long long)pages_stride, max_pages);
+  if ((long long)max_pages * p->c.page_size > kMaxCacheTokens)
+    return set_error(ctx, kErrUnsupported, "%s: a sequence may hold %lld tokens at most", what, kMaxCacheTokens);
+  if (!multiple_of(pages, 4) || !multiple_of(lengths, 4))
+    return set_error(ctx, kErrArg, "%s: pages and lengths must be 4-byte aligned", what);
+  p->pages = pages;
+  p->pages_stride = pages_stride;
+  p->max_pages = max_pages;
+  p->lengths = lengths;
+  p->batch = batch;
+  return kOk;
+}
+
+static int kv_queries(s3b_ctx* ctx, const char* what, KvAttnParams* p, const void* q, int64_t q_b, int64_t q_n, int64_t q_h,
+                      int nq, int heads, int causal, int window) {
+  if (nq < 0) return set_error(ctx, kErrArg, "%s: negative size", what);
+  if (heads <= 0 || heads % p->c.heads)
+    return set_error(ctx, kErrArg, "%s: %d query heads over %d key / value heads", what, heads, p->c.heads);
+  if (window < 0 || (window > 0 && !causal))
+    return set_error(ctx, kErrArg, "%s: a window must be positive and causal", what);
+  if ((long long)nq * heads > 0x3fffffffLL) return set_error(ctx, kErrUnsupported, "%s: %d queries of %d heads", what, nq, heads);
+  if (!q && nq > 0 && p->batch > 0) return set_error(ctx, kErrArg, "%s: null pointer", what);
+  if (!rows_aligned(q, 2, q_b, q_n, q_h)) return set_error(ctx, kErrArg, "%s: rows must start on 16-byte boundaries", what);
+  p->q = reinterpret_cast<const __half*>(q);
+  p->q_b = q_b;
+  p->q_n = q_n;
+  p->q_h = q_h;
+  p->nq = nq;
+  p->heads = heads;
+  p->causal = causal ? 1 : 0;
+  p->window = window;
+  return kOk;
+}
+
+static int kv_lists(s3b_ctx* ctx, const char* what, KvAttnParams* p, const int32_t* selected, int keep, int share) {
+  if (keep < 1 || share < 1) return set_error(ctx, kErrArg, "%s: lists of %d pages for blocks of %d queries", what, keep, share);
+  const long long rows = (long long)std::min(share, std::max(p->nq, 1)) * (p->heads / p->c.heads);
+  if (rows > kv_attention_most_rows(p->c.d))
+    return set_error(ctx, kErrUnsupported, "%s: %lld rows share a list, at most %d may", what, rows, kv_attention_most_rows(p->c.d));
+  if (p->batch > 0 && p->nq > 0 && !selected) return set_error(ctx, kErrArg, "%s: null pointer", what);
+  if (!multiple_of(selected, 4)) return set_error(ctx, kErrArg, "%s: selected must be 4-byte aligned", what);
+  p->selected = selected;
+  p->keep = keep;
+  p->share = std::min(share, std::max(p->nq, 1));
+  if (kv_attention_units(*p) > 0x7fffffffLL || kv_attention_units(*p) * keep > (1LL << 40))
+    return set_error(ctx, kErrUnsupported, "%s: %lld lists of %d pages", what, kv_attention_units(*p), keep);
+  return kOk;
+}
+
+// f16 queries and keys give sums below 2^40: with scales up to 2^56 every score lies above the kernels' first reference, -1e30
+static int kv_scale(s3b_ctx* ctx, const char* what, KvAttnParams* p, float scale) {
+  if (!(scale > 0.f) || scale > 0x1p56f) return set_error(ctx, kErrArg, "%s: scale must be positive and at most 2^56", what);
+  p->scale = scale;
+  return kOk;
+}
+
+static int kv_bounds_arg(s3b_ctx* ctx, const char* what, const s3b_kv_bounds* bounds, KvCache* c, KvBounds* out) {
+  if (!bounds || !bounds->codes || !bounds->steps) return set_error(ctx, kErrArg, "%s: null bounds", what);
+  c->type = S3B_Q4_0;
+  c->heads = bounds->heads;
+  c->d = bounds->d;
+  c->page_size = bounds->page_size;
+  c->n_pages = bounds->n_pages;
+  if (kv_cache_bytes(*c) < 0)
+    return set_error(ctx, kErrArg, "%s: bad bounds: %d heads, d %d, %lld pages of %d", what, c->heads, c->d, c->n_pages, c->page_size);
+  if (!multiple_of(bounds->codes, 16) || !multiple_of(bounds->steps, 4))
+    return set_error(ctx, kErrArg, "%s: codes must be 16-byte and steps 4-byte aligned", what);
+  out->codes = reinterpret_cast<int8_t*>(bounds->codes);
+  out->steps = bounds->steps;
+  return kOk;
+}
+
+static bool stream_capturing(s3b_ctx* ctx) {
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(ctx->stream, &capture) != cudaSuccess) cudaGetLastError();
+  return capture != cudaStreamCaptureStatusNone;
+}
+
+// what graphs keep of buffers in powers of two is less than what is in use
+static size_t power_of_two(size_t n, size_t least) {
+  while (least < n) least *= 2;
+  return least;
+}
+
+int s3b_op_cache_bounds(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_bounds* bounds, const int32_t* pages,
+                        int64_t pages_stride, int max_pages, const int32_t* lengths, int batch, int64_t recent) {
+  int rc = ctx_enter(ctx);
+  if (rc) return rc;
+  KvAttnParams p;
+  KvCache shape;
+  KvBounds out;
+  if ((rc = kv_cache_arg(ctx, cache, &p.c))) return rc;
+  if ((rc = kv_bounds_arg(ctx, "cache_bounds", bounds, &shape, &out))) return rc;
+  if (shape.heads != p.c.heads || shape.d != p.c.d || shape.page_size != p.c.page_size || shape.n_pages != p.c.n_pages)
+    return set_error(ctx, kErrArg, "cache_bounds: the bounds have another shape than the cache");
+  if (recent < 0) return set_error(ctx, kErrArg, "cache_bounds: %lld tokens", (long long)recent);
+  if ((rc = kv_sequences(ctx, "cache_bounds", &p, pages, pages_stride, max_pages, lengths, batch))) return rc;
+  if (batch == 0 || max_pages == 0 || recent == 0) return kOk;
+  rc = kv_bounds(p, out, std::min<long long>(recent, (long long)max_pages * p.c.page_size), ctx->d_err, ctx->stream);
+  if (rc) return set_error(ctx, launcher_status_code(rc), "cache_bounds launch failed (%d)", rc);
+  count_launch(ctx);
+  return kOk;
+}
+
+int s3b_op_cache_select(s3b_ctx* ctx, const s3b_kv_bounds* bounds, const void* q, int64_t q_b, int64_t q_n, int64_t q_h,
+                        int32_t* selected, int keep, int share, int sink, int recent, float* scores,
+                        const int32_t* pages, int64_t pages_stride, int max_pages, const int32_t* lengths, int batch,
+                        int nq, int heads, int causal, int window) {
+  const char* what = "cache_select";
+  int rc = ctx_enter(ctx);
+  if (rc) return rc;
+  KvAttnParams p;
+  KvBounds b;
+  if ((rc = kv_bounds_arg(ctx, what, bounds, &p.c, &b))) return rc;
+  if ((rc = kv_sequences(ctx, what, &p, pages, pages_stride, max_pages, lengths, batch))) return rc;
+  if ((rc = kv_queries(ctx, what, &p, q, q_b, q_n, q_h, nq, heads, causal, window))) return rc;
+  if ((rc = kv_lists(ctx, what, &p, selected, keep, share))) return rc;
+  if (sink < 0 || recent < 0 || (long long)sink + recent > keep)
+    return set_error(ctx, kErrArg, "cache_select: %d first and %d last pages of %d", sink, recent, keep);
+  if (!multiple_of(scores, 4)) return set_error(ctx, kErrArg, "cache_select: scores must be 4-byte aligned");
+  if (batch == 0 || nq == 0) return kOk;
+  const bool capturing = stream_capturing(ctx), all = scores != nullptr;
+  const long long units = kv_attention_units(p);
+  if (units * std::max(max_pages, 1) > (1LL << 40))
+    return set_error(ctx, kErrUnsupported, "cache_select: %lld lists over %d pages", units, max_pages);
+  bool grown;
+  if (!all) {
+    DevBuf* buf = graph_buf(ctx, "kv_select_scores", power_of_two((size_t)units * max_pages * 4, 1 << 20), capturing, &grown, &rc);
+    if (rc) return rc;
+    scores = buf->as<float>();
+  }
+  DevBuf* count = graph_buf(ctx, "kv_select_count", power_of_two((size_t)units * 4, 1 << 16), capturing, &grown, &rc);
+  if (rc) return rc;
+  if (grown && cudaMemsetAsync(count->p, 0, count->bytes, ctx->stream) != cudaSuccess)
+    return set_error(ctx, kErrCuda, "cache_select: clearing the counts");
+  rc = kv_select(p, b, sink, recent, scores, all, count->as<int>(), selected, ctx->d_err, ctx->stream);
+  if (rc) return set_error(ctx, launcher_status_code(rc), "cache_select launch failed (%d)", rc);
+  count_launch(ctx);
+  return kOk;
+}
+
+int s3b_op_cache_attention_selected(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* q, int64_t q_b, int64_t q_n,
+                                    int64_t q_h, void* out, int out_f32, int64_t o_b, int64_t o_n, int64_t o_h,
+                                    float* lse, const int32_t* selected, int keep, int share, const int32_t* pages,
+                                    int64_t pages_stride, int max_pages, const int32_t* lengths, int batch, int nq,
+                                    int heads, float scale, int causal, int window) {
+  const char* what = "cache_attention_selected";
+  int rc = ctx_enter(ctx);
+  if (rc) return rc;
+  KvAttnParams p;
+  if ((rc = kv_cache_arg(ctx, cache, &p.c))) return rc;
+  if ((rc = kv_sequences(ctx, what, &p, pages, pages_stride, max_pages, lengths, batch))) return rc;
+  if ((rc = kv_queries(ctx, what, &p, q, q_b, q_n, q_h, nq, heads, causal, window))) return rc;
+  if ((rc = kv_lists(ctx, what, &p, selected, keep, share))) return rc;
+  if ((rc = kv_scale(ctx, what, &p, scale))) return rc;
+  // a list's groups of 16 tokens are counted in 32 bits
+  if ((long long)keep * p.c.page_size > kMaxCacheTokens)
+    return set_error(ctx, kErrUnsupported, "%s: a list may name %lld tokens at most", what, kMaxCacheTokens);
+  if (!rows_aligned(out, out_f32 ? 4 : 2, o_b, o_n, o_h))
+    return set_error(ctx, kErrArg, "%s: rows must start on 16-byte boundaries", what);
+  if (!multiple_of(lse, 4)) return set_error(ctx, kErrArg, "%s: lse must be 4-byte aligned", what);
+  if (batch == 0 || nq == 0) return kOk;
+  if (!out) return set_error(ctx, kErrArg, "%s: null pointer", what);
+  p.out = out;
+  p.out_f32 = out_f32 ? 1 : 0;
+  p.o_b = o_b;
+  p.o_n = o_n;
+  p.o_h = o_h;
+  p.lse = lse;
+  KvAttnWork w;
+  w.sms = num_sms();
+  const bool capturing = stream_capturing(ctx);
+  const KvAttnBytes need = kv_attention_work(p, w.sms);
+  bool grown;
+  DevBuf* part = graph_buf(ctx, "kv_attn_part", need.part, capturing, &grown, &rc);
+  if (rc) return rc;
+  w.part = part->as<float>();
+  DevBuf* count = graph_buf(ctx, "kv_attn_count", power_of_two(need.count, 1 << 16), capturing, &grown, &rc);
+  if (rc) return rc;
+  if (grown && cudaMemsetAsync(count->p, 0, count->bytes, ctx->stream) != cudaSuccess)
+    return set_error(ctx, kErrCuda, "%s: clearing the counts", what);
+  w.count = count->as<int>();
+  rc = kv_attention_selected(p, w, ctx->d_err, ctx->stream);
+  if (rc) return set_error(ctx, launcher_status_code(rc), "%s launch failed (%d)", what, rc);
+  count_launch(ctx);
+  return kOk;
+}
+
+int s3b_op_cache_weights(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* q, int64_t q_b, int64_t q_n, int64_t q_h,
+                         const float* lse, float* weights, int64_t w_b, int64_t w_h, float decay, const int32_t* pages,
+                         int64_t pages_stride, int max_pages, const int32_t* lengths, int batch, int nq, int heads,
+                         float scale, int causal, int window) {
+  const char* what = "cache_weights";
+  int rc = ctx_enter(ctx);
+  if (rc) return rc;
+  KvAttnParams p;
+  if ((rc = kv_cache_arg(ctx, cache, &p.c))) return rc;
+  if ((rc = kv_sequences(ctx, what, &p, pages, pages_stride, max_pages, lengths, batch))) return rc;
+  if ((rc = kv_queries(ctx, what, &p, q, q_b, q_n, q_h, nq, heads, causal, window))) return rc;
+  if ((rc = kv_scale(ctx, what, &p, scale))) return rc;
+  if (!(decay >= 0.f) || std::isinf(decay)) return set_error(ctx, kErrArg, "cache_weights: decay must be finite and not negative");
+  if (!multiple_of(lse, 4) || !multiple_of(weights, 4))
+    return set_error(ctx, kErrArg, "cache_weights: lse and weights must be 4-byte aligned");
+  if (batch == 0 || max_pages == 0) return kOk;
+  if (!weights || (!lse && nq > 0)) return set_error(ctx, kErrArg, "cache_weights: null pointer");
+  const long long tokens = (long long)max_pages * p.c.page_size, kv = p.c.heads;
+  const bool by_head = (kv == 1 || w_h >= tokens) && (batch == 1 || w_b >= (kv - 1) * (kv > 1 ? w_h : 0) + tokens);
+  const bool by_batch = (batch == 1 || w_b >= tokens) && (kv == 1 || w_h >= (batch - 1) * (batch > 1 ? w_b : 0) + tokens);
+  if (!by_head && !by_batch) return set_error(ctx, kErrArg, "cache_weights: rows of %lld weights overlap", tokens);
+  p.lse = const_cast<float*>(lse);
+  KvWeights w;
+  w.w = weights;
+  w.w_b = w_b;
+  w.w_h = w_h;
+  w.decay = decay;
+  const int sms = num_sms();
+  const size_t need = kv_weights_work(p, sms);
+  if (need) {
+    bool grown;
+    DevBuf* part = graph_buf(ctx, "kv_weights_part", power_of_two(need, 1 << 20), stream_capturing(ctx), &grown, &rc);
+    if (rc) return rc;
+    w.part = part->as<float>();
+  }
+  rc = kv_weights(p, w, sms, ctx->d_err, ctx->stream);
+  if (rc) return set_error(ctx, launcher_status_code(rc), "cache_weights launch failed (%d)", rc);
+  count_launch(ctx, kv_weights_launches(p, sms));
+  return kOk;
+}
+
+int s3b_op_cache_evict(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_cache* to, const float* weights,
+                       int64_t w_b, int64_t w_h, const int32_t* pages, int64_t pages_stride, int max_pages,
+                       const int32_t* lengths, int batch, int keep, int sink, int recent, const int32_t* pages_out,
+                       int64_t out_stride, int32_t* lengths_out, int32_t* kept, float* weights_out) {
+  const char* what = "cache_evict";
+  int rc = ctx_enter(ctx);
+  if (rc) return rc;
+  KvAttnParams p;
+  KvEvict e;
+  if ((rc = kv_cache_arg(ctx, cache, &p.c))) return rc;
+  if ((rc = kv_cache_arg(ctx, to ? to : cache, &e.to))) return rc;
+  if (e.to.type != p.c.type || e.to.heads != p.c.heads || e.to.d != p.c.d)
+    return set_error(ctx, kErrArg, "cache_evict: the new pages are of a cache of another type, heads or d");
+  if ((rc = kv_sequences(ctx, what, &p, pages, pages_stride, max_pages, lengths, batch))) return rc;
+  if (keep < 0 || sink < 0 || recent < 0 || (long long)sink + recent > keep)
+    return set_error(ctx, kErrArg, "cache_evict: %d first and %d last tokens of %d", sink, recent, keep);
+  const long long new_pages = ((long long)keep + e.to.page_size - 1) / e.to.page_size;
+  if (batch > 1 && out_stride < new_pages)
+    return set_error(ctx, kErrArg, "cache_evict: rows of %lld new pages hold no %lld", (long long)out_stride, new_pages);
+  if (!multiple_of(weights, 4) || !multiple_of(pages_out, 4) || !multiple_of(lengths_out, 4) || !multiple_of(kept, 4) ||
+      !multiple_of(weights_out, 4))
+    return set_error(ctx, kErrArg, "cache_evict: arrays must be 4-byte aligned");
+  if (batch == 0) return kOk;
+  if (!lengths_out || (keep > 0 && (!kept || !pages_out || (!weights && max_pages > 0))))
+    return set_error(ctx, kErrArg, "cache_evict: null pointer");
+  if (lengths_out == lengths) return set_error(ctx, kErrArg, "cache_evict: lengths_out is the array of lengths");
+  if ((long long)batch * p.c.heads > (1LL << 40) / std::max(keep, 1))
+    return set_error(ctx, kErrUnsupported, "cache_evict: %d sequences of %d heads keep %d tokens", batch, p.c.heads, keep);
+  if (weights_out) {  // the weights that are read, from the first to the last
+    const long long b0 = std::min<long long>(0, (batch - 1) * w_b), b1 = std::max<long long>(0, (batch - 1) * w_b);
+    const long long h0 = std::min<long long>(0, (p.c.heads - 1) * w_h), h1 = std::max<long long>(0, (p.c.heads - 1) * w_h);
+    const uintptr_t from = reinterpret_cast<uintptr_t>(weights) + (b0 + h0) * 4;
+    const uintptr_t end = reinterpret_cast<uintptr_t>(weights) + (b1 + h1 + (long long)max_pages * p.c.page_size) * 4;
+    const uintptr_t out = reinterpret_cast<uintptr_t>(weights_out), out_end = out + (uintptr_t)batch * p.c.heads * keep * 4;
+    if (out < end && from < out_end) return set_error(ctx, kErrArg, "cache_evict: weights_out lies over the weights");
+  }
+  e.weights = weights;
+  e.w_b = w_b;
+  e.w_h = w_h;
+  e.pages_out = pages_out;
+  e.out_stride = out_stride;
+  e.lengths_out = lengths_out;
+  e.kept = kept;
+  e.weights_out = weights_out;
+  e.keep = keep;
+  e.sink = sink;
+  e.recent = recent;
+  rc = kv_evict(p, e, ctx->d_err, ctx->stream);
+  if (rc) return set_error(ctx, launcher_status_code(rc), "cache_evict launch failed (%d)", rc);
+  count_launch(ctx, keep > 0 ? 2 : 1);
+  return kOk;
+}
+
 int s3b_op_dequantize(s3b_ctx* ctx, const void* src, int type, int64_t ne0, int64_t nrows, float* dst) {
   int rc = ctx_enter(ctx);
   if (rc) return rc;

@@ -393,7 +393,14 @@ struct KvAttnParams {
   int batch = 0, nq = 0, heads = 0;
   float scale = 1.f;
   int causal = 0, window = 0;
+  // s3b_op_cache_attention_selected: lists of `keep` pages for blocks of `share` queries (0: all pages, one block)
+  const int* selected = nullptr;
+  int keep = 0, share = 0;
 };
+// Units of the attention over few rows: sequences x key / value heads x blocks of queries.
+inline long long kv_attention_units(const KvAttnParams& p) {
+  return (long long)p.batch * p.c.heads * (p.share ? (p.nq - 1) / p.share + 1 : 1);
+}
 // Workspace of the attention: parts of units that several CTAs share; their arrival counts, which are zero before and after
 // every launch; f16 images of the operands where they are staged.
 struct KvAttnWork {
@@ -413,5 +420,45 @@ size_t kv_attention_tc_parts(int sms);                 // bytes of the parts, th
 size_t kv_attention_tc_image(const KvAttnParams& p);
 int kv_attention_tc(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st);
 int kv_attention_tc_launches(const KvAttnParams& p);
+// The same over the pages of lists (p.selected), for up to kv_attention_most_rows(d) rows of a list.
+int kv_attention_most_rows(int d);
+int kv_attention_selected(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st);
+
+// s3b_kv_bounds: codes [n_pages][heads][2][d] (lowest, highest), steps [n_pages][heads].
+struct KvBounds {
+  int8_t* codes = nullptr;
+  float* steps = nullptr;
+};
+// Bounds of the pages that hold the last `recent` tokens of each sequence (p: cache, pages, lengths).
+int kv_bounds(const KvAttnParams& p, const KvBounds& out, long long recent, int* err, cudaStream_t st);
+// Chooses p.keep pages for each block of p.share queries and key / value head (p: queries, pages, lengths, masks; of p.c the
+// shape). scores: [units][max_pages], of all pages with `all`, else a workspace; count: [units], zero before and after.
+int kv_select(const KvAttnParams& p, const KvBounds& bounds, int sink, int recent, float* scores, bool all, int* count,
+              int* selected, int* err, cudaStream_t st);
+
+// s3b_op_cache_weights: w = decay * w + sum over rows of exp(scale q k - lse) (p: everything but out; p.lse is read).
+struct KvWeights {
+  float* w = nullptr;
+  long long w_b = 0, w_h = 0;
+  float decay = 1.f;
+  float* part = nullptr;  // workspace where the rows are split
+};
+size_t kv_weights_work(const KvAttnParams& p, int sms);
+int kv_weights(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st);
+int kv_weights_launches(const KvAttnParams& p, int sms);
+
+// s3b_op_cache_evict: `keep` tokens of each sequence and head, moved into `to` (p: source cache, pages, lengths).
+struct KvEvict {
+  KvCache to;
+  const float* weights = nullptr;
+  long long w_b = 0, w_h = 0;
+  const int* pages_out = nullptr;
+  long long out_stride = 0;
+  int* lengths_out = nullptr;
+  int* kept = nullptr;           // [batch][heads][keep]
+  float* weights_out = nullptr;  // the same shape, or none
+  int keep = 0, sink = 0, recent = 0;
+};
+int kv_evict(const KvAttnParams& p, const KvEvict& e, int* err, cudaStream_t st);
 
 }  // namespace s3b
