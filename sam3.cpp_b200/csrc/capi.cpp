@@ -1683,21 +1683,18 @@ int s3b_op_cache_select(s3b_ctx* ctx, const s3b_kv_bounds* bounds, const void* q
     return set_error(ctx, kErrArg, "cache_select: %d first and %d last pages of %d", sink, recent, keep);
   if (!multiple_of(scores, 4)) return set_error(ctx, kErrArg, "cache_select: scores must be 4-byte aligned");
   if (batch == 0 || nq == 0) return kOk;
-  const bool capturing = stream_capturing(ctx), all = scores != nullptr;
+  const bool all = scores != nullptr;
   const long long units = kv_attention_units(p);
   if (units * std::max(max_pages, 1) > (1LL << 40))
     return set_error(ctx, kErrUnsupported, "cache_select: %lld lists over %d pages", units, max_pages);
-  bool grown;
-  if (!all) {
-    DevBuf* buf = graph_buf(ctx, "kv_select_scores", power_of_two((size_t)units * max_pages * 4, 1 << 20), capturing, &grown, &rc);
+  const int sms = num_sms();
+  if (!all && kv_select_needs_scores(p, sms)) {
+    bool grown;
+    DevBuf* buf = graph_buf(ctx, "kv_select_scores", power_of_two((size_t)units * max_pages * 4, 1 << 20), stream_capturing(ctx), &grown, &rc);
     if (rc) return rc;
     scores = buf->as<float>();
   }
-  DevBuf* count = graph_buf(ctx, "kv_select_count", power_of_two((size_t)units * 4, 1 << 16), capturing, &grown, &rc);
-  if (rc) return rc;
-  if (grown && cudaMemsetAsync(count->p, 0, count->bytes, ctx->stream) != cudaSuccess)
-    return set_error(ctx, kErrCuda, "cache_select: clearing the counts");
-  rc = kv_select(p, b, sink, recent, scores, all, count->as<int>(), selected, ctx->d_err, ctx->stream);
+  rc = kv_select(p, b, sink, recent, scores, all, selected, sms, ctx->d_err, ctx->stream);
   if (rc) return set_error(ctx, launcher_status_code(rc), "cache_select launch failed (%d)", rc);
   count_launch(ctx);
   return kOk;

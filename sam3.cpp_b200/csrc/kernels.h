@@ -432,9 +432,10 @@ struct KvBounds {
 // Bounds of the pages that hold the last `recent` tokens of each sequence (p: cache, pages, lengths).
 int kv_bounds(const KvAttnParams& p, const KvBounds& out, long long recent, int* err, cudaStream_t st);
 // Chooses p.keep pages for each block of p.share queries and key / value head (p: queries, pages, lengths, masks; of p.c the
-// shape). scores: [units][max_pages], of all pages with `all`, else a workspace; count: [units], zero before and after.
-int kv_select(const KvAttnParams& p, const KvBounds& bounds, int sink, int recent, float* scores, bool all, int* count,
-              int* selected, int* err, cudaStream_t st);
+// shape). scores: [units][max_pages], of all pages with `all`, else a workspace, or none unless kv_select_needs_scores.
+int kv_select(const KvAttnParams& p, const KvBounds& bounds, int sink, int recent, float* scores, bool all, int* selected, int sms,
+              int* err, cudaStream_t st);
+bool kv_select_needs_scores(const KvAttnParams& p, int sms);
 
 // s3b_op_cache_weights: w = decay * w + sum over rows of exp(scale q k - lse) (p: everything but out; p.lse is read).
 struct KvWeights {

@@ -8,16 +8,19 @@ namespace s3b {
 
 namespace {
 
-constexpr int kThreads = 1024, kKeys = 16;  // of choose_kernel: a CTA keeps 16384 keys in registers
+constexpr int kThreads = 1024;
+constexpr int kMostKeys = 49152;  // weights of a CTA whose keys stay in its shared memory
 
 struct EvictArgs {
   KvAttnParams p;  // source cache, pages, lengths
   KvEvict e;
+  int keys;  // room for so many in a CTA's shared memory; those of more tokens are made from the weights again
 };
 
 // A unit is a sequence and a key / value head: one CTA, or a cluster of them (CL) that share the tokens.
 template <int CL>
 __global__ void __launch_bounds__(kThreads) choose_kernel(const __grid_constant__ EvictArgs a, int* err) {
+  extern __shared__ uint32_t s_keys[];
   __shared__ TopShared<kThreads> s_top;
   const KvAttnParams& p = a.p;
   const int unit = blockIdx.x / CL, rank = blockIdx.x % CL;
@@ -38,15 +41,23 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const __grid_constant_
     }
     return;
   }
-  const int share = (int)(((long long)len + 32 * CL - 1) / (32 * CL)) * 32, first = min((long long)rank * share, (long long)len);
+  const int share = CL > 1 ? (int)(((long long)len + 32 * CL - 1) / (32 * CL)) * 32 : len;
+  const int first = (int)min((long long)rank * share, (long long)len), n = min(share, len - first);
   const int sink = a.e.sink, from = len - a.e.recent;
-  top_select<kThreads, kKeys, CL>(
-      s_top, first, min(share, len - first), (uint32_t)keep,
-      [&](int i) { return i < sink || i >= from ? kTopForced : top_key(weights[i]); },
-      [&](uint32_t at, int i, uint32_t) {
-        kept[at] = i;
-        if (out) out[at] = weights[i];
-      });
+  weights += first;
+  auto key = [&](int i) { return first + i < sink || first + i >= from ? kTopForced : top_key(weights[i]); };
+  auto emit = [&](uint32_t at, int i) {
+    kept[at] = first + i;
+    if (out) out[at] = weights[i];
+  };
+  if (share <= a.keys) {
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n; i += kThreads) s_keys[i] = key(i);
+    __syncthreads();
+    top_select<kThreads, CL>(s_top, n, (uint32_t)keep, [&](int i) { return s_keys[i]; }, emit);
+  } else {
+    top_select<kThreads, CL>(s_top, n, (uint32_t)keep, key, emit);
+  }
 }
 
 template <typename V>
@@ -159,32 +170,24 @@ EvictKernel move_for(int d) {
   return d == 64 ? move_kernel<QT, 64> : d == 128 ? move_kernel<QT, 128> : move_kernel<QT, 256>;
 }
 
-int launch_cluster(EvictKernel k, unsigned grid, int threads, unsigned cluster, cudaStream_t st, const EvictArgs& a, int* err) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = cluster;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, k, a, err) == cudaSuccess ? 0 : -12;
+EvictKernel choose_for(int cl) {
+  return cl == 1 ? choose_kernel<1> : cl == 2 ? choose_kernel<2> : cl == 4 ? choose_kernel<4> : choose_kernel<8>;
 }
 
 }  // namespace
 
 int kv_evict(const KvAttnParams& p, const KvEvict& e, int* err, cudaStream_t st) {
-  const EvictArgs a{p, e};
   const long long units = (long long)p.batch * p.c.heads, moves = (units * ((e.keep + 15) / 16) + 3) / 4;
   if (units > 0x7fffffffLL / 8 || moves > 0x7fffffffLL) return -2;
-  // one CTA a unit as far as its registers hold a sequence's keys, and where the units alone fill the GPU
-  const bool cluster = (long long)p.max_pages * p.c.page_size > kThreads * kKeys && units < num_sms();
-  int rc = cluster ? launch_cluster(choose_kernel<8>, (unsigned)units * 8, kThreads, 8, st, a, err)
-                   : launch_dependent(choose_kernel<1>, dim3((unsigned)units), kThreads, 0, st, a, err);
+  // CTAs of a unit: 4096 tokens each or more, as far as there are SMs for them and clusters go
+  const long long tokens = (long long)p.max_pages * p.c.page_size;
+  int cl = 1;
+  while (cl < 8 && (long long)cl * 4096 < tokens && units * cl * 2 <= num_sms()) cl *= 2;
+  const long long share = cl > 1 ? (tokens + 32 * cl - 1) / (32 * cl) * 32 : tokens;
+  const EvictArgs a{p, e, (int)std::min<long long>(share, kMostKeys)};
+  const EvictKernel choose = choose_for(cl);
+  if (kernel_setup(choose, kMostKeys * 4) <= 0) return -13;
+  int rc = launch_clusters(choose, (unsigned)units * cl, kThreads, (size_t)a.keys * 4, cl, st, a, err);
   if (rc || e.keep == 0) return rc;
   const EvictKernel k = p.c.type == QT_Q4_0 ? move_for<QT_Q4_0>(p.c.d)
                                             : p.c.type == QT_Q4_1 ? move_for<QT_Q4_1>(p.c.d) : move_for<QT_Q8_0>(p.c.d);

@@ -9,17 +9,16 @@ namespace s3b {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSpan = 512;  // pages of a CTA: 16 at a time for each of 8 warps, four times
+constexpr int kMostKeys = 24576;  // pages of a CTA whose scores' keys stay in its shared memory
 
 struct SelectArgs {
   KvAttnParams p;  // c: heads, d, page_size, n_pages; q; pages, lengths; share, keep; causal, window
   KvBounds bounds;
   int sink, recent;
-  float* scores;   // [units][max_pages]
-  bool all;        // the scores of all pages are wanted
-  int* count;      // [units], zero between launches
+  float* scores;   // [units][max_pages], or none
+  bool all;        // they are wanted, of all pages
   int* selected;   // [units][keep]
-  int splits;      // CTAs of a unit
+  int keys;        // room for so many in a CTA's shared memory; those of more pages are made from the scores again
 };
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -29,20 +28,19 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A unit is a block of queries and a key / value head; its CTAs take 512 pages each, and the last of them to end chooses.
-// Whole numbers carry the score: sum over channels of max(c low, c high) = c+ high + c- low with c+ = max(c, 0), c- = min(c, 0), two
-// products of 8-bit codes (16 pages x 32 channels x 8 rows an instruction), exact in 32 bits; then two f32 products, each
-// rounded, so that the choice is the same whatever the order. Lane (g, t) holds 16 channels of 64 as the contraction's share of
-// its rows (pages g, g + 8; query row g): whole 16-byte words of both.
-template <int D, int NT>
+// A unit is a block of queries and a key / value head, of one CTA or a cluster of them (CL) that share its pages and then choose
+// together (kv_top.cuh). Whole numbers carry the score: sum over channels of max(c low, c high) = c+ high + c- low with
+// c+ = max(c, 0), c- = min(c, 0), two products of 8-bit codes (16 pages x 32 channels x 8 rows an instruction), exact in 32 bits;
+// then two f32 products, each rounded, so that the choice is the same whatever the order. Lane (g, t) holds 16 channels of 64 as
+// the contraction's share of its rows (pages g, g + 8; query row g): whole 16-byte words of both.
+template <int D, int NT, int CL>
 __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant__ SelectArgs a, int* err) {
   constexpr int NC = D / 64;
+  extern __shared__ uint32_t s_keys[];
   __shared__ TopShared<kThreads> s_top;
-  __shared__ int s_last;
   const KvAttnParams& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const long long unit = blockIdx.x / a.splits;
-  const int split = blockIdx.x % a.splits;
+  const long long unit = blockIdx.x / CL;
   const int blocks = (p.nq - 1) / p.share + 1;
   const int head = (int)(unit % p.c.heads), b = (int)(unit / p.c.heads / blocks);
   const int i0 = (int)(unit / p.c.heads % blocks) * p.share, i1 = min(i0 + p.share, p.nq);
@@ -55,17 +53,19 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
   row_span(p, len, i1 - 1, &none, &hi);
   const int pa = lo / p.c.page_size, pe = max(pa, (int)((hi + (long long)p.c.page_size - 1) / p.c.page_size));
   const int n = pe - pa;
+  // this CTA's pages
+  const int rank = CL > 1 ? blockIdx.x % CL : 0;
+  const int share = CL > 1 ? ((n + CL - 1) / CL + 31) / 32 * 32 : n;
+  const int begin = pa + (int)min((long long)n, (long long)rank * share), end = min(pe, begin + share);
   int* selected = a.selected + unit * p.keep;
   float* scores = a.scores + unit * p.max_pages;
-  const int begin = split * kSpan, end = min(begin + kSpan, p.max_pages);
-  const bool trivial = n <= p.keep;
-  if (trivial && split == 0)
+  const bool trivial = n <= p.keep, in_smem = share <= a.keys;
+  if (trivial && rank == 0)
     for (int e = threadIdx.x; e < p.keep; e += kThreads) selected[e] = e < n ? pa + e : -1;
   if (trivial && !a.all) return;
   if (a.all)
-    for (int j = begin + threadIdx.x; j < end; j += kThreads)
+    for (int j = rank * kThreads + threadIdx.x; j < p.max_pages; j += CL * kThreads)
       if (j < pa || j >= pe) scores[j] = -INFINITY;
-  if (begin >= pe || end <= pa) return;
 
   // ---- the query rows' codes, of either sign apart: column g of tile nt is row 8 nt + g
   uint32_t pos[NT][NC][4], neg[NT][NC][4];
@@ -124,8 +124,8 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
 
   // ---- scores of 16 pages at a time
   const int* table = p.pages + b * p.pages_stride;
+  const int sink = pa + a.sink, recent = pe - a.recent;
   for (int j0 = begin + 16 * warp; j0 < end; j0 += 16 * (kThreads / 32)) {
-    if (j0 >= pe || j0 + 16 <= pa) continue;
     uint4 low[2][NC], high[2][NC];
     float page_step[2];
 #pragma unroll
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
       page_step[u] = 0.f;
 #pragma unroll
       for (int c = 0; c < NC; ++c) low[u][c] = high[u][c] = make_uint4(0, 0, 0, 0);
-      if (j >= pa && j < pe) {
+      if (j < end) {
         long long page = table[j];
         if (page < 0 || page >= p.c.n_pages) {
           atomicCAS(err, 0, kDevErrIndex);
@@ -172,46 +172,58 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
       best[u] = fmaxf(best[u], __shfl_xor_sync(~0u, best[u], 1));
       best[u] = fmaxf(best[u], __shfl_xor_sync(~0u, best[u], 2));
       const int j = j0 + g + 8 * u;
-      if (t == 0 && j >= pa && j < pe) __stcg(scores + j, best[u]);
+      if (t == 0 && j < end) {
+        if (in_smem) s_keys[j - begin] = j < sink || j >= recent ? kTopForced : top_key(best[u]);
+        if (a.all || !in_smem) scores[j] = best[u];
+      }
     }
   }
   if (trivial) return;
-
-  // ---- the choice, by the CTA of the unit that ends last
-  const int needed = (pe - 1) / kSpan - pa / kSpan + 1;
-  __threadfence();
   __syncthreads();
-  if (needed > 1) {
-    if (threadIdx.x == 0) s_last = atomicAdd(a.count + unit, 1) == needed - 1;
-    __syncthreads();
-    if (!s_last) return;
-    __threadfence();
-    if (threadIdx.x == 0) a.count[unit] = 0;
+  auto emit = [&](uint32_t at, int i) { selected[at] = begin + i; };
+  if (in_smem) {
+    top_select<kThreads, CL>(s_top, end - begin, (uint32_t)p.keep, [&](int i) { return s_keys[i]; }, emit);
+  } else {
+    top_select<kThreads, CL>(
+        s_top, end - begin, (uint32_t)p.keep,
+        [&](int i) { return begin + i < sink || begin + i >= recent ? kTopForced : top_key(scores[begin + i]); }, emit);
   }
-  const int sink = a.sink, recent = a.recent;
-  top_select<kThreads, 16, 1>(
-      s_top, 0, n, (uint32_t)p.keep,
-      [&](int i) { return i < sink || i >= n - recent ? kTopForced : top_key(__ldcg(scores + pa + i)); },
-      [&](uint32_t at, int i, uint32_t) { selected[at] = pa + i; });
 }
 
 typedef void (*SelectKernel)(SelectArgs, int*);
 
-template <int D>
-SelectKernel select_for(int rows) {
-  return rows <= 8 ? select_kernel<D, 1> : D == 256 || rows <= 16 ? select_kernel<D, 2> : select_kernel<D, D == 256 ? 2 : 4>;
+template <int D, int CL>
+SelectKernel select_rows(int rows) {
+  return rows <= 8 ? select_kernel<D, 1, CL> : D == 256 || rows <= 16 ? select_kernel<D, 2, CL> : select_kernel<D, D == 256 ? 2 : 4, CL>;
 }
+template <int CL>
+SelectKernel select_for(int d, int rows) {
+  return d == 64 ? select_rows<64, CL>(rows) : d == 128 ? select_rows<128, CL>(rows) : select_rows<256, CL>(rows);
+}
+
+// CTAs of a unit: about 512 pages each (4 for each warp's step of 16), as far as there are SMs for them and clusters go
+int select_cluster(const KvAttnParams& p, int sms) {
+  int cl = 1;
+  while (cl < 8 && (long long)cl * 512 < p.max_pages && kv_attention_units(p) * cl * 2 <= 2LL * sms) cl *= 2;
+  return cl;
+}
+// pages of the largest share of a CTA
+long long select_share(const KvAttnParams& p, int cl) { return cl > 1 ? ((p.max_pages + cl - 1LL) / cl + 31) / 32 * 32 : p.max_pages; }
 
 }  // namespace
 
-int kv_select(const KvAttnParams& p, const KvBounds& bounds, int sink, int recent, float* scores, bool all, int* count,
-              int* selected, int* err, cudaStream_t st) {
-  SelectArgs a{p, bounds, sink, recent, scores, all, count, selected, std::max(1, (p.max_pages + kSpan - 1) / kSpan)};
-  const long long grid = kv_attention_units(p) * a.splits;
+bool kv_select_needs_scores(const KvAttnParams& p, int sms) { return select_share(p, select_cluster(p, sms)) > kMostKeys; }
+
+int kv_select(const KvAttnParams& p, const KvBounds& bounds, int sink, int recent, float* scores, bool all, int* selected, int sms,
+              int* err, cudaStream_t st) {
+  const int cl = select_cluster(p, sms);
+  const long long share = select_share(p, cl), grid = kv_attention_units(p) * cl;
   if (grid > 0x7fffffffLL) return -2;
-  const int rows = p.share * (p.heads / p.c.heads);
-  const SelectKernel k = p.c.d == 64 ? select_for<64>(rows) : p.c.d == 128 ? select_for<128>(rows) : select_for<256>(rows);
-  return launch_dependent(k, dim3((unsigned)grid), kThreads, 0, st, a, err);
+  const SelectArgs a{p, bounds, sink, recent, scores, all, selected, (int)std::min<long long>(share, kMostKeys)};
+  const int rows = p.share * (p.heads / p.c.heads), d = p.c.d;
+  const SelectKernel k = cl == 1 ? select_for<1>(d, rows) : cl == 2 ? select_for<2>(d, rows) : cl == 4 ? select_for<4>(d, rows) : select_for<8>(d, rows);
+  if (kernel_setup(k, kMostKeys * 4) <= 0) return -13;
+  return launch_clusters(k, (unsigned)grid, kThreads, (size_t)a.keys * 4, cl, st, a, err);
 }
 
 }  // namespace s3b

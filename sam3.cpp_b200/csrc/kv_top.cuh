@@ -20,90 +20,94 @@ __device__ __forceinline__ uint32_t cluster_load(const uint32_t* p, uint32_t ran
 
 template <int T>
 struct TopShared {
-  uint32_t hist[256 * 32];  // a digit's count, apart for each lane: no two lanes of a warp meet in a bank
-  uint32_t total[2][256];   // of this CTA, by digit; two of them, so that one round's may still be read during the next
+  static constexpr int kCopies = T >= 1024 ? 16 : 8;
+  uint32_t hist[256 * kCopies];  // a digit's counts, apart for lanes that differ modulo kCopies: keys of one size share their digits
+  uint32_t total[2][256];        // of this CTA, by digit; two of them, so that one round's may still be read during the next
+  uint32_t warp_sum[8];
   uint32_t above[T / 32], equal[T / 32], cta[2];
   uint32_t digit, left, count;
 };
 
 // Radix selection from the top, 8 bits a round: the digit in which the k-th largest lies, then the same among the keys that
-// share it. Each of a cluster's CTAs (CL: 1, or the cluster's size) has the places [first, first + n) of a line; within it each
-// warp has a run of rows of 32. key(i) is asked for place i (of the whole line) once where a thread's share fits KPT registers,
-// in every round otherwise. emit(position, place, key) is called for the taken ones, k of them in all (k <= the line's length,
-// and at least the number of forced keys).
-template <int T, int KPT, int CL, typename Key, typename Emit>
-__device__ void top_select(TopShared<T>& s, int first, int n, uint32_t k, Key key, Emit emit) {
-  constexpr int W = T / 32;
+// share it; it ends with the round in which all of those are taken. Each of a cluster's CL CTAs has n places of a line, one CTA's
+// behind another's; within a CTA each warp has a run of rows of 32. key(i) is asked for its place i in every round: from shared
+// memory where they fit. emit(position, place) is called for the taken ones, k of them in all (0 < k <= the line's length, and at
+// least the number of forced keys).
+template <int T, int CL, typename Key, typename Emit>
+__device__ void top_select(TopShared<T>& s, int n, uint32_t k, Key key, Emit emit) {
+  constexpr int W = T / 32, C = TopShared<T>::kCopies, P = T / 256;  // P threads a digit
+  static_assert(T >= 256 && T % 256 == 0 && C % P == 0, "threads of top_select");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows_all = (n + 31) / 32, rows_warp = (rows_all + W - 1) / W;
-  const int base = warp * rows_warp * 32;                       // of this warp's run, from `first`
-  const int rows = max(0, min(rows_warp, rows_all - warp * rows_warp));
-  const bool kept = rows_warp <= KPT;
-  uint32_t keys[KPT];
-  if (kept) {
-#pragma unroll
-    for (int r = 0; r < KPT; ++r) keys[r] = r < rows && base + r * 32 + lane < n ? key(first + base + r * 32 + lane) : 0u;
-  }
-  // f(row, whether there is a key, key): a whole warp each
+  const int from = min(warp * rows_warp, rows_all) * 32, to = min(n, from + rows_warp * 32);  // of this warp's run
+  // f(whether there is a key, place, key): a whole warp each
   auto each = [&](auto&& f) {
-    if (kept) {
+    constexpr int U = 4;
+    for (int i0 = from; i0 < to; i0 += 32 * U) {
+      uint32_t x[U];
 #pragma unroll
-      for (int r = 0; r < KPT; ++r)
-        if (r < rows) f(r, base + r * 32 + lane < n, keys[r]);
-    } else {
-      for (int r = 0; r < rows; ++r) {
-        const bool there = base + r * 32 + lane < n;
-        f(r, there, there ? key(first + base + r * 32 + lane) : 0u);
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + 32 * u + lane;
+        x[u] = i < to ? key(i) : 0u;
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + 32 * u < to) f(i0 + 32 * u + lane < to, i0 + 32 * u + lane, x[u]);
     }
   };
-  for (int e = threadIdx.x; e < 256 * 32; e += T) s.hist[e] = 0;
+#pragma unroll
+  for (int e = 0; e < 256 * C / T; ++e) s.hist[e * T + threadIdx.x] = 0;
   uint32_t prefix = 0, left = k;
   uint32_t from_above = 1, from_equal = 0;  // keys >= from_above are taken, then the first of those >= from_equal
 #pragma unroll 1
   for (int round = 0; round < 4; ++round) {
     const int shift = 24 - 8 * round;
     __syncthreads();
-    each([&](int, bool there, uint32_t x) {
-      if (there && (round == 0 || (x ^ prefix) >> (shift + 8) == 0)) atomicAdd(&s.hist[(x >> shift & 255) * 32 + lane], 1u);
+    each([&](bool there, int, uint32_t x) {
+      if (there && (round == 0 || (x ^ prefix) >> (shift + 8) == 0)) atomicAdd(&s.hist[(x >> shift & 255) * C + lane % C], 1u);
     });
     __syncthreads();
-    for (int bin = warp; bin < 256; bin += W) {
-      const uint32_t c = __reduce_add_sync(~0u, s.hist[bin * 32 + lane]);
-      s.hist[bin * 32 + lane] = 0;
-      if (lane == 0) s.total[round & 1][bin] = c;
+    {  // the digit's copies, P threads share them; rotated, so that a warp's lanes meet in no bank
+      uint32_t* h = s.hist + threadIdx.x / P * C;
+      uint32_t c = 0;
+#pragma unroll
+      for (int e = 0; e < C / P; ++e) {
+        const int at = (threadIdx.x % P) * (C / P) + (e + threadIdx.x / (P * (32 / C))) % (C / P);
+        c += h[at];
+        h[at] = 0;
+      }
+#pragma unroll
+      for (int x = 1; x < P; x <<= 1) c += __shfl_xor_sync(~0u, c, x);
+      if (threadIdx.x % P == 0) s.total[round & 1][threadIdx.x / P] = c;
     }
     if (CL > 1) cluster_sync_all();
     else __syncthreads();
-    if (warp == 0) {  // lane i: the 8 digits from 255 - 8 i down
-      uint32_t c[8], sum = 0;
+    uint32_t c = 0, end = 0;
+    if (warp < 8) {  // thread i: digit 255 - i, and how many have it or a higher one
+      const uint32_t* at = &s.total[round & 1][255 - threadIdx.x];
+      if (CL > 1) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        c[e] = 0;
-#pragma unroll
-        for (int r = 0; r < CL; ++r) {
-          const uint32_t* at = &s.total[round & 1][255 - 8 * lane - e];
-          c[e] += CL > 1 ? cluster_load(at, r) : *at;
-        }
-        sum += c[e];
+        for (int r = 0; r < CL; ++r) c += cluster_load(at, r);
+      } else {
+        c = *at;
       }
-      uint32_t end = sum;
+      end = c;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
         const uint32_t up = __shfl_up_sync(~0u, end, x);
         if (lane >= x) end += up;
       }
-      uint32_t before = end - sum;
-      if (before < left && left <= end) {
+      if (lane == 31) s.warp_sum[warp] = end;
+    }
+    __syncthreads();
+    if (warp < 8) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (before < left && left <= before + c[e]) {
-            s.digit = 255 - 8 * lane - e;
-            s.left = left - before;
-            s.count = c[e];
-          }
-          before += c[e];
-        }
+      for (int w = 0; w < 7; ++w)
+        if (w < warp) end += s.warp_sum[w];
+      if (end - c < left && left <= end) {
+        s.digit = 255 - threadIdx.x;
+        s.left = left - (end - c);
+        s.count = c;
       }
     }
     __syncthreads();
@@ -119,29 +123,52 @@ __device__ void top_select(TopShared<T>& s, int first, int n, uint32_t k, Key ke
   }
   // places of what each warp takes
   uint32_t above = 0, equal = 0;
-  each([&](int, bool there, uint32_t x) {
+  each([&](bool there, int, uint32_t x) {
     above += __popc(__ballot_sync(~0u, there && x >= from_above));
     equal += __popc(__ballot_sync(~0u, there && x >= from_equal && x < from_above));
   });
   if (lane == 0) s.above[warp] = above, s.equal[warp] = equal;
   __syncthreads();
-  uint32_t a = 0, q = 0;
-  for (int w = 0; w < warp; ++w) a += s.above[w], q += s.equal[w];
+  uint32_t a = lane < warp ? s.above[lane] : 0, q = lane < warp ? s.equal[lane] : 0;
+  a = __reduce_add_sync(~0u, a);
+  q = __reduce_add_sync(~0u, q);
   if (CL > 1) {
     if (threadIdx.x == T - 32) s.cta[0] = a + above, s.cta[1] = q + equal;  // the last warp's
     cluster_sync_all();
     const uint32_t rank = cluster_rank();
-    for (uint32_t r = 0; r < rank; ++r) a += cluster_load(&s.cta[0], r), q += cluster_load(&s.cta[1], r);
+    uint32_t ca = lane < (int)rank ? cluster_load(&s.cta[0], lane) : 0, cq = lane < (int)rank ? cluster_load(&s.cta[1], lane) : 0;
+    a += __reduce_add_sync(~0u, ca);
+    q += __reduce_add_sync(~0u, cq);
   }
-  each([&](int r, bool there, uint32_t x) {
+  each([&](bool there, int i, uint32_t x) {
     const bool is_above = there && x >= from_above, is_equal = there && x >= from_equal && x < from_above;
     const uint32_t ma = __ballot_sync(~0u, is_above), mq = __ballot_sync(~0u, is_equal), below = (1u << lane) - 1;
     const uint32_t pa = a + __popc(ma & below), pq = q + __popc(mq & below);
-    if (is_above || (is_equal && pq < left)) emit(pa + min(pq, left), first + base + r * 32 + lane, x);
+    if (is_above || (is_equal && pq < left)) emit(pa + min(pq, left), i);
     a += __popc(ma);
     q += __popc(mq);
   });
   if (CL > 1) cluster_sync_all();  // no CTA leaves while another reads its counts
+}
+
+// Launch of a kernel whose blocks form clusters of `cluster` (16: the kernel has to allow more than the portable 8), and that
+// may take its place while its predecessor runs.
+template <typename K, typename... A>
+int launch_clusters(K* kernel, unsigned grid, int threads, size_t smem, unsigned cluster, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? 0 : -12;
 }
 
 }  // namespace s3b
