@@ -31,14 +31,10 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const __grid_constant_
   const int keep = a.e.keep, m = min(len, keep);
   const float* weights = a.e.weights + b * a.e.w_b + head * a.e.w_h;
   int* kept = a.e.kept + (long long)unit * keep;
-  float* out = a.e.weights_out ? a.e.weights_out + (long long)unit * keep : nullptr;
   if (head == 0 && rank == 0 && threadIdx.x == 0) a.e.lengths_out[b] = m;
   if (keep == 0) return;
   if (len <= keep) {
-    for (int i = rank * kThreads + threadIdx.x; i < keep; i += CL * kThreads) {
-      kept[i] = i < len ? i : -1;
-      if (out) out[i] = i < len ? weights[i] : 0.f;
-    }
+    for (int i = rank * kThreads + threadIdx.x; i < keep; i += CL * kThreads) kept[i] = i < len ? i : -1;
     return;
   }
   const int share = CL > 1 ? (int)(((long long)len + 32 * CL - 1) / (32 * CL)) * 32 : len;
@@ -46,17 +42,12 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const __grid_constant_
   const int sink = a.e.sink, from = len - a.e.recent;
   weights += first;
   auto key = [&](int i) { return first + i < sink || first + i >= from ? kTopForced : top_key(weights[i]); };
-  auto emit = [&](uint32_t at, int i) {
-    kept[at] = first + i;
-    if (out) out[at] = weights[i];
-  };
+  auto emit = [&](uint32_t at, int i) { kept[at] = first + i; };
   if (share <= a.keys) {
-#pragma unroll 8
-    for (int i = threadIdx.x; i < n; i += kThreads) s_keys[i] = key(i);
-    __syncthreads();
-    top_select<kThreads, CL>(s_top, n, (uint32_t)keep, [&](int i) { return s_keys[i]; }, emit);
+    top_select<kThreads, CL>(
+        s_top, n, (uint32_t)keep, [&](int i) { return s_keys[i] = key(i); }, [&](int i) { return s_keys[i]; }, emit);
   } else {
-    top_select<kThreads, CL>(s_top, n, (uint32_t)keep, key, emit);
+    top_select<kThreads, CL>(s_top, n, (uint32_t)keep, key, key, emit);
   }
 }
 
@@ -94,8 +85,12 @@ __global__ void __launch_bounds__(128) move_kernel(const __grid_constant__ Evict
   const int i0 = (int)(item % groups) * 16;
   const int head = (int)(unit % p.c.heads), b = (int)(unit / p.c.heads);
   const int m = min(sequence_length(p, b, err), a.e.keep);
+  float* w_out = a.e.weights_out ? a.e.weights_out + unit * a.e.keep + i0 + lane : nullptr;
+  if (w_out && lane < 16 && i0 + lane >= m && i0 + lane < a.e.keep) *w_out = 0.f;
   if (i0 >= m) return;
   const int n = min(16, m - i0);
+  const int mine = a.e.kept[unit * a.e.keep + i0 + min(lane & 15, n - 1)];
+  if (w_out && lane < n) *w_out = a.e.weights[b * a.e.w_b + head * a.e.w_h + mine];
   const KvCache& to = a.e.to;
   long long new_page = a.e.pages_out[b * a.e.out_stride + i0 / to.page_size];
   if (new_page < 0 || new_page >= to.n_pages) {  // nowhere to go
@@ -105,7 +100,6 @@ __global__ void __launch_bounds__(128) move_kernel(const __grid_constant__ Evict
   uint8_t* dk = to.data + kv_group_offset<QT, D>(to, new_page, head, 0, i0 % to.page_size >> 4);
   uint8_t* dv = dk + (long long)(to.page_size >> 4) * L::kHalf;
   // lane i: the keys of the group that holds token i % 16, and the token's place there
-  const int mine = a.e.kept[unit * a.e.keep + i0 + min(lane & 15, n - 1)];
   long long page = p.pages[b * p.pages_stride + mine / p.c.page_size];
   if (page < 0 || page >= p.c.n_pages) {
     atomicCAS(err, 0, kDevErrIndex);
@@ -171,7 +165,7 @@ EvictKernel move_for(int d) {
 }
 
 EvictKernel choose_for(int cl) {
-  return cl == 1 ? choose_kernel<1> : cl == 2 ? choose_kernel<2> : cl == 4 ? choose_kernel<4> : choose_kernel<8>;
+  return cl == 1 ? choose_kernel<1> : cl == 2 ? choose_kernel<2> : cl == 4 ? choose_kernel<4> : cl == 8 ? choose_kernel<8> : choose_kernel<16>;
 }
 
 }  // namespace
@@ -182,11 +176,11 @@ int kv_evict(const KvAttnParams& p, const KvEvict& e, int* err, cudaStream_t st)
   // CTAs of a unit: 4096 tokens each or more, as far as there are SMs for them and clusters go
   const long long tokens = (long long)p.max_pages * p.c.page_size;
   int cl = 1;
-  while (cl < 8 && (long long)cl * 4096 < tokens && units * cl * 2 <= num_sms()) cl *= 2;
+  while (cl < 16 && (long long)cl * 4096 < tokens && units * cl * 2 <= num_sms()) cl *= 2;
   const long long share = cl > 1 ? (tokens + 32 * cl - 1) / (32 * cl) * 32 : tokens;
   const EvictArgs a{p, e, (int)std::min<long long>(share, kMostKeys)};
   const EvictKernel choose = choose_for(cl);
-  if (kernel_setup(choose, kMostKeys * 4) <= 0) return -13;
+  if (cluster_setup(choose, kMostKeys * 4, cl) <= 0) return -13;
   int rc = launch_clusters(choose, (unsigned)units * cl, kThreads, (size_t)a.keys * 4, cl, st, a, err);
   if (rc || e.keep == 0) return rc;
   const EvictKernel k = p.c.type == QT_Q4_0 ? move_for<QT_Q4_0>(p.c.d)

@@ -8,7 +8,6 @@ namespace s3b {
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kMostKeys = 24576;  // pages of a CTA whose scores' keys stay in its shared memory
 
 struct SelectArgs {
@@ -28,14 +27,19 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// 16 warps in clusters (long lines of pages), unless the codes of many rows or channels take the registers; 8 otherwise, so that
+// several lists' CTAs share an SM (32 x 8 lists of 256 pages: 11.5 us, with 16 warps 14.8)
+template <int D, int NT, int CL>
+__host__ __device__ constexpr int select_threads() { return CL == 1 || NT * D > 256 || D == 256 ? 256 : 512; }
+
 // A unit is a block of queries and a key / value head, of one CTA or a cluster of them (CL) that share its pages and then choose
 // together (kv_top.cuh). Whole numbers carry the score: sum over channels of max(c low, c high) = c+ high + c- low with
 // c+ = max(c, 0), c- = min(c, 0), two products of 8-bit codes (16 pages x 32 channels x 8 rows an instruction), exact in 32 bits;
 // then two f32 products, each rounded, so that the choice is the same whatever the order. Lane (g, t) holds 16 channels of 64 as
 // the contraction's share of its rows (pages g, g + 8; query row g): whole 16-byte words of both.
 template <int D, int NT, int CL>
-__global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant__ SelectArgs a, int* err) {
-  constexpr int NC = D / 64;
+__global__ void __launch_bounds__(select_threads<D, NT, CL>()) select_kernel(const __grid_constant__ SelectArgs a, int* err) {
+  constexpr int NC = D / 64, kThreads = select_threads<D, NT, CL>();
   extern __shared__ uint32_t s_keys[];
   __shared__ TopShared<kThreads> s_top;
   const KvAttnParams& p = a.p;
@@ -125,6 +129,16 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
   // ---- scores of 16 pages at a time
   const int* table = p.pages + b * p.pages_stride;
   const int sink = pa + a.sink, recent = pe - a.recent;
+  auto page_of = [&](int j) -> long long {
+    if (j >= end) return 0;
+    const long long page = table[j];
+    if (page >= 0 && page < p.c.n_pages) return page;
+    atomicCAS(err, 0, kDevErrIndex);
+    return 0;
+  };
+  long long next[2];  // pages of the step after, on their way while this one's bounds are
+#pragma unroll
+  for (int u = 0; u < 2; ++u) next[u] = page_of(begin + 16 * warp + g + 8 * u);
   for (int j0 = begin + 16 * warp; j0 < end; j0 += 16 * (kThreads / 32)) {
     uint4 low[2][NC], high[2][NC];
     float page_step[2];
@@ -135,12 +149,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
 #pragma unroll
       for (int c = 0; c < NC; ++c) low[u][c] = high[u][c] = make_uint4(0, 0, 0, 0);
       if (j < end) {
-        long long page = table[j];
-        if (page < 0 || page >= p.c.n_pages) {
-          atomicCAS(err, 0, kDevErrIndex);
-          page = 0;
-        }
-        const long long row = page * p.c.heads + head;
+        const long long row = next[u] * p.c.heads + head;
         const int8_t* at = a.bounds.codes + row * 2 * D + 16 * t;
         page_step[u] = a.bounds.steps[row];
 #pragma unroll
@@ -150,6 +159,8 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
         }
       }
     }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) next[u] = page_of(j0 + 16 * (kThreads / 32) + g + 8 * u);
     float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -182,29 +193,35 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
   __syncthreads();
   auto emit = [&](uint32_t at, int i) { selected[at] = begin + i; };
   if (in_smem) {
-    top_select<kThreads, CL>(s_top, end - begin, (uint32_t)p.keep, [&](int i) { return s_keys[i]; }, emit);
+    auto key = [&](int i) { return s_keys[i]; };
+    top_select<kThreads, CL>(s_top, end - begin, (uint32_t)p.keep, key, key, emit);
   } else {
-    top_select<kThreads, CL>(
-        s_top, end - begin, (uint32_t)p.keep,
-        [&](int i) { return begin + i < sink || begin + i >= recent ? kTopForced : top_key(scores[begin + i]); }, emit);
+    auto key = [&](int i) { return begin + i < sink || begin + i >= recent ? kTopForced : top_key(scores[begin + i]); };
+    top_select<kThreads, CL>(s_top, end - begin, (uint32_t)p.keep, key, key, emit);
   }
 }
 
-typedef void (*SelectKernel)(SelectArgs, int*);
-
+struct SelectKernel {
+  void (*kernel)(SelectArgs, int*);
+  int threads;
+};
+template <int D, int NT, int CL>
+SelectKernel select_of() {
+  return {select_kernel<D, NT, CL>, select_threads<D, NT, CL>()};
+}
 template <int D, int CL>
 SelectKernel select_rows(int rows) {
-  return rows <= 8 ? select_kernel<D, 1, CL> : D == 256 || rows <= 16 ? select_kernel<D, 2, CL> : select_kernel<D, D == 256 ? 2 : 4, CL>;
+  return rows <= 8 ? select_of<D, 1, CL>() : D == 256 || rows <= 16 ? select_of<D, 2, CL>() : select_of<D, D == 256 ? 2 : 4, CL>();
 }
 template <int CL>
 SelectKernel select_for(int d, int rows) {
   return d == 64 ? select_rows<64, CL>(rows) : d == 128 ? select_rows<128, CL>(rows) : select_rows<256, CL>(rows);
 }
 
-// CTAs of a unit: about 512 pages each (4 for each warp's step of 16), as far as there are SMs for them and clusters go
+// CTAs of a unit: about 512 pages each (two steps of 16 for each warp), as far as there are SMs for them and clusters go
 int select_cluster(const KvAttnParams& p, int sms) {
   int cl = 1;
-  while (cl < 8 && (long long)cl * 512 < p.max_pages && kv_attention_units(p) * cl * 2 <= 2LL * sms) cl *= 2;
+  while (cl < 16 && (long long)cl * 512 < p.max_pages && kv_attention_units(p) * cl * 2 <= sms) cl *= 2;
   return cl;
 }
 // pages of the largest share of a CTA
@@ -221,9 +238,9 @@ int kv_select(const KvAttnParams& p, const KvBounds& bounds, int sink, int recen
   if (grid > 0x7fffffffLL) return -2;
   const SelectArgs a{p, bounds, sink, recent, scores, all, selected, (int)std::min<long long>(share, kMostKeys)};
   const int rows = p.share * (p.heads / p.c.heads), d = p.c.d;
-  const SelectKernel k = cl == 1 ? select_for<1>(d, rows) : cl == 2 ? select_for<2>(d, rows) : cl == 4 ? select_for<4>(d, rows) : select_for<8>(d, rows);
-  if (kernel_setup(k, kMostKeys * 4) <= 0) return -13;
-  return launch_clusters(k, (unsigned)grid, kThreads, (size_t)a.keys * 4, cl, st, a, err);
+  const SelectKernel k = cl == 1 ? select_for<1>(d, rows) : cl == 2 ? select_for<2>(d, rows) : cl == 4 ? select_for<4>(d, rows) : cl == 8 ? select_for<8>(d, rows) : select_for<16>(d, rows);
+  if (cluster_setup(k.kernel, kMostKeys * 4, cl) <= 0) return -13;
+  return launch_clusters(k.kernel, (unsigned)grid, k.threads, (size_t)a.keys * 4, cl, st, a, err);
 }
 
 }  // namespace s3b

@@ -1,5 +1,7 @@
 // The k largest of n values, the first among equals, in order of their places: for choosing pages by score and tokens by weight.
 #pragma once
+#include <type_traits>
+
 #include "kv_cache.cuh"
 
 namespace s3b {
@@ -30,103 +32,136 @@ struct TopShared {
 
 // Radix selection from the top, 8 bits a round: the digit in which the k-th largest lies, then the same among the keys that
 // share it; it ends with the round in which all of those are taken. Each of a cluster's CL CTAs has n places of a line, one CTA's
-// behind another's; within a CTA each warp has a run of rows of 32. key(i) is asked for its place i in every round: from shared
-// memory where they fit. emit(position, place) is called for the taken ones, k of them in all (0 < k <= the line's length, and at
-// least the number of forced keys).
-template <int T, int CL, typename Key, typename Emit>
-__device__ void top_select(TopShared<T>& s, int n, uint32_t k, Key key, Emit emit) {
+// behind another's; within a CTA each warp has a run of rows of 32. make(i) gives the key of its place i in the first round,
+// key(i) after that: from shared memory where they fit. emit(position, place) is called for the taken ones, k of them in all
+// (0 < k <= the line's length, and at least the number of forced keys).
+// Measured (cycles of the SM): 32768 keys a CTA of 1024 threads, 16 of them: a round 4700 to 7000 to count (the atomics on shared
+// memory), 500 to add up, 4000 for the cluster to meet and find the digit. 256 keys, 256 threads: see the branch for few keys.
+template <int T, int CL, typename Make, typename Key, typename Emit>
+__device__ void top_select(TopShared<T>& s, int n, uint32_t k, Make make, Key key, Emit emit) {
   constexpr int W = T / 32, C = TopShared<T>::kCopies, P = T / 256;  // P threads a digit
   static_assert(T >= 256 && T % 256 == 0 && C % P == 0, "threads of top_select");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows_all = (n + 31) / 32, rows_warp = (rows_all + W - 1) / W;
   const int from = min(warp * rows_warp, rows_all) * 32, to = min(n, from + rows_warp * 32);  // of this warp's run
   // f(whether there is a key, place, key): a whole warp each
-  auto each = [&](auto&& f) {
-    constexpr int U = 4;
+  auto each_of = [&](auto&& of, auto unroll, auto&& f) {
+    constexpr int U = decltype(unroll)::value;
     for (int i0 = from; i0 < to; i0 += 32 * U) {
       uint32_t x[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = i0 + 32 * u + lane;
-        x[u] = i < to ? key(i) : 0u;
+        x[u] = i < to ? of(i) : 0u;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (i0 + 32 * u < to) f(i0 + 32 * u + lane < to, i0 + 32 * u + lane, x[u]);
     }
   };
-#pragma unroll
-  for (int e = 0; e < 256 * C / T; ++e) s.hist[e * T + threadIdx.x] = 0;
-  uint32_t prefix = 0, left = k;
+  auto each = [&](auto&& f) { each_of(key, std::integral_constant<int, 4>(), f); };
+  uint32_t left = k;
   uint32_t from_above = 1, from_equal = 0;  // keys >= from_above are taken, then the first of those >= from_equal
+  if (CL == 1 && n <= T) {
+    // Few keys, one a thread: the threshold bit by bit, by the block's votes (some 50 cycles each, and most searches end well
+    // before the last bit: 256 keys in 1000 cycles where two rounds below take 2500).
+    const int i = from + lane;  // a run is one row
+    const bool there = from < to && i < to;
+    const uint32_t x = there ? make(i) : 0u;
+    uint32_t count = 0;
+    from_equal = 0;
+    for (int bit = 31; bit >= 0 && count != k; --bit) {
+      const uint32_t at = from_equal | 1u << bit;
+      const uint32_t c = __syncthreads_count(there && x >= at);
+      if (c >= k) from_equal = at, count = c;
+    }
+    from_above = from_equal;
+    left = 0;
+    if (count != k) {  // equal ones are left out (no forced key is: they are at most k)
+      from_above = from_equal + 1;
+      left = k - __syncthreads_count(there && x >= from_above);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 256 * C / T; ++e) s.hist[e * T + threadIdx.x] = 0;
+    uint32_t prefix = 0;
 #pragma unroll 1
-  for (int round = 0; round < 4; ++round) {
-    const int shift = 24 - 8 * round;
-    __syncthreads();
-    each([&](bool there, int, uint32_t x) {
-      if (there && (round == 0 || (x ^ prefix) >> (shift + 8) == 0)) atomicAdd(&s.hist[(x >> shift & 255) * C + lane % C], 1u);
-    });
-    __syncthreads();
-    {  // the digit's copies, P threads share them; rotated, so that a warp's lanes meet in no bank
-      uint32_t* h = s.hist + threadIdx.x / P * C;
-      uint32_t c = 0;
-#pragma unroll
-      for (int e = 0; e < C / P; ++e) {
-        const int at = (threadIdx.x % P) * (C / P) + (e + threadIdx.x / (P * (32 / C))) % (C / P);
-        c += h[at];
-        h[at] = 0;
-      }
-#pragma unroll
-      for (int x = 1; x < P; x <<= 1) c += __shfl_xor_sync(~0u, c, x);
-      if (threadIdx.x % P == 0) s.total[round & 1][threadIdx.x / P] = c;
-    }
-    if (CL > 1) cluster_sync_all();
-    else __syncthreads();
-    uint32_t c = 0, end = 0;
-    if (warp < 8) {  // thread i: digit 255 - i, and how many have it or a higher one
-      const uint32_t* at = &s.total[round & 1][255 - threadIdx.x];
-      if (CL > 1) {
-#pragma unroll
-        for (int r = 0; r < CL; ++r) c += cluster_load(at, r);
+    for (int round = 0; round < 4; ++round) {
+      const int shift = 24 - 8 * round;
+      __syncthreads();
+      if (round == 0) {
+        each_of(make, std::integral_constant<int, 8>(), [&](bool there, int, uint32_t x) {
+          if (there) atomicAdd(&s.hist[(x >> 24) * C + lane % C], 1u);
+        });
       } else {
-        c = *at;
+        each([&](bool there, int, uint32_t x) {
+          if (there && (x ^ prefix) >> (shift + 8) == 0) atomicAdd(&s.hist[(x >> shift & 255) * C + lane % C], 1u);
+        });
       }
-      end = c;
+      __syncthreads();
+      {  // the digit's copies, P threads share them; rotated, so that a warp's lanes meet in no bank
+        uint32_t* h = s.hist + threadIdx.x / P * C;
+        uint32_t c = 0;
 #pragma unroll
-      for (int x = 1; x < 32; x <<= 1) {
-        const uint32_t up = __shfl_up_sync(~0u, end, x);
-        if (lane >= x) end += up;
-      }
-      if (lane == 31) s.warp_sum[warp] = end;
-    }
-    __syncthreads();
-    if (warp < 8) {
+        for (int e = 0; e < C / P; ++e) {
+          const int at = (threadIdx.x % P) * (C / P) + (e + threadIdx.x / (P * (32 / C))) % (C / P);
+          c += h[at];
+          h[at] = 0;
+        }
 #pragma unroll
-      for (int w = 0; w < 7; ++w)
-        if (w < warp) end += s.warp_sum[w];
-      if (end - c < left && left <= end) {
-        s.digit = 255 - threadIdx.x;
-        s.left = left - (end - c);
-        s.count = c;
+        for (int x = 1; x < P; x <<= 1) c += __shfl_xor_sync(~0u, c, x);
+        if (threadIdx.x % P == 0) s.total[round & 1][threadIdx.x / P] = c;
       }
+      if (CL > 1) cluster_sync_all();
+      else __syncthreads();
+      uint32_t c = 0, end = 0;
+      if (warp < 8) {  // thread i: digit 255 - i, and how many have it or a higher one
+        const uint32_t* at = &s.total[round & 1][255 - threadIdx.x];
+        if (CL > 1) {
+#pragma unroll
+          for (int r = 0; r < CL; ++r) c += cluster_load(at, r);
+        } else {
+          c = *at;
+        }
+        end = c;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+          const uint32_t up = __shfl_up_sync(~0u, end, x);
+          if (lane >= x) end += up;
+        }
+        if (lane == 31) s.warp_sum[warp] = end;
+      }
+      __syncthreads();
+      if (warp < 8) {
+#pragma unroll
+        for (int w = 0; w < 7; ++w)
+          if (w < warp) end += s.warp_sum[w];
+        if (end - c < left && left <= end) {
+          s.digit = 255 - threadIdx.x;
+          s.left = left - (end - c);
+          s.count = c;
+        }
+      }
+      __syncthreads();
+      prefix |= s.digit << shift;
+      left = s.left;
+      if (left == s.count) {  // all that share the digits so far
+        from_above = from_equal = prefix;
+        left = 0;
+        break;
+      }
+      from_equal = prefix;
+      from_above = prefix + 1;  // no overflow: the forced keys, all taken, end in the branch above
     }
-    __syncthreads();
-    prefix |= s.digit << shift;
-    left = s.left;
-    if (left == s.count) {  // all that share the digits so far
-      from_above = from_equal = prefix;
-      left = 0;
-      break;
-    }
-    from_equal = prefix;
-    from_above = prefix + 1;  // no overflow: the forced keys, all taken, end in the branch above
   }
-  // places of what each warp takes
+  // places of what each warp takes (counted by lanes: POPC runs at an eighth of the rate of an addition)
   uint32_t above = 0, equal = 0;
   each([&](bool there, int, uint32_t x) {
-    above += __popc(__ballot_sync(~0u, there && x >= from_above));
-    equal += __popc(__ballot_sync(~0u, there && x >= from_equal && x < from_above));
+    above += there && x >= from_above;
+    equal += there && x >= from_equal && x < from_above;
   });
+  above = __reduce_add_sync(~0u, above);
+  equal = __reduce_add_sync(~0u, equal);
   if (lane == 0) s.above[warp] = above, s.equal[warp] = equal;
   __syncthreads();
   uint32_t a = lane < warp ? s.above[lane] : 0, q = lane < warp ? s.equal[lane] : 0;
@@ -142,17 +177,34 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Key key, Emit emi
   }
   each([&](bool there, int i, uint32_t x) {
     const bool is_above = there && x >= from_above, is_equal = there && x >= from_equal && x < from_above;
-    const uint32_t ma = __ballot_sync(~0u, is_above), mq = __ballot_sync(~0u, is_equal), below = (1u << lane) - 1;
-    const uint32_t pa = a + __popc(ma & below), pq = q + __popc(mq & below);
-    if (is_above || (is_equal && pq < left)) emit(pa + min(pq, left), i);
+    const uint32_t ma = __ballot_sync(~0u, is_above), mq = left ? __ballot_sync(~0u, is_equal) : 0u, below = (1u << lane) - 1;
+    if (!(ma | mq)) return;
+    uint32_t at = a + __popc(ma & below);
     a += __popc(ma);
-    q += __popc(mq);
+    bool taken = is_above;
+    if (mq) {
+      const uint32_t before = q + __popc(mq & below);
+      taken |= is_equal && before < left;
+      at += min(before, left);
+      q += __popc(mq);
+    } else {
+      at += min(q, left);
+    }
+    if (taken) emit(at, i);
   });
   if (CL > 1) cluster_sync_all();  // no CTA leaves while another reads its counts
 }
 
-// Launch of a kernel whose blocks form clusters of `cluster` (16: the kernel has to allow more than the portable 8), and that
-// may take its place while its predecessor runs.
+// kernel_setup for a kernel whose blocks form clusters of `cluster`: 16 are more than every GPU takes, and have to be allowed.
+inline int allow_wide_cluster(const void* kernel, size_t, int) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess ? 1 : -13;
+}
+template <typename K>
+int cluster_setup(K* kernel, size_t smem, int cluster) {
+  return kernel_setup(reinterpret_cast<const void*>(kernel), smem, cluster > 8 ? allow_wide_cluster : nullptr, 0);
+}
+
+// Launch of such a kernel, which may take its place while its predecessor runs.
 template <typename K, typename... A>
 int launch_clusters(K* kernel, unsigned grid, int threads, size_t smem, unsigned cluster, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};

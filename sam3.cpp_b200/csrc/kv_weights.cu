@@ -9,6 +9,35 @@ namespace {
 
 constexpr int kWarps = 8, kTile = 8;
 
+// q4_1: a score's part from the minima is sum over blocks of minimum * (sum of the query over the block), a product of its own. The
+// sums enter it as f16 and f16 remainder, less by 2^6: 32 queries of one sign may sum to more than an f16 holds.
+constexpr float kSumsLess = 64.f;
+__device__ __forceinline__ float block_sum(const uint4& v) {  // of 8 values a lane and 4 lanes
+  const float2 x0 = __half22float2(u32_h2(v.x)), x1 = __half22float2(u32_h2(v.y));
+  const float2 x2 = __half22float2(u32_h2(v.z)), x3 = __half22float2(u32_h2(v.w));
+  float s = ((x0.x + x0.y) + (x1.x + x1.y)) + ((x2.x + x2.y) + (x3.x + x3.y));
+  s += __shfl_xor_sync(~0u, s, 1);
+  return s + __shfl_xor_sync(~0u, s, 2);
+}
+__device__ __forceinline__ uint2 split_sums(float a, float b) {
+  a *= 1.f / kSumsLess;
+  b *= 1.f / kSumsLess;
+  const __half2 m = __floats2half2_rn(a, b);
+  const float2 x = __half22float2(m);
+  return make_uint2(h2_u32(m), h2_u32(__floats2half2_rn(a - x.x, b - x.y)));
+}
+// the pairs of block nn of a lane's piece of one token
+template <int QT, int NBS>
+__device__ __forceinline__ void key_pairs(const uint32_t* piece, int nn, uint32_t (&x)[4]) {
+  if (QT == QT_Q8_0) {
+    byte_pairs(piece[2 * nn], x[0], x[1]);
+    byte_pairs(piece[2 * nn + 1], x[2], x[3]);
+  } else {
+    nibble_pairs<QT>(piece[nn], x);
+  }
+}
+
+// ---------------------------------------------------------------- many rows
 template <int QT, int D, int NG>
 struct Sweep {
   typedef KvL<QT, D> L;
@@ -102,15 +131,8 @@ __global__ void __launch_bounds__(32 * kWarps) sweep_kernel(const __grid_constan
       for (int nn = 0; nn < L::kNBS; ++nn) {
         const int n = sb * L::kNBS + nn;
         uint32_t x0[4], x1[4];
-        if (QT == QT_Q8_0) {
-          byte_pairs(k0[2 * nn], x0[0], x0[1]);
-          byte_pairs(k0[2 * nn + 1], x0[2], x0[3]);
-          byte_pairs(k1[2 * nn], x1[0], x1[1]);
-          byte_pairs(k1[2 * nn + 1], x1[2], x1[3]);
-        } else {
-          nibble_pairs<QT>(k0[nn], x0);
-          nibble_pairs<QT>(k1[nn], x1);
-        }
+        key_pairs<QT, L::kNBS>(k0, nn, x0);
+        key_pairs<QT, L::kNBS>(k1, nn, x1);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           ka[gg][n][2 * e] = x0[e];
@@ -154,19 +176,11 @@ __global__ void __launch_bounds__(32 * kWarps) sweep_kernel(const __grid_constan
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           const uint4 v = s_q[(nt * NB + n) * 32 + lane];
-          const float2 x0 = __half22float2(u32_h2(v.x)), x1 = __half22float2(u32_h2(v.y));
-          const float2 x2 = __half22float2(u32_h2(v.z)), x3 = __half22float2(u32_h2(v.w));
-          float s = ((x0.x + x0.y) + (x1.x + x1.y)) + ((x2.x + x2.y) + (x3.x + x3.y));
-          s += __shfl_xor_sync(~0u, s, 1);
-          s += __shfl_xor_sync(~0u, s, 2);
+          const float s = block_sum(v);
           if (n == 2 * t) lo = s;
           if (n == 2 * t + 1) hi = s;
         }
-        lo *= 0.015625f;  // 32 queries of one sign may sum to more than an f16 holds: all less 2^6
-        hi *= 0.015625f;
-        const __half2 m = __floats2half2_rn(lo, hi);
-        const float2 x = __half22float2(m);
-        s_min[nt * 32 + lane] = make_uint2(h2_u32(m), h2_u32(__floats2half2_rn(lo - x.x, hi - x.y)));
+        s_min[nt * 32 + lane] = split_sums(lo, hi);
       }
       __syncthreads();
     }
@@ -182,7 +196,7 @@ __global__ void __launch_bounds__(32 * kWarps) sweep_kernel(const __grid_constan
         for (int gg = 0; gg < NG; ++gg) {
           mma16816(s[gg], am[gg], m.x, m.y);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[gg][e] *= 64.f;
+          for (int e = 0; e < 4; ++e) s[gg][e] *= kSumsLess;
         }
       }
 #pragma unroll
@@ -229,6 +243,217 @@ __global__ void __launch_bounds__(32 * kWarps) sweep_kernel(const __grid_constan
     }
 }
 
+// ---------------------------------------------------------------- few rows
+// Rows of a unit that stay in a warp's registers as fragments: 32, 16 at d = 256.
+template <int QT, int D, int NT>
+struct Stream {
+  typedef KvL<QT, D> L;
+  static constexpr int kRegs = L::kVal / 128 + L::kNB * L::kPlanes;           // of a lane, for a group's keys and scales
+  static constexpr int kAhead = kRegs <= 16 ? 2 : 1;                          // groups on their way while one is worked on
+  static constexpr int kBlocks = NT * D >= 512 || kRegs > 32 ? 2 : NT == 4 ? 3 : 4;  // of 4 warps, on an SM: 255, 168 or 128 registers
+};
+
+// All groups of 16 tokens of all units are one line, cut into equal shares for the warps; a token belongs to one warp, so nothing is
+// joined. A warp reads the group's keys straight into registers, in the order of the fragments, two groups ahead where there is
+// room, keeps the unit's query rows as fragments and adds each token's weights over the rows in two shuffles.
+template <int QT, int D, int NT>
+__global__ void __launch_bounds__(128, Stream<QT, D, NT>::kBlocks) stream_kernel(const __grid_constant__ WeightArgs a, int* err) {
+  typedef KvL<QT, D> L;
+  typedef Stream<QT, D, NT> C;
+  constexpr int NB = L::kNB, NSB = D / L::kSB, PW = L::kNBS * L::kBits / 4, AH = C::kAhead;  // words of a lane's piece of a token
+  const KvAttnParams& p = a.p;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int group_heads = p.heads / p.c.heads, n_rows = p.nq * group_heads;
+  const int per_page = p.c.page_size >> 4;
+  const long long warp = (long long)blockIdx.x * 4 + (threadIdx.x >> 5), warps = (long long)gridDim.x * 4;
+  let_next();
+  wait_before();
+  // this warp's share of the line, and the sequence in which it begins
+  auto groups_of = [&](int b) { return (sequence_length(p, b, err) + 15) >> 4; };
+  long long total = 0;
+  for (int b = lane; b < p.batch; b += 32) total += groups_of(b);
+#pragma unroll
+  for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(~0u, total, x);
+  total *= p.c.heads;
+  long long pos = total * warp / warps, base = 0;
+  const long long end = total * (warp + 1) / warps;
+  if (pos >= end) return;
+  int b = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const long long n = b0 + lane < p.batch ? (long long)groups_of(b0 + lane) * p.c.heads : 0;
+    long long last = n;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const long long up = __shfl_up_sync(~0u, last, x);
+      if (lane >= x) last += up;
+    }
+    const uint32_t past = __ballot_sync(~0u, base + last > pos);
+    if (past) {
+      const int who = __ffs(past) - 1;
+      b = b0 + who;
+      base += __shfl_sync(~0u, last - n, who);
+      break;
+    }
+    base += __shfl_sync(~0u, last, 31);
+  }
+
+  const float sl2 = p.scale * kLog2e;
+  for (; pos < end; ++b) {
+    const int len = sequence_length(p, b, err), groups = (len + 15) >> 4;
+    const int* table = p.pages + b * p.pages_stride;
+    for (; pos < end && pos < base + (long long)groups * p.c.heads;) {
+      const int head = (int)((pos - base) / groups);
+      const int first = (int)(pos - base - (long long)head * groups);
+      const int n_it = (int)min((long long)groups - first, end - pos);
+      pos += n_it;
+      float* w = a.w.w + b * a.w.w_b + head * a.w.w_h;
+
+      // ---- query fragments: column g of tile nt is row 8 nt + g; the spans and ln sums of columns 2t, 2t + 1
+      uint32_t qf[NT][NB][4], qmin[NT][2];
+      float lse[NT][2];
+      int row_lo[NT][2], row_hi[NT][2], min_lo = 0x7FFFFFFF, max_lo = 0, min_hi = 0x7FFFFFFF, max_hi = 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = 8 * nt + g;
+        int lo = 0, hi = 0;
+        float mine = INFINITY;
+        const __half* q = nullptr;
+        if (r < n_rows) {
+          const int i = r / group_heads, h = head * group_heads + r % group_heads;
+          mine = p.lse[((long long)b * p.nq + i) * p.heads + h] * kLog2e;
+          if (mine != -INFINITY) {  // else a row that has seen nothing, and sees nothing here
+            row_span(p, len, i, &lo, &hi);
+            q = p.q + b * p.q_b + i * p.q_n + h * p.q_h + 8 * t;
+            min_lo = min(min_lo, lo), max_lo = max(max_lo, lo), min_hi = min(min_hi, hi), max_hi = max(max_hi, hi);
+          } else {
+            mine = INFINITY;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          lse[nt][c] = __shfl_sync(~0u, mine, 8 * t + 4 * c);
+          row_lo[nt][c] = __shfl_sync(~0u, lo, 8 * t + 4 * c);
+          row_hi[nt][c] = __shfl_sync(~0u, hi, 8 * t + 4 * c);
+        }
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const uint4 v = q ? *reinterpret_cast<const uint4*>(q + 32 * n) : make_uint4(0, 0, 0, 0);
+          qf[nt][n][0] = v.x, qf[nt][n][1] = v.y, qf[nt][n][2] = v.z, qf[nt][n][3] = v.w;
+          if (QT == QT_Q4_1) {
+            const float s = block_sum(v);
+            if (n == 2 * t) s0 = s;
+            if (n == 2 * t + 1) s1 = s;
+          }
+        }
+        if (QT == QT_Q4_1) {
+          const uint2 m = split_sums(s0, s1);
+          qmin[nt][0] = m.x, qmin[nt][1] = m.y;
+        }
+      }
+      min_lo = __reduce_min_sync(~0u, min_lo), max_lo = __reduce_max_sync(~0u, max_lo);
+      min_hi = __reduce_min_sync(~0u, min_hi), max_hi = __reduce_max_sync(~0u, max_hi);
+
+      // ---- groups on their way
+      long long src = 0;  // lane i: address of the keys of step (of a batch of 32) + i
+      uint32_t raw[AH][2][NSB][PW], sc[AH][2][NB / 2], mins[AH][2];
+      float old[AH];
+      const int mine_tok = g + 8 * (t & 1);  // of lanes t < 2: the token of the group whose weight they hold
+      auto seen = [&](int it) { return (first + it) * 16 < max_hi && (first + it) * 16 + 16 > min_lo; };
+      auto issue = [&](int it, int at) {
+        if ((it & 31) == 0) {
+          const int gi = first + it + lane;
+          if (it + lane < n_it) {
+            long long page = table[gi / per_page];
+            if (page < 0 || page >= p.c.n_pages) {
+              atomicCAS(err, 0, kDevErrIndex);
+              page = 0;
+            }
+            src = kv_group_offset<QT, D>(p.c, page, head, 0, gi % per_page);
+          }
+        }
+        const uint8_t* gp = p.c.data + __shfl_sync(~0u, src, it & 31);
+        const int tok = (first + it) * 16 + mine_tok;
+        old[at] = t < 2 && tok < len && (a.w.decay != 1.f || seen(it)) ? w[tok] : 0.f;
+        if (seen(it)) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int sb = 0; sb < NSB; ++sb) lds<PW * 4>(gp + L::k_val(g + 8 * u, sb * L::kNBS, t), raw[at][u][sb]);
+            lds<NB * 2>(gp + L::k_scale(g + 8 * u, 0), sc[at][u]);
+            if (QT == QT_Q4_1) mins[at][u] = 2 * t < NB ? *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g + 8 * u, 2 * t)) : 0u;
+          }
+        }
+      };
+#pragma unroll
+      for (int it = 0; it < AH; ++it)
+        if (it < n_it) issue(it, it);
+      for (int it0 = 0; it0 < n_it; it0 += AH) {
+#pragma unroll
+        for (int at = 0; at < AH; ++at) {
+          const int it = it0 + at;
+          if (it >= n_it) break;
+          const int tok0 = (first + it) * 16;
+          float sum[2] = {0.f, 0.f};
+          if (seen(it)) {
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+              if (QT == QT_Q4_1) {
+                const uint32_t am[4] = {mins[at][0], mins[at][1], mins[at][0], mins[at][1]};
+                mma16816(s[nt], am, qmin[nt][0], qmin[nt][1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nt][e] *= kSumsLess;
+              }
+            }
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+              uint32_t x0[4], x1[4];
+              key_pairs<QT, L::kNBS>(raw[at][0][n / L::kNBS], n % L::kNBS, x0);
+              key_pairs<QT, L::kNBS>(raw[at][1][n / L::kNBS], n % L::kNBS, x1);
+              const uint32_t a0[4] = {x0[0], x1[0], x0[1], x1[1]}, a1[4] = {x0[2], x1[2], x0[3], x1[3]};
+              const __half2 h0 = u32_h2(sc[at][0][n / 2]), h1 = u32_h2(sc[at][1][n / 2]);
+              const float f0 = n & 1 ? __high2float(h0) : __low2float(h0), f1 = n & 1 ? __high2float(h1) : __low2float(h1);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float c[4];
+                mma16816_first(c, a0, qf[nt][n][0], qf[nt][n][1]);
+                mma16816(c, a1, qf[nt][n][2], qf[nt][n][3]);
+                s[nt][0] = fmaf(f0, c[0], s[nt][0]);
+                s[nt][1] = fmaf(f0, c[1], s[nt][1]);
+                s[nt][2] = fmaf(f1, c[2], s[nt][2]);
+                s[nt][3] = fmaf(f1, c[3], s[nt][3]);
+              }
+            }
+            const bool whole = tok0 >= max_lo && tok0 + 16 <= min_hi;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float v = ex2_approx(fmaf(s[nt][e], sl2, -lse[nt][e & 1]));
+                if (!whole) {
+                  const int tok = tok0 + g + 8 * (e >> 1);
+                  if (tok < row_lo[nt][e & 1] || tok >= row_hi[nt][e & 1]) v = 0.f;
+                }
+                sum[e >> 1] += v;
+              }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              sum[u] += __shfl_xor_sync(~0u, sum[u], 1);
+              sum[u] += __shfl_xor_sync(~0u, sum[u], 2);
+            }
+          }
+          if (t < 2 && tok0 + mine_tok < len && (a.w.decay != 1.f || seen(it))) w[tok0 + mine_tok] = fmaf(a.w.decay, old[at], t & 1 ? sum[1] : sum[0]);
+          if (it + AH < n_it) issue(it + AH, at);
+        }
+      }
+    }
+    base += (long long)groups * p.c.heads;
+  }
+}
+
 template <int QT, int D, int NG>
 int launch_sweep(const KvAttnParams& p, const KvWeights& w, int* err, cudaStream_t st) {
   typedef Sweep<QT, D, NG> C;
@@ -242,10 +467,25 @@ int launch_sweep(const KvAttnParams& p, const KvWeights& w, int* err, cudaStream
   return launch_dependent(k, dim3((unsigned)grid), 32 * kWarps, C::kSmem, st, a, err);
 }
 
+template <int QT, int D, int NT>
+int launch_stream(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st) {
+  const WeightArgs a{p, w, 0};
+  return launch_dependent(stream_kernel<QT, D, NT>, dim3(sms * Stream<QT, D, NT>::kBlocks), 128, 0, st, a, err);
+}
+
+template <int QT, int D>
+int weights_for(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st) {
+  const long long rows = p.nq * (long long)(p.heads / p.c.heads);
+  if (rows <= 8) return launch_stream<QT, D, 1>(p, w, sms, err, st);
+  if (rows <= 16) return launch_stream<QT, D, 2>(p, w, sms, err, st);
+  if (D < 256 && rows <= 32) return launch_stream<QT, D, D < 256 ? 4 : 2>(p, w, sms, err, st);
+  return launch_sweep<QT, D, 1>(p, w, err, st);
+}
+
 template <int QT>
-int weights_d(const KvAttnParams& p, const KvWeights& w, int* err, cudaStream_t st) {
-  return p.c.d == 64 ? launch_sweep<QT, 64, 1>(p, w, err, st)
-                     : p.c.d == 128 ? launch_sweep<QT, 128, 1>(p, w, err, st) : launch_sweep<QT, 256, 1>(p, w, err, st);
+int weights_d(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st) {
+  return p.c.d == 64 ? weights_for<QT, 64>(p, w, sms, err, st)
+                     : p.c.d == 128 ? weights_for<QT, 128>(p, w, sms, err, st) : weights_for<QT, 256>(p, w, sms, err, st);
 }
 
 }  // namespace
@@ -254,9 +494,9 @@ size_t kv_weights_work(const KvAttnParams&, int) { return 0; }
 
 int kv_weights_launches(const KvAttnParams&, int) { return 1; }
 
-int kv_weights(const KvAttnParams& p, const KvWeights& w, int, int* err, cudaStream_t st) {
-  return p.c.type == QT_Q4_0 ? weights_d<QT_Q4_0>(p, w, err, st)
-                             : p.c.type == QT_Q4_1 ? weights_d<QT_Q4_1>(p, w, err, st) : weights_d<QT_Q8_0>(p, w, err, st);
+int kv_weights(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st) {
+  return p.c.type == QT_Q4_0 ? weights_d<QT_Q4_0>(p, w, sms, err, st)
+                             : p.c.type == QT_Q4_1 ? weights_d<QT_Q4_1>(p, w, sms, err, st) : weights_d<QT_Q8_0>(p, w, sms, err, st);
 }
 
 }  // namespace s3b
