@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
   // Units of at most so many chunks stay whole where there is a block for each: two or three more chunks for a block cost less
   // than joining parts (8 heads of 128, 2 chunks each: 10.3 us cut, 9.5 whole; 8 of 256, 3 chunks: 16.4, 14.3; 4 of 64, 3 chunks:
   // 9.3, 8.7; but 8 of 128, 3 chunks: 10.7, 11.6, and 4 chunks 10.9, 13.7).
-  constexpr int kWhole = 3;
+  constexpr int kWhole = 3, kWholeList = 8;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* s_q = smem + C::kMain;
   float* s_m = reinterpret_cast<float*>(s_q + C::kQBytes);  // [W][rows]
@@ -183,7 +183,10 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
     total *= seq_units;
     long long ctas = min((long long)gridDim.x, total), base = 0, p0 = 0, p1 = 0;
     int found = -1;
-    if (most <= kWhole && (long long)p.batch * seq_units <= gridDim.x) {
+    // Lists are short and of nearly one length: whole where a unit of its own costs a block no more than some chunks above an equal
+    // share, which is what joining parts costs.
+    const bool whole = SEL ? most - total / max(ctas, 1LL) <= kWholeList : most <= kWhole;
+    if (whole && (long long)p.batch * seq_units <= gridDim.x) {
       const int b = blockIdx.x / seq_units;
       if (b < p.batch) {
         const int n = chunks_of(b, &g0, &g1);
@@ -865,9 +868,13 @@ template <int QT, int D, int NT, bool SEL>
 int launch_rows_nt(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
   // Blocks of four warps, several on an SM, where there is a unit for each SM: a unit's beginning and end then run beside
   // other blocks' loops (32 sequences, 8 heads: 123 -> 96 us). One block an SM where few units are cut into many parts,
-  // which have to be joined (one sequence, 2 heads, 524288 tokens: 477 -> 119 us).
+  // which have to be joined (one sequence, 2 heads, 524288 tokens: 477 -> 119 us). Lists are short: two blocks an SM where there
+  // are units for those, so that each has its own.
   constexpr int kMost = Rows<QT, D, NT, 4>::kWarps;
-  if (kv_attention_units(p) >= w.sms) return launch_rows<QT, D, NT, 4, SEL>(p, w, err, st);
+  const long long units = kv_attention_units(p);
+  constexpr int kHalf = SEL && (kMost > 8) ? kMost / 2 : 4;
+  if (kHalf > 4 && units >= w.sms && units <= 2 * w.sms) return launch_rows<QT, D, NT, kHalf, SEL>(p, w, err, st);
+  if (units >= w.sms) return launch_rows<QT, D, NT, 4, SEL>(p, w, err, st);
   return launch_rows<QT, D, NT, kMost, SEL>(p, w, err, st);
 }
 

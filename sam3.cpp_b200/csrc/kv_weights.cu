@@ -248,19 +248,23 @@ __global__ void __launch_bounds__(32 * kWarps) sweep_kernel(const __grid_constan
 template <int QT, int D, int NT>
 struct Stream {
   typedef KvL<QT, D> L;
-  static constexpr int kRegs = L::kVal / 128 + L::kNB * L::kPlanes;           // of a lane, for a group's keys and scales
-  static constexpr int kAhead = kRegs <= 16 ? 2 : 1;                          // groups on their way while one is worked on
-  static constexpr int kBlocks = NT * D >= 512 || kRegs > 32 ? 2 : NT == 4 ? 3 : 4;  // of 4 warps, on an SM: 255, 168 or 128 registers
+  static constexpr int kBlocks = NT == 4 || NT * D >= 512 ? 3 : 4;  // of 4 warps, on an SM: 168 or 128 registers
+  static constexpr int kFit = (224 * 1024) / (4 * kBlocks * L::kHalf);
+  static constexpr int kStages = kFit > 8 ? 8 : kFit;                          // groups of a warp in shared memory
+  static constexpr int kSmem = 4 * kStages * L::kHalf;
+  static_assert(kStages >= 2, "stages of stream_kernel");
 };
 
 // All groups of 16 tokens of all units are one line, cut into equal shares for the warps; a token belongs to one warp, so nothing is
-// joined. A warp reads the group's keys straight into registers, in the order of the fragments, two groups ahead where there is
-// room, keeps the unit's query rows as fragments and adds each token's weights over the rows in two shuffles.
+// joined and no two warps wait for each other. A warp has its own ring of groups in shared memory, copied while those before them are
+// worked on, keeps the unit's query rows as fragments and adds each token's weights over the rows in two shuffles.
 template <int QT, int D, int NT>
 __global__ void __launch_bounds__(128, Stream<QT, D, NT>::kBlocks) stream_kernel(const __grid_constant__ WeightArgs a, int* err) {
   typedef KvL<QT, D> L;
   typedef Stream<QT, D, NT> C;
-  constexpr int NB = L::kNB, NSB = D / L::kSB, PW = L::kNBS * L::kBits / 4, AH = C::kAhead;  // words of a lane's piece of a token
+  constexpr int NB = L::kNB, NSB = D / L::kSB, PW = L::kNBS * L::kBits / 4, NS = C::kStages;  // words of a lane's piece of a token
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* ring = smem + (threadIdx.x >> 5) * NS * L::kHalf;
   const KvAttnParams& p = a.p;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group_heads = p.heads / p.c.heads, n_rows = p.nq * group_heads;
@@ -356,99 +360,114 @@ __global__ void __launch_bounds__(128, Stream<QT, D, NT>::kBlocks) stream_kernel
 
       // ---- groups on their way
       long long src = 0;  // lane i: address of the keys of step (of a batch of 32) + i
-      uint32_t raw[AH][2][NSB][PW], sc[AH][2][NB / 2], mins[AH][2];
-      float old[AH];
+      int to = 0;         // stage of the next one
       const int mine_tok = g + 8 * (t & 1);  // of lanes t < 2: the token of the group whose weight they hold
       auto seen = [&](int it) { return (first + it) * 16 < max_hi && (first + it) * 16 + 16 > min_lo; };
-      auto issue = [&](int it, int at) {
-        if ((it & 31) == 0) {
-          const int gi = first + it + lane;
-          if (it + lane < n_it) {
-            long long page = table[gi / per_page];
-            if (page < 0 || page >= p.c.n_pages) {
-              atomicCAS(err, 0, kDevErrIndex);
-              page = 0;
+      auto issue = [&](int it) {
+        if (it < n_it) {
+          if ((it & 31) == 0) {
+            const int gi = first + it + lane;
+            if (it + lane < n_it) {
+              long long page = table[gi / per_page];
+              if (page < 0 || page >= p.c.n_pages) {
+                atomicCAS(err, 0, kDevErrIndex);
+                page = 0;
+              }
+              src = kv_group_offset<QT, D>(p.c, page, head, 0, gi % per_page);
             }
-            src = kv_group_offset<QT, D>(p.c, page, head, 0, gi % per_page);
           }
-        }
-        const uint8_t* gp = p.c.data + __shfl_sync(~0u, src, it & 31);
-        const int tok = (first + it) * 16 + mine_tok;
-        old[at] = t < 2 && tok < len && (a.w.decay != 1.f || seen(it)) ? w[tok] : 0.f;
-        if (seen(it)) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-#pragma unroll
-            for (int sb = 0; sb < NSB; ++sb) lds<PW * 4>(gp + L::k_val(g + 8 * u, sb * L::kNBS, t), raw[at][u][sb]);
-            lds<NB * 2>(gp + L::k_scale(g + 8 * u, 0), sc[at][u]);
-            if (QT == QT_Q4_1) mins[at][u] = 2 * t < NB ? *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g + 8 * u, 2 * t)) : 0u;
-          }
-        }
-      };
-#pragma unroll
-      for (int it = 0; it < AH; ++it)
-        if (it < n_it) issue(it, it);
-      for (int it0 = 0; it0 < n_it; it0 += AH) {
-#pragma unroll
-        for (int at = 0; at < AH; ++at) {
-          const int it = it0 + at;
-          if (it >= n_it) break;
-          const int tok0 = (first + it) * 16;
-          float sum[2] = {0.f, 0.f};
+          const uint8_t* from = p.c.data + __shfl_sync(~0u, src, it & 31) + lane * 16;
           if (seen(it)) {
-            float s[NT][4];
+            const uint32_t at = smem_u32(ring + to * L::kHalf) + lane * 16;
+#pragma unroll
+            for (int x = 0; x < L::kHalf; x += 512)
+              if (x + 512 <= L::kHalf || x + lane * 16 < L::kHalf)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + x), "l"(from + x) : "memory");
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        to = to + 1 == NS ? 0 : to + 1;
+      };
+      auto touched = [&](int it) { return t < 2 && it < n_it && (first + it) * 16 + mine_tok < len && (a.w.decay != 1.f || seen(it)); };
+      for (int it = 0; it < NS - 1; ++it) issue(it);
+      float next = touched(0) ? w[first * 16 + mine_tok] : 0.f;
+      int stage = 0;
+      for (int it = 0; it < n_it; ++it) {
+        const int tok0 = (first + it) * 16;
+        asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
+        __syncwarp();  // the copies of all lanes are there, and all are done with the stage that is filled next
+        issue(it + NS - 1);
+        const uint8_t* gp = ring + stage * L::kHalf;
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        const float old = next;
+        if (touched(it + 1)) next = w[tok0 + 16 + mine_tok];
+        float sum[2] = {0.f, 0.f};
+        if (seen(it)) {
+          uint32_t k0[NSB][PW], k1[NSB][PW], s0[NB / 2], s1[NB / 2];
+#pragma unroll
+          for (int sb = 0; sb < NSB; ++sb) {
+            lds<PW * 4>(gp + L::k_val(g, sb * L::kNBS, t), k0[sb]);
+            lds<PW * 4>(gp + L::k_val(g + 8, sb * L::kNBS, t), k1[sb]);
+          }
+          lds<NB * 2>(gp + L::k_scale(g, 0), s0);
+          lds<NB * 2>(gp + L::k_scale(g + 8, 0), s1);
+          float s[NT][4];
+          uint32_t am[4] = {0, 0, 0, 0};
+          if (QT == QT_Q4_1 && 2 * t < NB) {
+            am[0] = am[2] = *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g, 2 * t));
+            am[1] = am[3] = *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g + 8, 2 * t));
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+            if (QT == QT_Q4_1) {
+              mma16816(s[nt], am, qmin[nt][0], qmin[nt][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[nt][e] *= kSumsLess;
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            uint32_t x0[4], x1[4];
+            key_pairs<QT, L::kNBS>(k0[n / L::kNBS], n % L::kNBS, x0);
+            key_pairs<QT, L::kNBS>(k1[n / L::kNBS], n % L::kNBS, x1);
+            const uint32_t a0[4] = {x0[0], x1[0], x0[1], x1[1]}, a1[4] = {x0[2], x1[2], x0[3], x1[3]};
+            const __half2 h0 = u32_h2(s0[n / 2]), h1 = u32_h2(s1[n / 2]);
+            const float f0 = n & 1 ? __high2float(h0) : __low2float(h0), f1 = n & 1 ? __high2float(h1) : __low2float(h1);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-              if (QT == QT_Q4_1) {
-                const uint32_t am[4] = {mins[at][0], mins[at][1], mins[at][0], mins[at][1]};
-                mma16816(s[nt], am, qmin[nt][0], qmin[nt][1]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[nt][e] *= kSumsLess;
-              }
-            }
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-              uint32_t x0[4], x1[4];
-              key_pairs<QT, L::kNBS>(raw[at][0][n / L::kNBS], n % L::kNBS, x0);
-              key_pairs<QT, L::kNBS>(raw[at][1][n / L::kNBS], n % L::kNBS, x1);
-              const uint32_t a0[4] = {x0[0], x1[0], x0[1], x1[1]}, a1[4] = {x0[2], x1[2], x0[3], x1[3]};
-              const __half2 h0 = u32_h2(sc[at][0][n / 2]), h1 = u32_h2(sc[at][1][n / 2]);
-              const float f0 = n & 1 ? __high2float(h0) : __low2float(h0), f1 = n & 1 ? __high2float(h1) : __low2float(h1);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                float c[4];
-                mma16816_first(c, a0, qf[nt][n][0], qf[nt][n][1]);
-                mma16816(c, a1, qf[nt][n][2], qf[nt][n][3]);
-                s[nt][0] = fmaf(f0, c[0], s[nt][0]);
-                s[nt][1] = fmaf(f0, c[1], s[nt][1]);
-                s[nt][2] = fmaf(f1, c[2], s[nt][2]);
-                s[nt][3] = fmaf(f1, c[3], s[nt][3]);
-              }
-            }
-            const bool whole = tok0 >= max_lo && tok0 + 16 <= min_hi;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                float v = ex2_approx(fmaf(s[nt][e], sl2, -lse[nt][e & 1]));
-                if (!whole) {
-                  const int tok = tok0 + g + 8 * (e >> 1);
-                  if (tok < row_lo[nt][e & 1] || tok >= row_hi[nt][e & 1]) v = 0.f;
-                }
-                sum[e >> 1] += v;
-              }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              sum[u] += __shfl_xor_sync(~0u, sum[u], 1);
-              sum[u] += __shfl_xor_sync(~0u, sum[u], 2);
+              float c[4];
+              mma16816_first(c, a0, qf[nt][n][0], qf[nt][n][1]);
+              mma16816(c, a1, qf[nt][n][2], qf[nt][n][3]);
+              s[nt][0] = fmaf(f0, c[0], s[nt][0]);
+              s[nt][1] = fmaf(f0, c[1], s[nt][1]);
+              s[nt][2] = fmaf(f1, c[2], s[nt][2]);
+              s[nt][3] = fmaf(f1, c[3], s[nt][3]);
             }
           }
-          if (t < 2 && tok0 + mine_tok < len && (a.w.decay != 1.f || seen(it))) w[tok0 + mine_tok] = fmaf(a.w.decay, old[at], t & 1 ? sum[1] : sum[0]);
-          if (it + AH < n_it) issue(it + AH, at);
+          const bool whole = tok0 >= max_lo && tok0 + 16 <= min_hi;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float v = ex2_approx(fmaf(s[nt][e], sl2, -lse[nt][e & 1]));
+              if (!whole) {
+                const int tok = tok0 + g + 8 * (e >> 1);
+                if (tok < row_lo[nt][e & 1] || tok >= row_hi[nt][e & 1]) v = 0.f;
+              }
+              sum[e >> 1] += v;
+            }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            sum[u] += __shfl_xor_sync(~0u, sum[u], 1);
+            sum[u] += __shfl_xor_sync(~0u, sum[u], 2);
+          }
         }
+        if (touched(it)) w[tok0 + mine_tok] = fmaf(a.w.decay, old, t & 1 ? sum[1] : sum[0]);
       }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();  // the ring begins again
     }
     base += (long long)groups * p.c.heads;
   }
@@ -469,8 +488,11 @@ int launch_sweep(const KvAttnParams& p, const KvWeights& w, int* err, cudaStream
 
 template <int QT, int D, int NT>
 int launch_stream(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st) {
+  typedef Stream<QT, D, NT> C;
+  auto* k = stream_kernel<QT, D, NT>;
+  if (kernel_setup(k, C::kSmem) <= 0) return -13;
   const WeightArgs a{p, w, 0};
-  return launch_dependent(stream_kernel<QT, D, NT>, dim3(sms * Stream<QT, D, NT>::kBlocks), 128, 0, st, a, err);
+  return launch_dependent(k, dim3(sms * C::kBlocks), 128, C::kSmem, st, a, err);
 }
 
 template <int QT, int D>
