@@ -42,11 +42,13 @@ int read_dev_err(s3b_ctx* ctx) {
   if (h != 0) {
     // cleared in the context stream's order, so no later kernel's code can be wiped by it
     cudaMemsetAsync(ctx->d_err, 0, sizeof(int), ctx->stream);
-    // blocks that gave up may have left the cache attention's counts unfinished
-    const auto count = ctx->ws.find("kv_attn_count");
-    if (count != ctx->ws.end() && count->second->bytes) cudaMemsetAsync(count->second->p, 0, count->second->bytes, ctx->stream);
-    for (const auto& b : ctx->graph_kept)
-      if (b.first == "kv_attn_count") cudaMemsetAsync(b.second->p, 0, b.second->bytes, ctx->stream);
+    // blocks that gave up may have left the cache calls' counts unfinished
+    for (const char* name : {"kv_attn_count", "kv_weights_count"}) {
+      const auto count = ctx->ws.find(name);
+      if (count != ctx->ws.end() && count->second->bytes) cudaMemsetAsync(count->second->p, 0, count->second->bytes, ctx->stream);
+      for (const auto& b : ctx->graph_kept)
+        if (b.first == name) cudaMemsetAsync(b.second->p, 0, b.second->bytes, ctx->stream);
+    }
     cudaStreamSynchronize(ctx->stream);
     if (h == kDevErrIndex)
       return set_error(ctx, kErrDevice, "a slot, page or length in device memory is out of range (code %d)", h);
@@ -1775,16 +1777,19 @@ int s3b_op_cache_weights(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* q,
   w.w_h = w_h;
   w.decay = decay;
   const int sms = num_sms();
-  const size_t need = kv_weights_work(p, sms);
-  if (need) {
-    bool grown;
-    DevBuf* part = graph_buf(ctx, "kv_weights_part", power_of_two(need, 1 << 20), stream_capturing(ctx), &grown, &rc);
-    if (rc) return rc;
-    w.part = part->as<float>();
-  }
+  const bool capturing = stream_capturing(ctx);
+  bool grown;
+  DevBuf* part = graph_buf(ctx, "kv_weights_part", kv_weights_part(sms), capturing, &grown, &rc);
+  if (rc) return rc;
+  w.part = part->as<float>();
+  DevBuf* count = graph_buf(ctx, "kv_weights_count", (size_t)sms * 4, capturing, &grown, &rc);
+  if (rc) return rc;
+  if (grown && cudaMemsetAsync(count->p, 0, count->bytes, ctx->stream) != cudaSuccess)
+    return set_error(ctx, kErrCuda, "cache_weights: clearing the counts");
+  w.count = count->as<int>();
   rc = kv_weights(p, w, sms, ctx->d_err, ctx->stream);
   if (rc) return set_error(ctx, launcher_status_code(rc), "cache_weights launch failed (%d)", rc);
-  count_launch(ctx, kv_weights_launches(p, sms));
+  count_launch(ctx);
   return kOk;
 }
 

@@ -442,11 +442,14 @@ struct KvWeights {
   float* w = nullptr;
   long long w_b = 0, w_h = 0;
   float decay = 1.f;
-  float* part = nullptr;  // workspace where the rows are split
+  float* part = nullptr;  // workspace of kv_weights_part(sms) bytes, and counts of one int for each SM, zero before and after
+  int* count = nullptr;
 };
-size_t kv_weights_work(const KvAttnParams& p, int sms);
+size_t kv_weights_part(int sms);
 int kv_weights(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st);
-int kv_weights_launches(const KvAttnParams& p, int sms);
+// The tensor-core kernel for many rows (kv_weights picks it).
+size_t kv_weights_tc_part(int sms);
+int kv_weights_tc(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st);
 
 // s3b_op_cache_evict: `keep` tokens of each sequence and head, moved into `to` (p: source cache, pages, lengths).
 struct KvEvict {

@@ -501,6 +501,7 @@ int weights_for(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cu
   if (rows <= 8) return launch_stream<QT, D, 1>(p, w, sms, err, st);
   if (rows <= 16) return launch_stream<QT, D, 2>(p, w, sms, err, st);
   if (D < 256 && rows <= 32) return launch_stream<QT, D, D < 256 ? 4 : 2>(p, w, sms, err, st);
+  if (rows > 128) return kv_weights_tc(p, w, sms, err, st);
   return launch_sweep<QT, D, 1>(p, w, err, st);
 }
 
@@ -512,9 +513,7 @@ int weights_d(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cuda
 
 }  // namespace
 
-size_t kv_weights_work(const KvAttnParams&, int) { return 0; }
-
-int kv_weights_launches(const KvAttnParams&, int) { return 1; }
+size_t kv_weights_part(int sms) { return kv_weights_tc_part(sms); }
 
 int kv_weights(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st) {
   return p.c.type == QT_Q4_0 ? weights_d<QT_Q4_0>(p, w, sms, err, st)

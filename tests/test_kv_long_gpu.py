@@ -427,6 +427,16 @@ def test_weights(s3b, engine, qtype, d, heads, kv, nq, page, lengths):
         assert abs(total - (nq * heads // kv if n else 0)) <= 1e-3 * nq * heads
 
 
+@pytest.mark.parametrize("qtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv,nq,lengths", [(1, 1, 129, [1]), (3, 1, 100, [130, 0, 1000]), (2, 2, 513, [129, 128, 127]), (8, 1, 64, [3000]), (4, 2, 700, [5000, 17])])
+@pytest.mark.parametrize("causal,window", [(False, 0), (True, 0), (True, 200)])
+def test_weights_of_many_rows(s3b, engine, qtype, d, heads, kv, nq, lengths, causal, window):
+    """Tiles of 128 tokens and 128 rows: one tile, heads that fill no tile, tiles that several blocks share, long walks."""
+    s = Sequences(s3b, engine, qtype, d, kv, 48, lengths, seed=nq + d)
+    check_weights(engine, s, s.queries(nq, heads), causal, window, 0.5)
+
+
 @pytest.mark.parametrize("qtype,d", [(2, 64), (3, 128), (8, 256)])
 @pytest.mark.parametrize("window", [0, 9, 100])
 @pytest.mark.parametrize("nq", [1, 7, 200])
