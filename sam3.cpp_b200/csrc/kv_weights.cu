@@ -249,9 +249,10 @@ template <int QT, int D, int NT>
 struct Stream {
   typedef KvL<QT, D> L;
   static constexpr int kBlocks = NT == 4 || NT * D >= 512 ? 3 : 4;  // of 4 warps, on an SM: 168 or 128 registers
-  static constexpr int kFit = (224 * 1024) / (4 * kBlocks * L::kHalf);
-  static constexpr int kStages = kFit > 8 ? 8 : kFit;                          // groups of a warp in shared memory
-  static constexpr int kSmem = 4 * kStages * L::kHalf;
+  static constexpr int kG = NT == 1 && D <= 128 ? 2 : 1;                        // groups of a step
+  static constexpr int kFit = (224 * 1024) / (4 * kBlocks * kG * L::kHalf);
+  static constexpr int kStages = kFit > 8 / kG ? 8 / kG : kFit;                // steps of a warp in shared memory
+  static constexpr int kSmem = 4 * kStages * kG * L::kHalf;
   static_assert(kStages >= 2, "stages of stream_kernel");
 };
 
@@ -262,9 +263,9 @@ template <int QT, int D, int NT>
 __global__ void __launch_bounds__(128, Stream<QT, D, NT>::kBlocks) stream_kernel(const __grid_constant__ WeightArgs a, int* err) {
   typedef KvL<QT, D> L;
   typedef Stream<QT, D, NT> C;
-  constexpr int NB = L::kNB, NSB = D / L::kSB, PW = L::kNBS * L::kBits / 4, NS = C::kStages;  // words of a lane's piece of a token
+  constexpr int NB = L::kNB, NSB = D / L::kSB, PW = L::kNBS * L::kBits / 4, NS = C::kStages, G = C::kG;  // PW: words of a lane's piece of a token
   extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* ring = smem + (threadIdx.x >> 5) * NS * L::kHalf;
+  uint8_t* ring = smem + (threadIdx.x >> 5) * NS * G * L::kHalf;
   const KvAttnParams& p = a.p;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group_heads = p.heads / p.c.heads, n_rows = p.nq * group_heads;
@@ -358,113 +359,131 @@ __global__ void __launch_bounds__(128, Stream<QT, D, NT>::kBlocks) stream_kernel
       min_lo = __reduce_min_sync(~0u, min_lo), max_lo = __reduce_max_sync(~0u, max_lo);
       min_hi = __reduce_min_sync(~0u, min_hi), max_hi = __reduce_max_sync(~0u, max_hi);
 
-      // ---- groups on their way
-      long long src = 0;  // lane i: address of the keys of step (of a batch of 32) + i
-      int to = 0;         // stage of the next one
-      const int mine_tok = g + 8 * (t & 1);  // of lanes t < 2: the token of the group whose weight they hold
-      auto seen = [&](int it) { return (first + it) * 16 < max_hi && (first + it) * 16 + 16 > min_lo; };
+      // ---- steps of G groups, on their way while others are worked on
+      const int steps = (n_it + G - 1) / G;
+      const bool all = a.w.decay != 1.f;                                      // tokens that no row sees change too
+      const int seen_from = min_lo >> 4, seen_to = (max_hi + 15) >> 4;        // groups that some row sees
+      auto seen = [&](int it) { return first + it * G < seen_to && first + it * G + G > seen_from; };
+      long long src = 0;  // lane i: address of the keys of group (of a batch of 32) + i
+      int to = 0;         // stage of the next step
       auto issue = [&](int it) {
-        if (it < n_it) {
-          if ((it & 31) == 0) {
-            const int gi = first + it + lane;
-            if (it + lane < n_it) {
-              long long page = table[gi / per_page];
-              if (page < 0 || page >= p.c.n_pages) {
-                atomicCAS(err, 0, kDevErrIndex);
-                page = 0;
-              }
-              src = kv_group_offset<QT, D>(p.c, page, head, 0, gi % per_page);
+        if (it < steps) {
+          if ((it * G & 31) == 0 && it * G + lane < n_it) {
+            const int gi = first + it * G + lane;
+            long long page = table[gi / per_page];
+            if (page < 0 || page >= p.c.n_pages) {
+              atomicCAS(err, 0, kDevErrIndex);
+              page = 0;
             }
+            src = kv_group_offset<QT, D>(p.c, page, head, 0, gi % per_page);
           }
-          const uint8_t* from = p.c.data + __shfl_sync(~0u, src, it & 31) + lane * 16;
           if (seen(it)) {
-            const uint32_t at = smem_u32(ring + to * L::kHalf) + lane * 16;
 #pragma unroll
-            for (int x = 0; x < L::kHalf; x += 512)
-              if (x + 512 <= L::kHalf || x + lane * 16 < L::kHalf)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + x), "l"(from + x) : "memory");
+            for (int gg = 0; gg < G; ++gg) {
+              const uint8_t* from = p.c.data + __shfl_sync(~0u, src, (it * G & 31) + gg) + lane * 16;
+              const uint32_t at = smem_u32(ring + (to * G + gg) * L::kHalf) + lane * 16;
+              if (gg == 0 || it * G + gg < n_it) {
+#pragma unroll
+                for (int x = 0; x < L::kHalf; x += 512)
+                  if (x + 512 <= L::kHalf || x + lane * 16 < L::kHalf)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + x), "l"(from + x) : "memory");
+              }
+            }
           }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         to = to + 1 == NS ? 0 : to + 1;
       };
-      auto touched = [&](int it) { return t < 2 && it < n_it && (first + it) * 16 + mine_tok < len && (a.w.decay != 1.f || seen(it)); };
+      // the token whose weight this lane holds: lane t of a quad has token g + 8 (t % 2) of group t / 2
+      const int mine_tok = first * 16 + (G == 2 ? 16 * (t >> 1) : 0) + g + 8 * (t & 1);
+      const int tok_end = min(len, (first + n_it) * 16);
+      auto mine = [&](int it) { return (G == 2 || t < 2) && mine_tok + it * (16 * G) < tok_end && (all || seen(it)); };
       for (int it = 0; it < NS - 1; ++it) issue(it);
-      float next = touched(0) ? w[first * 16 + mine_tok] : 0.f;
+      float next = mine(0) ? w[mine_tok] : 0.f;
       int stage = 0;
-      for (int it = 0; it < n_it; ++it) {
-        const int tok0 = (first + it) * 16;
+      for (int it = 0; it < steps; ++it) {
+        const int tok0 = (first + it * G) * 16;
         asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
         __syncwarp();  // the copies of all lanes are there, and all are done with the stage that is filled next
         issue(it + NS - 1);
-        const uint8_t* gp = ring + stage * L::kHalf;
+        const uint8_t* gp = ring + stage * (G * L::kHalf);
         stage = stage + 1 == NS ? 0 : stage + 1;
         const float old = next;
-        if (touched(it + 1)) next = w[tok0 + 16 + mine_tok];
-        float sum[2] = {0.f, 0.f};
+        if (mine(it + 1)) next = w[mine_tok + (it + 1) * (16 * G)];
+        float sum[G][2];
+#pragma unroll
+        for (int gg = 0; gg < G; ++gg) sum[gg][0] = sum[gg][1] = 0.f;
         if (seen(it)) {
-          uint32_t k0[NSB][PW], k1[NSB][PW], s0[NB / 2], s1[NB / 2];
+          const bool whole = tok0 >= max_lo && tok0 + 16 * G <= min_hi;
 #pragma unroll
-          for (int sb = 0; sb < NSB; ++sb) {
-            lds<PW * 4>(gp + L::k_val(g, sb * L::kNBS, t), k0[sb]);
-            lds<PW * 4>(gp + L::k_val(g + 8, sb * L::kNBS, t), k1[sb]);
-          }
-          lds<NB * 2>(gp + L::k_scale(g, 0), s0);
-          lds<NB * 2>(gp + L::k_scale(g + 8, 0), s1);
-          float s[NT][4];
-          uint32_t am[4] = {0, 0, 0, 0};
-          if (QT == QT_Q4_1 && 2 * t < NB) {
-            am[0] = am[2] = *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g, 2 * t));
-            am[1] = am[3] = *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g + 8, 2 * t));
-          }
+          for (int gg = 0; gg < G; ++gg, gp += L::kHalf) {
+            uint32_t k0[NSB][PW], k1[NSB][PW], s0[NB / 2], s1[NB / 2];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-            if (QT == QT_Q4_1) {
-              mma16816(s[nt], am, qmin[nt][0], qmin[nt][1]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[nt][e] *= kSumsLess;
+            for (int sb = 0; sb < NSB; ++sb) {
+              lds<PW * 4>(gp + L::k_val(g, sb * L::kNBS, t), k0[sb]);
+              lds<PW * 4>(gp + L::k_val(g + 8, sb * L::kNBS, t), k1[sb]);
             }
-          }
-#pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            uint32_t x0[4], x1[4];
-            key_pairs<QT, L::kNBS>(k0[n / L::kNBS], n % L::kNBS, x0);
-            key_pairs<QT, L::kNBS>(k1[n / L::kNBS], n % L::kNBS, x1);
-            const uint32_t a0[4] = {x0[0], x1[0], x0[1], x1[1]}, a1[4] = {x0[2], x1[2], x0[3], x1[3]};
-            const __half2 h0 = u32_h2(s0[n / 2]), h1 = u32_h2(s1[n / 2]);
-            const float f0 = n & 1 ? __high2float(h0) : __low2float(h0), f1 = n & 1 ? __high2float(h1) : __low2float(h1);
+            lds<NB * 2>(gp + L::k_scale(g, 0), s0);
+            lds<NB * 2>(gp + L::k_scale(g + 8, 0), s1);
+            float s[NT][4];
+            uint32_t am[4] = {0, 0, 0, 0};
+            if (QT == QT_Q4_1 && 2 * t < NB) {
+              am[0] = am[2] = *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g, 2 * t));
+              am[1] = am[3] = *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g + 8, 2 * t));
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              float c[4];
-              mma16816_first(c, a0, qf[nt][n][0], qf[nt][n][1]);
-              mma16816(c, a1, qf[nt][n][2], qf[nt][n][3]);
-              s[nt][0] = fmaf(f0, c[0], s[nt][0]);
-              s[nt][1] = fmaf(f0, c[1], s[nt][1]);
-              s[nt][2] = fmaf(f1, c[2], s[nt][2]);
-              s[nt][3] = fmaf(f1, c[3], s[nt][3]);
-            }
-          }
-          const bool whole = tok0 >= max_lo && tok0 + 16 <= min_hi;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+              for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+              if (QT == QT_Q4_1) {
+                mma16816(s[nt], am, qmin[nt][0], qmin[nt][1]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float v = ex2_approx(fmaf(s[nt][e], sl2, -lse[nt][e & 1]));
-              if (!whole) {
-                const int tok = tok0 + g + 8 * (e >> 1);
-                if (tok < row_lo[nt][e & 1] || tok >= row_hi[nt][e & 1]) v = 0.f;
+                for (int e = 0; e < 4; ++e) s[nt][e] *= kSumsLess;
               }
-              sum[e >> 1] += v;
             }
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            sum[u] += __shfl_xor_sync(~0u, sum[u], 1);
-            sum[u] += __shfl_xor_sync(~0u, sum[u], 2);
+            for (int n = 0; n < NB; ++n) {
+              uint32_t x0[4], x1[4];
+              key_pairs<QT, L::kNBS>(k0[n / L::kNBS], n % L::kNBS, x0);
+              key_pairs<QT, L::kNBS>(k1[n / L::kNBS], n % L::kNBS, x1);
+              const uint32_t a0[4] = {x0[0], x1[0], x0[1], x1[1]}, a1[4] = {x0[2], x1[2], x0[3], x1[3]};
+              const __half2 h0 = u32_h2(s0[n / 2]), h1 = u32_h2(s1[n / 2]);
+              const float f0 = n & 1 ? __high2float(h0) : __low2float(h0), f1 = n & 1 ? __high2float(h1) : __low2float(h1);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float c[4];
+                mma16816_first(c, a0, qf[nt][n][0], qf[nt][n][1]);
+                mma16816(c, a1, qf[nt][n][2], qf[nt][n][3]);
+                s[nt][0] = fmaf(f0, c[0], s[nt][0]);
+                s[nt][1] = fmaf(f0, c[1], s[nt][1]);
+                s[nt][2] = fmaf(f1, c[2], s[nt][2]);
+                s[nt][3] = fmaf(f1, c[3], s[nt][3]);
+              }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float v = ex2_approx(fmaf(s[nt][e], sl2, -lse[nt][e & 1]));
+                if (!whole) {
+                  const int tok = tok0 + 16 * gg + g + 8 * (e >> 1);
+                  if (tok < row_lo[nt][e & 1] || tok >= row_hi[nt][e & 1]) v = 0.f;
+                }
+                sum[gg][e >> 1] += v;
+              }
           }
+#pragma unroll
+          for (int gg = 0; gg < G; ++gg)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              sum[gg][u] += __shfl_xor_sync(~0u, sum[gg][u], 1);
+              sum[gg][u] += __shfl_xor_sync(~0u, sum[gg][u], 2);
+            }
         }
-        if (touched(it)) w[tok0 + mine_tok] = fmaf(a.w.decay, old, t & 1 ? sum[1] : sum[0]);
+        if (mine(it)) {
+          const float s0 = t & 1 ? sum[0][1] : sum[0][0], s1 = t & 1 ? sum[G - 1][1] : sum[G - 1][0];
+          w[mine_tok + it * (16 * G)] = fmaf(a.w.decay, old, G == 2 && (t & 2) ? s1 : s0);
+        }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       __syncwarp();  // the ring begins again
@@ -501,7 +520,9 @@ int weights_for(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cu
   if (rows <= 8) return launch_stream<QT, D, 1>(p, w, sms, err, st);
   if (rows <= 16) return launch_stream<QT, D, 2>(p, w, sms, err, st);
   if (D < 256 && rows <= 32) return launch_stream<QT, D, D < 256 ? 4 : 2>(p, w, sms, err, st);
-  if (rows > 128) return kv_weights_tc(p, w, sms, err, st);
+  // tiles of 128 rows: ahead from where a second one is well filled (us at 64 / 128 / 256 channels, 32 heads over 8000 tokens: 192 rows
+  // 65 / 83 / 111 against 50 / 79 / 155, 256 rows 66 / 83 / 111 against 65 / 103 / 203)
+  if (rows > (D == 256 ? 128 : D == 128 ? 192 : 256)) return kv_weights_tc(p, w, sms, err, st);
   return launch_sweep<QT, D, 1>(p, w, err, st);
 }
 

@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(Wt<QT, D>::kThreads, 1) weights_tiles_kernel(c
         const int info = n % I * kTile;
         const float* lse = s_lse + info;
         const uint32_t at = tmem + lane_off + C::kS + e * kTile;
-        const bool whole = s_span[n % I * 4] <= s.tok0 && s_span[n % I * 4 + 1] >= s.tok0 + kTile;
+        const bool whole = s_span[n % I * 4] <= s.tok0 && s_span[n % I * 4 + 1] >= min(s.tok0 + kTile, s.len);
         const unsigned long long scale2 = f2_pack(sl2, sl2);
         unsigned long long acc[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
         auto add = [&](const uint32_t (&r)[32], int c0, auto masked) {
