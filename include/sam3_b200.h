@@ -634,85 +634,130 @@ typedef struct s3b_kv_bounds {
     float* steps;
 } s3b_kv_bounds;
 
+/* The values that the bounds of n pages stand for, code * step: out f32
+ * [n][heads][2][d], 16-byte aligned; pages int64 [n] (device), one outside the
+ * bounds gives zeros. Needs no context: enqueued on `cuda_stream` of the current
+ * device. */
+int s3b_kv_bounds_values(const s3b_kv_bounds* bounds, const int64_t* pages, int64_t n, float* out, void* cuda_stream);
+
+/* What the calls below take of their sequences and queries; fields that a call
+ * does not name are not read. As the arguments of s3b_op_cache_attention:
+ *   pages, pages_stride, max_pages, lengths, batch   the sequences
+ *   q, q_b, q_n, q_h, nq, heads                      the queries
+ *   causal, window, scale                            masks, scale
+ *   out, o_b, o_n, o_h, out_f32, lse                 the attention's results
+ * and lists of pages for blocks of `share` consecutive queries (the last block may
+ * be shorter) and each head of the cache:
+ *   selected [batch][ceil(nq / share)][heads of the cache][keep]: places in the
+ *            page table; a list ends at its first negative entry
+ * At most 32 rows (share x heads / heads of the cache; 16 at d = 256) have a list. */
+typedef struct s3b_kv_call {
+    const int32_t* pages;
+    int64_t pages_stride;
+    const int32_t* lengths;
+    const void* q;
+    int64_t q_b;
+    int64_t q_n;
+    int64_t q_h;
+    void* out;
+    int64_t o_b;
+    int64_t o_n;
+    int64_t o_h;
+    float* lse;
+    int32_t* selected;
+    int32_t max_pages;
+    int32_t batch;
+    int32_t nq;
+    int32_t heads;
+    int32_t causal;
+    int32_t window;
+    int32_t keep;
+    int32_t share;
+    int32_t out_f32;
+    float scale;
+} s3b_kv_call;
+
 /* Writes the bounds of the pages that hold the last `recent` tokens of each
  * sequence (recent >= max_pages * page_size: of all its pages), over the tokens
- * that the sequence has there. Other pages keep theirs. pages, pages_stride,
- * max_pages, lengths and batch as in s3b_op_cache_attention, and errors of theirs
- * too (a page outside the cache is skipped). Two sequences may share a page if
- * they have the same tokens of it. */
-int s3b_op_cache_bounds(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_bounds* bounds, const int32_t* pages,
-                        int64_t pages_stride, int max_pages, const int32_t* lengths, int batch, int64_t recent);
+ * that the sequence has there. Other pages keep theirs. Takes the sequences of
+ * `call`; errors in device memory as in s3b_op_cache_attention (a page outside the
+ * cache is skipped). Two sequences may share a page if they have the same tokens of
+ * it. */
+int s3b_op_cache_bounds(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_bounds* bounds, const s3b_kv_call* call,
+                        int64_t recent);
 
-/* Chooses for every block of `share` consecutive queries (the last block may be
- * shorter) and key / value head the `keep` pages to attend to, by a bound of
+/* Chooses the `keep` pages that each block of queries attends to, by a bound of
  * their scores. A query row in 8 bits is c = rint(q * (127 / max |q|)) (a NaN
  * counts as 0, an infinity as f16's largest); its score of a page is
  *   ((float) sum over channels of max(c * lowest, c * highest) * step) * (max |q| / 127)
  * (whole numbers, then two f32 roundings: the same on every run), and a block's
- * score of a page the largest of its rows (queries x heads / bounds->heads, at
- * most 32, 16 at d = 256). Of the pages that hold a token which some query of the
- * block sees (causal and window as in s3b_op_cache_attention), the first `sink`
- * and the last `recent` are taken, then those of highest score, the lower page
- * first among equals; all of them where there are no more than `keep`.
- *   selected  [batch][blocks][heads of the cache][keep]: positions in the page
- *             table, ascending, -1 behind the last; blocks = ceil(nq / share)
- *   scores    f32 [batch][blocks][heads of the cache][max_pages], -inf for pages
- *             that the block does not see, or NULL
- * keep >= 1, sink + recent <= keep. The call only enqueues work; its workspace is the
- * context's, as that of s3b_op_cache_attention, and the same holds under capture. */
-int s3b_op_cache_select(s3b_ctx* ctx, const s3b_kv_bounds* bounds, const void* q, int64_t q_b, int64_t q_n, int64_t q_h,
-                        int32_t* selected, int keep, int share, int sink, int recent, float* scores,
-                        const int32_t* pages, int64_t pages_stride, int max_pages, const int32_t* lengths, int batch,
-                        int nq, int heads, int causal, int window);
+ * score of a page the largest of its rows. Of the pages that hold a token which some
+ * query of the block sees, the first `sink` and the last `recent` are taken, then
+ * those of highest score, the lower page first among equals; all of them where there
+ * are no more than `keep`. Takes the sequences, queries and masks of `call` and
+ * writes its lists, ascending, -1 behind the last.
+ *   scores  f32 [batch][blocks][heads of the cache][max_pages], -inf for pages that
+ *           the block does not see, or NULL
+ * keep >= 1, sink + recent <= keep. The call only enqueues work; a workspace (of
+ * lists over very many pages) is the context's, as that of s3b_op_cache_attention,
+ * and the same holds under capture. */
+int s3b_op_cache_select(s3b_ctx* ctx, const s3b_kv_bounds* bounds, const s3b_kv_call* call, int sink, int recent,
+                        float* scores);
 
 /* s3b_op_cache_attention over the tokens of selected pages only: the queries of a
- * block and the heads of a group see the pages that their list names (selected as
- * s3b_op_cache_select writes it, in any order; a list ends at its first negative
- * entry, and a page that it names twice counts twice). A row that sees no token of them
- * is zero, its lse -inf. An entry beyond max_pages is skipped and the next s3b_sync
- * returns S3B_ERR_DEVICE. At most 32 rows a block (16 at d = 256). Weights are
- * rounded to f16 once, with their products with the block scales: f16 outputs are
- * off by 2.9e-4 of their norm. */
-int s3b_op_cache_attention_selected(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* q, int64_t q_b, int64_t q_n,
-                                    int64_t q_h, void* out, int out_f32, int64_t o_b, int64_t o_n, int64_t o_h,
-                                    float* lse, const int32_t* selected, int keep, int share, const int32_t* pages,
-                                    int64_t pages_stride, int max_pages, const int32_t* lengths, int batch, int nq,
-                                    int heads, float scale, int causal, int window);
+ * block and the heads of a group see the pages that their list names, in any order;
+ * a page that it names twice counts twice. A row that sees no token of them is
+ * zero, its lse -inf. An entry beyond max_pages is skipped and the next s3b_sync
+ * returns S3B_ERR_DEVICE. Takes all of `call`; lse may be NULL. Weights are rounded
+ * to f16 once, with their products with the block scales: f16 outputs are off by
+ * 2.9e-4 of their norm. */
+int s3b_op_cache_attention_selected(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_call* call);
 
-/* Adds the attention weight that each token gets from these queries to what it
- * has gathered: for each sequence, key / value head and token below lengths[b]
+/* Adds the attention weight that each token gets from the queries of `call` to what
+ * it has gathered: for each sequence, key / value head and token below lengths[b]
  *   w = decay * w + sum over the rows that see it of exp(scale q k - lse)
- * with lse [batch][nq][heads] as s3b_op_cache_attention returns it (rows of -inf
- * add nothing). weights: f32, token t of sequence b and head h at weights +
+ * with call's lse [batch][nq][heads] as s3b_op_cache_attention has written it (rows
+ * of -inf add nothing). weights: f32, token t of sequence b and head h at weights +
  * b * w_b + h * w_h + t, rows of max_pages * page_size values that do not overlap;
  * those behind a sequence's last token are left as they are. decay is finite and
- * >= 0. Sums are f32, in the same order on every run. Other arguments as there. */
-int s3b_op_cache_weights(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* q, int64_t q_b, int64_t q_n, int64_t q_h,
-                         const float* lse, float* weights, int64_t w_b, int64_t w_h, float decay, const int32_t* pages,
-                         int64_t pages_stride, int max_pages, const int32_t* lengths, int batch, int nq, int heads,
-                         float scale, int causal, int window);
+ * >= 0. Sums are f32, in the same order on every run. The workspace is the
+ * context's, as there. */
+int s3b_op_cache_weights(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_call* call, float* weights, int64_t w_b,
+                         int64_t w_h, float decay);
 
-/* Keeps `keep` tokens of each sequence and head and moves them, in their order, to
- * the first places of other pages: the first `sink` and last `recent` tokens, then
- * those of highest weight, the earlier first among equals (a NaN is below every
- * weight); all tokens of a sequence that has no more than `keep`. Codes and scales
- * are copied as they are. A head's token at a place need not be the same as another
- * head's.
- *   weights      as in s3b_op_cache_weights (rows may overlap)
+/* What s3b_op_cache_evict keeps, and where.
  *   to           the cache of the new pages, of the same type, heads and d (NULL:
  *                the same cache); its page_size may differ
+ *   weights      as in s3b_op_cache_weights (rows may overlap)
  *   pages_out    [batch][out_stride >= ceil(keep / to->page_size)]: none of them
  *                may be a page that this call reads, nor named twice
  *   lengths_out  [batch]: min(lengths[b], keep); not the array of lengths
  *   kept         [batch][heads][keep]: positions that the tokens had, -1 behind the last
- *   weights_out  f32 [batch][heads][keep]: their weights, 0 behind the last; or NULL
- * The source pages are left as they are, places behind the last token too. A page of
- * pages_out outside its cache is not written, and the next s3b_sync returns
- * S3B_ERR_DEVICE. sink + recent <= keep. */
-int s3b_op_cache_evict(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_cache* to, const float* weights,
-                       int64_t w_b, int64_t w_h, const int32_t* pages, int64_t pages_stride, int max_pages,
-                       const int32_t* lengths, int batch, int keep, int sink, int recent, const int32_t* pages_out,
-                       int64_t out_stride, int32_t* lengths_out, int32_t* kept, float* weights_out);
+ *   weights_out  f32 [batch][heads][keep]: their weights, 0 behind the last; or NULL */
+typedef struct s3b_kv_evict {
+    const s3b_kv_cache* to;
+    const float* weights;
+    int64_t w_b;
+    int64_t w_h;
+    const int32_t* pages_out;
+    int64_t out_stride;
+    int32_t* lengths_out;
+    int32_t* kept;
+    float* weights_out;
+    int32_t keep;
+    int32_t sink;
+    int32_t recent;
+} s3b_kv_evict;
+
+/* Keeps `keep` tokens of each sequence of `call` and each head and moves them, in
+ * their order, to the first places of other pages: the first `sink` and last `recent`
+ * tokens, then those of highest weight, the earlier first among equals (a NaN is
+ * below every weight); all tokens of a sequence that has no more than `keep`. Codes
+ * and scales are copied as they are. A head's token at a place need not be the same as
+ * another head's. The source pages are left as they are, places behind the last token
+ * too. A page of pages_out outside its cache is not written, and the next s3b_sync
+ * returns S3B_ERR_DEVICE. sink + recent <= keep. */
+int s3b_op_cache_evict(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_call* call, const s3b_kv_evict* evict);
 
 /* ---------------------------------------------------------------- host format helpers */
 

@@ -12,8 +12,10 @@ module ``sam3_b200``.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
+import struct
 import subprocess
 
 import numpy as np
@@ -48,6 +50,11 @@ class KVBoundsDesc(ctypes.Structure):
     """s3b_kv_bounds: bounds of the keys of a cache's pages in caller-owned device memory."""
     _fields_ = [("heads", ctypes.c_int32), ("d", ctypes.c_int32), ("page_size", ctypes.c_int32), ("n_pages", ctypes.c_int64),
                 ("codes", ctypes.c_void_p), ("steps", ctypes.c_void_p)]
+
+
+# s3b_kv_call and s3b_kv_evict as bytes, in the order of their fields: one pack costs a sixth of as many ctypes arguments.
+_CALL = struct.Struct("<QqQ Qqqq Qqqq QQ iiii iiii if")
+_EVICT = struct.Struct("<QQqq QqQQQ iii4x")
 
 
 # Every symbol declared in include/sam3_b200.h: (name, restype, argtypes)
@@ -118,15 +125,12 @@ SYMBOLS = [
     ("s3b_op_cache_read", _I, [_P, ctypes.POINTER(KVCacheDesc), _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I]),
     ("s3b_op_cache_attention", _I, [_P, ctypes.POINTER(KVCacheDesc), _P, _I64, _I64, _I64, _P, _I, _I64, _I64, _I64, _P,
                                     _P, _I64, _I, _P, _I, _I, _I, _F, _I, _I]),
-    ("s3b_op_cache_bounds", _I, [_P, ctypes.POINTER(KVCacheDesc), ctypes.POINTER(KVBoundsDesc), _P, _I64, _I, _P, _I, _I64]),
-    ("s3b_op_cache_select", _I, [_P, ctypes.POINTER(KVBoundsDesc), _P, _I64, _I64, _I64, _P, _I, _I, _I, _I, _P, _P, _I64, _I, _P, _I,
-                                 _I, _I, _I, _I]),
-    ("s3b_op_cache_attention_selected", _I, [_P, ctypes.POINTER(KVCacheDesc), _P, _I64, _I64, _I64, _P, _I, _I64, _I64, _I64, _P, _P,
-                                             _I, _I, _P, _I64, _I, _P, _I, _I, _I, _F, _I, _I]),
-    ("s3b_op_cache_weights", _I, [_P, ctypes.POINTER(KVCacheDesc), _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _F, _P, _I64, _I, _P, _I,
-                                  _I, _I, _F, _I, _I]),
-    ("s3b_op_cache_evict", _I, [_P, ctypes.POINTER(KVCacheDesc), ctypes.POINTER(KVCacheDesc), _P, _I64, _I64, _P, _I64, _I, _P, _I, _I,
-                                _I, _I, _P, _I64, _P, _P, _P]),
+    ("s3b_kv_bounds_values", _I, [ctypes.POINTER(KVBoundsDesc), _P, _I64, _P, _P]),
+    ("s3b_op_cache_bounds", _I, [_P, ctypes.POINTER(KVCacheDesc), ctypes.POINTER(KVBoundsDesc), _P, _I64]),
+    ("s3b_op_cache_select", _I, [_P, ctypes.POINTER(KVBoundsDesc), _P, _I, _I, _P]),
+    ("s3b_op_cache_attention_selected", _I, [_P, ctypes.POINTER(KVCacheDesc), _P]),
+    ("s3b_op_cache_weights", _I, [_P, ctypes.POINTER(KVCacheDesc), _P, _P, _I64, _I64, _F]),
+    ("s3b_op_cache_evict", _I, [_P, ctypes.POINTER(KVCacheDesc), _P, _P]),
     ("s3b_row_size", _I64, [_I, _I64]),
     ("s3b_quantize_rows", _I, [_I, _P, _I64, _I64, _P]),
     ("s3b_dequantize_rows", _I, [_I, _P, _I64, _I64, _P]),
@@ -209,7 +213,8 @@ def dequantize_rows(qtype: int, raw: np.ndarray, ne0: int) -> np.ndarray:
 # Row types of the cache operators and index types by size. Torch is imported where tensors are first needed: by KVCache.
 _ROW_TYPES: dict = {}
 _INDEX_TYPES: dict = {}
-_FLOAT: list = []
+_F16: list = []
+_F32: list = []
 
 
 def _index(what: str, name: str, t, itemsize: int, dims: int, device: int) -> int:
@@ -238,7 +243,8 @@ class KVCache:
         if not _ROW_TYPES:
             _INDEX_TYPES.update({4: torch.int32, 8: torch.int64})
             _ROW_TYPES.update({torch.float16: S3B_F16, torch.float32: S3B_F32})
-            _FLOAT.append(torch.float32)
+            _F16.append(torch.float16)
+            _F32.append(torch.float32)
         if data is None:
             data = torch.zeros(nbytes, dtype=torch.uint8, device=device)
             if data.is_cuda:  # the first write may come on the engine's own stream
@@ -273,8 +279,15 @@ class KVBounds:
         self.ref = ctypes.byref(self.desc)
 
     def values(self, pages):
-        """The bounds f32 [n, heads, 2, d] of the pages int64 [n], on torch's stream."""
-        return self.codes[pages] * self.steps[pages][..., None, None]
+        """The bounds f32 [n, heads, 2, d] of the pages int64 [n], on torch's stream (s3b_kv_bounds_values)."""
+        import torch
+        n = _index("KVBounds.values", "pages", pages, 8, 1, self.device)
+        out = torch.empty(n, self.heads, 2, self.d, device=pages.device)
+        with torch.cuda.device(self.device) if torch.cuda.current_device() != self.device else contextlib.nullcontext():
+            rc = lib().s3b_kv_bounds_values(self.ref, pages.data_ptr(), n, out.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream)
+        if rc:
+            raise S3BError(f"s3b_kv_bounds_values: {ERRORS.get(rc, rc)}")
+        return out
 
 
 def sam_best_mask(iou, multimask: bool) -> int:
@@ -803,47 +816,63 @@ class Engine:
             self._check(rc, "s3b_op_cache_attention")
 
     # -- long caches: reading and keeping less
-    def _sequences(self, what: str, pages, lengths) -> int:
-        """Sequences of a page table int32 [batch, max_pages] and its lengths int32 [batch]."""
-        b = _index(what, "lengths", lengths, 4, 1, self.device)
-        if _index(what, "pages", pages, 4, 2, self.device) != b:
-            raise S3BError(f"{what}: pages must be int32 [{b}, max_pages] with contiguous rows, lengths int32 [{b}]")
-        return b
+    def _sequences(self, what: str, pages, lengths):
+        """Batch, pointer, row stride and width of a page table int32 [batch, max_pages], and the pointer of its lengths int32 [batch]."""
+        device, shape = self.device, pages.shape
+        if len(shape) != 2 or lengths.shape != shape[:1] or pages.dtype is not _INDEX_TYPES[4] or lengths.dtype is not _INDEX_TYPES[4] or \
+                pages.get_device() != device or lengths.get_device() != device:
+            raise S3BError(f"{what}: pages must be int32 [batch, max_pages], lengths int32 [batch] on cuda:{device}")
+        b, width = shape
+        row, step = pages.stride()
+        if (step != 1 and width > 1) or (b > 1 and lengths.stride(0) != 1):
+            raise S3BError(f"{what}: pages must have contiguous rows, lengths be contiguous")
+        return b, pages.data_ptr(), row, width, lengths.data_ptr()
 
-    def _query(self, what: str, owner, q):
-        """Shape and strides of the queries f16 [batch, nq, heads, d] over a cache or bounds on this engine's GPU. The stride of a
-        dimension of one entry means nothing and is given as 0."""
+    def _query(self, what: str, owner, q, batch: int):
+        """Shape, pointer and strides of the queries f16 [batch, nq, heads, d] over a cache or bounds on this engine's GPU. The stride
+        of a dimension of one entry means nothing and is given as 0."""
         shape, device = q.shape, self.device
-        if len(shape) != 4 or _ROW_TYPES.get(q.dtype) != S3B_F16 or shape[3] != owner.d or q.get_device() != device or \
-                owner.device != device or (q.stride(3) != 1 and q.numel()):
-            raise S3BError(f"{what}: q must be f16 [batch, nq, heads, {owner.d}] with contiguous rows, on the engine's and the cache's GPU")
-        b, nq, heads, _ = shape
-        q_b, q_n, q_h, _ = q.stride()
-        return b, nq, heads, q_b if b > 1 else 0, q_n if nq > 1 else 0, q_h if heads > 1 else 0
+        if len(shape) != 4 or q.dtype is not _F16[0] or shape[3] != owner.d or shape[0] != batch or q.get_device() != device or owner.device != device:
+            raise S3BError(f"{what}: q must be f16 [{batch}, nq, heads, {owner.d}], on the engine's and the cache's GPU")
+        q_b, q_n, q_h, step = q.stride()
+        _, nq, heads, _ = shape
+        if step != 1 and nq * heads * batch:
+            raise S3BError(f"{what}: the rows of q must be contiguous")
+        return shape, nq, heads, q.data_ptr(), q_b if batch > 1 else 0, q_n if nq > 1 else 0, q_h if heads > 1 else 0
 
-    def _dense(self, what: str, name: str, t, dtype, shape):
-        """Checks a contiguous tensor of `dtype` and `shape` on this engine's GPU."""
+    def _dense(self, what: str, name: str, t, dtype, shape) -> int:
+        """Pointer of a contiguous tensor of `dtype` and `shape` on this engine's GPU."""
         if t.dtype is not dtype or t.shape != shape or t.get_device() != self.device or not t.is_contiguous():
             raise S3BError(f"{what}: {name} must be contiguous {dtype} {list(shape)} on cuda:{self.device}")
+        return t.data_ptr()
+
+    def _lists(self, what: str, selected, b: int, nq: int, share: int, heads: int):
+        """Pointer and length of the lists int32 [batch, ceil(nq / share), heads of the cache, keep]."""
+        shape = selected.shape
+        if share < 1 or len(shape) != 4:
+            raise S3BError(f"{what}: selected must have 4 dimensions, share be positive")
+        return self._dense(what, "selected", selected, _INDEX_TYPES[4], (b, -(-nq // share), heads, shape[3])), shape[3]
 
     def _rows_of_weights(self, what: str, cache: KVCache, weights, b: int, tokens: int):
         """Strides of weights f32 [batch, heads, tokens or more] with contiguous rows."""
         shape = weights.shape
-        if len(shape) != 3 or _ROW_TYPES.get(weights.dtype) != S3B_F32 or shape[0] != b or shape[1] != cache.heads or shape[2] < tokens or \
-                weights.get_device() != self.device or cache.device != self.device or (shape[2] > 1 and weights.stride(2) != 1):
-            raise S3BError(f"{what}: weights must be f32 [{b}, {cache.heads}, >= {tokens}] with contiguous rows, on the engine's and the cache's GPU")
-        w_b, w_h, _ = weights.stride()
+        if len(shape) != 3 or weights.dtype is not _F32[0] or shape[0] != b or shape[1] != cache.heads or shape[2] < tokens or \
+                weights.get_device() != self.device or cache.device != self.device:
+            raise S3BError(f"{what}: weights must be f32 [{b}, {cache.heads}, >= {tokens}], on the engine's and the cache's GPU")
+        w_b, w_h, step = weights.stride()
+        if step != 1 and shape[2] > 1:
+            raise S3BError(f"{what}: the rows of weights must be contiguous")
         return w_b if b > 1 else 0, w_h if cache.heads > 1 else 0
 
     def cache_bounds(self, cache: KVCache, bounds: KVBounds, pages, lengths, new: int | None = None):
         """Writes the bounds of the pages that hold the last `new` tokens of each sequence (None: of all its pages)
         (s3b_op_cache_bounds): pages int32 [batch, max_pages], lengths int32 [batch]."""
         what = "cache_bounds"
-        b = self._sequences(what, pages, lengths)
+        b, table, row, width, lens = self._sequences(what, pages, lengths)
         if cache.device != self.device or bounds.device != self.device:
             raise S3BError(f"{what}: cache and bounds must be on cuda:{self.device}")
-        rc = self._L.s3b_op_cache_bounds(self.h, cache.ref, bounds.ref, pages.data_ptr(), pages.stride(0), pages.shape[1],
-                                         lengths.data_ptr(), b, (1 << 62) if new is None else new)
+        call = _CALL.pack(table, row, lens, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, width, b, 0, 0, 0, 0, 0, 0, 0, 0.0)
+        rc = self._L.s3b_op_cache_bounds(self.h, cache.ref, bounds.ref, call, (1 << 62) if new is None else new)
         if rc:
             self._check(rc, "s3b_op_cache_bounds")
 
@@ -853,20 +882,14 @@ class Engine:
         int32 [batch, ceil(nq / share), bounds.heads, keep] gets the pages' places in the page table, ascending, -1 behind the last;
         scores f32 [batch, ceil(nq / share), bounds.heads, max_pages] or None."""
         what = "cache_select"
-        b, nq, heads, q_b, q_n, q_h = self._query(what, bounds, q)
-        if self._sequences(what, pages, lengths) != b:
-            raise S3BError(f"{what}: pages and lengths must have the queries' batch of {b}")
-        if share < 1 or selected.dim() != 4:
-            raise S3BError(f"{what}: selected must have 4 dimensions, share be positive")
-        lists = (b, -(-nq // share), bounds.heads)
-        keep = selected.shape[3]
-        self._dense(what, "selected", selected, _INDEX_TYPES[4], (*lists, keep))
-        max_pages = pages.shape[1]
+        b, table, row, width, lens = self._sequences(what, pages, lengths)
+        _, nq, heads, at, q_b, q_n, q_h = self._query(what, bounds, q, b)
+        lists, keep = self._lists(what, selected, b, nq, share, bounds.heads)
         if scores is not None:
-            self._dense(what, "scores", scores, _FLOAT[0], (*lists, max_pages))
-        rc = self._L.s3b_op_cache_select(self.h, bounds.ref, q.data_ptr(), q_b, q_n, q_h, selected.data_ptr(), keep, share, sink, recent,
-                                         _ptr(scores), pages.data_ptr(), pages.stride(0), max_pages, lengths.data_ptr(), b, nq, heads,
-                                         1 if causal else 0, window)
+            scores = self._dense(what, "scores", scores, _F32[0], (b, -(-nq // share), bounds.heads, width))
+        call = _CALL.pack(table, row, lens, at, q_b, q_n, q_h, 0, 0, 0, 0, 0, lists, width, b, nq, heads, 1 if causal else 0, window, keep,
+                          share, 0, 0.0)
+        rc = self._L.s3b_op_cache_select(self.h, bounds.ref, call, sink, recent, scores)
         if rc:
             self._check(rc, "s3b_op_cache_select")
 
@@ -875,24 +898,18 @@ class Engine:
         """cache_attention over the pages that the lists of cache_select name (s3b_op_cache_attention_selected): selected int32
         [batch, ceil(nq / share), cache.heads, keep], the other arguments as there."""
         what = "cache_attention_selected"
-        b, nq, heads, q_b, q_n, q_h = self._query(what, cache, q)
-        device = self.device
-        o_type = _ROW_TYPES.get(out.dtype)
-        if o_type is None or out.shape != q.shape or out.get_device() != device or (out.stride(3) != 1 and out.numel()):
+        b, table, row, width, lens = self._sequences(what, pages, lengths)
+        shape, nq, heads, at, q_b, q_n, q_h = self._query(what, cache, q, b)
+        o_type, device = _ROW_TYPES.get(out.dtype), self.device
+        o_b, o_n, o_h, step = out.stride() if out.dim() == 4 else (0, 0, 0, 0)
+        if o_type is None or out.shape != shape or out.get_device() != device or (step != 1 and b * nq * heads):
             raise S3BError(f"{what}: out must be f16 or f32 of q's shape with contiguous rows on cuda:{device}")
-        if self._sequences(what, pages, lengths) != b:
-            raise S3BError(f"{what}: pages and lengths must have the queries' batch of {b}")
-        if share < 1 or selected.dim() != 4:
-            raise S3BError(f"{what}: selected must have 4 dimensions, share be positive")
-        keep = selected.shape[3]
-        self._dense(what, "selected", selected, _INDEX_TYPES[4], (b, -(-nq // share), cache.heads, keep))
-        if lse is not None:
-            self._dense(what, "lse", lse, _FLOAT[0], (b, nq, heads))
-        o_b, o_n, o_h, _ = out.stride()
-        rc = self._L.s3b_op_cache_attention_selected(
-            self.h, cache.ref, q.data_ptr(), q_b, q_n, q_h, out.data_ptr(), 0 if o_type == S3B_F16 else 1, o_b if b > 1 else 0,
-            o_n if nq > 1 else 0, o_h if heads > 1 else 0, _ptr(lse), selected.data_ptr(), keep, share, pages.data_ptr(), pages.stride(0),
-            pages.shape[1], lengths.data_ptr(), b, nq, heads, scale, 1 if causal else 0, window)
+        lists, keep = self._lists(what, selected, b, nq, share, cache.heads)
+        lse = 0 if lse is None else self._dense(what, "lse", lse, _F32[0], (b, nq, heads))
+        call = _CALL.pack(table, row, lens, at, q_b, q_n, q_h, out.data_ptr(), o_b if b > 1 else 0, o_n if nq > 1 else 0,
+                          o_h if heads > 1 else 0, lse, lists, width, b, nq, heads, 1 if causal else 0, window, keep, share,
+                          0 if o_type == S3B_F16 else 1, scale)
+        rc = self._L.s3b_op_cache_attention_selected(self.h, cache.ref, call)
         if rc:
             self._check(rc, "s3b_op_cache_attention_selected")
 
@@ -902,15 +919,13 @@ class Engine:
         [batch, nq, heads] of the attention, weights f32 [batch, cache.heads, max_pages * page_size or more], the other arguments as in
         cache_attention."""
         what = "cache_weights"
-        b, nq, heads, q_b, q_n, q_h = self._query(what, cache, q)
-        if self._sequences(what, pages, lengths) != b:
-            raise S3BError(f"{what}: pages and lengths must have the queries' batch of {b}")
-        self._dense(what, "lse", lse, _FLOAT[0], (b, nq, heads))
-        max_pages = pages.shape[1]
-        w_b, w_h = self._rows_of_weights(what, cache, weights, b, max_pages * cache.page_size)
-        rc = self._L.s3b_op_cache_weights(self.h, cache.ref, q.data_ptr(), q_b, q_n, q_h, lse.data_ptr(), weights.data_ptr(), w_b, w_h,
-                                          decay, pages.data_ptr(), pages.stride(0), max_pages, lengths.data_ptr(), b, nq, heads, scale,
-                                          1 if causal else 0, window)
+        b, table, row, width, lens = self._sequences(what, pages, lengths)
+        _, nq, heads, at, q_b, q_n, q_h = self._query(what, cache, q, b)
+        lse = self._dense(what, "lse", lse, _F32[0], (b, nq, heads))
+        w_b, w_h = self._rows_of_weights(what, cache, weights, b, width * cache.page_size)
+        call = _CALL.pack(table, row, lens, at, q_b, q_n, q_h, 0, 0, 0, 0, lse, 0, width, b, nq, heads, 1 if causal else 0, window, 0, 0, 0,
+                          scale)
+        rc = self._L.s3b_op_cache_weights(self.h, cache.ref, call, weights.data_ptr(), w_b, w_h, decay)
         if rc:
             self._check(rc, "s3b_op_cache_weights")
 
@@ -920,19 +935,20 @@ class Engine:
         and gets their positions (-1 behind the last); pages_out int32 [batch, ceil(keep / page_size) or more], lengths_out int32
         [batch], weights_out f32 of kept's shape or None; to: the cache of the new pages, if another."""
         what = "cache_evict"
-        b, device = self._sequences(what, pages, lengths), self.device
-        target = cache if to is None else to
-        if kept.dim() != 3 or target.device != device:
-            raise S3BError(f"{what}: kept must have 3 dimensions, the new pages' cache be on cuda:{device}")
-        keep = kept.shape[2]
-        self._dense(what, "kept", kept, _INDEX_TYPES[4], (b, cache.heads, keep))
-        w_b, w_h = self._rows_of_weights(what, cache, weights, b, pages.shape[1] * cache.page_size)
-        if self._sequences(what, pages_out, lengths_out) != b or pages_out.shape[1] * target.page_size < keep:
+        b, table, row, width, lens = self._sequences(what, pages, lengths)
+        b_out, table_out, row_out, width_out, lens_out = self._sequences(what, pages_out, lengths_out)
+        target, shape = cache if to is None else to, kept.shape
+        if len(shape) != 3 or target.device != self.device:
+            raise S3BError(f"{what}: kept must have 3 dimensions, the new pages' cache be on cuda:{self.device}")
+        keep = shape[2]
+        if b_out != b or width_out * target.page_size < keep:
             raise S3BError(f"{what}: pages_out must hold {keep} tokens for each of {b} sequences, lengths_out be int32 [{b}]")
-        if weights_out is not None:
-            self._dense(what, "weights_out", weights_out, _FLOAT[0], kept.shape)
-        rc = self._L.s3b_op_cache_evict(self.h, cache.ref, None if to is None else to.ref, weights.data_ptr(), w_b, w_h, pages.data_ptr(),
-                                        pages.stride(0), pages.shape[1], lengths.data_ptr(), b, keep, sink, recent, pages_out.data_ptr(),
-                                        pages_out.stride(0), lengths_out.data_ptr(), kept.data_ptr(), _ptr(weights_out))
+        positions = self._dense(what, "kept", kept, _INDEX_TYPES[4], (b, cache.heads, keep))
+        w_b, w_h = self._rows_of_weights(what, cache, weights, b, width * cache.page_size)
+        moved = 0 if weights_out is None else self._dense(what, "weights_out", weights_out, _F32[0], shape)
+        call = _CALL.pack(table, row, lens, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, width, b, 0, 0, 0, 0, 0, 0, 0, 0.0)
+        evict = _EVICT.pack(0 if to is None else ctypes.addressof(to.desc), weights.data_ptr(), w_b, w_h, table_out, row_out, lens_out, positions,
+                            moved, keep, sink, recent)
+        rc = self._L.s3b_op_cache_evict(self.h, cache.ref, call, evict)
         if rc:
             self._check(rc, "s3b_op_cache_evict")

@@ -1558,54 +1558,57 @@ int s3b_op_cache_attention(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* 
   return kOk;
 }
 
-// The arguments that the calls on long caches share, into p: the sequences, then the queries over them.
-static int kv_sequences(s3b_ctx* ctx, const char* what, KvAttnParams* p, const int32_t* pages, int64_t pages_stride,
-                        int max_pages, const int32_t* lengths, int batch) {
+// What the calls on long caches take of an s3b_kv_call, into p: the sequences, the queries over them, the lists of pages.
+static int kv_sequences(s3b_ctx* ctx, const char* what, KvAttnParams* p, const s3b_kv_call* call) {
+  if (!call) return set_error(ctx, kErrArg, "%s: null call", what);
+  const int batch = call->batch, max_pages = call->max_pages;
   if (batch < 0 || max_pages < 0) return set_error(ctx, kErrArg, "%s: negative size", what);
-  if (batch > 0 && (!lengths || (!pages && max_pages > 0))) return set_error(ctx, kErrArg, "%s: null pointer", what);
-  if (max_pages > 0 && batch > 1 && pages_stride != 0 && pages_stride < max_pages)
-    return set_error(ctx, kErrArg, "%s: page table rows of %lld hold no %d pages", what, (long long)pages_stride, max_pages);
+  if (batch > 0 && (!call->lengths || (!call->pages && max_pages > 0))) return set_error(ctx, kErrArg, "%s: null pointer", what);
+  if (max_pages > 0 && batch > 1 && call->pages_stride != 0 && call->pages_stride < max_pages)
+    return set_error(ctx, kErrArg, "%s: page table rows of %lld hold no %d pages", what, (long long)call->pages_stride, max_pages);
   if ((long long)max_pages * p->c.page_size > kMaxCacheTokens)
     return set_error(ctx, kErrUnsupported, "%s: a sequence may hold %lld tokens at most", what, kMaxCacheTokens);
-  if (!multiple_of(pages, 4) || !multiple_of(lengths, 4))
+  if (!multiple_of(call->pages, 4) || !multiple_of(call->lengths, 4))
     return set_error(ctx, kErrArg, "%s: pages and lengths must be 4-byte aligned", what);
-  p->pages = pages;
-  p->pages_stride = pages_stride;
+  p->pages = call->pages;
+  p->pages_stride = call->pages_stride;
   p->max_pages = max_pages;
-  p->lengths = lengths;
+  p->lengths = call->lengths;
   p->batch = batch;
   return kOk;
 }
 
-static int kv_queries(s3b_ctx* ctx, const char* what, KvAttnParams* p, const void* q, int64_t q_b, int64_t q_n, int64_t q_h,
-                      int nq, int heads, int causal, int window) {
+static int kv_queries(s3b_ctx* ctx, const char* what, KvAttnParams* p, const s3b_kv_call* call) {
+  const int nq = call->nq, heads = call->heads;
   if (nq < 0) return set_error(ctx, kErrArg, "%s: negative size", what);
   if (heads <= 0 || heads % p->c.heads)
     return set_error(ctx, kErrArg, "%s: %d query heads over %d key / value heads", what, heads, p->c.heads);
-  if (window < 0 || (window > 0 && !causal))
+  if (call->window < 0 || (call->window > 0 && !call->causal))
     return set_error(ctx, kErrArg, "%s: a window must be positive and causal", what);
   if ((long long)nq * heads > 0x3fffffffLL) return set_error(ctx, kErrUnsupported, "%s: %d queries of %d heads", what, nq, heads);
-  if (!q && nq > 0 && p->batch > 0) return set_error(ctx, kErrArg, "%s: null pointer", what);
-  if (!rows_aligned(q, 2, q_b, q_n, q_h)) return set_error(ctx, kErrArg, "%s: rows must start on 16-byte boundaries", what);
-  p->q = reinterpret_cast<const __half*>(q);
-  p->q_b = q_b;
-  p->q_n = q_n;
-  p->q_h = q_h;
+  if (!call->q && nq > 0 && p->batch > 0) return set_error(ctx, kErrArg, "%s: null pointer", what);
+  if (!rows_aligned(call->q, 2, call->q_b, call->q_n, call->q_h))
+    return set_error(ctx, kErrArg, "%s: rows must start on 16-byte boundaries", what);
+  p->q = reinterpret_cast<const __half*>(call->q);
+  p->q_b = call->q_b;
+  p->q_n = call->q_n;
+  p->q_h = call->q_h;
   p->nq = nq;
   p->heads = heads;
-  p->causal = causal ? 1 : 0;
-  p->window = window;
+  p->causal = call->causal ? 1 : 0;
+  p->window = call->window;
   return kOk;
 }
 
-static int kv_lists(s3b_ctx* ctx, const char* what, KvAttnParams* p, const int32_t* selected, int keep, int share) {
+static int kv_lists(s3b_ctx* ctx, const char* what, KvAttnParams* p, const s3b_kv_call* call) {
+  const int keep = call->keep, share = call->share;
   if (keep < 1 || share < 1) return set_error(ctx, kErrArg, "%s: lists of %d pages for blocks of %d queries", what, keep, share);
   const long long rows = (long long)std::min(share, std::max(p->nq, 1)) * (p->heads / p->c.heads);
   if (rows > kv_attention_most_rows(p->c.d))
     return set_error(ctx, kErrUnsupported, "%s: %lld rows share a list, at most %d may", what, rows, kv_attention_most_rows(p->c.d));
-  if (p->batch > 0 && p->nq > 0 && !selected) return set_error(ctx, kErrArg, "%s: null pointer", what);
-  if (!multiple_of(selected, 4)) return set_error(ctx, kErrArg, "%s: selected must be 4-byte aligned", what);
-  p->selected = selected;
+  if (p->batch > 0 && p->nq > 0 && !call->selected) return set_error(ctx, kErrArg, "%s: null pointer", what);
+  if (!multiple_of(call->selected, 4)) return set_error(ctx, kErrArg, "%s: selected must be 4-byte aligned", what);
+  p->selected = call->selected;
   p->keep = keep;
   p->share = std::min(share, std::max(p->nq, 1));
   if (kv_attention_units(*p) > 0x7fffffffLL || kv_attention_units(*p) * keep > (1LL << 40))
@@ -1636,6 +1639,25 @@ static int kv_bounds_arg(s3b_ctx* ctx, const char* what, const s3b_kv_bounds* bo
   return kOk;
 }
 
+int s3b_kv_bounds_values(const s3b_kv_bounds* bounds, const int64_t* pages, int64_t n, float* out, void* cuda_stream) {
+  KvCache shape;
+  KvBounds b;
+  if (!bounds || !bounds->codes || !bounds->steps || n < 0) return kErrArg;
+  shape.type = S3B_Q4_0;
+  shape.heads = bounds->heads;
+  shape.d = bounds->d;
+  shape.page_size = bounds->page_size;
+  shape.n_pages = bounds->n_pages;
+  b.codes = reinterpret_cast<int8_t*>(bounds->codes);
+  b.steps = bounds->steps;
+  if (kv_cache_bytes(shape) < 0 || !multiple_of(b.codes, 16) || !multiple_of(b.steps, 4) || !multiple_of(pages, 8) || !multiple_of(out, 16) || n > (1LL << 40))
+    return kErrArg;
+  if (n == 0) return kOk;
+  if (!pages || !out) return kErrArg;
+  const int rc = kv_bounds_values(shape, b, reinterpret_cast<const long long*>(pages), n, out, static_cast<cudaStream_t>(cuda_stream));
+  return rc ? kErrCuda : kOk;
+}
+
 static bool stream_capturing(s3b_ctx* ctx) {
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(ctx->stream, &capture) != cudaSuccess) cudaGetLastError();
@@ -1648,8 +1670,8 @@ static size_t power_of_two(size_t n, size_t least) {
   return least;
 }
 
-int s3b_op_cache_bounds(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_bounds* bounds, const int32_t* pages,
-                        int64_t pages_stride, int max_pages, const int32_t* lengths, int batch, int64_t recent) {
+int s3b_op_cache_bounds(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_bounds* bounds, const s3b_kv_call* call,
+                        int64_t recent) {
   int rc = ctx_enter(ctx);
   if (rc) return rc;
   KvAttnParams p;
@@ -1660,76 +1682,69 @@ int s3b_op_cache_bounds(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_bo
   if (shape.heads != p.c.heads || shape.d != p.c.d || shape.page_size != p.c.page_size || shape.n_pages != p.c.n_pages)
     return set_error(ctx, kErrArg, "cache_bounds: the bounds have another shape than the cache");
   if (recent < 0) return set_error(ctx, kErrArg, "cache_bounds: %lld tokens", (long long)recent);
-  if ((rc = kv_sequences(ctx, "cache_bounds", &p, pages, pages_stride, max_pages, lengths, batch))) return rc;
-  if (batch == 0 || max_pages == 0 || recent == 0) return kOk;
-  rc = kv_bounds(p, out, std::min<long long>(recent, (long long)max_pages * p.c.page_size), ctx->d_err, ctx->stream);
+  if ((rc = kv_sequences(ctx, "cache_bounds", &p, call))) return rc;
+  if (p.batch == 0 || p.max_pages == 0 || recent == 0) return kOk;
+  rc = kv_bounds(p, out, std::min<long long>(recent, (long long)p.max_pages * p.c.page_size), ctx->d_err, ctx->stream);
   if (rc) return set_error(ctx, launcher_status_code(rc), "cache_bounds launch failed (%d)", rc);
   count_launch(ctx);
   return kOk;
 }
 
-int s3b_op_cache_select(s3b_ctx* ctx, const s3b_kv_bounds* bounds, const void* q, int64_t q_b, int64_t q_n, int64_t q_h,
-                        int32_t* selected, int keep, int share, int sink, int recent, float* scores,
-                        const int32_t* pages, int64_t pages_stride, int max_pages, const int32_t* lengths, int batch,
-                        int nq, int heads, int causal, int window) {
+int s3b_op_cache_select(s3b_ctx* ctx, const s3b_kv_bounds* bounds, const s3b_kv_call* call, int sink, int recent, float* scores) {
   const char* what = "cache_select";
   int rc = ctx_enter(ctx);
   if (rc) return rc;
   KvAttnParams p;
   KvBounds b;
   if ((rc = kv_bounds_arg(ctx, what, bounds, &p.c, &b))) return rc;
-  if ((rc = kv_sequences(ctx, what, &p, pages, pages_stride, max_pages, lengths, batch))) return rc;
-  if ((rc = kv_queries(ctx, what, &p, q, q_b, q_n, q_h, nq, heads, causal, window))) return rc;
-  if ((rc = kv_lists(ctx, what, &p, selected, keep, share))) return rc;
-  if (sink < 0 || recent < 0 || (long long)sink + recent > keep)
-    return set_error(ctx, kErrArg, "cache_select: %d first and %d last pages of %d", sink, recent, keep);
+  if ((rc = kv_sequences(ctx, what, &p, call))) return rc;
+  if ((rc = kv_queries(ctx, what, &p, call))) return rc;
+  if ((rc = kv_lists(ctx, what, &p, call))) return rc;
+  if (sink < 0 || recent < 0 || (long long)sink + recent > p.keep)
+    return set_error(ctx, kErrArg, "cache_select: %d first and %d last pages of %d", sink, recent, p.keep);
   if (!multiple_of(scores, 4)) return set_error(ctx, kErrArg, "cache_select: scores must be 4-byte aligned");
-  if (batch == 0 || nq == 0) return kOk;
+  if (p.batch == 0 || p.nq == 0) return kOk;
   const bool all = scores != nullptr;
   const long long units = kv_attention_units(p);
-  if (units * std::max(max_pages, 1) > (1LL << 40))
-    return set_error(ctx, kErrUnsupported, "cache_select: %lld lists over %d pages", units, max_pages);
+  if (units * std::max(p.max_pages, 1) > (1LL << 40))
+    return set_error(ctx, kErrUnsupported, "cache_select: %lld lists over %d pages", units, p.max_pages);
   const int sms = num_sms();
   if (!all && kv_select_needs_scores(p, sms)) {
     bool grown;
-    DevBuf* buf = graph_buf(ctx, "kv_select_scores", power_of_two((size_t)units * max_pages * 4, 1 << 20), stream_capturing(ctx), &grown, &rc);
+    DevBuf* buf = graph_buf(ctx, "kv_select_scores", power_of_two((size_t)units * p.max_pages * 4, 1 << 20), stream_capturing(ctx), &grown, &rc);
     if (rc) return rc;
     scores = buf->as<float>();
   }
-  rc = kv_select(p, b, sink, recent, scores, all, selected, sms, ctx->d_err, ctx->stream);
+  rc = kv_select(p, b, sink, recent, scores, all, call->selected, sms, ctx->d_err, ctx->stream);
   if (rc) return set_error(ctx, launcher_status_code(rc), "cache_select launch failed (%d)", rc);
   count_launch(ctx);
   return kOk;
 }
 
-int s3b_op_cache_attention_selected(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* q, int64_t q_b, int64_t q_n,
-                                    int64_t q_h, void* out, int out_f32, int64_t o_b, int64_t o_n, int64_t o_h,
-                                    float* lse, const int32_t* selected, int keep, int share, const int32_t* pages,
-                                    int64_t pages_stride, int max_pages, const int32_t* lengths, int batch, int nq,
-                                    int heads, float scale, int causal, int window) {
+int s3b_op_cache_attention_selected(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_call* call) {
   const char* what = "cache_attention_selected";
   int rc = ctx_enter(ctx);
   if (rc) return rc;
   KvAttnParams p;
   if ((rc = kv_cache_arg(ctx, cache, &p.c))) return rc;
-  if ((rc = kv_sequences(ctx, what, &p, pages, pages_stride, max_pages, lengths, batch))) return rc;
-  if ((rc = kv_queries(ctx, what, &p, q, q_b, q_n, q_h, nq, heads, causal, window))) return rc;
-  if ((rc = kv_lists(ctx, what, &p, selected, keep, share))) return rc;
-  if ((rc = kv_scale(ctx, what, &p, scale))) return rc;
+  if ((rc = kv_sequences(ctx, what, &p, call))) return rc;
+  if ((rc = kv_queries(ctx, what, &p, call))) return rc;
+  if ((rc = kv_lists(ctx, what, &p, call))) return rc;
+  if ((rc = kv_scale(ctx, what, &p, call->scale))) return rc;
   // a list's groups of 16 tokens are counted in 32 bits
-  if ((long long)keep * p.c.page_size > kMaxCacheTokens)
+  if ((long long)p.keep * p.c.page_size > kMaxCacheTokens)
     return set_error(ctx, kErrUnsupported, "%s: a list may name %lld tokens at most", what, kMaxCacheTokens);
-  if (!rows_aligned(out, out_f32 ? 4 : 2, o_b, o_n, o_h))
+  if (!rows_aligned(call->out, call->out_f32 ? 4 : 2, call->o_b, call->o_n, call->o_h))
     return set_error(ctx, kErrArg, "%s: rows must start on 16-byte boundaries", what);
-  if (!multiple_of(lse, 4)) return set_error(ctx, kErrArg, "%s: lse must be 4-byte aligned", what);
-  if (batch == 0 || nq == 0) return kOk;
-  if (!out) return set_error(ctx, kErrArg, "%s: null pointer", what);
-  p.out = out;
-  p.out_f32 = out_f32 ? 1 : 0;
-  p.o_b = o_b;
-  p.o_n = o_n;
-  p.o_h = o_h;
-  p.lse = lse;
+  if (!multiple_of(call->lse, 4)) return set_error(ctx, kErrArg, "%s: lse must be 4-byte aligned", what);
+  if (p.batch == 0 || p.nq == 0) return kOk;
+  if (!call->out) return set_error(ctx, kErrArg, "%s: null pointer", what);
+  p.out = call->out;
+  p.out_f32 = call->out_f32 ? 1 : 0;
+  p.o_b = call->o_b;
+  p.o_n = call->o_n;
+  p.o_h = call->o_h;
+  p.lse = call->lse;
   KvAttnWork w;
   w.sms = num_sms();
   const bool capturing = stream_capturing(ctx);
@@ -1749,76 +1764,78 @@ int s3b_op_cache_attention_selected(s3b_ctx* ctx, const s3b_kv_cache* cache, con
   return kOk;
 }
 
-int s3b_op_cache_weights(s3b_ctx* ctx, const s3b_kv_cache* cache, const void* q, int64_t q_b, int64_t q_n, int64_t q_h,
-                         const float* lse, float* weights, int64_t w_b, int64_t w_h, float decay, const int32_t* pages,
-                         int64_t pages_stride, int max_pages, const int32_t* lengths, int batch, int nq, int heads,
-                         float scale, int causal, int window) {
+int s3b_op_cache_weights(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_call* call, float* weights, int64_t w_b,
+                         int64_t w_h, float decay) {
   const char* what = "cache_weights";
   int rc = ctx_enter(ctx);
   if (rc) return rc;
   KvAttnParams p;
   if ((rc = kv_cache_arg(ctx, cache, &p.c))) return rc;
-  if ((rc = kv_sequences(ctx, what, &p, pages, pages_stride, max_pages, lengths, batch))) return rc;
-  if ((rc = kv_queries(ctx, what, &p, q, q_b, q_n, q_h, nq, heads, causal, window))) return rc;
-  if ((rc = kv_scale(ctx, what, &p, scale))) return rc;
+  if ((rc = kv_sequences(ctx, what, &p, call))) return rc;
+  if ((rc = kv_queries(ctx, what, &p, call))) return rc;
+  if ((rc = kv_scale(ctx, what, &p, call->scale))) return rc;
   if (!(decay >= 0.f) || std::isinf(decay)) return set_error(ctx, kErrArg, "cache_weights: decay must be finite and not negative");
-  if (!multiple_of(lse, 4) || !multiple_of(weights, 4))
+  if (!multiple_of(call->lse, 4) || !multiple_of(weights, 4))
     return set_error(ctx, kErrArg, "cache_weights: lse and weights must be 4-byte aligned");
-  if (batch == 0 || max_pages == 0) return kOk;
-  if (!weights || (!lse && nq > 0)) return set_error(ctx, kErrArg, "cache_weights: null pointer");
-  const long long tokens = (long long)max_pages * p.c.page_size, kv = p.c.heads;
+  if (p.batch == 0 || p.max_pages == 0) return kOk;
+  if (!weights || (!call->lse && p.nq > 0)) return set_error(ctx, kErrArg, "cache_weights: null pointer");
+  const long long tokens = (long long)p.max_pages * p.c.page_size, kv = p.c.heads, batch = p.batch;
   const bool by_head = (kv == 1 || w_h >= tokens) && (batch == 1 || w_b >= (kv - 1) * (kv > 1 ? w_h : 0) + tokens);
   const bool by_batch = (batch == 1 || w_b >= tokens) && (kv == 1 || w_h >= (batch - 1) * (batch > 1 ? w_b : 0) + tokens);
   if (!by_head && !by_batch) return set_error(ctx, kErrArg, "cache_weights: rows of %lld weights overlap", tokens);
-  p.lse = const_cast<float*>(lse);
+  p.lse = call->lse;
   KvWeights w;
   w.w = weights;
   w.w_b = w_b;
   w.w_h = w_h;
   w.decay = decay;
   const int sms = num_sms();
-  const bool capturing = stream_capturing(ctx);
-  bool grown;
-  DevBuf* part = graph_buf(ctx, "kv_weights_part", kv_weights_part(sms), capturing, &grown, &rc);
-  if (rc) return rc;
-  w.part = part->as<float>();
-  DevBuf* count = graph_buf(ctx, "kv_weights_count", (size_t)sms * 4, capturing, &grown, &rc);
-  if (rc) return rc;
-  if (grown && cudaMemsetAsync(count->p, 0, count->bytes, ctx->stream) != cudaSuccess)
-    return set_error(ctx, kErrCuda, "cache_weights: clearing the counts");
-  w.count = count->as<int>();
+  if (const size_t need = kv_weights_part(p, sms)) {
+    const bool capturing = stream_capturing(ctx);
+    bool grown;
+    DevBuf* part = graph_buf(ctx, "kv_weights_part", need, capturing, &grown, &rc);
+    if (rc) return rc;
+    w.part = part->as<float>();
+    DevBuf* count = graph_buf(ctx, "kv_weights_count", (size_t)sms * 4, capturing, &grown, &rc);
+    if (rc) return rc;
+    if (grown && cudaMemsetAsync(count->p, 0, count->bytes, ctx->stream) != cudaSuccess)
+      return set_error(ctx, kErrCuda, "cache_weights: clearing the counts");
+    w.count = count->as<int>();
+  }
   rc = kv_weights(p, w, sms, ctx->d_err, ctx->stream);
   if (rc) return set_error(ctx, launcher_status_code(rc), "cache_weights launch failed (%d)", rc);
   count_launch(ctx);
   return kOk;
 }
 
-int s3b_op_cache_evict(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_cache* to, const float* weights,
-                       int64_t w_b, int64_t w_h, const int32_t* pages, int64_t pages_stride, int max_pages,
-                       const int32_t* lengths, int batch, int keep, int sink, int recent, const int32_t* pages_out,
-                       int64_t out_stride, int32_t* lengths_out, int32_t* kept, float* weights_out) {
+int s3b_op_cache_evict(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_call* call, const s3b_kv_evict* evict) {
   const char* what = "cache_evict";
   int rc = ctx_enter(ctx);
   if (rc) return rc;
   KvAttnParams p;
   KvEvict e;
   if ((rc = kv_cache_arg(ctx, cache, &p.c))) return rc;
-  if ((rc = kv_cache_arg(ctx, to ? to : cache, &e.to))) return rc;
+  if (!evict) return set_error(ctx, kErrArg, "cache_evict: nothing to keep");
+  if ((rc = kv_cache_arg(ctx, evict->to ? evict->to : cache, &e.to))) return rc;
   if (e.to.type != p.c.type || e.to.heads != p.c.heads || e.to.d != p.c.d)
     return set_error(ctx, kErrArg, "cache_evict: the new pages are of a cache of another type, heads or d");
-  if ((rc = kv_sequences(ctx, what, &p, pages, pages_stride, max_pages, lengths, batch))) return rc;
+  if ((rc = kv_sequences(ctx, what, &p, call))) return rc;
+  const int batch = p.batch, max_pages = p.max_pages, keep = evict->keep, sink = evict->sink, recent = evict->recent;
+  const int64_t w_b = evict->w_b, w_h = evict->w_h, out_stride = evict->out_stride;
+  const float* weights = evict->weights;
+  float* weights_out = evict->weights_out;
   if (keep < 0 || sink < 0 || recent < 0 || (long long)sink + recent > keep)
     return set_error(ctx, kErrArg, "cache_evict: %d first and %d last tokens of %d", sink, recent, keep);
   const long long new_pages = ((long long)keep + e.to.page_size - 1) / e.to.page_size;
   if (batch > 1 && out_stride < new_pages)
     return set_error(ctx, kErrArg, "cache_evict: rows of %lld new pages hold no %lld", (long long)out_stride, new_pages);
-  if (!multiple_of(weights, 4) || !multiple_of(pages_out, 4) || !multiple_of(lengths_out, 4) || !multiple_of(kept, 4) ||
+  if (!multiple_of(weights, 4) || !multiple_of(evict->pages_out, 4) || !multiple_of(evict->lengths_out, 4) || !multiple_of(evict->kept, 4) ||
       !multiple_of(weights_out, 4))
     return set_error(ctx, kErrArg, "cache_evict: arrays must be 4-byte aligned");
   if (batch == 0) return kOk;
-  if (!lengths_out || (keep > 0 && (!kept || !pages_out || (!weights && max_pages > 0))))
+  if (!evict->lengths_out || (keep > 0 && (!evict->kept || !evict->pages_out || (!weights && max_pages > 0))))
     return set_error(ctx, kErrArg, "cache_evict: null pointer");
-  if (lengths_out == lengths) return set_error(ctx, kErrArg, "cache_evict: lengths_out is the array of lengths");
+  if (evict->lengths_out == call->lengths) return set_error(ctx, kErrArg, "cache_evict: lengths_out is the array of lengths");
   if ((long long)batch * p.c.heads > (1LL << 40) / std::max(keep, 1))
     return set_error(ctx, kErrUnsupported, "cache_evict: %d sequences of %d heads keep %d tokens", batch, p.c.heads, keep);
   if (weights_out) {  // the weights that are read, from the first to the last
@@ -1832,10 +1849,10 @@ int s3b_op_cache_evict(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_cac
   e.weights = weights;
   e.w_b = w_b;
   e.w_h = w_h;
-  e.pages_out = pages_out;
+  e.pages_out = evict->pages_out;
   e.out_stride = out_stride;
-  e.lengths_out = lengths_out;
-  e.kept = kept;
+  e.lengths_out = evict->lengths_out;
+  e.kept = evict->kept;
   e.weights_out = weights_out;
   e.keep = keep;
   e.sink = sink;

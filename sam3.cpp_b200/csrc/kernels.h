@@ -431,6 +431,8 @@ struct KvBounds {
 };
 // Bounds of the pages that hold the last `recent` tokens of each sequence (p: cache, pages, lengths).
 int kv_bounds(const KvAttnParams& p, const KvBounds& out, long long recent, int* err, cudaStream_t st);
+// f32 [n][heads][2][d] of the pages (shape: heads, d, n_pages).
+int kv_bounds_values(const KvCache& shape, const KvBounds& bounds, const long long* pages, long long n, float* out, cudaStream_t st);
 // Chooses p.keep pages for each block of p.share queries and key / value head (p: queries, pages, lengths, masks; of p.c the
 // shape). scores: [units][max_pages], of all pages with `all`, else a workspace, or none unless kv_select_needs_scores.
 int kv_select(const KvAttnParams& p, const KvBounds& bounds, int sink, int recent, float* scores, bool all, int* selected, int sms,
@@ -442,10 +444,10 @@ struct KvWeights {
   float* w = nullptr;
   long long w_b = 0, w_h = 0;
   float decay = 1.f;
-  float* part = nullptr;  // workspace of kv_weights_part(sms) bytes, and counts of one int for each SM, zero before and after
+  float* part = nullptr;  // workspace of kv_weights_part bytes (none: 0), and with it an int for each SM, zero before and after
   int* count = nullptr;
 };
-size_t kv_weights_part(int sms);
+size_t kv_weights_part(const KvAttnParams& p, int sms);
 int kv_weights(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st);
 // The tensor-core kernel for many rows (kv_weights picks it).
 size_t kv_weights_tc_part(int sms);

@@ -122,6 +122,26 @@ __global__ void __launch_bounds__(128) bounds_kernel(const __grid_constant__ Bou
   }
 }
 
+// What the codes of n pages stand for: f32 [n][heads][2][d], 4 values a thread.
+__global__ void __launch_bounds__(256) values_kernel(const int8_t* codes, const float* steps, const long long* pages, long long n, long long n_pages,
+                                                     int heads, int d, float* out) {
+  const int quads = d / 2;  // of a page and head
+  let_next();
+  wait_before();
+  const long long all = n * heads * quads;
+  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < all; e += (long long)gridDim.x * 256) {
+    const long long row = e / quads, i = row / heads, page = pages[i];
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (page >= 0 && page < n_pages) {
+      const long long at = page * heads + (row - i * heads);
+      const char4 c = *reinterpret_cast<const char4*>(codes + at * 2 * d + (e - row * quads) * 4);
+      const float step = steps[at];
+      v = make_float4(c.x * step, c.y * step, c.z * step, c.w * step);
+    }
+    reinterpret_cast<float4*>(out)[e] = v;
+  }
+}
+
 typedef void (*BoundsKernel)(BoundsArgs, int*);
 
 template <int QT>
@@ -130,6 +150,12 @@ BoundsKernel bounds_for(int d) {
 }
 
 }  // namespace
+
+int kv_bounds_values(const KvCache& shape, const KvBounds& bounds, const long long* pages, long long n, float* out, cudaStream_t st) {
+  const long long blocks = (n * shape.heads * (shape.d / 2) + 255) / 256;
+  return launch_dependent(values_kernel, dim3((unsigned)std::min(blocks, 1LL << 20)), 256, 0, st, (const int8_t*)bounds.codes, (const float*)bounds.steps, pages, n,
+                          shape.n_pages, shape.heads, shape.d, out);
+}
 
 int kv_bounds(const KvAttnParams& p, const KvBounds& out, long long recent, int* err, cudaStream_t st) {
   BoundsArgs a{p, out, recent, p.max_pages};

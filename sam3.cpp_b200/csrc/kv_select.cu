@@ -38,7 +38,7 @@ __host__ __device__ constexpr int select_threads() { return CL == 1 || NT * D > 
 // then two f32 products, each rounded, so that the choice is the same whatever the order. Lane (g, t) holds 16 channels of 64 as
 // the contraction's share of its rows (pages g, g + 8; query row g): whole 16-byte words of both.
 template <int D, int NT, int CL>
-__global__ void __launch_bounds__(select_threads<D, NT, CL>()) select_kernel(const __grid_constant__ SelectArgs a, int* err) {
+__global__ void __launch_bounds__(select_threads<D, NT, CL>(), CL == 1 ? 2 : 1) select_kernel(const __grid_constant__ SelectArgs a, int* err) {
   constexpr int NC = D / 64, kThreads = select_threads<D, NT, CL>();
   extern __shared__ uint32_t s_keys[];
   __shared__ TopShared<kThreads> s_top;
@@ -71,11 +71,16 @@ __global__ void __launch_bounds__(select_threads<D, NT, CL>()) select_kernel(con
     for (int j = rank * kThreads + threadIdx.x; j < p.max_pages; j += CL * kThreads)
       if (j < pa || j >= pe) scores[j] = -INFINITY;
 
-  // ---- the query rows' codes, of either sign apart: column g of tile nt is row 8 nt + g
+  // ---- the query rows' codes, of either sign apart: column g of tile nt is row 8 nt + g. Where they would take too many registers
+  // they stay in shared memory, and the warps share the work of making them.
+  constexpr bool kShared = NT * D >= 512;
+  __shared__ uint4 s_codes[kShared ? NT * NC * 32 * 2 : 1];  // [tile][64 channels][positive, negative][lane]
+  __shared__ float s_step[NT * 8];
   uint32_t pos[NT][NC][4], neg[NT][NC][4];
   float step[NT][2];  // of columns 2t, 2t + 1; < 0: no such row
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
+    if (kShared && nt != warp) continue;  // a warp a tile
     const int r = 8 * nt + g;
     const int i = i0 + r / group_heads, h = head * group_heads + r % group_heads;
     const __half* q = p.q + b * p.q_b + i * p.q_n + h * p.q_h + 16 * t;
@@ -106,24 +111,41 @@ __global__ void __launch_bounds__(select_threads<D, NT, CL>()) select_kernel(con
     const float peak = __half2float(__ushort_as_half((unsigned short)top));
     const float inv = peak != 0.f ? __fdiv_rn(127.f, peak) : 0.f;
     const float mine = r < n_rows ? __fdiv_rn(peak, 127.f) : -1.f;
-    step[nt][0] = __shfl_sync(~0u, mine, 8 * t);
-    step[nt][1] = __shfl_sync(~0u, mine, 8 * t + 4);
+    if (kShared) {
+      if (t == 0) s_step[r] = mine;
+    } else {
+      step[nt][0] = __shfl_sync(~0u, mine, 8 * t);
+      step[nt][1] = __shfl_sync(~0u, mine, 8 * t + 4);
+    }
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int c = 0; c < NC; ++c) {
+      uint32_t wp[4], wn[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 x0 = __half22float2(u32_h2(raw[c][2 * e])), x1 = __half22float2(u32_h2(raw[c][2 * e + 1]));
         const float x[4] = {x0.x, x0.y, x1.x, x1.y};
-        uint32_t wp = 0, wn = 0;
+        wp[e] = wn[e] = 0;
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
           const int code = max(-127, min(127, __float2int_rn(__fmul_rn(x[f], inv))));
-          wp |= (uint32_t)max(code, 0) << (8 * f);
-          wn |= (uint32_t)(min(code, 0) & 255) << (8 * f);
+          wp[e] |= (uint32_t)max(code, 0) << (8 * f);
+          wn[e] |= (uint32_t)(min(code, 0) & 255) << (8 * f);
         }
-        pos[nt][c][e] = wp;
-        neg[nt][c][e] = wn;
+        if (!kShared) pos[nt][c][e] = wp[e], neg[nt][c][e] = wn[e];
       }
+      if (kShared) {
+        s_codes[((nt * NC + c) * 2 + 0) * 32 + lane] = make_uint4(wp[0], wp[1], wp[2], wp[3]);
+        s_codes[((nt * NC + c) * 2 + 1) * 32 + lane] = make_uint4(wn[0], wn[1], wn[2], wn[3]);
+      }
+    }
+  }
+  if (kShared) {
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      step[nt][0] = s_step[8 * nt + 2 * t];
+      step[nt][1] = s_step[8 * nt + 2 * t + 1];
+    }
   }
 
   // ---- scores of 16 pages at a time
@@ -167,10 +189,12 @@ __global__ void __launch_bounds__(select_threads<D, NT, CL>()) select_kernel(con
       int acc[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        mma_s8(acc, high[0][c].x, high[1][c].x, high[0][c].y, high[1][c].y, pos[nt][c][0], pos[nt][c][1]);
-        mma_s8(acc, high[0][c].z, high[1][c].z, high[0][c].w, high[1][c].w, pos[nt][c][2], pos[nt][c][3]);
-        mma_s8(acc, low[0][c].x, low[1][c].x, low[0][c].y, low[1][c].y, neg[nt][c][0], neg[nt][c][1]);
-        mma_s8(acc, low[0][c].z, low[1][c].z, low[0][c].w, low[1][c].w, neg[nt][c][2], neg[nt][c][3]);
+        const uint4 qp = kShared ? s_codes[((nt * NC + c) * 2 + 0) * 32 + lane] : make_uint4(pos[nt][c][0], pos[nt][c][1], pos[nt][c][2], pos[nt][c][3]);
+        const uint4 qn = kShared ? s_codes[((nt * NC + c) * 2 + 1) * 32 + lane] : make_uint4(neg[nt][c][0], neg[nt][c][1], neg[nt][c][2], neg[nt][c][3]);
+        mma_s8(acc, high[0][c].x, high[1][c].x, high[0][c].y, high[1][c].y, qp.x, qp.y);
+        mma_s8(acc, high[0][c].z, high[1][c].z, high[0][c].w, high[1][c].w, qp.z, qp.w);
+        mma_s8(acc, low[0][c].x, low[1][c].x, low[0][c].y, low[1][c].y, qn.x, qn.y);
+        mma_s8(acc, low[0][c].z, low[1][c].z, low[0][c].w, low[1][c].w, qn.z, qn.w);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {

@@ -174,6 +174,8 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Make make, Key ke
     uint32_t ca = lane < (int)rank ? cluster_load(&s.cta[0], lane) : 0, cq = lane < (int)rank ? cluster_load(&s.cta[1], lane) : 0;
     a += __reduce_add_sync(~0u, ca);
     q += __reduce_add_sync(~0u, cq);
+    // no CTA leaves while another reads its counts: this one has read those of others
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   }
   each([&](bool there, int i, uint32_t x) {
     const bool is_above = there && x >= from_above, is_equal = there && x >= from_equal && x < from_above;
@@ -192,7 +194,7 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Make make, Key ke
     }
     if (taken) emit(at, i);
   });
-  if (CL > 1) cluster_sync_all();  // no CTA leaves while another reads its counts
+  if (CL > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
 // kernel_setup for a kernel whose blocks form clusters of `cluster`: 16 are more than every GPU takes, and have to be allowed.

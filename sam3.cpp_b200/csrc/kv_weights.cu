@@ -514,15 +514,19 @@ int launch_stream(const KvAttnParams& p, const KvWeights& w, int sms, int* err, 
   return launch_dependent(k, dim3(sms * C::kBlocks), 128, C::kSmem, st, a, err);
 }
 
+// Whether the tiles of 128 rows take the call: they are ahead from where a second one is well filled (us at 64 / 128 / 256 channels,
+// 32 heads over 8000 tokens: 192 rows 65 / 83 / 111 against 50 / 79 / 155, 256 rows 66 / 83 / 111 against 65 / 103 / 203).
+bool many_rows(const KvAttnParams& p) {
+  return p.nq * (long long)(p.heads / p.c.heads) > (p.c.d == 256 ? 128 : p.c.d == 128 ? 192 : 256);
+}
+
 template <int QT, int D>
 int weights_for(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st) {
   const long long rows = p.nq * (long long)(p.heads / p.c.heads);
   if (rows <= 8) return launch_stream<QT, D, 1>(p, w, sms, err, st);
   if (rows <= 16) return launch_stream<QT, D, 2>(p, w, sms, err, st);
   if (D < 256 && rows <= 32) return launch_stream<QT, D, D < 256 ? 4 : 2>(p, w, sms, err, st);
-  // tiles of 128 rows: ahead from where a second one is well filled (us at 64 / 128 / 256 channels, 32 heads over 8000 tokens: 192 rows
-  // 65 / 83 / 111 against 50 / 79 / 155, 256 rows 66 / 83 / 111 against 65 / 103 / 203)
-  if (rows > (D == 256 ? 128 : D == 128 ? 192 : 256)) return kv_weights_tc(p, w, sms, err, st);
+  if (many_rows(p)) return kv_weights_tc(p, w, sms, err, st);
   return launch_sweep<QT, D, 1>(p, w, err, st);
 }
 
@@ -534,7 +538,7 @@ int weights_d(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cuda
 
 }  // namespace
 
-size_t kv_weights_part(int sms) { return kv_weights_tc_part(sms); }
+size_t kv_weights_part(const KvAttnParams& p, int sms) { return many_rows(p) ? kv_weights_tc_part(sms) : 0; }
 
 int kv_weights(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st) {
   return p.c.type == QT_Q4_0 ? weights_d<QT_Q4_0>(p, w, sms, err, st)

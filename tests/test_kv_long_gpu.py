@@ -105,6 +105,32 @@ def test_bounds(s3b, engine, qtype, d, page, heads, lengths):
     assert (bounds.codes[~touched] == 77).all() and (bounds.steps[~touched] == 7).all()
 
 
+def test_values_of_bounds(s3b, engine):
+    """Pages in any order, twice, and outside; none at all; another stream; refusals."""
+    cache = s3b.KVCache(2, 9, 16, 3, 128)
+    bounds = s3b.KVBounds(cache)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    bounds.codes.copy_(torch.randint(-127, 128, bounds.codes.shape, device="cuda", generator=g))
+    bounds.steps.copy_(torch.rand(bounds.steps.shape, device="cuda", generator=g))
+    pages = torch.tensor([8, 0, 3, 3, -1, 9, 1], device="cuda")
+    want = bounds.codes[pages.clamp(0, 8)] * bounds.steps[pages.clamp(0, 8)][..., None, None]
+    want[4:6] = 0
+    assert torch.equal(bounds.values(pages), want) and bounds.values(pages[:0]).shape == (0, 3, 2, 128)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = bounds.values(pages)
+    side.synchronize()
+    assert torch.equal(got, want)
+    with pytest.raises(s3b.S3BError):
+        bounds.values(pages.int())
+    out, L = torch.empty(7, 3, 2, 128, device="cuda"), engine._L
+    assert L.s3b_kv_bounds_values(bounds.ref, pages.data_ptr() + 4, 1, out.data_ptr(), None) == -1
+    assert L.s3b_kv_bounds_values(bounds.ref, pages.data_ptr(), 1, out.data_ptr() + 4, None) == -1
+    assert L.s3b_kv_bounds_values(bounds.ref, pages.data_ptr(), -1, out.data_ptr(), None) == -1
+    assert L.s3b_kv_bounds_values(bounds.ref, None, 1, out.data_ptr(), None) == -1 and L.s3b_kv_bounds_values(None, None, 0, None, None) == -1
+
+
 @pytest.mark.parametrize("new", [1, 2, 16, 17, 33, 500, 0])
 def test_bounds_of_the_newest_tokens(s3b, engine, new):
     """Only the pages that hold the last `new` tokens are written, each over all of its tokens."""

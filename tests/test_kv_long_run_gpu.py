@@ -327,34 +327,35 @@ def raw(s3b, engine):
     """The C calls over one small cache, arguments by name."""
     w = _world(s3b, engine, n=300)
     o = _outs(w, 4, 50)
-    L, h, P = engine._L, engine.h, ctypes.c_void_p
-    kv, d, max_pages = 2, 64, w["pages"].shape[1]
+    L, h = engine._L, engine.h
+    d, max_pages = 64, w["pages"].shape[1]
 
     def at(t, off=0):
-        return P(t.data_ptr() + off) if t is not None else None
+        return t.data_ptr() + off if t is not None else 0
+
+    def the_call(pages=w["pages"], stride=max_pages, width=max_pages, lengths=w["lengths"], batch=1, q=w["q"], q_h=d, out=o["out"], lse=o["lse"], sel=o["selected"],
+                 keep=4, share=1, nq=3, heads=4, scale=0.1, causal=0, window=0, pages_off=0, q_off=0, out_off=0, lse_off=0):
+        return s3b._CALL.pack(at(pages, pages_off), stride, at(lengths), at(q, q_off), 12 * d, 4 * d, q_h, at(out, out_off), 12 * d, 4 * d, d, at(lse, lse_off), at(sel),
+                              width, batch, nq, heads, causal, window, keep, share, 0, scale)
 
     class Calls:
-        def bounds(self, pages=w["pages"], stride=max_pages, width=max_pages, lengths=w["lengths"], batch=1, recent=5, desc=None, off=0):
-            return L.s3b_op_cache_bounds(h, w["cache"].ref, ctypes.byref(desc) if desc else w["bounds"].ref, at(pages, off), stride, width, at(lengths), batch, recent)
+        def bounds(self, recent=5, desc=None, off=0, **kw):
+            return L.s3b_op_cache_bounds(h, w["cache"].ref, ctypes.byref(desc) if desc else w["bounds"].ref, the_call(pages_off=off, **kw), recent)
 
-        def select(self, q=w["q"], q_h=d, sel=o["selected"], keep=4, share=1, sink=0, recent=0, scores=None, stride=max_pages, width=max_pages, batch=1, nq=3, heads=4,
-                   causal=0, window=0, off=0, desc=None):
-            return L.s3b_op_cache_select(h, ctypes.byref(desc) if desc else w["bounds"].ref, at(q, off), 12 * d, 4 * d, q_h, at(sel), keep, share, sink, recent, at(scores), at(w["pages"]), stride,
-                                         width, at(w["lengths"]), batch, nq, heads, causal, window)
+        def select(self, sink=0, recent=0, scores=None, off=0, desc=None, **kw):
+            return L.s3b_op_cache_select(h, ctypes.byref(desc) if desc else w["bounds"].ref, the_call(q_off=off, **kw), sink, recent, at(scores) or None)
 
-        def attend(self, q=w["q"], out=o["out"], sel=o["selected"], keep=4, share=1, width=max_pages, batch=1, nq=3, heads=4, scale=0.1, causal=0, window=0, off=0):
-            return L.s3b_op_cache_attention_selected(h, w["cache"].ref, at(q), 12 * d, 4 * d, d, at(out, off), 0, 12 * d, 4 * d, d, None, at(sel), keep, share, at(w["pages"]), max_pages,
-                                                     width, at(w["lengths"]), batch, nq, heads, scale, causal, window)
+        def attend(self, off=0, **kw):
+            return L.s3b_op_cache_attention_selected(h, w["cache"].ref, the_call(out_off=off, **kw))
 
-        def weights(self, q=w["q"], lse=o["lse"], wt=o["weights"], w_b=2 * 16 * max_pages, w_h=16 * max_pages, decay=1.0, batch=1, nq=3, heads=4, scale=0.1, causal=0, window=0,
-                    off=0):
-            return L.s3b_op_cache_weights(h, w["cache"].ref, at(q), 12 * d, 4 * d, d, at(lse), at(wt, off), w_b, w_h, decay, at(w["pages"]), max_pages, max_pages, at(w["lengths"]), batch,
-                                          nq, heads, scale, causal, window)
+        def weights(self, wt=o["weights"], w_b=2 * 16 * max_pages, w_h=16 * max_pages, decay=1.0, off=0, **kw):
+            return L.s3b_op_cache_weights(h, w["cache"].ref, the_call(**kw), at(wt, off) or None, w_b, w_h, decay)
 
         def evict(self, to=None, wt=o["weights"], keep=50, sink=0, recent=0, pages_out=w["pages_out"], stride=max_pages, lengths_out=o["lengths_out"], kept=o["kept"],
-                  weights_out=o["weights_out"], batch=1, off=0):
-            return L.s3b_op_cache_evict(h, w["cache"].ref, ctypes.byref(to) if to else None, at(wt), 0, 16 * max_pages, at(w["pages"]), max_pages, max_pages, at(w["lengths"]), batch, keep,
-                                        sink, recent, at(pages_out), stride, at(lengths_out), at(kept, off), at(weights_out))
+                  weights_out=o["weights_out"], off=0, **kw):
+            e = s3b._EVICT.pack(ctypes.addressof(to) if to else 0, at(wt), 0, 16 * max_pages, at(pages_out), stride, at(lengths_out), at(kept, off), at(weights_out), keep,
+                                sink, recent)
+            return L.s3b_op_cache_evict(h, w["cache"].ref, the_call(**kw), e)
     c = Calls()
     c.w, c.o, c.max_pages = w, o, max_pages
     yield c
@@ -385,6 +386,13 @@ def test_raw_calls_pass(raw, engine):
     ("evict", dict(sink=30, recent=21), -1), ("evict", dict(sink=-1), -1), ("evict", dict(off=2), -1), ("evict", dict(batch=2, stride=3), -1)])
 def test_refusals(raw, call, args, code):
     assert getattr(raw, call)(**args) == code
+
+
+def test_refuses_no_call(engine, raw):
+    w, L, h = raw.w, engine._L, engine.h
+    assert L.s3b_op_cache_bounds(h, w["cache"].ref, w["bounds"].ref, None, 1) == -1 and L.s3b_op_cache_select(h, w["bounds"].ref, None, 0, 0, None) == -1
+    assert L.s3b_op_cache_attention_selected(h, w["cache"].ref, None) == -1 and L.s3b_op_cache_weights(h, w["cache"].ref, None, raw.o["weights"].data_ptr(), 0, 304, 1.0) == -1
+    assert L.s3b_op_cache_evict(h, w["cache"].ref, None, None) == -1
 
 
 def test_refuses_other_shapes(s3b, raw):
