@@ -41,13 +41,14 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const __grid_constant_
   const int first = (int)min((long long)rank * share, (long long)len), n = min(share, len - first);
   const int sink = a.e.sink, from = len - a.e.recent;
   weights += first;
-  auto key = [&](int i) { return first + i < sink || first + i >= from ? kTopForced : top_key(weights[i]); };
+  auto fetch = [&](int i) { return weights[i]; };
+  auto make = [&](int i, float w) { return first + i < sink || first + i >= from ? kTopForced : top_key(w); };
   auto emit = [&](uint32_t at, int i) { kept[at] = first + i; };
   if (share <= a.keys) {
     top_select<kThreads, CL>(
-        s_top, n, (uint32_t)keep, [&](int i) { return s_keys[i] = key(i); }, [&](int i) { return s_keys[i]; }, emit);
+        s_top, n, (uint32_t)keep, fetch, [&](int i, float w) { return s_keys[i] = make(i, w); }, [&](int i) { return s_keys[i]; }, emit);
   } else {
-    top_select<kThreads, CL>(s_top, n, (uint32_t)keep, key, key, emit);
+    top_select<kThreads, CL>(s_top, n, (uint32_t)keep, fetch, make, [&](int i) { return make(i, weights[i]); }, emit);
   }
 }
 

@@ -218,10 +218,11 @@ __global__ void __launch_bounds__(select_threads<D, NT, CL>(), CL == 1 ? 2 : 1) 
   auto emit = [&](uint32_t at, int i) { selected[at] = begin + i; };
   if (in_smem) {
     auto key = [&](int i) { return s_keys[i]; };
-    top_select<kThreads, CL>(s_top, end - begin, (uint32_t)p.keep, key, key, emit);
+    top_select<kThreads, CL>(s_top, end - begin, (uint32_t)p.keep, key, [](int, uint32_t x) { return x; }, key, emit);
   } else {
-    auto key = [&](int i) { return begin + i < sink || begin + i >= recent ? kTopForced : top_key(scores[begin + i]); };
-    top_select<kThreads, CL>(s_top, end - begin, (uint32_t)p.keep, key, key, emit);
+    auto fetch = [&](int i) { return scores[begin + i]; };
+    auto make = [&](int i, float x) { return begin + i < sink || begin + i >= recent ? kTopForced : top_key(x); };
+    top_select<kThreads, CL>(s_top, end - begin, (uint32_t)p.keep, fetch, make, [&](int i) { return make(i, scores[begin + i]); }, emit);
   }
 }
 

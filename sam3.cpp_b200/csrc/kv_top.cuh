@@ -32,13 +32,14 @@ struct TopShared {
 
 // Radix selection from the top, 8 bits a round: the digit in which the k-th largest lies, then the same among the keys that
 // share it; it ends with the round in which all of those are taken. Each of a cluster's CL CTAs has n places of a line, one CTA's
-// behind another's; within a CTA each warp has a run of rows of 32. make(i) gives the key of its place i in the first round,
-// key(i) after that: from shared memory where they fit. emit(position, place) is called for the taken ones, k of them in all
-// (0 < k <= the line's length, and at least the number of forced keys).
+// behind another's; within a CTA each warp has a run of rows of 32. In the first round make(i, fetch(i)) gives the key of its place
+// i (all of a step's fetches come before its makes, which may write: 18000 cycles otherwise, 128 KB at one load's latency after
+// the other's), key(i) after that: from shared memory where they fit. emit(position, place) is called for the taken ones, k of
+// them in all (0 < k <= the line's length, and at least the number of forced keys).
 // Measured (cycles of the SM): 32768 keys a CTA of 1024 threads, 16 of them: a round 4700 to 7000 to count (the atomics on shared
 // memory), 500 to add up, 4000 for the cluster to meet and find the digit. 256 keys, 256 threads: see the branch for few keys.
-template <int T, int CL, typename Make, typename Key, typename Emit>
-__device__ void top_select(TopShared<T>& s, int n, uint32_t k, Make make, Key key, Emit emit) {
+template <int T, int CL, typename Fetch, typename Make, typename Key, typename Emit>
+__device__ void top_select(TopShared<T>& s, int n, uint32_t k, Fetch fetch, Make make, Key key, Emit emit) {
   constexpr int W = T / 32, C = TopShared<T>::kCopies, P = T / 256;  // P threads a digit
   static_assert(T >= 256 && T % 256 == 0 && C % P == 0, "threads of top_select");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -48,11 +49,11 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Make make, Key ke
   auto each_of = [&](auto&& of, auto unroll, auto&& f) {
     constexpr int U = decltype(unroll)::value;
     for (int i0 = from; i0 < to; i0 += 32 * U) {
-      uint32_t x[U];
+      decltype(of(0)) x[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = i0 + 32 * u + lane;
-        x[u] = i < to ? of(i) : 0u;
+        x[u] = i < to ? of(i) : decltype(of(0))(0);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -67,7 +68,7 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Make make, Key ke
     // before the last bit: 256 keys in 1000 cycles where two rounds below take 2500).
     const int i = from + lane;  // a run is one row
     const bool there = from < to && i < to;
-    const uint32_t x = there ? make(i) : 0u;
+    const uint32_t x = there ? make(i, fetch(i)) : 0u;
     uint32_t count = 0;
     from_equal = 0;
     for (int bit = 31; bit >= 0 && count != k; --bit) {
@@ -90,8 +91,8 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Make make, Key ke
       const int shift = 24 - 8 * round;
       __syncthreads();
       if (round == 0) {
-        each_of(make, std::integral_constant<int, 8>(), [&](bool there, int, uint32_t x) {
-          if (there) atomicAdd(&s.hist[(x >> 24) * C + lane % C], 1u);
+        each_of(fetch, std::integral_constant<int, 8>(), [&](bool there, int i, decltype(fetch(0)) v) {
+          if (there) atomicAdd(&s.hist[(make(i, v) >> 24) * C + lane % C], 1u);
         });
       } else {
         each([&](bool there, int, uint32_t x) {
