@@ -174,14 +174,17 @@ EvictKernel choose_for(int cl) {
 int kv_evict(const KvAttnParams& p, const KvEvict& e, int* err, cudaStream_t st) {
   const long long units = (long long)p.batch * p.c.heads, moves = (units * ((e.keep + 15) / 16) + 3) / 4;
   if (units > 0x7fffffffLL / 8 || moves > 0x7fffffffLL) return -2;
-  // CTAs of a unit: 4096 tokens each or more, as far as there are SMs for them and clusters go
+  // CTAs of a unit: 4096 tokens each or more, as far as there are SMs for them. Of clusters of 16, each in a GPC of its own, few run at
+  // a time: they are taken for half of the SMs (8 heads of 65536 tokens: 18.2 us in clusters of 16, 12.7 of 8; 4 heads 14.6, 18.2).
   const long long tokens = (long long)p.max_pages * p.c.page_size;
+  const int sms = num_sms();
   int cl = 1;
-  while (cl < 16 && (long long)cl * 4096 < tokens && units * cl * 2 <= num_sms()) cl *= 2;
+  while (cl < 16 && cl * 4096LL < tokens && units * cl * 2 <= (cl == 8 ? sms / 2 : sms)) cl *= 2;
+  EvictKernel choose = choose_for(cl);
+  if (cl == 16 && cluster_setup(choose, kMostKeys * 4, kThreads, cl) <= 0) choose = choose_for(cl = 8);
+  if (cluster_setup(choose, kMostKeys * 4, kThreads, cl) <= 0) return -13;
   const long long share = cl > 1 ? (tokens + 32 * cl - 1) / (32 * cl) * 32 : tokens;
   const EvictArgs a{p, e, (int)std::min<long long>(share, kMostKeys)};
-  const EvictKernel choose = choose_for(cl);
-  if (cluster_setup(choose, kMostKeys * 4, cl) <= 0) return -13;
   int rc = launch_clusters(choose, (unsigned)units * cl, kThreads, (size_t)a.keys * 4, cl, st, a, err);
   if (rc || e.keep == 0) return rc;
   const EvictKernel k = p.c.type == QT_Q4_0 ? move_for<QT_Q4_0>(p.c.d)

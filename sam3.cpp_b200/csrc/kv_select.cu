@@ -243,29 +243,44 @@ SelectKernel select_for(int d, int rows) {
   return d == 64 ? select_rows<64, CL>(rows) : d == 128 ? select_rows<128, CL>(rows) : select_rows<256, CL>(rows);
 }
 
-// CTAs of a unit: about 512 pages each (two steps of 16 for each warp), as far as there are SMs for them and clusters go
-int select_cluster(const KvAttnParams& p, int sms) {
+struct SelectPlan {
+  SelectKernel k;
+  int cl;           // CTAs of a unit
+  long long share;  // pages of the largest share of a CTA
+};
+// CTAs of a unit: about 512 pages each (two steps of 16 for each warp), on half of the SMs: large clusters find no place on all of
+// them (8 lists of 8192 pages: 24.2 us in clusters of 16, 14.4 of 8; 16 lists of 16384: 32.5 of 8, 25.8 of 4).
+bool select_plan(const KvAttnParams& p, int sms, SelectPlan* plan) {
+  const int rows = p.share * (p.heads / p.c.heads), d = p.c.d;
   int cl = 1;
-  while (cl < 16 && (long long)cl * 512 < p.max_pages && kv_attention_units(p) * cl * 2 <= sms) cl *= 2;
-  return cl;
+  while (cl < 16 && cl * 512LL < p.max_pages && kv_attention_units(p) * cl * 4 <= sms) cl *= 2;
+  auto of = [&](int n) {
+    return n == 1 ? select_for<1>(d, rows) : n == 2 ? select_for<2>(d, rows) : n == 4 ? select_for<4>(d, rows)
+           : n == 8 ? select_for<8>(d, rows) : select_for<16>(d, rows);
+  };
+  plan->k = of(cl);
+  if (cl == 16 && cluster_setup(plan->k.kernel, kMostKeys * 4, plan->k.threads, cl) <= 0) plan->k = of(cl = 8);
+  plan->cl = cl;
+  plan->share = cl > 1 ? ((p.max_pages + cl - 1LL) / cl + 31) / 32 * 32 : p.max_pages;
+  return cluster_setup(plan->k.kernel, kMostKeys * 4, plan->k.threads, cl) > 0;
 }
-// pages of the largest share of a CTA
-long long select_share(const KvAttnParams& p, int cl) { return cl > 1 ? ((p.max_pages + cl - 1LL) / cl + 31) / 32 * 32 : p.max_pages; }
 
 }  // namespace
 
-bool kv_select_needs_scores(const KvAttnParams& p, int sms) { return select_share(p, select_cluster(p, sms)) > kMostKeys; }
+bool kv_select_needs_scores(const KvAttnParams& p, int sms) {
+  if (p.max_pages <= kMostKeys) return false;
+  SelectPlan plan;
+  return !select_plan(p, sms, &plan) || plan.share > kMostKeys;
+}
 
 int kv_select(const KvAttnParams& p, const KvBounds& bounds, int sink, int recent, float* scores, bool all, int* selected, int sms,
               int* err, cudaStream_t st) {
-  const int cl = select_cluster(p, sms);
-  const long long share = select_share(p, cl), grid = kv_attention_units(p) * cl;
+  SelectPlan plan;
+  if (!select_plan(p, sms, &plan)) return -13;
+  const long long grid = kv_attention_units(p) * plan.cl;
   if (grid > 0x7fffffffLL) return -2;
-  const SelectArgs a{p, bounds, sink, recent, scores, all, selected, (int)std::min<long long>(share, kMostKeys)};
-  const int rows = p.share * (p.heads / p.c.heads), d = p.c.d;
-  const SelectKernel k = cl == 1 ? select_for<1>(d, rows) : cl == 2 ? select_for<2>(d, rows) : cl == 4 ? select_for<4>(d, rows) : cl == 8 ? select_for<8>(d, rows) : select_for<16>(d, rows);
-  if (cluster_setup(k.kernel, kMostKeys * 4, cl) <= 0) return -13;
-  return launch_clusters(k.kernel, (unsigned)grid, k.threads, (size_t)a.keys * 4, cl, st, a, err);
+  const SelectArgs a{p, bounds, sink, recent, scores, all, selected, (int)std::min<long long>(plan.share, kMostKeys)};
+  return launch_clusters(plan.k.kernel, (unsigned)grid, plan.k.threads, (size_t)a.keys * 4, plan.cl, st, a, err);
 }
 
 }  // namespace s3b

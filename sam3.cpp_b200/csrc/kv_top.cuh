@@ -198,13 +198,29 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Fetch fetch, Make
   if (CL > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
-// kernel_setup for a kernel whose blocks form clusters of `cluster`: 16 are more than every GPU takes, and have to be allowed.
-inline int allow_wide_cluster(const void* kernel, size_t, int) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess ? 1 : -13;
+// kernel_setup for a kernel whose blocks form clusters of `cluster`. 16 are more than every GPU takes: they have to be allowed, and
+// where none finds its place the set-up fails (and a smaller cluster is taken).
+inline int wide_clusters(const void* kernel, size_t smem, int threads) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 16;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(16);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0)
+    return n;
+  cudaGetLastError();
+  return -13;
 }
 template <typename K>
-int cluster_setup(K* kernel, size_t smem, int cluster) {
-  return kernel_setup(reinterpret_cast<const void*>(kernel), smem, cluster > 8 ? allow_wide_cluster : nullptr, 0);
+int cluster_setup(K* kernel, size_t smem, int threads, int cluster) {
+  return kernel_setup(reinterpret_cast<const void*>(kernel), smem, cluster > 8 ? wide_clusters : nullptr, threads);
 }
 
 // Launch of such a kernel, which may take its place while its predecessor runs.
