@@ -71,9 +71,47 @@ __global__ void __launch_bounds__(select_threads<D, NT, CL>(), CL == 1 ? 2 : 1) 
     for (int j = rank * kThreads + threadIdx.x; j < p.max_pages; j += CL * kThreads)
       if (j < pa || j >= pe) scores[j] = -INFINITY;
 
+  // ---- bounds of 16 pages a warp; those of the first step are on their way while the queries are made into codes
+  constexpr int kPass = 16 * (kThreads / 32);
+  const int* table = p.pages + b * p.pages_stride;
+  auto page_of = [&](int j) -> long long {
+    if (j >= end) return 0;
+    const long long page = table[j];
+    if (page >= 0 && page < p.c.n_pages) return page;
+    atomicCAS(err, 0, kDevErrIndex);
+    return 0;
+  };
+  const int sink = pa + a.sink, recent = pe - a.recent;
+  uint4 low[2][NC], high[2][NC];
+  float page_step[2];
+  long long next[2];  // pages of the step after
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int j = j0 + g + 8 * u;
+      page_step[u] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) low[u][c] = high[u][c] = make_uint4(0, 0, 0, 0);
+      if (j < end) {
+        const long long row = next[u] * p.c.heads + head;
+        const int8_t* at = a.bounds.codes + row * 2 * D + 16 * t;
+        page_step[u] = a.bounds.steps[row];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          low[u][c] = *reinterpret_cast<const uint4*>(at + 64 * c);
+          high[u][c] = *reinterpret_cast<const uint4*>(at + D + 64 * c);
+        }
+      }
+      next[u] = page_of(j + kPass);
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < 2; ++u) next[u] = page_of(begin + 16 * warp + g + 8 * u);
+  load(begin + 16 * warp);
+
   // ---- the query rows' codes, of either sign apart: column g of tile nt is row 8 nt + g. Where they would take too many registers
   // they stay in shared memory, and the warps share the work of making them.
-  constexpr bool kShared = NT * D >= 512;
+  constexpr bool kShared = D == 256 || NT * D >= 512;
   __shared__ uint4 s_codes[kShared ? NT * NC * 32 * 2 : 1];  // [tile][64 channels][positive, negative][lane]
   __shared__ float s_step[NT * 8];
   uint32_t pos[NT][NC][4], neg[NT][NC][4];
@@ -149,40 +187,7 @@ __global__ void __launch_bounds__(select_threads<D, NT, CL>(), CL == 1 ? 2 : 1) 
   }
 
   // ---- scores of 16 pages at a time
-  const int* table = p.pages + b * p.pages_stride;
-  const int sink = pa + a.sink, recent = pe - a.recent;
-  auto page_of = [&](int j) -> long long {
-    if (j >= end) return 0;
-    const long long page = table[j];
-    if (page >= 0 && page < p.c.n_pages) return page;
-    atomicCAS(err, 0, kDevErrIndex);
-    return 0;
-  };
-  long long next[2];  // pages of the step after, on their way while this one's bounds are
-#pragma unroll
-  for (int u = 0; u < 2; ++u) next[u] = page_of(begin + 16 * warp + g + 8 * u);
-  for (int j0 = begin + 16 * warp; j0 < end; j0 += 16 * (kThreads / 32)) {
-    uint4 low[2][NC], high[2][NC];
-    float page_step[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int j = j0 + g + 8 * u;
-      page_step[u] = 0.f;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) low[u][c] = high[u][c] = make_uint4(0, 0, 0, 0);
-      if (j < end) {
-        const long long row = next[u] * p.c.heads + head;
-        const int8_t* at = a.bounds.codes + row * 2 * D + 16 * t;
-        page_step[u] = a.bounds.steps[row];
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          low[u][c] = *reinterpret_cast<const uint4*>(at + 64 * c);
-          high[u][c] = *reinterpret_cast<const uint4*>(at + D + 64 * c);
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) next[u] = page_of(j0 + 16 * (kThreads / 32) + g + 8 * u);
+  for (int j0 = begin + 16 * warp; j0 < end; j0 += kPass) {
     float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -212,6 +217,7 @@ __global__ void __launch_bounds__(select_threads<D, NT, CL>(), CL == 1 ? 2 : 1) 
         if (a.all || !in_smem) scores[j] = best[u];
       }
     }
+    load(j0 + kPass);
   }
   if (trivial) return;
   __syncthreads();

@@ -63,24 +63,28 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Fetch fetch, Make
   auto each = [&](auto&& f) { each_of(key, std::integral_constant<int, 4>(), f); };
   uint32_t left = k;
   uint32_t from_above = 1, from_equal = 0;  // keys >= from_above are taken, then the first of those >= from_equal
-  if (CL == 1 && n <= T) {
-    // Few keys, one a thread: the threshold bit by bit, by the block's votes (some 50 cycles each, and most searches end well
+  if (CL == 1 && n <= 2 * T) {
+    // Few keys, one or two a thread: the threshold bit by bit, by the block's votes (some 50 cycles each, and most searches end well
     // before the last bit: 256 keys in 1000 cycles where two rounds below take 2500).
-    const int i = from + lane;  // a run is one row
-    const bool there = from < to && i < to;
-    const uint32_t x = there ? make(i, fetch(i)) : 0u;
+    const bool two = n > T;  // a run is one row, or two
+    const int i = from + lane, i2 = i + 32;
+    const bool there = i < to, there2 = i2 < to;
+    const uint32_t x = there ? make(i, fetch(i)) : 0u, x2 = there2 ? make(i2, fetch(i2)) : 0u;
+    auto votes = [&](uint32_t at) {
+      uint32_t c = __syncthreads_count(there && x >= at);
+      if (two) c += __syncthreads_count(there2 && x2 >= at);
+      return c;
+    };
     uint32_t count = 0;
-    from_equal = 0;
     for (int bit = 31; bit >= 0 && count != k; --bit) {
-      const uint32_t at = from_equal | 1u << bit;
-      const uint32_t c = __syncthreads_count(there && x >= at);
+      const uint32_t at = from_equal | 1u << bit, c = votes(at);
       if (c >= k) from_equal = at, count = c;
     }
     from_above = from_equal;
     left = 0;
     if (count != k) {  // equal ones are left out (no forced key is: they are at most k)
       from_above = from_equal + 1;
-      left = k - __syncthreads_count(there && x >= from_above);
+      left = k - votes(from_above);
     }
   } else {
 #pragma unroll
