@@ -27,27 +27,25 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 warps in clusters (long lines of pages), unless the codes of many rows or channels take the registers; 8 otherwise, so that
-// several lists' CTAs share an SM (32 x 8 lists of 256 pages: 11.5 us, with 16 warps 14.8)
-template <int D, int NT, int CL>
-__host__ __device__ constexpr int select_threads() { return CL == 1 || NT * D > 256 || D == 256 ? 256 : 512; }
-
 // A unit is a block of queries and a key / value head, of one CTA or a cluster of them (CL) that share its pages and then choose
 // together (kv_top.cuh). Whole numbers carry the score: sum over channels of max(c low, c high) = c+ high + c- low with
 // c+ = max(c, 0), c- = min(c, 0), two products of 8-bit codes (16 pages x 32 channels x 8 rows an instruction), exact in 32 bits;
 // then two f32 products, each rounded, so that the choice is the same whatever the order. Lane (g, t) holds 16 channels of 64 as
-// the contraction's share of its rows (pages g, g + 8; query row g): whole 16-byte words of both.
-template <int D, int NT, int CL>
-__global__ void __launch_bounds__(select_threads<D, NT, CL>(), CL == 1 ? 2 : 1) select_kernel(const __grid_constant__ SelectArgs a, int* err) {
-  constexpr int NC = D / 64, kThreads = select_threads<D, NT, CL>();
+// the contraction's share of its rows (pages g, g + 8; query row g): whole 16-byte words of both. 16 warps where there is a CTA or
+// less for each SM, else 8, so that several share one (32 x 8 lists of 256 pages: 14.8 us with 16, 11.5 with 8).
+template <int D, int NT, int CL, int kThreads>
+__global__ void __launch_bounds__(kThreads, 512 / kThreads) select_kernel(const __grid_constant__ SelectArgs a, int* err) {
+  constexpr int NC = D / 64;
   extern __shared__ uint32_t s_keys[];
   __shared__ TopShared<kThreads> s_top;
+  __shared__ uint4 s_codes[NT * NC * 2 * 32];  // [tile][64 channels][positive, negative][lane]
+  __shared__ float s_step[NT * 8];
   const KvAttnParams& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const long long unit = blockIdx.x / CL;
+  const int unit = blockIdx.x / CL;
   const int blocks = (p.nq - 1) / p.share + 1;
-  const int head = (int)(unit % p.c.heads), b = (int)(unit / p.c.heads / blocks);
-  const int i0 = (int)(unit / p.c.heads % blocks) * p.share, i1 = min(i0 + p.share, p.nq);
+  const int head = unit % p.c.heads, b = unit / p.c.heads / blocks;
+  const int i0 = unit / p.c.heads % blocks * p.share, i1 = min(i0 + p.share, p.nq);
   const int group_heads = p.heads / p.c.heads, n_rows = (i1 - i0) * group_heads;
   let_next();
   wait_before();
@@ -55,14 +53,14 @@ __global__ void __launch_bounds__(select_threads<D, NT, CL>(), CL == 1 ? 2 : 1) 
   int lo, hi, none;
   row_span(p, len, i0, &lo, &none);
   row_span(p, len, i1 - 1, &none, &hi);
-  const int pa = lo / p.c.page_size, pe = max(pa, (int)((hi + (long long)p.c.page_size - 1) / p.c.page_size));
+  const int pa = lo / p.c.page_size, pe = max(pa, hi > 0 ? (hi - 1) / p.c.page_size + 1 : 0);
   const int n = pe - pa;
   // this CTA's pages
   const int rank = CL > 1 ? blockIdx.x % CL : 0;
   const int share = CL > 1 ? ((n + CL - 1) / CL + 31) / 32 * 32 : n;
   const int begin = pa + (int)min((long long)n, (long long)rank * share), end = min(pe, begin + share);
-  int* selected = a.selected + unit * p.keep;
-  float* scores = a.scores + unit * p.max_pages;
+  int* selected = a.selected + (long long)unit * p.keep;
+  float* scores = a.scores + (long long)unit * p.max_pages;
   const bool trivial = n <= p.keep, in_smem = share <= a.keys;
   if (trivial && rank == 0)
     for (int e = threadIdx.x; e < p.keep; e += kThreads) selected[e] = e < n ? pa + e : -1;
@@ -109,81 +107,56 @@ __global__ void __launch_bounds__(select_threads<D, NT, CL>(), CL == 1 ? 2 : 1) 
   for (int u = 0; u < 2; ++u) next[u] = page_of(begin + 16 * warp + g + 8 * u);
   load(begin + 16 * warp);
 
-  // ---- the query rows' codes, of either sign apart: column g of tile nt is row 8 nt + g. Where they would take too many registers
-  // they stay in shared memory, and the warps share the work of making them.
-  constexpr bool kShared = D == 256 || NT * D >= 512;
-  __shared__ uint4 s_codes[kShared ? NT * NC * 32 * 2 : 1];  // [tile][64 channels][positive, negative][lane]
-  __shared__ float s_step[NT * 8];
-  uint32_t pos[NT][NC][4], neg[NT][NC][4];
-  float step[NT][2];  // of columns 2t, 2t + 1; < 0: no such row
+  // ---- the query rows' codes, of either sign apart, a warp a row: D / 32 neighbouring channels a lane
+  constexpr int V = D / 32, kWarps = kThreads / 32;
+  for (int r = warp; r < 8 * NT; r += kWarps) {
+    uint32_t w[V / 2], top = 0;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    if (kShared && nt != warp) continue;  // a warp a tile
-    const int r = 8 * nt + g;
-    const int i = i0 + r / group_heads, h = head * group_heads + r % group_heads;
-    const __half* q = p.q + b * p.q_b + i * p.q_n + h * p.q_h + 16 * t;
-    uint32_t raw[NC][8];
-    uint32_t top = 0;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-      if (r < n_rows) {
-        v[0] = *reinterpret_cast<const uint4*>(q + 64 * c);
-        v[1] = *reinterpret_cast<const uint4*>(q + 64 * c + 8);
-      }
-      const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        // a NaN counts as 0, infinities as f16's largest
-        __half2 x = u32_h2(w[e]);
-        x = __hmin2(__hmax2(x, u32_h2(0xFBFFFBFFu)), u32_h2(0x7BFF7BFFu));
-        uint32_t y = h2_u32(x);
-        if ((w[e] & 0x7FFFu) > 0x7C00u) y &= 0xFFFF0000u;
-        if ((w[e] & 0x7FFF0000u) > 0x7C000000u) y &= 0x0000FFFFu;
-        raw[c][e] = y;
-        top = max(top, max(y & 0x7FFFu, y >> 16 & 0x7FFFu));
-      }
+    for (int e = 0; e < V / 2; ++e) w[e] = 0;
+    if (r < n_rows) {
+      const int i = i0 + r / group_heads, h = head * group_heads + r % group_heads;
+      lds<V * 2>(reinterpret_cast<const uint8_t*>(p.q + b * p.q_b + i * p.q_n + h * p.q_h + V * lane), w);
     }
-    top = max(top, __shfl_xor_sync(~0u, top, 1));
-    top = max(top, __shfl_xor_sync(~0u, top, 2));
-    const float peak = __half2float(__ushort_as_half((unsigned short)top));
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) {
+      // a NaN counts as 0, infinities as f16's largest
+      uint32_t y = h2_u32(__hmin2(__hmax2(u32_h2(w[e]), u32_h2(0xFBFFFBFFu)), u32_h2(0x7BFF7BFFu)));
+      if ((w[e] & 0x7FFFu) > 0x7C00u) y &= 0xFFFF0000u;
+      if ((w[e] & 0x7FFF0000u) > 0x7C000000u) y &= 0x0000FFFFu;
+      w[e] = y;
+      top = max(top, max(y & 0x7FFFu, y >> 16 & 0x7FFFu));
+    }
+    const float peak = __half2float(__ushort_as_half((unsigned short)__reduce_max_sync(~0u, top)));
     const float inv = peak != 0.f ? __fdiv_rn(127.f, peak) : 0.f;
-    const float mine = r < n_rows ? __fdiv_rn(peak, 127.f) : -1.f;
-    if (kShared) {
-      if (t == 0) s_step[r] = mine;
-    } else {
-      step[nt][0] = __shfl_sync(~0u, mine, 8 * t);
-      step[nt][1] = __shfl_sync(~0u, mine, 8 * t + 4);
+    if (lane == 0) s_step[r] = r < n_rows ? __fdiv_rn(peak, 127.f) : -1.f;  // < 0: no such row
+    unsigned long long wp = 0, wn = 0;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float2 x = __half22float2(u32_h2(w[e / 2]));
+      const int code = max(-127, min(127, __float2int_rn(__fmul_rn(e & 1 ? x.y : x.x, inv))));
+      wp |= (unsigned long long)max(code, 0) << (8 * e);
+      wn |= (unsigned long long)(min(code, 0) & 255) << (8 * e);
     }
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      uint32_t wp[4], wn[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 x0 = __half22float2(u32_h2(raw[c][2 * e])), x1 = __half22float2(u32_h2(raw[c][2 * e + 1]));
-        const float x[4] = {x0.x, x0.y, x1.x, x1.y};
-        wp[e] = wn[e] = 0;
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          const int code = max(-127, min(127, __float2int_rn(__fmul_rn(x[f], inv))));
-          wp[e] |= (uint32_t)max(code, 0) << (8 * f);
-          wn[e] |= (uint32_t)(min(code, 0) & 255) << (8 * f);
-        }
-        if (!kShared) pos[nt][c][e] = wp[e], neg[nt][c][e] = wn[e];
-      }
-      if (kShared) {
-        s_codes[((nt * NC + c) * 2 + 0) * 32 + lane] = make_uint4(wp[0], wp[1], wp[2], wp[3]);
-        s_codes[((nt * NC + c) * 2 + 1) * 32 + lane] = make_uint4(wn[0], wn[1], wn[2], wn[3]);
-      }
+    // lane (r % 8, t) of tile r / 8 takes the channels 16 t .. 16 t + 15 of each 64
+    const int ch = V * lane;
+    uint8_t* at = reinterpret_cast<uint8_t*>(s_codes) + (((r >> 3) * NC + ch / 64) * 64 + (r & 7) * 4 + ch % 64 / 16) * 16 + ch % 16;
+    if (V == 2) {
+      *reinterpret_cast<uint16_t*>(at) = (uint16_t)wp;
+      *reinterpret_cast<uint16_t*>(at + 512) = (uint16_t)wn;
+    } else if (V == 4) {
+      *reinterpret_cast<uint32_t*>(at) = (uint32_t)wp;
+      *reinterpret_cast<uint32_t*>(at + 512) = (uint32_t)wn;
+    } else {
+      *reinterpret_cast<unsigned long long*>(at) = wp;
+      *reinterpret_cast<unsigned long long*>(at + 512) = wn;
     }
   }
-  if (kShared) {
-    __syncthreads();
+  __syncthreads();
+  float step[NT][2];  // of rows 2t, 2t + 1 of a tile
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      step[nt][0] = s_step[8 * nt + 2 * t];
-      step[nt][1] = s_step[8 * nt + 2 * t + 1];
-    }
+  for (int nt = 0; nt < NT; ++nt) {
+    step[nt][0] = s_step[8 * nt + 2 * t];
+    step[nt][1] = s_step[8 * nt + 2 * t + 1];
   }
 
   // ---- scores of 16 pages at a time
@@ -194,8 +167,7 @@ __global__ void __launch_bounds__(select_threads<D, NT, CL>(), CL == 1 ? 2 : 1) 
       int acc[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const uint4 qp = kShared ? s_codes[((nt * NC + c) * 2 + 0) * 32 + lane] : make_uint4(pos[nt][c][0], pos[nt][c][1], pos[nt][c][2], pos[nt][c][3]);
-        const uint4 qn = kShared ? s_codes[((nt * NC + c) * 2 + 1) * 32 + lane] : make_uint4(neg[nt][c][0], neg[nt][c][1], neg[nt][c][2], neg[nt][c][3]);
+        const uint4 qp = s_codes[((nt * NC + c) * 2 + 0) * 32 + lane], qn = s_codes[((nt * NC + c) * 2 + 1) * 32 + lane];
         mma_s8(acc, high[0][c].x, high[1][c].x, high[0][c].y, high[1][c].y, qp.x, qp.y);
         mma_s8(acc, high[0][c].z, high[1][c].z, high[0][c].w, high[1][c].w, qp.z, qp.w);
         mma_s8(acc, low[0][c].x, low[1][c].x, low[0][c].y, low[1][c].y, qn.x, qn.y);
@@ -236,17 +208,13 @@ struct SelectKernel {
   void (*kernel)(SelectArgs, int*);
   int threads;
 };
-template <int D, int NT, int CL>
-SelectKernel select_of() {
-  return {select_kernel<D, NT, CL>, select_threads<D, NT, CL>()};
-}
-template <int D, int CL>
+template <int D, int CL, int T>
 SelectKernel select_rows(int rows) {
-  return rows <= 8 ? select_of<D, 1, CL>() : D == 256 || rows <= 16 ? select_of<D, 2, CL>() : select_of<D, D == 256 ? 2 : 4, CL>();
+  return {rows <= 8 ? select_kernel<D, 1, CL, T> : D == 256 || rows <= 16 ? select_kernel<D, 2, CL, T> : select_kernel<D, D == 256 ? 2 : 4, CL, T>, T};
 }
-template <int CL>
+template <int CL, int T>
 SelectKernel select_for(int d, int rows) {
-  return d == 64 ? select_rows<64, CL>(rows) : d == 128 ? select_rows<128, CL>(rows) : select_rows<256, CL>(rows);
+  return d == 64 ? select_rows<64, CL, T>(rows) : d == 128 ? select_rows<128, CL, T>(rows) : select_rows<256, CL, T>(rows);
 }
 
 struct SelectPlan {
@@ -261,8 +229,9 @@ bool select_plan(const KvAttnParams& p, int sms, SelectPlan* plan) {
   int cl = 1;
   while (cl < 16 && cl * 512LL < p.max_pages && kv_attention_units(p) * cl * 4 <= sms) cl *= 2;
   auto of = [&](int n) {
-    return n == 1 ? select_for<1>(d, rows) : n == 2 ? select_for<2>(d, rows) : n == 4 ? select_for<4>(d, rows)
-           : n == 8 ? select_for<8>(d, rows) : select_for<16>(d, rows);
+    return n == 1 ? (kv_attention_units(p) <= sms ? select_for<1, 512>(d, rows) : select_for<1, 256>(d, rows))
+           : n == 2 ? select_for<2, 512>(d, rows) : n == 4 ? select_for<4, 512>(d, rows)
+           : n == 8 ? select_for<8, 512>(d, rows) : select_for<16, 512>(d, rows);
   };
   plan->k = of(cl);
   if (cl == 16 && cluster_setup(plan->k.kernel, kMostKeys * 4, plan->k.threads, cl) <= 0) plan->k = of(cl = 8);
