@@ -650,7 +650,9 @@ int s3b_kv_bounds_values(const s3b_kv_bounds* bounds, const int64_t* pages, int6
  * be shorter) and each head of the cache:
  *   selected [batch][ceil(nq / share)][heads of the cache][keep]: places in the
  *            page table; a list ends at its first negative entry
- * At most 32 rows (share x heads / heads of the cache; 16 at d = 256) have a list. */
+ * At most 32 rows (share x heads / heads of the cache; 16 at d = 256) have a list.
+ * Calls of one context use its workspace: a captured one is replayed on the
+ * context's stream, or ordered with its other calls. */
 typedef struct s3b_kv_call {
     const int32_t* pages;
     int64_t pages_stride;
@@ -720,8 +722,8 @@ int s3b_op_cache_attention_selected(s3b_ctx* ctx, const s3b_kv_cache* cache, con
  * of -inf add nothing). weights: f32, token t of sequence b and head h at weights +
  * b * w_b + h * w_h + t, rows of max_pages * page_size values that do not overlap;
  * those behind a sequence's last token are left as they are. decay is finite and
- * >= 0. Sums are f32, in the same order on every run. The workspace is the
- * context's, as there. */
+ * >= 0; with 0 what was there does not count. Sums are f32, in the same order on
+ * every run. The workspace is the context's, as there. */
 int s3b_op_cache_weights(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_call* call, float* weights, int64_t w_b,
                          int64_t w_h, float decay);
 

@@ -816,6 +816,13 @@ class Engine:
             self._check(rc, "s3b_op_cache_attention")
 
     # -- long caches: reading and keeping less
+    @staticmethod
+    def _call(*fields) -> bytes:
+        try:
+            return _CALL.pack(*fields)
+        except struct.error as e:
+            raise S3BError(f"an argument is out of its range: {e}") from None
+
     def _sequences(self, what: str, pages, lengths):
         """Batch, pointer, row stride and width of a page table int32 [batch, max_pages], and the pointer of its lengths int32 [batch]."""
         device, shape = self.device, pages.shape
@@ -871,8 +878,8 @@ class Engine:
         b, table, row, width, lens = self._sequences(what, pages, lengths)
         if cache.device != self.device or bounds.device != self.device:
             raise S3BError(f"{what}: cache and bounds must be on cuda:{self.device}")
-        call = _CALL.pack(table, row, lens, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, width, b, 0, 0, 0, 0, 0, 0, 0, 0.0)
-        rc = self._L.s3b_op_cache_bounds(self.h, cache.ref, bounds.ref, call, (1 << 62) if new is None else new)
+        call = self._call(table, row, lens, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, width, b, 0, 0, 0, 0, 0, 0, 0, 0.0)
+        rc = self._L.s3b_op_cache_bounds(self.h, cache.ref, bounds.ref, call, (1 << 62) if new is None else min(new, 1 << 62))
         if rc:
             self._check(rc, "s3b_op_cache_bounds")
 
@@ -885,9 +892,11 @@ class Engine:
         b, table, row, width, lens = self._sequences(what, pages, lengths)
         _, nq, heads, at, q_b, q_n, q_h = self._query(what, bounds, q, b)
         lists, keep = self._lists(what, selected, b, nq, share, bounds.heads)
+        if sink < 0 or recent < 0 or sink + recent > keep:
+            raise S3BError(f"{what}: {sink} first and {recent} last pages of {keep}")
         if scores is not None:
             scores = self._dense(what, "scores", scores, _F32[0], (b, -(-nq // share), bounds.heads, width))
-        call = _CALL.pack(table, row, lens, at, q_b, q_n, q_h, 0, 0, 0, 0, 0, lists, width, b, nq, heads, 1 if causal else 0, window, keep,
+        call = self._call(table, row, lens, at, q_b, q_n, q_h, 0, 0, 0, 0, 0, lists, width, b, nq, heads, 1 if causal else 0, window, keep,
                           share, 0, 0.0)
         rc = self._L.s3b_op_cache_select(self.h, bounds.ref, call, sink, recent, scores)
         if rc:
@@ -906,7 +915,7 @@ class Engine:
             raise S3BError(f"{what}: out must be f16 or f32 of q's shape with contiguous rows on cuda:{device}")
         lists, keep = self._lists(what, selected, b, nq, share, cache.heads)
         lse = 0 if lse is None else self._dense(what, "lse", lse, _F32[0], (b, nq, heads))
-        call = _CALL.pack(table, row, lens, at, q_b, q_n, q_h, out.data_ptr(), o_b if b > 1 else 0, o_n if nq > 1 else 0,
+        call = self._call(table, row, lens, at, q_b, q_n, q_h, out.data_ptr(), o_b if b > 1 else 0, o_n if nq > 1 else 0,
                           o_h if heads > 1 else 0, lse, lists, width, b, nq, heads, 1 if causal else 0, window, keep, share,
                           0 if o_type == S3B_F16 else 1, scale)
         rc = self._L.s3b_op_cache_attention_selected(self.h, cache.ref, call)
@@ -923,7 +932,7 @@ class Engine:
         _, nq, heads, at, q_b, q_n, q_h = self._query(what, cache, q, b)
         lse = self._dense(what, "lse", lse, _F32[0], (b, nq, heads))
         w_b, w_h = self._rows_of_weights(what, cache, weights, b, width * cache.page_size)
-        call = _CALL.pack(table, row, lens, at, q_b, q_n, q_h, 0, 0, 0, 0, lse, 0, width, b, nq, heads, 1 if causal else 0, window, 0, 0, 0,
+        call = self._call(table, row, lens, at, q_b, q_n, q_h, 0, 0, 0, 0, lse, 0, width, b, nq, heads, 1 if causal else 0, window, 0, 0, 0,
                           scale)
         rc = self._L.s3b_op_cache_weights(self.h, cache.ref, call, weights.data_ptr(), w_b, w_h, decay)
         if rc:
@@ -941,12 +950,14 @@ class Engine:
         if len(shape) != 3 or target.device != self.device:
             raise S3BError(f"{what}: kept must have 3 dimensions, the new pages' cache be on cuda:{self.device}")
         keep = shape[2]
+        if sink < 0 or recent < 0 or sink + recent > keep:
+            raise S3BError(f"{what}: {sink} first and {recent} last tokens of {keep}")
         if b_out != b or width_out * target.page_size < keep:
             raise S3BError(f"{what}: pages_out must hold {keep} tokens for each of {b} sequences, lengths_out be int32 [{b}]")
         positions = self._dense(what, "kept", kept, _INDEX_TYPES[4], (b, cache.heads, keep))
         w_b, w_h = self._rows_of_weights(what, cache, weights, b, width * cache.page_size)
         moved = 0 if weights_out is None else self._dense(what, "weights_out", weights_out, _F32[0], shape)
-        call = _CALL.pack(table, row, lens, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, width, b, 0, 0, 0, 0, 0, 0, 0, 0.0)
+        call = self._call(table, row, lens, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, width, b, 0, 0, 0, 0, 0, 0, 0, 0.0)
         evict = _EVICT.pack(0 if to is None else ctypes.addressof(to.desc), weights.data_ptr(), w_b, w_h, table_out, row_out, lens_out, positions,
                             moved, keep, sink, recent)
         rc = self._L.s3b_op_cache_evict(self.h, cache.ref, call, evict)

@@ -161,7 +161,7 @@ int kv_bounds(const KvAttnParams& p, const KvBounds& out, long long recent, int*
   BoundsArgs a{p, out, recent, p.max_pages};
   const long long spanned = (recent + p.c.page_size - 2) / p.c.page_size + 1;  // pages that so many tokens can touch
   if (spanned < a.many) a.many = (int)spanned;
-  const long long blocks = std::min(((long long)p.batch * a.many * p.c.heads + 3) / 4, 1LL << 30);
+  const long long blocks = std::min(((long long)p.batch * a.many * p.c.heads + 3) / 4, 1LL << 17);  // they walk over wider tables
   const BoundsKernel k = p.c.type == QT_Q4_0 ? bounds_for<QT_Q4_0>(p.c.d)
                                              : p.c.type == QT_Q4_1 ? bounds_for<QT_Q4_1>(p.c.d) : bounds_for<QT_Q8_0>(p.c.d);
   return launch_dependent(k, dim3((unsigned)blocks), 128, 0, st, a, err);

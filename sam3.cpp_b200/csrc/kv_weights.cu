@@ -41,25 +41,61 @@ __device__ __forceinline__ void key_pairs(const uint32_t* piece, int nn, uint32_
 template <int QT, int D, int NG>
 struct Sweep {
   typedef KvL<QT, D> L;
-  static constexpr int kRows = 64;                                  // query rows staged at a time
+  static constexpr int kRows = 128;                                 // query rows staged at a time
   static constexpr int kQ = kRows * D * 2;                          // their fragments
   static constexpr int kMin = QT == QT_Q4_1 ? kRows * 4 * 8 : 0;    // q4_1: sums of the query over the blocks
   static constexpr int kSmem = kQ + kMin + kRows * 12;
-  static constexpr int kTokens = kWarps * NG * 16;                  // of a CTA's pass
+  static constexpr int kTokens = kWarps * NG * 16;                  // of a CTA's step
+  static constexpr int kBlocks = D == 256 ? 2 : D == 128 ? 3 : 4;   // that an SM's registers take
 };
 
 struct WeightArgs {
   KvAttnParams p;
   KvWeights w;
-  int token_blocks;  // of a sequence: max tokens / kTokens
 };
+
+// decay * old + sum; with a decay of 0 what was there does not count, whatever it is
+__device__ __forceinline__ float weigh(float decay, float old, float sum) { return decay != 0.f ? fmaf(decay, old, sum) : sum; }
+
+// The sequence of the line's place `pos` where sequence b has span(b) places, and the place of its first. The whole warp; pos lies
+// inside the line.
+template <typename Span>
+__device__ __forceinline__ int sequence_at(int batch, long long pos, long long* base, Span span) {
+  const int lane = threadIdx.x & 31;
+  *base = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const long long n = b0 + lane < batch ? span(b0 + lane) : 0;
+    long long last = n;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const long long up = __shfl_up_sync(~0u, last, x);
+      if (lane >= x) last += up;
+    }
+    const uint32_t past = __ballot_sync(~0u, *base + last > pos);
+    if (past) {
+      const int who = __ffs(past) - 1;
+      *base += __shfl_sync(~0u, last - n, who);
+      return b0 + who;
+    }
+    *base += __shfl_sync(~0u, last, 31);
+  }
+}
+template <typename Span>
+__device__ __forceinline__ long long line_length(int batch, Span span) {
+  long long total = 0;
+  for (int b = threadIdx.x & 31; b < batch; b += 32) total += span(b);
+#pragma unroll
+  for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(~0u, total, x);
+  return total;
+}
 
 // A unit is a sequence and a key / value head. Each warp holds NG groups of 16 tokens, their codes as the exact f16 integers of
 // the A operand, and sweeps over all rows of the unit, 8 at a time, with the rows' fragments in shared memory: for every block of
 // 32 channels two m16n8k16 products and the block's scale on the f32 result, then the weight exp2(s - lse) of each (row, token),
-// summed per token in f32 registers in the order of the rows. No atomics: a token belongs to one warp.
+// summed per token in f32 registers in the order of the rows. No atomics: a token belongs to one warp. The blocks of 128 tokens of all
+// units are one line, cut into equal shares for the CTAs; up to 128 rows stay in shared memory from one to the next.
 template <int QT, int D, int NG>
-__global__ void __launch_bounds__(32 * kWarps) sweep_kernel(const __grid_constant__ WeightArgs a, int* err) {
+__global__ void __launch_bounds__(32 * kWarps, Sweep<QT, D, NG>::kBlocks) sweep_kernel(const __grid_constant__ WeightArgs a, int* err) {
   typedef KvL<QT, D> L;
   typedef Sweep<QT, D, NG> C;
   constexpr int NB = L::kNB;
@@ -73,174 +109,195 @@ __global__ void __launch_bounds__(32 * kWarps) sweep_kernel(const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group_heads = p.heads / p.c.heads, n_rows = p.nq * group_heads;
   const int per_page = p.c.page_size >> 4;
-  const long long unit = blockIdx.x / a.token_blocks;
-  const int head = (int)(unit % p.c.heads), b = (int)(unit / p.c.heads);
+  const float sl2 = p.scale * kLog2e;
   let_next();
   wait_before();
-  const int len = sequence_length(p, b, err);
-  const int tok_cta = blockIdx.x % a.token_blocks * C::kTokens;
-  if (tok_cta >= len) return;
-  const float sl2 = p.scale * kLog2e;
-  const int* table = p.pages + b * p.pages_stride;
-  float* w = a.w.w + b * a.w.w_b + head * a.w.w_h;
-
-  // ---- this warp's tokens: group gg, tokens g and g + 8
-  int tok0[NG];
-  uint32_t ka[NG][NB][8];   // A fragments of the two products of a block
-  uint32_t sc[NG][NB];      // scales of tokens g, g + 8
-  uint32_t am[NG][4];       // minima
-#pragma unroll
-  for (int gg = 0; gg < NG; ++gg) {
-    tok0[gg] = tok_cta + (warp * NG + gg) * 16;
-    if (tok0[gg] >= len) {
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        sc[gg][n] = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ka[gg][n][e] = 0;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) am[gg][e] = 0;
+  auto blocks_of = [&](int b) { return (sequence_length(p, b, err) + C::kTokens - 1) / C::kTokens; };
+  auto span = [&](int b) { return (long long)blocks_of(b) * p.c.heads; };
+  const long long total = line_length(p.batch, span);
+  long long pos = total * blockIdx.x / gridDim.x, base;
+  const long long end = total * (blockIdx.x + 1) / gridDim.x;
+  if (pos >= end) return;
+  int b = sequence_at(p.batch, pos, &base, span);
+  long long staged = -1;  // the unit whose rows are in shared memory, all of them
+  for (; pos < end; ++pos) {
+    while (pos >= base + span(b)) base += span(b++);
+    const int len = sequence_length(p, b, err), blocks = blocks_of(b);
+    const int head = (int)((pos - base) / blocks);
+    const int tok_cta = (int)(pos - base - (long long)head * blocks) * C::kTokens;
+    const long long unit = (long long)b * p.c.heads + head;
+    const int* table = p.pages + b * p.pages_stride;
+    float* w = a.w.w + b * a.w.w_b + head * a.w.w_h;
+    int first, last, none;
+    row_span(p, len, 0, &first, &none);
+    row_span(p, len, p.nq - 1, &none, &last);
+    if (tok_cta >= last || tok_cta + C::kTokens <= first) {  // no row sees any of them
+      const int tok = tok_cta + threadIdx.x;
+      if (a.w.decay != 1.f && threadIdx.x < C::kTokens && tok < len) w[tok] = weigh(a.w.decay, w[tok], 0.f);
       continue;
     }
-    const int gi = tok0[gg] >> 4;
-    long long page = table[gi / per_page];
-    if (page < 0 || page >= p.c.n_pages) {
-      atomicCAS(err, 0, kDevErrIndex);
-      page = 0;
-    }
-    const uint8_t* gp = p.c.data + kv_group_offset<QT, D>(p.c, page, head, 0, gi % per_page);
-    uint32_t s0[NB / 2], s1[NB / 2];
-    lds<NB * 2>(gp + L::k_scale(g, 0), s0);
-    lds<NB * 2>(gp + L::k_scale(g + 8, 0), s1);
-#pragma unroll
-    for (int n = 0; n < NB; ++n) sc[gg][n] = __byte_perm(s0[n / 2], s1[n / 2], n & 1 ? 0x7632 : 0x5410);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) am[gg][e] = 0;
-    if (QT == QT_Q4_1 && 2 * t < NB) {
-      am[gg][0] = am[gg][2] = *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g, 2 * t));
-      am[gg][1] = am[gg][3] = *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g + 8, 2 * t));
-    }
-#pragma unroll
-    for (int sb = 0; sb < D / L::kSB; ++sb) {
-      constexpr int PB = L::kNBS * L::kBits;
-      uint32_t k0[PB / 4], k1[PB / 4];
-      lds<PB>(gp + L::k_val(g, sb * L::kNBS, t), k0);
-      lds<PB>(gp + L::k_val(g + 8, sb * L::kNBS, t), k1);
-#pragma unroll
-      for (int nn = 0; nn < L::kNBS; ++nn) {
-        const int n = sb * L::kNBS + nn;
-        uint32_t x0[4], x1[4];
-        key_pairs<QT, L::kNBS>(k0, nn, x0);
-        key_pairs<QT, L::kNBS>(k1, nn, x1);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          ka[gg][n][2 * e] = x0[e];
-          ka[gg][n][2 * e + 1] = x1[e];
-        }
-      }
-    }
-  }
 
-  float sum[NG][2];
+    // ---- this warp's tokens: group gg, tokens g and g + 8
+    int tok0[NG];
+    uint32_t ka[NG][NB][8];   // A fragments of the two products of a block
+    uint32_t sc[NG][NB];      // scales of tokens g, g + 8
+    uint32_t am[NG][4];       // minima
 #pragma unroll
-  for (int gg = 0; gg < NG; ++gg) sum[gg][0] = sum[gg][1] = 0.f;
-  for (int row0 = 0; row0 < n_rows; row0 += C::kRows) {
-    const int rows = min(C::kRows, n_rows - row0), tiles = (rows + kTile - 1) / kTile;
-    __syncthreads();
-    for (int e = threadIdx.x; e < tiles * NB * 32; e += 32 * kWarps) {
-      const int l = e & 31, n = e / 32 % NB, r = e / (32 * NB) * 8 + (l >> 2);
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        const int i = (row0 + r) / group_heads, h = head * group_heads + (row0 + r) % group_heads;
-        v = *reinterpret_cast<const uint4*>(p.q + b * p.q_b + i * p.q_n + h * p.q_h + 32 * n + 8 * (l & 3));
-      }
-      s_q[e] = v;
-    }
-    for (int r = threadIdx.x; r < tiles * kTile; r += 32 * kWarps) {
-      float lse = INFINITY;
-      int lo = 0, hi = 0;
-      if (r < rows) {
-        const int i = (row0 + r) / group_heads, h = head * group_heads + (row0 + r) % group_heads;
-        lse = p.lse[((long long)b * p.nq + i) * p.heads + h] * kLog2e;
-        if (lse != -INFINITY) row_span(p, len, i, &lo, &hi);  // else a row that has seen nothing, and sees nothing here
-      }
-      s_lse[r] = lse;
-      s_lo[r] = lo;
-      s_hi[r] = hi;
-    }
-    __syncthreads();
-    if (QT == QT_Q4_1) {  // sums of the query over blocks 2t, 2t + 1 as f16 and f16 remainder: a warp a row tile
-      for (int nt = warp; nt < tiles; nt += kWarps) {
-        float lo = 0.f, hi = 0.f;
+    for (int gg = 0; gg < NG; ++gg) {
+      tok0[gg] = tok_cta + (warp * NG + gg) * 16;
+      if (tok0[gg] >= len) {
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          const uint4 v = s_q[(nt * NB + n) * 32 + lane];
-          const float s = block_sum(v);
-          if (n == 2 * t) lo = s;
-          if (n == 2 * t + 1) hi = s;
+          sc[gg][n] = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ka[gg][n][e] = 0;
         }
-        s_min[nt * 32 + lane] = split_sums(lo, hi);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) am[gg][e] = 0;
+        continue;
+      }
+      const int gi = tok0[gg] >> 4;
+      long long page = table[gi / per_page];
+      if (page < 0 || page >= p.c.n_pages) {
+        atomicCAS(err, 0, kDevErrIndex);
+        page = 0;
+      }
+      const uint8_t* gp = p.c.data + kv_group_offset<QT, D>(p.c, page, head, 0, gi % per_page);
+      uint32_t s0[NB / 2], s1[NB / 2];
+      lds<NB * 2>(gp + L::k_scale(g, 0), s0);
+      lds<NB * 2>(gp + L::k_scale(g + 8, 0), s1);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) sc[gg][n] = __byte_perm(s0[n / 2], s1[n / 2], n & 1 ? 0x7632 : 0x5410);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) am[gg][e] = 0;
+      if (QT == QT_Q4_1 && 2 * t < NB) {
+        am[gg][0] = am[gg][2] = *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g, 2 * t));
+        am[gg][1] = am[gg][3] = *reinterpret_cast<const uint32_t*>(gp + L::kSc + L::k_scale(g + 8, 2 * t));
+      }
+#pragma unroll
+      for (int sb = 0; sb < D / L::kSB; ++sb) {
+        constexpr int PB = L::kNBS * L::kBits;
+        uint32_t k0[PB / 4], k1[PB / 4];
+        lds<PB>(gp + L::k_val(g, sb * L::kNBS, t), k0);
+        lds<PB>(gp + L::k_val(g + 8, sb * L::kNBS, t), k1);
+#pragma unroll
+        for (int nn = 0; nn < L::kNBS; ++nn) {
+          const int n = sb * L::kNBS + nn;
+          uint32_t x0[4], x1[4];
+          key_pairs<QT, L::kNBS>(k0, nn, x0);
+          key_pairs<QT, L::kNBS>(k1, nn, x1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            ka[gg][n][2 * e] = x0[e];
+            ka[gg][n][2 * e + 1] = x1[e];
+          }
+        }
+      }
+    }
+
+    float sum[NG][2];
+#pragma unroll
+    for (int gg = 0; gg < NG; ++gg) sum[gg][0] = sum[gg][1] = 0.f;
+    for (int row0 = 0; row0 < n_rows; row0 += C::kRows) {
+      const int rows = min(C::kRows, n_rows - row0), tiles = (rows + kTile - 1) / kTile;
+      if (staged != unit) {
+      __syncthreads();
+      for (int e = threadIdx.x; e < tiles * NB * 32; e += 32 * kWarps) {
+        const int l = e & 31, n = e / 32 % NB, r = e / (32 * NB) * 8 + (l >> 2);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < rows) {
+          const int i = (row0 + r) / group_heads, h = head * group_heads + (row0 + r) % group_heads;
+          v = *reinterpret_cast<const uint4*>(p.q + b * p.q_b + i * p.q_n + h * p.q_h + 32 * n + 8 * (l & 3));
+        }
+        s_q[e] = v;
+      }
+      for (int r = threadIdx.x; r < tiles * kTile; r += 32 * kWarps) {
+        float lse = INFINITY;
+        int lo = 0, hi = 0;
+        if (r < rows) {
+          const int i = (row0 + r) / group_heads, h = head * group_heads + (row0 + r) % group_heads;
+          lse = p.lse[((long long)b * p.nq + i) * p.heads + h] * kLog2e;
+          if (lse != -INFINITY) row_span(p, len, i, &lo, &hi);  // else a row that has seen nothing, and sees nothing here
+        }
+        s_lse[r] = lse;
+        s_lo[r] = lo;
+        s_hi[r] = hi;
       }
       __syncthreads();
-    }
-    for (int nt = 0; nt < tiles; ++nt) {
-      float s[NG][4];
+      if (QT == QT_Q4_1) {  // sums of the query over blocks 2t, 2t + 1 as f16 and f16 remainder: a warp a row tile
+        for (int nt = warp; nt < tiles; nt += kWarps) {
+          float lo = 0.f, hi = 0.f;
 #pragma unroll
-      for (int gg = 0; gg < NG; ++gg)
+          for (int n = 0; n < NB; ++n) {
+            const uint4 v = s_q[(nt * NB + n) * 32 + lane];
+            const float s = block_sum(v);
+            if (n == 2 * t) lo = s;
+            if (n == 2 * t + 1) hi = s;
+          }
+          s_min[nt * 32 + lane] = split_sums(lo, hi);
+        }
+        __syncthreads();
+      }
+      if (n_rows <= C::kRows) staged = unit;
+      }
+      for (int nt = 0; nt < tiles; ++nt) {
+        float s[NG][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[gg][e] = 0.f;
-      if (QT == QT_Q4_1) {
-        const uint2 m = s_min[nt * 32 + lane];
+        for (int gg = 0; gg < NG; ++gg)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[gg][e] = 0.f;
+        if (QT == QT_Q4_1) {
+          const uint2 m = s_min[nt * 32 + lane];
+#pragma unroll
+          for (int gg = 0; gg < NG; ++gg) {
+            mma16816(s[gg], am[gg], m.x, m.y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[gg][e] *= kSumsLess;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const uint4 q = s_q[(nt * NB + n) * 32 + lane];
+#pragma unroll
+          for (int gg = 0; gg < NG; ++gg) {
+            const uint32_t(&k)[8] = ka[gg][n];
+            const uint32_t a0[4] = {k[0], k[1], k[2], k[3]}, a1[4] = {k[4], k[5], k[6], k[7]};
+            float c[4];
+            mma16816_first(c, a0, q.x, q.y);
+            mma16816(c, a1, q.z, q.w);
+            const float2 f = __half22float2(u32_h2(sc[gg][n]));
+            s[gg][0] = fmaf(f.x, c[0], s[gg][0]);
+            s[gg][1] = fmaf(f.x, c[1], s[gg][1]);
+            s[gg][2] = fmaf(f.y, c[2], s[gg][2]);
+            s[gg][3] = fmaf(f.y, c[3], s[gg][3]);
+          }
+        }
+        const int r = nt * kTile + 2 * t;
+        const float2 lse = *reinterpret_cast<const float2*>(s_lse + r);
+        const int2 lo = *reinterpret_cast<const int2*>(s_lo + r), hi = *reinterpret_cast<const int2*>(s_hi + r);
 #pragma unroll
         for (int gg = 0; gg < NG; ++gg) {
-          mma16816(s[gg], am[gg], m.x, m.y);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[gg][e] *= kSumsLess;
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const uint4 q = s_q[(nt * NB + n) * 32 + lane];
-#pragma unroll
-        for (int gg = 0; gg < NG; ++gg) {
-          const uint32_t(&k)[8] = ka[gg][n];
-          const uint32_t a0[4] = {k[0], k[1], k[2], k[3]}, a1[4] = {k[4], k[5], k[6], k[7]};
-          float c[4];
-          mma16816_first(c, a0, q.x, q.y);
-          mma16816(c, a1, q.z, q.w);
-          const float2 f = __half22float2(u32_h2(sc[gg][n]));
-          s[gg][0] = fmaf(f.x, c[0], s[gg][0]);
-          s[gg][1] = fmaf(f.x, c[1], s[gg][1]);
-          s[gg][2] = fmaf(f.y, c[2], s[gg][2]);
-          s[gg][3] = fmaf(f.y, c[3], s[gg][3]);
-        }
-      }
-      const int r = nt * kTile + 2 * t;
-      const float2 lse = *reinterpret_cast<const float2*>(s_lse + r);
-      const int2 lo = *reinterpret_cast<const int2*>(s_lo + r), hi = *reinterpret_cast<const int2*>(s_hi + r);
-#pragma unroll
-      for (int gg = 0; gg < NG; ++gg) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int tok = tok0[gg] + g + 8 * u;
-          const float e0 = ex2_approx(fmaf(s[gg][2 * u], sl2, -lse.x)), e1 = ex2_approx(fmaf(s[gg][2 * u + 1], sl2, -lse.y));
-          sum[gg][u] += tok >= lo.x && tok < hi.x ? e0 : 0.f;
-          sum[gg][u] += tok >= lo.y && tok < hi.y ? e1 : 0.f;
+          for (int u = 0; u < 2; ++u) {
+            const int tok = tok0[gg] + g + 8 * u;
+            const float e0 = ex2_approx(fmaf(s[gg][2 * u], sl2, -lse.x)), e1 = ex2_approx(fmaf(s[gg][2 * u + 1], sl2, -lse.y));
+            sum[gg][u] += tok >= lo.x && tok < hi.x ? e0 : 0.f;
+            sum[gg][u] += tok >= lo.y && tok < hi.y ? e1 : 0.f;
+          }
         }
       }
     }
+#pragma unroll
+    for (int gg = 0; gg < NG; ++gg)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float v = sum[gg][u];
+        v += __shfl_xor_sync(~0u, v, 1);
+        v += __shfl_xor_sync(~0u, v, 2);
+        const int tok = tok0[gg] + g + 8 * u;
+        if (t == 0 && tok < len) w[tok] = weigh(a.w.decay, w[tok], v);
+      }
   }
-#pragma unroll
-  for (int gg = 0; gg < NG; ++gg)
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float v = sum[gg][u];
-      v += __shfl_xor_sync(~0u, v, 1);
-      v += __shfl_xor_sync(~0u, v, 2);
-      const int tok = tok0[gg] + g + 8 * u;
-      if (t == 0 && tok < len) w[tok] = fmaf(a.w.decay, w[tok], v);
-    }
 }
 
 // ---------------------------------------------------------------- few rows
@@ -274,33 +331,12 @@ __global__ void __launch_bounds__(128, Stream<QT, D, NT>::kBlocks) stream_kernel
   let_next();
   wait_before();
   // this warp's share of the line, and the sequence in which it begins
-  auto groups_of = [&](int b) { return (sequence_length(p, b, err) + 15) >> 4; };
-  long long total = 0;
-  for (int b = lane; b < p.batch; b += 32) total += groups_of(b);
-#pragma unroll
-  for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(~0u, total, x);
-  total *= p.c.heads;
-  long long pos = total * warp / warps, base = 0;
+  auto span = [&](int b) { return (long long)((sequence_length(p, b, err) + 15) >> 4) * p.c.heads; };
+  const long long total = line_length(p.batch, span);
+  long long pos = total * warp / warps, base;
   const long long end = total * (warp + 1) / warps;
   if (pos >= end) return;
-  int b = 0;
-  for (int b0 = 0;; b0 += 32) {
-    const long long n = b0 + lane < p.batch ? (long long)groups_of(b0 + lane) * p.c.heads : 0;
-    long long last = n;
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-      const long long up = __shfl_up_sync(~0u, last, x);
-      if (lane >= x) last += up;
-    }
-    const uint32_t past = __ballot_sync(~0u, base + last > pos);
-    if (past) {
-      const int who = __ffs(past) - 1;
-      b = b0 + who;
-      base += __shfl_sync(~0u, last - n, who);
-      break;
-    }
-    base += __shfl_sync(~0u, last, 31);
-  }
+  int b = sequence_at(p.batch, pos, &base, span);
 
   const float sl2 = p.scale * kLog2e;
   for (; pos < end; ++b) {
@@ -482,7 +518,7 @@ __global__ void __launch_bounds__(128, Stream<QT, D, NT>::kBlocks) stream_kernel
         }
         if (mine(it)) {
           const float s0 = t & 1 ? sum[0][1] : sum[0][0], s1 = t & 1 ? sum[G - 1][1] : sum[G - 1][0];
-          w[mine_tok + it * (16 * G)] = fmaf(a.w.decay, old, G == 2 && (t & 2) ? s1 : s0);
+          w[mine_tok + it * (16 * G)] = weigh(a.w.decay, old, G == 2 && (t & 2) ? s1 : s0);
         }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -493,16 +529,12 @@ __global__ void __launch_bounds__(128, Stream<QT, D, NT>::kBlocks) stream_kernel
 }
 
 template <int QT, int D, int NG>
-int launch_sweep(const KvAttnParams& p, const KvWeights& w, int* err, cudaStream_t st) {
+int launch_sweep(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st) {
   typedef Sweep<QT, D, NG> C;
   auto* k = sweep_kernel<QT, D, NG>;
   if (kernel_setup(k, C::kSmem) <= 0) return -13;
-  const long long tokens = (long long)p.max_pages * p.c.page_size;
-  WeightArgs a{p, w, (int)((tokens + C::kTokens - 1) / C::kTokens)};
-  const long long grid = (long long)p.batch * p.c.heads * a.token_blocks;
-  if (grid == 0) return 0;
-  if (grid > 0x7fffffffLL) return -2;
-  return launch_dependent(k, dim3((unsigned)grid), 32 * kWarps, C::kSmem, st, a, err);
+  const WeightArgs a{p, w};
+  return launch_dependent(k, dim3(sms * C::kBlocks), 32 * kWarps, C::kSmem, st, a, err);
 }
 
 template <int QT, int D, int NT>
@@ -510,15 +542,14 @@ int launch_stream(const KvAttnParams& p, const KvWeights& w, int sms, int* err, 
   typedef Stream<QT, D, NT> C;
   auto* k = stream_kernel<QT, D, NT>;
   if (kernel_setup(k, C::kSmem) <= 0) return -13;
-  const WeightArgs a{p, w, 0};
+  const WeightArgs a{p, w};
   return launch_dependent(k, dim3(sms * C::kBlocks), 128, C::kSmem, st, a, err);
 }
 
-// Whether the tiles of 128 rows take the call: they are ahead from where a second one is well filled (us at 64 / 128 / 256 channels,
-// 32 heads over 8000 tokens: 192 rows 65 / 83 / 111 against 50 / 79 / 155, 256 rows 66 / 83 / 111 against 65 / 103 / 203).
-bool many_rows(const KvAttnParams& p) {
-  return p.nq * (long long)(p.heads / p.c.heads) > (p.c.d == 256 ? 128 : p.c.d == 128 ? 192 : 256);
-}
+// Whether the tiles of 128 rows take the call: they are ahead from where a second one is used, at d = 64 from where it is half full (4
+// sequences of 8000 tokens, 8 heads, us at d = 64 / 128 / 256: 128 rows 77 / 88 / 112 against 38 / 51 / 82 here, 192 rows 65 / 83 /
+// 111 against 63 / 92 / 155, 256 rows 66 / 83 / 111 against 78 / 103 / 203).
+bool many_rows(const KvAttnParams& p) { return p.nq * (long long)(p.heads / p.c.heads) > (p.c.d == 64 ? 192 : 128); }
 
 template <int QT, int D>
 int weights_for(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cudaStream_t st) {
@@ -527,7 +558,7 @@ int weights_for(const KvAttnParams& p, const KvWeights& w, int sms, int* err, cu
   if (rows <= 16) return launch_stream<QT, D, 2>(p, w, sms, err, st);
   if (D < 256 && rows <= 32) return launch_stream<QT, D, D < 256 ? 4 : 2>(p, w, sms, err, st);
   if (many_rows(p)) return kv_weights_tc(p, w, sms, err, st);
-  return launch_sweep<QT, D, 1>(p, w, err, st);
+  return launch_sweep<QT, D, 1>(p, w, sms, err, st);
 }
 
 template <int QT>

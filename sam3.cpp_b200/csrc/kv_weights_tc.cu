@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(Wt<QT, D>::kThreads, 1) weights_tiles_kernel(c
       sum += s_red[turn * kTile + row];
       float* to = a.w.w + s.b * a.w.w_b + s.head * a.w.w_h;
       if (s.whole) {
-        if (tok < s.len) to[tok] = fmaf(a.w.decay, to[tok], sum);
+        if (tok < s.len) to[tok] = a.w.decay != 0.f ? fmaf(a.w.decay, to[tok], sum) : sum;
         continue;
       }
       const long long c0 = ((s.start + 1) * ctas - 1) / total, c1 = ((s.start + a.chunks) * ctas - 1) / total;
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(Wt<QT, D>::kThreads, 1) weights_tiles_kernel(c
         sum = 0.f;
         const int second = s.start > total * c0 / ctas;
         for (long long k = c0; k <= c1; ++k) sum += __ldcg(a.part + (2 * k + (k == c0 ? second : 0)) * kTile + row);
-        if (tok < s.len) to[tok] = fmaf(a.w.decay, to[tok], sum);
+        if (tok < s.len) to[tok] = a.w.decay != 0.f ? fmaf(a.w.decay, to[tok], sum) : sum;
         if (row == 0) a.count[c0] = 0;
       }
     }

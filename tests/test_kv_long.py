@@ -102,3 +102,21 @@ def test_strides_are_refused(s3b, name, shape, strides):
                                         ("q", (1, 5, 4, 128)), ("weights", (1, 4, PAGES * PAGE))])
 def test_sizes_that_do_not_fit_are_refused(s3b, name, shape):
     _check(s3b, name, _Strided(0, SHAPES[name][0], *shape))
+
+
+@pytest.mark.parametrize("wrong", [dict(window=1 << 40, causal=True), dict(share=0), dict(share=-1), dict(sink=2, recent=2), dict(sink=-1), dict(recent=-1), dict(sink=1 << 40)])
+def test_numbers_out_of_range_are_refused(s3b, wrong):
+    engine, _ = _calls(s3b)
+    cache = s3b.KVCache(2, PAGES, PAGE, KV, D, data=_Strided(0, torch.uint8, s3b.kv_cache_bytes(2, KV, D, PAGE, PAGES)))
+    bounds = s3b.KVBounds.__new__(s3b.KVBounds)
+    bounds.device, bounds.heads, bounds.d, bounds.ref = 0, KV, D, None
+    q, pages, lengths = _Strided(0, torch.float16, 1, 5, 4, D), _Strided(0, torch.int32, 1, PAGES), _Strided(0, torch.int32, 1)
+    args = dict(share=2, sink=0, recent=1)
+    args.update(wrong)
+    with pytest.raises(s3b.S3BError):
+        engine.cache_select(bounds, q, _Strided(0, torch.int32, 1, 3, KV, KEEP), pages, lengths, **args)
+    if "sink" in wrong or "recent" in wrong:
+        with pytest.raises(s3b.S3BError):
+            engine.cache_evict(cache, _Strided(0, torch.float32, 1, KV, PAGES * PAGE), pages, lengths, _Strided(0, torch.int32, 1, 3), _Strided(0, torch.int32, 1),
+                               _Strided(0, torch.int32, 1, KV, 3), **wrong)
+    assert engine._L.calls == 0

@@ -486,6 +486,46 @@ def test_weights_of_rows_that_saw_nothing(s3b, engine):
     assert torch.isfinite(w).all() and (w - v).abs().max() <= 1e-6 * v.max() and w[0, 0, 99] > 0 and (w[0, 0, 100:] == 0).all()
 
 
+@pytest.mark.parametrize("nq,heads", [(1, 2), (20, 2), (200, 2)])
+def test_weights_with_a_decay_of_zero(s3b, engine, nq, heads):
+    """What was there does not count, whatever it is; tokens that no row sees end at 0, those behind the last keep theirs."""
+    s = Sequences(s3b, engine, 2, 64, 2, 16, [300, 17], seed=nq)
+    w = torch.full((2, 2, 304), math.nan, device="cuda")
+    v = torch.zeros(2, 2, 304, device="cuda")
+    q, lse = s.queries(nq, heads), torch.full((2, nq, heads), 3.0, device="cuda")
+    for x in (w, v):
+        engine.cache_weights(s.cache, q, lse, x, s.pages, s.lengths, 0.1, decay=0.0, causal=True, window=5)
+    engine.sync()
+    for b, n in enumerate(s.lens):
+        assert torch.equal(w[b, :, :n], v[b, :, :n]) and torch.isnan(w[b, :, n:]).all()
+    assert (w[0, :, :300 - nq - 4] == 0).all() and (w[0, :, 299] > 0).all()
+
+
+@pytest.mark.parametrize("nq", [1, 40, 300])
+def test_wide_page_tables_cost_nothing(s3b, engine, nq):
+    """Tables of 2^27 tokens with short sequences: the lengths say what is done."""
+    s = Sequences(s3b, engine, 2, 128, 2, 64, [200, 0, 1000], seed=nq)
+    wide = torch.zeros(1, 1 << 21, dtype=torch.int32, device="cuda")
+    table = wide.expand(3, -1).clone()
+    table[:, :s.pages.shape[1]] = s.pages
+    q, lse = s.queries(nq, 4), torch.full((3, nq, 4), 3.0, device="cuda")
+    w, v = torch.ones(3, 2, 64 << 21, device="cuda"), torch.ones(3, 2, 1024, device="cuda")
+    engine.cache_weights(s.cache, q, lse, w, table, s.lengths, 0.1, causal=True)
+    engine.cache_weights(s.cache, q, lse, v, s.pages, s.lengths, 0.1, causal=True)
+    bounds, again = s3b.KVBounds(s.cache), s3b.KVBounds(s.cache)
+    engine.cache_bounds(s.cache, bounds, table, s.lengths)
+    engine.cache_bounds(s.cache, again, s.pages, s.lengths)
+    a, b = (torch.empty(3, -(-nq // 8), 2, 4, dtype=torch.int32, device="cuda") for _ in "ab")
+    engine.cache_select(bounds, q, a, table, s.lengths, share=8)
+    engine.cache_select(bounds, q, b, s.pages, s.lengths, share=8)
+    x, y = torch.empty_like(q), torch.empty_like(q)
+    engine.cache_attention_selected(s.cache, q, x, a, table, s.lengths, 0.1, share=8)
+    engine.cache_attention_selected(s.cache, q, y, b, s.pages, s.lengths, 0.1, share=8)
+    engine.sync()
+    assert torch.equal(w[:, :, :1024], v) and (w[:, :, 1024:] == 1).all()
+    assert torch.equal(bounds.codes, again.codes) and torch.equal(a, b) and torch.equal(x, y)
+
+
 @pytest.mark.parametrize("nq", [1, 70])
 def test_weights_rows_apart(s3b, engine, nq):
     """Weights and queries as slices of larger tensors, sequences inside and heads outside."""
