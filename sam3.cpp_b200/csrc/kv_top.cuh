@@ -45,20 +45,22 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Fetch fetch, Make
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows_all = (n + 31) / 32, rows_warp = (rows_all + W - 1) / W;
   const int from = min(warp * rows_warp, rows_all) * 32, to = min(n, from + rows_warp * 32);  // of this warp's run
-  // f(whether there is a key, place, key): a whole warp each
+  // f(whether there is a key, place, key): a whole warp each. Full steps know that there is.
   auto each_of = [&](auto&& of, auto unroll, auto&& f) {
     constexpr int U = decltype(unroll)::value;
-    for (int i0 = from; i0 < to; i0 += 32 * U) {
-      decltype(of(0)) x[U];
+    decltype(of(0)) x[U];
+    int i0 = from + lane;
+    for (; i0 - lane + 32 * U <= to; i0 += 32 * U) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + 32 * u + lane;
-        x[u] = i < to ? of(i) : decltype(of(0))(0);
-      }
+      for (int u = 0; u < U; ++u) x[u] = of(i0 + 32 * u);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i0 + 32 * u < to) f(i0 + 32 * u + lane < to, i0 + 32 * u + lane, x[u]);
+      for (int u = 0; u < U; ++u) f(std::true_type(), i0 + 32 * u, x[u]);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = i0 + 32 * u < to ? of(i0 + 32 * u) : decltype(of(0))(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 - lane + 32 * u < to) f(i0 + 32 * u < to, i0 + 32 * u, x[u]);
   };
   auto each = [&](auto&& f) { each_of(key, std::integral_constant<int, 4>(), f); };
   uint32_t left = k;
@@ -95,11 +97,11 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Fetch fetch, Make
       const int shift = 24 - 8 * round;
       __syncthreads();
       if (round == 0) {
-        each_of(fetch, std::integral_constant<int, 8>(), [&](bool there, int i, decltype(fetch(0)) v) {
+        each_of(fetch, std::integral_constant<int, 8>(), [&](auto there, int i, decltype(fetch(0)) v) {
           if (there) atomicAdd(&s.hist[(make(i, v) >> 24) * C + lane % C], 1u);
         });
       } else {
-        each([&](bool there, int, uint32_t x) {
+        each([&](auto there, int, uint32_t x) {
           if (there && (x ^ prefix) >> (shift + 8) == 0) atomicAdd(&s.hist[(x >> shift & 255) * C + lane % C], 1u);
         });
       }
@@ -161,7 +163,7 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Fetch fetch, Make
   }
   // places of what each warp takes (counted by lanes: POPC runs at an eighth of the rate of an addition)
   uint32_t above = 0, equal = 0;
-  each([&](bool there, int, uint32_t x) {
+  each([&](auto there, int, uint32_t x) {
     above += there && x >= from_above;
     equal += there && x >= from_equal && x < from_above;
   });
@@ -182,7 +184,7 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Fetch fetch, Make
     // no CTA leaves while another reads its counts: this one has read those of others
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   }
-  each([&](bool there, int i, uint32_t x) {
+  each([&](auto there, int i, uint32_t x) {
     const bool is_above = there && x >= from_above, is_equal = there && x >= from_equal && x < from_above;
     const uint32_t ma = __ballot_sync(~0u, is_above), mq = left ? __ballot_sync(~0u, is_equal) : 0u, below = (1u << lane) - 1;
     if (!(ma | mq)) return;
