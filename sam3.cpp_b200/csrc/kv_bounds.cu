@@ -32,6 +32,10 @@ __device__ __forceinline__ void fold(__half2 (&lo)[R], __half2 (&hi)[R], int lan
 // keys' layout hold, as f16 pairs: the row as cache_read gives it in f16 (one rounding, which keeps the order of values, so that
 // least and largest of the rounded are the rounded least and largest), two values an instruction. Then the 8 lanes of a t share
 // the channels out among themselves, the larger half of the exchange first, and the row's largest magnitude sets the step.
+// Measured: 2 x 65536 tokens, 4 heads of 128 in pages of 64: q4_0 37.7 MB of keys in 18.7 us, 2.0 TB/s; q4_1 18.7, q8_0 26.5.
+// Half of the cycles issue (55% of the ALU's: minima, maxima, unpacking), the rest waits for a page's first words behind length
+// and page table. Four tokens ahead instead of two (23.2 us), blocks that stay and read the next page's place ahead (19.4) and more
+// blocks by fewer registers (18.9) were no faster.
 template <int QT, int D>
 __global__ void __launch_bounds__(128) bounds_kernel(const __grid_constant__ BoundsArgs a, int* err) {
   typedef KvL<QT, D> L;

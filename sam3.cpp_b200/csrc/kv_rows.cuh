@@ -84,7 +84,9 @@ struct ScaleRange {
 // With SEL a unit is a block of p.share queries and a key / value head, and its tokens are those of the pages that its list
 // names: steps of W groups go over the list's pages, a page's first token stands at entry * page_size, and the masks go by
 // that. Its weights keep what their rounding to f16 left until they are multiplied by a scale: the output is off by 2.9e-4 of its
-// norm then, two movmatrix and 2 NB products more for 16 tokens and 8 rows.
+// norm then, two movmatrix and 2 NB products more for 16 tokens and 8 rows. Measured: 32 x 8 lists of 32 pages of 64, 4 heads a list of
+// d = 128, q4_0: 75 MB in 27 us (37 with shares of equal size, whose parts had to be joined); 256 lists of 64 pages, 16 rows of
+// d = 256, q8_0: 131 us, 136 TFLOP/s. Issue bounds both (45 to 52% of the cycles; at d = 256 the output's registers leave 8 warps an SM).
 constexpr int kNoTok = 0x7FFFFF00;  // position of a group that is none: past every span
 
 template <int QT, int D, int NT, int W>

@@ -36,8 +36,9 @@ struct TopShared {
 // i (all of a step's fetches come before its makes, which may write: 18000 cycles otherwise, 128 KB at one load's latency after
 // the other's), key(i) after that: from shared memory where they fit. emit(position, place) is called for the taken ones, k of
 // them in all (0 < k <= the line's length, and at least the number of forced keys).
-// Measured (cycles of the SM): 32768 keys a CTA of 1024 threads, 16 of them: a round 4700 to 7000 to count (the atomics on shared
-// memory), 500 to add up, 4000 for the cluster to meet and find the digit. 256 keys, 256 threads: see the branch for few keys.
+// Measured (cycles of the SM), 16 CTAs of 1024 threads and 32768 keys each: a round 5000 to 7000 to count (instructions, and the
+// atomics on shared memory), 500 to add up, 3700 for the cluster to meet and find the digit; 6000 to count what is taken, 9000 to
+// write it. 256 keys, 256 threads: see the branch for few keys.
 template <int T, int CL, typename Fetch, typename Make, typename Key, typename Emit>
 __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Fetch fetch, Make make, Key key, Emit emit) {
   constexpr int W = T / 32, C = TopShared<T>::kCopies, P = T / 256;  // P threads a digit

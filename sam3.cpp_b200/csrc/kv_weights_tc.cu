@@ -11,6 +11,11 @@
 // The line of (tile of 128 tokens, 128 query rows) of all sequences and heads is cut into equal shares for the CTAs. A tile that
 // several CTAs share leaves its sums in the workspace; the last CTA to arrive adds them in the order of the shares.
 //
+// Measured: 4096 rows over 28736 tokens, one head of 256, q4_0: 102 us, 590 TFLOP/s of the product itself and twice that in the tensor
+// cores (65% of the kernel's cycles; what is left is K's way into TMEM at each tile's beginning, when no product runs, and the
+// chain product - exponentials of the two S regions); a chunk of 128 rows takes 1.4 us at d = 256, 0.8 at 64. The same on mma.sync
+// fragments took 434 us.
+//
 // Roles: warps 0-3 and 4-7 take turns at S of every other 128 rows, and dequantise half of K's channels each; warps 8-11
 // copy the query rows (asynchronously, in the 128-byte swizzle); warp 12 issues the products; warp 13 reads the rows' ln sums.
 #include <algorithm>
