@@ -15,8 +15,8 @@
 // copy reaches; one sequence of 524288 tokens, 16 heads on 2, q4_1: 168 MB in 53 us. Instruction issue bounds it (62% of
 // the cycles issue, the integer pipe is half busy): some 350 instructions for 16 tokens of a head, most of them unpacking
 // codes and scaling partial scores and weights. Looking at the scales of each step (ScaleRange) is 3% of the time. The output's
-// and the query's registers leave 33 of the 48 variants 4 to 84 bytes of spills a thread (one query tile of d = 128 in q4_0: 24
-// and 32, in q4_1 16 and 32).
+// and the query's registers leave 32 of the 48 variants 4 to 84 bytes of spills a thread (one query tile of d = 128 in q4_0: 32,
+// in q4_1 16 and 32).
 #pragma once
 #include <algorithm>
 
@@ -150,10 +150,11 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
   const int all_rows = p.nq * group_heads;
   const int per_page = p.c.page_size >> 4;
   // units of a sequence: its heads, and with SEL the blocks of `share` queries
-  const int seq_units = SEL ? p.c.heads * ((p.nq - 1) / p.share + 1) : p.c.heads;
+  const int list_units = SEL ? p.c.heads * ((p.nq - 1) / p.share + 1) : 0;
+  auto seq_units = [&]() { return SEL ? list_units : p.c.heads; };
 
   auto chunks_of = [&](int b, int* g0, int* g1) -> int {
-    if (SEL) {  // groups of the longest list that a unit of the sequence can have
+    if (SEL) {  // groups of the longest list that names each page of the sequence once
       *g0 = 0;
       *g1 = min(p.keep, (sequence_length(p, b, err) + p.c.page_size - 1) / p.c.page_size) * per_page;
     } else {
@@ -182,25 +183,25 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
 #pragma unroll
     for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(~0u, total, x);
     most = __reduce_max_sync(~0u, most);
-    total *= seq_units;
+    total *= seq_units();
     long long ctas = min((long long)gridDim.x, total), base = 0, p0 = 0, p1 = 0;
     int found = -1;
     // Lists are short and of nearly one length: whole where a unit of its own costs a block no more than some chunks above an equal
     // share, which is what joining parts costs.
     const bool whole = SEL ? most - total / max(ctas, 1LL) <= kWholeList : most <= kWhole;
-    if (whole && (long long)p.batch * seq_units <= gridDim.x) {
-      const int b = blockIdx.x / seq_units;
+    if (whole && (long long)p.batch * seq_units() <= gridDim.x) {
+      const int b = blockIdx.x / seq_units();
       if (b < p.batch) {
         const int n = chunks_of(b, &g0, &g1);
         found = b;
-        p0 = (blockIdx.x - b * seq_units) * n;
+        p0 = (blockIdx.x - b * seq_units()) * n;
         p1 = p0 + n;
       }
     } else if ((int)blockIdx.x < ctas) {
       p0 = total * blockIdx.x / ctas;
       p1 = total * (blockIdx.x + 1) / ctas;
       for (int b0 = 0; b0 < p.batch && found < 0; b0 += 32) {
-        const long long n = b0 + lane < p.batch ? (long long)chunks_of(b0 + lane, &g0, &g1) * seq_units : 0;
+        const long long n = b0 + lane < p.batch ? (long long)chunks_of(b0 + lane, &g0, &g1) * seq_units() : 0;
         long long end = n;
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) {
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
       row_span(p, len, p.nq - 1, &max_lo, &max_hi);
     }
     const int* table = p.pages + b * p.pages_stride;
-    for (; pos < p1 && pos < base + (long long)n_chunks * seq_units;) {
+    for (; pos < p1 && pos < base + (long long)n_chunks * seq_units();) {
       const int seq_unit = (int)((pos - base) / n_chunks);
       const int head = SEL ? seq_unit % p.c.heads : seq_unit;
       const int i0 = SEL ? seq_unit / p.c.heads * p.share : 0;  // the unit's first query
@@ -277,15 +278,17 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
 
       // ---- this warp's groups: G from g0 + (chunk * W + warp) * G
       const int first = g0 + (ca * W + warp) * G;
-      const int* list = SEL ? p.selected + ((long long)b * seq_units + seq_unit) * p.keep : nullptr;
+      const int* list = SEL ? p.selected + ((long long)b * seq_units() + seq_unit) * p.keep : nullptr;
       int g_end = g1;
       if (SEL) {  // the list ends at its first negative entry
-        int n = g1 / per_page;
+        int n = p.keep;
         for (int e = lane; e < n; e += 32)
           if (list[e] < 0) n = e;
         g_end = __reduce_min_sync(~0u, n) * per_page;
       }
-      const int n_it = first < g_end ? min(cb - ca, (g_end - first + W * G - 1) / (W * G)) : 0;
+      // a list that names pages twice, or others than the sequence's, may be longer than the sequence: its last part takes the rest
+      const int most_it = SEL && cb == n_chunks ? 0x7FFFFFFF : cb - ca;
+      const int n_it = first < g_end ? min(most_it, (g_end - first + W * G - 1) / (W * G)) : 0;
       long long src = 0;     // lane i: address of group i % G of step (of a batch of 32 / G) + i / G
       int src_tok = kNoTok;  // and the position of its first token (SEL), which lane (stage * G + group) keeps from the copy on
       int stage_tok = kNoTok;
@@ -738,7 +741,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
       }
       __syncthreads();
       const bool split = ca > 0 || cb < n_chunks;
-      const long long unit = (long long)b * seq_units + seq_unit;
+      const long long unit = (long long)b * seq_units() + seq_unit;
       constexpr int kPart = C::kRows * (D + 2);
       float* part = a.part + (2 * (long long)blockIdx.x + (unit_start > p0 ? 1 : 0)) * kPart;
       auto finish = [&](int r, int d4, float4 v, float top, float sum) {
@@ -841,7 +844,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
       __syncthreads();
     }
     if (!ok) break;
-    base += (long long)n_chunks * seq_units;
+    base += (long long)n_chunks * seq_units();
   }
   if (!ok) {
     // bounded: copies of this warp that were issued and not waited for

@@ -390,6 +390,20 @@ def test_attention_selected_behind_the_sequence(s3b, engine):
     check_attention(s3b, engine, s, s.queries(1, 1), selected, 1)
 
 
+@pytest.mark.parametrize("qtype,d,page", [(2, 64, 16), (3, 128, 16), (8, 256, 32)])
+def test_attention_selected_by_any_list(s3b, engine, qtype, d, page):
+    """Pages named twice count twice; pages behind the sequence, first in the list, take no page's place; lists longer than the
+    sequence, in one block and cut into parts."""
+    s = Sequences(s3b, engine, qtype, d, 1, page, [3 * page - 5, 40 * page], seed=d, width=60)
+    g = torch.Generator().manual_seed(d)
+    for keep in (7, 200):
+        selected = torch.randint(0, 60, (2, 2, 1, keep), generator=g, dtype=torch.int32)
+        selected[0, 0, 0, :4] = torch.tensor([50, 59, 2, 2])
+        selected[0, 0, 0, 4:] = torch.randint(0, 3, (keep - 4,), generator=g, dtype=torch.int32)
+        selected[1, 1, 0, keep - 2:] = -1
+        check_attention(s3b, engine, s, s.queries(2, 2), selected.cuda(), 1)
+
+
 @pytest.mark.parametrize("size", [1e-3, 1.0, 300.0])
 @pytest.mark.parametrize("qtype", TYPES)
 def test_attention_selected_of_values_of_any_size(s3b, engine, qtype, size):
