@@ -820,7 +820,7 @@ class Engine:
     def _call(*fields) -> bytes:
         try:
             return _CALL.pack(*fields)
-        except struct.error as e:
+        except (struct.error, OverflowError) as e:
             raise S3BError(f"an argument is out of its range: {e}") from None
 
     def _sequences(self, what: str, pages, lengths):

@@ -1650,7 +1650,8 @@ int s3b_kv_bounds_values(const s3b_kv_bounds* bounds, const int64_t* pages, int6
   shape.n_pages = bounds->n_pages;
   b.codes = reinterpret_cast<int8_t*>(bounds->codes);
   b.steps = bounds->steps;
-  if (kv_cache_bytes(shape) < 0 || !multiple_of(b.codes, 16) || !multiple_of(b.steps, 4) || !multiple_of(pages, 8) || !multiple_of(out, 16) || n > (1LL << 40))
+  if (kv_cache_bytes(shape) < 0 || !multiple_of(b.codes, 16) || !multiple_of(b.steps, 4) || !multiple_of(pages, 8) || !multiple_of(out, 16) ||
+      n > (1LL << 40) / shape.heads)
     return kErrArg;
   if (n == 0) return kOk;
   if (!pages || !out) return kErrArg;

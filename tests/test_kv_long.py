@@ -120,3 +120,15 @@ def test_numbers_out_of_range_are_refused(s3b, wrong):
             engine.cache_evict(cache, _Strided(0, torch.float32, 1, KV, PAGES * PAGE), pages, lengths, _Strided(0, torch.int32, 1, 3), _Strided(0, torch.int32, 1),
                                _Strided(0, torch.int32, 1, KV, 3), **wrong)
     assert engine._L.calls == 0
+
+
+@pytest.mark.parametrize("scale", [1e300, -1e300])
+def test_a_scale_that_is_no_f32_is_refused(s3b, scale):
+    engine, _ = _calls(s3b)
+    cache = s3b.KVCache(2, PAGES, PAGE, KV, D, data=_Strided(0, torch.uint8, s3b.kv_cache_bytes(2, KV, D, PAGE, PAGES)))
+    q, pages, lengths = _Strided(0, torch.float16, 1, 5, 4, D), _Strided(0, torch.int32, 1, PAGES), _Strided(0, torch.int32, 1)
+    with pytest.raises(s3b.S3BError):
+        engine.cache_attention_selected(cache, q, q, _Strided(0, torch.int32, 1, 3, KV, KEEP), pages, lengths, scale, share=2)
+    with pytest.raises(s3b.S3BError):
+        engine.cache_weights(cache, q, _Strided(0, torch.float32, 1, 5, 4), _Strided(0, torch.float32, 1, KV, PAGES * PAGE), pages, lengths, scale)
+    assert engine._L.calls == 0

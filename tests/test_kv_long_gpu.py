@@ -659,3 +659,35 @@ def test_evict_nothing_kept(s3b, engine):
                        torch.empty(2, 1, 0, dtype=torch.int32, device="cuda"))
     engine.sync()
     assert lengths_out.tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("qtype,d", [(2, 64), (3, 128), (8, 256), (2, 256)])
+@pytest.mark.parametrize("nq", [1, 40, 300])
+def test_memory_that_was_never_written(s3b, engine, qtype, d, nq):
+    """A cache in memory of all ones (scales of NaN) gives the same bits as one in zeros, wherever no token lies; so do the places that
+    an eviction into such a cache leaves."""
+    heads, page, n, most, keep = 2, 48, 437, 12, 100
+    pages, lengths = torch.arange(most, dtype=torch.int32, device="cuda")[None], torch.tensor([n], dtype=torch.int32, device="cuda")
+    results = []
+    for fill in (0, 255):
+        g = torch.Generator(device="cuda").manual_seed(d + nq)
+        c, to = (s3b.KVCache(qtype, most, page, heads, d, data=torch.full((s3b.kv_cache_bytes(qtype, heads, d, page, most),), fill, dtype=torch.uint8, device="cuda"))
+                 for _ in "ab")
+        k, v = (torch.randn(n, heads, d, device="cuda", generator=g).half() for _ in "kv")
+        engine.cache_write(c, k, v, torch.arange(n, device="cuda"))
+        q, bounds = torch.randn(1, nq, heads, d, device="cuda", generator=g).half(), s3b.KVBounds(c)
+        out, dense, again = torch.empty_like(q), torch.empty_like(q), torch.empty_like(q)
+        lse, weights = torch.empty(1, nq, heads, device="cuda"), torch.zeros(1, heads, most * page, device="cuda")
+        selected, scores = torch.empty(1, nq, heads, 6, dtype=torch.int32, device="cuda"), torch.empty(1, nq, heads, most, device="cuda")
+        kept, length = torch.empty(1, heads, keep, dtype=torch.int32, device="cuda"), torch.empty(1, dtype=torch.int32, device="cuda")
+        engine.cache_attention(c, q, dense, pages, lengths, d ** -0.5, lse=lse)
+        engine.cache_bounds(c, bounds, pages, lengths)
+        engine.cache_select(bounds, q, selected, pages, lengths, scores=scores)
+        engine.cache_attention_selected(c, q, out, selected, pages, lengths, d ** -0.5)
+        engine.cache_weights(c, q, lse, weights, pages, lengths, d ** -0.5)
+        engine.cache_evict(c, weights, pages, lengths, pages, length, kept, to=to)
+        engine.cache_attention(to, q, again, pages, length, d ** -0.5)
+        engine.sync()
+        assert all(torch.isfinite(x).all() for x in (out, weights, again))
+        results.append((out, lse, weights, selected, scores, bounds.codes, bounds.steps, kept, again))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
