@@ -200,7 +200,7 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Fetch fetch, Make
     } else {
       at += min(q, left);
     }
-    if (taken) emit(at, i);
+    if (taken && at < k) emit(at, i);  // more only where the caller changes the values meanwhile
   });
   if (CL > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
