@@ -32,7 +32,8 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
 // c+ = max(c, 0), c- = min(c, 0), two products of 8-bit codes (16 pages x 32 channels x 8 rows an instruction), exact in 32 bits;
 // then two f32 products, each rounded, so that the choice is the same whatever the order. Lane (g, t) holds 16 channels of 64 as
 // the contraction's share of its rows (pages g, g + 8; query row g): whole 16-byte words of both. 16 warps where there is a CTA or
-// less for each SM, else 8, so that several share one (32 x 8 lists of 256 pages: 14.8 us with 16, 11.5 with 8).
+// less for each SM, else 8, so that several share one (32 x 8 lists of 256 pages: 14.8 us with 16, 11.5 with 8), and
+// fewer for many lists of few pages (select_plan).
 // Measured: 8 lists of 301 pages, d = 64: 7.2 us; 32 x 8 lists of up to 256 pages, d = 128: 8.8 us (the call's host time) for 9.6 MB;
 // 2 lists of 16384 pages, d = 64: 13.6 us. A chain of latencies bounds it: length, table, codes, the votes or rounds of the
 // choice. Products are 2% of it.
@@ -227,11 +228,19 @@ struct SelectPlan {
 };
 // CTAs of a unit: about 512 pages each (two steps of 16 for each warp), on half of the SMs: large clusters find no place on all of
 // them (8 lists of 8192 pages: 24.2 us in clusters of 16, 14.4 of 8; 16 lists of 16384: 32.5 of 8, 25.8 of 4).
+// Many lists of few pages: small CTAs, as many warps as two keys a lane and a list's latencies ask for, more of them on an SM (with 8
+// warps and so: 68880 lists of one page 296 -> 105 us, 4096 of 64 pages 51 -> 27 in one warp; 16000 of 100 pages 184 -> 93 in two;
+// 8192 of 250 pages 127 -> 103 in four; but 256 of 100 pages 7.2 -> 9.0).
 bool select_plan(const KvAttnParams& p, int sms, SelectPlan* plan) {
   const int rows = p.share * (p.heads / p.c.heads), d = p.c.d;
   int cl = 1;
   while (cl < 16 && cl * 512LL < p.max_pages && kv_attention_units(p) * cl * 4 <= sms) cl *= 2;
   auto of = [&](int n) {
+    if (n == 1 && kv_attention_units(p) > 4LL * sms) {
+      if (p.max_pages <= 64) return select_for<1, 32>(d, rows);
+      if (p.max_pages <= 128) return select_for<1, 64>(d, rows);
+      if (p.max_pages <= 256) return select_for<1, 128>(d, rows);
+    }
     return n == 1 ? (kv_attention_units(p) <= sms ? select_for<1, 512>(d, rows) : select_for<1, 256>(d, rows))
            : n == 2 ? select_for<2, 512>(d, rows) : n == 4 ? select_for<4, 512>(d, rows)
            : n == 8 ? select_for<8, 512>(d, rows) : select_for<16, 512>(d, rows);

@@ -23,8 +23,9 @@ __device__ __forceinline__ uint32_t cluster_load(const uint32_t* p, uint32_t ran
 template <int T>
 struct TopShared {
   static constexpr int kCopies = T >= 1024 ? 16 : 8;
-  uint32_t hist[256 * kCopies];  // a digit's counts, apart for lanes that differ modulo kCopies: keys of one size share their digits
-  uint32_t total[2][256];        // of this CTA, by digit; two of them, so that one round's may still be read during the next
+  static constexpr int kDigits = T >= 256 ? 256 : 1;  // small blocks take few keys, by votes alone
+  uint32_t hist[kDigits * kCopies];  // a digit's counts, apart for lanes that differ modulo kCopies: keys of one size share their digits
+  uint32_t total[2][kDigits];        // of this CTA, by digit; two of them, so that one round's may still be read during the next
   uint32_t warp_sum[8];
   uint32_t above[T / 32], equal[T / 32], cta[2];
   uint32_t digit, left, count;
@@ -41,8 +42,8 @@ struct TopShared {
 // write it. 256 keys, 256 threads: see the branch for few keys.
 template <int T, int CL, typename Fetch, typename Make, typename Key, typename Emit>
 __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Fetch fetch, Make make, Key key, Emit emit) {
-  constexpr int W = T / 32, C = TopShared<T>::kCopies, P = T / 256;  // P threads a digit
-  static_assert(T >= 256 && T % 256 == 0 && C % P == 0, "threads of top_select");
+  constexpr int W = T / 32, C = TopShared<T>::kCopies, P = T >= 256 ? T / 256 : 1;  // P threads a digit
+  static_assert(T >= 256 ? T % 256 == 0 && C % P == 0 : T % 32 == 0 && CL == 1, "threads of top_select");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows_all = (n + 31) / 32, rows_warp = (rows_all + W - 1) / W;
   const int from = min(warp * rows_warp, rows_all) * 32, to = min(n, from + rows_warp * 32);  // of this warp's run
@@ -66,7 +67,7 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Fetch fetch, Make
   auto each = [&](auto&& f) { each_of(key, std::integral_constant<int, 4>(), f); };
   uint32_t left = k;
   uint32_t from_above = 1, from_equal = 0;  // keys >= from_above are taken, then the first of those >= from_equal
-  if (CL == 1 && n <= 2 * T) {
+  if (T < 256 || (CL == 1 && n <= 2 * T)) {
     // Few keys, one or two a thread: the threshold bit by bit, by the block's votes (some 50 cycles each, and most searches end well
     // before the last bit: 256 keys in 1000 cycles where two rounds below take 2500).
     const bool two = n > T;  // a run is one row, or two
@@ -89,7 +90,7 @@ __device__ void top_select(TopShared<T>& s, int n, uint32_t k, Fetch fetch, Make
       from_above = from_equal + 1;
       left = k - votes(from_above);
     }
-  } else {
+  } else if constexpr (T >= 256) {
 #pragma unroll
     for (int e = 0; e < 256 * C / T; ++e) s.hist[e * T + threadIdx.x] = 0;
     uint32_t prefix = 0;

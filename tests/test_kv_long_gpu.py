@@ -238,6 +238,19 @@ def test_select_of_many_pages(s3b, engine, page, length, keep, sink, recent):
     check_select(s3b, engine, s, s.queries(2, 4), keep, 2, sink, recent, True, 0)
 
 
+@pytest.mark.parametrize("d,heads,kv,nq,share", [(64, 2, 2, 151, 1), (128, 16, 2, 300, 2), (256, 4, 1, 601, 2), (64, 4, 1, 1201, 4), (64, 4, 1, 2400, 8)])
+@pytest.mark.parametrize("pages", [1, 40, 64, 65, 128, 129, 256, 257])
+def test_select_of_many_lists(s3b, engine, d, heads, kv, nq, share, pages):
+    """More lists than four an SM, whose blocks are as small as their pages allow; some of them of equal pages."""
+    s = Sequences(s3b, engine, 2, d, kv, 16, [16 * pages - 3, 8 * pages], seed=pages + d)
+    bounds = s3b.KVBounds(s.cache)
+    engine.cache_bounds(s.cache, bounds, s.pages, s.lengths)
+    engine.sync()
+    bounds.codes[::3] = bounds.codes[0]
+    bounds.steps[::3] = bounds.steps[0]
+    check_select(s3b, engine, s, s.queries(nq, heads), 1 + pages // 3, share, min(1, pages // 3), 0, True, 0, bounds)
+
+
 def test_select_ties(s3b, engine):
     """Equal pages: the lower ones; a query of zeros scores all pages 0."""
     s = Sequences(s3b, engine, 2, 64, 1, 16, [16 * 900], seed=5)
