@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
   float* s_f = s_l + W * C::kRows;
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_f + W * C::kRows);
   __shared__ long long s_total, s_ctas, s_base, s_p0, s_p1;
-  __shared__ int s_b, s_abort_word, s_last;
+  __shared__ int s_b, s_abort_word, s_last, s_empty;
   volatile int* s_abort = &s_abort_word;
   static_assert(W * NS * 8 <= 1024, "barriers of rows_kernel");
 
@@ -174,15 +174,17 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
   // total chunks, this CTA's share of them and the sequence in which it begins
   if (warp == 0) {
     long long total = 0;
-    int most = 0, g0, g1;
+    int most = 0, least = 1, g0, g1;
     for (int b = lane; b < p.batch; b += 32) {
       const int n = chunks_of(b, &g0, &g1);
       total += n;
       most = max(most, n);
+      least = min(least, n);
     }
 #pragma unroll
     for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(~0u, total, x);
     most = __reduce_max_sync(~0u, most);
+    least = __reduce_min_sync(~0u, least);
     total *= seq_units();
     long long ctas = min((long long)gridDim.x, total), base = 0, p0 = 0, p1 = 0;
     int found = -1;
@@ -225,18 +227,25 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
       s_p0 = p0;
       s_p1 = p1;
       s_b = found;
+      s_empty = least <= 0;
     }
   }
   __syncthreads();
 
-  // sequences of which no query sees a token
-  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    int g0, g1;
-    if (chunks_of(b, &g0, &g1)) continue;
-    for (int e = threadIdx.x; e < p.nq * p.heads * (D / 4); e += 32 * W) {
-      const int h = e / (D / 4) % p.heads, i = e / (D / 4) / p.heads;
-      store_out(p, b * p.o_b + i * p.o_n + h * p.o_h + e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-      if (p.lse && e % (D / 4) == 0) p.lse[((long long)b * p.nq + i) * p.heads + h] = -INFINITY;
+  // Sequences of which no query sees a token: their rows in pieces of kClear, which the blocks take in turn. With lists a sequence has
+  // any number of rows (one of 4096 queries of 32 heads of 128 beside one that reads lists of 32 pages: 2.72 ms by one block, 0.86 so).
+  constexpr int kClear = 128;
+  if (s_empty) {
+    const int rows = p.nq * p.heads, pieces = (rows - 1) / kClear + 1;
+    for (long long x = blockIdx.x; x < (long long)p.batch * pieces; x += gridDim.x) {
+      const int b = (int)(x / pieces), r0 = (int)(x - (long long)b * pieces) * kClear;
+      int g0, g1;
+      if (chunks_of(b, &g0, &g1)) continue;
+      for (int e = threadIdx.x; e < min(kClear, rows - r0) * (D / 4); e += 32 * W) {
+        const int r = r0 + e / (D / 4), i = r / p.heads, h = r - i * p.heads;
+        store_out(p, b * p.o_b + i * p.o_n + h * p.o_h + e % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+        if (p.lse && e % (D / 4) == 0) p.lse[((long long)b * p.nq + i) * p.heads + h] = -INFINITY;
+      }
     }
   }
   const long long p0 = s_p0, p1 = s_p1, total = s_total, ctas = s_ctas;

@@ -1,0 +1,76 @@
+"""Long caches at the edges of what the calls take. Plain forms, tolerances and inputs as in test_kv_long_gpu.py."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+from test_kv_long_gpu import Sequences  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+def needs(gigabytes):
+    if torch.cuda.mem_get_info()[0] < gigabytes * 2 ** 30:
+        pytest.skip(f"needs {gigabytes} GB of device memory")
+
+
+# ---------------------------------------------------------------- empty sequences
+def test_an_empty_sequence_of_2_to_the_25_queries(s3b, engine):
+    """More than 2^31 pieces of four outputs: all rows are zero, all ln sums -inf."""
+    needs(22)
+    nq, d, share = 2 ** 25 + 3, 256, 16
+    cache = s3b.KVCache(2, 1, 16, 1, d)
+    q = torch.ones(1, 1, 1, d, dtype=torch.float16, device="cuda").expand(1, nq, 1, d)
+    out, lse = torch.full((1, nq, 1, d), 9.0, dtype=torch.float16, device="cuda"), torch.full((1, nq, 1), 9.0, device="cuda")
+    selected = torch.zeros(1, -(-nq // share), 1, 1, dtype=torch.int32, device="cuda")
+    engine.cache_attention_selected(cache, q, out, selected, torch.zeros(1, 1, dtype=torch.int32, device="cuda"),
+                                    torch.zeros(1, dtype=torch.int32, device="cuda"), 0.1, share=share, lse=lse)
+    engine.sync()
+    assert (lse == -math.inf).all()
+    words = out.view(-1).view(torch.int64)
+    for i in range(0, len(words), 2 ** 28):
+        assert not words[i:i + 2 ** 28].any()
+    del out, words
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("qtype,d,heads,kv,nq,share,lengths", [
+    (2, 128, 32, 8, 2050, 4, [300, 0, 170]), (3, 64, 3, 1, 4099, 10, [0, 0, 65, 0]), (8, 256, 2, 2, 3001, 16, [64, 0]), (2, 64, 1, 1, 127, 1, [0, 5, 0]),
+    (2, 64, 1, 1, 129, 1, [0, 0])])
+@pytest.mark.parametrize("out_type", [torch.float16, torch.float32])
+def test_empty_sequences_beside_others(s3b, engine, qtype, d, heads, kv, nq, share, lengths, out_type):
+    """Rows of empty sequences are zero, those of the others as without them, and nothing between the rows is written."""
+    s = Sequences(s3b, engine, qtype, d, kv, 16, lengths, seed=nq)
+    q, scale = s.queries(nq, heads), d ** -0.5
+    batch, blocks, keep = len(lengths), -(-nq // share), 3
+    selected = torch.randint(0, 4, (batch, blocks, kv, keep), generator=torch.Generator().manual_seed(1), dtype=torch.int32).cuda()
+    selected.clamp_(max=s.pages.shape[1] - 1)
+    wide = torch.full((batch, nq, heads + 1, d + 16), 9.0, dtype=out_type, device="cuda")
+    lse = torch.full((batch, nq, heads), 9.0, device="cuda")
+    out = wide[:, :, :heads, 8:d + 8]
+    engine.cache_attention_selected(s.cache, q, out, selected, s.pages, s.lengths, scale, share=share, lse=lse)
+    engine.sync()
+    for b, n in enumerate(lengths):
+        if not n:
+            assert (out[b] == 0).all() and (lse[b] == -math.inf).all()
+            continue
+        alone, alone_lse = torch.empty(1, nq, heads, d, dtype=out_type, device="cuda"), torch.empty(1, nq, heads, device="cuda")
+        engine.cache_attention_selected(s.cache, q[b:b + 1], alone, selected[b:b + 1], s.pages[b:b + 1], s.lengths[b:b + 1], scale, share=share, lse=alone_lse)
+        engine.sync()
+        # blocks may share a unit in another way: f32 sums in another order, then the output's rounding
+        assert (alone[0].double() - out[b].double()).norm() <= 2.0 ** -10 * alone[0].double().norm()
+        assert (alone_lse[0] - lse[b]).abs().max() <= 2.0 ** -16
+    assert (wide[:, :, heads] == 9).all() and (wide[..., :8] == 9).all() and (wide[..., d + 8:] == 9).all()
+
+
+@pytest.mark.parametrize("nq,heads,lengths", [(1, 8, [0, 40, 0]), (7, 32, [0] * 5 + [100] + [0] * 300), (32, 4, [0])])
+def test_empty_sequences_of_the_dense_attention(s3b, engine, nq, heads, lengths):
+    """The same rows by the call over all pages, which shares the kernel."""
+    s = Sequences(s3b, engine, 2, 64, 4, 16, lengths, seed=nq)
+    q = s.queries(nq, heads)
+    out, lse = torch.full(q.shape, 9.0, device="cuda"), torch.full(q.shape[:3], 9.0, device="cuda")
+    engine.cache_attention(s.cache, q, out, s.pages, s.lengths, 0.1, lse=lse)
+    engine.sync()
+    none = s.lengths == 0
+    assert (out[none] == 0).all() and (lse[none] == -math.inf).all()
+    assert torch.isfinite(lse[~none]).all() and (out[~none] != 9).all()
