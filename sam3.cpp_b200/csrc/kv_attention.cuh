@@ -20,6 +20,11 @@ __device__ __forceinline__ int sequence_length(const KvAttnParams& p, int b, int
   return n;
 }
 
+// Pages of a sequence of len tokens: unsigned, the sum passes 2^31 for the longest of them.
+__device__ __forceinline__ int sequence_pages(const KvAttnParams& p, int len) {
+  return (int)((unsigned)(len + (unsigned)p.c.page_size - 1) / (unsigned)p.c.page_size);
+}
+
 // Tokens [lo, hi) that query i of a sequence of len tokens sees.
 __device__ __forceinline__ void row_span(const KvAttnParams& p, int len, int i, int* lo, int* hi) {
   *lo = 0;

@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
   auto chunks_of = [&](int b, int* g0, int* g1) -> int {
     if (SEL) {  // groups of the longest list that names each page of the sequence once
       *g0 = 0;
-      *g1 = min(p.keep, (sequence_length(p, b, err) + p.c.page_size - 1) / p.c.page_size) * per_page;
+      *g1 = min(p.keep, sequence_pages(p, sequence_length(p, b, err))) * per_page;
     } else {
       group_span(p, sequence_length(p, b, err), 0, p.nq - 1, g0, g1);
     }
@@ -308,10 +308,12 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
           int entry = gi / per_page;
           if (SEL) {
             entry = list[entry];
-            if (entry < (len + p.c.page_size - 1) / p.c.page_size) {
+            if (entry >= p.max_pages) {
+              atomicCAS(err, 0, kDevErrIndex);
+              entry = 0;
+            } else if (entry * p.c.page_size < len) {
               src_tok = entry * p.c.page_size + gi % per_page * 16;
             } else {  // behind the sequence's last page: nothing of it is seen
-              if (entry >= p.max_pages) atomicCAS(err, 0, kDevErrIndex);
               entry = 0;
             }
           }

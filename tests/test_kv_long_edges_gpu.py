@@ -74,3 +74,36 @@ def test_empty_sequences_of_the_dense_attention(s3b, engine, nq, heads, lengths)
     none = s.lengths == 0
     assert (out[none] == 0).all() and (lse[none] == -math.inf).all()
     assert torch.isfinite(lse[~none]).all() and (out[~none] != 9).all()
+
+
+# ---------------------------------------------------------------- positions near 2^31
+def test_a_sequence_of_nearly_2_to_the_31_tokens(s3b, engine):
+    """The last page's end, rounded up to whole pages, passes 2^31. All entries of the table name two pages in turn."""
+    page, width = 8208, 261632
+    length = page * width  # 2^31 - 8192, the longest that there is
+    cache = s3b.KVCache(2, 2, page, 1, 64)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(2 * page, 1, 64, device="cuda", generator=g).half() for _ in "kv")
+    engine.cache_write(cache, k, v, torch.arange(2 * page, device="cuda"))
+    pages = (torch.arange(width, dtype=torch.int32, device="cuda") % 2)[None]
+    lengths = torch.tensor([length], dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 2, 1, 64, device="cuda", generator=g).half()
+    selected = torch.tensor([[0, width - 1, -1], [width - 1, width - 2, 7]], dtype=torch.int32, device="cuda")[None, :, None]
+    out, lse = torch.full(q.shape, 9.0, device="cuda"), torch.full((1, 2, 1), 9.0, device="cuda")
+    # with a window, query 0 sees the last 9000 tokens up to the one before the last
+    for window in (0, 9000):
+        engine.cache_attention_selected(cache, q, out, selected, pages, lengths, 0.125, causal=True, window=window, lse=lse)
+        engine.sync()
+        held = [torch.empty(2 * page, 1, 64, device="cuda") for _ in "kv"]
+        engine.cache_read(cache, torch.arange(2 * page, device="cuda"), *held)
+        engine.sync()
+        for i in range(2):
+            names = [x for x in selected[0, i, 0].tolist() if x >= 0]
+            at = torch.cat([torch.arange(page, device="cuda") + x * page for x in names])
+            hi = length - 1 + i
+            seen = (at < hi) & (at >= (hi - window if window else 0))
+            row = (at // page % 2 * page + at % page)[seen]
+            z = held[0][row, 0].double() @ q[0, i, 0].double() * 0.125
+            want = z.softmax(0) @ held[1][row, 0].double()
+            assert (out[0, i, 0] - want).norm() <= 2.0 ** -10 * want.norm()  # at most two roundings to f16, of half a step each
+            assert abs(lse[0, i, 0].item() - z.logsumexp(0).item()) <= 2.0 ** -16
