@@ -650,6 +650,7 @@ int s3b_kv_bounds_values(const s3b_kv_bounds* bounds, const int64_t* pages, int6
  * be shorter) and each head of the cache:
  *   selected [batch][ceil(nq / share)][heads of the cache][keep]: places in the
  *            page table; a list ends at its first negative entry
+ *            (keep * page_size at most 2^31 - 8192)
  * At most 32 rows (share x heads / heads of the cache; 16 at d = 256) have a list.
  * Calls of one context use its workspace: a captured one is replayed on the
  * context's stream, or ordered with its other calls. */
@@ -758,7 +759,7 @@ typedef struct s3b_kv_evict {
  * and scales are copied as they are. A head's token at a place need not be the same as
  * another head's. The source pages are left as they are, places behind the last token
  * too. A page of pages_out outside its cache is not written, and the next s3b_sync
- * returns S3B_ERR_DEVICE. sink + recent <= keep. */
+ * returns S3B_ERR_DEVICE. sink + recent <= keep <= 2^31 - 8192. */
 int s3b_op_cache_evict(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_call* call, const s3b_kv_evict* evict);
 
 /* ---------------------------------------------------------------- host format helpers */

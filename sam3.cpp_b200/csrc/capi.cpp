@@ -1603,6 +1603,9 @@ static int kv_queries(s3b_ctx* ctx, const char* what, KvAttnParams* p, const s3b
 static int kv_lists(s3b_ctx* ctx, const char* what, KvAttnParams* p, const s3b_kv_call* call) {
   const int keep = call->keep, share = call->share;
   if (keep < 1 || share < 1) return set_error(ctx, kErrArg, "%s: lists of %d pages for blocks of %d queries", what, keep, share);
+  // a list's groups of 16 tokens, and its places, are counted in 32 bits
+  if ((long long)keep * p->c.page_size > kMaxCacheTokens)
+    return set_error(ctx, kErrUnsupported, "%s: a list may name %lld tokens at most", what, kMaxCacheTokens);
   const long long rows = (long long)std::min(share, std::max(p->nq, 1)) * (p->heads / p->c.heads);
   if (rows > kv_attention_most_rows(p->c.d))
     return set_error(ctx, kErrUnsupported, "%s: %lld rows share a list, at most %d may", what, rows, kv_attention_most_rows(p->c.d));
@@ -1732,9 +1735,6 @@ int s3b_op_cache_attention_selected(s3b_ctx* ctx, const s3b_kv_cache* cache, con
   if ((rc = kv_queries(ctx, what, &p, call))) return rc;
   if ((rc = kv_lists(ctx, what, &p, call))) return rc;
   if ((rc = kv_scale(ctx, what, &p, call->scale))) return rc;
-  // a list's groups of 16 tokens are counted in 32 bits
-  if ((long long)p.keep * p.c.page_size > kMaxCacheTokens)
-    return set_error(ctx, kErrUnsupported, "%s: a list may name %lld tokens at most", what, kMaxCacheTokens);
   if (!rows_aligned(call->out, call->out_f32 ? 4 : 2, call->o_b, call->o_n, call->o_h))
     return set_error(ctx, kErrArg, "%s: rows must start on 16-byte boundaries", what);
   if (!multiple_of(call->lse, 4)) return set_error(ctx, kErrArg, "%s: lse must be 4-byte aligned", what);
@@ -1827,6 +1827,7 @@ int s3b_op_cache_evict(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_cal
   float* weights_out = evict->weights_out;
   if (keep < 0 || sink < 0 || recent < 0 || (long long)sink + recent > keep)
     return set_error(ctx, kErrArg, "cache_evict: %d first and %d last tokens of %d", sink, recent, keep);
+  if (keep > kMaxCacheTokens) return set_error(ctx, kErrUnsupported, "cache_evict: %lld tokens at most may be kept", kMaxCacheTokens);
   const long long new_pages = ((long long)keep + e.to.page_size - 1) / e.to.page_size;
   if (batch > 1 && out_stride < new_pages)
     return set_error(ctx, kErrArg, "cache_evict: rows of %lld new pages hold no %lld", (long long)out_stride, new_pages);

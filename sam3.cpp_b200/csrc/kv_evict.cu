@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const __grid_constant_
   if (head == 0 && rank == 0 && threadIdx.x == 0) a.e.lengths_out[b] = m;
   if (keep == 0) return;
   if (len <= keep) {
-    for (int i = rank * kThreads + threadIdx.x; i < keep; i += CL * kThreads) kept[i] = i < len ? i : -1;
+    for (long long i = rank * kThreads + threadIdx.x; i < keep; i += CL * kThreads) kept[i] = i < len ? (int)i : -1;
     return;
   }
   const int share = CL > 1 ? (int)(((long long)len + 32 * CL - 1) / (32 * CL)) * 32 : len;

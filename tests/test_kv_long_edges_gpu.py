@@ -5,6 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 from test_kv_long_gpu import Sequences  # noqa: E402
+from test_kv_long_run_gpu import raw  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +108,37 @@ def test_a_sequence_of_nearly_2_to_the_31_tokens(s3b, engine):
             want = z.softmax(0) @ held[1][row, 0].double()
             assert (out[0, i, 0] - want).norm() <= 2.0 ** -10 * want.norm()  # at most two roundings to f16, of half a step each
             assert abs(lse[0, i, 0].item() - z.logsumexp(0).item()) <= 2.0 ** -16
+
+
+# ---------------------------------------------------------------- the longest lists
+@pytest.mark.parametrize("call,keep", [("evict", 2 ** 31 - 1), ("evict", 2 ** 31 - 8191), ("select", 2 ** 31 - 1), ("select", 2 ** 27), ("select", 2 ** 27 - 511),
+                                       ("attend", 2 ** 31 - 1), ("attend", 2 ** 27 - 511)])
+def test_longer_lists_than_tokens_are_refused(raw, engine, call, keep):  # noqa: F811
+    before = {name: x.clone() for name, x in raw.o.items() if x is not None}
+    assert getattr(raw, call)(keep=keep) == -6
+    engine.sync()
+    for name, x in before.items():
+        assert torch.equal(raw.o[name].view(torch.uint8), x.view(torch.uint8)), name
+
+
+def test_the_longest_eviction(s3b, engine):
+    """Room for 2^31 - 8192 kept positions of a short sequence: all behind the last are -1, and nothing around them is written."""
+    needs(14)
+    keep, guard, n, page = 2 ** 31 - 8192, 1 << 16, 40, 1 << 20
+    s = Sequences(s3b, engine, 2, 64, 1, 16, [n], seed=1)
+    to = s3b.KVCache(2, 1, page, 1, 64)
+    around = torch.full((keep + 2 * guard,), 9, dtype=torch.int32, device="cuda")
+    kept = around[guard:guard + keep].view(1, 1, keep)
+    pages_out = torch.zeros(1, 2048, dtype=torch.int32, device="cuda")
+    lengths_out = torch.zeros(1, dtype=torch.int32, device="cuda")
+    engine.cache_evict(s.cache, torch.rand(1, 1, 48, device="cuda"), s.pages, s.lengths, pages_out, lengths_out, kept, to=to)
+    engine.sync()
+    assert lengths_out.item() == n and kept[0, 0, :n].tolist() == list(range(n))
+    assert (around[:guard] == 9).all() and (around[guard + keep:] == 9).all()
+    for i in range(n, keep, 2 ** 29):
+        assert (kept[0, 0, i:i + 2 ** 29] == -1).all()
+    k, v = s.rows(0)
+    moved = [torch.empty_like(k) for _ in "kv"]
+    engine.cache_read(to, torch.arange(n, device="cuda"), *moved)
+    engine.sync()
+    assert torch.equal(moved[0], k) and torch.equal(moved[1], v)
