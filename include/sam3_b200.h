@@ -702,8 +702,8 @@ int s3b_op_cache_bounds(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_bo
  *   scores  f32 [batch][blocks][heads of the cache][max_pages], -inf for pages that
  *           the block does not see, or NULL
  * keep >= 1, sink + recent <= keep. The call only enqueues work; a workspace (of
- * lists over very many pages) is the context's, as that of s3b_op_cache_attention,
- * and the same holds under capture. */
+ * lists over very many pages: 256 MB, or one list's scores) is the context's, as
+ * that of s3b_op_cache_attention, and the same holds under capture. */
 int s3b_op_cache_select(s3b_ctx* ctx, const s3b_kv_bounds* bounds, const s3b_kv_call* call, int sink, int recent,
                         float* scores);
 

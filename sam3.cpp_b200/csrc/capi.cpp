@@ -1713,15 +1713,20 @@ int s3b_op_cache_select(s3b_ctx* ctx, const s3b_kv_bounds* bounds, const s3b_kv_
   if (units * std::max(p.max_pages, 1) > (1LL << 40))
     return set_error(ctx, kErrUnsupported, "cache_select: %lld lists over %d pages", units, p.max_pages);
   const int sms = num_sms();
+  long long at_once = units;  // lists of a launch
   if (!all && kv_select_needs_scores(p, sms)) {
+    // scores go by the table's width: as many lists at a time as 256 MB hold, by launches that use them in turn
+    at_once = std::min(units, std::max(1LL, (64LL << 20) / p.max_pages));
     bool grown;
-    DevBuf* buf = graph_buf(ctx, "kv_select_scores", power_of_two((size_t)units * p.max_pages * 4, 1 << 20), stream_capturing(ctx), &grown, &rc);
+    DevBuf* buf = graph_buf(ctx, "kv_select_scores", power_of_two((size_t)at_once * p.max_pages * 4, 1 << 20), stream_capturing(ctx), &grown, &rc);
     if (rc) return rc;
     scores = buf->as<float>();
   }
-  rc = kv_select(p, b, sink, recent, scores, all, call->selected, sms, ctx->d_err, ctx->stream);
-  if (rc) return set_error(ctx, launcher_status_code(rc), "cache_select launch failed (%d)", rc);
-  count_launch(ctx);
+  for (long long first = 0; first < units; first += at_once) {
+    rc = kv_select(p, b, sink, recent, scores, all, call->selected, first, std::min(at_once, units - first), sms, ctx->d_err, ctx->stream);
+    if (rc) return set_error(ctx, launcher_status_code(rc), "cache_select launch failed (%d)", rc);
+    count_launch(ctx);
+  }
   return kOk;
 }
 

@@ -434,9 +434,10 @@ int kv_bounds(const KvAttnParams& p, const KvBounds& out, long long recent, int*
 // f32 [n][heads][2][d] of the pages (shape: heads, d, n_pages).
 int kv_bounds_values(const KvCache& shape, const KvBounds& bounds, const long long* pages, long long n, float* out, cudaStream_t st);
 // Chooses p.keep pages for each block of p.share queries and key / value head (p: queries, pages, lengths, masks; of p.c the
-// shape). scores: [units][max_pages], of all pages with `all`, else a workspace, or none unless kv_select_needs_scores.
-int kv_select(const KvAttnParams& p, const KvBounds& bounds, int sink, int recent, float* scores, bool all, int* selected, int sms,
-              int* err, cudaStream_t st);
+// shape): the n lists from `first` on. scores: [units][max_pages], of all pages with `all`, else a workspace [n][max_pages], or none
+// unless kv_select_needs_scores.
+int kv_select(const KvAttnParams& p, const KvBounds& bounds, int sink, int recent, float* scores, bool all, int* selected, long long first,
+              long long n, int sms, int* err, cudaStream_t st);
 bool kv_select_needs_scores(const KvAttnParams& p, int sms);
 
 // s3b_op_cache_weights: w = decay * w + sum over rows of exp(scale q k - lse) (p: everything but out; p.lse is read).

@@ -14,7 +14,8 @@ struct SelectArgs {
   KvAttnParams p;  // c: heads, d, page_size, n_pages; q; pages, lengths; share, keep; causal, window
   KvBounds bounds;
   int sink, recent;
-  float* scores;   // [units][max_pages], or none
+  int first;       // the launch's first unit
+  float* scores;   // [units][max_pages] with `all`, else from the launch's first on, or none
   bool all;        // they are wanted, of all pages
   int* selected;   // [units][keep]
   int keys;        // room for so many in a CTA's shared memory; those of more pages are made from the scores again
@@ -46,7 +47,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) select_kernel(const 
   __shared__ float s_step[NT * 8];
   const KvAttnParams& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int unit = blockIdx.x / CL;
+  const int in_launch = blockIdx.x / CL, unit = a.first + in_launch;
   const int blocks = (p.nq - 1) / p.share + 1;
   const int head = unit % p.c.heads, b = unit / p.c.heads / blocks;
   const int i0 = unit / p.c.heads % blocks * p.share, i1 = min(i0 + p.share, p.nq);
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) select_kernel(const 
   const int share = CL > 1 ? ((n + CL - 1) / CL + 31) / 32 * 32 : n;
   const int begin = pa + (int)min((long long)n, (long long)rank * share), end = min(pe, begin + share);
   int* selected = a.selected + (long long)unit * p.keep;
-  float* scores = a.scores + (long long)unit * p.max_pages;
+  float* scores = a.scores + (long long)(a.all ? unit : in_launch) * p.max_pages;
   const bool trivial = n <= p.keep, in_smem = share <= a.keys;
   if (trivial && rank == 0)
     for (int e = threadIdx.x; e < p.keep; e += kThreads) selected[e] = e < n ? pa + e : -1;
@@ -260,13 +261,13 @@ bool kv_select_needs_scores(const KvAttnParams& p, int sms) {
   return !select_plan(p, sms, &plan) || plan.share > kMostKeys;
 }
 
-int kv_select(const KvAttnParams& p, const KvBounds& bounds, int sink, int recent, float* scores, bool all, int* selected, int sms,
-              int* err, cudaStream_t st) {
+int kv_select(const KvAttnParams& p, const KvBounds& bounds, int sink, int recent, float* scores, bool all, int* selected, long long first,
+              long long n, int sms, int* err, cudaStream_t st) {
   SelectPlan plan;
   if (!select_plan(p, sms, &plan)) return -13;
-  const long long grid = kv_attention_units(p) * plan.cl;
+  const long long grid = n * plan.cl;
   if (grid > 0x7fffffffLL) return -2;
-  const SelectArgs a{p, bounds, sink, recent, scores, all, selected, (int)std::min<long long>(plan.share, kMostKeys)};
+  const SelectArgs a{p, bounds, sink, recent, (int)first, scores, all, selected, (int)std::min<long long>(plan.share, kMostKeys)};
   return launch_clusters(plan.k.kernel, (unsigned)grid, plan.k.threads, (size_t)a.keys * 4, plan.cl, st, a, err);
 }
 

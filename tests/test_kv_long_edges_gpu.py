@@ -4,7 +4,7 @@ import math
 import pytest
 
 torch = pytest.importorskip("torch")
-from test_kv_long_gpu import Sequences  # noqa: E402
+from test_kv_long_gpu import Sequences, plain_choice, plain_scores  # noqa: E402
 from test_kv_long_run_gpu import raw  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
@@ -108,6 +108,64 @@ def test_a_sequence_of_nearly_2_to_the_31_tokens(s3b, engine):
             want = z.softmax(0) @ held[1][row, 0].double()
             assert (out[0, i, 0] - want).norm() <= 2.0 ** -10 * want.norm()  # at most two roundings to f16, of half a step each
             assert abs(lse[0, i, 0].item() - z.logsumexp(0).item()) <= 2.0 ** -16
+
+
+# ---------------------------------------------------------------- how a choice holds its keys
+class Bounded:
+    """Sequences over one page table of `pages` pages, of which only random bounds are looked at."""
+
+    def __init__(self, s3b, heads, d, pages, lengths, seed=0):
+        self.heads, self.d, self.page, self.lens = heads, d, 16, lengths
+        self.g = torch.Generator(device="cuda").manual_seed(seed)
+        self.cache = s3b.KVCache(2, pages, 16, heads, d)
+        self.pages = torch.randperm(pages, device="cuda", generator=self.g).to(torch.int32).expand(len(lengths), -1)
+        self.lengths = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        self.bounds = s3b.KVBounds(self.cache)
+        low = torch.randint(-127, 128, (pages, heads, d), device="cuda", generator=self.g)
+        high = torch.randint(-127, 128, (pages, heads, d), device="cuda", generator=self.g)
+        self.bounds.codes[:, :, 0], self.bounds.codes[:, :, 1] = torch.minimum(low, high), torch.maximum(low, high)
+        self.bounds.steps.copy_(torch.rand(pages, heads, device="cuda", generator=self.g))
+        # a quarter of the pages are equal, so that the choice ends among equals
+        self.bounds.codes[::4], self.bounds.steps[::4] = self.bounds.codes[0], self.bounds.steps[0]
+
+    def queries(self, nq, heads):
+        return torch.randn(len(self.lens), nq, heads, self.d, device="cuda", generator=self.g).half()
+
+
+def test_select_of_many_lists_of_very_many_pages(s3b, engine):
+    """Lists whose scores, kept at once, would take 270 MB: the same as a few at a time."""
+    batch, pages, keep = 160, 430000, 50
+    s = Bounded(s3b, 1, 64, pages, [16 * pages - 16 * 1000 * i for i in range(batch)], seed=3)
+    q = s.queries(1, 1)
+    selected, few = (torch.full((batch, 1, 1, keep), 9, dtype=torch.int32, device="cuda") for _ in "ab")
+    engine.cache_select(s.bounds, q, selected, s.pages, s.lengths)
+    for b in range(0, batch, 40):
+        engine.cache_select(s.bounds, q[b:b + 40], few[b:b + 40], s.pages[b:b + 40], s.lengths[b:b + 40])
+    engine.sync()
+    assert torch.equal(selected, few)
+    at = s.pages[0].long()
+    for b in (0, 159):
+        n = -(-s.lens[b] // 16)
+        want = plain_scores(q[b, :, 0], s.bounds.codes[at, 0], s.bounds.steps[at, 0])[0, :n]
+        assert selected[b, 0, 0].tolist() == plain_choice(want.tolist(), keep, 0, 1)
+
+
+@pytest.mark.parametrize("width", [32769, 1 << 21])
+def test_select_by_tables_far_wider_than_their_sequences(s3b, engine, width):
+    """Some thousand lists over a table whose scores would not fit the GPU, or would fill much of it: the lists of a narrow table."""
+    s = Sequences(s3b, engine, 2, 64, 4, 64, [1000, 3000], seed=4)
+    table = torch.full((2, width), -7, dtype=torch.int32, device="cuda")
+    table[:, :s.pages.shape[1]] = s.pages
+    bounds = s3b.KVBounds(s.cache)
+    engine.cache_bounds(s.cache, bounds, s.pages, s.lengths)
+    q = s.queries(4096, 4)
+    before = torch.cuda.mem_get_info()[0]
+    wide, narrow = (torch.full((2, 4096, 4, 4), 9, dtype=torch.int32, device="cuda") for _ in "ab")
+    engine.cache_select(bounds, q, wide, table, s.lengths, causal=True)
+    engine.cache_select(bounds, q, narrow, s.pages, s.lengths, causal=True)
+    engine.sync()
+    assert torch.equal(wide, narrow)
+    assert before - torch.cuda.mem_get_info()[0] <= 2 ** 29  # no workspace of all scores stays behind
 
 
 # ---------------------------------------------------------------- the longest lists
