@@ -653,7 +653,8 @@ int s3b_kv_bounds_values(const s3b_kv_bounds* bounds, const int64_t* pages, int6
  *            (keep * page_size at most 2^31 - 8192)
  * At most 32 rows (share x heads / heads of the cache; 16 at d = 256) have a list.
  * Calls of one context use its workspace: a captured one is replayed on the
- * context's stream, or ordered with its other calls. */
+ * context's stream, or ordered with its other calls. What a call reads in device
+ * memory, lengths and page tables too, stays as it is until the call has run. */
 typedef struct s3b_kv_call {
     const int32_t* pages;
     int64_t pages_stride;

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
     }
   }
   const long long p0 = s_p0, p1 = s_p1, total = s_total, ctas = s_ctas;
-  if (p0 >= p1) return;
+  if (p0 >= p1 || s_b < 0) return;
 
   const float sl2 = p.scale * kLog2e;
   const long long v_offset = (long long)per_page * L::kHalf;  // of a page's values from its keys
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
   bool ok = true;
 
   long long pos = p0, base = s_base;
-  for (int b = s_b; pos < p1; ++b) {
+  for (int b = s_b; pos < p1 && b < p.batch; ++b) {
     int g0, g1;
     const int n_chunks = chunks_of(b, &g0, &g1);
     const int len = sequence_length(p, b, err);

@@ -59,13 +59,13 @@ struct WeightArgs {
 // decay * old + sum; with a decay of 0 what was there does not count, whatever it is
 __device__ __forceinline__ float weigh(float decay, float old, float sum) { return decay != 0.f ? fmaf(decay, old, sum) : sum; }
 
-// The sequence of the line's place `pos` where sequence b has span(b) places, and the place of its first. The whole warp; pos lies
-// inside the line.
+// The sequence of the line's place `pos` where sequence b has span(b) places, and the place of its first; `batch` where the lengths
+// have become shorter since they were added up. The whole warp.
 template <typename Span>
 __device__ __forceinline__ int sequence_at(int batch, long long pos, long long* base, Span span) {
   const int lane = threadIdx.x & 31;
   *base = 0;
-  for (int b0 = 0;; b0 += 32) {
+  for (int b0 = 0; b0 < batch; b0 += 32) {
     const long long n = b0 + lane < batch ? span(b0 + lane) : 0;
     long long last = n;
 #pragma unroll
@@ -81,6 +81,7 @@ __device__ __forceinline__ int sequence_at(int batch, long long pos, long long* 
     }
     *base += __shfl_sync(~0u, last, 31);
   }
+  return batch;
 }
 template <typename Span>
 __device__ __forceinline__ long long line_length(int batch, Span span) {
@@ -116,17 +117,45 @@ __global__ void __launch_bounds__(32 * kWarps, Sweep<QT, D, NG>::kBlocks) sweep_
   const float sl2 = p.scale * kLog2e;
   let_next();
   wait_before();
-  auto blocks_of = [&](int b) { return (sequence_length(p, b, err) + C::kTokens - 1) / C::kTokens; };
-  auto span = [&](int b) { return (long long)blocks_of(b) * p.c.heads; };
-  const long long total = line_length(p.batch, span);
-  long long pos = total * blockIdx.x / gridDim.x, base;
-  const long long end = total * (blockIdx.x + 1) / gridDim.x;
-  if (pos >= end) return;
-  int b = sequence_at(p.batch, pos, &base, span);
+  // this CTA's share of the line and its present sequence, read by one warp or thread for all of them: a length that a caller changes
+  // meanwhile may cost it tokens, but no barrier a thread, and the walk ends with the batch
+  __shared__ long long s_total, s_base;
+  __shared__ int s_b, s_len;
+  auto blocks_of = [&](int len) { return (len + C::kTokens - 1) / C::kTokens; };
+  if (warp == 0) {
+    auto span = [&](int b) { return (long long)blocks_of(sequence_length(p, b, err)) * p.c.heads; };
+    const long long total = line_length(p.batch, span), first = total * blockIdx.x / gridDim.x;
+    long long base;
+    const int b = sequence_at(p.batch, first, &base, span);
+    if (lane == 0) {
+      s_total = total;
+      s_base = base;
+      s_b = b;
+      s_len = b < p.batch ? sequence_length(p, b, err) : 0;
+    }
+  }
+  __syncthreads();
+  long long pos = s_total * blockIdx.x / gridDim.x, base = s_base;
+  const long long end = s_total * (blockIdx.x + 1) / gridDim.x;
+  int b = s_b, len = s_len, blocks = blocks_of(len);
   long long staged = -1;  // the unit whose rows are in shared memory, all of them
   for (; pos < end; ++pos) {
-    while (pos >= base + span(b)) base += span(b++);
-    const int len = sequence_length(p, b, err), blocks = blocks_of(b);
+    if (pos >= base + (long long)blocks * p.c.heads) {
+      __syncthreads();  // the sequence before is known to all
+      if (threadIdx.x == 0) {
+        while (b < p.batch && pos >= base + (long long)blocks * p.c.heads) {
+          base += (long long)blocks * p.c.heads;
+          len = ++b < p.batch ? sequence_length(p, b, err) : 0;
+          blocks = blocks_of(len);
+        }
+        s_base = base;
+        s_b = b;
+        s_len = len;
+      }
+      __syncthreads();
+      base = s_base, b = s_b, len = s_len, blocks = blocks_of(len);
+    }
+    if (b >= p.batch) return;
     const int head = (int)((pos - base) / blocks);
     const int tok_cta = (int)(pos - base - (long long)head * blocks) * C::kTokens;
     const long long unit = (long long)b * p.c.heads + head;
@@ -346,7 +375,7 @@ __global__ void __launch_bounds__(128, Stream<QT, D, NT>::kBlocks) stream_kernel
   int b = sequence_at(p.batch, pos, &base, span);
 
   const float sl2 = p.scale * kLog2e;
-  for (; pos < end; ++b) {
+  for (; pos < end && b < p.batch; ++b) {
     const int len = sequence_length(p, b, err), groups = (len + 15) >> 4;
     const int* table = p.pages + b * p.pages_stride;
     for (; pos < end && pos < base + (long long)groups * p.c.heads;) {

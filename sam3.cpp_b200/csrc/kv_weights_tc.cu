@@ -50,10 +50,14 @@ struct WtArgs {
   int chunks;   // of 128 query rows of a head
 };
 
-// One CTA's walk over its share [pos, end) of the line, tile by tile. Every role takes the same steps.
+// One CTA's walk over its share [pos, end) of the line, tile by tile. Every role takes the same steps, by lengths that are read once
+// (those of its first kLens sequences: as many as 128 tokens each and more than 1024 sequences for each SM would need).
+constexpr int kLens = 1024;
 struct WtWalk {
   long long pos, end, base;
   int b;
+  const int* lens;  // of the sequences from b_first on, in shared memory
+  int b_first;
 };
 struct WtSeg {
   int b, head, len, tok0;
@@ -64,8 +68,8 @@ struct WtSeg {
 
 __device__ __forceinline__ bool wt_next(const WtArgs& a, int* err, WtWalk& w, WtSeg& s) {
   const KvAttnParams& p = a.p;
-  while (w.pos < w.end) {
-    s.len = sequence_length(p, w.b, err);
+  while (w.pos < w.end && w.b < p.batch) {
+    s.len = w.b - w.b_first < kLens ? w.lens[w.b - w.b_first] : sequence_length(p, w.b, err);
     const int tiles = (s.len + kTile - 1) / kTile;
     const long long span = (long long)tiles * p.c.heads * a.chunks;
     if (w.pos >= w.base + span) {
@@ -126,6 +130,7 @@ __global__ void __launch_bounds__(Wt<QT, D>::kThreads, 1) weights_tiles_kernel(c
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort_word, s_stop[2], s_last, s_b;
   __shared__ long long s_total, s_base;
+  __shared__ int s_lens[kLens];
   volatile int* s_abort = &s_abort_word;
 
   const KvAttnParams& p = a.p;
@@ -185,6 +190,17 @@ __global__ void __launch_bounds__(Wt<QT, D>::kThreads, 1) weights_tiles_kernel(c
         base += __shfl_sync(~0u, end, 31);
       }
     }
+    // lengths from there on, as far as the share goes
+    long long past = base;
+    const long long p1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : 0;
+    for (int b0 = found; b0 < p.batch && b0 - found < kLens && past < p1; b0 += 32) {
+      const int len = b0 + lane < p.batch ? sequence_length(p, b0 + lane, err) : 0;
+      s_lens[b0 - found + lane] = len;
+      long long n = (long long)((len + kTile - 1) / kTile) * p.c.heads * a.chunks;
+#pragma unroll
+      for (int x = 16; x; x >>= 1) n += __shfl_xor_sync(~0u, n, x);
+      past += n;
+    }
     if (lane == 0) {
       s_total = total;
       s_base = base;
@@ -198,7 +214,7 @@ __global__ void __launch_bounds__(Wt<QT, D>::kThreads, 1) weights_tiles_kernel(c
   const long long total = s_total, ctas = min((long long)gridDim.x, total);
   const bool works = blockIdx.x < ctas;
   const long long p0 = works ? total * blockIdx.x / ctas : 0;
-  WtWalk w{p0, works ? total * (blockIdx.x + 1) / ctas : 0, s_base, s_b};
+  WtWalk w{p0, works ? total * (blockIdx.x + 1) / ctas : 0, s_base, s_b, s_lens, s_b};
   WtSeg s;
   const float sl2 = p.scale * kLog2e;
   uint32_t n = 0;     // chunks so far
@@ -369,7 +385,7 @@ __global__ void __launch_bounds__(Wt<QT, D>::kThreads, 1) weights_tiles_kernel(c
         if (tok < s.len) to[tok] = a.w.decay != 0.f ? fmaf(a.w.decay, to[tok], sum) : sum;
         continue;
       }
-      const long long c0 = ((s.start + 1) * ctas - 1) / total, c1 = ((s.start + a.chunks) * ctas - 1) / total;
+      const long long c0 = ((s.start + 1) * ctas - 1) / total, c1 = min(ctas - 1, ((s.start + a.chunks) * ctas - 1) / total);
       __stcg(a.part + (2 * (long long)blockIdx.x + (s.start > p0 ? 1 : 0)) * kTile + row, sum);
       __threadfence();
       asm volatile("bar.sync 2, 128;" ::: "memory");

@@ -200,3 +200,39 @@ def test_the_longest_eviction(s3b, engine):
     engine.cache_read(to, torch.arange(n, device="cuda"), *moved)
     engine.sync()
     assert torch.equal(moved[0], k) and torch.equal(moved[1], v)
+
+
+# ---------------------------------------------------------------- lengths that change meanwhile
+@pytest.mark.parametrize("nq,d", [(1, 64), (9, 128), (9, 256), (30, 64), (30, 128), (200, 64), (200, 256)])
+def test_weights_end_whatever_the_lengths_become(s3b, engine, nq, d):
+    """Another stream writes the lengths while weights are gathered: what comes of it is the caller's, but the calls end, write nothing
+    outside their rows, and leave later calls as they were."""
+    lens = [(37 * i) % 900 for i in range(400)]
+    e = s3b.Engine(0)  # on a stream of its own
+    s = Sequences(s3b, engine, 2, d, 2, 16, lens, seed=nq)
+    tokens = s.pages.shape[1] * 16
+    around = torch.full((402, 2, tokens), 5.0, device="cuda")
+    weights = around[1:401]
+    q, lse = s.queries(nq, 4), torch.full((400, nq, 4), 4.0, device="cuda")
+    others = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0] * 400, lens[::-1], [900] * 400, [16] * 399 + [0])]
+    good, side = s.lengths.clone(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(60):
+        e.cache_weights(s.cache, q, lse, weights, s.pages, s.lengths, 0.1, causal=bool(i % 2), window=50 if i % 4 == 3 else 0)
+        with torch.cuda.stream(side):
+            for x in others:
+                s.lengths.copy_(x)
+    torch.cuda.synchronize()
+    e.close()
+    assert (around[0] == 5).all() and (around[401] == 5).all()
+    s.lengths.copy_(good)
+    e = s3b.Engine(0)
+    a, b = torch.zeros(400, 2, tokens, device="cuda"), torch.zeros(400, 2, tokens, device="cuda")
+    torch.cuda.synchronize()
+    e.cache_weights(s.cache, q, lse, a, s.pages, s.lengths, 0.1)
+    for i in range(0, 400, 50):
+        e.cache_weights(s.cache, q[i:i + 50], lse[i:i + 50], b[i:i + 50], s.pages[i:i + 50], s.lengths[i:i + 50], 0.1)
+    e.sync()
+    e.close()
+    # where many CTAs share a tile its parts are cut elsewhere: f32 sums of at most 400 terms in another order
+    assert (a - b).abs().max() <= 400 * 2.0 ** -24 * a.max()
