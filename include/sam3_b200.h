@@ -735,7 +735,7 @@ int s3b_op_cache_weights(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_c
  *   weights      as in s3b_op_cache_weights (rows may overlap)
  *   pages_out    [batch][out_stride >= ceil(keep / to->page_size)]: none of them
  *                may be a page that this call reads, nor named twice
- *   lengths_out  [batch]: min(lengths[b], keep); not the array of lengths
+ *   lengths_out  [batch]: min(lengths[b], keep); no part of the array of lengths
  *   kept         [batch][heads][keep]: positions that the tokens had, -1 behind the last
  *   weights_out  f32 [batch][heads][keep]: their weights, 0 behind the last; or NULL */
 typedef struct s3b_kv_evict {

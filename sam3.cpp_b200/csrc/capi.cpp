@@ -1842,7 +1842,8 @@ int s3b_op_cache_evict(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_cal
   if (batch == 0) return kOk;
   if (!evict->lengths_out || (keep > 0 && (!evict->kept || !evict->pages_out || (!weights && max_pages > 0))))
     return set_error(ctx, kErrArg, "cache_evict: null pointer");
-  if (evict->lengths_out == call->lengths) return set_error(ctx, kErrArg, "cache_evict: lengths_out is the array of lengths");
+  if (evict->lengths_out < call->lengths + batch && call->lengths < evict->lengths_out + batch)
+    return set_error(ctx, kErrArg, "cache_evict: lengths_out lies over the lengths");
   if ((long long)batch * p.c.heads > (1LL << 40) / std::max(keep, 1))
     return set_error(ctx, kErrUnsupported, "cache_evict: %d sequences of %d heads keep %d tokens", batch, p.c.heads, keep);
   if (weights_out) {  // the weights that are read, from the first to the last

@@ -4,7 +4,7 @@ import math
 import pytest
 
 torch = pytest.importorskip("torch")
-from test_kv_long_gpu import Sequences, plain_choice, plain_scores  # noqa: E402
+from test_kv_long_gpu import Sequences, plain_choice, plain_scores, some_weights  # noqa: E402
 from test_kv_long_run_gpu import raw  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
@@ -236,3 +236,25 @@ def test_weights_end_whatever_the_lengths_become(s3b, engine, nq, d):
     e.close()
     # where many CTAs share a tile its parts are cut elsewhere: f32 sums of at most 400 terms in another order
     assert (a - b).abs().max() <= 400 * 2.0 ** -24 * a.max()
+
+
+# ---------------------------------------------------------------- arrays over each other
+@pytest.mark.parametrize("off,refused", [(-3, False), (-2, True), (-1, True), (0, True), (1, True), (2, True), (3, False)])
+def test_new_lengths_over_the_lengths_are_refused(s3b, engine, off, refused):
+    """One sequence's new length would be read as another's."""
+    s = Sequences(s3b, engine, 2, 64, 2, 16, [40, 33, 50], seed=2, spare=3)
+    both = torch.full((9,), -5, dtype=torch.int32, device="cuda")
+    both[3:6] = s.lengths
+    kept = torch.full((3, 2, 10), 9, dtype=torch.int32, device="cuda")
+    free = sorted(set(range(s.cache.n_pages)) - set(s.pages.flatten().tolist()))
+    pages_out = torch.tensor(free[:3], dtype=torch.int32, device="cuda")[:, None]
+    args = (s.cache, some_weights(s), s.pages, both[3:6], pages_out, both[3 + off:6 + off], kept)
+    if refused:
+        with pytest.raises(s3b.S3BError, match="over the lengths"):
+            engine.cache_evict(*args)
+        engine.sync()
+        assert (kept == 9).all() and both[3:6].tolist() == s.lens
+    else:
+        engine.cache_evict(*args)
+        engine.sync()
+        assert both[3 + off:6 + off].tolist() == [10, 10, 10] and both[3:6].tolist() == s.lens and (kept < 50).all()
