@@ -4,7 +4,7 @@ import math
 import pytest
 
 torch = pytest.importorskip("torch")
-from test_kv_long_gpu import Sequences, plain_choice, plain_scores, some_weights  # noqa: E402
+from test_kv_long_gpu import Sequences, check_evict, plain_choice, plain_scores, some_weights  # noqa: E402
 from test_kv_long_run_gpu import raw  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
@@ -132,6 +132,33 @@ class Bounded:
         return torch.randn(len(self.lens), nq, heads, self.d, device="cuda", generator=self.g).half()
 
 
+@pytest.mark.parametrize("batch,heads,pages,keep", [
+    (160, 1, 600, 40), (32, 5, 700, 300), (160, 1, 24576, 100), (160, 1, 24577, 5000), (53, 3, 26000, 26),  # a block of 8 warps a list
+    (40, 1, 1025, 33), (10, 4, 3000, 1500), (40, 1, 24576, 24000), (38, 1, 25001, 200),                      # 16 warps
+    (20, 1, 50000, 64), (5, 1, 200000, 1000), (1, 2, 400000, 77)])                                           # clusters of 2, 8 and 16
+def test_select_rounds(s3b, engine, batch, heads, pages, keep):
+    """Lists whose threshold is found digit by digit, in one block and in clusters, with keys in shared memory and remade from the
+    scores where more than 24576 pages fall to a block."""
+    lengths = [16 * pages - (i % 5) * (pages // 7) * 16 - i % 16 for i in range(batch)]
+    s = Bounded(s3b, heads, 64, pages, lengths, seed=pages)
+    q = s.queries(1, heads)
+    selected, again = (torch.full((batch, 1, heads, keep), 9, dtype=torch.int32, device="cuda") for _ in "ab")
+    scores = torch.full((batch, 1, heads, pages), 5.0, device="cuda")
+    engine.cache_select(s.bounds, q, selected, s.pages, s.lengths, sink=1, recent=2, scores=scores)
+    engine.cache_select(s.bounds, q, again, s.pages, s.lengths, sink=1, recent=2)
+    engine.sync()
+    assert torch.equal(selected, again)
+    some = range(batch) if pages < 2000 else sorted({0, batch // 3, batch - 1})
+    at = s.pages[0].long()
+    for b in some:
+        n = -(-lengths[b] // 16)
+        for h in range(heads):
+            want = plain_scores(q[b, :, h], s.bounds.codes[at, h], s.bounds.steps[at, h])[0]
+            assert torch.equal(scores[b, 0, h, :n], want[:n]) and (scores[b, 0, h, n:] == -math.inf).all()
+            chosen = plain_choice(want[:n].tolist(), keep, 1, 2)
+            assert selected[b, 0, h].tolist() == chosen + [-1] * (keep - len(chosen)), (b, h)
+
+
 def test_select_of_many_lists_of_very_many_pages(s3b, engine):
     """Lists whose scores, kept at once, would take 270 MB: the same as a few at a time."""
     batch, pages, keep = 160, 430000, 50
@@ -166,6 +193,18 @@ def test_select_by_tables_far_wider_than_their_sequences(s3b, engine, width):
     engine.sync()
     assert torch.equal(wide, narrow)
     assert before - torch.cuda.mem_get_info()[0] <= 2 ** 29  # no workspace of all scores stays behind
+
+
+# ---------------------------------------------------------------- how an eviction holds its keys
+@pytest.mark.parametrize("lengths,heads,keep", [
+    ([3000, 2049], 75, 1000), ([2500], 80, 2499), ([49152], 76, 300), ([50001], 75, 20000),  # a block a head: in shared memory, remade
+    ([800003], 1, 3000), ([800003, 790000], 1, 700000), ([120000], 10, 50)])                   # clusters of 16, remade, and of 8
+@pytest.mark.parametrize("ties", [False, True])
+def test_evict_rounds(s3b, engine, lengths, heads, keep, ties):
+    """Tokens whose threshold is found digit by digit, by one block or a cluster, with keys in shared memory and remade from the
+    weights where more than 49152 tokens fall to a block."""
+    s = Sequences(s3b, engine, 2, 64, heads, 16, lengths, seed=lengths[0], spare=len(lengths) * (keep // 16 + 1))
+    check_evict(s3b, engine, s, some_weights(s, ties), keep, 4, 100 if keep > 104 else 0)
 
 
 # ---------------------------------------------------------------- the longest lists
