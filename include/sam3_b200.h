@@ -712,9 +712,11 @@ int s3b_op_cache_select(s3b_ctx* ctx, const s3b_kv_bounds* bounds, const s3b_kv_
  * block and the heads of a group see the pages that their list names, in any order;
  * a page that it names twice counts twice. A row that sees no token of them is
  * zero, its lse -inf. An entry beyond max_pages is skipped and the next s3b_sync
- * returns S3B_ERR_DEVICE. Takes all of `call`; lse may be NULL. Weights are rounded
- * to f16 once, with their products with the block scales: f16 outputs are off by
- * 2.9e-4 of their norm. */
+ * returns S3B_ERR_DEVICE. Takes all of `call`; lse may be NULL. For f16 outputs
+ * the products of weights and block scales are rounded to f16, once: they are off by
+ * up to 3e-4 of their norm (2.1e-4 by their own rounding). For f32 outputs what that
+ * rounding leaves is kept: they are off by some 1e-6 of their norm, for 2 to 17% of
+ * the time. */
 int s3b_op_cache_attention_selected(s3b_ctx* ctx, const s3b_kv_cache* cache, const s3b_kv_call* call);
 
 /* Adds the attention weight that each token gets from the queries of `call` to what

@@ -28,8 +28,8 @@ int kv_attention_launches(const KvAttnParams& p) {
 
 int kv_attention(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
   if (p.nq * (long long)(p.heads / p.c.heads) > kv_attention_most_rows(p.c.d)) return kv_attention_tc(p, w, err, st);
-  return p.c.type == QT_Q4_0 ? attend_d<QT_Q4_0, false>(p, w, err, st)
-                             : p.c.type == QT_Q4_1 ? attend_d<QT_Q4_1, false>(p, w, err, st) : attend_d<QT_Q8_0, false>(p, w, err, st);
+  return p.c.type == QT_Q4_0 ? attend_d<QT_Q4_0, kAllPages>(p, w, err, st)
+                             : p.c.type == QT_Q4_1 ? attend_d<QT_Q4_1, kAllPages>(p, w, err, st) : attend_d<QT_Q8_0, kAllPages>(p, w, err, st);
 }
 
 }  // namespace s3b

@@ -83,10 +83,14 @@ struct ScaleRange {
 // 8, whose few parts are joined beside other blocks' work here.)
 // With SEL a unit is a block of p.share queries and a key / value head, and its tokens are those of the pages that its list
 // names: steps of W groups go over the list's pages, a page's first token stands at entry * page_size, and the masks go by
-// that. Its weights keep what their rounding to f16 left until they are multiplied by a scale: the output is off by 2.9e-4 of its
-// norm then, two movmatrix and 2 NB products more for 16 tokens and 8 rows. Measured: 32 x 8 lists of 32 pages of 64, 4 heads a list of
+// that. Its weights keep what their rounding to f16 left until they are multiplied by a scale: an f16 output is off by up to 3e-4 of
+// its norm then (2.1e-4 by its own rounding), two movmatrix and 2 NB products more for 16 tokens and 8 rows. For f32 outputs what
+// the products' rounding leaves is multiplied too, 4 NB and in q4_1 two more m16n8k16: off by 1e-7 to 7e-7 where f16 weights alone
+// left 1e-6 to 3e-5, for 2% (512 pages a list) to 17% (1024 lists of 32 pages, 32 rows each, q4_1) of the time. As a branch in
+// one kernel it cost f16 outputs up to 10%. Measured: 32 x 8 lists of 32 pages of 64, 4 heads a list of
 // d = 128, q4_0: 75 MB in 27 us (37 with shares of equal size, whose parts had to be joined); 256 lists of 64 pages, 16 rows of
 // d = 256, q8_0: 131 us, 136 TFLOP/s. Issue bounds both (45 to 52% of the cycles; at d = 256 the output's registers leave 8 warps an SM).
+enum { kAllPages, kLists, kListsF32 };  // what rows_kernel attends over; the last with f32 outputs
 constexpr int kNoTok = 0x7FFFFF00;  // position of a group that is none: past every span
 
 template <int QT, int D, int NT, int W>
@@ -120,12 +124,13 @@ struct RowsArgs {
   int* count;   // [units], zero between launches
 };
 
-template <int QT, int D, int NT, int W, bool SEL>
+template <int QT, int D, int NT, int W, int OF>
 __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
     rows_kernel(const __grid_constant__ RowsArgs a, int* err) {
   typedef KvL<QT, D> L;
   typedef Rows<QT, D, NT, W> C;
   constexpr int NB = L::kNB, NS = C::kStages, G = C::kG;
+  constexpr bool SEL = OF != kAllPages, EXACT = OF == kListsF32;
   typedef ScaleRange<QT, NB> Range;
   constexpr float kBias = Range::kBias;
   constexpr float kLazy = 2.9f;  // log2 by which a score may pass the reference: 2^(kBias + 2.9) < 65504
@@ -658,6 +663,10 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
             for (int nt = 0; nt < NT; ++nt) {
               mma16816(omin[nt], am, w0[nt], w1[nt]);
               mma16816(omin[nt], as, w0[nt], w1[nt]);
+              if (EXACT) {
+                mma16816(omin[nt], am, r0_all[gg][nt], r1_all[gg][nt]);
+                mma16816(omin[nt], as, r0_all[gg][nt], r1_all[gg][nt]);
+              }
             }
           }
 #pragma unroll
@@ -684,13 +693,20 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
               const uint2 sc = *reinterpret_cast<const uint2*>(vp + L::v_scale(2 * t, n));
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                // with SEL the product of the unrounded weight and the scale, rounded once
-                const uint32_t b0 = h2_u32(SEL ? __hfma2(u32_h2(w0[nt]), u32_h2(sc.x), __hmul2(u32_h2(r0_all[gg][nt]), u32_h2(sc.x)))
-                                               : __hmul2(u32_h2(w0[nt]), u32_h2(sc.x)));
-                const uint32_t b1 = h2_u32(SEL ? __hfma2(u32_h2(w1[nt]), u32_h2(sc.y), __hmul2(u32_h2(r1_all[gg][nt]), u32_h2(sc.y)))
-                                               : __hmul2(u32_h2(w1[nt]), u32_h2(sc.y)));
+                // of lists the product of the unrounded weight and the scale, rounded once
+                uint32_t b0 = h2_u32(__hmul2(u32_h2(w0[nt]), u32_h2(sc.x))), b1 = h2_u32(__hmul2(u32_h2(w1[nt]), u32_h2(sc.y)));
+                if (SEL && !EXACT) {
+                  b0 = h2_u32(__hfma2(u32_h2(w0[nt]), u32_h2(sc.x), __hmul2(u32_h2(r0_all[gg][nt]), u32_h2(sc.x))));
+                  b1 = h2_u32(__hfma2(u32_h2(w1[nt]), u32_h2(sc.y), __hmul2(u32_h2(r1_all[gg][nt]), u32_h2(sc.y))));
+                }
                 mma16816(o[nt][2 * n], a0, b0, b1);
                 mma16816(o[nt][2 * n + 1], a1, b0, b1);
+                if (EXACT) {  // what the product's rounding left, and the scale times what the weight's left
+                  const uint32_t c0 = h2_u32(__hfma2(u32_h2(r0_all[gg][nt]), u32_h2(sc.x), __hfma2(u32_h2(w0[nt]), u32_h2(sc.x), __hneg2(u32_h2(b0)))));
+                  const uint32_t c1 = h2_u32(__hfma2(u32_h2(r1_all[gg][nt]), u32_h2(sc.y), __hfma2(u32_h2(w1[nt]), u32_h2(sc.y), __hneg2(u32_h2(b1)))));
+                  mma16816(o[nt][2 * n], a0, c0, c1);
+                  mma16816(o[nt][2 * n + 1], a1, c0, c1);
+                }
               }
             }
           }
@@ -867,10 +883,10 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
   }
 }
 
-template <int QT, int D, int NT, int W, bool SEL>
+template <int QT, int D, int NT, int W, int OF>
 int launch_rows(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
   typedef Rows<QT, D, NT, W> C;
-  auto* k = rows_kernel<QT, D, NT, W, SEL>;
+  auto* k = rows_kernel<QT, D, NT, W, OF>;
   if (kernel_setup(k, C::kSmem) <= 0) return -13;
   RowsArgs a;
   a.p = p;
@@ -880,7 +896,7 @@ int launch_rows(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream
 }
 
 // ---------------------------------------------------------------- dispatch
-template <int QT, int D, int NT, bool SEL>
+template <int QT, int D, int NT, int OF>
 int launch_rows_nt(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
   // Blocks of four warps, several on an SM, where there is a unit for each SM: a unit's beginning and end then run beside
   // other blocks' loops (32 sequences, 8 heads: 123 -> 96 us). One block an SM where few units are cut into many parts,
@@ -888,24 +904,24 @@ int launch_rows_nt(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStr
   // are units for those, so that each has its own.
   constexpr int kMost = Rows<QT, D, NT, 4>::kWarps;
   const long long units = kv_attention_units(p);
-  constexpr int kHalf = SEL && (kMost > 8) ? kMost / 2 : 4;
-  if (kHalf > 4 && units >= w.sms && units <= 2 * w.sms) return launch_rows<QT, D, NT, kHalf, SEL>(p, w, err, st);
-  if (units >= w.sms) return launch_rows<QT, D, NT, 4, SEL>(p, w, err, st);
-  return launch_rows<QT, D, NT, kMost, SEL>(p, w, err, st);
+  constexpr int kHalf = OF != kAllPages && (kMost > 8) ? kMost / 2 : 4;
+  if (kHalf > 4 && units >= w.sms && units <= 2 * w.sms) return launch_rows<QT, D, NT, kHalf, OF>(p, w, err, st);
+  if (units >= w.sms) return launch_rows<QT, D, NT, 4, OF>(p, w, err, st);
+  return launch_rows<QT, D, NT, kMost, OF>(p, w, err, st);
 }
 
-template <int QT, int D, bool SEL>
+template <int QT, int D, int OF>
 int attend(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
-  const int rows = (SEL ? p.share : p.nq) * (p.heads / p.c.heads);
-  if (rows <= 8) return launch_rows_nt<QT, D, 1, SEL>(p, w, err, st);
-  if (D == 256 || rows <= 16) return launch_rows_nt<QT, D, 2, SEL>(p, w, err, st);
-  return launch_rows_nt<QT, D, D == 256 ? 2 : 4, SEL>(p, w, err, st);
+  const int rows = (OF != kAllPages ? p.share : p.nq) * (p.heads / p.c.heads);
+  if (rows <= 8) return launch_rows_nt<QT, D, 1, OF>(p, w, err, st);
+  if (D == 256 || rows <= 16) return launch_rows_nt<QT, D, 2, OF>(p, w, err, st);
+  return launch_rows_nt<QT, D, D == 256 ? 2 : 4, OF>(p, w, err, st);
 }
 
-template <int QT, bool SEL>
+template <int QT, int OF>
 int attend_d(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
-  return p.c.d == 64 ? attend<QT, 64, SEL>(p, w, err, st)
-                     : p.c.d == 128 ? attend<QT, 128, SEL>(p, w, err, st) : attend<QT, 256, SEL>(p, w, err, st);
+  return p.c.d == 64 ? attend<QT, 64, OF>(p, w, err, st)
+                     : p.c.d == 128 ? attend<QT, 128, OF>(p, w, err, st) : attend<QT, 256, OF>(p, w, err, st);
 }
 
 }  // namespace s3b

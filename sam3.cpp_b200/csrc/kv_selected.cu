@@ -4,8 +4,9 @@
 namespace s3b {
 
 int kv_attention_selected(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st) {
-  return p.c.type == QT_Q4_0 ? attend_d<QT_Q4_0, true>(p, w, err, st)
-                             : p.c.type == QT_Q4_1 ? attend_d<QT_Q4_1, true>(p, w, err, st) : attend_d<QT_Q8_0, true>(p, w, err, st);
+  if (p.out_f32) return kv_attention_selected_f32(p, w, err, st);
+  return p.c.type == QT_Q4_0 ? attend_d<QT_Q4_0, kLists>(p, w, err, st)
+                             : p.c.type == QT_Q4_1 ? attend_d<QT_Q4_1, kLists>(p, w, err, st) : attend_d<QT_Q8_0, kLists>(p, w, err, st);
 }
 
 }  // namespace s3b

@@ -4,7 +4,7 @@ import math
 import pytest
 
 torch = pytest.importorskip("torch")
-from test_kv_long_gpu import Sequences, check_evict, plain_choice, plain_scores, some_weights  # noqa: E402
+from test_kv_long_gpu import Sequences, check_evict, plain_attention, plain_choice, plain_scores, some_weights  # noqa: E402
 from test_kv_long_run_gpu import raw  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
@@ -297,3 +297,36 @@ def test_new_lengths_over_the_lengths_are_refused(s3b, engine, off, refused):
         engine.cache_evict(*args)
         engine.sync()
         assert both[3 + off:6 + off].tolist() == [10, 10, 10] and both[3:6].tolist() == s.lens and (kept < 50).all()
+
+
+# ---------------------------------------------------------------- f32 outputs
+@pytest.mark.parametrize("qtype", [2, 3, 8])
+@pytest.mark.parametrize("d,heads,kv,nq,share", [(64, 8, 2, 9, 1), (64, 4, 1, 16, 8), (128, 4, 2, 8, 4), (128, 8, 1, 6, 2), (256, 2, 1, 20, 4), (256, 4, 2, 12, 6)])
+def test_f32_outputs_keep_the_weights(s3b, engine, qtype, d, heads, kv, nq, share):
+    """Weights and their products with the block scales keep 2^-22 and more on the way to an f32 output. Few tokens and small queries,
+    so that the bound is far below f16's half step, 2^-11: the score's error E and ex2's as in test_kv_long_gpu.py, the weight and the
+    product with a remainder each (2^-21), six accumulations of one group of 16 tokens (16 products and the sum before, each cut at
+    2^-24 of the largest) and 16 warps' sums. In q4_1 a value enters in two terms (test_kv_long_gpu.py)."""
+    s = Sequences(s3b, engine, qtype, d, kv, 16, [2, 3, 5, 9, 16], seed=d + nq)
+    q, scale, group = s.queries(nq, heads, 0.1), 0.9 * d ** -0.5, heads // kv
+    out, lse = torch.full(q.shape, 9.0, device="cuda"), torch.full(q.shape[:3], 9.0, device="cuda")
+    selected = torch.zeros(5, -(-nq // share), kv, 2, dtype=torch.int32, device="cuda")
+    selected[..., 1] = -1
+    engine.cache_attention_selected(s.cache, q, out, selected, s.pages, s.lengths, scale, share=share, lse=lse)
+    engine.sync()
+    for b in range(5):
+        for h in range(kv):
+            want, _, want_lse, _ = plain_attention(s, q, torch.arange(s.lens[b], device="cuda"), b, h, 0, nq, False, 0, scale)
+            k, v = (x[:, h].double() for x in s.rows(b))
+            x = q[b, :, h * group:(h + 1) * group].reshape(-1, d).double()
+            e = ((d + 16) * 2.0 ** -24 * scale * (x.abs() @ k.abs().T)).amax(1, keepdim=True)
+            p = (x @ k.T * scale).softmax(-1)
+            blocks = v.view(-1, d // 32, 32)
+            size = v.abs()
+            if qtype == 3:
+                size = size + (blocks.abs().amax(-1) + 2 * (blocks.amax(-1) - blocks.amin(-1))).repeat_interleave(32, -1)
+            err = (2 * torch.expm1(e) + 2.0 ** -19 + 2.0 ** -21 + (6 * 17 + 16) * 2.0 ** -24) * (p @ size) + 1e-30
+            assert err.max() < 2.0 ** -14 * size.max()
+            got = out[b, :, h * group:(h + 1) * group].reshape(-1, d).double()
+            assert ((got - want).abs() <= err).all(), (b, h, ((got - want).abs() / err).max())
+            assert ((lse[b, :, h * group:(h + 1) * group].reshape(-1) - want_lse).abs() <= 2 * e[:, 0] + 2.0 ** -18).all()
