@@ -637,7 +637,8 @@ typedef struct s3b_kv_bounds {
 /* The values that the bounds of n pages stand for, code * step: out f32
  * [n][heads][2][d], 16-byte aligned; pages int64 [n] (device), one outside the
  * bounds gives zeros. Needs no context: enqueued on `cuda_stream` of the current
- * device. */
+ * device. Bounds that s3b_op_cache_bounds writes on a context's stream are waited
+ * for by the caller (s3b_sync, or that stream). */
 int s3b_kv_bounds_values(const s3b_kv_bounds* bounds, const int64_t* pages, int64_t n, float* out, void* cuda_stream);
 
 /* What the calls below take of their sequences and queries; fields that a call

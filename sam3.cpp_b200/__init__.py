@@ -265,7 +265,8 @@ class KVCache:
 
 class KVBounds:
     """Bounds of the keys of each page and head of a cache (s3b_kv_bounds), for cache_select: codes int8 [n_pages, heads, 2, d]
-    (lowest, highest) and steps f32 [n_pages, heads], made here (zeros, there when the constructor returns)."""
+    (lowest, highest) and steps f32 [n_pages, heads], made here (zeros, there when the constructor returns). Engine.cache_bounds writes
+    them on the engine's stream: a program that reads them on another waits for that (Engine.sync, or an engine on torch's stream)."""
 
     def __init__(self, cache: KVCache):
         import torch
@@ -279,7 +280,8 @@ class KVBounds:
         self.ref = ctypes.byref(self.desc)
 
     def values(self, pages):
-        """The bounds f32 [n, heads, 2, d] of the pages int64 [n], on torch's stream (s3b_kv_bounds_values)."""
+        """The bounds f32 [n, heads, 2, d] of the pages int64 [n] (s3b_kv_bounds_values), on torch's stream: what an engine on a stream of
+        its own has still to write there is waited for first (Engine.sync)."""
         import torch
         n = _index("KVBounds.values", "pages", pages, 8, 1, self.device)
         out = torch.empty(n, self.heads, 2, self.d, device=pages.device)
@@ -905,7 +907,7 @@ class Engine:
     def cache_attention_selected(self, cache: KVCache, q, out, selected, pages, lengths, scale: float, share: int = 1,
                                  causal: bool = False, window: int = 0, lse=None):
         """cache_attention over the pages that the lists of cache_select name (s3b_op_cache_attention_selected): selected int32
-        [batch, ceil(nq / share), cache.heads, keep], the other arguments as there."""
+        [batch, ceil(nq / share), cache.heads, keep], the other arguments as there. Weights are rounded to f16 for f16 outputs only."""
         what = "cache_attention_selected"
         b, table, row, width, lens = self._sequences(what, pages, lengths)
         shape, nq, heads, at, q_b, q_n, q_h = self._query(what, cache, q, b)

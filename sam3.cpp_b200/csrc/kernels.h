@@ -423,7 +423,7 @@ int kv_attention_tc_launches(const KvAttnParams& p);
 // The same over the pages of lists (p.selected), for up to kv_attention_most_rows(d) rows of a list.
 int kv_attention_most_rows(int d);
 int kv_attention_selected(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st);
-int kv_attention_selected_f32(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st);  // with f32 outputs
+int kv_attention_selected_f32(const KvAttnParams& p, const KvAttnWork& w, int* err, cudaStream_t st);  // its part with f32 outputs
 
 // s3b_kv_bounds: codes [n_pages][heads][2][d] (lowest, highest), steps [n_pages][heads].
 struct KvBounds {

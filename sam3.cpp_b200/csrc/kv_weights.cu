@@ -234,44 +234,44 @@ __global__ void __launch_bounds__(32 * kWarps, Sweep<QT, D, NG>::kBlocks) sweep_
     for (int row0 = 0; row0 < n_rows; row0 += C::kRows) {
       const int rows = min(C::kRows, n_rows - row0), tiles = (rows + kTile - 1) / kTile;
       if (staged != unit) {
-      __syncthreads();
-      for (int e = threadIdx.x; e < tiles * NB * 32; e += 32 * kWarps) {
-        const int l = e & 31, n = e / 32 % NB, r = e / (32 * NB) * 8 + (l >> 2);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < rows) {
-          const int i = (row0 + r) / group_heads, h = head * group_heads + (row0 + r) % group_heads;
-          v = *reinterpret_cast<const uint4*>(p.q + b * p.q_b + i * p.q_n + h * p.q_h + 32 * n + 8 * (l & 3));
-        }
-        s_q[e] = v;
-      }
-      for (int r = threadIdx.x; r < tiles * kTile; r += 32 * kWarps) {
-        float lse = INFINITY;
-        int lo = 0, hi = 0;
-        if (r < rows) {
-          const int i = (row0 + r) / group_heads, h = head * group_heads + (row0 + r) % group_heads;
-          lse = p.lse[((long long)b * p.nq + i) * p.heads + h] * kLog2e;
-          if (lse != -INFINITY) row_span(p, len, i, &lo, &hi);  // else a row that has seen nothing, and sees nothing here
-        }
-        s_lse[r] = lse;
-        s_lo[r] = lo;
-        s_hi[r] = hi;
-      }
-      __syncthreads();
-      if (QT == QT_Q4_1) {  // sums of the query over blocks 2t, 2t + 1 as f16 and f16 remainder: a warp a row tile
-        for (int nt = warp; nt < tiles; nt += kWarps) {
-          float lo = 0.f, hi = 0.f;
-#pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            const uint4 v = s_q[(nt * NB + n) * 32 + lane];
-            const float s = block_sum(v);
-            if (n == 2 * t) lo = s;
-            if (n == 2 * t + 1) hi = s;
+        __syncthreads();
+        for (int e = threadIdx.x; e < tiles * NB * 32; e += 32 * kWarps) {
+          const int l = e & 31, n = e / 32 % NB, r = e / (32 * NB) * 8 + (l >> 2);
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (r < rows) {
+            const int i = (row0 + r) / group_heads, h = head * group_heads + (row0 + r) % group_heads;
+            v = *reinterpret_cast<const uint4*>(p.q + b * p.q_b + i * p.q_n + h * p.q_h + 32 * n + 8 * (l & 3));
           }
-          s_min[nt * 32 + lane] = split_sums(lo, hi);
+          s_q[e] = v;
+        }
+        for (int r = threadIdx.x; r < tiles * kTile; r += 32 * kWarps) {
+          float lse = INFINITY;
+          int lo = 0, hi = 0;
+          if (r < rows) {
+            const int i = (row0 + r) / group_heads, h = head * group_heads + (row0 + r) % group_heads;
+            lse = p.lse[((long long)b * p.nq + i) * p.heads + h] * kLog2e;
+            if (lse != -INFINITY) row_span(p, len, i, &lo, &hi);  // else a row that has seen nothing, and sees nothing here
+          }
+          s_lse[r] = lse;
+          s_lo[r] = lo;
+          s_hi[r] = hi;
         }
         __syncthreads();
-      }
-      if (n_rows <= C::kRows) staged = unit;
+        if (QT == QT_Q4_1) {  // sums of the query over blocks 2t, 2t + 1 as f16 and f16 remainder: a warp a row tile
+          for (int nt = warp; nt < tiles; nt += kWarps) {
+            float lo = 0.f, hi = 0.f;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+              const uint4 v = s_q[(nt * NB + n) * 32 + lane];
+              const float s = block_sum(v);
+              if (n == 2 * t) lo = s;
+              if (n == 2 * t + 1) hi = s;
+            }
+            s_min[nt * 32 + lane] = split_sums(lo, hi);
+          }
+          __syncthreads();
+        }
+        if (n_rows <= C::kRows) staged = unit;
       }
       for (int nt = 0; nt < tiles; ++nt) {
         float s[NG][4];
@@ -352,6 +352,7 @@ struct Stream {
 // Measured: 32 sequences of 1384 to 16384 tokens, 32 heads on 8, d = 128, q4_0: 177 MB in 48 us, 3.7 TB/s of the 6.5 that a copy
 // reaches. Instruction issue bounds it (63% of the cycles): 220 for 16 tokens of a head, a third of them unpacking. Loads
 // straight into registers, one or two groups ahead, took 72 us, rings of one group a step 59, five blocks an SM instead of four 61.
+// 9 of the 24 variants spill 20 to 116 bytes a thread (four query tiles of d = 128: 56 to 116).
 template <int QT, int D, int NT>
 __global__ void __launch_bounds__(128, Stream<QT, D, NT>::kBlocks) stream_kernel(const __grid_constant__ WeightArgs a, int* err) {
   typedef KvL<QT, D> L;
