@@ -15,9 +15,9 @@
 // copy reaches; one sequence of 524288 tokens, 16 heads on 2, q4_1: 168 MB in 53 us. Instruction issue bounds it (62% of
 // the cycles issue, the integer pipe is half busy): some 350 instructions for 16 tokens of a head, most of them unpacking
 // codes and scaling partial scores and weights. Looking at the scales of each step (ScaleRange) is 3% of the time. The output's
-// and the query's registers leave 32 of the 48 variants over all pages 4 to 84 bytes of spills a thread (one query tile of d = 128 in
-// q4_0: 32 and 40, in q4_1 16 and 40), 54 of the 65 over lists up to 140 (one query tile of d = 128 in q4_1: 112), 59 of those with
-// f32 outputs up to 120.
+// and the query's registers leave 32 of the 48 variants over all pages 4 to 92 bytes of spills a thread (one query tile of d = 128 in
+// q4_0: 40 and 44, in q4_1 16), 52 of the 65 over lists up to 148 (one query tile of d = 128 in q4_1: 100 and 116), 57 of those with
+// f32 outputs up to 128.
 #pragma once
 #include <algorithm>
 
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
   bool ok = true;
 
   long long pos = p0, base = s_base;
-  for (int b = s_b; pos < p1 && b < p.batch; ++b) {
+  for (int b = s_b;; ++b) {
     int g0, g1;
     const int n_chunks = chunks_of(b, &g0, &g1);
     const int len = sequence_length(p, b, err);
@@ -871,7 +871,7 @@ __global__ void __launch_bounds__(32 * W, Rows<QT, D, NT, W>::kCtas)
       fence_proxy_async_smem();  // the ring is written by copies again
       __syncthreads();
     }
-    if (!ok) break;
+    if (!ok || pos >= p1 || b == p.batch - 1) break;
     base += (long long)n_chunks * seq_units();
   }
   if (!ok) {
